@@ -22,6 +22,8 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
 ]
+# Sources whose results hang on the last bit of a formula, or on denormals: compiled without fast math.
+EXACT_MATH = {"moe_route.cu", "mx4_quant.cu"}
 # The C++ library is the shared one that torch has loaded.  A compiler that ships only libstdc++.a would put a second copy
 # into the extension; streams of one copy then use the locale of the other, and formatting the number in an error message
 # ends the process instead of raising.
@@ -46,7 +48,7 @@ def _digest() -> str:
         with open(os.path.join(CSRC, f), "rb") as fh:
             h.update(f.encode())
             h.update(fh.read())
-    h.update(" ".join(NVCC_FLAGS + LINK_FLAGS).encode())
+    h.update(" ".join(NVCC_FLAGS + LINK_FLAGS + sorted(EXACT_MATH)).encode())
     return h.hexdigest()
 
 
@@ -70,7 +72,8 @@ def build(verbose: bool = False, force: bool = False) -> str:
     for f in cu:
         out = os.path.join(OBJ, f + ".o")
         extra = ["-Xptxas", "-v"] if verbose else []
-        jobs.append(([nvcc, *NVCC_FLAGS, *extra, "-c", os.path.join(CSRC, f), "-o", out], out))
+        flags = [x for x in NVCC_FLAGS if not (f in EXACT_MATH and x == "--use_fast_math")]
+        jobs.append(([nvcc, *flags, *extra, "-c", os.path.join(CSRC, f), "-o", out], out))
     cxx = os.environ.get("CXX", "g++")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     for f in cpp:

@@ -313,6 +313,108 @@ Tensor moe_gather(DispatchKeySet ks, const Tensor& buf, const Tensor& slot, cons
   return records(buf, w) ? Gather::apply(buf, slot, w, Keys{ks}) : op_gather().below(ks, buf, slot, w);
 }
 
+// ---------------------------------------------------------------------------------------------- routing
+using RouteSig = Pair(const Tensor&, const c10::optional<Tensor>&, int64_t, bool, int64_t, int64_t, bool, double);
+using RouteBwdSig = Tensor(const Tensor&, const Tensor&, const Tensor&, bool, bool, double);
+const Op<RouteSig>& op_route() { APB_OP(o, "moe_route", RouteSig); return o; }
+const Op<RouteBwdSig>& op_route_bwd() { APB_OP(o, "moe_route_bwd", RouteBwdSig); return o; }
+struct Route : torch::autograd::Function<Route> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& bias, int64_t k, bool sigmoid, int64_t groups,
+                               int64_t top_groups, bool renorm, double scale, Keys key) {
+    auto [w, idx] = op_route().below(key.ks, x, bias, k, sigmoid, groups, top_groups, renorm, scale);
+    ctx->save_for_backward({x, idx});
+    ctx->mark_non_differentiable({idx});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["sigmoid"] = sigmoid;
+    ctx->saved_data["renorm"] = renorm;
+    ctx->saved_data["scale"] = scale;
+    return {w, idx};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const auto s = ctx->get_saved_variables();
+    Tensor dx;
+    if (g[0].defined())
+      dx = op_route_bwd()(g[0], s[0], s[1], ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
+    return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Pair moe_route(DispatchKeySet ks, const Tensor& x, const c10::optional<Tensor>& bias, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups,
+               bool renorm, double scale) {
+  if (!records(x)) return op_route().below(ks, x, bias, k, sigmoid, groups, top_groups, renorm, scale);
+  auto o = Route::apply(x, bias, k, sigmoid, groups, top_groups, renorm, scale, Keys{ks});
+  return {o[0], o[1]};
+}
+
+// ---------------------------------------------------------------------------------------------- MXFP4 (straight through the rounding)
+using MxRoundSig = Tensor(const Tensor&, int64_t);
+using MxValuesSig = Tensor(const Tensor&, const Tensor&, int64_t, ScalarType);
+using MxLinearSig = Tensor(const Tensor&, const Tensor&, const Tensor&, ScalarType);
+const Op<MxRoundSig>& op_mx_round() { APB_OP(o, "mx4_round", MxRoundSig); return o; }
+const Op<MxValuesSig>& op_mx_values() { APB_OP(o, "mx4_dequantize", MxValuesSig); return o; }
+const Op<MxLinearSig>& op_mx_linear() { APB_OP(o, "mx4_linear", MxLinearSig); return o; }
+const Op<MmNdSig>& op_mx_matmul() { APB_OP(o, "mx4_matmul", MmNdSig); return o; }
+
+// Zeros up to multiples of 8 in the last dim and, if asked for, in the one before: the 16-bit products address rows of whole 16 bytes.
+Tensor pad8(const Tensor& t, bool rows, bool columns) {
+  const int64_t c = columns ? (8 - t.size(-1) % 8) % 8 : 0, r = rows ? (8 - t.size(-2) % 8) % 8 : 0;
+  return c == 0 && r == 0 ? t : at::constant_pad_nd(t, {0, c, 0, r}, 0);
+}
+Tensor times(const Tensor& a, const Tensor& b, bool trans_b, ScalarType dtype) {
+  return b.dim() == 3 ? op_grouped_mm()(a, b, trans_b, dtype) : op_mm_nd()(a, b, trans_b, dtype);
+}
+Tensor pad_last(const Tensor& t) { return t.size(-1) % 8 == 0 ? t : at::constant_pad_nd(t, {0, 8 - t.size(-1) % 8}, 0); }
+Tensor cut(const Tensor& t, int64_t dim, int64_t size) { return t.size(dim) == size ? t : t.narrow(dim, 0, size); }
+
+struct MxRound : torch::autograd::Function<MxRound> {
+  static Tensor forward(AutogradContext*, const Tensor& x, int64_t dim, Keys k) { return op_mx_round().below(k.ks, x, dim); }
+  static variable_list backward(AutogradContext*, const variable_list& g) { return {g[0], Tensor(), Tensor()}; }
+};
+Tensor mx4_round(DispatchKeySet ks, const Tensor& x, int64_t dim) {
+  return records(x) ? MxRound::apply(x, dim, Keys{ks}) : op_mx_round().below(ks, x, dim);
+}
+struct MxLinear : torch::autograd::Function<MxLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& codes, const Tensor& scales, ScalarType dtype, Keys k) {
+    ctx->save_for_backward({codes, scales});
+    ctx->saved_data["k"] = x.size(-1);
+    ctx->saved_data["dtype"] = x.scalar_type();
+    return op_mx_linear().below(k.ks, x, codes, scales, dtype);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const auto s = ctx->get_saved_variables();
+    const int64_t k = ctx->saved_data["k"].toInt();
+    const Tensor dy = pad_last(g[0]);
+    const Tensor w = pad8(op_mx_values()(s[0], s[1], (k + 31) / 32 * 32, dy.scalar_type()), true, false);
+    return {cut(times(dy, w, false, ctx->saved_data["dtype"].toScalarType()), -1, k), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor mx4_linear(DispatchKeySet ks, const Tensor& x, const Tensor& codes, const Tensor& scales, ScalarType dtype) {
+  return records(x) ? MxLinear::apply(x, codes, scales, dtype, Keys{ks}) : op_mx_linear().below(ks, x, codes, scales, dtype);
+}
+struct MxMatmul : torch::autograd::Function<MxMatmul> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, bool trans_b, ScalarType dtype, Keys k) {
+    ctx->save_for_backward({x, w});
+    ctx->saved_data["tb"] = trans_b;
+    return op_mx_matmul().below(k.ks, x, w, trans_b, dtype);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1], dy = pad_last(g[0]);
+    const bool tb = ctx->saved_data["tb"].toBool();
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0))
+      dx = cut(times(dy, pad8(op_mx_round()(w, tb ? -1 : -2).to(dy.scalar_type()), true, true), !tb, x.scalar_type()), -1, x.size(-1));
+    if (ctx->needs_input_grad(1)) {
+      const Tensor xq = pad_last(op_mx_round()(x, -1).to(dy.scalar_type()));
+      const Op<WgradSig>& wgrad = w.dim() == 3 ? op_grouped_wgrad() : op_mm_wgrad();
+      dw = cut(cut(tb ? wgrad(dy, xq, w.scalar_type()) : wgrad(xq, dy, w.scalar_type()), -1, w.size(-1)), -2, w.size(-2));
+    }
+    return {dx, dw, Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor mx4_matmul(DispatchKeySet ks, const Tensor& x, const Tensor& w, bool trans_b, ScalarType dtype) {
+  return records(x, w) ? MxMatmul::apply(x, w, trans_b, dtype, Keys{ks}) : op_mx_matmul().below(ks, x, w, trans_b, dtype);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(apb200, AutogradCUDA, m) {
@@ -328,4 +430,8 @@ TORCH_LIBRARY_IMPL(apb200, AutogradCUDA, m) {
   m.impl("embedding", embedding);
   m.impl("moe_scatter", moe_scatter);
   m.impl("moe_gather", moe_gather);
+  m.impl("moe_route", moe_route);
+  m.impl("mx4_round", mx4_round);
+  m.impl("mx4_linear", mx4_linear);
+  m.impl("mx4_matmul", mx4_matmul);
 }

@@ -65,6 +65,17 @@ int apb_moe_gather(const void* buf, const long long* slot, const void* w, int w_
                    int nb, int is_bf16, int num_sms, cudaStream_t st);
 int apb_moe_gate_grad(const void* buf, const long long* slot, const void* g, float* dw, long long T, int k, int d, int E, int C, int nb,
                       int is_bf16, cudaStream_t st);
+int apb_moe_route(const void* logits, const float* bias, float* w, long long* idx, long long tokens, int E, int k, int sigmoid, int groups,
+                  int top_groups, int renorm, float scale, int is_bf16, cudaStream_t st);
+int apb_moe_route_bwd(const float* dw, const void* logits, const long long* idx, void* dx, long long tokens, int E, int k, int sigmoid, int renorm,
+                      float scale, int is_bf16, cudaStream_t st);
+int apb_mx4_quantize(const void* x, void* codes, void* scales, long long G, long long R, long long K, long long gs, long long ld, int transposed,
+                     int is_bf16, cudaStream_t st);
+int apb_mx4_round(const void* x, void* y, long long G, long long R, long long K, long long gs, long long ld, int transposed, int is_bf16,
+                  cudaStream_t st);
+int apb_mx4_dequantize(const void* codes, const void* scales, void* y, long long G, long long R, long long K, int is_bf16, cudaStream_t st);
+int apb_gemm_mx4(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long kp,
+                 int out_fp32, int form, uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_symm_header_bytes();
 int apb_symm_wait_probe(const uint32_t* flag, unsigned target, unsigned limit_ms, uint32_t* status, cudaStream_t st);
 int apb_symm_collective(int mode, const unsigned long long* peer_ptrs, int rank, int n, unsigned epoch, const void* src,
@@ -558,11 +569,14 @@ std::map<std::string, std::vector<std::array<int, 3>>> kernel_footprints() {
 // ask for, and every call of an operator for which register_cuda_impl has installed another function go to the table of ops/library.py.
 enum Entry : int {
   MM_ND, MM_WGRAD, GROUPED_MM, GROUPED_MM_WGRAD, DTYPE_CAST, RMS_NORM, RMS_NORM_BWD, ROPE, SWIGLU, SWIGLU_BWD, CROSS_ENTROPY, CROSS_ENTROPY_BWD,
-  EMBEDDING, EMBEDDING_BWD, MOE_SLOTS, MOE_SCATTER, MOE_GATHER, MOE_GATE_GRAD, CAST_MANY, NUM_ENTRIES
+  EMBEDDING, EMBEDDING_BWD, MOE_SLOTS, MOE_SCATTER, MOE_GATHER, MOE_GATE_GRAD, CAST_MANY, MOE_ROUTE, MOE_ROUTE_BWD, MX4_QUANTIZE, MX4_DEQUANTIZE,
+  MX4_ROUND, MX4_MM, MX4_LINEAR, MX4_MATMUL, NUM_ENTRIES
 };
+static_assert(NUM_ENTRIES <= 32, "a bit per entry");
 constexpr const char* ENTRY_NAMES[NUM_ENTRIES] = {
     "mm_nd", "mm_wgrad", "grouped_mm", "grouped_mm_wgrad", "dtype_cast", "rms_norm", "rms_norm_bwd", "rope", "swiglu", "swiglu_bwd", "cross_entropy",
-    "cross_entropy_bwd", "embedding", "embedding_bwd", "moe_slots", "moe_scatter", "moe_gather", "moe_gate_grad", "cast_many"};
+    "cross_entropy_bwd", "embedding", "embedding_bwd", "moe_slots", "moe_scatter", "moe_gather", "moe_gate_grad", "cast_many", "moe_route",
+    "moe_route_bwd", "mx4_quantize", "mx4_dequantize", "mx4_round", "mx4_mm", "mx4_linear", "mx4_matmul"};
 struct Native {
   py::object table;  // operator name -> Python function, as it is at the time of a call
   py::object status_buffer;
@@ -809,6 +823,188 @@ Tensor op_moe_gate_grad(const Tensor& buf, const Tensor& slot, const Tensor& g) 
   return in_python<Tensor>(MOE_GATE_GRAD, buf, slot, g);
 }
 
+// ---- routing to experts, MXFP4 (ops/moe_ops.py, ops/mx4_ops.py).  The functions of ops/cuda_impl.py call these, too; they count their launches.
+Two moe_route(const Tensor& logits_, const c10::optional<Tensor>& bias, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups, bool renorm,
+              double scale) {
+  c10::cuda::CUDAGuard g(logits_.device());
+  TORCH_CHECK(logits_.dim() >= 1 && logits_.size(-1) >= 1, "moe_route: logits [.., experts]");
+  const int64_t E = logits_.size(-1);
+  TORCH_CHECK(E <= 1024 && groups >= 1 && groups <= 64 && E % groups == 0 && top_groups >= 1 && top_groups <= groups && k >= 1 && k <= 32 &&
+                  k <= top_groups * (E / groups),
+              "moe_route: ", k, " of ", E, " experts in ", top_groups, " of ", groups, " groups");
+  Tensor logits = dense(logits_), b;
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->is_cuda() && bias->device() == logits.device() && bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == E,
+                "moe_route: bias is fp32 [experts] on the logits' device");
+    b = bias->contiguous();
+  }
+  auto shape = logits.sizes().vec();
+  shape.back() = k;
+  Tensor w = at::empty(shape, logits.options().dtype(at::kFloat)), idx = at::empty(shape, logits.options().dtype(at::kLong));
+  const int64_t tokens = logits.numel() / E;
+  check(apb_moe_route(logits.data_ptr(), b.defined() ? b.data_ptr<float>() : nullptr, w.data_ptr<float>(), (long long*)idx.data_ptr<int64_t>(), tokens,
+                      (int)E, (int)k, sigmoid, (int)groups, (int)top_groups, renorm, (float)scale, is_bf16(logits), stream()),
+        "apb_moe_route");
+  count(tokens > 0);
+  return {w, idx};
+}
+Tensor moe_route_bwd(const Tensor& dw_, const Tensor& logits_, const Tensor& idx_, bool sigmoid, bool renorm, double scale) {
+  c10::cuda::CUDAGuard g(logits_.device());
+  TORCH_CHECK(logits_.dim() >= 1 && logits_.size(-1) >= 1 && dw_.sizes() == idx_.sizes() && idx_.dim() == logits_.dim() &&
+                  idx_.scalar_type() == at::kLong && dw_.is_cuda() && idx_.is_cuda(),
+              "moe_route_bwd: dweights and idx [.., k], logits [.., experts]");
+  const int64_t E = logits_.size(-1), k = idx_.size(-1), tokens = logits_.numel() / E;
+  TORCH_CHECK(E <= 1024 && k >= 1 && k <= 32 && k <= E && idx_.numel() == tokens * k, "moe_route_bwd: ", k, " of ", E, " experts");
+  Tensor logits = dense(logits_), dw = dw_.to(at::kFloat).contiguous(), idx = idx_.contiguous(), dx = at::empty_like(logits);
+  check(apb_moe_route_bwd(dw.data_ptr<float>(), logits.data_ptr(), (const long long*)idx.data_ptr<int64_t>(), dx.data_ptr(), tokens, (int)E, (int)k,
+                          sigmoid, renorm, (float)scale, is_bf16(logits), stream()),
+        "apb_moe_route_bwd");
+  count(tokens > 0);
+  return dx;
+}
+
+// How a kernel goes through the matrices of x [R, K] or [G, R, K]: with unit stride along K, or along R; others are copied.
+struct MxView {
+  Tensor x;
+  int64_t G, R, K, gs, ld;
+  bool transposed;
+  MxView(const Tensor& x_, const char* what) : x(x_) {
+    TORCH_CHECK(x.dim() == 2 || x.dim() == 3, what, ": [R, K] or [E, R, K] expected");
+    is_bf16(x);
+    G = x.dim() == 3 ? x.size(0) : 1;
+    R = x.size(-2);
+    K = x.size(-1);
+    const bool rows = x.stride(-1) == 1 || K <= 1, columns = x.stride(-2) == 1 || R <= 1;
+    if (!rows && !columns) x = x.contiguous();
+    transposed = !rows && columns;
+    gs = x.dim() == 3 ? x.stride(0) : 0;
+    ld = x.stride(transposed ? -1 : -2);
+  }
+};
+int64_t mx_blocks(int64_t k) { return (k + 31) / 32; }
+
+Two mx4_quantize(const Tensor& x_) {
+  c10::cuda::CUDAGuard g(x_.device());
+  const MxView v(x_, "mx4_quantize");
+  auto shape = x_.sizes().vec();
+  shape.back() = mx_blocks(v.K) * 16;
+  Tensor codes = at::empty(shape, x_.options().dtype(at::kByte));
+  shape.pop_back();
+  shape.back() = (v.R + 127) / 128;
+  shape.insert(shape.end(), {(v.K + 127) / 128, 512});
+  Tensor scales = at::empty(shape, codes.options());
+  check(apb_mx4_quantize(v.x.data_ptr(), codes.data_ptr(), scales.data_ptr(), v.G, v.R, v.K, v.gs, v.ld, v.transposed, is_bf16(v.x), stream()),
+        "apb_mx4_quantize");
+  count(codes.numel() > 0);
+  return {codes, scales};
+}
+void mx_codes_check(const Tensor& codes, const Tensor& scales, const char* what) {
+  const int64_t d = codes.dim();
+  TORCH_CHECK((d == 2 || d == 3) && codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && codes.size(-1) % 16 == 0 &&
+                  scales.is_cuda() && scales.device() == codes.device() && scales.dim() == d + 1 && scales.size(-1) == 512 &&
+                  scales.size(-2) == (codes.size(-1) + 63) / 64 && scales.size(-3) == (codes.size(-2) + 127) / 128 &&
+                  (d == 2 || scales.size(0) == codes.size(0)),
+              what, ": codes [R, Kp / 2] (or [E, R, Kp / 2]) and their scales [ceil(R / 128), ceil(Kp / 128), 512], uint8");
+}
+Tensor mx4_dequantize(const Tensor& codes_, const Tensor& scales_, int64_t k, at::ScalarType dtype) {
+  c10::cuda::CUDAGuard g(codes_.device());
+  mx_codes_check(codes_, scales_, "mx4_dequantize");
+  TORCH_CHECK(k >= 0 && mx_blocks(k) * 16 == codes_.size(-1), "mx4_dequantize: ", k, " columns of ", codes_.size(-1), " bytes");
+  TORCH_CHECK(float_or_bf16(dtype), "mx4_dequantize: bf16 or fp32");
+  Tensor codes = dense(codes_), scales = dense(scales_);
+  auto shape = codes.sizes().vec();
+  shape.back() = k;
+  Tensor y = at::empty(shape, codes.options().dtype(dtype));
+  check(apb_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), y.data_ptr(), codes.dim() == 3 ? codes.size(0) : 1, codes.size(-2), k,
+                           dtype == at::kBFloat16, stream()),
+        "apb_mx4_dequantize");
+  count(y.numel() > 0);
+  return y;
+}
+Tensor mx4_round(const Tensor& x, int64_t dim) {
+  c10::cuda::CUDAGuard g(x.device());
+  TORCH_CHECK(dim == -1 || dim == -2, "mx4_round: dim -1 or -2");
+  TORCH_CHECK(x.dim() >= (dim == -1 ? 1 : 2), "mx4_round: too few dims");
+  Tensor y = at::empty(x.sizes(), x.options());
+  if (x.numel() == 0) return y;
+  const int64_t last = x.size(-1);
+  Tensor m = dim == -1 ? (x.dim() == 2 || x.dim() == 3 ? x : x.reshape({-1, last})) : (x.dim() <= 3 ? x : x.reshape({-1, x.size(-2), last}));
+  if (m.stride(-1) != 1 && last > 1) m = m.contiguous();
+  const MxView v(dim == -1 ? m : m.transpose(-1, -2), "mx4_round");
+  // (the result is dense in x's order: rows stay rows; a view of one row or column may be taken either way)
+  const bool columns = dim == -2;
+  check(apb_mx4_round(m.data_ptr(), y.data_ptr(), v.G, v.R, v.K, m.dim() == 3 ? m.stride(0) : 0, m.stride(-2), columns, is_bf16(m), stream()),
+        "apb_mx4_round");
+  count();
+  return y;
+}
+Tensor mx4_mm_form(const Tensor& a_, const Tensor& sa, const Tensor& b_, const Tensor& sb, at::ScalarType dtype, int64_t form) {
+  c10::cuda::CUDAGuard g(a_.device());
+  mx_codes_check(a_, sa, "mx4_mm");
+  mx_codes_check(b_, sb, "mx4_mm");
+  TORCH_CHECK(float_or_bf16(dtype), "mx4_mm: a result in bf16 or fp32");
+  TORCH_CHECK(b_.is_cuda() && b_.device() == a_.device() && a_.dim() == b_.dim() && a_.size(-1) == b_.size(-1) && (a_.dim() == 2 || a_.size(0) == b_.size(0)),
+              "mx4_mm: operands ", a_.sizes(), " and ", b_.sizes(), " do not multiply");
+  Tensor a = dense(a_), b = dense(b_), as = dense(sa), bs = dense(sb);
+  auto shape = a.sizes().vec();
+  shape.back() = b.size(-2);
+  Tensor c = at::empty(shape, a.options().dtype(dtype));
+  check(apb_gemm_mx4(a.data_ptr(), as.data_ptr(), b.data_ptr(), bs.data_ptr(), c.data_ptr(), a.dim() == 3 ? a.size(0) : 1, a.size(-2), b.size(-2),
+                     2 * a.size(-1), dtype == at::kFloat, (int)form, reinterpret_cast<uint32_t*>(status_of(a).data_ptr()), num_sms(), stream()),
+        "apb_gemm_mx4");
+  count(c.numel() > 0 && a.size(-1) > 0);
+  return c;
+}
+Tensor mx4_mm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, at::ScalarType dtype) { return mx4_mm_form(a, sa, b, sb, dtype, -1); }
+Tensor mx4_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
+  TORCH_CHECK(x.dim() >= 1 && codes.dim() >= 2 && mx_blocks(x.size(-1)) * 16 == codes.size(-1) &&
+                  (codes.dim() == 2 || (x.dim() == 3 && x.size(0) == codes.size(0))),
+              "mx4_linear: x ", x.sizes(), " and codes ", codes.sizes(), " do not multiply");
+  auto [a, sa] = mx4_quantize(codes.dim() == 3 || x.dim() == 2 ? x : x.reshape({x.numel() / std::max<int64_t>(x.size(-1), 1), x.size(-1)}));
+  Tensor c = mx4_mm(a, sa, codes, scales, dtype);
+  if (codes.dim() == 3 || x.dim() == 2) return c;
+  auto shape = x.sizes().vec();
+  shape.back() = codes.size(-2);
+  return c.view(shape);
+}
+Tensor mx4_matmul(const Tensor& x, const Tensor& w, bool trans_b, at::ScalarType dtype) {
+  TORCH_CHECK(w.dim() == 2 || w.dim() == 3, "mx4_matmul: w is a matrix or a stack of them");
+  auto [b, sb] = mx4_quantize(trans_b ? w : w.transpose(-1, -2));
+  return mx4_linear(x, b, sb, dtype);
+}
+
+Two op_moe_route(const Tensor& x, const c10::optional<Tensor>& bias, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups, bool renorm,
+                 double scale) {
+  if (ours(MOE_ROUTE)) return moe_route(x, bias, k, sigmoid, groups, top_groups, renorm, scale);
+  return in_python<Two>(MOE_ROUTE, x, bias, k, sigmoid, groups, top_groups, renorm, scale);
+}
+Tensor op_moe_route_bwd(const Tensor& dw, const Tensor& x, const Tensor& idx, bool sigmoid, bool renorm, double scale) {
+  if (ours(MOE_ROUTE_BWD)) return moe_route_bwd(dw, x, idx, sigmoid, renorm, scale);
+  return in_python<Tensor>(MOE_ROUTE_BWD, dw, x, idx, sigmoid, renorm, scale);
+}
+Two op_mx4_quantize(const Tensor& x) { return ours(MX4_QUANTIZE) ? mx4_quantize(x) : in_python<Two>(MX4_QUANTIZE, x); }
+Tensor op_mx4_dequantize(const Tensor& codes, const Tensor& scales, int64_t k, at::ScalarType dtype) {
+  if (ours(MX4_DEQUANTIZE)) return mx4_dequantize(codes, scales, k, dtype);
+  py::gil_scoped_acquire gil;
+  return in_python<Tensor>(MX4_DEQUANTIZE, codes, scales, k, py_dtype(dtype));
+}
+Tensor op_mx4_round(const Tensor& x, int64_t dim) { return ours(MX4_ROUND) ? mx4_round(x, dim) : in_python<Tensor>(MX4_ROUND, x, dim); }
+Tensor op_mx4_mm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, at::ScalarType dtype) {
+  if (ours(MX4_MM)) return mx4_mm(a, sa, b, sb, dtype);
+  py::gil_scoped_acquire gil;
+  return in_python<Tensor>(MX4_MM, a, sa, b, sb, py_dtype(dtype));
+}
+Tensor op_mx4_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
+  if (ours(MX4_LINEAR)) return mx4_linear(x, codes, scales, dtype);
+  py::gil_scoped_acquire gil;
+  return in_python<Tensor>(MX4_LINEAR, x, codes, scales, py_dtype(dtype));
+}
+Tensor op_mx4_matmul(const Tensor& x, const Tensor& w, bool trans_b, at::ScalarType dtype) {
+  if (ours(MX4_MATMUL)) return mx4_matmul(x, w, trans_b, dtype);
+  py::gil_scoped_acquire gil;
+  return in_python<Tensor>(MX4_MATMUL, x, w, trans_b, py_dtype(dtype));
+}
+
 // What register_cuda_impl installed for ``name``: ``on`` if it is not the function that the native entry stands for.
 void native_installed(const std::string& name, bool on) {
   for (int e = 0; e < NUM_ENTRIES; ++e)
@@ -850,6 +1046,14 @@ void register_native(py::dict table, py::object status_buffer, bool diag_library
   lib->impl(ENTRY_NAMES[MOE_GATHER], op_moe_gather);
   lib->impl(ENTRY_NAMES[MOE_GATE_GRAD], op_moe_gate_grad);
   lib->impl(ENTRY_NAMES[CAST_MANY], op_cast_many);
+  lib->impl(ENTRY_NAMES[MOE_ROUTE], op_moe_route);
+  lib->impl(ENTRY_NAMES[MOE_ROUTE_BWD], op_moe_route_bwd);
+  lib->impl(ENTRY_NAMES[MX4_QUANTIZE], op_mx4_quantize);
+  lib->impl(ENTRY_NAMES[MX4_DEQUANTIZE], op_mx4_dequantize);
+  lib->impl(ENTRY_NAMES[MX4_ROUND], op_mx4_round);
+  lib->impl(ENTRY_NAMES[MX4_MM], op_mx4_mm);
+  lib->impl(ENTRY_NAMES[MX4_LINEAR], op_mx4_linear);
+  lib->impl(ENTRY_NAMES[MX4_MATMUL], op_mx4_matmul);
 }
 
 }  // namespace
@@ -904,6 +1108,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_scatter", &moe_scatter);
   m.def("moe_gather", &moe_gather);
   m.def("moe_gate_grad", &moe_gate_grad);
+  m.def("moe_route", &moe_route);
+  m.def("moe_route_bwd", &moe_route_bwd);
+  m.def("mx4_quantize", &mx4_quantize);
+  m.def("mx4_dequantize", [](const Tensor& codes, const Tensor& scales, int64_t k, bool fp32) {
+    return mx4_dequantize(codes, scales, k, fp32 ? at::kFloat : at::kBFloat16);
+  });
+  m.def("mx4_round", &mx4_round);
+  m.def("mx4_mm", [](const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, bool fp32, int64_t form) {  // form -1: chosen
+    return mx4_mm_form(a, sa, b, sb, fp32 ? at::kFloat : at::kBFloat16, form);
+  });
+  m.def("mx4_linear", [](const Tensor& x, const Tensor& codes, const Tensor& scales, bool fp32) {
+    return mx4_linear(x, codes, scales, fp32 ? at::kFloat : at::kBFloat16);
+  });
+  m.def("mx4_matmul", [](const Tensor& x, const Tensor& w, bool trans_b, bool fp32) {
+    return mx4_matmul(x, w, trans_b, fp32 ? at::kFloat : at::kBFloat16);
+  });
   m.def("symm_header_bytes", &symm_header_bytes);
   m.def("symm_wait_probe", &symm_wait_probe);
   m.def("symm_collective", &symm_collective);

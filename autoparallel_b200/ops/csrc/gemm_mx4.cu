@@ -1,0 +1,400 @@
+// Products of MXFP4 matrices on the block-scaled tensor cores of sm_100a (formats and layout in ops/mx4_ops.py):
+//
+//   C[g][M, N] = A[g][M, K] * B[g][N, K]^T, both in 4 bits with a scale for 32 values along K; sums in fp32, C bf16 or fp32
+//
+// Persistent and warp-specialised like the 16-bit GEMM (gemm_core.cuh): TMA -> shared memory -> tcgen05.mma kind::mxf4 -> TMEM -> epilogue.  A stage is
+// 256 values of K (rows of 128 bytes, 128-byte swizzle, as 64 bf16 would be) and the scale tiles that belong to them, which the MMA thread has copied
+// to TMEM (tcgen05.cp) in front of the stage's MMAs.
+//   warp 0: TMA producer | warp 1: TMEM owner, scale copies, MMAs | warps 2..9: epilogue, two per TMEM lane quarter, each half of the tile's columns
+//
+// TMEM: two accumulators of up to 256 columns and 64 columns of scales do not fit 512, so the accumulators overlap by 64 columns: 0 ... 255 and
+// 192 ... 447, scales from 448 on.  The epilogue reads the shared columns first, and the next tile's MMAs start as soon as that is done.
+#include <algorithm>
+
+#include "gemm_core.cuh"
+
+namespace apb {
+
+constexpr int MX_BK = 256, MX_ROW_BYTES = MX_BK / 2;         // values and bytes of K in a stage
+constexpr int MX_SCALE_TILE = 512, MX_STAGE_TILES = 2;       // bytes of a scale tile, and how many lie along a stage
+constexpr int MX_ACC1 = 192, MX_SCALE_COL = 448;  // first columns of the second accumulator and of the scales
+constexpr int MX_EPI_WARPS = 8, MX_GEMM_THREADS = 64 + 32 * MX_EPI_WARPS;
+constexpr int MX_OP_BYTES = 128 * MX_ROW_BYTES;              // 128 rows of an operand
+constexpr int MX_SC_BYTES = MX_STAGE_TILES * MX_SCALE_TILE;  // and their scales
+constexpr int MX_STAGING = MX_EPI_WARPS * 4096;
+constexpr int MX_BAR_BYTES = 256;
+
+// BT: tiles of 128 rows of B that a CTA stages (PAIR: one of the pair's two); its column tile is 128 * BT, the pair's 256
+template <bool PAIR, int BT>
+struct MxShape {
+  static constexpr int SB_TILES = PAIR ? 2 : BT;  // every CTA needs the scales of all columns
+  static constexpr int STAGE = MX_OP_BYTES * (1 + BT) + MX_SC_BYTES * (1 + SB_TILES);
+  static constexpr int STAGES = (227 * 1024 - 1024 - MX_BAR_BYTES - MX_STAGING) / STAGE;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + MX_STAGING + MX_BAR_BYTES;
+};
+
+struct MxGemmParams {
+  GemmParams p;  // M, N, C, ldc, out_fp32, status and the tile order
+  int tiles, num_m, num_kb, k_steps;  // k_steps: MMAs of 64 along K
+  int col_tile, vec_store, grouped;
+};
+
+// Epilogue of a warp's 32 rows and ``ncols`` columns, 64 at a time, from column ``c_first`` up or down; ``release`` after the first 64.
+template <typename Release>
+__device__ __forceinline__ void mx_store(const MxGemmParams& q, uint8_t* C, uint8_t* stg, uint32_t taddr, int row0, int n0, int ncols, bool down,
+                                         int lane, Release release) {
+  const GemmParams& p = q.p;
+  const int esz = p.out_fp32 ? 4 : 2;
+  const int chunks = row0 < p.M ? (min(ncols, p.N - n0) + 63) / 64 : 0;  // (those past the matrix are not read)
+  if (chunks <= 0 || (down && chunks * 64 < ncols)) release();           // the shared columns are none of this warp's, or past the matrix
+  const bool early = chunks > 0 && !(down && chunks * 64 < ncols);
+#pragma unroll 1
+  for (int i = 0; i < chunks; ++i) {
+    const int c = (down ? chunks - 1 - i : i) * 64;
+    uint32_t r[2][32];
+    tmem_ld_32x32(taddr + c, r[0]);
+    tmem_ld_32x32(taddr + c + 32, r[1]);
+    tmem_ld_wait_for(r[0]);
+    tmem_ld_wait_for(r[1]);
+    if (early && i == 0) release();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // fp32: 32 columns at a time; bf16: all 64 in the first
+      if (h == 1 && !p.out_fp32) break;
+      uint4 v[8];
+      if (p.out_fp32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = make_uint4(r[h][4 * j], r[h][4 * j + 1], r[h][4 * j + 2], r[h][4 * j + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t* x = r[j >> 2] + 8 * (j & 3);
+          v[j] = make_uint4(pack_bf16(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_bf16(__uint_as_float(x[2]), __uint_as_float(x[3])),
+                            pack_bf16(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_bf16(__uint_as_float(x[6]), __uint_as_float(x[7])));
+        }
+      }
+      __syncwarp();  // the block before has been read out
+#pragma unroll
+      for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = v[j];
+      __syncwarp();
+      const int col0 = n0 + c + 32 * h;  // of the 128 bytes
+      if (q.vec_store) {
+        const int unit = lane & 7, sub = lane >> 3, col = col0 + unit * (16 / esz);
+#pragma unroll 4
+        for (int j = 0; j < 8; ++j) {
+          const int row = 4 * j + sub;
+          const uint4 x = *reinterpret_cast<const uint4*>(stg + row * 128 + ((unit ^ (row & 7)) << 4));
+          if (col < p.N && row0 + row < p.M) *reinterpret_cast<uint4*>(C + ((row0 + row) * p.ldc + col) * esz) = x;
+        }
+      } else {  // rows that are no whole vectors: element by element, a row at a time
+        for (int row = 0; row < 32 && row0 + row < p.M; ++row)
+          for (int e = lane; e < 128 / esz; e += 32) {
+            const uint8_t* src = stg + row * 128 + (((e * esz / 16) ^ (row & 7)) << 4) + e * esz % 16;
+            if (col0 + e >= p.N) continue;
+            uint8_t* dst = C + ((row0 + row) * p.ldc + col0 + e) * esz;
+            if (p.out_fp32) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+            else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+          }
+      }
+    }
+  }
+}
+
+template <bool PAIR, int BT>
+__device__ __forceinline__ void mx_gemm_cta(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmSA, const CUtensorMap& tmSB,
+                                            const MxGemmParams& q, uint8_t* smem_raw) {
+  using S = MxShape<PAIR, BT>;
+  constexpr int ST = S::STAGES, TM = PAIR ? 256 : 128;
+  constexpr int A_AT = 0, B_AT = MX_OP_BYTES, OP_STAGE = MX_OP_BYTES * (1 + BT), SC_STAGE = S::STAGE - OP_STAGE;
+  const GemmParams& p = q.p;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // operands of all stages first (1024-byte atoms), then the scales
+  uint8_t* ops = smem;
+  uint8_t* scs = smem + ST * OP_STAGE;
+  uint8_t* staging = smem + ST * S::STAGE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + MX_STAGING);
+  uint64_t* full = bars;               // [ST]  PAIR: the even CTA's are used
+  uint64_t* empty = bars + ST;         // [ST]
+  uint64_t* acc_full = bars + 2 * ST;  // [2]
+  uint64_t* go = bars + 2 * ST + 2;    // the columns that two accumulators share have been read; one arrival per epilogue warp, PAIR: of both CTAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 3);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  static_assert((2 * ST + 4) * 8 <= MX_BAR_BYTES, "barrier block");
+  const uint32_t half = PAIR ? cluster_ctarank() : 0u;  // 0: issues the MMAs, owns the shared barriers
+  const int unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, num_units = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&acc_full[0], 1);
+    mbar_init(&acc_full[1], 1);
+    mbar_init(go, (PAIR ? 2 : 1) * MX_EPI_WARPS);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmSA);
+    tma_prefetch_desc(&tmSB);
+  }
+  if (warp == 1) {
+    if (PAIR) {
+      tmem_alloc_pair(tmem_slot, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  wait_previous();
+
+  auto fail = [&](uint32_t code) {
+    atomicCAS(p.status, 0u, code);
+    *abort_flag = 1;
+  };
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      const uint32_t full_pair = PAIR ? map_to_cta(full, 0) : 0u;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = unit; t < q.tiles && ok; t += num_units) {
+        int grp, tm, tn;
+        plain_tile(p, q.num_m, q.grouped, t, grp, tm, tn);
+        const int m0 = tm * TM + (int)half * 128, col = tn * q.col_tile;
+        const int n0 = col + (PAIR ? (int)half * 128 : 0);  // rows of B that this CTA stages
+        for (int kb = 0; kb < q.num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
+            ok = false;
+            fail(ST_TIMEOUT_EMPTY);
+            break;
+          }
+          uint8_t *op = ops + stage * OP_STAGE, *sc = scs + stage * SC_STAGE;
+          auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y) {
+            if (PAIR) tma_load_3d_pair(dst, map, full_pair + stage * 8, x, y, grp);
+            else tma_load_3d(dst, map, &full[stage], x, y, grp);
+          };
+          if (half == 0) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * S::STAGE);
+          load(op + A_AT, &tmA, kb * MX_ROW_BYTES, m0);
+          load(op + B_AT, &tmB, kb * MX_ROW_BYTES, n0);
+          load(sc, &tmSA, kb * (MX_SC_BYTES / 4), m0 / 128);
+          load(sc + MX_SC_BYTES, &tmSB, kb * (MX_SC_BYTES / 4), col / 128);
+          if (++stage == ST) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      let_next_in();
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ scale copies and MMAs
+    if (half == 0 && elect_one()) {
+      const uint32_t idesc[2] = {make_idesc_mx4(TM, q.col_tile, 0), make_idesc_mx4(TM, q.col_tile, 2)};
+      const uint64_t a_desc = make_smem_desc(smem_u32(ops + A_AT), 16, 1024), b_desc = make_smem_desc(smem_u32(ops + B_AT), 16, 1024);
+      const uint64_t sa_desc = make_scale_desc(smem_u32(scs)), sb_desc = make_scale_desc(smem_u32(scs + MX_SC_BYTES));
+      const uint32_t empty_even = PAIR ? map_to_cta(empty, 0) : 0u, empty_odd = PAIR ? map_to_cta(empty, 1) : 0u;
+      const uint32_t sa_tmem = tmem + MX_SCALE_COL, sb_tmem = sa_tmem + 4 * MX_STAGE_TILES;
+      int stage = 0;
+      uint32_t phase = 0, seq = 0;
+      bool ok = true;
+      for (int t = unit; t < q.tiles && ok; t += num_units, ++seq) {
+        if (seq > 0 && !mbar_wait(go, (seq - 1) & 1u, abort_flag)) {
+          fail(ST_TIMEOUT_TMEM_EMPTY);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem + (seq & 1u) * MX_ACC1;
+        for (int kb = 0; kb < q.num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, abort_flag)) {
+            ok = false;
+            fail(ST_TIMEOUT_FULL);
+            break;
+          }
+          tc_fence_after();
+          auto copy = [&](uint32_t taddr, uint64_t desc) {
+            if (PAIR) tmem_copy_scales_pair(taddr, desc);
+            else tmem_copy_scales(taddr, desc);
+          };
+          const int steps = min(MX_BK / 64, q.k_steps - kb * (MX_BK / 64));
+#pragma unroll
+          for (int a = 0; a < MX_STAGE_TILES; ++a) {  // (the tiles of a row group lie after each other; a column of scales for 32 rows)
+            copy(sa_tmem + 4 * a, sa_desc + desc_offset(stage * SC_STAGE + a * MX_SCALE_TILE));
+#pragma unroll
+            for (int b = 0; b < S::SB_TILES; ++b)
+              copy(sb_tmem + 4 * (a * S::SB_TILES + b), sb_desc + desc_offset(stage * SC_STAGE + b * MX_SC_BYTES + a * MX_SCALE_TILE));
+          }
+          const uint64_t ad = a_desc + desc_offset(stage * OP_STAGE), bd = b_desc + desc_offset(stage * OP_STAGE);
+#pragma unroll
+          for (int s = 0; s < MX_BK / 64; ++s) {
+            if (s >= steps) break;
+            const uint32_t sa = sa_tmem + 4 * (s / 2), sb = sb_tmem + 4 * S::SB_TILES * (s / 2);
+            const uint32_t more = kb > 0 || s > 0 ? 1u : 0u;
+            if (PAIR) umma_mx4_pair(d_tmem, ad + desc_offset(32 * s), bd + desc_offset(32 * s), idesc[s & 1], sa, sb, more);
+            else umma_mx4(d_tmem, ad + desc_offset(32 * s), bd + desc_offset(32 * s), idesc[s & 1], sa, sb, more);
+          }
+          if (PAIR) {
+            umma_commit_pair(empty_even + stage * 8);
+            umma_commit_pair(empty_odd + stage * 8);
+          } else {
+            umma_commit(&empty[stage]);
+          }
+          if (++stage == ST) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        if (PAIR) {
+          umma_commit_pair(map_to_cta(&acc_full[seq & 1u], 0));
+          umma_commit_pair(map_to_cta(&acc_full[seq & 1u], 1));
+        } else {
+          umma_commit(&acc_full[seq & 1u]);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int quarter = warp & 3, part = (warp - 2) >> 2, cols = q.col_tile / 2;
+    const uint32_t go_even = PAIR ? map_to_cta(go, 0) : 0u;
+    const int esz = p.out_fp32 ? 4 : 2;
+    uint32_t seq = 0;
+    for (int t = unit; t < q.tiles; t += num_units, ++seq) {
+      int grp, tm, tn;
+      plain_tile(p, q.num_m, q.grouped, t, grp, tm, tn);
+      const uint32_t buf = seq & 1u;
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster_plain(go_even);
+          else mbar_arrive(go);
+        }
+      };
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], seq >> 1 & 1u, abort_flag))) {
+        fail(ST_TIMEOUT_TMEM_FULL);
+        break;
+      }
+      tc_fence_after();
+      // the shared columns: the last of the first accumulator (the second half's), the first of the second (the first half's)
+      const bool mine = buf == 0 ? part == 1 : part == 0;
+      if (!mine) release();
+      mx_store(q, reinterpret_cast<uint8_t*>(p.C) + (long long)grp * p.M * p.ldc * esz, staging + (warp - 2) * 4096,
+               tmem + (uint32_t(quarter * 32) << 16) + buf * MX_ACC1 + part * cols, tm * TM + (int)half * 128 + quarter * 32,
+               tn * q.col_tile + part * cols, cols, buf == 0, lane, [&]() {
+                 if (mine) release();
+               });
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    if (PAIR) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int BT>
+__global__ void __launch_bounds__(MX_GEMM_THREADS, GEMM_MIN_CTAS)
+gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
+                const __grid_constant__ CUtensorMap tmSB, MxGemmParams q) {
+  extern __shared__ uint8_t smem_raw[];
+  mx_gemm_cta<false, BT>(tmA, tmB, tmSA, tmSB, q, smem_raw);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GEMM_THREADS, GEMM_MIN_CTAS)
+gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
+                     const __grid_constant__ CUtensorMap tmSB, MxGemmParams q) {
+  extern __shared__ uint8_t smem_raw[];
+  mx_gemm_cta<true, 1>(tmA, tmB, tmSA, tmSB, q, smem_raw);
+}
+
+// [G][rows][bytes] of codes in boxes of 128 bytes x ``box_rows`` (128-byte swizzle), or [G][row tiles][scale words] in boxes of a stage's words.
+static int mx_map(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t rows, uint64_t G, uint32_t box_inner, uint32_t box_rows, bool scales) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return 1;
+  const uint64_t esz = scales ? 4 : 1;
+  cuuint64_t dims[3] = {inner, rows, G};
+  cuuint64_t strides[2] = {inner * esz, inner * rows * esz};
+  cuuint32_t box[3] = {box_inner, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, scales ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, scales ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 2;
+}
+
+}  // namespace apb
+
+using namespace apb;
+
+extern "C" int apb_gemm_resident_pairs(int num_sms);
+extern "C" int apb_gemm_get_reserved_sms();
+
+// A, B: codes [G, M, kp / 2] and [G, N, kp / 2]; SA, SB: scales [G, M / 128, kp / 128, 512]; kp a multiple of 32; C [G, M, N]; all dense, 16-byte bases.
+// ``form``: 0 = one CTA on 128 x 128 tiles, 1 = one CTA on 128 x 256, 2 = pairs on 256 x 256, -1 = chosen here.
+// Returns 0, or an argument / driver / launch error (nothing launched).
+extern "C" int apb_gemm_mx4(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long kp,
+                            int out_fp32, int form, uint32_t* status, int num_sms, cudaStream_t stream) {
+  if (G < 0 || M < 0 || N < 0 || kp < 0 || kp % 32 || M >= 1ll << 31 || N >= 1ll << 31 || kp >= 1ll << 30 || G >= 1ll << 31) return 3;
+  if (G == 0 || M == 0 || N == 0) return 0;
+  for (const void* ptr : {A, SA, B, SB, (const void*)C})
+    if (reinterpret_cast<uintptr_t>(ptr) & 15) return 3;
+  if (kp == 0) return zero_result(C, G * M, N, N, out_fp32, stream);
+  if (form < 0) form = M > 128 && N > 128 ? 2 : N > 128 ? 1 : 0;
+  const bool pair = form == 2;
+  MxGemmParams q{};
+  GemmParams& p = q.p;
+  p.M = (int)M;
+  p.N = (int)N;
+  p.C = C;
+  p.ldc = N;
+  p.out_fp32 = out_fp32;
+  p.status = status;
+  q.col_tile = form == 0 ? 128 : 256;
+  q.vec_store = N % (out_fp32 ? 4 : 8) == 0;
+  q.grouped = G > 1;
+  q.num_m = (int)((M + (pair ? 255 : 127)) / (pair ? 256 : 128));
+  p.num_n_tiles = (int)((N + q.col_tile - 1) / q.col_tile);
+  q.num_kb = (int)((kp + MX_BK - 1) / MX_BK);
+  q.k_steps = (int)((kp + 63) / 64);
+  const long long tiles = G * q.num_m * p.num_n_tiles;
+  if (tiles >= 1ll << 30) return 3;
+  q.tiles = (int)tiles;
+  set_tile_order(p, q.num_m, p.num_n_tiles);
+  const uint64_t words = (uint64_t)((kp + 127) / 128) * (MX_SCALE_TILE / 4);
+  CUtensorMap tmA, tmB, tmSA, tmSB;
+  int e = mx_map(&tmA, A, kp / 2, M, G, MX_ROW_BYTES, 128, false);
+  if (!e) e = mx_map(&tmB, B, kp / 2, N, G, MX_ROW_BYTES, form == 1 ? 256 : 128, false);
+  if (!e) e = mx_map(&tmSA, SA, words, (M + 127) / 128, G, MX_SC_BYTES / 4, 1, true);
+  if (!e) e = mx_map(&tmSB, SB, words, (N + 127) / 128, G, MX_SC_BYTES / 4, form == 0 ? 1 : 2, true);
+  if (e) return e;
+  const int reserved = apb_gemm_get_reserved_sms();
+  auto launch = [&](auto kern, int units, int smem) {
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    launch_after(kern, (unsigned)units, MX_GEMM_THREADS, smem, stream, tmA, tmB, tmSA, tmSB, q);
+    return cudaGetLastError() == cudaSuccess ? 0 : 4;
+  };
+  if (pair) {
+    const int resident = std::max(1, apb_gemm_resident_pairs(num_sms) - reserved / 2);
+    return launch(gemm_mx4_pair_kernel, 2 * std::min(q.tiles, resident), MxShape<true, 1>::SMEM);
+  }
+  const int usable = std::max(1, num_sms - reserved);
+  return form == 1 ? launch(gemm_mx4_kernel<2>, std::min(q.tiles, usable), MxShape<false, 2>::SMEM)
+                   : launch(gemm_mx4_kernel<1>, std::min(q.tiles, usable), MxShape<false, 1>::SMEM);
+}

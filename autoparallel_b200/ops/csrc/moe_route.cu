@@ -1,0 +1,409 @@
+// Routing of tokens to experts: scores, choice of the top k (of the top groups), gate weights, and the gradient of the logits.
+// Semantics in ops/moe_ops.py; everything in fp32, in one pass over the logits.
+//
+// This file is compiled without --use_fast_math: the choice between two experts hangs on the last bit of a sigmoid, and has to be the same
+// wherever the formula is evaluated as written (expf, IEEE division, denormals kept).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "launch.cuh"
+
+namespace apb {
+
+constexpr int ROUTE_WARPS = 8, ROUTE_MAX_GROUPS = 64;
+
+struct RouteParams {
+  const void* x;
+  const float* bias;
+  float* w;
+  long long* idx;
+  long long tokens;
+  int E, k, groups, size, top_groups, renorm, vec;
+  float scale;
+  uint32_t mask;  // 2^b - 1, at least E - 1
+};
+
+template <typename T>
+__device__ __forceinline__ float route_load(const T* p) {
+  if constexpr (std::is_same<T, float>::value) return *p;
+  else return __bfloat162float(*p);
+}
+// V elements of a row from ``e0`` on; those past E are -inf
+template <typename T, int V>
+__device__ __forceinline__ void route_load_row(const T* row, int e0, int E, bool vec, float (&x)[V]) {
+  if (vec) {
+    constexpr int PER = 16 / sizeof(T);
+    uint4 v[V / PER];
+#pragma unroll
+    for (int c = 0; c < V / PER; ++c) {
+      constexpr uint32_t NONE = std::is_same<T, float>::value ? 0xFF800000u : 0xFF80FF80u;
+      v[c] = make_uint4(NONE, NONE, NONE, NONE);
+      if (e0 + c * PER < E) v[c] = *reinterpret_cast<const uint4*>(row + e0 + c * PER);
+    }
+#pragma unroll
+    for (int c = 0; c < V / PER; ++c) {
+      const uint32_t u[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, float>::value) {
+          x[c * PER + i] = __uint_as_float(u[i]);
+        } else {
+          x[c * PER + 2 * i] = __uint_as_float(u[i] << 16);
+          x[c * PER + 2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = e0 + i < E ? route_load(row + e0 + i) : -CUDART_INF_F;
+  }
+}
+
+__device__ __forceinline__ float route_sigmoid(float x) { return __frcp_rn(1.0f + expf(-x)); }
+
+// Order of the floats as unsigned integers.  -0 counts as 0 and every NaN as the same one, larger than all numbers: the sum with 0 makes
+// them so (the result of an addition is the canonical NaN).  0 is smaller than the order of any float.
+__device__ __forceinline__ uint32_t route_order(float c) {
+  const uint32_t u = __float_as_uint(c + 0.0f);
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float route_unorder(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+
+template <int L>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+#pragma unroll
+  for (int d = 1; d < L; d *= 2) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int d = 1; d < L; d *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int d = 1; d < L; d *= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// The experts outside a token's best groups get order 0: they cannot be chosen.
+template <int L, int V>
+__device__ __forceinline__ void route_groups(const RouteParams& p, bool sigmoid, int warp, int tok, int sub, uint32_t (&o)[V]) {
+  constexpr int TPW = 32 / L, ROW = L * V + L * V / 32 + 1;  // (one word more every 32: groups of 32 begin in different banks)
+  __shared__ uint32_t rows[ROUTE_WARPS][TPW * ROW];
+  __shared__ uint32_t vals[ROUTE_WARPS][TPW * ROUTE_MAX_GROUPS];
+  uint32_t *row = rows[warp] + tok * ROW, *val = vals[warp] + tok * ROUTE_MAX_GROUPS;
+#pragma unroll
+  for (int i = 0; i < V; ++i) row[sub * V + i + (sub * V + i) / 32] = o[i];
+  __syncwarp();
+  for (int g = sub; g < p.groups; g += L) {
+    uint32_t a = 0, b = 0;
+    for (int i = 0; i < p.size; ++i) {
+      const int e = g * p.size + i;
+      const uint32_t v = row[e + e / 32];
+      b = max(b, min(a, v));
+      a = max(a, v);
+    }
+    val[g] = sigmoid && p.size > 1 ? route_order(route_unorder(a) + route_unorder(b)) : a;
+  }
+  __syncwarp();
+  unsigned long long kept = 0;  // bit i: this lane's i-th group
+  for (int g = sub, i = 0; g < p.groups; g += L, ++i) {
+    const uint32_t mine = val[g];
+    int before = 0;
+    for (int h = 0; h < p.groups; ++h) before += val[h] > mine || (val[h] == mine && h < g);
+    if (before < p.top_groups) kept |= 1ull << i;
+  }
+  __syncwarp();
+  for (int g = sub, i = 0; g < p.groups; g += L, ++i) val[g] = kept >> i & 1;
+  __syncwarp();
+  int g = sub * V / p.size, r = sub * V - g * p.size;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (g < p.groups && !val[g]) o[i] = 0;
+    if (++r == p.size) {
+      r = 0;
+      ++g;
+    }
+  }
+  __syncwarp();
+}
+
+// L lanes hold a token, V experts each (lane after lane), and lane j ends up with its j-th choice: k <= L.
+//
+// The choice takes keys in place of the choice values: the upper bits of the value's order, and in the lower b bits (2^b >= E) the expert's number,
+// inverted, so that the larger of two keys is the one to be chosen.  All keys differ, which makes a step of the selection - the largest key below
+// the last - max(key - last) + last in wrapping arithmetic: two instructions a key.  What the lower bits of a value lose matters only
+// where two neighbours in the result (the last chosen and the best of the rest among them) agree in the upper ones: then the warp
+// repeats the selection with whole values and numbers (256 experts, fp32: about 1 token in 100; bf16 logits without bias: never, they have 16 bits).
+template <typename T, int L, int V, bool SIGMOID>
+__global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_kernel(RouteParams p) {
+  after_previous();
+  constexpr int TPW = 32 / L;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tok = lane / L, sub = lane % L;
+  const long long t = ((long long)blockIdx.x * ROUTE_WARPS + warp) * TPW + tok;
+  const bool in = t < p.tokens;
+  const T* row = reinterpret_cast<const T*>(p.x) + (in ? t : p.tokens - 1) * p.E;  // (lanes without a token follow the last one)
+  const int e0 = sub * V;
+  float x[V];
+  route_load_row<T, V>(row, e0, p.E, p.vec, x);
+  float m_all = -CUDART_INF_F, total_all = 0.f;
+  if (!SIGMOID && !p.renorm) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) m_all = fmaxf(m_all, x[i]);
+    m_all = lanes_max<L>(m_all);
+    if (m_all == -CUDART_INF_F) m_all = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) total_all += expf(x[i] - m_all);
+    total_all = lanes_sum<L>(total_all);
+  }
+  uint32_t o[V], key[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float c = SIGMOID ? route_sigmoid(x[i]) : x[i];
+    if (p.bias != nullptr && e0 + i < p.E) c += p.bias[e0 + i];
+    o[i] = e0 + i < p.E ? route_order(c) : 0u;
+  }
+  if (p.groups > 1) route_groups<L, V>(p, SIGMOID, warp, tok, sub, o);
+#pragma unroll
+  for (int i = 0; i < V; ++i) key[i] = o[i] == 0 ? 0u : (o[i] & ~p.mask) | (p.mask - (e0 + i));
+
+  uint32_t last = 0, mine = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) last = max(last, key[i]);
+  last = lanes_max<L>(last);
+  for (int j = 0; j < p.k; ++j) {
+    if (sub == j) mine = last;
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) best = max(best, key[i] - last);
+    last += lanes_max<L>(best);
+  }
+  const bool chosen = sub < p.k;
+  int e = chosen ? (int)(p.mask - (mine & p.mask)) : 0;
+  float xe = route_load(row + e);
+  float se = SIGMOID ? route_sigmoid(xe) : 0.f;
+  const bool whole = !SIGMOID && std::is_same<T, __nv_bfloat16>::value && p.bias == nullptr;  // (16 bits of value: the keys have them all)
+  if (!whole) {
+    float c = SIGMOID ? se : xe;
+    if (p.bias != nullptr) c += p.bias[e];
+    const uint32_t oe = route_order(c);
+    const uint32_t next_key = __shfl_down_sync(0xffffffffu, mine, 1, L), next_o = __shfl_down_sync(0xffffffffu, oe, 1, L);
+    const bool unsure = sub + 1 < p.k ? ((mine ^ next_key) & ~p.mask) == 0 && oe != next_o : sub + 1 == p.k && ((mine ^ last) & ~p.mask) == 0;
+    if (__any_sync(0xffffffffu, unsure)) {
+      uint32_t lo = 0xFFFFFFFFu;
+      int le = -1;
+      for (int j = 0; j < p.k; ++j) {
+        uint32_t bo = 0;
+        int be = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if ((o[i] < lo || (o[i] == lo && e0 + i > le)) && o[i] > bo) {
+            bo = o[i];
+            be = e0 + i;
+          }
+#pragma unroll
+        for (int d = 1; d < L; d *= 2) {
+          const uint32_t ho = __shfl_xor_sync(0xffffffffu, bo, d);
+          const int he = __shfl_xor_sync(0xffffffffu, be, d);
+          if (ho > bo || (ho == bo && he < be)) {
+            bo = ho;
+            be = he;
+          }
+        }
+        lo = bo;
+        le = be;
+        if (sub == j) e = be;
+      }
+      xe = route_load(row + e);
+      se = SIGMOID ? route_sigmoid(xe) : 0.f;
+    }
+  }
+  float s, total;
+  if (SIGMOID) {
+    s = chosen ? se : 0.f;
+    total = p.renorm ? lanes_sum<L>(s) : 1.f;
+  } else if (p.renorm) {
+    float m = lanes_max<L>(chosen ? xe : -CUDART_INF_F);
+    if (m == -CUDART_INF_F) m = 0.f;
+    s = chosen ? expf(xe - m) : 0.f;
+    total = lanes_sum<L>(s);
+  } else {
+    s = expf(xe - m_all);
+    total = total_all;
+  }
+  if (in && chosen) {
+    p.w[t * p.k + sub] = (total == 0.f ? 0.f : s / total) * p.scale;
+    p.idx[t * p.k + sub] = e;
+  }
+}
+
+struct RouteBwdParams {
+  const float* dw;
+  const void* x;
+  const long long* idx;
+  void* dx;
+  long long tokens;
+  int E, k, renorm, vec;
+  float scale;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void route_store_row(T* row, int e0, int E, bool vec, const float (&v)[V]) {
+  if (vec) {
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < V / PER; ++c) {
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, float>::value) {
+          u[i] = __float_as_uint(v[c * PER + i]);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[c * PER + 2 * i], v[c * PER + 2 * i + 1]);
+          u[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      if (e0 + c * PER < E) *reinterpret_cast<uint4*>(row + e0 + c * PER) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (e0 + i < E) {
+        if constexpr (std::is_same<T, float>::value) row[e0 + i] = v[i];
+        else row[e0 + i] = __float2bfloat16(v[i]);
+      }
+  }
+}
+
+// With p the weights before the scale and g = dweights * scale:
+//   softmax over the chosen  dx_j = p_j (g_j - sum g p)          softmax over all  dx_e = p_e (g_e - sum g p), g_e = 0 for the others
+//   sigmoid                  dx_j = g_j s_j (1 - s_j), with the sum of the chosen S: g_j <- (g_j - sum g p) / S first
+// The row is written whole (zeros, or the gradient of the experts that were not chosen), then the chosen ones over it.
+template <typename T, int L, int V, bool SIGMOID>
+__global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_bwd_kernel(RouteBwdParams p) {
+  after_previous();
+  constexpr int TPW = 32 / L;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tok = lane / L, sub = lane % L;
+  const long long t = ((long long)blockIdx.x * ROUTE_WARPS + warp) * TPW + tok;
+  const bool in = t < p.tokens;
+  const long long tt = in ? t : p.tokens - 1;
+  const T* row = reinterpret_cast<const T*>(p.x) + tt * p.E;
+  T* out = reinterpret_cast<T*>(p.dx) + tt * p.E;
+  const int e0 = sub * V;
+  long long e = sub < p.k ? p.idx[tt * p.k + sub] : -1;
+  const bool chosen = e >= 0 && e < p.E;  // (a number that names no expert has no gradient)
+  const float g = chosen ? p.dw[tt * p.k + sub] * p.scale : 0.f;
+  const float xe = chosen ? route_load(row + e) : -CUDART_INF_F;
+  float v[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = 0.f;
+  float mine;
+  if (SIGMOID) {
+    const float s = chosen ? route_sigmoid(xe) : 0.f;
+    float ds = g;
+    if (p.renorm) {
+      const float total = lanes_sum<L>(s);
+      const float dot = lanes_sum<L>(chosen ? g * s / total : 0.f);
+      ds = total == 0.f ? 0.f : (g - dot) / total;
+    }
+    mine = ds * s * (1.f - s);
+  } else if (p.renorm) {
+    float m = lanes_max<L>(xe);
+    if (m == -CUDART_INF_F) m = 0.f;
+    const float s = chosen ? expf(xe - m) : 0.f, total = lanes_sum<L>(s), q = total == 0.f ? 0.f : s / total;
+    mine = q * (g - lanes_sum<L>(g * q));
+  } else {
+    float x[V];
+    route_load_row<T, V>(row, e0, p.E, p.vec, x);
+    float m = -CUDART_INF_F, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
+    m = lanes_max<L>(m);
+    if (m == -CUDART_INF_F) m = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      x[i] = expf(x[i] - m);
+      total += x[i];
+    }
+    total = lanes_sum<L>(total);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const float q = chosen ? expf(xe - m) * inv : 0.f, dot = lanes_sum<L>(g * q);
+    mine = q * (g - dot);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = x[i] * inv * -dot;
+  }
+  if (in) route_store_row<T, V>(out, e0, p.E, p.vec, v);
+  __syncwarp();
+  if (in && chosen) {
+    if constexpr (std::is_same<T, float>::value) out[e] = mine;
+    else out[e] = __float2bfloat16(mine);
+  }
+}
+
+// f(L, V) for the smallest number of lanes that holds the experts, 16 a lane where that is enough, and a choice a lane.
+template <typename F>
+static int route_shape(int E, int k, F f) {
+  auto c = [](auto v) { return v; };
+#define APB_ROUTE(L, V) return f(c(std::integral_constant<int, L>{}), c(std::integral_constant<int, V>{}))
+  if (k <= 4 && E <= 32) APB_ROUTE(4, 8);
+  if (k <= 8 && E <= 64) APB_ROUTE(8, 8);
+  if (k <= 8 && E <= 128) APB_ROUTE(8, 16);
+  if (k <= 16 && E <= 128) APB_ROUTE(16, 8);
+  if (k <= 16 && E <= 256) APB_ROUTE(16, 16);
+  if (E <= 256) APB_ROUTE(32, 8);
+  if (E <= 512) APB_ROUTE(32, 16);
+  APB_ROUTE(32, 32);
+#undef APB_ROUTE
+}
+static bool route_args_ok(long long tokens, int E, int k) { return tokens >= 0 && E >= 1 && E <= 1024 && k >= 1 && k <= 32 && k <= E; }
+template <int L>
+static dim3 route_grid(long long tokens) {
+  constexpr int PER = ROUTE_WARPS * (32 / L);
+  return dim3((unsigned)((tokens + PER - 1) / PER));
+}
+
+}  // namespace apb
+
+using namespace apb;
+
+// logits [tokens, E] (bf16 or fp32, rows after each other, 16-byte base), bias fp32 [E] or null -> w fp32 [tokens, k], idx [tokens, k].
+// Returns 0, or an argument / launch error (nothing launched).
+extern "C" int apb_moe_route(const void* logits, const float* bias, float* w, long long* idx, long long tokens, int E, int k, int sigmoid, int groups,
+                             int top_groups, int renorm, float scale, int is_bf16, cudaStream_t st) {
+  if (!route_args_ok(tokens, E, k) || groups < 1 || groups > ROUTE_MAX_GROUPS || E % groups || top_groups < 1 || top_groups > groups ||
+      k > top_groups * (E / groups) || (reinterpret_cast<uintptr_t>(logits) & 15))
+    return 3;
+  if (tokens == 0) return 0;
+  uint32_t mask = 1;
+  while ((int)mask < E - 1) mask = 2 * mask + 1;
+  const RouteParams p{logits, bias, w, idx, tokens, E, k, groups, E / groups, top_groups, renorm, E % (is_bf16 ? 8 : 4) == 0, scale, mask};
+  return route_shape(E, k, [&](auto l, auto v) {
+    constexpr int L = decltype(l)::value, V = decltype(v)::value;
+    auto launch = [&](auto kern) { launch_after(kern, route_grid<L>(tokens), 32 * ROUTE_WARPS, 0, st, p); };
+    if (is_bf16) sigmoid ? launch(moe_route_kernel<__nv_bfloat16, L, V, true>) : launch(moe_route_kernel<__nv_bfloat16, L, V, false>);
+    else sigmoid ? launch(moe_route_kernel<float, L, V, true>) : launch(moe_route_kernel<float, L, V, false>);
+    return cudaGetLastError() == cudaSuccess ? 0 : 4;
+  });
+}
+
+// dw fp32 [tokens, k], logits and dx [tokens, E], idx [tokens, k].
+extern "C" int apb_moe_route_bwd(const float* dw, const void* logits, const long long* idx, void* dx, long long tokens, int E, int k, int sigmoid,
+                                 int renorm, float scale, int is_bf16, cudaStream_t st) {
+  if (!route_args_ok(tokens, E, k) || ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dx)) & 15)) return 3;
+  if (tokens == 0) return 0;
+  const RouteBwdParams p{dw, logits, idx, dx, tokens, E, k, renorm, E % (is_bf16 ? 8 : 4) == 0, scale};
+  return route_shape(E, k, [&](auto l, auto v) {
+    constexpr int L = decltype(l)::value, V = decltype(v)::value;
+    auto launch = [&](auto kern) { launch_after(kern, route_grid<L>(tokens), 32 * ROUTE_WARPS, 0, st, p); };
+    if (is_bf16) sigmoid ? launch(moe_route_bwd_kernel<__nv_bfloat16, L, V, true>) : launch(moe_route_bwd_kernel<__nv_bfloat16, L, V, false>);
+    else sigmoid ? launch(moe_route_bwd_kernel<float, L, V, true>) : launch(moe_route_bwd_kernel<float, L, V, false>);
+    return cudaGetLastError() == cudaSuccess ? 0 : 4;
+  });
+}

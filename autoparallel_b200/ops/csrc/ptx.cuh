@@ -246,6 +246,45 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t cluster_addr) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// ----------------------------------------------------------------------------- block-scaled 4-bit MMA
+// D[tmem] (+)= (A * scale_a) * (B * scale_b): E2M1 operands, K-major, two values a byte, 64 of them along K per MMA; UE8M0 scales for each 32, in
+// TMEM: rows 32 i ... 32 i + 31 in lanes 0 ... 31 (and again in every other lane quarter) of column i, a byte for each of four blocks along K,
+// of which the instruction descriptor names two.
+__device__ __forceinline__ void umma_mx4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa_tmem, uint32_t sb_tmem,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_mx4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa_tmem, uint32_t sb_tmem,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+      : "memory");
+}
+// 32 rows of 16 bytes (512 bytes, 8 rows after each other) from shared memory to 4 TMEM columns of all four lane quarters; in order with the MMAs
+// of the same thread.  The pair form copies in both CTAs, from the same place of their shared memory to the same columns.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Descriptor of those 512 bytes: no swizzle, groups of 8 rows 128 bytes apart.
+__device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+// Instruction descriptor for kind::mxf4 with E2M1 A / B (K-major) and UE8M0 scales; ``blocks``: 0 for the first two scale bytes, 2 for the others.
+__host__ __device__ constexpr uint32_t make_idesc_mx4(uint32_t m, uint32_t n, uint32_t blocks) {
+  return (blocks << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 7) << 27) | (blocks << 29);
+}
+
 // 32 lanes x 32 columns of fp32: thread t of the warp gets lane (base+t), columns [col, col+32).
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(

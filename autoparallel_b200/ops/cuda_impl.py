@@ -308,6 +308,45 @@ def _moe_gate_grad(buf, slot, g):
     return dw
 
 
+# ----------------------------------------------------------------------------------- routing, MXFP4 (these count their own launches)
+def _fp32_result(name, dtype) -> bool:
+    if dtype not in _NATIVE_OUT:
+        raise ValueError(f"{name}: a result of {dtype} is not offered (bf16 or fp32)")
+    return dtype is torch.float32
+
+
+def _moe_route(logits, bias, top_k, sigmoid, num_groups, top_groups, renormalize, scale):
+    return _C.moe_route(logits, bias, top_k, sigmoid, num_groups, top_groups, renormalize, scale)
+
+
+def _moe_route_bwd(dweights, logits, idx, sigmoid, renormalize, scale):
+    return _C.moe_route_bwd(dweights, logits, idx, sigmoid, renormalize, scale)
+
+
+def _mx4_quantize(x):
+    return _C.mx4_quantize(x)
+
+
+def _mx4_dequantize(codes, scales, k, dtype):
+    return _C.mx4_dequantize(codes, scales, k, _fp32_result("mx4_dequantize", dtype))
+
+
+def _mx4_round(x, dim):
+    return _C.mx4_round(x, dim)
+
+
+def _mx4_mm(a, a_scales, b, b_scales, out_dtype):
+    return _C.mx4_mm(a, a_scales, b, b_scales, _fp32_result("mx4_mm", out_dtype), -1)
+
+
+def _mx4_linear(x, codes, scales, out_dtype):
+    return _C.mx4_linear(x, codes, scales, _fp32_result("mx4_linear", out_dtype))
+
+
+def _mx4_matmul(x, w, trans_b, out_dtype):
+    return _C.mx4_matmul(x, w, trans_b, _fp32_result("mx4_matmul", out_dtype))
+
+
 # ----------------------------------------------------------------------------------- pointwise etc.
 def _dtype_cast(x, dtype):
     if x.dtype == dtype:
@@ -482,6 +521,14 @@ def _register() -> None:
     R("moe_gather", _moe_gather)
     R("moe_gate_grad", _moe_gate_grad)
     R("grouped_mm_wgrad", _grouped_mm_wgrad)
+    R("moe_route", _moe_route)
+    R("moe_route_bwd", _moe_route_bwd)
+    R("mx4_quantize", _mx4_quantize)
+    R("mx4_dequantize", _mx4_dequantize)
+    R("mx4_round", _mx4_round)
+    R("mx4_mm", _mx4_mm)
+    R("mx4_linear", _mx4_linear)
+    R("mx4_matmul", _mx4_matmul)
     R("dtype_cast", _dtype_cast)
     R("cast_many", _cast_many)
     R("rms_norm", _rms_norm)

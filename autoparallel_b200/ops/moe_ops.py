@@ -16,6 +16,7 @@ keeps variable-size expert partitions and needs a new ``PartitionedShard`` place
 unaligned all-to-all conversions for them; fixed per-block capacity makes that placement
 unnecessary here.
 
+    moe_route(logits [..,E], bias, k, ...)          -> weights [..,k] fp32, idx [..,k]   (choice of experts, see below)
     moe_slots(gate_idx [T,k], E, C, nb)            -> slot [T,k]   (row of the block's [E*C] buffer, E*C = dropped)
     moe_scatter(src [T,d], slot, w [T,k], E, C, nb) -> buf [E,nb,C,d]   buf[slot[t,j]] = w[t,j] * src[t]
     moe_gather(buf [E,nb,C,d], slot, w [T,k])       -> out [T,d]        out[t] = sum_j w[t,j] * buf[slot[t,j]]
@@ -103,7 +104,87 @@ def _grouped_mm_wgrad(a, b, out_dtype):
     return torch.bmm(a.transpose(1, 2), b).to(out_dtype)
 
 
+# ------------------------------------------------------------------------------------ routing
+# Scores of the experts, the choice of ``top_k`` of them for every token and their gate weights, from router logits [.., E]:
+#
+#   softmax: choice c = x + bias, score s = softmax(x)        sigmoid: s = 1 / (1 + e^-x), c = s + bias
+#   with groups, the experts are cut into ``num_groups`` equal runs; a group counts as its largest c (softmax) or the sum of its two largest (sigmoid), the
+#   ``top_groups`` best groups stay and the others' experts cannot be chosen;
+#   idx = the experts with the ``top_k`` largest c, descending; w = s[idx], divided by their sum if ``renormalize``, times ``scale``
+#
+# Everything in fp32.  Ties (of experts, of groups) go to the lower index; a NaN counts as larger than everything.  The bias balances the load: it
+# enters the choice alone and has no gradient.  A row of nothing but -inf (all experts masked), and a sum of chosen sigmoid scores that is zero, give
+# weights and gradients of zero.  (Reference: softmax or sigmoid scores, the bias for the choice and the scale in the router of the DeepSeek-V3 test
+# model, autoparallel/_testing/models/dsv3.py:388-444.)
+lib.define("moe_route(Tensor logits, Tensor? bias, int top_k, bool sigmoid, int num_groups, int top_groups, bool renormalize, float scale)"
+           " -> (Tensor, Tensor)")
+lib.define("moe_route_bwd(Tensor dweights, Tensor logits, Tensor idx, bool sigmoid, bool renormalize, float scale) -> Tensor")
+
+ROUTE_MAX_EXPERTS, ROUTE_MAX_CHOICES, ROUTE_MAX_GROUPS = 1024, 32, 64
+
+
+def _route_scores(x, sigmoid):
+    if sigmoid:
+        return 1 / (1 + torch.exp(-x))
+    m = x.amax(-1, keepdim=True)
+    e = torch.exp(x - m.masked_fill(m == -torch.inf, 0.0))
+    total = e.sum(-1, keepdim=True)
+    return torch.where(m == -torch.inf, 0.0, e / total)
+
+
+def _moe_route(logits, bias, top_k, sigmoid, num_groups, top_groups, renormalize, scale):
+    x = logits.float().reshape(-1, logits.shape[-1])
+    T, E = x.shape
+    score = _route_scores(x, sigmoid)
+    choice = score if sigmoid else x
+    if bias is not None:
+        choice = choice + bias
+    if num_groups > 1:
+        size = E // num_groups
+        best = choice.view(T, num_groups, size).sort(dim=-1, descending=True).values[..., : 2 if sigmoid else 1].sum(-1)
+        kept = torch.zeros(T, num_groups, dtype=torch.bool, device=x.device)
+        kept.scatter_(1, best.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups], True)
+        out = ~kept.repeat_interleave(size, 1)
+    else:
+        out = torch.zeros_like(choice, dtype=torch.bool)
+    # two stable sorts: by choice, then what cannot be chosen behind the rest
+    order = choice.sort(dim=-1, descending=True, stable=True).indices
+    order = order.gather(1, out.gather(1, order).to(torch.uint8).sort(dim=-1, stable=True).indices)
+    idx = order[:, :top_k]
+    w = score.gather(1, idx)
+    if renormalize:
+        if not sigmoid:  # over the chosen ones alone, so that scores too small for fp32 beside the others do not count as zero
+            xc = x.gather(1, idx)
+            w = _route_scores(xc, False)
+        else:
+            total = w.sum(-1, keepdim=True)
+            w = torch.where(total == 0, 0.0, w / total)
+    return (w * scale).view(*logits.shape[:-1], top_k), idx.view(*logits.shape[:-1], top_k)
+
+
+def _moe_route_bwd(dweights, logits, idx, sigmoid, renormalize, scale):
+    x = logits.float().reshape(-1, logits.shape[-1])
+    k = idx.shape[-1]
+    i, g = idx.reshape(-1, k), dweights.float().reshape(-1, k) * scale
+    if sigmoid:
+        s = 1 / (1 + torch.exp(-x.gather(1, i)))
+        if renormalize:
+            total = s.sum(-1, keepdim=True)
+            g = torch.where(total == 0, 0.0, (g - (g * s / total).sum(-1, keepdim=True)) / total)
+        dx = torch.zeros_like(x).scatter(1, i, g * s * (1 - s))
+    elif renormalize:
+        p = _route_scores(x.gather(1, i), False)
+        dx = torch.zeros_like(x).scatter(1, i, p * (g - (g * p).sum(-1, keepdim=True)))
+    else:
+        p = _route_scores(x, False)
+        ds = torch.zeros_like(x).scatter(1, i, g)
+        dx = p * (ds - (g * p.gather(1, i)).sum(-1, keepdim=True))
+    return dx.to(logits.dtype).view(logits.shape)
+
+
 _REFS = {
+    "moe_route": _moe_route,
+    "moe_route_bwd": _moe_route_bwd,
     "moe_slots": _moe_slots,
     "moe_scatter": _moe_scatter,
     "moe_gather": _moe_gather,
@@ -112,6 +193,8 @@ _REFS = {
     "grouped_mm_wgrad": _grouped_mm_wgrad,
 }
 _META = {
+    "moe_route": lambda x, b, k, *_: (x.new_empty((*x.shape[:-1], k), dtype=torch.float32), x.new_empty((*x.shape[:-1], k), dtype=torch.long)),
+    "moe_route_bwd": lambda dw, x, *_: x.new_empty(x.shape),
     "moe_slots": lambda gi, E, C, nb: gi.new_empty(gi.shape),
     "moe_scatter": lambda src, slot, w, E, C, nb: src.new_empty((E, nb, C, src.shape[1])),
     "moe_gather": lambda buf, slot, w: buf.new_empty((slot.shape[0], buf.shape[3])),
@@ -124,7 +207,7 @@ for _name, _fn in _REFS.items():
     lib.impl(_name, _META[_name], "Meta")
     lib.impl(_name, _make_cuda_entry(_name), "CUDA")
     reference_impls[_name] = _fn
-# On a GPU every operator above resolves to a kernel wrapper of ``ops/cuda_impl.py`` (``csrc/moe_kernels.cu`` for the four index
+# On a GPU every operator above resolves to a kernel wrapper of ``ops/cuda_impl.py`` (``csrc/moe_route.cu``, ``csrc/moe_kernels.cu`` for the four index
 # operators, the grouped tcgen05 GEMM for the products); the formulas in this file are their CPU semantics and the GPU tests' oracle.
 
 
@@ -169,12 +252,47 @@ def _gmm_bwd(ctx, dc):
     return da, db, None, None
 
 
+def _route_setup(ctx, inputs, output):
+    logits, _, _, sigmoid, _, _, renormalize, scale = inputs
+    ctx.save_for_backward(logits, output[1])
+    ctx.mark_non_differentiable(output[1])
+    ctx.how = (sigmoid, renormalize, scale)
+
+
+def _route_bwd(ctx, dweights, _didx):
+    logits, idx = ctx.saved_tensors
+    return (ops.moe_route_bwd(dweights, logits, idx, *ctx.how),) + (None,) * 7
+
+
+_ag("moe_route", _route_bwd, _route_setup)
 _ag("moe_scatter", _scatter_bwd, _scatter_setup)
 _ag("moe_gather", _gather_bwd, _gather_setup)
 _ag("grouped_mm", _gmm_bwd, _gmm_setup)
 
 
 # ------------------------------------------------------------------------------------ Python API
+def moe_route(logits, top_k: int, score: str = "softmax", bias=None, num_groups: int = 1, top_groups: int = 1, renormalize: bool = True,
+              scale: float = 1.0):
+    """(gate weights [.., top_k] fp32, experts [.., top_k] int64) from router logits [.., E] (bf16 or fp32); ``bias`` [E] fp32 enters the choice
+    alone.  The weights are differentiable with respect to the logits."""
+    E = logits.shape[-1] if logits.ndim else 0
+
+    def need(ok, what):
+        if not ok:
+            raise ValueError(f"moe_route: {what}")
+
+    need(logits.dtype in (torch.bfloat16, torch.float32), f"logits are {logits.dtype}; bf16 or fp32 expected")
+    need(score in ("softmax", "sigmoid"), f"score is 'softmax' or 'sigmoid', not {score!r}")
+    need(1 <= E <= ROUTE_MAX_EXPERTS, f"{E} experts (1 to {ROUTE_MAX_EXPERTS})")
+    need(1 <= num_groups <= min(E, ROUTE_MAX_GROUPS) and E % num_groups == 0, f"{E} experts in {num_groups} groups (at most {ROUTE_MAX_GROUPS} equal ones)")
+    need(1 <= top_groups <= num_groups, f"{top_groups} of {num_groups} groups")
+    need(1 <= top_k <= min(ROUTE_MAX_CHOICES, top_groups * (E // num_groups)),
+         f"{top_k} choices out of {top_groups * (E // num_groups)} experts (at most {ROUTE_MAX_CHOICES})")
+    need(bias is None or (tuple(bias.shape) == (E,) and bias.dtype == torch.float32 and bias.device == logits.device),
+         f"bias is fp32 [{E}] on the logits' device")
+    return ops.moe_route(logits, bias, top_k, score == "sigmoid", num_groups, top_groups, renormalize, float(scale))
+
+
 def moe_slots(gate_idx, num_experts: int, capacity: int, num_blocks: int):
     return ops.moe_slots(gate_idx, num_experts, capacity, num_blocks)
 
