@@ -64,6 +64,18 @@ __device__ __forceinline__ void route_load_row(const T* row, int e0, int E, bool
 }
 
 __device__ __forceinline__ float route_sigmoid(float x) { return __frcp_rn(1.0f + expf(-x)); }
+// e^x and the sigmoid from the hardware's approximations: e^x to a few 1e-7 of itself for |x| up to 10 or so, the sigmoid to 5e-7 absolute
+// (the error of e^-x grows with |x|, its weight in the sigmoid falls faster).
+__device__ __forceinline__ float route_exp_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+__device__ __forceinline__ float route_sigmoid_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + route_exp_fast(-x)));
+  return y;
+}
 
 // Order of the floats as unsigned integers.  -0 counts as 0 and every NaN as the same one, larger than all numbers: the sum with 0 makes
 // them so (the result of an addition is the canonical NaN).  0 is smaller than the order of any float.
@@ -92,56 +104,160 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// The experts outside a token's best groups get order 0: they cannot be chosen.
+// How far two choice values have to be apart for their order to be sure, when they come from the fast sigmoid: twice its error, and the rounding of
+// the sum with the bias.
+__device__ __forceinline__ float route_margin(float c) { return 1e-6f + 2.4e-7f * fabsf(c); }
+
+// Orders of the choice values of a lane's experts; 0 for what cannot be chosen.
+template <typename T, int V, bool SIGMOID, bool FAST>
+__device__ __forceinline__ void route_values(const RouteParams& p, int e0, const float (&x)[V], uint32_t (&o)[V]) {
+  float c[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) c[i] = !SIGMOID ? x[i] : FAST ? route_sigmoid_fast(x[i]) : route_sigmoid(x[i]);
+  if (p.bias != nullptr) {
+    if (p.vec) {  // (a multiple of 4 experts: in or out together)
+#pragma unroll
+      for (int i = 0; i < V; i += 4)
+        if (e0 + i < p.E) {
+          const float4 b = *reinterpret_cast<const float4*>(p.bias + e0 + i);
+          c[i] += b.x, c[i + 1] += b.y, c[i + 2] += b.z, c[i + 3] += b.w;
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (e0 + i < p.E) c[i] += p.bias[e0 + i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = e0 + i < p.E ? route_order(c[i]) : 0u;
+}
+
+// The experts outside a token's best groups get order 0.  Returns whether the fast values leave the choice of groups open.
+//
+// Groups of whole lanes (32 of 256 experts on 16 lanes of 16) stay in registers; others go through shared memory, a lane a group.
 template <int L, int V>
-__device__ __forceinline__ void route_groups(const RouteParams& p, bool sigmoid, int warp, int tok, int sub, uint32_t (&o)[V]) {
-  constexpr int TPW = 32 / L, ROW = L * V + L * V / 32 + 1;  // (one word more every 32: groups of 32 begin in different banks)
-  __shared__ uint32_t rows[ROUTE_WARPS][TPW * ROW];
-  __shared__ uint32_t vals[ROUTE_WARPS][TPW * ROUTE_MAX_GROUPS];
-  uint32_t *row = rows[warp] + tok * ROW, *val = vals[warp] + tok * ROUTE_MAX_GROUPS;
-#pragma unroll
-  for (int i = 0; i < V; ++i) row[sub * V + i + (sub * V + i) / 32] = o[i];
-  __syncwarp();
-  for (int g = sub; g < p.groups; g += L) {
+constexpr int route_row_words() { return L * V + L * V / 32 + 1; }  // (one word more every 32: groups of 32 begin in different banks)
+template <int L, int V>
+constexpr int route_smem() { return ROUTE_WARPS * (32 / L) * (route_row_words<L, V>() + ROUTE_MAX_GROUPS) * 4; }
+template <int L, int V, bool SIGMOID, bool FAST>
+__device__ __forceinline__ bool route_groups(const RouteParams& p, int warp, int tok, int sub, uint32_t (&o)[V]) {
+  extern __shared__ uint32_t route_words[];
+  auto value = [&](uint32_t a, uint32_t b) { return SIGMOID && p.size > 1 ? route_order(route_unorder(a) + route_unorder(b)) : a; };
+  uint32_t kept_min = 0xFFFFFFFFu, dropped_max = 0;
+  if (p.size % V == 0) {
+    const int per = p.size / V, g = sub / per, first = g * per;
     uint32_t a = 0, b = 0;
-    for (int i = 0; i < p.size; ++i) {
-      const int e = g * p.size + i;
-      const uint32_t v = row[e + e / 32];
-      b = max(b, min(a, v));
-      a = max(a, v);
-    }
-    val[g] = sigmoid && p.size > 1 ? route_order(route_unorder(a) + route_unorder(b)) : a;
-  }
-  __syncwarp();
-  unsigned long long kept = 0;  // bit i: this lane's i-th group
-  for (int g = sub, i = 0; g < p.groups; g += L, ++i) {
-    const uint32_t mine = val[g];
-    int before = 0;
-    for (int h = 0; h < p.groups; ++h) before += val[h] > mine || (val[h] == mine && h < g);
-    if (before < p.top_groups) kept |= 1ull << i;
-  }
-  __syncwarp();
-  for (int g = sub, i = 0; g < p.groups; g += L, ++i) val[g] = kept >> i & 1;
-  __syncwarp();
-  int g = sub * V / p.size, r = sub * V - g * p.size;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (g < p.groups && !val[g]) o[i] = 0;
-    if (++r == p.size) {
-      r = 0;
-      ++g;
+    for (int i = 0; i < V; ++i) {
+      if (SIGMOID) b = max(b, min(a, o[i]));
+      a = max(a, o[i]);
     }
+    const uint32_t a0 = a, b0 = b;
+    for (int d = 1; d < per; ++d) {
+      const int from = tok * L + first + (sub - first + d) % per;
+      const uint32_t a1 = __shfl_sync(0xffffffffu, a0, from & 31), b1 = __shfl_sync(0xffffffffu, b0, from & 31);
+      b = max(max(b, b1), min(a, a1));
+      a = max(a, a1);
+    }
+    const uint32_t mine = g < p.groups ? value(a, b) : 0u;
+    int before = 0;
+    for (int h = 0; h < p.groups; ++h) {
+      const uint32_t v = __shfl_sync(0xffffffffu, mine, tok * L + h * per);
+      before += v > mine || (v == mine && h < g);
+    }
+    const bool kept = before < p.top_groups;
+    if (kept) kept_min = mine;
+    else dropped_max = mine;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = kept ? o[i] : 0u;
+  } else {
+    constexpr int WORDS = route_row_words<L, V>() + ROUTE_MAX_GROUPS;
+    uint32_t *row = route_words + (warp * (32 / L) + tok) * WORDS, *val = row + route_row_words<L, V>();
+#pragma unroll
+    for (int i = 0; i < V; ++i) row[sub * V + i + (sub * V + i) / 32] = o[i];
+    __syncwarp();
+    for (int g = sub; g < p.groups; g += L) {
+      uint32_t a = 0, b = 0;
+      for (int i = 0; i < p.size; ++i) {
+        const int e = g * p.size + i;
+        const uint32_t v = row[e + e / 32];
+        b = max(b, min(a, v));
+        a = max(a, v);
+      }
+      val[g] = value(a, b);
+    }
+    __syncwarp();
+    unsigned long long kept = 0;  // bit i: this lane's i-th group
+    for (int g = sub, i = 0; g < p.groups; g += L, ++i) {
+      const uint32_t mine = val[g];
+      int before = 0;
+      for (int h = 0; h < p.groups; ++h) before += val[h] > mine || (val[h] == mine && h < g);
+      if (before < p.top_groups) {
+        kept |= 1ull << i;
+        kept_min = min(kept_min, mine);
+      } else {
+        dropped_max = max(dropped_max, mine);
+      }
+    }
+    __syncwarp();
+    for (int g = sub, i = 0; g < p.groups; g += L, ++i) val[g] = kept >> i & 1;
+    __syncwarp();
+    int g = sub * V / p.size, r = sub * V - g * p.size;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (g < p.groups && !val[g]) o[i] = 0;
+      if (++r == p.size) {
+        r = 0;
+        ++g;
+      }
+    }
+    __syncwarp();
   }
-  __syncwarp();
+  if (!SIGMOID || !FAST) return false;
+  const uint32_t lowest = ~lanes_max<L>(~kept_min), highest = lanes_max<L>(dropped_max);
+  if (highest == 0) return false;
+  const float low = route_unorder(lowest);
+  return !(low - route_unorder(highest) > 2.f * route_margin(low));
+}
+
+// Lane j's choice from whole values and numbers: the largest (value, -number) below the last.
+template <int L, int V>
+__device__ __forceinline__ int route_select_exact(const uint32_t (&o)[V], int e0, int k, int sub) {
+  uint32_t lo = 0xFFFFFFFFu;
+  int le = -1, mine = 0;
+  for (int j = 0; j < k; ++j) {
+    uint32_t bo = 0;
+    int be = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if ((o[i] < lo || (o[i] == lo && e0 + i > le)) && o[i] > bo) {
+        bo = o[i];
+        be = e0 + i;
+      }
+#pragma unroll
+    for (int d = 1; d < L; d *= 2) {
+      const uint32_t ho = __shfl_xor_sync(0xffffffffu, bo, d);
+      const int he = __shfl_xor_sync(0xffffffffu, be, d);
+      if (ho > bo || (ho == bo && he < be)) {
+        bo = ho;
+        be = he;
+      }
+    }
+    lo = bo;
+    le = be;
+    if (sub == j) mine = be;
+  }
+  return mine;
 }
 
 // L lanes hold a token, V experts each (lane after lane), and lane j ends up with its j-th choice: k <= L.
 //
 // The choice takes keys in place of the choice values: the upper bits of the value's order, and in the lower b bits (2^b >= E) the expert's number,
 // inverted, so that the larger of two keys is the one to be chosen.  All keys differ, which makes a step of the selection - the largest key below
-// the last - max(key - last) + last in wrapping arithmetic: two instructions a key.  What the lower bits of a value lose matters only
-// where two neighbours in the result (the last chosen and the best of the rest among them) agree in the upper ones: then the warp
-// repeats the selection with whole values and numbers (256 experts, fp32: about 1 token in 100; bf16 logits without bias: never, they have 16 bits).
+// the last - max(key - last) + last in wrapping arithmetic: two instructions a key.  Two things are left out at first: the lower bits of a
+// value, and for sigmoid scores the last bits of a sigmoid, which is taken from the hardware's approximations.  They matter only where neighbours in the
+// result (the last chosen and the best of the rest among them) are closer than that; their exact values tell, and then the warp does the choice
+// again with exact values and numbers (256 experts: about 1 token in 100; bf16 logits without bias: never, the keys have all their 16 bits).
 template <typename T, int L, int V, bool SIGMOID>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_kernel(RouteParams p) {
   after_previous();
@@ -151,76 +267,61 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_kernel(RouteParams
   const bool in = t < p.tokens;
   const T* row = reinterpret_cast<const T*>(p.x) + (in ? t : p.tokens - 1) * p.E;  // (lanes without a token follow the last one)
   const int e0 = sub * V;
-  float x[V];
-  route_load_row<T, V>(row, e0, p.E, p.vec, x);
-  float m_all = -CUDART_INF_F, total_all = 0.f;
-  if (!SIGMOID && !p.renorm) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) m_all = fmaxf(m_all, x[i]);
-    m_all = lanes_max<L>(m_all);
-    if (m_all == -CUDART_INF_F) m_all = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) total_all += expf(x[i] - m_all);
-    total_all = lanes_sum<L>(total_all);
-  }
-  uint32_t o[V], key[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float c = SIGMOID ? route_sigmoid(x[i]) : x[i];
-    if (p.bias != nullptr && e0 + i < p.E) c += p.bias[e0 + i];
-    o[i] = e0 + i < p.E ? route_order(c) : 0u;
-  }
-  if (p.groups > 1) route_groups<L, V>(p, SIGMOID, warp, tok, sub, o);
-#pragma unroll
-  for (int i = 0; i < V; ++i) key[i] = o[i] == 0 ? 0u : (o[i] & ~p.mask) | (p.mask - (e0 + i));
-
-  uint32_t last = 0, mine = 0;
-#pragma unroll
-  for (int i = 0; i < V; ++i) last = max(last, key[i]);
-  last = lanes_max<L>(last);
-  for (int j = 0; j < p.k; ++j) {
-    if (sub == j) mine = last;
-    uint32_t best = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) best = max(best, key[i] - last);
-    last += lanes_max<L>(best);
-  }
   const bool chosen = sub < p.k;
-  int e = chosen ? (int)(p.mask - (mine & p.mask)) : 0;
-  float xe = route_load(row + e);
-  float se = SIGMOID ? route_sigmoid(xe) : 0.f;
-  const bool whole = !SIGMOID && std::is_same<T, __nv_bfloat16>::value && p.bias == nullptr;  // (16 bits of value: the keys have them all)
-  if (!whole) {
+  float m_all = -CUDART_INF_F, total_all = 0.f;
+  uint32_t mine = 0, last = 0;
+  bool unsure;
+  {
+    float x[V];
+    uint32_t o[V], key[V];
+    route_load_row<T, V>(row, e0, p.E, p.vec, x);
+    if (!SIGMOID && !p.renorm) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) m_all = fmaxf(m_all, x[i]);
+      m_all = lanes_max<L>(m_all);
+      if (m_all == -CUDART_INF_F) m_all = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) total_all += route_exp_fast(x[i] - m_all);
+      total_all = lanes_sum<L>(total_all);
+    }
+    route_values<T, V, SIGMOID, true>(p, e0, x, o);
+    unsure = p.groups > 1 && route_groups<L, V, SIGMOID, true>(p, warp, tok, sub, o);
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = o[i] == 0 ? 0u : (o[i] & ~p.mask) | (p.mask - (e0 + i));
+#pragma unroll
+    for (int i = 0; i < V; ++i) last = max(last, key[i]);
+    last = lanes_max<L>(last);
+    for (int j = 0; j < p.k; ++j) {
+      if (sub == j) mine = last;
+      uint32_t best = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) best = max(best, key[i] - last);
+      last += lanes_max<L>(best);
+    }
+    if (sub == p.k) mine = last;  // the best of the rest; 0 if there is none
+  }
+  int e = mine != 0 ? (int)(p.mask - (mine & p.mask)) : 0;
+  float xe = route_load(row + e), se = SIGMOID ? route_sigmoid(xe) : 0.f;
+  if (SIGMOID || std::is_same<T, float>::value || p.bias != nullptr) {
     float c = SIGMOID ? se : xe;
     if (p.bias != nullptr) c += p.bias[e];
-    const uint32_t oe = route_order(c);
-    const uint32_t next_key = __shfl_down_sync(0xffffffffu, mine, 1, L), next_o = __shfl_down_sync(0xffffffffu, oe, 1, L);
-    const bool unsure = sub + 1 < p.k ? ((mine ^ next_key) & ~p.mask) == 0 && oe != next_o : sub + 1 == p.k && ((mine ^ last) & ~p.mask) == 0;
+    const uint32_t next = __shfl_down_sync(0xffffffffu, mine, 1, L);
+    const float next_c = __shfl_down_sync(0xffffffffu, c, 1, L), next_x = __shfl_down_sync(0xffffffffu, xe, 1, L);
+    if (sub + 1 < L) {
+      const bool close = SIGMOID ? !(c - next_c > route_margin(c)) && !(p.bias == nullptr && xe == next_x) : c != next_c;
+      unsure |= chosen && next != 0 && close && (SIGMOID || ((mine ^ next) & ~p.mask) == 0);
+      if (SIGMOID) unsure |= chosen && next != 0 && ((mine ^ next) & ~p.mask) == 0 && c != next_c;
+    } else if (chosen && last != 0) {  // (every lane has a choice: the next key's upper end stands for the best of the rest)
+      const float lo = route_unorder(mine & ~p.mask);
+      unsure |= SIGMOID ? !(lo - route_unorder(last | p.mask) > route_margin(lo)) : ((mine ^ last) & ~p.mask) == 0;
+    }
     if (__any_sync(0xffffffffu, unsure)) {
-      uint32_t lo = 0xFFFFFFFFu;
-      int le = -1;
-      for (int j = 0; j < p.k; ++j) {
-        uint32_t bo = 0;
-        int be = 0;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if ((o[i] < lo || (o[i] == lo && e0 + i > le)) && o[i] > bo) {
-            bo = o[i];
-            be = e0 + i;
-          }
-#pragma unroll
-        for (int d = 1; d < L; d *= 2) {
-          const uint32_t ho = __shfl_xor_sync(0xffffffffu, bo, d);
-          const int he = __shfl_xor_sync(0xffffffffu, be, d);
-          if (ho > bo || (ho == bo && he < be)) {
-            bo = ho;
-            be = he;
-          }
-        }
-        lo = bo;
-        le = be;
-        if (sub == j) e = be;
-      }
+      float x[V];
+      uint32_t o[V];
+      route_load_row<T, V>(row, e0, p.E, p.vec, x);
+      route_values<T, V, SIGMOID, false>(p, e0, x, o);
+      if (p.groups > 1) route_groups<L, V, SIGMOID, false>(p, warp, tok, sub, o);
+      e = route_select_exact<L, V>(o, e0, p.k, sub);
       xe = route_load(row + e);
       se = SIGMOID ? route_sigmoid(xe) : 0.f;
     }
@@ -329,7 +430,7 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_bwd_kernel(RouteBw
     if (m == -CUDART_INF_F) m = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      x[i] = expf(x[i] - m);
+      x[i] = route_exp_fast(x[i] - m);
       total += x[i];
     }
     total = lanes_sum<L>(total);
@@ -386,7 +487,9 @@ extern "C" int apb_moe_route(const void* logits, const float* bias, float* w, lo
   const RouteParams p{logits, bias, w, idx, tokens, E, k, groups, E / groups, top_groups, renorm, E % (is_bf16 ? 8 : 4) == 0, scale, mask};
   return route_shape(E, k, [&](auto l, auto v) {
     constexpr int L = decltype(l)::value, V = decltype(v)::value;
-    auto launch = [&](auto kern) { launch_after(kern, route_grid<L>(tokens), 32 * ROUTE_WARPS, 0, st, p); };
+    const size_t smem = groups > 1 && p.size % V != 0 ? route_smem<L, V>() : 0;
+    static_assert(route_smem<L, V>() <= 48 * 1024, "shared memory without opting in");
+    auto launch = [&](auto kern) { launch_after(kern, route_grid<L>(tokens), 32 * ROUTE_WARPS, smem, st, p); };
     if (is_bf16) sigmoid ? launch(moe_route_kernel<__nv_bfloat16, L, V, true>) : launch(moe_route_kernel<__nv_bfloat16, L, V, false>);
     else sigmoid ? launch(moe_route_kernel<float, L, V, true>) : launch(moe_route_kernel<float, L, V, false>);
     return cudaGetLastError() == cudaSuccess ? 0 : 4;

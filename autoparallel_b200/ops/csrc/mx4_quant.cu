@@ -68,49 +68,52 @@ __device__ __forceinline__ uint32_t mx_encode_block(float (&v)[8], uint32_t code
   return mx_encode(v);
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-template <typename T>
-__device__ __forceinline__ float mx_load(const T* p) {
-  if constexpr (std::is_same<T, float>::value) return *p;
-  else return __bfloat162float(*p);
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if constexpr (std::is_same<T, float>::value) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 4);
-    const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
+// 32 bytes, where both the address and the row lengths allow it in one access (``wide``), otherwise in two.
+__device__ __forceinline__ void load32(const void* p, bool wide, uint32_t (&u)[8]) {
+  if (wide) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+                 : "l"(p));
   } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(u[i] << 16);
-      v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-    }
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+    u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w, u[4] = b.x, u[5] = b.y, u[6] = b.z, u[7] = b.w;
   }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-  if constexpr (std::is_same<T, float>::value) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+__device__ __forceinline__ void store32(void* p, bool wide, const uint32_t (&u)[8]) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
+                 "r"(u[6]), "r"(u[7])
+                 : "memory");
   } else {
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      u[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(u[4], u[5], u[6], u[7]);
   }
 }
 template <typename T>
 __device__ __forceinline__ void store1(T* p, float v) {
   if constexpr (std::is_same<T, float>::value) *p = v;
   else *p = __float2bfloat16(v);
+}
+
+// A word of values: one fp32, or two bf16.  Largest magnitude as bits; value ``i`` of the 32 / sizeof(T) in 8 words; the other way.
+template <typename T>
+__device__ __forceinline__ uint32_t word_max(uint32_t m, uint32_t u) {
+  if constexpr (std::is_same<T, float>::value) return max(m, u & 0x7FFFFFFFu);
+  else return __vmaxu2(m, u & 0x7FFF7FFFu);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t word_max_bits(uint32_t m) {
+  if constexpr (std::is_same<T, float>::value) return m;
+  else return max(m & 0xFFFF0000u, m << 16);
+}
+template <typename T, int N>
+__device__ __forceinline__ float word_value(const uint32_t (&u)[N], int i) {
+  if constexpr (std::is_same<T, float>::value) return __uint_as_float(u[i]);
+  else return __uint_as_float(i & 1 ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16);
+}
+__device__ __forceinline__ uint32_t two_bf16(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 struct MxTile {
@@ -128,62 +131,92 @@ __device__ __forceinline__ MxTile mx_tile(const MxParams& p, uint8_t** scale_til
 // byte of (row, block) in a scale tile
 __device__ __forceinline__ int scale_at(int row, int blk) { return (row & 31) * 16 + (row >> 5) * 4 + blk; }
 
-// Unit stride along K.  A thread has 8 columns of a row, four threads a block, 16 a row of the tile; all its rows are loaded before the first is used.
+// Unit stride along K.  A thread has 32 bytes of a row (16 bf16 or 8 fp32), two or four threads a block; the loads of four rows are under way together.
 // ROUND: the values in place of codes and scales.
 template <typename T, bool ROUND>
 __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
   after_previous();
+  constexpr int PER = 32 / (int)sizeof(T), ROW_THREADS = MX_TILE / PER, PASS = MX_THREADS / ROW_THREADS, ROWS = 4;
   __shared__ __align__(16) uint8_t tile[512];
   uint8_t* scale_tile = nullptr;
   const MxTile at = mx_tile(p, &scale_tile);
-  const int kp = (p.K + 31) / 32 * 32, col = (threadIdx.x & 15) * 8, k = at.k0 + col, r_first = threadIdx.x >> 4;
+  const int kp = (p.K + 31) / 32 * 32, col = (threadIdx.x % ROW_THREADS) * PER, k = at.k0 + col, r_first = threadIdx.x / ROW_THREADS;
   const T* x = reinterpret_cast<const T*>(p.x) + at.g * p.gs;
-  constexpr int ROWS = 4;  // under way together
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float v[ROWS][8];
+  for (int pass = 0; pass < MX_TILE / PASS; pass += ROWS) {
+    uint32_t u[ROWS][8];
+    if (pass > 0 && at.r0 + pass * PASS >= p.R) {  // (whole passes without rows: only their scales are written)
+      if (!ROUND && threadIdx.x < 128) {
+        for (int i = threadIdx.x; i < (MX_TILE - pass * PASS) * 4; i += 128) tile[scale_at(pass * PASS + i / 4, i & 3)] = 127;
+      }
+      break;
+    }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int r = at.r0 + r_first + 16 * (ROWS * half + i);
+      const int r = at.r0 + r_first + PASS * (pass + i);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) v[i][c] = 0.f;
+      for (int c = 0; c < 8; ++c) u[i][c] = 0;
       if (r < p.R) {
         const T* src = x + r * p.ld + k;
         if (p.vec) {
-          if (k < p.K) load8(src, v[i]);
+          if (k + PER <= p.K) {
+            load32(src, p.vec > 1, u[i]);
+          } else if (k < p.K) {  // (rows of whole 16 bytes)
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            u[i][0] = v.x, u[i][1] = v.y, u[i][2] = v.z, u[i][3] = v.w;
+          }
         } else {
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            if (k + c < p.K) v[i][c] = mx_load(src + c);
+          for (int c = 0; c < PER; ++c)
+            if (k + c < p.K) {
+              if constexpr (std::is_same<T, float>::value) u[i][c] = __float_as_uint(src[c]);
+              else u[i][c / 2] |= (uint32_t)__bfloat16_as_ushort(src[c]) << (16 * (c & 1));
+            }
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int rr = r_first + 16 * (ROWS * half + i), r = at.r0 + rr;
-      uint32_t amax = 0;
+      const int rr = r_first + PASS * (pass + i), r = at.r0 + rr;
+      uint32_t m = 0;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) amax = max(amax, abs_bits(v[i][c]));
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      for (int c = 0; c < 8; ++c) m = word_max<T>(m, u[i][c]);
+      uint32_t amax = word_max_bits<T>(m);
+#pragma unroll
+      for (int d = 1; d < 32 / PER; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
       const uint32_t code = mx_scale_code(amax);
-      const uint32_t packed = mx_encode_block(v[i], code);
       const bool in = r < p.R && k < kp;
-      if (ROUND) {
-        if (in) {
-          mx_decode(packed, mx_scale(code), v[i]);
-          T* dst = reinterpret_cast<T*>(p.y) + (at.g * p.R + r) * p.K + k;
-          if (p.vec) {
-            if (k < p.K) store8(dst, v[i]);
-          } else {
+      uint32_t packed[PER / 8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              if (k + c < p.K) store1(dst + c, v[i][c]);
-          }
+      for (int h = 0; h < PER / 8; ++h) {
+        float v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = word_value<T>(u[i], 8 * h + c);
+        packed[h] = mx_encode_block(v, code);
+        if (ROUND) {
+          mx_decode(packed[h], mx_scale(code), v);
+#pragma unroll
+          for (int c = 0; c < (PER == 8 ? 8 : 4); ++c) u[i][(PER == 8 ? 0 : 4 * h) + c] = PER == 8 ? __float_as_uint(v[c]) : two_bf16(v[2 * c & 7], v[(2 * c & 7) + 1]);
+        }
+      }
+      if (ROUND) {
+        T* dst = reinterpret_cast<T*>(p.y) + (at.g * p.R + r) * p.K + k;
+        if (!in) continue;
+        if (p.vec) {
+          if (k + PER <= p.K) store32(dst, p.vec > 1, u[i]);
+          else if (k < p.K) *reinterpret_cast<uint4*>(dst) = make_uint4(u[i][0], u[i][1], u[i][2], u[i][3]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < PER; ++c)
+            if (k + c < p.K) store1(dst + c, word_value<T>(u[i], c));
         }
       } else {
-        if (in) *reinterpret_cast<uint32_t*>(p.codes + (at.g * p.R + r) * (kp / 2) + k / 2) = packed;
-        if ((threadIdx.x & 3) == 0) tile[scale_at(rr, col / 32)] = (uint8_t)(in ? code : 127u);
+        if (in) {
+          uint8_t* dst = p.codes + (at.g * p.R + r) * (kp / 2) + k / 2;
+          if constexpr (PER == 16) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
+          else *reinterpret_cast<uint32_t*>(dst) = packed[0];
+        }
+        if (col % 32 == 0) tile[scale_at(rr, col / 32)] = (uint8_t)(in ? code : 127u);
       }
     }
   }
@@ -198,77 +231,89 @@ template <typename T, bool ROUND>
 __global__ void __launch_bounds__(MX_THREADS) mx4_columns_kernel(MxParams p) {
   after_previous();
   constexpr int STRIDE = 80;  // bytes of a row of codes in shared memory (64 used)
+  constexpr int W = 2 * (int)sizeof(T) / 4;  // words of two rows in a column
   __shared__ __align__(16) uint8_t tile[512];
   __shared__ __align__(16) uint8_t rows[ROUND ? 16 : MX_TILE * STRIDE];
   uint8_t* scale_tile = nullptr;
   const MxTile at = mx_tile(p, &scale_tile);
   const int kp = (p.K + 31) / 32 * 32, rr = (threadIdx.x & 63) * 2, r = at.r0 + rr, blk = threadIdx.x >> 6, k = at.k0 + blk * 32;
   const T* x = reinterpret_cast<const T*>(p.x) + at.g * p.gs + r;
-  float v[2][32];
+  uint32_t u[32][W];
+  const bool whole = p.vec && k + 32 <= p.K && r < p.R;
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    v[0][i] = v[1][i] = 0.f;
-    if (k + i < p.K) {
-      const T* src = x + (k + i) * p.ld;
-      if (p.vec) {
-        if (r < p.R) {
-          if constexpr (std::is_same<T, float>::value) {
-            const float2 f = *reinterpret_cast<const float2*>(src);
-            v[0][i] = f.x;
-            v[1][i] = f.y;
-          } else {
-            const uint32_t u = *reinterpret_cast<const uint32_t*>(src);
-            v[0][i] = __uint_as_float(u << 16);
-            v[1][i] = __uint_as_float(u & 0xFFFF0000u);
-          }
-        }
+    for (int i = 0; i < 32; ++i) {
+      const T* src = x + (long long)(k + i) * p.ld;
+      if constexpr (W == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(src);
+        u[i][0] = v.x, u[i][1] = v.y;
       } else {
-        if (r < p.R) v[0][i] = mx_load(src);
-        if (r + 1 < p.R) v[1][i] = mx_load(src + 1);
+        u[i][0] = *reinterpret_cast<const uint32_t*>(src);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const T* src = x + (long long)(k + i) * p.ld;
+#pragma unroll
+      for (int w = 0; w < W; ++w) u[i][w] = 0;
+      if (k + i < p.K) {
+        if constexpr (W == 2) {
+          if (r < p.R) u[i][0] = __float_as_uint(src[0]);
+          if (r + 1 < p.R) u[i][1] = __float_as_uint(src[1]);
+        } else {
+          if (r < p.R) u[i][0] = __bfloat16_as_ushort(src[0]);
+          if (r + 1 < p.R) u[i][0] |= (uint32_t)__bfloat16_as_ushort(src[1]) << 16;
+        }
       }
     }
   }
+  uint32_t m[W] = {};
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+#pragma unroll
+    for (int w = 0; w < W; ++w) m[w] = word_max<T>(m[w], u[i][w]);
+  uint32_t code[2], packed[2][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) amax = max(amax, abs_bits(v[h][i]));
-    const uint32_t code = mx_scale_code(amax);
-    uint32_t packed[4];
+    code[h] = mx_scale_code(W == 2 ? m[W == 2 ? h : 0] : h == 0 ? m[0] << 16 : m[0] & 0xFFFF0000u);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      float w[8];
+      float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = v[h][8 * q + i];
-      packed[q] = mx_encode_block(w, code);
-      if (ROUND) {
-        mx_decode(packed[q], mx_scale(code), w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[h][8 * q + i] = w[i];
-      }
-    }
-    if (!ROUND) {
-      *reinterpret_cast<uint4*>(rows + (rr + h) * STRIDE + blk * 16) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-      tile[scale_at(rr + h, blk)] = (uint8_t)(r + h < p.R && k < kp ? code : 127u);
+      for (int i = 0; i < 8; ++i) v[i] = word_value<T>(u[8 * q + i], h);
+      packed[h][q] = mx_encode_block(v, code[h]);
     }
   }
   if (ROUND) {
     T* y = reinterpret_cast<T*>(p.y) + at.g * p.R * p.K + r;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      if (k + i >= p.K) break;
-      T* dst = y + (long long)(k + i) * p.R;
-      if (p.vec) {
-        if (r < p.R) {
-          if constexpr (std::is_same<T, float>::value) *reinterpret_cast<float2*>(dst) = make_float2(v[0][i], v[1][i]);
-          else *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(v[0][i], v[1][i]);
+    for (int q = 0; q < 4; ++q) {
+      float a[8], b[8];
+      mx_decode(packed[0][q], mx_scale(code[0]), a);
+      mx_decode(packed[1][q], mx_scale(code[1]), b);
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          T* dst = y + (long long)(k + 8 * q + i) * p.R;
+          if constexpr (W == 2) *reinterpret_cast<float2*>(dst) = make_float2(a[i], b[i]);
+          else *reinterpret_cast<uint32_t*>(dst) = two_bf16(a[i], b[i]);
         }
       } else {
-        if (r < p.R) store1(dst, v[0][i]);
-        if (r + 1 < p.R) store1(dst + 1, v[1][i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          T* dst = y + (long long)(k + 8 * q + i) * p.R;
+          if (k + 8 * q + i < p.K && r < p.R) store1(dst, a[i]);
+          if (k + 8 * q + i < p.K && r + 1 < p.R) store1(dst + 1, b[i]);
+        }
       }
     }
   } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      *reinterpret_cast<uint4*>(rows + (rr + h) * STRIDE + blk * 16) = make_uint4(packed[h][0], packed[h][1], packed[h][2], packed[h][3]);
+      tile[scale_at(rr + h, blk)] = (uint8_t)(r + h < p.R && k < kp ? code[h] : 127u);
+    }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -281,6 +326,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_columns_kernel(MxParams p) {
   }
 }
 
+// A thread has 16 values of a row: 8 bytes of codes, all its rows under way together.
 template <typename T>
 __global__ void __launch_bounds__(MX_THREADS) mx4_dequantize_kernel(MxParams p) {
   after_previous();
@@ -288,27 +334,37 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_dequantize_kernel(MxParams p) 
   uint8_t* scale_tile = nullptr;
   const MxTile at = mx_tile(p, &scale_tile);
   if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(tile)[threadIdx.x] = reinterpret_cast<const uint32_t*>(scale_tile)[threadIdx.x];
-  const int kp = (p.K + 31) / 32 * 32, col = (threadIdx.x & 15) * 8, k = at.k0 + col, r_first = threadIdx.x >> 4;
-  uint32_t packed[8];
+  const int kp = (p.K + 31) / 32 * 32, col = (threadIdx.x & 7) * 16, k = at.k0 + col, r_first = threadIdx.x >> 3;
+  uint2 packed[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = at.r0 + r_first + 16 * i;
-    packed[i] = 0;
-    if (r < p.R && k < p.K) packed[i] = *reinterpret_cast<const uint32_t*>(p.codes + (at.g * p.R + r) * (kp / 2) + k / 2);
+  for (int i = 0; i < 4; ++i) {
+    const int r = at.r0 + r_first + 32 * i;
+    packed[i] = make_uint2(0, 0);
+    if (r < p.R && k < p.K) packed[i] = *reinterpret_cast<const uint2*>(p.codes + (at.g * p.R + r) * (kp / 2) + k / 2);
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int rr = r_first + 16 * i, r = at.r0 + rr;
+  for (int i = 0; i < 4; ++i) {
+    const int rr = r_first + 32 * i, r = at.r0 + rr;
     if (r >= p.R || k >= p.K) continue;
-    float v[8];
-    mx_decode(packed[i], mx_scale(tile[scale_at(rr, col / 32)]), v);
+    const float scale = mx_scale(tile[scale_at(rr, col / 32)]);
+    float v[16];
+    float (&lo)[8] = *reinterpret_cast<float (*)[8]>(v), (&hi)[8] = *reinterpret_cast<float (*)[8]>(v + 8);
+    mx_decode(packed[i].x, scale, lo);
+    mx_decode(packed[i].y, scale, hi);
     T* dst = reinterpret_cast<T*>(p.y) + (at.g * p.R + r) * p.K + k;
-    if (p.vec) {
-      store8(dst, v);
+    if (p.vec && k + 16 <= p.K) {
+      constexpr int PER = 32 / (int)sizeof(T);
+#pragma unroll
+      for (int h = 0; h < 16 / PER; ++h) {
+        uint32_t u[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) u[c] = PER == 8 ? __float_as_uint(v[(PER == 8 ? 8 * h : 0) + c]) : two_bf16(v[2 * c], v[2 * c + 1]);
+        store32(dst + PER * h, p.vec > 1, u);
+      }
     } else {
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
+      for (int c = 0; c < 16; ++c)
         if (k + c < p.K) store1(dst + c, v[c]);
     }
   }
@@ -337,7 +393,9 @@ static int mx_from_values(MxParams& p, unsigned grid, int transposed, int is_bf1
     is_bf16 ? launch_after(mx4_columns_kernel<__nv_bfloat16, ROUND>, grid, MX_THREADS, 0, st, p)
             : launch_after(mx4_columns_kernel<float, ROUND>, grid, MX_THREADS, 0, st, p);
   } else {
-    p.vec = p.ld * esz % 16 == 0 && p.gs * esz % 16 == 0 && p.K % 8 == 0 && aligned(p.x, 16);
+    // rows that begin on 32 or on 16 bytes, and end there (so do those of the result)
+    auto whole = [&](int bytes) { return p.ld * esz % bytes == 0 && p.gs * esz % bytes == 0 && (long long)p.K * esz % bytes == 0 && aligned(p.x, bytes) && (!ROUND || aligned(p.y, bytes)); };
+    p.vec = whole(32) ? 2 : whole(16) ? 1 : 0;
     is_bf16 ? launch_after(mx4_rows_kernel<__nv_bfloat16, ROUND>, grid, MX_THREADS, 0, st, p)
             : launch_after(mx4_rows_kernel<float, ROUND>, grid, MX_THREADS, 0, st, p);
   }
@@ -384,7 +442,8 @@ extern "C" int apb_mx4_dequantize(const void* codes, const void* scales, void* y
   p.codes = (uint8_t*)const_cast<void*>(codes);
   p.scales = (uint8_t*)const_cast<void*>(scales);
   p.y = y;
-  p.vec = K % 8 == 0;
+  const int esz = is_bf16 ? 2 : 4;
+  p.vec = K * esz % 32 == 0 && aligned(y, 32) ? 2 : K * esz % 16 == 0 ? 1 : 0;
   is_bf16 ? launch_after(mx4_dequantize_kernel<__nv_bfloat16>, grid, MX_THREADS, 0, st, p)
           : launch_after(mx4_dequantize_kernel<float>, grid, MX_THREADS, 0, st, p);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
