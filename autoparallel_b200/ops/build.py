@@ -23,7 +23,7 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
 ]
 # Sources whose results hang on the last bit of a formula, or on denormals: compiled without fast math.
-EXACT_MATH = {"moe_route.cu", "mx4_quant.cu"}
+EXACT_MATH = {"moe_route.cu", "mx4_quant.cu", "gemm_mx4_rows.cu"}
 # The C++ library is the shared one that torch has loaded.  A compiler that ships only libstdc++.a would put a second copy
 # into the extension; streams of one copy then use the locale of the other, and formatting the number in an error message
 # ends the process instead of raising.

@@ -11,16 +11,12 @@
 // 192 ... 447, scales from 448 on.  The epilogue reads the shared columns first, and the next tile's MMAs start as soon as that is done.
 #include <algorithm>
 
-#include "gemm_core.cuh"
+#include "mx4.cuh"
 
 namespace apb {
 
-constexpr int MX_BK = 256, MX_ROW_BYTES = MX_BK / 2;         // values and bytes of K in a stage
-constexpr int MX_SCALE_TILE = 512, MX_STAGE_TILES = 2;       // bytes of a scale tile, and how many lie along a stage
 constexpr int MX_ACC1 = 192, MX_SCALE_COL = 448;  // first columns of the second accumulator and of the scales
 constexpr int MX_EPI_WARPS = 8, MX_GEMM_THREADS = 64 + 32 * MX_EPI_WARPS;
-constexpr int MX_OP_BYTES = 128 * MX_ROW_BYTES;              // 128 rows of an operand
-constexpr int MX_SC_BYTES = MX_STAGE_TILES * MX_SCALE_TILE;  // and their scales
 constexpr int MX_STAGING = MX_EPI_WARPS * 4096;
 constexpr int MX_BAR_BYTES = 256;
 
@@ -36,8 +32,15 @@ struct MxShape {
 struct MxGemmParams {
   GemmParams p;  // M, N, C, ldc, out_fp32, status and the tile order
   int tiles, num_m, num_kb, k_steps;  // k_steps: MMAs of 64 along K
-  int col_tile, vec_store, grouped;
+  int col_tile, store, grouped;
 };
+enum : int { MX_SCALAR = 0, MX_STAGED = 1, MX_DIRECT = 2 };
+
+__device__ __forceinline__ void st_32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+               "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 
 // Epilogue of a warp's 32 rows and ``ncols`` columns, 64 at a time, from column ``c_first`` up or down; ``release`` after the first 64.
 template <typename Release>
@@ -57,6 +60,27 @@ __device__ __forceinline__ void mx_store(const MxGemmParams& q, uint8_t* C, uint
     tmem_ld_wait_for(r[0]);
     tmem_ld_wait_for(r[1]);
     if (early && i == 0) release();
+    if (q.store == MX_DIRECT) {
+      uint8_t* dst = C + ((row0 + lane) * p.ldc + n0 + c) * esz;
+      if (row0 + lane < p.M) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 32; j += 16) {
+            const int col = n0 + c + 32 * h + j;
+            if (p.out_fp32) {
+              if (col < p.N) st_32(dst + (32 * h + j) * 4, r[h] + j);
+              if (col + 8 < p.N) st_32(dst + (32 * h + j + 8) * 4, r[h] + j + 8);
+            } else if (col < p.N) {
+              uint32_t v[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = pack_bf16(__uint_as_float(r[h][j + 2 * e]), __uint_as_float(r[h][j + 2 * e + 1]));
+              st_32(dst + (32 * h + j) * 2, v);
+            }
+          }
+      }
+      continue;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // fp32: 32 columns at a time; bf16: all 64 in the first
       if (h == 1 && !p.out_fp32) break;
@@ -77,7 +101,7 @@ __device__ __forceinline__ void mx_store(const MxGemmParams& q, uint8_t* C, uint
       for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = v[j];
       __syncwarp();
       const int col0 = n0 + c + 32 * h;  // of the 128 bytes
-      if (q.vec_store) {
+      if (q.store == MX_STAGED) {
         const int unit = lane & 7, sub = lane >> 3, col = col0 + unit * (16 / esz);
 #pragma unroll 4
         for (int j = 0; j < 8; ++j) {
@@ -324,25 +348,12 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   mx_gemm_cta<true, 1>(tmA, tmB, tmSA, tmSB, q, smem_raw);
 }
 
-// [G][rows][bytes] of codes in boxes of 128 bytes x ``box_rows`` (128-byte swizzle), or [G][row tiles][scale words] in boxes of a stage's words.
-static int mx_map(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t rows, uint64_t G, uint32_t box_inner, uint32_t box_rows, bool scales) {
-  EncodeTiledFn enc = get_encode();
-  if (!enc) return 1;
-  const uint64_t esz = scales ? 4 : 1;
-  cuuint64_t dims[3] = {inner, rows, G};
-  cuuint64_t strides[2] = {inner * esz, inner * rows * esz};
-  cuuint32_t box[3] = {box_inner, box_rows, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(m, scales ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, scales ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : 2;
-}
-
 }  // namespace apb
 
 using namespace apb;
 
+static int g_force_staged = 0;
+extern "C" void apb_mx4_staged(int on) { g_force_staged = on; }
 extern "C" int apb_gemm_resident_pairs(int num_sms);
 extern "C" int apb_gemm_get_reserved_sms();
 
@@ -367,7 +378,8 @@ extern "C" int apb_gemm_mx4(const void* A, const void* SA, const void* B, const 
   p.out_fp32 = out_fp32;
   p.status = status;
   q.col_tile = form == 0 ? 128 : 256;
-  q.vec_store = N % (out_fp32 ? 4 : 8) == 0;
+  const long long row_bytes = N * (out_fp32 ? 4 : 2);
+  q.store = row_bytes % 32 == 0 && (reinterpret_cast<uintptr_t>(C) & 31) == 0 && !g_force_staged ? MX_DIRECT : row_bytes % 16 == 0 ? MX_STAGED : MX_SCALAR;
   q.grouped = G > 1;
   q.num_m = (int)((M + (pair ? 255 : 127)) / (pair ? 256 : 128));
   p.num_n_tiles = (int)((N + q.col_tile - 1) / q.col_tile);

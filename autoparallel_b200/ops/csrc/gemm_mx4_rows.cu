@@ -1,0 +1,359 @@
+// MXFP4 products with few rows of A, sm_100a: a projection of some tokens (decoding), with the rounding of the activations in the same launch.
+//
+//   C[g][M, N] = A[g][M, K] * B[g][N, K]^T, M <= 32; B in 4 bits; A bf16 or fp32 values that are rounded here, or codes and scales
+//
+// Bound by reading B once.  B's rows take the 128 rows of the MMA and A's few rows its N, so that a stage brings in 16 KB of B and next to
+// nothing of A.  A cluster of S CTAs takes a slice of K each for one tile of 128 rows of B: with as many CTAs as two to an SM, all of B's bytes that
+// fit the chip's shared memory are on their way as soon as the launch has begun.  The slices' sums meet in shared memory: every CTA sends each other
+// one its share of the rows, and adds up what it gets in the order of the slices - the same result every time.
+//   warp 0: TMA producer | warp 1: TMEM owner, scale copies, MMAs | warps 2..9: rounding of A, a stage a warp, then the epilogue
+#include <algorithm>
+
+#include "mx4.cuh"
+
+namespace apb {
+
+constexpr int MR_WARPS = 8, MR_THREADS = 64 + 32 * MR_WARPS, MR_MAX_STAGES = 8;
+constexpr int MR_SMEM = 112 * 1024;  // two CTAs to an SM
+
+struct MxRowsParams {
+  const void* x;  // values of A (rounded here), or null
+  void* C;
+  int M, N, K, n_tiles, num_kb, k_steps, slices, stages, vec, out_fp32;
+  long long gs, ld;
+  uint32_t* status;
+};
+
+// NT: columns of the MMA (rows of A, padded)
+template <int NT>
+struct MxRowsShape {
+  static constexpr int STAGE = MX_OP_BYTES + 2 * MX_SC_BYTES + NT * MX_ROW_BYTES;
+  static constexpr int PART = NT * 128 * 4;  // sums of all slices for a CTA's share of the rows
+  static constexpr int STAGES = std::min(MR_MAX_STAGES, (MR_SMEM - 1024 - 256 - PART) / STAGE);
+  static constexpr int SMEM = 1024 + STAGES * STAGE + PART + 256;
+  static constexpr uint32_t COLS = NT <= 16 ? 32 : 2 * NT;  // TMEM: NT of sums, 16 of scales
+};
+
+// Four rows of a stage of A, one warp: a lane has 8 values of each, four lanes a block.
+template <typename T>
+struct MxRowsUnit {
+  static constexpr int W = 8 * (int)sizeof(T) / 4;
+  uint32_t u[4][W];
+  __device__ __forceinline__ void load(const MxRowsParams& p, const T* x, int r0, int k) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int c = 0; c < W; ++c) u[i][c] = 0;
+      if (r0 + i >= p.M) continue;
+      const T* src = x + (r0 + i) * p.ld + k;
+      if (p.vec) {
+        if (k < p.K) {
+#pragma unroll
+          for (int c = 0; c < W; c += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(src) + c);
+            u[i][c] = v.x, u[i][c + 1] = v.y, u[i][c + 2] = v.z, u[i][c + 3] = v.w;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (k + c < p.K) mx_put(u[i], c, src[c]);
+      }
+    }
+  }
+  __device__ __forceinline__ void round(const MxRowsParams& p, int r0, uint8_t* op, uint8_t* sc, int lane) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + i;
+      if (r >= p.M) break;
+      uint32_t m = 0;
+#pragma unroll
+      for (int c = 0; c < W; ++c) m = mx_word_max<T>(m, u[i][c]);
+      uint32_t amax = mx_word_max_bits<T>(m);
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const uint32_t code = mx_scale_code(amax);
+      float v[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] = mx_word_value<T>(u[i], c);
+      *reinterpret_cast<uint32_t*>(op + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = mx_encode_block(v, code);
+      if ((lane & 3) == 0) sc[(lane >> 4) * MX_SCALE_TILE + mx_scale_at(r, lane >> 2 & 3)] = (uint8_t)code;
+    }
+  }
+};
+
+template <int NT, typename T>  // T: type of A's values; void: codes
+__global__ void __launch_bounds__(MR_THREADS, 2)
+gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSB, const __grid_constant__ CUtensorMap tmA,
+                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ MxRowsParams p) {
+  using S = MxRowsShape<NT>;
+  constexpr bool VALUES = !std::is_same<T, void>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sB = smem;                                       // [stages] 16 KB of B, then
+  uint8_t* sA = sB + p.stages * MX_OP_BYTES;                // [stages] NT rows of A, then
+  uint8_t* sSc = sA + p.stages * NT * MX_ROW_BYTES;         // [stages] scales of B, of A
+  float* part = reinterpret_cast<float*>(sSc + p.stages * 2 * MX_SC_BYTES);  // [slices][NT][rows of this CTA's share]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(part) + S::PART);
+  uint64_t *full = bars, *empty = bars + MR_MAX_STAGES, *acc_full = bars + 2 * MR_MAX_STAGES, *parts_in = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(parts_in + 1);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  static_assert((2 * MR_MAX_STAGES + 3) * 8 <= 256, "barrier block");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = p.slices > 1 ? (int)cluster_ctarank() : 0, tile_id = blockIdx.x / p.slices;
+  const int grp = tile_id / p.n_tiles, n0 = (tile_id - grp * p.n_tiles) * 128;
+  const int kb0 = p.num_kb * rank / p.slices, kb1 = p.num_kb * (rank + 1) / p.slices;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full[s], VALUES ? 1 + (p.M + 3) / 4 : 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(parts_in, p.slices * MR_WARPS);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmSB);
+    if (!VALUES) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmSA);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, S::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (p.slices > 1) {
+    cluster_arrive();  // every CTA's barriers are there before a peer's sums arrive
+    cluster_wait();
+  }
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  wait_previous();
+
+  auto fail = [&](uint32_t code) {
+    atomicCAS(p.status, 0u, code);
+    *abort_flag = 1;
+  };
+  if (warp == 0) {
+    if (elect_one()) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, stage = i % p.stages;
+        if (!mbar_wait(&empty[stage], (i / p.stages & 1) ^ 1, abort_flag)) {
+          fail(ST_TIMEOUT_EMPTY);
+          break;
+        }
+        mbar_expect_tx(&full[stage], MX_OP_BYTES + MX_SC_BYTES + (VALUES ? 0 : NT * MX_ROW_BYTES + MX_SC_BYTES));
+        uint8_t* sc = sSc + stage * 2 * MX_SC_BYTES;
+        tma_load_3d(sB + stage * MX_OP_BYTES, &tmB, &full[stage], kb * MX_ROW_BYTES, n0, grp);
+        tma_load_3d(sc, &tmSB, &full[stage], kb * (MX_SC_BYTES / 4), n0 / 128, grp);
+        if (!VALUES) {
+          tma_load_3d(sA + stage * NT * MX_ROW_BYTES, &tmA, &full[stage], kb * MX_ROW_BYTES, 0, grp);
+          tma_load_3d(sc + MX_SC_BYTES, &tmSA, &full[stage], kb * (MX_SC_BYTES / 4), 0, grp);
+        }
+      }
+      let_next_in();
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc[2] = {make_idesc_mx4(128, NT, 0), make_idesc_mx4(128, NT, 2)};
+      const uint64_t b_desc = make_smem_desc(smem_u32(sB), 16, 1024), a_desc = make_smem_desc(smem_u32(sA), 16, 1024);
+      const uint64_t sc_desc = make_scale_desc(smem_u32(sSc));
+      const uint32_t sb_tmem = tmem + NT, sa_tmem = sb_tmem + 4 * MX_STAGE_TILES;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, stage = i % p.stages;
+        if (!mbar_wait(&full[stage], i / p.stages & 1, abort_flag)) {
+          ok = false;
+          fail(ST_TIMEOUT_FULL);
+          break;
+        }
+        tc_fence_after();
+        const int steps = min(MX_BK / 64, p.k_steps - kb * (MX_BK / 64));
+#pragma unroll
+        for (int a = 0; a < MX_STAGE_TILES; ++a) {
+          tmem_copy_scales(sb_tmem + 4 * a, sc_desc + desc_offset(stage * 2 * MX_SC_BYTES + a * MX_SCALE_TILE));
+          tmem_copy_scales(sa_tmem + 4 * a, sc_desc + desc_offset(stage * 2 * MX_SC_BYTES + MX_SC_BYTES + a * MX_SCALE_TILE));
+        }
+#pragma unroll
+        for (int s = 0; s < MX_BK / 64; ++s) {
+          if (s >= steps) break;
+          umma_mx4(tmem, b_desc + desc_offset(stage * MX_OP_BYTES + 32 * s), a_desc + desc_offset(stage * NT * MX_ROW_BYTES + 32 * s), idesc[s & 1],
+                   sb_tmem + 4 * (s / 2), sa_tmem + 4 * (s / 2), i > 0 || s > 0 ? 1u : 0u);
+        }
+        umma_commit(&empty[stage]);
+      }
+      if (ok) umma_commit(acc_full);
+    }
+  } else {
+    const int w = warp - 2;
+    if constexpr (VALUES) {
+      const T* x = reinterpret_cast<const T*>(p.x) + grp * p.gs;
+      // Units of four rows of a stage.  Every unit of a ring slot belongs to one warp, in every round of the ring: a warp that skipped a round could
+      // not tell from a barrier's parity whether the slot is free or two rounds behind.
+      const int groups = (p.M + 3) / 4, units = p.stages * groups, count = kb1 - kb0;
+      struct At {
+        int round, unit;
+      };
+      auto stage_of = [&](const At& a) { return a.unit / groups; };
+      auto block_of = [&](const At& a) { return a.round * p.stages + stage_of(a); };  // k-block of this CTA
+      auto after = [&](At a) {
+        a.unit += MR_WARPS;
+        if (a.unit >= units) a = {a.round + 1, w};
+        return a;
+      };
+      auto load = [&](MxRowsUnit<T>& u, const At& a) {
+        if (block_of(a) < count) u.load(p, x, a.unit % groups * 4, (kb0 + block_of(a)) * MX_BK + lane * 8);
+      };
+      MxRowsUnit<T> next;
+      At at{0, w};
+      const int rounds = w < units ? (count + p.stages - 1) / p.stages : 0;
+      if (rounds > 0) load(next, at);
+      while (at.round < rounds) {
+        const MxRowsUnit<T> unit = next;
+        const At then = after(at);
+        if (then.round < rounds) load(next, then);
+        if (block_of(at) < count) {
+          const int stage = stage_of(at);
+          if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], (at.round & 1) ^ 1, abort_flag))) {
+            fail(ST_TIMEOUT_EMPTY);
+            break;
+          }
+          unit.round(p, at.unit % groups * 4, sA + stage * NT * MX_ROW_BYTES, sSc + stage * 2 * MX_SC_BYTES + MX_SC_BYTES, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[stage]);
+        }
+        at = then;
+      }
+    }
+    // ---- epilogue: a warp has 32 rows of B (a TMEM lane quarter) and half of A's rows
+    const int quarter = warp & 3, half = w >> 2, share = 128 / p.slices;  // share: rows of B that a CTA of the cluster adds up
+    const bool done = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_flag));
+    if (!done) fail(ST_TIMEOUT_TMEM_FULL);
+    tc_fence_after();
+    if (done) {
+      const int row = quarter * 32 + lane, owner = row / share;
+      const uint32_t dst = p.slices > 1 ? map_to_cta(part + (rank * NT) * share + row % share, owner) : smem_u32(part + row);
+      constexpr int COLS = NT / 2;
+#pragma unroll
+      for (int c0 = 0; c0 < COLS; c0 += 8) {
+        if (half * COLS + c0 >= p.M) break;
+        uint32_t r[8];
+        tmem_ld_32x8(tmem + (uint32_t(quarter * 32) << 16) + half * COLS + c0, r);
+        tmem_ld_wait_for8(r);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t at = dst + (half * COLS + c0 + c) * share * 4;
+          if (p.slices > 1) st_cluster_u32(at, r[c]);
+          else asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(r[c]) : "memory");
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) {
+      if (p.slices > 1) {
+        for (int s = 0; s < p.slices; ++s) mbar_arrive_cluster(map_to_cta(parts_in, s));
+      } else {
+        mbar_arrive(parts_in);
+      }
+    }
+    const bool got = __all_sync(0xffffffffu, mbar_wait_cluster(parts_in, 0, abort_flag));
+    if (!got) fail(ST_TIMEOUT_TMEM_FULL);
+    if (got && done) {
+      const int first = n0 + rank * share;
+      for (int i = threadIdx.x - 64; i < p.M * share; i += 32 * MR_WARPS) {
+        const int m = i / share, r = i - m * share;
+        float v = 0.f;
+        for (int s = 0; s < p.slices; ++s) v += part[(s * NT + m) * share + r];
+        if (first + r >= p.N) continue;
+        const long long at = ((long long)grp * p.M + m) * p.N + first + r;
+        if (p.out_fp32) reinterpret_cast<float*>(p.C)[at] = v;
+        else reinterpret_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16(v);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::COLS);
+  }
+}
+
+}  // namespace apb
+
+using namespace apb;
+
+// Slices of K for a product of ``tiles`` tiles of 128 rows of B: as many as are resident at once, each with a stage at least.
+static int mx_rows_slices(long long tiles, int num_kb, long long resident) {
+  int s = 1;
+  while (s < 4 && tiles * 2 * s <= resident && 4 * s <= num_kb) s *= 2;
+  return s;
+}
+
+// A: values [G, M, K] with unit stride along K (x_type 0: fp32, 1: bf16), or codes (x_type 2) with scales SA; B: codes [G, N, kp / 2], scales SB;
+// C [G, M, N] dense.  ``slices`` 0: chosen here.
+extern "C" int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K,
+                                 long long gs, long long ld, int x_type, int out_fp32, int slices, uint32_t* status, int num_sms, cudaStream_t stream) {
+  if (G < 0 || M < 0 || N < 0 || K < 0 || M > 32 || N >= 1ll << 31 || K >= 1ll << 30 || G >= 1ll << 31) return 3;
+  if (G == 0 || M == 0 || N == 0) return 0;
+  if ((reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(SB) | reinterpret_cast<uintptr_t>(C)) & 15) return 3;
+  if (x_type == 2 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(SA)) & 15)) return 3;
+  if (K == 0) return zero_result(C, G * M, N, N, out_fp32, stream);
+  const long long kp = (K + 31) / 32 * 32, n_tiles = (N + 127) / 128, tiles = G * n_tiles;
+  MxRowsParams p{};
+  p.x = x_type == 2 ? nullptr : A;
+  p.C = C;
+  p.M = (int)M, p.N = (int)N, p.K = (int)K, p.n_tiles = (int)n_tiles;
+  p.num_kb = (int)((kp + MX_BK - 1) / MX_BK);
+  p.k_steps = (int)((kp + 63) / 64);
+  p.slices = slices > 0 ? slices : mx_rows_slices(tiles, p.num_kb, 2ll * num_sms);
+  if ((p.slices & (p.slices - 1)) || p.slices > 8 || p.slices > p.num_kb || tiles * p.slices >= 1ll << 31) return 3;
+  p.out_fp32 = out_fp32;
+  p.gs = gs, p.ld = ld;
+  p.status = status;
+  const int esz = x_type == 1 ? 2 : 4;
+  p.vec = x_type != 2 && ld * esz % 16 == 0 && gs * esz % 16 == 0 && K % 8 == 0 && (reinterpret_cast<uintptr_t>(A) & 15) == 0;
+  const uint64_t words = (uint64_t)((kp + 127) / 128) * (MX_SCALE_TILE / 4);
+  const int nt = M <= 16 ? 16 : 32;
+  CUtensorMap tmB, tmSB, tmA{}, tmSA{};
+  int e = mx_map(&tmB, B, kp / 2, N, G, MX_ROW_BYTES, 128, false);
+  if (!e) e = mx_map(&tmSB, SB, words, n_tiles, G, MX_SC_BYTES / 4, 1, true);
+  if (!e && x_type == 2) e = mx_map(&tmA, A, kp / 2, M, G, MX_ROW_BYTES, nt, false);
+  if (!e && x_type == 2) e = mx_map(&tmSA, SA, words, 1, G, MX_SC_BYTES / 4, 1, true);
+  if (e) return e;
+  auto launch = [&](auto kern, int smem, int stages) {
+    p.stages = stages;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = p.slices, attr[n].val.clusterDim.y = 1, attr[n].val.clusterDim.z = 1;
+    ++n;
+    if (!apb_gemm_makes_room()) attr[n++] = overlap_attribute();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * p.slices));
+    cfg.blockDim = dim3(MR_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kern, tmB, tmSB, tmA, tmSA, p) == cudaSuccess ? 0 : 4;
+  };
+#define APB_MX_ROWS(NT, T) return launch(gemm_mx4_rows_kernel<NT, T>, MxRowsShape<NT>::SMEM, MxRowsShape<NT>::STAGES)
+  if (x_type == 2) {
+    if (nt == 16) APB_MX_ROWS(16, void);
+    APB_MX_ROWS(32, void);
+  }
+  if (x_type == 1) {
+    if (nt == 16) APB_MX_ROWS(16, __nv_bfloat16);
+    APB_MX_ROWS(32, __nv_bfloat16);
+  }
+  if (nt == 16) APB_MX_ROWS(16, float);
+  APB_MX_ROWS(32, float);
+#undef APB_MX_ROWS
+}

@@ -12,7 +12,7 @@
 
 #include <type_traits>
 
-#include "launch.cuh"
+#include "mx4.cuh"
 
 namespace apb {
 
@@ -27,46 +27,6 @@ struct MxParams {
   int R, K, row_tiles, k_tiles, vec;
   long long gs, ld;  // elements of x between matrices and between rows (or columns, where the rows have unit stride)
 };
-
-// 8 values to 4 bytes of codes: value 2i in the low half of byte i
-__device__ __forceinline__ uint32_t mx_encode(const float (&v)[8]) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
-      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
-      : "=r"(r)
-      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
-  return r;
-}
-// The code s e e m of a value v, moved to the top of an fp32 mantissa and the bottom of its exponent, is v * 2^-126, exactly (0.5 as a denormal).
-__device__ __forceinline__ void mx_decode(uint32_t codes, float scale, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t c = codes >> (4 * i);
-    v[i] = (__uint_as_float((c & 8u) << 28 | (c & 7u) << 22) * 0x1p126f) * scale;
-  }
-}
-
-// Largest magnitude of 32 values (as bits: a NaN is larger than everything) -> scale code, and the factor that takes the values to E2M1's range:
-// 2^(127 - code), 0 for a block that holds an infinity or a NaN (its codes are zeros).
-__device__ __forceinline__ uint32_t mx_scale_code(uint32_t amax_bits) {
-  const int field = (int)(amax_bits >> 23);
-  return field == 255 ? 255u : (uint32_t)max(field - 2, 0);
-}
-__device__ __forceinline__ float mx_factor(uint32_t code) { return __uint_as_float((254u - code) << 23); }  // (code <= 252)
-__device__ __forceinline__ float mx_scale(uint32_t code) {
-  return __uint_as_float(code == 255u ? 0x7FC00000u : code == 0u ? 0x00400000u : code << 23);
-}
-__device__ __forceinline__ uint32_t mx_encode_block(float (&v)[8], uint32_t code) {
-  if (code == 255u) return 0u;
-  const float f = mx_factor(code);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] *= f;
-  return mx_encode(v);
-}
 
 // 32 bytes, where both the address and the row lengths allow it in one access (``wide``), otherwise in two.
 __device__ __forceinline__ void load32(const void* p, bool wide, uint32_t (&u)[8]) {
@@ -95,27 +55,6 @@ __device__ __forceinline__ void store1(T* p, float v) {
   else *p = __float2bfloat16(v);
 }
 
-// A word of values: one fp32, or two bf16.  Largest magnitude as bits; value ``i`` of the 32 / sizeof(T) in 8 words; the other way.
-template <typename T>
-__device__ __forceinline__ uint32_t word_max(uint32_t m, uint32_t u) {
-  if constexpr (std::is_same<T, float>::value) return max(m, u & 0x7FFFFFFFu);
-  else return __vmaxu2(m, u & 0x7FFF7FFFu);
-}
-template <typename T>
-__device__ __forceinline__ uint32_t word_max_bits(uint32_t m) {
-  if constexpr (std::is_same<T, float>::value) return m;
-  else return max(m & 0xFFFF0000u, m << 16);
-}
-template <typename T, int N>
-__device__ __forceinline__ float word_value(const uint32_t (&u)[N], int i) {
-  if constexpr (std::is_same<T, float>::value) return __uint_as_float(u[i]);
-  else return __uint_as_float(i & 1 ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16);
-}
-__device__ __forceinline__ uint32_t two_bf16(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 struct MxTile {
   long long g;
   int r0, k0;
@@ -128,9 +67,6 @@ __device__ __forceinline__ MxTile mx_tile(const MxParams& p, uint8_t** scale_til
   if (p.scales != nullptr) *scale_tile = p.scales + t * 512;  // (tiles lie in the order of the grid)
   return {rest / p.row_tiles, rt * MX_TILE, kt * MX_TILE};
 }
-// byte of (row, block) in a scale tile
-__device__ __forceinline__ int scale_at(int row, int blk) { return (row & 31) * 16 + (row >> 5) * 4 + blk; }
-
 // Unit stride along K.  A thread has 32 bytes of a row (16 bf16 or 8 fp32), two or four threads a block; the loads of four rows are under way together.
 // ROUND: the values in place of codes and scales.
 template <typename T, bool ROUND>
@@ -147,7 +83,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
     uint32_t u[ROWS][8];
     if (pass > 0 && at.r0 + pass * PASS >= p.R) {  // (whole passes without rows: only their scales are written)
       if (!ROUND && threadIdx.x < 128) {
-        for (int i = threadIdx.x; i < (MX_TILE - pass * PASS) * 4; i += 128) tile[scale_at(pass * PASS + i / 4, i & 3)] = 127;
+        for (int i = threadIdx.x; i < (MX_TILE - pass * PASS) * 4; i += 128) tile[mx_scale_at(pass * PASS + i / 4, i & 3)] = 127;
       }
       break;
     }
@@ -168,10 +104,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
         } else {
 #pragma unroll
           for (int c = 0; c < PER; ++c)
-            if (k + c < p.K) {
-              if constexpr (std::is_same<T, float>::value) u[i][c] = __float_as_uint(src[c]);
-              else u[i][c / 2] |= (uint32_t)__bfloat16_as_ushort(src[c]) << (16 * (c & 1));
-            }
+            if (k + c < p.K) mx_put(u[i], c, src[c]);
         }
       }
     }
@@ -180,8 +113,8 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
       const int rr = r_first + PASS * (pass + i), r = at.r0 + rr;
       uint32_t m = 0;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) m = word_max<T>(m, u[i][c]);
-      uint32_t amax = word_max_bits<T>(m);
+      for (int c = 0; c < 8; ++c) m = mx_word_max<T>(m, u[i][c]);
+      uint32_t amax = mx_word_max_bits<T>(m);
 #pragma unroll
       for (int d = 1; d < 32 / PER; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
       const uint32_t code = mx_scale_code(amax);
@@ -191,12 +124,17 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
       for (int h = 0; h < PER / 8; ++h) {
         float v[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = word_value<T>(u[i], 8 * h + c);
+        for (int c = 0; c < 8; ++c) v[c] = mx_word_value<T>(u[i], 8 * h + c);
         packed[h] = mx_encode_block(v, code);
         if (ROUND) {
           mx_decode(packed[h], mx_scale(code), v);
+          if constexpr (PER == 8) {
 #pragma unroll
-          for (int c = 0; c < (PER == 8 ? 8 : 4); ++c) u[i][(PER == 8 ? 0 : 4 * h) + c] = PER == 8 ? __float_as_uint(v[c]) : two_bf16(v[2 * c & 7], v[(2 * c & 7) + 1]);
+            for (int c = 0; c < 8; ++c) u[i][c] = __float_as_uint(v[c]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) u[i][4 * h + c] = pack_bf16(v[2 * c], v[2 * c + 1]);
+          }
         }
       }
       if (ROUND) {
@@ -208,7 +146,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
         } else {
 #pragma unroll
           for (int c = 0; c < PER; ++c)
-            if (k + c < p.K) store1(dst + c, word_value<T>(u[i], c));
+            if (k + c < p.K) store1(dst + c, mx_word_value<T>(u[i], c));
         }
       } else {
         if (in) {
@@ -216,7 +154,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
           if constexpr (PER == 16) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
           else *reinterpret_cast<uint32_t*>(dst) = packed[0];
         }
-        if (col % 32 == 0) tile[scale_at(rr, col / 32)] = (uint8_t)(in ? code : 127u);
+        if (col % 32 == 0) tile[mx_scale_at(rr, col / 32)] = (uint8_t)(in ? code : 127u);
       }
     }
   }
@@ -272,7 +210,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_columns_kernel(MxParams p) {
 #pragma unroll
   for (int i = 0; i < 32; ++i)
 #pragma unroll
-    for (int w = 0; w < W; ++w) m[w] = word_max<T>(m[w], u[i][w]);
+    for (int w = 0; w < W; ++w) m[w] = mx_word_max<T>(m[w], u[i][w]);
   uint32_t code[2], packed[2][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -281,7 +219,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_columns_kernel(MxParams p) {
     for (int q = 0; q < 4; ++q) {
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = word_value<T>(u[8 * q + i], h);
+      for (int i = 0; i < 8; ++i) v[i] = mx_word_value<T>(u[8 * q + i], h);
       packed[h][q] = mx_encode_block(v, code[h]);
     }
   }
@@ -297,7 +235,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_columns_kernel(MxParams p) {
         for (int i = 0; i < 8; ++i) {
           T* dst = y + (long long)(k + 8 * q + i) * p.R;
           if constexpr (W == 2) *reinterpret_cast<float2*>(dst) = make_float2(a[i], b[i]);
-          else *reinterpret_cast<uint32_t*>(dst) = two_bf16(a[i], b[i]);
+          else *reinterpret_cast<uint32_t*>(dst) = pack_bf16(a[i], b[i]);
         }
       } else {
 #pragma unroll
@@ -312,7 +250,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_columns_kernel(MxParams p) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       *reinterpret_cast<uint4*>(rows + (rr + h) * STRIDE + blk * 16) = make_uint4(packed[h][0], packed[h][1], packed[h][2], packed[h][3]);
-      tile[scale_at(rr + h, blk)] = (uint8_t)(r + h < p.R && k < kp ? code[h] : 127u);
+      tile[mx_scale_at(rr + h, blk)] = (uint8_t)(r + h < p.R && k < kp ? code[h] : 127u);
     }
     __syncthreads();
 #pragma unroll
@@ -347,7 +285,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_dequantize_kernel(MxParams p) 
   for (int i = 0; i < 4; ++i) {
     const int rr = r_first + 32 * i, r = at.r0 + rr;
     if (r >= p.R || k >= p.K) continue;
-    const float scale = mx_scale(tile[scale_at(rr, col / 32)]);
+    const float scale = mx_scale(tile[mx_scale_at(rr, col / 32)]);
     float v[16];
     float (&lo)[8] = *reinterpret_cast<float (*)[8]>(v), (&hi)[8] = *reinterpret_cast<float (*)[8]>(v + 8);
     mx_decode(packed[i].x, scale, lo);
@@ -359,7 +297,10 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_dequantize_kernel(MxParams p) 
       for (int h = 0; h < 16 / PER; ++h) {
         uint32_t u[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) u[c] = PER == 8 ? __float_as_uint(v[(PER == 8 ? 8 * h : 0) + c]) : two_bf16(v[2 * c], v[2 * c + 1]);
+        for (int c = 0; c < 8; ++c) {
+          if constexpr (PER == 8) u[c] = __float_as_uint(v[8 * h + c]);
+          else u[c] = pack_bf16(v[2 * c], v[2 * c + 1]);
+        }
         store32(dst + PER * h, p.vec > 1, u);
       }
     } else {
