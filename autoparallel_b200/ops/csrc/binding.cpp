@@ -76,7 +76,6 @@ int apb_mx4_round(const void* x, void* y, long long G, long long R, long long K,
 int apb_mx4_dequantize(const void* codes, const void* scales, void* y, long long G, long long R, long long K, int is_bf16, cudaStream_t st);
 int apb_gemm_mx4(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long kp,
                  int out_fp32, int form, uint32_t* status, int num_sms, cudaStream_t stream);
-void apb_mx4_staged(int);
 int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K,
                       long long gs, long long ld, int x_type, int out_fp32, int slices, uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_symm_header_bytes();
@@ -1161,7 +1160,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return mx4_dequantize(codes, scales, k, fp32 ? at::kFloat : at::kBFloat16);
   });
   m.def("mx4_round", &mx4_round);
-  m.def("mx_staged", [](int64_t n) { apb_mx4_staged((int)n); });
   m.def("mx_rows", [](int64_t n) { mx_rows_fused = (int)n; });
   m.def("mx_rows_s", [](const Tensor& x, const Tensor& c, const Tensor& s, int64_t n) { return mx4_linear_rows(x, c, s, at::kBFloat16, (int)n); });
   m.def("mx4_mm", [](const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, bool fp32, int64_t form) {  // form -1: chosen

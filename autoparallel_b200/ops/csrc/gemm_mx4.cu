@@ -7,15 +7,15 @@
 // to TMEM (tcgen05.cp) in front of the stage's MMAs.
 //   warp 0: TMA producer | warp 1: TMEM owner, scale copies, MMAs | warps 2..9: epilogue, two per TMEM lane quarter, each half of the tile's columns
 //
-// TMEM: two accumulators of up to 256 columns and 64 columns of scales do not fit 512, so the accumulators overlap by 64 columns: 0 ... 255 and
-// 192 ... 447, scales from 448 on.  The epilogue reads the shared columns first, and the next tile's MMAs start as soon as that is done.
+// TMEM: two accumulators of up to 256 columns and 24 columns of scales do not fit 512, so the accumulators overlap by 32 columns: 0 ... 255 and
+// 224 ... 479, scales from 480 on.  The epilogue reads the shared columns first, and the next tile's MMAs start as soon as that is done.
 #include <algorithm>
 
 #include "mx4.cuh"
 
 namespace apb {
 
-constexpr int MX_ACC1 = 192, MX_SCALE_COL = 448;  // first columns of the second accumulator and of the scales
+constexpr int MX_ACC1 = 224, MX_SCALE_COL = 480;  // first columns of the second accumulator and of the scales
 constexpr int MX_EPI_WARPS = 8, MX_GEMM_THREADS = 64 + 32 * MX_EPI_WARPS;
 constexpr int MX_STAGING = MX_EPI_WARPS * 4096;
 constexpr int MX_BAR_BYTES = 256;
@@ -42,15 +42,59 @@ __device__ __forceinline__ void st_32(void* p, const uint32_t* v) {
                : "memory");
 }
 
-// Epilogue of a warp's 32 rows and ``ncols`` columns, 64 at a time, from column ``c_first`` up or down; ``release`` after the first 64.
+// 32 columns of a row straight to C, in whole sectors; ``ncols`` of them lie in the matrix (whole sectors, too).
+__device__ __forceinline__ void mx_store_row(uint8_t* dst, const uint32_t (&r)[32], int ncols, bool fp32) {
+  if (fp32) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8)
+      if (j < ncols) st_32(dst + 4 * j, r + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j += 16) {
+      uint32_t v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = pack_bf16(__uint_as_float(r[j + 2 * e]), __uint_as_float(r[j + 2 * e + 1]));
+      if (j < ncols) st_32(dst + 2 * j, v);
+    }
+  }
+}
+
+// Epilogue of a warp's 32 rows and ``ncols`` columns (a multiple of 64), 32 at a time: from the first up, or ``down`` from the last; ``release`` as soon
+// as the first 32 that way are in registers.  A load from TMEM takes some 400 cycles under load, so the next 32 columns are on their way while the
+// last are stored.
 template <typename Release>
-__device__ __forceinline__ void mx_store(const MxGemmParams& q, uint8_t* C, uint8_t* stg, uint32_t taddr, int row0, int n0, int ncols, bool down,
-                                         int lane, Release release) {
+__device__ __forceinline__ void mx_store_direct(const MxGemmParams& q, uint8_t* C, uint32_t taddr, int row0, int n0, int ncols, bool down, int lane,
+                                                Release release) {
   const GemmParams& p = q.p;
   const int esz = p.out_fp32 ? 4 : 2;
-  const int chunks = row0 < p.M ? (min(ncols, p.N - n0) + 63) / 64 : 0;  // (those past the matrix are not read)
-  if (chunks <= 0 || (down && chunks * 64 < ncols)) release();           // the shared columns are none of this warp's, or past the matrix
+  const int chunks = ncols / 32, in = row0 + lane < p.M ? p.N - n0 : 0;  // columns of this row that lie in the matrix
+  uint8_t* dst = C + ((row0 + lane) * p.ldc + n0) * esz;
+  auto column = [&](int i) { return (down ? chunks - 1 - i : i) * 32; };
+  uint32_t a[32], b[32];
+  tmem_ld_32x32(taddr + column(0), a);
+  tmem_ld_wait_for(a);
+  release();
+#pragma unroll 1
+  for (int i = 0; i < chunks; i += 2) {
+    tmem_ld_32x32(taddr + column(i + 1), b);
+    mx_store_row(dst + column(i) * esz, a, in - column(i), p.out_fp32);
+    tmem_ld_wait_for(b);
+    const bool more = i + 2 < chunks;
+    if (more) tmem_ld_32x32(taddr + column(i + 2), a);
+    mx_store_row(dst + column(i + 1) * esz, b, in - column(i + 1), p.out_fp32);
+    if (more) tmem_ld_wait_for(a);
+  }
+}
+
+// The same where rows are no whole sectors, 64 columns at a time: through shared memory in 16-byte pieces of whole 128-byte lines, or element by element.
+template <typename Release>
+__device__ __forceinline__ void mx_store_staged(const MxGemmParams& q, uint8_t* C, uint8_t* stg, uint32_t taddr, int row0, int n0, int ncols, bool down,
+                                                int lane, Release release) {
+  const GemmParams& p = q.p;
+  const int esz = p.out_fp32 ? 4 : 2;
+  const int chunks = row0 < p.M ? (min(ncols, p.N - n0) + 63) / 64 : 0;
   const bool early = chunks > 0 && !(down && chunks * 64 < ncols);
+  if (!early) release();
 #pragma unroll 1
   for (int i = 0; i < chunks; ++i) {
     const int c = (down ? chunks - 1 - i : i) * 64;
@@ -60,27 +104,6 @@ __device__ __forceinline__ void mx_store(const MxGemmParams& q, uint8_t* C, uint
     tmem_ld_wait_for(r[0]);
     tmem_ld_wait_for(r[1]);
     if (early && i == 0) release();
-    if (q.store == MX_DIRECT) {
-      uint8_t* dst = C + ((row0 + lane) * p.ldc + n0 + c) * esz;
-      if (row0 + lane < p.M) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < 32; j += 16) {
-            const int col = n0 + c + 32 * h + j;
-            if (p.out_fp32) {
-              if (col < p.N) st_32(dst + (32 * h + j) * 4, r[h] + j);
-              if (col + 8 < p.N) st_32(dst + (32 * h + j + 8) * 4, r[h] + j + 8);
-            } else if (col < p.N) {
-              uint32_t v[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = pack_bf16(__uint_as_float(r[h][j + 2 * e]), __uint_as_float(r[h][j + 2 * e + 1]));
-              st_32(dst + (32 * h + j) * 2, v);
-            }
-          }
-      }
-      continue;
-    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // fp32: 32 columns at a time; bf16: all 64 in the first
       if (h == 1 && !p.out_fp32) break;
@@ -185,6 +208,8 @@ __device__ __forceinline__ void mx_gemm_cta(const CUtensorMap& tmA, const CUtens
     atomicCAS(p.status, 0u, code);
     *abort_flag = 1;
   };
+  // columns of a tile's MMAs: a wide one with 128 columns or fewer takes half of them
+  auto width = [&](int col) { return q.col_tile > 128 && p.N - col <= 128 ? 128 : q.col_tile; };
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (elect_one()) {
@@ -196,7 +221,7 @@ __device__ __forceinline__ void mx_gemm_cta(const CUtensorMap& tmA, const CUtens
         int grp, tm, tn;
         plain_tile(p, q.num_m, q.grouped, t, grp, tm, tn);
         const int m0 = tm * TM + (int)half * 128, col = tn * q.col_tile;
-        const int n0 = col + (PAIR ? (int)half * 128 : 0);  // rows of B that this CTA stages
+        const int n0 = col + (PAIR ? (int)half * width(col) / 2 : 0);  // rows of B that this CTA stages
         for (int kb = 0; kb < q.num_kb; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
             ok = false;
@@ -224,7 +249,6 @@ __device__ __forceinline__ void mx_gemm_cta(const CUtensorMap& tmA, const CUtens
   } else if (warp == 1) {
     // ------------------------------------------------------------------ scale copies and MMAs
     if (half == 0 && elect_one()) {
-      const uint32_t idesc[2] = {make_idesc_mx4(TM, q.col_tile, 0), make_idesc_mx4(TM, q.col_tile, 2)};
       const uint64_t a_desc = make_smem_desc(smem_u32(ops + A_AT), 16, 1024), b_desc = make_smem_desc(smem_u32(ops + B_AT), 16, 1024);
       const uint64_t sa_desc = make_scale_desc(smem_u32(scs)), sb_desc = make_scale_desc(smem_u32(scs + MX_SC_BYTES));
       const uint32_t empty_even = PAIR ? map_to_cta(empty, 0) : 0u, empty_odd = PAIR ? map_to_cta(empty, 1) : 0u;
@@ -239,6 +263,9 @@ __device__ __forceinline__ void mx_gemm_cta(const CUtensorMap& tmA, const CUtens
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem + (seq & 1u) * MX_ACC1;
+        int grp, tm, tn;
+        plain_tile(p, q.num_m, q.grouped, t, grp, tm, tn);
+        const uint32_t idesc[2] = {make_idesc_mx4(TM, width(tn * q.col_tile), 0), make_idesc_mx4(TM, width(tn * q.col_tile), 2)};
         for (int kb = 0; kb < q.num_kb; ++kb) {
           if (!mbar_wait(&full[stage], phase, abort_flag)) {
             ok = false;
@@ -289,7 +316,7 @@ __device__ __forceinline__ void mx_gemm_cta(const CUtensorMap& tmA, const CUtens
     }
   } else {
     // ------------------------------------------------------------------ epilogue
-    const int quarter = warp & 3, part = (warp - 2) >> 2, cols = q.col_tile / 2;
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
     const uint32_t go_even = PAIR ? map_to_cta(go, 0) : 0u;
     const int esz = p.out_fp32 ? 4 : 2;
     uint32_t seq = 0;
@@ -297,6 +324,7 @@ __device__ __forceinline__ void mx_gemm_cta(const CUtensorMap& tmA, const CUtens
       int grp, tm, tn;
       plain_tile(p, q.num_m, q.grouped, t, grp, tm, tn);
       const uint32_t buf = seq & 1u;
+      const int cols = width(tn * q.col_tile) / 2;
       auto release = [&]() {
         tc_fence_before();
         __syncwarp();
@@ -313,11 +341,14 @@ __device__ __forceinline__ void mx_gemm_cta(const CUtensorMap& tmA, const CUtens
       // the shared columns: the last of the first accumulator (the second half's), the first of the second (the first half's)
       const bool mine = buf == 0 ? part == 1 : part == 0;
       if (!mine) release();
-      mx_store(q, reinterpret_cast<uint8_t*>(p.C) + (long long)grp * p.M * p.ldc * esz, staging + (warp - 2) * 4096,
-               tmem + (uint32_t(quarter * 32) << 16) + buf * MX_ACC1 + part * cols, tm * TM + (int)half * 128 + quarter * 32,
-               tn * q.col_tile + part * cols, cols, buf == 0, lane, [&]() {
-                 if (mine) release();
-               });
+      uint8_t* C = reinterpret_cast<uint8_t*>(p.C) + (long long)grp * p.M * p.ldc * esz;
+      const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16) + buf * MX_ACC1 + part * cols;
+      const int row0 = tm * TM + (int)half * 128 + quarter * 32, col0 = tn * q.col_tile + part * cols;
+      auto read = [&]() {
+        if (mine) release();
+      };
+      if (q.store == MX_DIRECT) mx_store_direct(q, C, taddr, row0, col0, cols, buf == 0, lane, read);
+      else mx_store_staged(q, C, staging + (warp - 2) * 4096, taddr, row0, col0, cols, buf == 0, lane, read);
     }
   }
 
@@ -352,8 +383,6 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 
 using namespace apb;
 
-static int g_force_staged = 0;
-extern "C" void apb_mx4_staged(int on) { g_force_staged = on; }
 extern "C" int apb_gemm_resident_pairs(int num_sms);
 extern "C" int apb_gemm_get_reserved_sms();
 
@@ -367,7 +396,10 @@ extern "C" int apb_gemm_mx4(const void* A, const void* SA, const void* B, const 
   for (const void* ptr : {A, SA, B, SB, (const void*)C})
     if (reinterpret_cast<uintptr_t>(ptr) & 15) return 3;
   if (kp == 0) return zero_result(C, G * M, N, N, out_fp32, stream);
-  if (form < 0) form = M > 128 && N > 128 ? 2 : N > 128 ? 1 : 0;
+  // Small tiles where they all run at once: 999 x 1408 x 2048 5.8 us (single 128 x 256 7.4, pairs 7.5), 128 x 4096 x 4096 7.1 (9.7, 9.7); otherwise pairs
+  // (8192 x 8192 x 8192 178 us, single 128 x 256 237, 128 x 128 257; 2048 x 4096 x 4096 17.4, 18.9, 22.0), or 128 x 256 where a pair's second half
+  // would have no rows.
+  if (form < 0) form = G * ((M + 127) / 128) * ((N + 127) / 128) <= num_sms ? 0 : M > 128 ? 2 : 1;
   const bool pair = form == 2;
   MxGemmParams q{};
   GemmParams& p = q.p;
@@ -379,7 +411,7 @@ extern "C" int apb_gemm_mx4(const void* A, const void* SA, const void* B, const 
   p.status = status;
   q.col_tile = form == 0 ? 128 : 256;
   const long long row_bytes = N * (out_fp32 ? 4 : 2);
-  q.store = row_bytes % 32 == 0 && (reinterpret_cast<uintptr_t>(C) & 31) == 0 && !g_force_staged ? MX_DIRECT : row_bytes % 16 == 0 ? MX_STAGED : MX_SCALAR;
+  q.store = row_bytes % 32 == 0 && (reinterpret_cast<uintptr_t>(C) & 31) == 0 ? MX_DIRECT : row_bytes % 16 == 0 ? MX_STAGED : MX_SCALAR;
   q.grouped = G > 1;
   q.num_m = (int)((M + (pair ? 255 : 127)) / (pair ? 256 : 128));
   p.num_n_tiles = (int)((N + q.col_tile - 1) / q.col_tile);
