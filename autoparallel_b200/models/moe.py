@@ -68,6 +68,15 @@ class MoEConfig:
     #: YaRN context extension of the rotary tables, e.g. {"factor": 4.0, "original_max_seq_len": 1024}
     rope_yarn: Optional[dict] = None
     expert_mode: str = "local_map"
+    #: None: softmax of the biased router logits, ``topk`` and a division; "softmax" / "sigmoid": one operator (``ops.moe_route``), in which
+    #: the router's bias enters the choice of experts alone
+    router_score: Optional[str] = None
+    router_groups: int = 1      # the experts in groups, of which a token's experts come from the ``router_top_groups`` best
+    router_top_groups: int = 1
+    router_renormalize: bool = True
+    router_scale: float = 1.0
+    #: "bf16", or "mx4": the routed experts' products in microscaled 4-bit floating point (``ops.mx4_matmul``), gradients straight through the rounding
+    expert_format: str = "bf16"
     dispatch_blocks: int = 8  # planner mode: token blocks with their own per-expert capacity (a multiple of the shard count)
 
     def rope_dim(self) -> int:
@@ -91,7 +100,14 @@ def moe_debug(**kw) -> MoEConfig:
     return MoEConfig(**base)
 
 
-def _expert_region(x, gate_w, gate_idx, w1, w3, w2, *, ep_axis: str, num_experts: int, capacity: int):
+def _expert_ffn(h, w1, w3, w2, expert_format: str):
+    """SwiGLU of every expert: h [E, rows, d], w1, w3 [E, d, hidden], w2 [E, hidden, d]; one grouped launch for each product."""
+    if expert_format == "mx4":
+        return K.mx4_matmul(K.swiglu(K.mx4_matmul(h, w1, trans_b=False), K.mx4_matmul(h, w3, trans_b=False)), w2, trans_b=False)
+    return K.grouped_mm(K.swiglu(K.grouped_mm(h, w1), K.grouped_mm(h, w3)), w2)
+
+
+def _expert_region(x, gate_w, gate_idx, w1, w3, w2, *, ep_axis: str, num_experts: int, capacity: int, expert_format: str = "bf16"):
     """Runs on local shards.  x [T, d] tokens of this rank; gate_w / gate_idx [T, k]; w1, w3
     [E_loc, d, h], w2 [E_loc, h, d] local experts.  Returns [T, d]."""
     T, d = x.shape
@@ -104,7 +120,7 @@ def _expert_region(x, gate_w, gate_idx, w1, w3, w2, *, ep_axis: str, num_experts
     send = K.moe_dispatch(x, slot, num_experts, capacity, 1)        # [E, 1, C, d]
     recv = all_to_all(send.reshape(n * e_loc * capacity, d), ep_axis, 0, 0).view(n, e_loc, capacity, d)
     h = recv.permute(1, 0, 2, 3).reshape(e_loc, n * capacity, d)    # expert-major
-    y = K.grouped_mm(K.swiglu(K.grouped_mm(h, w1), K.grouped_mm(h, w3)), w2)   # [E_loc, n*C, d]: one grouped GEMM launch each
+    y = _expert_ffn(h, w1, w3, w2, expert_format)                   # [E_loc, n*C, d]
     back = y.view(e_loc, n, capacity, d).permute(1, 0, 2, 3).reshape(n * e_loc * capacity, d)
     got = all_to_all(back, ep_axis, 0, 0)                           # [E*C, d] in this rank's slot order
     return K.moe_combine(got.view(num_experts, 1, capacity, d), slot, gate_w)
@@ -166,6 +182,8 @@ class MLAttention(nn.Module):
 class MoEFFN(nn.Module):
     def __init__(self, cfg: MoEConfig):
         super().__init__()
+        if cfg.expert_format not in ("bf16", "mx4"):
+            raise ValueError(f"expert_format is 'bf16' or 'mx4', not {cfg.expert_format!r}")
         self.cfg = cfg
         E, d, h = cfg.num_experts, cfg.dim, cfg.expert_hidden
         self.router = nn.Linear(d, E, bias=False)
@@ -177,12 +195,20 @@ class MoEFFN(nn.Module):
         self.shared_w3 = nn.Linear(d, cfg.shared_hidden, bias=False)
         self.shared_w2 = nn.Linear(cfg.shared_hidden, d, bias=False)
 
+    def route(self, x):
+        """Gate weights and experts [.., top_k] of the tokens ``x`` [.., d]."""
+        cfg = self.cfg
+        if cfg.router_score is not None:
+            return K.moe_route(self.router(x), cfg.top_k, score=cfg.router_score, bias=self.router_bias.float(), num_groups=cfg.router_groups,
+                               top_groups=cfg.router_top_groups, renormalize=cfg.router_renormalize, scale=cfg.router_scale)
+        scores = torch.softmax((self.router(x).float() + self.router_bias), dim=-1)
+        gate_w, gate_idx = torch.topk(scores, cfg.top_k, dim=-1)
+        return gate_w / gate_w.sum(-1, keepdim=True), gate_idx
+
     def forward(self, x):
         cfg = self.cfg
         b, s, d = x.shape
-        scores = torch.softmax((self.router(x).float() + self.router_bias), dim=-1)
-        gate_w, gate_idx = torch.topk(scores, cfg.top_k, dim=-1)
-        gate_w = gate_w / gate_w.sum(-1, keepdim=True)
+        gate_w, gate_idx = self.route(x)
         shared = self.shared_w2(K.swiglu(self.shared_w1(x), self.shared_w3(x)))
         if cfg.expert_mode == "planner":
             return shared + self._routed_planner(x.reshape(b * s, d), gate_w.to(x.dtype).reshape(b * s, -1),
@@ -193,7 +219,8 @@ class MoEFFN(nn.Module):
         # Argument order = order of first use inside the region: the graph capture lists the region's
         # inputs in that order and insists that the declared placements line up with it.
         def region(gi, xf, w1, w3, w2, gw):
-            return _expert_region(xf, gw, gi, w1, w3, w2, ep_axis=cfg.ep_axis, num_experts=cfg.num_experts, capacity=capacity)
+            return _expert_region(xf, gw, gi, w1, w3, w2, ep_axis=cfg.ep_axis, num_experts=cfg.num_experts, capacity=capacity,
+                                  expert_format=cfg.expert_format)
 
         tok_pl = (Shard(0),)
         routed = local_map(region, out_placements=(tok_pl,), in_placements=(tok_pl,) * 6)(
@@ -212,8 +239,7 @@ class MoEFFN(nn.Module):
         """How many of the ``tokens x top_k`` assignments of ``x`` [b, s, d] the configured capacity drops when the
         tokens are split into ``blocks`` equal blocks (ranks of the expert-parallel axis, or dispatch blocks)."""
         cfg = self.cfg
-        scores = torch.softmax(self.router(x).float() + self.router_bias, dim=-1)
-        idx = torch.topk(scores, cfg.top_k, dim=-1).indices.reshape(blocks, -1)          # [blocks, tokens/block * k]
+        idx = self.route(x)[1].reshape(blocks, -1)                                        # [blocks, tokens/block * k]
         cap = self.capacity(idx.shape[1] // cfg.top_k)
         counts = torch.zeros(blocks, cfg.num_experts, dtype=torch.long, device=x.device).scatter_add_(1, idx, torch.ones_like(idx))
         return int((counts - cap).clamp_min(0).sum().item())
@@ -226,7 +252,7 @@ class MoEFFN(nn.Module):
         capacity = self.capacity(T // nb)
         slot = K.moe_slots(gate_idx, E, capacity, nb)
         h = K.moe_dispatch(xf, slot, E, capacity, nb).view(E, nb * capacity, d)
-        y = K.grouped_mm(K.swiglu(K.grouped_mm(h, self.w1), K.grouped_mm(h, self.w3)), self.w2)
+        y = _expert_ffn(h, self.w1, self.w3, self.w2, cfg.expert_format)
         return K.moe_combine(y.view(E, nb, capacity, d), slot, gate_w)
 
     def init_weights(self, std: float):

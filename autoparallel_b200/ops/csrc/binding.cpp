@@ -76,6 +76,7 @@ int apb_mx4_round(const void* x, void* y, long long G, long long R, long long K,
 int apb_mx4_dequantize(const void* codes, const void* scales, void* y, long long G, long long R, long long K, int is_bf16, cudaStream_t st);
 int apb_gemm_mx4(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long kp,
                  int out_fp32, int form, uint32_t* status, int num_sms, cudaStream_t stream);
+int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, int values, int num_sms);
 int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K,
                       long long gs, long long ld, int x_type, int out_fp32, int slices, uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_symm_header_bytes();
@@ -951,14 +952,6 @@ Tensor mx4_mm_form(const Tensor& a_, const Tensor& sa, const Tensor& b_, const T
   auto shape = a.sizes().vec();
   shape.back() = b.size(-2);
   Tensor c = at::empty(shape, a.options().dtype(dtype));
-  if (form >= 3) {
-    check(apb_gemm_mx4_rows(a.data_ptr(), as.data_ptr(), b.data_ptr(), bs.data_ptr(), c.data_ptr(), a.dim() == 3 ? a.size(0) : 1, a.size(-2), b.size(-2),
-                            2 * a.size(-1), 0, 0, 2, dtype == at::kFloat, (int)form - 3, reinterpret_cast<uint32_t*>(status_of(a).data_ptr()), num_sms(),
-                            stream()),
-          "apb_gemm_mx4_rows");
-    count(c.numel() > 0 && a.size(-1) > 0);
-    return c;
-  }
   check(apb_gemm_mx4(a.data_ptr(), as.data_ptr(), b.data_ptr(), bs.data_ptr(), c.data_ptr(), a.dim() == 3 ? a.size(0) : 1, a.size(-2), b.size(-2),
                      2 * a.size(-1), dtype == at::kFloat, (int)form, reinterpret_cast<uint32_t*>(status_of(a).data_ptr()), num_sms(), stream()),
         "apb_gemm_mx4");
@@ -966,51 +959,35 @@ Tensor mx4_mm_form(const Tensor& a_, const Tensor& sa, const Tensor& b_, const T
   return c;
 }
 Tensor mx4_mm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, at::ScalarType dtype) { return mx4_mm_form(a, sa, b, sb, dtype, -1); }
-int mx_rows_fused = 8;
-// Few rows: a few are rounded in the product's own launch, others by a launch before it into a workspace.
-Tensor mx4_linear_rows(const Tensor& x_, const Tensor& codes_, const Tensor& scales_, at::ScalarType dtype, int slices = 0) {
+Tensor mx4_linear(const Tensor& x_, const Tensor& codes_, const Tensor& scales_, at::ScalarType dtype) {
   c10::cuda::CUDAGuard g(x_.device());
   mx_codes_check(codes_, scales_, "mx4_linear");
+  TORCH_CHECK(x_.dim() >= 1 && mx_blocks(x_.size(-1)) * 16 == codes_.size(-1) &&
+                  (codes_.dim() == 2 || (x_.dim() == 3 && x_.size(0) == codes_.size(0))),
+              "mx4_linear: x ", x_.sizes(), " and codes ", codes_.sizes(), " do not multiply");
   TORCH_CHECK(codes_.is_cuda() && codes_.device() == x_.device() && float_or_bf16(dtype), "mx4_linear: weights on x's device, a result in bf16 or fp32");
-  Tensor x = x_.stride(-1) == 1 || x_.size(-1) <= 1 ? x_ : x_.contiguous(), codes = dense(codes_), scales = dense(scales_);
-  auto shape = x.sizes().vec();
-  shape.back() = codes.size(-2);
-  Tensor c = at::empty(shape, x.options().dtype(dtype));
-  const int64_t G = x.dim() == 3 ? x.size(0) : 1, M = x.size(-2), K = x.size(-1), gs = x.dim() == 3 ? x.stride(0) : 0, ld = x.stride(-2);
-  const bool empty = c.numel() == 0 || K == 0;
+  const int64_t K = x_.size(-1), N = codes_.size(-2);
+  const MxView v(codes_.dim() == 3 || x_.dim() == 2 ? x_ : x_.reshape({x_.numel() / std::max<int64_t>(K, 1), K}), "mx4_linear");
+  auto shape = x_.sizes().vec();
+  shape.back() = N;
+  Tensor c = at::empty(shape, x_.options().dtype(dtype)), codes = dense(codes_), scales = dense(scales_), rounded;
+  const bool empty = c.numel() == 0 || K == 0, bf16 = is_bf16(v.x), fp32 = dtype == at::kFloat;
   const cudaStream_t st = stream();
-  const void* a = x.data_ptr();
-  void* sa = nullptr;
-  Tensor ws;
-  if (M > mx_rows_fused && !empty) {
-    const int64_t code_bytes = G * M * mx_blocks(K) * 16, scale_bytes = G * ((K + 127) / 128) * 512;
-    ws = at::empty({code_bytes + scale_bytes}, codes.options());
-    a = ws.data_ptr();
-    sa = static_cast<uint8_t*>(ws.data_ptr()) + code_bytes;
-    check(apb_mx4_quantize(x.data_ptr(), ws.data_ptr(), sa, G, M, K, gs, ld, false, is_bf16(x), st), "apb_mx4_quantize");
+  uint32_t* status = reinterpret_cast<uint32_t*>(status_of(x_).data_ptr());
+  if (!v.transposed && apb_gemm_mx4_rows_takes(v.G, v.R, N, 1, num_sms())) {  // a few rows are rounded in the product's launch
+    check(apb_gemm_mx4_rows(v.x.data_ptr(), nullptr, codes.data_ptr(), scales.data_ptr(), c.data_ptr(), v.G, v.R, N, K, v.gs, v.ld, bf16, fp32, 0, status,
+                            num_sms(), st),
+          "apb_gemm_mx4_rows");
+    count(!empty);
+    return c;
   }
-  check(apb_gemm_mx4_rows(a, sa, codes.data_ptr(), scales.data_ptr(), c.data_ptr(), G, M, codes.size(-2), K, gs, ld, sa != nullptr ? 2 : is_bf16(x),
-                          dtype == at::kFloat, slices, reinterpret_cast<uint32_t*>(status_of(x).data_ptr()), num_sms(), st),
-        "apb_gemm_mx4_rows");
-  count(empty ? 0 : sa != nullptr ? 2 : 1);
+  const int64_t code_bytes = v.G * v.R * mx_blocks(K) * 16, scale_bytes = v.G * ((v.R + 127) / 128) * ((K + 127) / 128) * 512;
+  rounded = at::empty({code_bytes + scale_bytes}, codes.options());
+  uint8_t *a = static_cast<uint8_t*>(rounded.data_ptr()), *sa = a + code_bytes;
+  check(apb_mx4_quantize(v.x.data_ptr(), a, sa, v.G, v.R, K, v.gs, v.ld, v.transposed, bf16, st), "apb_mx4_quantize");
+  check(apb_gemm_mx4(a, sa, codes.data_ptr(), scales.data_ptr(), c.data_ptr(), v.G, v.R, N, mx_blocks(K) * 32, fp32, -1, status, num_sms(), st), "apb_gemm_mx4");
+  count(empty ? 0 : 2);
   return c;
-}
-Tensor mx4_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, at::ScalarType dtype) {
-  TORCH_CHECK(x.dim() >= 1 && codes.dim() >= 2 && mx_blocks(x.size(-1)) * 16 == codes.size(-1) &&
-                  (codes.dim() == 2 || (x.dim() == 3 && x.size(0) == codes.size(0))),
-              "mx4_linear: x ", x.sizes(), " and codes ", codes.sizes(), " do not multiply");
-  const Tensor m = codes.dim() == 3 || x.dim() == 2 ? x : x.reshape({x.numel() / std::max<int64_t>(x.size(-1), 1), x.size(-1)});
-  Tensor c;
-  if (m.size(-2) <= 32 && mx_rows_fused >= 0) {
-    c = mx4_linear_rows(m, codes, scales, dtype);
-  } else {
-    auto [a, sa] = mx4_quantize(m);
-    c = mx4_mm(a, sa, codes, scales, dtype);
-  }
-  if (codes.dim() == 3 || x.dim() == 2) return c;
-  auto shape = x.sizes().vec();
-  shape.back() = codes.size(-2);
-  return c.view(shape);
 }
 Tensor mx4_matmul(const Tensor& x, const Tensor& w, bool trans_b, at::ScalarType dtype) {
   TORCH_CHECK(w.dim() == 2 || w.dim() == 3, "mx4_matmul: w is a matrix or a stack of them");
@@ -1103,6 +1080,9 @@ void register_native(py::dict table, py::object status_buffer, bool diag_library
 
 }  // namespace
 
+// For autograd.cpp: whether the operator runs this extension's function.
+bool apb_mx4_matmul_ours() { return native().table.ptr() != nullptr && ours(MX4_MATMUL); }
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kernel_footprints", &kernel_footprints);
   m.def("register_native", &register_native);
@@ -1160,8 +1140,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return mx4_dequantize(codes, scales, k, fp32 ? at::kFloat : at::kBFloat16);
   });
   m.def("mx4_round", &mx4_round);
-  m.def("mx_rows", [](int64_t n) { mx_rows_fused = (int)n; });
-  m.def("mx_rows_s", [](const Tensor& x, const Tensor& c, const Tensor& s, int64_t n) { return mx4_linear_rows(x, c, s, at::kBFloat16, (int)n); });
   m.def("mx4_mm", [](const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, bool fp32, int64_t form) {  // form -1: chosen
     return mx4_mm_form(a, sa, b, sb, fp32 ? at::kFloat : at::kBFloat16, form);
   });

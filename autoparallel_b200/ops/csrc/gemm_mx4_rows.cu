@@ -295,6 +295,19 @@ static int mx_rows_slices(long long tiles, int num_kb, long long resident) {
   return s;
 }
 
+// Whether a product with M rows of A is this file's.  us, this kernel / the persistent ones of gemm_mx4.cu (behind a launch that rounds A, where A comes
+// as ``values``):
+//   values, rounded here   1 x 14336 x 4096 8.0 / 12.6, 4 rows 9.0 / 11.9, 8 10.6 / 12.2, 16 14.4 / 12.3; 1 x 4096 x 14336 9.4 / 24.4; 64 experts of 1408 x
+//                          2048 (704 tiles): 1 row 20.4 / 25.9, 4 rows 23.6 / 24.4, 16 41 / 26.  Every CTA rounds all of A's slice, so more rows are
+//                          better rounded once, by a launch before.
+//   codes                  16 x 14336 x 4096 8.6 / 10.1, 32 9.9 / 10.1, 17 x 4096 x 14336 9.4 / 15.3, 32 x 4096 x 4096 7.1 / 9.6; 704 tiles 16 rows 32 / 24:
+//                          a second wave of CTAs pays its start again.
+extern "C" int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, int values, int num_sms) {
+  const long long tiles = G * ((N + 127) / 128);
+  if (values) return M <= 4 || (M <= 8 && tiles <= 2 * num_sms);
+  return M <= 32 && tiles <= num_sms;
+}
+
 // A: values [G, M, K] with unit stride along K (x_type 0: fp32, 1: bf16), or codes (x_type 2) with scales SA; B: codes [G, N, kp / 2], scales SB;
 // C [G, M, N] dense.  ``slices`` 0: chosen here.
 extern "C" int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K,

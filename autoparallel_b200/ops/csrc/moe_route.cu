@@ -410,11 +410,11 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_bwd_kernel(RouteBw
     const float s = chosen ? route_sigmoid(xe) : 0.f;
     float ds = g;
     if (p.renorm) {
-      const float total = lanes_sum<L>(s);
-      const float dot = lanes_sum<L>(chosen ? g * s / total : 0.f);
+      const float total = lanes_sum<L>(s), q = total == 0.f ? 0.f : s / total;  // (1 for a single choice: no gradient, not a rounding error's)
+      const float dot = lanes_sum<L>(g * q);  // (by every lane: tokens whose scores are all zero share warps with others)
       ds = total == 0.f ? 0.f : (g - dot) / total;
     }
-    mine = ds * s * (1.f - s);
+    mine = ds * s * (chosen ? route_sigmoid(-xe) : 0.f);  // (1 - s, also where s rounds to 1)
   } else if (p.renorm) {
     float m = lanes_max<L>(xe);
     if (m == -CUDART_INF_F) m = 0.f;

@@ -167,11 +167,12 @@ def _moe_route_bwd(dweights, logits, idx, sigmoid, renormalize, scale):
     k = idx.shape[-1]
     i, g = idx.reshape(-1, k), dweights.float().reshape(-1, k) * scale
     if sigmoid:
-        s = 1 / (1 + torch.exp(-x.gather(1, i)))
+        xc = x.gather(1, i)
+        s, rest = 1 / (1 + torch.exp(-xc)), 1 / (1 + torch.exp(xc))  # (rest: 1 - s, also where s rounds to 1)
         if renormalize:
             total = s.sum(-1, keepdim=True)
-            g = torch.where(total == 0, 0.0, (g - (g * s / total).sum(-1, keepdim=True)) / total)
-        dx = torch.zeros_like(x).scatter(1, i, g * s * (1 - s))
+            g = torch.where(total == 0, 0.0, (g - (g * (s / total)).sum(-1, keepdim=True)) / total)
+        dx = torch.zeros_like(x).scatter(1, i, g * s * rest)
     elif renormalize:
         p = _route_scores(x.gather(1, i), False)
         dx = torch.zeros_like(x).scatter(1, i, p * (g - (g * p).sum(-1, keepdim=True)))
@@ -276,20 +277,17 @@ def moe_route(logits, top_k: int, score: str = "softmax", bias=None, num_groups:
     """(gate weights [.., top_k] fp32, experts [.., top_k] int64) from router logits [.., E] (bf16 or fp32); ``bias`` [E] fp32 enters the choice
     alone.  The weights are differentiable with respect to the logits."""
     E = logits.shape[-1] if logits.ndim else 0
-
-    def need(ok, what):
-        if not ok:
-            raise ValueError(f"moe_route: {what}")
-
-    need(logits.dtype in (torch.bfloat16, torch.float32), f"logits are {logits.dtype}; bf16 or fp32 expected")
-    need(score in ("softmax", "sigmoid"), f"score is 'softmax' or 'sigmoid', not {score!r}")
-    need(1 <= E <= ROUTE_MAX_EXPERTS, f"{E} experts (1 to {ROUTE_MAX_EXPERTS})")
-    need(1 <= num_groups <= min(E, ROUTE_MAX_GROUPS) and E % num_groups == 0, f"{E} experts in {num_groups} groups (at most {ROUTE_MAX_GROUPS} equal ones)")
-    need(1 <= top_groups <= num_groups, f"{top_groups} of {num_groups} groups")
-    need(1 <= top_k <= min(ROUTE_MAX_CHOICES, top_groups * (E // num_groups)),
-         f"{top_k} choices out of {top_groups * (E // num_groups)} experts (at most {ROUTE_MAX_CHOICES})")
-    need(bias is None or (tuple(bias.shape) == (E,) and bias.dtype == torch.float32 and bias.device == logits.device),
-         f"bias is fp32 [{E}] on the logits' device")
+    size = E // num_groups if num_groups > 0 else 0
+    # (one test for the calls that are right: this is the path of single tokens)
+    if not (logits.dtype in (torch.bfloat16, torch.float32) and score in ("softmax", "sigmoid") and 1 <= E <= ROUTE_MAX_EXPERTS
+            and 1 <= num_groups <= ROUTE_MAX_GROUPS and size * num_groups == E and 1 <= top_groups <= num_groups
+            and 1 <= top_k <= ROUTE_MAX_CHOICES and top_k <= top_groups * size
+            and (bias is None or (bias.shape == (E,) and bias.dtype == torch.float32 and bias.device == logits.device))):
+        raise ValueError(
+            f"moe_route: logits [.., E] in bf16 or fp32 with at most {ROUTE_MAX_EXPERTS} experts (here {tuple(logits.shape)} {logits.dtype}), score 'softmax' or "
+            f"'sigmoid' ({score!r}), at most {ROUTE_MAX_GROUPS} equal groups and as many top groups ({num_groups}, {top_groups}), at most "
+            f"{ROUTE_MAX_CHOICES} choices and as many experts in the top groups ({top_k}), a bias in fp32 [E] on the logits' device "
+            f"({None if bias is None else (tuple(bias.shape), bias.dtype, bias.device)})")
     return ops.moe_route(logits, bias, top_k, score == "sigmoid", num_groups, top_groups, renormalize, float(scale))
 
 

@@ -108,7 +108,7 @@ def _dequantize(codes, scales, k, dtype):
 
 
 def _round(x, dim):
-    if dim in (-2, x.ndim - 2):
+    if dim == -2:
         return _round(x.transpose(-1, -2), -1).transpose(-1, -2).contiguous()
     return _values(*_blocks(x))[..., : x.shape[-1]].to(x.dtype).contiguous()
 
@@ -272,11 +272,18 @@ def mx4_mm(a, a_scales, b, b_scales, out_dtype: torch.dtype = torch.bfloat16) ->
 def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x`` [.., K] (rounded to 4 bits on the way) by weights ``mx4_quantize(w)`` of ``w`` [N, K] -> [.., N]; with weights of experts [E, N, K],
     ``x`` [E, M, K] -> [E, M, N].  The result has ``x``'s type unless another is asked for."""
-    _check_float("mx4_linear", x=x)
-    _check_codes("mx4_linear", codes, scales)
-    _need(x.ndim >= 1 and padded(x.shape[-1]) == 2 * codes.shape[-1], f"mx4_linear: x {tuple(x.shape)} and codes {tuple(codes.shape)} do not multiply")
-    _need(codes.ndim == 2 or (x.ndim == 3 and x.shape[0] == codes.shape[0]), f"mx4_linear: weights of {codes.shape[0]} experts take x [E, M, K], not {tuple(x.shape)}")
-    return ops.mx4_linear(x, codes, scales, _out_dtype("mx4_linear", out_dtype, x.dtype))
+    dtype = out_dtype or x.dtype
+    xs, cs = x.shape, codes.shape
+    # (one test for the calls that are right: this is the path of single tokens)
+    if not (x.dtype in _FLOATS and dtype in _FLOATS and codes.dtype is scales.dtype is torch.uint8 and xs and len(cs) in (2, 3)
+            and (xs[-1] + 31) // 32 * 16 == cs[-1] and tuple(scales.shape) == (*cs[:-2], *scale_shape(cs[-2], xs[-1]))
+            and (len(cs) == 2 or (len(xs) == 3 and xs[0] == cs[0]))):
+        _check_float("mx4_linear", x=x)
+        _check_codes("mx4_linear", codes, scales)
+        _need(x.ndim >= 1 and padded(xs[-1]) == 2 * cs[-1], f"mx4_linear: x {tuple(xs)} and codes {tuple(cs)} do not multiply")
+        _need(codes.ndim == 2 or (x.ndim == 3 and xs[0] == cs[0]), f"mx4_linear: weights of {cs[0]} experts take x [E, M, K], not {tuple(xs)}")
+        _out_dtype("mx4_linear", dtype, None)
+    return ops.mx4_linear(x, codes, scales, dtype)
 
 
 def mx4_matmul(x: torch.Tensor, w: torch.Tensor, trans_b: bool = True, out_dtype: torch.dtype | None = None) -> torch.Tensor:

@@ -72,6 +72,13 @@ def _flops(op, args, in_shapes: list[list[int]], out_shapes: list[list[int]]) ->
     if op is apb.grouped_mm_wgrad.default:
         a, b = in_shapes[0], in_shapes[1]
         return 2.0 * _numel(a) * b[2]
+    # 4-bit products run at four times the 16-bit rate that the operations are divided by
+    if op is apb.mx4_matmul.default:
+        return 0.5 * _numel(in_shapes[0]) * in_shapes[1][-2 if args[2] else -1]
+    if op is apb.mx4_linear.default:
+        return 0.5 * _numel(in_shapes[0]) * in_shapes[1][-2]
+    if op is apb.mx4_mm.default:
+        return 0.5 * 2 * _numel(in_shapes[0]) * in_shapes[2][-2]
     if op is apb.gemm.default or op is aten.mm.default:
         a = in_shapes[0]
         return 2.0 * _numel(a) * out_shapes[0][-1] if op is aten.mm.default else 2.0 * _numel(a) * out_shapes[0][-1]

@@ -40,6 +40,7 @@ _EXPENSIVE = {
     apb.mm_nd.default,
     apb.mm_wgrad.default,
     apb.gemm.default,
+    apb.mx4_matmul.default,
     apb.attention.default,
     aten.mm.default,
     aten.bmm.default,

@@ -252,6 +252,87 @@ def _grouped_mm_wgrad(ctx):
     return expand_rows(ctx, [(S(0), S(0), S(0)), (P, S(1), S(1)), (S(1), S(2), R), (S(2), R, S(2))])
 
 
+# ---- routing and MXFP4 products (ops/moe_ops.py, ops/mx4_ops.py).  A 4-bit matrix is split where the pieces are matrices of the same layout by
+# themselves: rows and columns in whole scale tiles of 128, and the blocked dim of 16-bit operands in whole blocks of 32, which are rounded one by one.
+def _splits(ctx, extent, unit):
+    return extent % (unit * ctx.mesh.size()) == 0
+
+
+@register_rule(apb.moe_route.default)
+def _moe_route(ctx):
+    # (weights, idx, logits[, bias]): a token's experts stay together
+    return expand_rows(ctx, [(S(i),) * 3 + (R,) * (len(ctx.in_vals) - 1) for i in _lead_dims(ctx.in_vals[0])])
+
+
+@register_rule(apb.moe_route_bwd.default)
+def _moe_route_bwd(ctx):
+    return expand_rows(ctx, [(S(i),) * 4 for i in _lead_dims(ctx.in_vals[0])])
+
+
+@register_rule(apb.mx4_round.default)
+def _mx4_round(ctx):
+    x = ctx.in_vals[0]
+    blocked = x.ndim + ctx.args[1]
+    return expand_rows(ctx, [(S(i), S(i)) for i in range(x.ndim) if i != blocked or _splits(ctx, x.shape[i], 32)])
+
+
+@register_rule(apb.mx4_quantize.default)
+def _mx4_quantize(ctx):
+    # (codes, scales, x): the scales' tiles of rows and of columns are dims of their own
+    x = ctx.in_vals[0]
+    return expand_rows(ctx, [(S(i),) * 3 for i in range(x.ndim) if i < x.ndim - 2 or _splits(ctx, x.shape[i], 128)])
+
+
+@register_rule(apb.mx4_dequantize.default)
+def _mx4_dequantize(ctx):
+    # (values, codes, scales); the columns are counted in an argument and stay whole
+    codes = ctx.in_vals[0]
+    return expand_rows(ctx, [(S(i),) * 3 for i in _lead_dims(codes) if i < codes.ndim - 2 or _splits(ctx, codes.shape[i], 128)])
+
+
+@register_rule(apb.mx4_mm.default)
+def _mx4_mm(ctx):
+    # (out, a, scales of a, b, scales of b)
+    a, _, b, _ = ctx.in_vals
+    m, k = a.ndim - 2, a.ndim - 1
+    rows = [(S(0),) * 5] if a.ndim == 3 else []
+    if _splits(ctx, a.shape[m], 128):
+        rows.append((S(m), S(m), S(m), R, R))
+    if _splits(ctx, b.shape[m], 128):
+        rows.append((S(k), R, R, S(m), S(m)))
+    if _splits(ctx, 2 * a.shape[k], 128):
+        rows.append((P, S(k), S(k), S(k), S(k)))
+    return expand_rows(ctx, rows)
+
+
+@register_rule(apb.mx4_linear.default)
+def _mx4_linear(ctx):
+    # (y, x, codes, scales)
+    x, codes, _ = ctx.in_vals
+    grouped, last, n = codes.ndim == 3, x.ndim - 1, codes.ndim - 2
+    rows = [(S(0),) * 4] if grouped else []
+    rows += [(S(i), S(i), R, R) for i in range(1 if grouped else 0, last)]
+    if _splits(ctx, codes.shape[n], 128):
+        rows.append((S(last), R, S(n), S(n)))
+    if _splits(ctx, x.shape[last], 128):
+        rows.append((P, S(last), S(n + 1), S(n + 1)))
+    return expand_rows(ctx, rows)
+
+
+@register_rule(apb.mx4_matmul.default)
+def _mx4_matmul(ctx):
+    # like mm_nd and grouped_mm; the contraction in whole blocks
+    x, w = ctx.in_vals
+    grouped, last = w.ndim == 3, x.ndim - 1
+    kdim, ndim = (w.ndim - 1, w.ndim - 2) if ctx.args[2] else (w.ndim - 2, w.ndim - 1)
+    rows = [(S(0), S(0), S(0))] if grouped else []
+    rows += [(S(i), S(i), R) for i in range(1 if grouped else 0, last)]
+    rows.append((S(last), R, S(ndim)))
+    if _splits(ctx, x.shape[last], 32):
+        rows.append((P, S(last), S(kdim)))
+    return expand_rows(ctx, rows)
+
+
 @register_rule(apb.embedding.default)
 def _embedding(ctx):
     # (out [*ids, D], weight [V, D], ids): split the tokens, or the hidden dim of the table; a table split by rows
