@@ -67,7 +67,114 @@ __device__ __forceinline__ MxTile mx_tile(const MxParams& p, uint8_t** scale_til
   if (p.scales != nullptr) *scale_tile = p.scales + t * 512;  // (tiles lie in the order of the grid)
   return {rest / p.row_tiles, rt * MX_TILE, kt * MX_TILE};
 }
-// Unit stride along K.  A thread has 32 bytes of a row (16 bf16 or 8 fp32), two or four threads a block; the loads of four rows are under way together.
+// 32 bytes of a row (16 bf16 or 8 fp32, a half or a quarter of a block; the block's other threads are neighbours): the block's scale code, and the
+// codes, or (``VALUES``) the values in place of what came in.
+template <typename T, bool VALUES>
+__device__ __forceinline__ uint32_t mx_round_32(uint32_t (&u)[8], uint32_t (&packed)[4 / (int)sizeof(T)]) {
+  constexpr int PER = 32 / (int)sizeof(T);
+  uint32_t m = 0;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) m = mx_word_max<T>(m, u[c]);
+  uint32_t amax = mx_word_max_bits<T>(m);
+#pragma unroll
+  for (int d = 1; d < 32 / PER; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+  const uint32_t code = mx_scale_code(amax);
+#pragma unroll
+  for (int h = 0; h < PER / 8; ++h) {
+    float v[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = mx_word_value<T>(u, 8 * h + c);
+    packed[h] = mx_encode_block(v, code);
+    if (VALUES) {
+      mx_decode(packed[h], mx_scale(code), v);
+      if constexpr (PER == 8) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) u[c] = __float_as_uint(v[c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) u[4 * h + c] = pack_bf16(v[2 * c], v[2 * c + 1]);
+      }
+    }
+  }
+  return code;
+}
+template <int PER>
+__device__ __forceinline__ void mx_store_codes(const MxParams& p, const MxTile& at, int r, int k, int kp, const uint32_t (&packed)[PER / 8]) {
+  if (r >= p.R || k >= kp) return;
+  uint8_t* dst = p.codes + (at.g * p.R + r) * (kp / 2) + k / 2;
+  if constexpr (PER == 16) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
+  else *reinterpret_cast<uint32_t*>(dst) = packed[0];
+}
+
+// Rows of 128 columns in shared memory, 16 bytes apart from the next but one's banks.
+template <typename T>
+constexpr int mx_pitch() { return MX_TILE * (int)sizeof(T) + 16; }
+
+// A row of the tile between memory and shared memory, a warp, element by element: for rows that begin anywhere.
+template <typename T>
+__device__ __forceinline__ void mx_row_in(T* row, const T* src, int columns, int lane) {
+#pragma unroll
+  for (int c = 0; c < MX_TILE; c += 32) row[c + lane] = c + lane < columns ? src[c + lane] : T(0.f);
+}
+template <typename T>
+__device__ __forceinline__ void mx_row_out(T* dst, const T* row, int columns, int lane) {
+#pragma unroll
+  for (int c = 0; c < MX_TILE; c += 32)
+    if (c + lane < columns) dst[c + lane] = row[c + lane];
+}
+
+// Unit stride along K, rows that are no whole 16 bytes: 32 rows at a time through shared memory, read and written element by element but in whole sectors.
+template <typename T, bool ROUND>
+__global__ void __launch_bounds__(MX_THREADS) mx4_rows_any_kernel(MxParams p) {
+  after_previous();
+  constexpr int PER = 32 / (int)sizeof(T), ROW_THREADS = MX_TILE / PER, CHUNK = 32;
+  __shared__ __align__(16) uint8_t tile[512];
+  __shared__ __align__(16) uint8_t rows[CHUNK * mx_pitch<T>()];
+  uint8_t* scale_tile = nullptr;
+  const MxTile at = mx_tile(p, &scale_tile);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kp = (p.K + 31) / 32 * 32, columns = min(MX_TILE, p.K - at.k0);
+  const T* x = reinterpret_cast<const T*>(p.x) + at.g * p.gs + at.k0;
+  T* y = reinterpret_cast<T*>(p.y) + at.g * p.R * (long long)p.K + at.k0;
+  auto row = [&](int r) { return reinterpret_cast<T*>(rows + r * mx_pitch<T>()); };
+  for (int r0 = 0; r0 < MX_TILE; r0 += CHUNK) {
+    if (at.r0 + r0 < p.R) {
+#pragma unroll
+      for (int i = 0; i < CHUNK / 8; ++i) {
+        const int r = at.r0 + r0 + warp + 8 * i;
+        mx_row_in(row(warp + 8 * i), x + r * p.ld, r < p.R ? columns : 0, lane);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < CHUNK * ROW_THREADS / MX_THREADS; ++i) {
+      const int rr = i * (MX_THREADS / ROW_THREADS) + threadIdx.x / ROW_THREADS, col = threadIdx.x % ROW_THREADS * PER, r = at.r0 + r0 + rr, k = at.k0 + col;
+      uint4* own = reinterpret_cast<uint4*>(rows + rr * mx_pitch<T>() + col * sizeof(T));
+      uint32_t u[8], packed[PER / 8];
+      const uint4 a = own[0], b = own[1];
+      u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w, u[4] = b.x, u[5] = b.y, u[6] = b.z, u[7] = b.w;
+      const uint32_t code = mx_round_32<T, ROUND>(u, packed);
+      if (ROUND) {
+        own[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        own[1] = make_uint4(u[4], u[5], u[6], u[7]);
+      } else {
+        mx_store_codes<PER>(p, at, r, k, kp, packed);
+        if (col % 32 == 0) tile[mx_scale_at(r0 + rr, col / 32)] = (uint8_t)(r < p.R && k < kp ? code : 127u);
+      }
+    }
+    __syncthreads();
+    if (ROUND) {
+#pragma unroll
+      for (int i = 0; i < CHUNK / 8; ++i) {
+        const int r = at.r0 + r0 + warp + 8 * i;
+        if (r < p.R) mx_row_out(y + (long long)r * p.K, row(warp + 8 * i), columns, lane);
+      }
+      __syncthreads();
+    }
+  }
+  if (!ROUND && threadIdx.x < 128) reinterpret_cast<uint32_t*>(scale_tile)[threadIdx.x] = reinterpret_cast<const uint32_t*>(tile)[threadIdx.x];
+}
+
+// Unit stride along K, rows of whole 16 bytes.  A thread has 32 bytes of a row (16 bf16 or 8 fp32), two or four threads a block; the loads of four rows are under way together.
 // ROUND: the values in place of codes and scales.
 template <typename T, bool ROUND>
 __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
@@ -94,66 +201,27 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
       for (int c = 0; c < 8; ++c) u[i][c] = 0;
       if (r < p.R) {
         const T* src = x + r * p.ld + k;
-        if (p.vec) {
-          if (k + PER <= p.K) {
-            load32(src, p.vec > 1, u[i]);
-          } else if (k < p.K) {  // (rows of whole 16 bytes)
-            const uint4 v = *reinterpret_cast<const uint4*>(src);
-            u[i][0] = v.x, u[i][1] = v.y, u[i][2] = v.z, u[i][3] = v.w;
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < PER; ++c)
-            if (k + c < p.K) mx_put(u[i], c, src[c]);
+        if (k + PER <= p.K) {
+          load32(src, p.vec > 1, u[i]);
+        } else if (k < p.K) {  // (rows of whole 16 bytes)
+          const uint4 v = *reinterpret_cast<const uint4*>(src);
+          u[i][0] = v.x, u[i][1] = v.y, u[i][2] = v.z, u[i][3] = v.w;
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const int rr = r_first + PASS * (pass + i), r = at.r0 + rr;
-      uint32_t m = 0;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) m = mx_word_max<T>(m, u[i][c]);
-      uint32_t amax = mx_word_max_bits<T>(m);
-#pragma unroll
-      for (int d = 1; d < 32 / PER; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-      const uint32_t code = mx_scale_code(amax);
       const bool in = r < p.R && k < kp;
       uint32_t packed[PER / 8];
-#pragma unroll
-      for (int h = 0; h < PER / 8; ++h) {
-        float v[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = mx_word_value<T>(u[i], 8 * h + c);
-        packed[h] = mx_encode_block(v, code);
-        if (ROUND) {
-          mx_decode(packed[h], mx_scale(code), v);
-          if constexpr (PER == 8) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) u[i][c] = __float_as_uint(v[c]);
-          } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) u[i][4 * h + c] = pack_bf16(v[2 * c], v[2 * c + 1]);
-          }
-        }
-      }
+      const uint32_t code = mx_round_32<T, ROUND>(u[i], packed);
       if (ROUND) {
         T* dst = reinterpret_cast<T*>(p.y) + (at.g * p.R + r) * p.K + k;
         if (!in) continue;
-        if (p.vec) {
-          if (k + PER <= p.K) store32(dst, p.vec > 1, u[i]);
-          else if (k < p.K) *reinterpret_cast<uint4*>(dst) = make_uint4(u[i][0], u[i][1], u[i][2], u[i][3]);
-        } else {
-#pragma unroll
-          for (int c = 0; c < PER; ++c)
-            if (k + c < p.K) store1(dst + c, mx_word_value<T>(u[i], c));
-        }
+        if (k + PER <= p.K) store32(dst, p.vec > 1, u[i]);
+        else if (k < p.K) *reinterpret_cast<uint4*>(dst) = make_uint4(u[i][0], u[i][1], u[i][2], u[i][3]);
       } else {
-        if (in) {
-          uint8_t* dst = p.codes + (at.g * p.R + r) * (kp / 2) + k / 2;
-          if constexpr (PER == 16) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
-          else *reinterpret_cast<uint32_t*>(dst) = packed[0];
-        }
+        mx_store_codes<PER>(p, at, r, k, kp, packed);
         if (col % 32 == 0) tile[mx_scale_at(rr, col / 32)] = (uint8_t)(in ? code : 127u);
       }
     }
@@ -178,7 +246,18 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_columns_kernel(MxParams p) {
   const T* x = reinterpret_cast<const T*>(p.x) + at.g * p.gs + r;
   uint32_t u[32][W];
   const bool whole = p.vec && k + 32 <= p.K && r < p.R;
-  if (whole) {
+  if (!p.vec && k + 32 <= p.K && r + 1 < p.R) {  // (a column begins anywhere)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const T* src = x + (long long)(k + i) * p.ld;
+      if constexpr (W == 2) {
+        u[i][0] = __float_as_uint(src[0]);
+        u[i][1] = __float_as_uint(src[1]);
+      } else {
+        u[i][0] = __bfloat16_as_ushort(src[0]) | (uint32_t)__bfloat16_as_ushort(src[1]) << 16;
+      }
+    }
+  } else if (whole) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const T* src = x + (long long)(k + i) * p.ld;
@@ -264,11 +343,13 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_columns_kernel(MxParams p) {
   }
 }
 
-// A thread has 16 values of a row: 8 bytes of codes, all its rows under way together.
-template <typename T>
+// A thread has 16 values of a row: 8 bytes of codes, all its rows under way together.  STAGED: rows that are no whole 16 bytes leave through shared
+// memory, element by element but in whole sectors.
+template <typename T, bool STAGED>
 __global__ void __launch_bounds__(MX_THREADS) mx4_dequantize_kernel(MxParams p) {
   after_previous();
   __shared__ __align__(16) uint8_t tile[512];
+  __shared__ __align__(16) uint8_t rows[STAGED ? 32 * mx_pitch<T>() : 16];
   uint8_t* scale_tile = nullptr;
   const MxTile at = mx_tile(p, &scale_tile);
   if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(tile)[threadIdx.x] = reinterpret_cast<const uint32_t*>(scale_tile)[threadIdx.x];
@@ -284,29 +365,44 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_dequantize_kernel(MxParams p) 
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int rr = r_first + 32 * i, r = at.r0 + rr;
-    if (r >= p.R || k >= p.K) continue;
-    const float scale = mx_scale(tile[mx_scale_at(rr, col / 32)]);
+    constexpr int PER = 32 / (int)sizeof(T);
     float v[16];
+    const float scale = mx_scale(tile[mx_scale_at(rr, col / 32)]);
     float (&lo)[8] = *reinterpret_cast<float (*)[8]>(v), (&hi)[8] = *reinterpret_cast<float (*)[8]>(v + 8);
     mx_decode(packed[i].x, scale, lo);
     mx_decode(packed[i].y, scale, hi);
-    T* dst = reinterpret_cast<T*>(p.y) + (at.g * p.R + r) * p.K + k;
-    if (p.vec && k + 16 <= p.K) {
-      constexpr int PER = 32 / (int)sizeof(T);
+    uint32_t u[16 / PER][8];
+#pragma unroll
+    for (int h = 0; h < 16 / PER; ++h)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if constexpr (PER == 8) u[h][c] = __float_as_uint(v[8 * h + c]);
+        else u[h][c] = pack_bf16(v[2 * c], v[2 * c + 1]);
+      }
+    if (STAGED) {
+      uint4* own = reinterpret_cast<uint4*>(rows + r_first * mx_pitch<T>() + col * sizeof(T));
 #pragma unroll
       for (int h = 0; h < 16 / PER; ++h) {
-        uint32_t u[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          if constexpr (PER == 8) u[c] = __float_as_uint(v[8 * h + c]);
-          else u[c] = pack_bf16(v[2 * c], v[2 * c + 1]);
-        }
-        store32(dst + PER * h, p.vec > 1, u);
+        own[2 * h] = make_uint4(u[h][0], u[h][1], u[h][2], u[h][3]);
+        own[2 * h + 1] = make_uint4(u[h][4], u[h][5], u[h][6], u[h][7]);
       }
-    } else {
+      __syncthreads();
+      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
-      for (int c = 0; c < 16; ++c)
-        if (k + c < p.K) store1(dst + c, v[c]);
+      for (int j = 0; j < 4; ++j) {
+        const int out = at.r0 + 32 * i + warp + 8 * j;
+        if (out < p.R)
+          mx_row_out(reinterpret_cast<T*>(p.y) + (at.g * p.R + out) * (long long)p.K + at.k0, reinterpret_cast<const T*>(rows + (warp + 8 * j) * mx_pitch<T>()),
+                     min(MX_TILE, p.K - at.k0), lane);
+      }
+      __syncthreads();
+    } else if (r < p.R && k < p.K) {
+      T* dst = reinterpret_cast<T*>(p.y) + (at.g * p.R + r) * p.K + k;
+#pragma unroll
+      for (int h = 0; h < 16 / PER; ++h) {
+        if (k + PER * (h + 1) <= p.K) store32(dst + PER * h, p.vec > 1, u[h]);
+        else if (k + PER * h < p.K) *reinterpret_cast<uint4*>(dst + PER * h) = make_uint4(u[h][0], u[h][1], u[h][2], u[h][3]);  // (rows of whole 16 bytes)
+      }
     }
   }
 }
@@ -337,8 +433,12 @@ static int mx_from_values(MxParams& p, unsigned grid, int transposed, int is_bf1
     // rows that begin on 32 or on 16 bytes, and end there (so do those of the result)
     auto whole = [&](int bytes) { return p.ld * esz % bytes == 0 && p.gs * esz % bytes == 0 && (long long)p.K * esz % bytes == 0 && aligned(p.x, bytes) && (!ROUND || aligned(p.y, bytes)); };
     p.vec = whole(32) ? 2 : whole(16) ? 1 : 0;
-    is_bf16 ? launch_after(mx4_rows_kernel<__nv_bfloat16, ROUND>, grid, MX_THREADS, 0, st, p)
-            : launch_after(mx4_rows_kernel<float, ROUND>, grid, MX_THREADS, 0, st, p);
+    if (p.vec)
+      is_bf16 ? launch_after(mx4_rows_kernel<__nv_bfloat16, ROUND>, grid, MX_THREADS, 0, st, p)
+              : launch_after(mx4_rows_kernel<float, ROUND>, grid, MX_THREADS, 0, st, p);
+    else
+      is_bf16 ? launch_after(mx4_rows_any_kernel<__nv_bfloat16, ROUND>, grid, MX_THREADS, 0, st, p)
+              : launch_after(mx4_rows_any_kernel<float, ROUND>, grid, MX_THREADS, 0, st, p);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
@@ -385,7 +485,11 @@ extern "C" int apb_mx4_dequantize(const void* codes, const void* scales, void* y
   p.y = y;
   const int esz = is_bf16 ? 2 : 4;
   p.vec = K * esz % 32 == 0 && aligned(y, 32) ? 2 : K * esz % 16 == 0 ? 1 : 0;
-  is_bf16 ? launch_after(mx4_dequantize_kernel<__nv_bfloat16>, grid, MX_THREADS, 0, st, p)
-          : launch_after(mx4_dequantize_kernel<float>, grid, MX_THREADS, 0, st, p);
+  if (p.vec)
+    is_bf16 ? launch_after(mx4_dequantize_kernel<__nv_bfloat16, false>, grid, MX_THREADS, 0, st, p)
+            : launch_after(mx4_dequantize_kernel<float, false>, grid, MX_THREADS, 0, st, p);
+  else
+    is_bf16 ? launch_after(mx4_dequantize_kernel<__nv_bfloat16, true>, grid, MX_THREADS, 0, st, p)
+            : launch_after(mx4_dequantize_kernel<float, true>, grid, MX_THREADS, 0, st, p);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }

@@ -225,6 +225,12 @@ def _check_float(name, **tensors):
         _need(t.dtype in _FLOATS, f"{name}: {key} is {t.dtype}; bf16 or fp32 expected")
 
 
+def _are_codes(codes, scales) -> bool:
+    cs = codes.shape
+    return (codes.dtype is scales.dtype is torch.uint8 and 2 <= len(cs) <= 3 and cs[-1] % 16 == 0
+            and scales.shape == (*cs[:-2], (cs[-2] + 127) // 128, (cs[-1] + 63) // 64, 512))
+
+
 def _check_codes(name, codes, scales):
     _need(codes.dtype == torch.uint8 and scales.dtype == torch.uint8, f"{name}: codes and scales are uint8")
     _need(codes.ndim in (2, 3) and codes.shape[-1] % 16 == 0, f"{name}: codes [R, Kp / 2] or [E, R, Kp / 2] of whole blocks, not {tuple(codes.shape)}")
@@ -240,17 +246,21 @@ def _out_dtype(name, dtype, default):
 
 def mx4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of ``x`` [R, K] or [E, R, K]; blocks along the last dim, whose stride may also be that of a transposed matrix."""
-    _check_float("mx4_quantize", x=x)
-    _need(x.ndim in (2, 3), f"mx4_quantize: a matrix or a stack of matrices, not {x.ndim} dims")
+    if not (x.dtype in _FLOATS and 2 <= x.ndim <= 3):
+        _check_float("mx4_quantize", x=x)
+        _need(False, f"mx4_quantize: a matrix or a stack of matrices, not {x.ndim} dims")
     return ops.mx4_quantize(x)
 
 
 def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, k: int | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of codes and scales; ``k``: columns (default: whole blocks)."""
-    _check_codes("mx4_dequantize", codes, scales)
-    k = 2 * codes.shape[-1] if k is None else k
-    _need(padded(k) == 2 * codes.shape[-1], f"mx4_dequantize: {k} columns do not belong to {codes.shape[-1]} bytes a row")
-    return ops.mx4_dequantize(codes, scales, k, _out_dtype("mx4_dequantize", dtype, None))
+    cs = codes.shape
+    k = 2 * cs[-1] if k is None else k
+    if not (_are_codes(codes, scales) and (k + 31) // 32 * 16 == cs[-1] and dtype in _FLOATS):
+        _check_codes("mx4_dequantize", codes, scales)
+        _need(padded(k) == 2 * cs[-1], f"mx4_dequantize: {k} columns do not belong to {cs[-1]} bytes a row")
+        _out_dtype("mx4_dequantize", dtype, None)
+    return ops.mx4_dequantize(codes, scales, k, dtype)
 
 
 def mx4_round(x: torch.Tensor, dim: int = -1) -> torch.Tensor:
@@ -275,8 +285,7 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_d
     dtype = out_dtype or x.dtype
     xs, cs = x.shape, codes.shape
     # (one test for the calls that are right: this is the path of single tokens)
-    if not (x.dtype in _FLOATS and dtype in _FLOATS and codes.dtype is scales.dtype is torch.uint8 and xs and len(cs) in (2, 3)
-            and (xs[-1] + 31) // 32 * 16 == cs[-1] and tuple(scales.shape) == (*cs[:-2], *scale_shape(cs[-2], xs[-1]))
+    if not (x.dtype in _FLOATS and dtype in _FLOATS and _are_codes(codes, scales) and xs and (xs[-1] + 31) // 32 * 16 == cs[-1]
             and (len(cs) == 2 or (len(xs) == 3 and xs[0] == cs[0]))):
         _check_float("mx4_linear", x=x)
         _check_codes("mx4_linear", codes, scales)
@@ -289,8 +298,11 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_d
 def mx4_matmul(x: torch.Tensor, w: torch.Tensor, trans_b: bool = True, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x`` [.., K] by ``w`` ([N, K] if ``trans_b`` else [K, N]), or ``x`` [E, M, K] by ``w`` [E, N, K] / [E, K, N], both rounded to 4 bits
     on the way in blocks along K."""
-    _check_float("mx4_matmul", x=x, w=w)
-    _need(w.ndim == 2 and x.ndim >= 1 or w.ndim == 3 and x.ndim == 3 and x.shape[0] == w.shape[0],
-          f"mx4_matmul: x {tuple(x.shape)}, w {tuple(w.shape)}: [.., K] by a matrix, or [E, M, K] by a stack")
-    _need(x.shape[-1] == w.shape[-1 if trans_b else -2], f"mx4_matmul: x {tuple(x.shape)} and w {tuple(w.shape)} do not multiply")
-    return ops.mx4_matmul(x, w, trans_b, _out_dtype("mx4_matmul", out_dtype, x.dtype))
+    dtype = out_dtype or x.dtype
+    xs, ws = x.shape, w.shape
+    fits = xs and (len(ws) == 2 or (len(ws) == len(xs) == 3 and xs[0] == ws[0])) and xs[-1] == ws[-1 if trans_b else -2]
+    if not (fits and x.dtype in _FLOATS and w.dtype in _FLOATS and dtype in _FLOATS):
+        _check_float("mx4_matmul", x=x, w=w)
+        _need(fits, f"mx4_matmul: x {tuple(xs)}, w {tuple(ws)}: [.., K] by a matrix, or [E, M, K] by a stack, of the same K")
+        _out_dtype("mx4_matmul", dtype, None)
+    return ops.mx4_matmul(x, w, trans_b, dtype)
