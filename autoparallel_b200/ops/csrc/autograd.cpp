@@ -355,6 +355,8 @@ using MxValuesSig = Tensor(const Tensor&, const Tensor&, int64_t, ScalarType);
 using MxLinearSig = Tensor(const Tensor&, const Tensor&, const Tensor&, ScalarType);
 const Op<MxRoundSig>& op_mx_round() { APB_OP(o, "mx4_round", MxRoundSig); return o; }
 const Op<MxValuesSig>& op_mx_values() { APB_OP(o, "mx4_dequantize", MxValuesSig); return o; }
+using MxMmValuesSig = Tensor(const Tensor&, const Tensor&, const Tensor&, int64_t, ScalarType);
+const Op<MxMmValuesSig>& op_mx_mm_values() { APB_OP(o, "mx4_mm_values", MxMmValuesSig); return o; }
 const Op<MxLinearSig>& op_mx_linear() { APB_OP(o, "mx4_linear", MxLinearSig); return o; }
 const Op<MmNdSig>& op_mx_matmul() { APB_OP(o, "mx4_matmul", MmNdSig); return o; }
 
@@ -385,17 +387,15 @@ struct MxLinear : torch::autograd::Function<MxLinear> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     const auto s = ctx->get_saved_variables();
-    const int64_t k = ctx->saved_data["k"].toInt();
-    const Tensor dy = pad_last(g[0]);
-    const Tensor w = pad8(op_mx_values()(s[0], s[1], (k + 31) / 32 * 32, dy.scalar_type()), true, false);
-    return {cut(times(dy, w, false, ctx->saved_data["dtype"].toScalarType()), -1, k), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {op_mx_mm_values()(g[0], s[0], s[1], ctx->saved_data["k"].toInt(), ctx->saved_data["dtype"].toScalarType()), Tensor(), Tensor(), Tensor(),
+            Tensor()};
   }
 };
 Tensor mx4_linear(DispatchKeySet ks, const Tensor& x, const Tensor& codes, const Tensor& scales, ScalarType dtype) {
   return records(x) ? MxLinear::apply(x, codes, scales, dtype, Keys{ks}) : op_mx_linear().below(ks, x, codes, scales, dtype);
 }
-// Saves the operands in 4 bits, which the product needs anyway, and takes the values of the gradients' 16-bit products from them: less memory held, and less
-// to read than the 16-bit operands (64 experts' 2048 x 1408: 76 us, rounding them again 121).
+// Saves the operands in 4 bits, which the product needs anyway, and takes the values of the gradients' products from them: less memory held, and less
+// to read than the 16-bit operands.
 using MxQuantSig = Pair(const Tensor&);
 using MxMmSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, ScalarType);
 const Op<MxQuantSig>& op_mx_quantize() { APB_OP(o, "mx4_quantize", MxQuantSig); return o; }
@@ -423,11 +423,10 @@ struct MxMatmul : torch::autograd::Function<MxMatmul> {
     const auto s = ctx->get_saved_variables();
     const bool tb = ctx->saved_data["tb"].toBool();
     const int64_t k = ctx->saved_data["k"].toInt(), kp = (k + 31) / 32 * 32, n = ctx->saved_data["n"].toInt();
-    const Tensor dy = pad_last(g[0]);
     Tensor dx, dw;
-    if (ctx->needs_input_grad(0))
-      dx = cut(times(dy, pad8(op_mx_values()(s[2], s[3], kp, dy.scalar_type()), true, false), false, ctx->saved_data["x"].toScalarType()), -1, k);
+    if (ctx->needs_input_grad(0)) dx = op_mx_mm_values()(g[0], s[2], s[3], k, ctx->saved_data["x"].toScalarType());
     if (ctx->needs_input_grad(1)) {
+      const Tensor dy = pad_last(g[0]);
       const Tensor xq = op_mx_values()(s[0], s[1], kp, dy.scalar_type());  // [rows, kp], or [E, rows, kp]
       const Tensor d = xq.dim() == 3 ? dy : dy.reshape({xq.size(0), dy.size(-1)});
       const Op<WgradSig>& wgrad = xq.dim() == 3 ? op_grouped_wgrad() : op_mm_wgrad();

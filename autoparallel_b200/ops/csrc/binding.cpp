@@ -79,6 +79,9 @@ int apb_gemm_mx4(const void* A, const void* SA, const void* B, const void* SB, v
 int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, int values, int num_sms);
 int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K,
                       long long gs, long long ld, int x_type, int out_fp32, int slices, uint32_t* status, int num_sms, cudaStream_t stream);
+int apb_gemm_mx4_values_takes(long long G, long long M, long long N, long long K);
+int apb_gemm_mx4_values(const void* A, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K, int out_fp32,
+                        uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_symm_header_bytes();
 int apb_symm_wait_probe(const uint32_t* flag, unsigned target, unsigned limit_ms, uint32_t* status, cudaStream_t st);
 int apb_symm_collective(int mode, const unsigned long long* peer_ptrs, int rank, int n, unsigned epoch, const void* src,
@@ -573,13 +576,13 @@ std::map<std::string, std::vector<std::array<int, 3>>> kernel_footprints() {
 enum Entry : int {
   MM_ND, MM_WGRAD, GROUPED_MM, GROUPED_MM_WGRAD, DTYPE_CAST, RMS_NORM, RMS_NORM_BWD, ROPE, SWIGLU, SWIGLU_BWD, CROSS_ENTROPY, CROSS_ENTROPY_BWD,
   EMBEDDING, EMBEDDING_BWD, MOE_SLOTS, MOE_SCATTER, MOE_GATHER, MOE_GATE_GRAD, CAST_MANY, MOE_ROUTE, MOE_ROUTE_BWD, MX4_QUANTIZE, MX4_DEQUANTIZE,
-  MX4_ROUND, MX4_MM, MX4_LINEAR, MX4_MATMUL, NUM_ENTRIES
+  MX4_ROUND, MX4_MM, MX4_LINEAR, MX4_MATMUL, MX4_MM_VALUES, NUM_ENTRIES
 };
 static_assert(NUM_ENTRIES <= 32, "a bit per entry");
 constexpr const char* ENTRY_NAMES[NUM_ENTRIES] = {
     "mm_nd", "mm_wgrad", "grouped_mm", "grouped_mm_wgrad", "dtype_cast", "rms_norm", "rms_norm_bwd", "rope", "swiglu", "swiglu_bwd", "cross_entropy",
     "cross_entropy_bwd", "embedding", "embedding_bwd", "moe_slots", "moe_scatter", "moe_gather", "moe_gate_grad", "cast_many", "moe_route",
-    "moe_route_bwd", "mx4_quantize", "mx4_dequantize", "mx4_round", "mx4_mm", "mx4_linear", "mx4_matmul"};
+    "moe_route_bwd", "mx4_quantize", "mx4_dequantize", "mx4_round", "mx4_mm", "mx4_linear", "mx4_matmul", "mx4_mm_values"};
 struct Native {
   py::object table;  // operator name -> Python function, as it is at the time of a call
   py::object status_buffer;
@@ -995,6 +998,29 @@ Tensor mx4_matmul(const Tensor& x, const Tensor& w, bool trans_b, at::ScalarType
   return mx4_linear(x, b, sb, dtype);
 }
 
+// a [.., N] (bf16) times the values of codes [N, kp / 2], or stacks of both; an empty result: not the kernel's form.
+c10::optional<Tensor> mx4_mm_values(const Tensor& a_, const Tensor& codes_, const Tensor& scales_, int64_t k, at::ScalarType dtype, bool always = false) {
+  c10::cuda::CUDAGuard g(a_.device());
+  mx_codes_check(codes_, scales_, "mx4_mm_values");
+  const int64_t N = codes_.size(-2);
+  TORCH_CHECK(a_.dim() >= 1 && a_.size(-1) == N && k >= 0 && mx_blocks(k) * 16 == codes_.size(-1) && codes_.is_cuda() && codes_.device() == a_.device() &&
+                  (codes_.dim() == 2 || (a_.dim() == 3 && a_.size(0) == codes_.size(0))),
+              "mx4_mm_values: a ", a_.sizes(), ", codes ", codes_.sizes(), ", ", k, " columns");
+  TORCH_CHECK(float_or_bf16(a_.scalar_type()) && float_or_bf16(dtype), "mx4_mm_values: bf16 or fp32");
+  const int64_t G = codes_.dim() == 3 ? codes_.size(0) : 1, M = N == 0 ? 0 : a_.numel() / (G * N > 0 ? G * N : 1);
+  const bool fp32 = dtype == at::kFloat;
+  if (a_.scalar_type() != at::kBFloat16 || N == 0 || N % 8 || !(always || apb_gemm_mx4_values_takes(G, M, N, k))) return c10::nullopt;
+  Tensor a = dense(a_), codes = dense(codes_), scales = dense(scales_);
+  auto shape = a.sizes().vec();
+  shape.back() = k;
+  Tensor c = at::empty(shape, a.options().dtype(dtype));
+  check(apb_gemm_mx4_values(a.data_ptr(), codes.data_ptr(), scales.data_ptr(), c.data_ptr(), G, M, N, k, fp32,
+                            reinterpret_cast<uint32_t*>(status_of(a).data_ptr()), num_sms(), stream()),
+        "apb_gemm_mx4_values");
+  count(c.numel() > 0);
+  return c;
+}
+
 Two op_moe_route(const Tensor& x, const c10::optional<Tensor>& bias, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups, bool renorm,
                  double scale) {
   if (ours(MOE_ROUTE)) return moe_route(x, bias, k, sigmoid, groups, top_groups, renorm, scale);
@@ -1025,6 +1051,14 @@ Tensor op_mx4_matmul(const Tensor& x, const Tensor& w, bool trans_b, at::ScalarT
   if (ours(MX4_MATMUL)) return mx4_matmul(x, w, trans_b, dtype);
   py::gil_scoped_acquire gil;
   return in_python<Tensor>(MX4_MATMUL, x, w, trans_b, py_dtype(dtype));
+}
+Tensor op_mx4_mm_values(const Tensor& a, const Tensor& codes, const Tensor& scales, int64_t k, at::ScalarType dtype) {
+  if (ours(MX4_MM_VALUES)) {
+    auto c = mx4_mm_values(a, codes, scales, k, dtype);
+    if (c.has_value()) return *c;
+  }
+  py::gil_scoped_acquire gil;
+  return in_python<Tensor>(MX4_MM_VALUES, a, codes, scales, k, py_dtype(dtype));
 }
 
 // What register_cuda_impl installed for ``name``: ``on`` if it is not the function that the native entry stands for.
@@ -1076,6 +1110,7 @@ void register_native(py::dict table, py::object status_buffer, bool diag_library
   lib->impl(ENTRY_NAMES[MX4_MM], op_mx4_mm);
   lib->impl(ENTRY_NAMES[MX4_LINEAR], op_mx4_linear);
   lib->impl(ENTRY_NAMES[MX4_MATMUL], op_mx4_matmul);
+  lib->impl(ENTRY_NAMES[MX4_MM_VALUES], op_mx4_mm_values);
 }
 
 }  // namespace
@@ -1140,6 +1175,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return mx4_dequantize(codes, scales, k, fp32 ? at::kFloat : at::kBFloat16);
   });
   m.def("mx4_round", &mx4_round);
+  m.def("mx4_mm_values", [](const Tensor& a, const Tensor& codes, const Tensor& scales, int64_t k, bool fp32, bool always) {  // always: whatever the size
+    return mx4_mm_values(a, codes, scales, k, fp32 ? at::kFloat : at::kBFloat16, always);
+  });
   m.def("mx4_mm", [](const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, bool fp32, int64_t form) {  // form -1: chosen
     return mx4_mm_form(a, sa, b, sb, fp32 ? at::kFloat : at::kBFloat16, form);
   });

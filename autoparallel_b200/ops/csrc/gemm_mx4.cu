@@ -36,57 +36,7 @@ struct MxGemmParams {
 };
 enum : int { MX_SCALAR = 0, MX_STAGED = 1, MX_DIRECT = 2 };
 
-__device__ __forceinline__ void st_32(void* p, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
-               "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-
-// 32 columns of a row straight to C, in whole sectors; ``ncols`` of them lie in the matrix (whole sectors, too).
-__device__ __forceinline__ void mx_store_row(uint8_t* dst, const uint32_t (&r)[32], int ncols, bool fp32) {
-  if (fp32) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 8)
-      if (j < ncols) st_32(dst + 4 * j, r + j);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; j += 16) {
-      uint32_t v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = pack_bf16(__uint_as_float(r[j + 2 * e]), __uint_as_float(r[j + 2 * e + 1]));
-      if (j < ncols) st_32(dst + 2 * j, v);
-    }
-  }
-}
-
-// Epilogue of a warp's 32 rows and ``ncols`` columns (a multiple of 64), 32 at a time: from the first up, or ``down`` from the last; ``release`` as soon
-// as the first 32 that way are in registers.  A load from TMEM takes some 400 cycles under load, so the next 32 columns are on their way while the
-// last are stored.
-template <typename Release>
-__device__ __forceinline__ void mx_store_direct(const MxGemmParams& q, uint8_t* C, uint32_t taddr, int row0, int n0, int ncols, bool down, int lane,
-                                                Release release) {
-  const GemmParams& p = q.p;
-  const int esz = p.out_fp32 ? 4 : 2;
-  const int chunks = ncols / 32, in = row0 + lane < p.M ? p.N - n0 : 0;  // columns of this row that lie in the matrix
-  uint8_t* dst = C + ((row0 + lane) * p.ldc + n0) * esz;
-  auto column = [&](int i) { return (down ? chunks - 1 - i : i) * 32; };
-  uint32_t a[32], b[32];
-  tmem_ld_32x32(taddr + column(0), a);
-  tmem_ld_wait_for(a);
-  release();
-#pragma unroll 1
-  for (int i = 0; i < chunks; i += 2) {
-    tmem_ld_32x32(taddr + column(i + 1), b);
-    mx_store_row(dst + column(i) * esz, a, in - column(i), p.out_fp32);
-    tmem_ld_wait_for(b);
-    const bool more = i + 2 < chunks;
-    if (more) tmem_ld_32x32(taddr + column(i + 2), a);
-    mx_store_row(dst + column(i + 1) * esz, b, in - column(i + 1), p.out_fp32);
-    if (more) tmem_ld_wait_for(a);
-  }
-}
-
-// The same where rows are no whole sectors, 64 columns at a time: through shared memory in 16-byte pieces of whole 128-byte lines, or element by element.
+// The epilogue where rows are no whole sectors (mx_store_direct where they are), 64 columns at a time: through shared memory in 16-byte pieces of whole 128-byte lines, or element by element.
 template <typename Release>
 __device__ __forceinline__ void mx_store_staged(const MxGemmParams& q, uint8_t* C, uint8_t* stg, uint32_t taddr, int row0, int n0, int ncols, bool down,
                                                 int lane, Release release) {
@@ -347,7 +297,7 @@ __device__ __forceinline__ void mx_gemm_cta(const CUtensorMap& tmA, const CUtens
       auto read = [&]() {
         if (mine) release();
       };
-      if (q.store == MX_DIRECT) mx_store_direct(q, C, taddr, row0, col0, cols, buf == 0, lane, read);
+      if (q.store == MX_DIRECT) mx_store_direct(p, C, taddr, row0, col0, cols, buf == 0, lane, read);
       else mx_store_staged(q, C, staging + (warp - 2) * 4096, taddr, row0, col0, cols, buf == 0, lane, read);
     }
   }

@@ -77,6 +77,55 @@ constexpr int MX_SCALE_TILE = 512, MX_STAGE_TILES = 2;
 constexpr int MX_OP_BYTES = 128 * MX_ROW_BYTES;              // 128 rows of an operand
 constexpr int MX_SC_BYTES = MX_STAGE_TILES * MX_SCALE_TILE;  // and their scales
 
+__device__ __forceinline__ void st_32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+               "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// 32 columns of a row straight to C, in whole sectors; ``ncols`` of them lie in the matrix (whole sectors, too).
+__device__ __forceinline__ void mx_store_row(uint8_t* dst, const uint32_t (&r)[32], int ncols, bool fp32) {
+  if (fp32) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8)
+      if (j < ncols) st_32(dst + 4 * j, r + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j += 16) {
+      uint32_t v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = pack_bf16(__uint_as_float(r[j + 2 * e]), __uint_as_float(r[j + 2 * e + 1]));
+      if (j < ncols) st_32(dst + 2 * j, v);
+    }
+  }
+}
+
+// Epilogue of a warp's 32 rows and ``ncols`` columns (a multiple of 64), 32 at a time: from the first up, or ``down`` from the last; ``release`` as soon
+// as the first 32 that way are in registers.  A load from TMEM takes some 400 cycles under load, so the next 32 columns are on their way while the
+// last are stored.
+template <typename Release>
+__device__ __forceinline__ void mx_store_direct(const GemmParams& p, uint8_t* C, uint32_t taddr, int row0, int n0, int ncols, bool down, int lane,
+                                                Release release) {
+  const int esz = p.out_fp32 ? 4 : 2;
+  const int chunks = ncols / 32, in = row0 + lane < p.M ? p.N - n0 : 0;  // columns of this row that lie in the matrix
+  uint8_t* dst = C + ((row0 + lane) * p.ldc + n0) * esz;
+  auto column = [&](int i) { return (down ? chunks - 1 - i : i) * 32; };
+  uint32_t a[32], b[32];
+  tmem_ld_32x32(taddr + column(0), a);
+  tmem_ld_wait_for(a);
+  release();
+#pragma unroll 1
+  for (int i = 0; i < chunks; i += 2) {
+    tmem_ld_32x32(taddr + column(i + 1), b);
+    mx_store_row(dst + column(i) * esz, a, in - column(i), p.out_fp32);
+    tmem_ld_wait_for(b);
+    const bool more = i + 2 < chunks;
+    if (more) tmem_ld_32x32(taddr + column(i + 2), a);
+    mx_store_row(dst + column(i + 1) * esz, b, in - column(i + 1), p.out_fp32);
+    if (more) tmem_ld_wait_for(a);
+  }
+}
+
 // [G][rows][bytes] of codes in boxes of 128 bytes x ``box_rows`` (128-byte swizzle), or [G][row tiles][scale words] in boxes of a stage's words.
 inline int mx_map(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t rows, uint64_t G, uint32_t box_inner, uint32_t box_rows, bool scales) {
   EncodeTiledFn enc = get_encode();

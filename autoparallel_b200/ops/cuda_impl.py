@@ -347,6 +347,19 @@ def _mx4_matmul(x, w, trans_b, out_dtype):
     return _C.mx4_matmul(x, w, trans_b, _fp32_result("mx4_matmul", out_dtype))
 
 
+def _mx4_mm_values(a, codes, scales, k, out_dtype):
+    c = _C.mx4_mm_values(a, codes, scales, k, _fp32_result("mx4_mm_values", out_dtype), False)
+    if c is not None:
+        return c
+    # the values as a matrix of their own (whole blocks, and rows and columns of whole 16 bytes), and the 16-bit product
+    w = _C.mx4_dequantize(codes, scales, 2 * codes.shape[-1], a.dtype is torch.float32)
+    extra = -a.shape[-1] % 8
+    if extra:
+        a, w = torch.nn.functional.pad(a, (0, extra)), torch.nn.functional.pad(w, (0, 0, 0, extra))
+    out = (L.ops.grouped_mm if w.ndim == 3 else L.ops.mm_nd)(a, w, False, out_dtype)
+    return out if out.shape[-1] == k else out[..., :k].contiguous()
+
+
 # ----------------------------------------------------------------------------------- pointwise etc.
 def _dtype_cast(x, dtype):
     if x.dtype == dtype:
@@ -529,6 +542,7 @@ def _register() -> None:
     R("mx4_mm", _mx4_mm)
     R("mx4_linear", _mx4_linear)
     R("mx4_matmul", _mx4_matmul)
+    R("mx4_mm_values", _mx4_mm_values)
     R("dtype_cast", _dtype_cast)
     R("cast_many", _cast_many)
     R("rms_norm", _rms_norm)

@@ -22,6 +22,7 @@ Operators (``apb200::``; the functions below them check arguments and fill in de
     mx4_mm(a, sa, b, sb, dtype)                      a [.., M, K] x b [.., N, K] -> [.., M, N], sums in fp32
     mx4_linear(x, codes, scales, dtype)              activations (rounded on the way) by weights held in 4 bits; gradient of ``x``
     mx4_matmul(x, w, trans_b, dtype)                 both operands rounded on the way; gradients of both
+    mx4_mm_values(a, codes, scales, k, dtype)        a [.., N] (16 or 32 bits) by the values [N, k] of codes: the gradient of ``x`` in the two above
 
 The rounding has no useful derivative; gradients go straight through it: with ``q`` for rounding and ``y = q(x) q(w)^T``,
 ``dx = dy q(w)`` and ``dw = dy^T q(x)``, 16-bit products of the framework's own GEMM.
@@ -46,6 +47,7 @@ lib.define("mx4_round(Tensor x, int dim) -> Tensor")
 lib.define("mx4_mm(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, ScalarType out_dtype) -> Tensor")
 lib.define("mx4_linear(Tensor x, Tensor codes, Tensor scales, ScalarType out_dtype) -> Tensor")
 lib.define("mx4_matmul(Tensor x, Tensor w, bool trans_b, ScalarType out_dtype) -> Tensor")
+lib.define("mx4_mm_values(Tensor a, Tensor codes, Tensor scales, int k, ScalarType out_dtype) -> Tensor")
 
 
 def padded(k: int) -> int:
@@ -129,18 +131,23 @@ def _matmul(x, w, trans_b, out_dtype):
     return torch.matmul(_round(x, -1).float(), wq.transpose(-1, -2) if trans_b else wq).to(out_dtype)
 
 
+def _mm_values(a, codes, scales, k, out_dtype):
+    return torch.matmul(a.float(), _dequantize(codes, scales, k, torch.float32)).to(out_dtype)
+
+
 def _u8(x, *shape):
     return x.new_empty(shape, dtype=torch.uint8)
 
 
 _REFS = {"mx4_quantize": _quantize, "mx4_dequantize": _dequantize, "mx4_round": _round, "mx4_mm": _mm, "mx4_linear": _linear,
-         "mx4_matmul": _matmul}
+         "mx4_matmul": _matmul, "mx4_mm_values": _mm_values}
 _META = {
     "mx4_quantize": lambda x: (_u8(x, *x.shape[:-1], padded(x.shape[-1]) // 2), _u8(x, *x.shape[:-2], *scale_shape(x.shape[-2], x.shape[-1]))),
     "mx4_dequantize": lambda codes, scales, k, dtype: codes.new_empty((*codes.shape[:-1], k), dtype=dtype),
     "mx4_round": lambda x, dim: x.new_empty(x.shape),
     "mx4_mm": lambda a, sa, b, sb, dtype: a.new_empty((*a.shape[:-1], b.shape[-2]), dtype=dtype),
     "mx4_linear": lambda x, codes, scales, dtype: x.new_empty((*x.shape[:-1], codes.shape[-2]), dtype=dtype),
+    "mx4_mm_values": lambda a, codes, scales, k, dtype: a.new_empty((*a.shape[:-1], k), dtype=dtype),
     "mx4_matmul": lambda x, w, trans_b, dtype: x.new_empty((*x.shape[:-1], w.shape[-2 if trans_b else -1]), dtype=dtype),
 }
 for _name, _fn in _REFS.items():
@@ -178,9 +185,7 @@ def _linear_setup(ctx, inputs, output):
 
 def _linear_bwd(ctx, dy):
     codes, scales = ctx.saved_tensors
-    w = ops.mx4_dequantize(codes, scales, padded(ctx.k), dy.dtype)  # (whole blocks: rows of whole 16 bytes)
-    dx = _times(_pad8(dy, -1), _pad8(w, -2), False, ctx.dtype)
-    return (dx[..., : ctx.k] if dx.shape[-1] != ctx.k else dx), None, None, None
+    return ops.mx4_mm_values(dy, codes, scales, ctx.k, ctx.dtype), None, None, None
 
 
 def _matmul_setup(ctx, inputs, output):
@@ -293,6 +298,17 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_d
         _need(codes.ndim == 2 or (x.ndim == 3 and xs[0] == cs[0]), f"mx4_linear: weights of {cs[0]} experts take x [E, M, K], not {tuple(xs)}")
         _out_dtype("mx4_linear", dtype, None)
     return ops.mx4_linear(x, codes, scales, dtype)
+
+
+def mx4_mm_values(a: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, k: int | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``a`` [.., N] by the values [N, k] that codes and scales stand for -> [.., k]; with a stack of codes [E, N, ..], ``a`` [E, M, N] -> [E, M, k]."""
+    _check_float("mx4_mm_values", a=a)
+    _check_codes("mx4_mm_values", codes, scales)
+    k = 2 * codes.shape[-1] if k is None else k
+    _need(padded(k) == 2 * codes.shape[-1], f"mx4_mm_values: {k} columns do not belong to {codes.shape[-1]} bytes a row")
+    _need(a.ndim >= 1 and a.shape[-1] == codes.shape[-2] and (codes.ndim == 2 or a.ndim == 3 and a.shape[0] == codes.shape[0]),
+          f"mx4_mm_values: a {tuple(a.shape)} and codes {tuple(codes.shape)} do not multiply")
+    return ops.mx4_mm_values(a, codes, scales, k, _out_dtype("mx4_mm_values", out_dtype, a.dtype))
 
 
 def mx4_matmul(x: torch.Tensor, w: torch.Tensor, trans_b: bool = True, out_dtype: torch.dtype | None = None) -> torch.Tensor:

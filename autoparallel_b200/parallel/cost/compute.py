@@ -77,6 +77,8 @@ def _flops(op, args, in_shapes: list[list[int]], out_shapes: list[list[int]]) ->
         return 0.5 * _numel(in_shapes[0]) * in_shapes[1][-2 if args[2] else -1]
     if op is apb.mx4_linear.default:
         return 0.5 * _numel(in_shapes[0]) * in_shapes[1][-2]
+    if op is apb.mx4_mm_values.default:
+        return 2.0 * _numel(in_shapes[0]) * args[3]
     if op is apb.mx4_mm.default:
         return 0.5 * 2 * _numel(in_shapes[0]) * in_shapes[2][-2]
     if op is apb.gemm.default or op is aten.mm.default:

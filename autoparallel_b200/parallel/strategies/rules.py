@@ -319,6 +319,18 @@ def _mx4_linear(ctx):
     return expand_rows(ctx, rows)
 
 
+@register_rule(apb.mx4_mm_values.default)
+def _mx4_mm_values(ctx):
+    # (out, a, codes, scales); the columns are counted in an argument and stay whole
+    a, codes, _ = ctx.in_vals
+    grouped, last, n = codes.ndim == 3, a.ndim - 1, codes.ndim - 2
+    rows = [(S(0),) * 4] if grouped else []
+    rows += [(S(i), S(i), R, R) for i in range(1 if grouped else 0, last)]
+    if _splits(ctx, codes.shape[n], 128):
+        rows.append((P, S(last), S(n), S(n)))
+    return expand_rows(ctx, rows)
+
+
 @register_rule(apb.mx4_matmul.default)
 def _mx4_matmul(ctx):
     # like mm_nd and grouped_mm; the contraction in whole blocks

@@ -114,6 +114,7 @@ def test_gradients_go_straight_through(lead, trans_b):
     codes, scales = K.mx4_quantize(w.detach() if trans_b else w.detach().transpose(-1, -2))
     (dl,) = torch.autograd.grad(K.mx4_linear(x, codes, scales), x, dy)
     assert torch.allclose(dl.double(), ref, rtol=1e-5, atol=1e-5)
+    assert torch.allclose(K.mx4_mm_values(dy, codes, scales, k).double(), ref, rtol=1e-5, atol=1e-5)
     (dr,) = torch.autograd.grad(K.mx4_round(x), x, torch.ones_like(x))
     assert (dr == 1).all()
 
@@ -128,6 +129,7 @@ def test_refusals():
         lambda: K.mx4_linear(x.double(), codes, scales), lambda: K.mx4_linear(x, codes, scales, out_dtype=torch.float16),
         lambda: K.mx4_linear(x, codes, scales[..., :100]), lambda: K.mx4_linear(x, codes[None], scales[None]),
         lambda: K.mx4_matmul(x, w, trans_b=False), lambda: K.mx4_matmul(x, w[None]), lambda: K.mx4_matmul(x.half(), w.half()),
+        lambda: K.mx4_mm_values(x, codes, scales), lambda: K.mx4_mm_values(x[:, :8], codes, scales, 100), lambda: K.mx4_mm_values(x[:, :8], codes[None], scales[None]),
         lambda: K.mx4_mm(codes, scales, codes[None], scales[None]), lambda: K.mx4_mm(codes, scales, *K.mx4_quantize(w[:, :32])),
     ):
         with pytest.raises(ValueError, match="mx4_"):
@@ -218,6 +220,8 @@ def test_rules_of_codes(mesh_1d):
         (R,) * 5, (S(1), R, R, S(0), S(0)), (P, S(1), S(1), S(1), S(1))}
     assert found(apb.mx4_linear.default, rules._mx4_linear, w[:64], codes, scales, torch.float32) == {
         (R,) * 4, (S(0), S(0), R, R), (S(1), R, S(0), S(0)), (P, S(1), S(1), S(1))}
+    assert found(apb.mx4_mm_values.default, rules._mx4_mm_values, w[:64], codes, scales, 1024, torch.float32) == {
+        (R,) * 4, (S(0), S(0), R, R), (P, S(1), S(0), S(0))}
     e = torch.randn(8, 16, 64)
     ce, se = apb.mx4_quantize(e)
     assert found(apb.mx4_linear.default, rules._mx4_linear, e, ce, se, torch.float32) == {(R,) * 4, (S(0),) * 4, (S(1), S(1), R, R)}

@@ -201,6 +201,36 @@ def test_gradients(lead, m, n, k, trans_b, dtype):
     assert (dr == 1).all()
 
 
+@pytest.mark.parametrize("E,M,N,k", [(0, 1, 8, 16), (0, 5, 64, 256), (0, 128, 128, 272), (0, 129, 200, 512), (0, 256, 72, 1000), (0, 300, 1408, 2048), (0, 2000, 520, 640),
+                                     (3, 40, 136, 96), (64, 160, 264, 512), (2, 513, 640, 1040)])
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+def test_products_with_the_values_of_codes(kernels, E, M, N, k, out_dtype):
+    """The kernel that turns codes to values on the way (whatever the size), and the operator, against 64 bits; the values themselves bit by bit."""
+    lead = (E,) if E else ()
+    a, w = torch.randn(*lead, M, N, device="cuda", dtype=BF16), randn(*lead, N, k, seed=2)
+    if M == 5:
+        w[3, :32], w[4, :40] = torch.finfo(F32).max, 2.0**-127  # the ends of the scales
+    codes, scales = K.mx4_quantize(w)
+    values = K.mx4_dequantize(codes, scales, k, F32).double()
+    want = a.double() @ values
+    bound = (a.double().abs() @ values.abs()) * (N * 2.0**-24) + (want.abs() * 2.0**-8 if out_dtype == BF16 else 0) + 1e-300
+    for c in (kernels.extension().mx4_mm_values(a, codes, scales, k, out_dtype == F32, True), K.mx4_mm_values(a, codes, scales, k, out_dtype)):
+        if c is None:
+            assert k * (4 if out_dtype == F32 else 2) % 32  # (rows of no whole sectors: the composition)
+            continue
+        near = ((c.double() - want).abs() <= bound) | (c == want.to(F32).to(out_dtype))  # (or both beyond the type's range)
+        assert c.shape == want.shape and c.dtype == out_dtype and near.all()
+    n = min(M, N)
+    eye = torch.eye(N, device="cuda", dtype=BF16)[:n].expand(*lead, n, N).contiguous()
+    c = kernels.extension().mx4_mm_values(eye, codes, scales, k, True, True)
+    if c is not None:
+        assert torch.equal(c.double(), values[..., :n, :])
+    before = K.mx4_mm_values(a, codes, scales, k, F32)
+    w[..., N - 1, k - 1] = torch.nan
+    c, first = K.mx4_mm_values(a, *K.mx4_quantize(w), k, F32), (k - 1) // 32 * 32
+    assert c[..., first:].isnan().all() and torch.equal(c[..., :first], before[..., :first])
+
+
 def test_an_installed_function_is_what_runs():
     from autoparallel_b200.ops import library, register_cuda_impl
 
@@ -225,6 +255,7 @@ def test_native_entries_answer_as_the_python_ones():
     r = torch.randn(6, 16, device="cuda")
     route = library.ops.moe_route(r, None, 4, False, 1, 1, True, 1.0)
     for name, args in (("mx4_quantize", (x,)), ("mx4_dequantize", (*a, 96, BF16)), ("mx4_round", (x, -2)), ("mx4_mm", (*a, *b, F32)),
+                       ("mx4_mm_values", (x.bfloat16(), *K.mx4_quantize(randn(96, 64, seed=2)), 64, BF16)),
                        ("mx4_linear", (x, *b, BF16)), ("mx4_linear", (x[:3], *b, BF16)), ("mx4_matmul", (x, w, True, F32)),
                        ("moe_route", (r, None, 4, False, 1, 1, True, 1.0)), ("moe_route_bwd", (route[0], r, route[1], False, True, 1.0))):
         results = []
