@@ -79,7 +79,7 @@ int apb_gemm_mx4(const void* A, const void* SA, const void* B, const void* SB, v
 int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, int values, int num_sms);
 int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K,
                       long long gs, long long ld, int x_type, int out_fp32, int slices, uint32_t* status, int num_sms, cudaStream_t stream);
-int apb_gemm_mx4_values_takes(long long G, long long M, long long N, long long K);
+int apb_gemm_mx4_values_takes(long long G, long long M, long long K, int num_sms);
 int apb_gemm_mx4_values(const void* A, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K, int out_fp32,
                         uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_symm_header_bytes();
@@ -1009,7 +1009,7 @@ c10::optional<Tensor> mx4_mm_values(const Tensor& a_, const Tensor& codes_, cons
   TORCH_CHECK(float_or_bf16(a_.scalar_type()) && float_or_bf16(dtype), "mx4_mm_values: bf16 or fp32");
   const int64_t G = codes_.dim() == 3 ? codes_.size(0) : 1, M = N == 0 ? 0 : a_.numel() / (G * N > 0 ? G * N : 1);
   const bool fp32 = dtype == at::kFloat;
-  if (a_.scalar_type() != at::kBFloat16 || N == 0 || N % 8 || !(always || apb_gemm_mx4_values_takes(G, M, N, k))) return c10::nullopt;
+  if (a_.scalar_type() != at::kBFloat16 || N == 0 || N % 8 || !(always || apb_gemm_mx4_values_takes(G, M, k, num_sms()))) return c10::nullopt;
   Tensor a = dense(a_), codes = dense(codes_), scales = dense(scales_);
   auto shape = a.sizes().vec();
   shape.back() = k;

@@ -298,7 +298,14 @@ using namespace apb;
 
 extern "C" int apb_gemm_get_reserved_sms();
 
-extern "C" int apb_gemm_mx4_values_takes(long long G, long long M, long long N, long long K) { return 1; }
+// Whether this kernel is the better choice against the values as a matrix of their own and the 16-bit product: with few rows, where the matrix is most of
+// what is moved, and tiles for every SM.  us, this / that: 64 experts of 1408 x 2048, 16 rows 69 / 147, 160 rows 88 / 165, 1280 rows 448 / 392; 16 of 2048 x
+// 2048, 512 rows 73 / 84; one of 4096 x 4096, 2048 rows (128 tiles) 60 / 54, of 4096 x 14336, 1024 rows 116 / 104, of 14336 x 4096, 16 rows (16 tiles)
+// 153 / 48.  Three slots of values for two, sixteen warps for eight change nothing: the MMAs, whose operand of 128 rows comes in 16 of its columns at a time, are
+// the bound.
+extern "C" int apb_gemm_mx4_values_takes(long long G, long long M, long long K, int num_sms) {
+  return M <= 512 && G * ((M + 255) / 256) * ((K + MV_COLS - 1) / MV_COLS) >= num_sms;
+}
 
 // A [G, M, N] bf16 (N % 8 == 0), B codes [G, N, kp / 2] and SB, C [G, M, K]; all dense, 16-byte bases.
 // Returns 0, or an argument / driver / launch error (nothing launched; 3: not this kernel's form).
