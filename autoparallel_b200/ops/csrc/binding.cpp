@@ -1056,6 +1056,20 @@ Tensor op_mx4_mm_values(const Tensor& a, const Tensor& codes, const Tensor& scal
   if (ours(MX4_MM_VALUES)) {
     auto c = mx4_mm_values(a, codes, scales, k, dtype);
     if (c.has_value()) return *c;
+    if (a.scalar_type() == at::kBFloat16 && a.size(-1) % 8 == 0 && a.size(-1) > 0 && !native().diag_library_gemm) {
+      // the values as a matrix of their own (whole blocks: rows of whole 16 bytes), and the 16-bit product
+      Tensor w = mx4_dequantize(codes, scales, 2 * codes.size(-1), at::kBFloat16);
+      if (w.dim() == 2) {
+        c = mm_nd(a, w, false, dtype == at::kFloat, status_of(a));
+      } else {
+        c = at::empty({a.size(0), a.size(1), w.size(2)}, a.options().dtype(dtype));
+        gemm_grouped(dense(a), w, *c, false, true, status_of(a));
+      }
+      if (c.has_value()) {
+        count(c->numel() > 0);
+        return c->size(-1) == k ? *c : c->narrow(-1, 0, k).contiguous();
+      }
+    }
   }
   py::gil_scoped_acquire gil;
   return in_python<Tensor>(MX4_MM_VALUES, a, codes, scales, k, py_dtype(dtype));
