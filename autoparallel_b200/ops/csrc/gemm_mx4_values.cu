@@ -8,6 +8,8 @@
 //
 // B takes the 128 rows of the MMA (twice: a tile has 256 columns of C), A's rows its N, up to 256 and a multiple of 16: an MMA's time is what it reads from
 // shared memory, so that 160 rows cost 160 and not 256.  The two accumulators take all of TMEM, so that what is turned is used by as many rows as there may be.
+// Measured: 64 experts of 1408 x 2048, 160 rows 88 us (0.67 PFLOP/s; 37 % of the tensor cores' cycles, 20 % of DRAM, 45 % of the issue slots), 1280 rows 448
+// (1.05); the MMAs, whose operand of 128 rows is read again for every 16 of its columns, and the turning of codes wait for each other's slots.
 //   warp 0: TMA producer (A, codes, scales) | warp 1: TMEM owner, MMAs | warps 2..9: codes to values, then the tile's epilogue
 #include <algorithm>
 

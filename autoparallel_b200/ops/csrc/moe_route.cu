@@ -1,6 +1,13 @@
 // Routing of tokens to experts: scores, choice of the top k (of the top groups), gate weights, and the gradient of the logits.
 // Semantics in ops/moe_ops.py; everything in fp32, in one pass over the logits.
 //
+// L lanes have a token, V experts each, all in registers; the k best are found by k rounds of "largest, lowest index first".  That takes instructions, and
+// they are the bound, not memory (131072 x 128: 67 % of the issue slots, 13 % of DRAM; backward 52 and 26), so a token has the fewest lanes that hold it.
+//   forward   8192 x 64 bf16, 8 of softmax: 3.0 us, 131072 x 64: 16.7, 131072 x 128, 6: 27.4 (1.5 TB/s); 16383 x 256 fp32 sigmoid, 8 of the 4 best of 8
+//             groups: 22.0, 65536 x 256 bf16 the same way: 53.5, without groups and sigmoid 25.6
+//   backward  2.1, 7.9, 15.6 (4.5 TB/s), 8.0, 13.7, 13.8: the scores are computed again from the logits, which the forward would write as 4 bytes an expert
+//             for this to read; a choice's gradient is written by the lane that has the choice, so there are no atomics
+//
 // This file is compiled without --use_fast_math: the choice between two experts hangs on the last bit of a sigmoid, and has to be the same
 // wherever the formula is evaluated as written (expf, IEEE division, denormals kept).
 #include <cuda_bf16.h>
@@ -448,7 +455,9 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_bwd_kernel(RouteBw
   }
 }
 
-// f(L, V) for the smallest number of lanes that holds the experts, 16 a lane where that is enough, and a choice a lane.
+// f(L, V) for the smallest number of lanes that holds the experts, up to 16 a lane, and a choice a lane.  Forward, us, this / twice the lanes / twice the
+// experts a lane: 131072 x 64 16.7 / 33.3 / 24.3, 131072 x 128 27.4 / 35.6, 65536 x 256 in groups 53.5 / 67.1 / 66.9, without 25.6 / 34.8 / 21.7 (32 experts a
+// lane would be faster there alone).
 template <typename F>
 static int route_shape(int E, int k, F f) {
   auto c = [](auto v) { return v; };

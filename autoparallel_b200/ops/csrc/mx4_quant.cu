@@ -4,7 +4,12 @@
 //   mx4_dequantize  the other way
 //   mx4_round       x -> the values that its codes stand for, x's layout
 //
-// All are bound by memory: a CTA takes a tile of 128 rows x 128 columns, which is one scale tile, and reads and writes whole sectors of it.
+// All are bound by memory: a CTA takes a tile of 128 rows x 128 columns, which is one scale tile, and reads and writes whole sectors of it.  A block's
+// largest magnitude is an integer maximum of the values' bits, its scale a shift of them, the rounding the hardware's conversion (to nearest, ties to
+// even), a value from its code the bits moved to an exponent and one multiplication.
+// Measured for 64 x 1280 x 2048 bf16 (335 MB of values, 89 MB of codes), share of the copy rate: mx4_quantize 75 us (87 %), 64 x 2048 x 1408 with unit stride
+// along the rows 80 (88 %), mx4_dequantize 75 to 80 (85 to 90 %), mx4_round 107 along K (96 %) and 117 to 128 along the rows.  Rows that are no whole 16
+// bytes (16 x 695 x 1429) take 1.5 to 2 times as long per byte.
 // Compiled without --use_fast_math: denormals count.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
