@@ -6,8 +6,8 @@
 // nothing of A.  A cluster of S CTAs takes a slice of K each for one tile of 128 rows of B: with as many CTAs as two to an SM, all of B's bytes that
 // fit the chip's shared memory are on their way as soon as the launch has begun.  The slices' sums meet in shared memory: every CTA sends each other
 // one its share of the rows, and adds up what it gets in the order of the slices - the same result every time.
-// Measured: 1 x 14336 x 4096 from bf16 8.0 us (31 MB of weights: 3.9 TB/s, 60 % of the copy rate; a launch with its TMEM, first bytes and last stores is
-// 3 of them), 17 x 4096 x 14336 from codes 9.4, 32 x 4096 x 4096 7.1.
+// Measured: 1 x 14336 x 4096 from bf16 8.0 us with the weights in L2, 9.9 from memory (31 MB: 3.2 TB/s; a launch with its TMEM, first bytes and last stores is
+// 3 us), 17 x 4096 x 14336 from codes 9.4, 32 x 4096 x 4096 7.1; 64 experts of 1408 x 2048, one row each, from memory 24.6 (4.0 TB/s).
 //   warp 0: TMA producer | warp 1: TMEM owner, scale copies, MMAs | warps 2..9: rounding of A, a stage a warp, then the epilogue
 #include <algorithm>
 
@@ -280,6 +280,10 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_const
   }
   tc_fence_before();
   __syncthreads();
+  if (p.slices > 1 && *abort_flag) {  // (one that gave up waiting: the others, which may still write to it, leave or come here first)
+    cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, S::COLS);
