@@ -75,7 +75,8 @@ class MoEConfig:
     router_top_groups: int = 1
     router_renormalize: bool = True
     router_scale: float = 1.0
-    #: "bf16", or "mx4": the routed experts' products in microscaled 4-bit floating point (``ops.mx4_matmul``), gradients straight through the rounding
+    #: "bf16", or "mx4": the routed experts' products in microscaled 4-bit floating point (``ops.mx4_matmul``), gradients straight through
+    #: the rounding
     expert_format: str = "bf16"
     dispatch_blocks: int = 8  # planner mode: token blocks with their own per-expert capacity (a multiple of the shard count)
 
@@ -199,7 +200,8 @@ class MoEFFN(nn.Module):
         """Gate weights and experts [.., top_k] of the tokens ``x`` [.., d]."""
         cfg = self.cfg
         if cfg.router_score is not None:
-            return K.moe_route(self.router(x), cfg.top_k, score=cfg.router_score, bias=self.router_bias.float(), num_groups=cfg.router_groups,
+            return K.moe_route(self.router(x), cfg.top_k, score=cfg.router_score, bias=self.router_bias.float(),
+                               num_groups=cfg.router_groups,
                                top_groups=cfg.router_top_groups, renormalize=cfg.router_renormalize, scale=cfg.router_scale)
         scores = torch.softmax((self.router(x).float() + self.router_bias), dim=-1)
         gate_w, gate_idx = torch.topk(scores, cfg.top_k, dim=-1)

@@ -237,7 +237,8 @@ gemm_mx4_values_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
       tc_fence_after();
       int grp, m0, col;
       place(t, grp, m0, col);
-      const int rows = min(p.M - m0, q.rows), column = col + 128 * half + 32 * quarter + (lane & ~7) + (lane >> 1 & 3) + (lane & 1) * 4, esz = p.out_fp32 ? 4 : 2;
+      const int rows = min(p.M - m0, q.rows), esz = p.out_fp32 ? 4 : 2;
+      const int column = col + 128 * half + 32 * quarter + (lane & ~7) + (lane >> 1 & 3) + (lane & 1) * 4;
       const bool in = column < p.N;
       const long long step = p.ldc * esz;
       uint8_t* C = reinterpret_cast<uint8_t*>(p.C) + (((long long)grp * p.M + m0) * p.ldc + column) * esz;

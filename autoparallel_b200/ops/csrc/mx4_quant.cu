@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_any_kernel(MxParams p) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < CHUNK * ROW_THREADS / MX_THREADS; ++i) {
-      const int rr = i * (MX_THREADS / ROW_THREADS) + threadIdx.x / ROW_THREADS, col = threadIdx.x % ROW_THREADS * PER, r = at.r0 + r0 + rr, k = at.k0 + col;
+      const int rr = i * (MX_THREADS / ROW_THREADS) + threadIdx.x / ROW_THREADS, col = threadIdx.x % ROW_THREADS * PER;
+      const int r = at.r0 + r0 + rr, k = at.k0 + col;
       uint4* own = reinterpret_cast<uint4*>(rows + rr * mx_pitch<T>() + col * sizeof(T));
       uint32_t u[8], packed[PER / 8];
       const uint4 a = own[0], b = own[1];
@@ -179,7 +180,8 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_any_kernel(MxParams p) {
   if (!ROUND && threadIdx.x < 128) reinterpret_cast<uint32_t*>(scale_tile)[threadIdx.x] = reinterpret_cast<const uint32_t*>(tile)[threadIdx.x];
 }
 
-// Unit stride along K, rows of whole 16 bytes.  A thread has 32 bytes of a row (16 bf16 or 8 fp32), two or four threads a block; the loads of four rows are under way together.
+// Unit stride along K, rows of whole 16 bytes.  A thread has 32 bytes of a row (16 bf16 or 8 fp32), two or four threads a block; the loads of four rows are
+// under way together.
 // ROUND: the values in place of codes and scales.
 template <typename T, bool ROUND>
 __global__ void __launch_bounds__(MX_THREADS) mx4_rows_kernel(MxParams p) {
@@ -436,7 +438,9 @@ static int mx_from_values(MxParams& p, unsigned grid, int transposed, int is_bf1
             : launch_after(mx4_columns_kernel<float, ROUND>, grid, MX_THREADS, 0, st, p);
   } else {
     // rows that begin on 32 or on 16 bytes, and end there (so do those of the result)
-    auto whole = [&](int bytes) { return p.ld * esz % bytes == 0 && p.gs * esz % bytes == 0 && (long long)p.K * esz % bytes == 0 && aligned(p.x, bytes) && (!ROUND || aligned(p.y, bytes)); };
+    auto whole = [&](int bytes) {
+      return p.ld * esz % bytes == 0 && p.gs * esz % bytes == 0 && (long long)p.K * esz % bytes == 0 && aligned(p.x, bytes) && (!ROUND || aligned(p.y, bytes));
+    };
     p.vec = whole(32) ? 2 : whole(16) ? 1 : 0;
     if (p.vec)
       is_bf16 ? launch_after(mx4_rows_kernel<__nv_bfloat16, ROUND>, grid, MX_THREADS, 0, st, p)

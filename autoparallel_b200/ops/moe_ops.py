@@ -108,14 +108,14 @@ def _grouped_mm_wgrad(a, b, out_dtype):
 # Scores of the experts, the choice of ``top_k`` of them for every token and their gate weights, from router logits [.., E]:
 #
 #   softmax: choice c = x + bias, score s = softmax(x)        sigmoid: s = 1 / (1 + e^-x), c = s + bias
-#   with groups, the experts are cut into ``num_groups`` equal runs; a group counts as its largest c (softmax) or the sum of its two largest (sigmoid), the
-#   ``top_groups`` best groups stay and the others' experts cannot be chosen;
+#   with groups, the experts are cut into ``num_groups`` equal runs; a group counts as its largest c (softmax) or the sum of its two largest
+#   (sigmoid), the ``top_groups`` best groups stay and the others' experts cannot be chosen;
 #   idx = the experts with the ``top_k`` largest c, descending; w = s[idx], divided by their sum if ``renormalize``, times ``scale``
 #
-# Everything in fp32.  Ties (of experts, of groups) go to the lower index; a NaN counts as larger than everything.  The bias balances the load: it
-# enters the choice alone and has no gradient.  A row of nothing but -inf (all experts masked), and a sum of chosen sigmoid scores that is zero, give
-# weights and gradients of zero.  (Reference: softmax or sigmoid scores, the bias for the choice and the scale in the router of the DeepSeek-V3 test
-# model, autoparallel/_testing/models/dsv3.py:388-444.)
+# Everything in fp32.  Ties (of experts, of groups) go to the lower index; a NaN counts as larger than everything.  The bias balances the
+# load: it enters the choice alone and has no gradient.  A row of nothing but -inf (all experts masked), and a sum of chosen sigmoid scores
+# that is zero, give weights and gradients of zero.  (Reference: softmax or sigmoid scores, the bias for the choice and the scale in the
+# router of the DeepSeek-V3 test model, autoparallel/_testing/models/dsv3.py:388-444.)
 lib.define("moe_route(Tensor logits, Tensor? bias, int top_k, bool sigmoid, int num_groups, int top_groups, bool renormalize, float scale)"
            " -> (Tensor, Tensor)")
 lib.define("moe_route_bwd(Tensor dweights, Tensor logits, Tensor idx, bool sigmoid, bool renormalize, float scale) -> Tensor")
@@ -194,7 +194,8 @@ _REFS = {
     "grouped_mm_wgrad": _grouped_mm_wgrad,
 }
 _META = {
-    "moe_route": lambda x, b, k, *_: (x.new_empty((*x.shape[:-1], k), dtype=torch.float32), x.new_empty((*x.shape[:-1], k), dtype=torch.long)),
+    "moe_route": lambda x, b, k, *_: (x.new_empty((*x.shape[:-1], k), dtype=torch.float32),
+                                      x.new_empty((*x.shape[:-1], k), dtype=torch.long)),
     "moe_route_bwd": lambda dw, x, *_: x.new_empty(x.shape),
     "moe_slots": lambda gi, E, C, nb: gi.new_empty(gi.shape),
     "moe_scatter": lambda src, slot, w, E, C, nb: src.new_empty((E, nb, C, src.shape[1])),
@@ -208,8 +209,8 @@ for _name, _fn in _REFS.items():
     lib.impl(_name, _META[_name], "Meta")
     lib.impl(_name, _make_cuda_entry(_name), "CUDA")
     reference_impls[_name] = _fn
-# On a GPU every operator above resolves to a kernel wrapper of ``ops/cuda_impl.py`` (``csrc/moe_route.cu``, ``csrc/moe_kernels.cu`` for the four index
-# operators, the grouped tcgen05 GEMM for the products); the formulas in this file are their CPU semantics and the GPU tests' oracle.
+# On a GPU every operator above resolves to a kernel wrapper of ``ops/cuda_impl.py`` (``csrc/moe_route.cu``, ``csrc/moe_kernels.cu`` for the
+# four index operators, the grouped tcgen05 GEMM for the products); the formulas in this file are their CPU semantics and the GPU tests' oracle.
 
 
 # ------------------------------------------------------------------------------------ autograd
@@ -274,8 +275,8 @@ _ag("grouped_mm", _gmm_bwd, _gmm_setup)
 # ------------------------------------------------------------------------------------ Python API
 def moe_route(logits, top_k: int, score: str = "softmax", bias=None, num_groups: int = 1, top_groups: int = 1, renormalize: bool = True,
               scale: float = 1.0):
-    """(gate weights [.., top_k] fp32, experts [.., top_k] int64) from router logits [.., E] (bf16 or fp32); ``bias`` [E] fp32 enters the choice
-    alone.  The weights are differentiable with respect to the logits."""
+    """(gate weights [.., top_k] fp32, experts [.., top_k] int64) from router logits [.., E] (bf16 or fp32); ``bias`` [E] fp32 enters the
+    choice alone.  The weights are differentiable with respect to the logits."""
     E = logits.shape[-1] if logits.ndim else 0
     size = E // num_groups if num_groups > 0 else 0
     # (one test for the calls that are right: this is the path of single tokens)
@@ -284,8 +285,8 @@ def moe_route(logits, top_k: int, score: str = "softmax", bias=None, num_groups:
             and 1 <= top_k <= ROUTE_MAX_CHOICES and top_k <= top_groups * size
             and (bias is None or (bias.shape == (E,) and bias.dtype == torch.float32 and bias.device == logits.device))):
         raise ValueError(
-            f"moe_route: logits [.., E] in bf16 or fp32 with at most {ROUTE_MAX_EXPERTS} experts (here {tuple(logits.shape)} {logits.dtype}), score 'softmax' or "
-            f"'sigmoid' ({score!r}), at most {ROUTE_MAX_GROUPS} equal groups and as many top groups ({num_groups}, {top_groups}), at most "
+            f"moe_route: logits [.., E] in bf16 or fp32 with at most {ROUTE_MAX_EXPERTS} experts (here {tuple(logits.shape)} "
+            f"{logits.dtype}), score 'softmax' or 'sigmoid' ({score!r}), at most {ROUTE_MAX_GROUPS} equal groups and as many top groups ({num_groups}, {top_groups}), at most "
             f"{ROUTE_MAX_CHOICES} choices and as many experts in the top groups ({top_k}), a bias in fp32 [E] on the logits' device "
             f"({None if bias is None else (tuple(bias.shape), bias.dtype, bias.device)})")
     return ops.moe_route(logits, bias, top_k, score == "sigmoid", num_groups, top_groups, renormalize, float(scale))

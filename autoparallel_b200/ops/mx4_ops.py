@@ -18,17 +18,17 @@ Operators (``apb200::``; the functions below them check arguments and fill in de
 
     mx4_quantize(x)                                  codes and scales of ``x`` [R, K] or [E, R, K]; blocks along the last dim
     mx4_dequantize(codes, scales, k, dtype)          the values they stand for
-    mx4_round(x, dim)                                the same without the codes: ``x`` with blocks of 32 along ``dim`` (the last, or the one before)
+    mx4_round(x, dim)                                the same without the codes: ``x``, blocks along ``dim`` (the last, or the one before)
     mx4_mm(a, sa, b, sb, dtype)                      a [.., M, K] x b [.., N, K] -> [.., M, N], sums in fp32
     mx4_linear(x, codes, scales, dtype)              activations (rounded on the way) by weights held in 4 bits; gradient of ``x``
     mx4_matmul(x, w, trans_b, dtype)                 both operands rounded on the way; gradients of both
-    mx4_mm_values(a, codes, scales, k, dtype)        a [.., N] (16 or 32 bits) by the values [N, k] of codes: the gradient of ``x`` in the two above
+    mx4_mm_values(a, codes, scales, k, dtype)        a [.., N] (16 or 32 bits) by the values [N, k] of codes: gradients of ``x`` above
 
 The rounding has no useful derivative; gradients go straight through it: with ``q`` for rounding and ``y = q(x) q(w)^T``,
 ``dx = dy q(w)`` and ``dw = dy^T q(x)``, 16-bit products of the framework's own GEMM.
 
-The planner shards ``mx4_matmul`` like ``mm_nd`` / ``grouped_mm``; a contraction is split only into whole blocks.  The reference has no 4-bit
-formats; its float8 products are the nearest thing (autoparallel/graph_passes/async_tp/asynctp_ops.py:363-393).
+The planner shards ``mx4_matmul`` like ``mm_nd`` / ``grouped_mm``; a contraction is split only into whole blocks.  The reference has no
+4-bit formats; its float8 products are the nearest thing (autoparallel/graph_passes/async_tp/asynctp_ops.py:363-393).
 """
 from __future__ import annotations
 
@@ -142,7 +142,8 @@ def _u8(x, *shape):
 _REFS = {"mx4_quantize": _quantize, "mx4_dequantize": _dequantize, "mx4_round": _round, "mx4_mm": _mm, "mx4_linear": _linear,
          "mx4_matmul": _matmul, "mx4_mm_values": _mm_values}
 _META = {
-    "mx4_quantize": lambda x: (_u8(x, *x.shape[:-1], padded(x.shape[-1]) // 2), _u8(x, *x.shape[:-2], *scale_shape(x.shape[-2], x.shape[-1]))),
+    "mx4_quantize": lambda x: (_u8(x, *x.shape[:-1], padded(x.shape[-1]) // 2),
+                               _u8(x, *x.shape[:-2], *scale_shape(x.shape[-2], x.shape[-1]))),
     "mx4_dequantize": lambda codes, scales, k, dtype: codes.new_empty((*codes.shape[:-1], k), dtype=dtype),
     "mx4_round": lambda x, dim: x.new_empty(x.shape),
     "mx4_mm": lambda a, sa, b, sb, dtype: a.new_empty((*a.shape[:-1], b.shape[-2]), dtype=dtype),
@@ -238,9 +239,11 @@ def _are_codes(codes, scales) -> bool:
 
 def _check_codes(name, codes, scales):
     _need(codes.dtype == torch.uint8 and scales.dtype == torch.uint8, f"{name}: codes and scales are uint8")
-    _need(codes.ndim in (2, 3) and codes.shape[-1] % 16 == 0, f"{name}: codes [R, Kp / 2] or [E, R, Kp / 2] of whole blocks, not {tuple(codes.shape)}")
+    _need(codes.ndim in (2, 3) and codes.shape[-1] % 16 == 0,
+          f"{name}: codes [R, Kp / 2] or [E, R, Kp / 2] of whole blocks, not {tuple(codes.shape)}")
     want = (*codes.shape[:-2], *scale_shape(codes.shape[-2], 2 * codes.shape[-1]))
-    _need(tuple(scales.shape) == want, f"{name}: scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)} (expected {want})")
+    _need(tuple(scales.shape) == want,
+          f"{name}: scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)} (expected {want})")
 
 
 def _out_dtype(name, dtype, default):
@@ -285,8 +288,8 @@ def mx4_mm(a, a_scales, b, b_scales, out_dtype: torch.dtype = torch.bfloat16) ->
 
 
 def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``x`` [.., K] (rounded to 4 bits on the way) by weights ``mx4_quantize(w)`` of ``w`` [N, K] -> [.., N]; with weights of experts [E, N, K],
-    ``x`` [E, M, K] -> [E, M, N].  The result has ``x``'s type unless another is asked for."""
+    """``x`` [.., K] (rounded to 4 bits on the way) by weights ``mx4_quantize(w)`` of ``w`` [N, K] -> [.., N]; with weights of experts
+    [E, N, K], ``x`` [E, M, K] -> [E, M, N].  The result has ``x``'s type unless another is asked for."""
     dtype = out_dtype or x.dtype
     xs, cs = x.shape, codes.shape
     # (one test for the calls that are right: this is the path of single tokens)
@@ -295,13 +298,16 @@ def mx4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_d
         _check_float("mx4_linear", x=x)
         _check_codes("mx4_linear", codes, scales)
         _need(x.ndim >= 1 and padded(xs[-1]) == 2 * cs[-1], f"mx4_linear: x {tuple(xs)} and codes {tuple(cs)} do not multiply")
-        _need(codes.ndim == 2 or (x.ndim == 3 and xs[0] == cs[0]), f"mx4_linear: weights of {cs[0]} experts take x [E, M, K], not {tuple(xs)}")
+        _need(codes.ndim == 2 or (x.ndim == 3 and xs[0] == cs[0]),
+              f"mx4_linear: weights of {cs[0]} experts take x [E, M, K], not {tuple(xs)}")
         _out_dtype("mx4_linear", dtype, None)
     return ops.mx4_linear(x, codes, scales, dtype)
 
 
-def mx4_mm_values(a: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, k: int | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``a`` [.., N] by the values [N, k] that codes and scales stand for -> [.., k]; with a stack of codes [E, N, ..], ``a`` [E, M, N] -> [E, M, k]."""
+def mx4_mm_values(a: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, k: int | None = None,
+                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``a`` [.., N] by the values [N, k] that codes and scales stand for -> [.., k]; with a stack of codes [E, N, ..], ``a``
+    [E, M, N] -> [E, M, k]."""
     _check_float("mx4_mm_values", a=a)
     _check_codes("mx4_mm_values", codes, scales)
     k = 2 * codes.shape[-1] if k is None else k

@@ -252,8 +252,9 @@ def _grouped_mm_wgrad(ctx):
     return expand_rows(ctx, [(S(0), S(0), S(0)), (P, S(1), S(1)), (S(1), S(2), R), (S(2), R, S(2))])
 
 
-# ---- routing and MXFP4 products (ops/moe_ops.py, ops/mx4_ops.py).  A 4-bit matrix is split where the pieces are matrices of the same layout by
-# themselves: rows and columns in whole scale tiles of 128, and the blocked dim of 16-bit operands in whole blocks of 32, which are rounded one by one.
+# ---- routing and MXFP4 products (ops/moe_ops.py, ops/mx4_ops.py).  A 4-bit matrix is split where the pieces are matrices of the same layout
+# by themselves: rows and columns in whole scale tiles of 128, and the blocked dim of 16-bit operands in whole blocks of 32, which are rounded
+# one by one.
 def _splits(ctx, extent, unit):
     return extent % (unit * ctx.mesh.size()) == 0
 

@@ -1,5 +1,5 @@
-"""Routing to experts on the CPU: the operator's formula against a plain one in 64 bits, its gradient against differences, ties, masks, refusals, the
-sharding rules and the MoE model's options."""
+"""Routing to experts on the CPU: the operator's formula against a plain one in 64 bits, its gradient against differences, ties, masks,
+refusals, the sharding rules and the MoE model's options."""
 import pytest
 import torch
 
@@ -28,7 +28,8 @@ def plain(x, top_k, score="softmax", bias=None, num_groups=1, top_groups=1, reno
 
 CASES = [
     dict(top_k=2), dict(top_k=1), dict(top_k=8, renormalize=False, scale=2.5), dict(top_k=5, score="sigmoid"),
-    dict(top_k=5, score="sigmoid", renormalize=False), dict(top_k=4, num_groups=4, top_groups=2), dict(top_k=6, score="sigmoid", num_groups=4, top_groups=2),
+    dict(top_k=5, score="sigmoid", renormalize=False), dict(top_k=4, num_groups=4, top_groups=2),
+    dict(top_k=6, score="sigmoid", num_groups=4, top_groups=2),
     dict(top_k=3, score="sigmoid", num_groups=16, top_groups=5, scale=0.5), dict(top_k=16),
 ]
 
@@ -63,7 +64,8 @@ def test_gradient_is_the_formulas(how):
         return (p * how.get("scale", 1.0) * dw.double()).sum(-1)
 
     z, h = x.double(), 1e-5
-    ref = torch.stack([(value(z + h * torch.eye(16).double()[e]) - value(z - h * torch.eye(16).double()[e])) / (2 * h) for e in range(16)], -1)
+    unit = torch.eye(16).double()
+    ref = torch.stack([(value(z + h * unit[e]) - value(z - h * unit[e])) / (2 * h) for e in range(16)], -1)
     assert torch.allclose(dx.double(), ref, rtol=1e-4, atol=1e-6)
 
 
@@ -79,7 +81,8 @@ def test_ties_go_to_the_lower_index():
 
 def test_masked_experts():
     low = torch.finfo(torch.bfloat16).min
-    x = torch.tensor([[-torch.inf] * 6, [-torch.inf, 1.0, -torch.inf, 2.0, -torch.inf, -torch.inf], [low] * 5 + [0.0], [low] * 6]).bfloat16()
+    x = torch.tensor([[-torch.inf] * 6, [-torch.inf, 1.0, -torch.inf, 2.0, -torch.inf, -torch.inf], [low] * 5 + [0.0],
+                      [low] * 6]).bfloat16()
     for renormalize in (True, False):
         xg = x.float().requires_grad_()
         w, idx = K.moe_route(xg, 3, renormalize=renormalize)
@@ -132,7 +135,8 @@ def test_refusals(bad):
 def test_meta_shapes():
     w, idx = torch.ops.apb200.moe_route(torch.empty(5, 7, 16, device="meta"), None, 3, False, 1, 1, True, 1.0)
     assert w.shape == idx.shape == (5, 7, 3) and w.dtype == torch.float32 and idx.dtype == torch.long
-    assert torch.ops.apb200.moe_route_bwd(w, torch.empty(5, 7, 16, device="meta", dtype=torch.bfloat16), idx, False, True, 1.0).dtype == torch.bfloat16
+    assert torch.ops.apb200.moe_route_bwd(w, torch.empty(5, 7, 16, device="meta", dtype=torch.bfloat16), idx, False, True,
+                                          1.0).dtype == torch.bfloat16
 
 
 def test_softmax_option_of_the_model_matches_its_own_formula():

@@ -55,7 +55,8 @@ def logits(T, E, dtype, seed=0, spread=1.5):
     return (spread * torch.randn(T, E, device="cuda", generator=torch.Generator("cuda").manual_seed(seed))).to(dtype)
 
 
-@pytest.mark.parametrize("E,k", [(1, 1), (2, 2), (3, 1), (8, 2), (31, 4), (32, 8), (33, 5), (60, 6), (64, 8), (65, 9), (128, 6), (128, 16), (130, 3),
+@pytest.mark.parametrize("E,k", [(1, 1), (2, 2), (3, 1), (8, 2), (31, 4), (32, 8), (33, 5), (60, 6), (64, 8), (65, 9), (128, 6),
+                                 (128, 16), (130, 3),
                                  (160, 17), (256, 8), (257, 8), (512, 32), (1000, 10), (1024, 32)])
 @pytest.mark.parametrize("T", [1, 2, 37, 1000])
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -68,8 +69,10 @@ def test_sizes(T, E, k, dtype):
             check(x, k, score, bias, renormalize=renormalize, scale=2.5)
 
 
-@pytest.mark.parametrize("E,groups,top_groups,k", [(256, 8, 4, 8), (256, 8, 1, 8), (64, 8, 3, 6), (64, 64, 10, 8), (60, 4, 2, 5), (160, 8, 3, 6),
-                                                   (16, 4, 2, 4), (240, 5, 2, 8), (1024, 64, 4, 16), (1000, 10, 5, 32), (48, 3, 2, 8), (40, 2, 2, 10)])
+@pytest.mark.parametrize("E,groups,top_groups,k", [(256, 8, 4, 8), (256, 8, 1, 8), (64, 8, 3, 6), (64, 64, 10, 8), (60, 4, 2, 5),
+                                                   (160, 8, 3, 6),
+                                                   (16, 4, 2, 4), (240, 5, 2, 8), (1024, 64, 4, 16), (1000, 10, 5, 32), (48, 3, 2, 8),
+                                                   (40, 2, 2, 10)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_groups(E, groups, top_groups, k, score, dtype):
@@ -118,7 +121,8 @@ def test_masks_and_infinities():
 
 def test_strides_offsets_and_leading_dims():
     base = logits(130, 200, F32)
-    for x in (base[:, 3:67], base[::2, :64], base.t()[:64, :64], base[1:].reshape(-1)[1:1 + 128 * 64].view(128, 64), base[:, :64].reshape(2, 65, 64)):
+    for x in (base[:, 3:67], base[::2, :64], base.t()[:64, :64], base[1:].reshape(-1)[1:1 + 128 * 64].view(128, 64),
+              base[:, :64].reshape(2, 65, 64)):
         check(x, 8)
         check(x.bfloat16(), 8, "sigmoid", groups=4, top_groups=2)
     w, idx = K.moe_route(torch.zeros(0, 64, device="cuda"), 8)

@@ -86,7 +86,8 @@ def test_products(lead, m, n, k):
     want = plain_round(x) @ plain_round(w).transpose(-1, -2)
     a, b = K.mx4_quantize(x), K.mx4_quantize(w)
     tol = dict(rtol=k * 2.0**-23, atol=k * 2.0**-23 * want.abs().max().item())  # k fp32 additions
-    for y in (K.mx4_mm(*a, *b, out_dtype=torch.float32), K.mx4_linear(x, *b), K.mx4_matmul(x, w), K.mx4_matmul(x, w.transpose(-1, -2).contiguous(), trans_b=False)):
+    for y in (K.mx4_mm(*a, *b, out_dtype=torch.float32), K.mx4_linear(x, *b), K.mx4_matmul(x, w),
+              K.mx4_matmul(x, w.transpose(-1, -2).contiguous(), trans_b=False)):
         assert y.dtype == torch.float32 and torch.allclose(y.double(), want, **tol)
     if not lead:
         y = K.mx4_linear(x.view(1, m, 1, k), *b, out_dtype=torch.bfloat16)
@@ -124,12 +125,14 @@ def test_refusals():
     codes, scales = K.mx4_quantize(w)
     for call in (
         lambda: K.mx4_quantize(x.half()), lambda: K.mx4_quantize(x[0]), lambda: K.mx4_round(x, 0 - 3), lambda: K.mx4_round(x.long()),
-        lambda: K.mx4_dequantize(codes, scales, 100), lambda: K.mx4_dequantize(codes, scales[:, :0]), lambda: K.mx4_dequantize(codes.int(), scales),
+        lambda: K.mx4_dequantize(codes, scales, 100), lambda: K.mx4_dequantize(codes, scales[:, :0]),
+        lambda: K.mx4_dequantize(codes.int(), scales),
         lambda: K.mx4_dequantize(codes, scales, dtype=torch.float16), lambda: K.mx4_linear(x[:, :32], codes, scales),
         lambda: K.mx4_linear(x.double(), codes, scales), lambda: K.mx4_linear(x, codes, scales, out_dtype=torch.float16),
         lambda: K.mx4_linear(x, codes, scales[..., :100]), lambda: K.mx4_linear(x, codes[None], scales[None]),
         lambda: K.mx4_matmul(x, w, trans_b=False), lambda: K.mx4_matmul(x, w[None]), lambda: K.mx4_matmul(x.half(), w.half()),
-        lambda: K.mx4_mm_values(x, codes, scales), lambda: K.mx4_mm_values(x[:, :8], codes, scales, 100), lambda: K.mx4_mm_values(x[:, :8], codes[None], scales[None]),
+        lambda: K.mx4_mm_values(x, codes, scales), lambda: K.mx4_mm_values(x[:, :8], codes, scales, 100),
+        lambda: K.mx4_mm_values(x[:, :8], codes[None], scales[None]),
         lambda: K.mx4_mm(codes, scales, codes[None], scales[None]), lambda: K.mx4_mm(codes, scales, *K.mx4_quantize(w[:, :32])),
     ):
         with pytest.raises(ValueError, match="mx4_"):
@@ -237,7 +240,8 @@ def test_planned_moe_model_with_4_bit_experts(mesh_1d):
     from autoparallel_b200.models.moe import MoETransformer, moe_debug
 
     for mode in ("planner", "local_map"):
-        cfg = moe_debug(expert_mode=mode, expert_format="mx4", router_score="sigmoid", router_groups=4, router_top_groups=2, router_scale=2.5, ep_axis="dp")
+        cfg = moe_debug(expert_mode=mode, expert_format="mx4", router_score="sigmoid", router_groups=4, router_top_groups=2,
+                        router_scale=2.5, ep_axis="dp")
         with torch.device("meta"):
             model = MoETransformer(cfg)
 
@@ -255,7 +259,8 @@ def test_planned_moe_model_with_4_bit_experts(mesh_1d):
 
 
 def test_layer_with_4_bit_experts_follows_the_16_bit_one():
-    """Same weights: the outputs differ by what 4 bits round away (a quarter of a value at most, less on average), the gradients exist and are finite."""
+    """Same weights: the outputs differ by what 4 bits round away (a quarter of a value at most, less on average), the gradients exist
+    and are finite."""
     from autoparallel_b200.models.moe import MoEFFN, moe_debug
 
     torch.manual_seed(0)
@@ -278,6 +283,7 @@ def test_example():
     import sys
 
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    r = subprocess.run([sys.executable, "examples/example_moe_mx4.py", "--steps", "2"], capture_output=True, text=True, timeout=600, cwd=root)
+    r = subprocess.run([sys.executable, "examples/example_moe_mx4.py", "--steps", "2"], capture_output=True, text=True, timeout=600,
+                       cwd=root)
     assert r.returncode == 0, r.stderr[-2000:]
     assert "mx4_matmul" in r.stdout and "served" in r.stdout

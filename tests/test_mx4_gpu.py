@@ -38,13 +38,15 @@ def check_conversions(x):
     assert torch.equal(codes.cpu(), rc) and torch.equal(scales.cpu(), rs)
     for dtype in (BF16, F32):
         y = K.mx4_dequantize(codes, scales, x.shape[-1], dtype)
-        assert y.is_contiguous() and torch.equal(y.cpu().nan_to_num(123.0), ref("mx4_dequantize", rc, rs, x.shape[-1], dtype).nan_to_num(123.0))
+        assert y.is_contiguous() and torch.equal(y.cpu().nan_to_num(123.0),
+                                                 ref("mx4_dequantize", rc, rs, x.shape[-1], dtype).nan_to_num(123.0))
     for dim in (-1, -2):
         y = K.mx4_round(x, dim)
         assert y.dtype == x.dtype and torch.equal(y.cpu().nan_to_num(123.0), ref("mx4_round", x, dim).nan_to_num(123.0))
 
 
-@pytest.mark.parametrize("shape", [(1, 1), (1, 31), (1, 32), (3, 33), (127, 128), (128, 129), (129, 127), (300, 1000), (64, 4096), (1, 8192),
+@pytest.mark.parametrize("shape", [(1, 1), (1, 31), (1, 32), (3, 33), (127, 128), (128, 129), (129, 127), (300, 1000), (64, 4096),
+                                   (1, 8192),
                                    (2, 100, 72), (5, 130, 264), (3, 1, 40)])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_conversions(shape, dtype):
@@ -57,7 +59,8 @@ def test_conversions(shape, dtype):
 def test_conversions_of_views(dtype):
     base = randn(4, 140, 168, dtype=dtype)
     for x in (base[0, 3:, 5:], base[1, :, :96], base[:, ::2, :64], base[:, 1:130, 8:], base[::2], base[2].t()[7:, 4:], base[:, :, ::2],
-              base.permute(1, 0, 2), base.permute(2, 0, 1), base[0].expand(3, 140, 168), base[0, :1].expand(140, 168), base[0, :, :1].expand(140, 168),
+              base.permute(1, 0, 2), base.permute(2, 0, 1), base[0].expand(3, 140, 168), base[0, :1].expand(140, 168),
+              base[0, :, :1].expand(140, 168),
               base.view(-1)[1:1 + 64 * 96].view(64, 96), base.view(-1)[4:4 + 64 * 96].view(64, 96)):
         check_conversions(x)
 
@@ -70,7 +73,8 @@ def test_special_values():
         x[6, :32] = torch.finfo(dtype).max
         x[7] = x[7] * 2.0**-126                  # denormals
         x[8, :32] = 2.0**-127
-        x[9, :16] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 4.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0, -7.9], device="cuda")
+        x[9, :16] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 4.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0, -7.9],
+                                 device="cuda")
         x[9, 16:32] = 0
         check_conversions(x)
         check_conversions(x.t().contiguous().t())
@@ -89,10 +93,13 @@ def check_product(x, w, y, out_dtype):
 
 PRODUCTS = [
     # (experts, M, N, K): one of every kind of tile and tail
-    (0, 1, 1, 1), (0, 1, 128, 32), (0, 5, 7, 33), (0, 32, 129, 2080), (0, 33, 128, 256), (0, 128, 128, 64), (0, 128, 256, 512), (0, 129, 257, 96),
-    (0, 300, 520, 1000), (0, 257, 132, 512), (0, 513, 392, 300), (0, 700, 1000, 777), (0, 999, 1408, 2048), (0, 2048, 2048, 1024), (0, 3000, 1160, 160),
+    (0, 1, 1, 1), (0, 1, 128, 32), (0, 5, 7, 33), (0, 32, 129, 2080), (0, 33, 128, 256), (0, 128, 128, 64), (0, 128, 256, 512),
+    (0, 129, 257, 96),
+    (0, 300, 520, 1000), (0, 257, 132, 512), (0, 513, 392, 300), (0, 700, 1000, 777), (0, 999, 1408, 2048), (0, 2048, 2048, 1024),
+    (0, 3000, 1160, 160),
     (0, 8, 20000, 4500), (0, 1, 20000, 8192), (0, 100, 40000, 600),
-    (3, 130, 264, 160), (2, 257, 129, 2080), (4, 5, 264, 163), (64, 16, 1408, 256), (64, 3, 300, 1056), (5, 1280, 704, 512), (300, 1, 128, 64),
+    (3, 130, 264, 160), (2, 257, 129, 2080), (4, 5, 264, 163), (64, 16, 1408, 256), (64, 3, 300, 1056), (5, 1280, 704, 512),
+    (300, 1, 128, 64),
 ]
 
 
@@ -113,7 +120,8 @@ def test_products(E, M, N, k, out_dtype):
 
 
 @pytest.mark.parametrize("form", [0, 1, 2])
-@pytest.mark.parametrize("E,M,N,k", [(0, 1, 1, 1), (0, 200, 300, 1000), (2, 257, 129, 2080), (0, 600, 640, 512), (3, 100, 1000, 333), (2, 260, 1408, 1280),
+@pytest.mark.parametrize("E,M,N,k", [(0, 1, 1, 1), (0, 200, 300, 1000), (2, 257, 129, 2080), (0, 600, 640, 512), (3, 100, 1000, 333),
+                                     (2, 260, 1408, 1280),
                                      (0, 700, 2064, 300), (0, 256, 6000, 1024), (9, 700, 1760, 1100), (64, 300, 1152, 640)])
 def test_every_tile_shape(kernels, form, E, M, N, k):
     lead = (E,) if E else ()
@@ -126,7 +134,8 @@ def test_every_tile_shape(kernels, form, E, M, N, k):
 @pytest.mark.parametrize("M", [1, 2, 4, 5, 8, 9, 16, 17, 32])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_few_rows(M, dtype):
-    """Rounded in the product's launch or before it, with one slice of K and with several, rounds of the ring, and rows that are no whole vectors."""
+    """Rounded in the product's launch or before it, with one slice of K and with several, rounds of the ring, and rows that are no
+    whole vectors."""
     for N, k in ((256, 64), (4096, 4096), (300, 1003), (40000, 4096), (2000, 14336)):
         base = randn(M, k + 3, seed=M, dtype=dtype)
         w = randn(N, k, seed=5, dtype=BF16)
@@ -166,7 +175,8 @@ def test_broken_blocks_stay_in_their_rows_and_columns():
         assert torch.equal(y.isnan(), bad)
 
 
-@pytest.mark.parametrize("lead,m,n,k,trans_b", [((), 64, 96, 128, True), ((), 37, 40, 72, False), ((), 37, 41, 75, True), ((), 300, 264, 520, False),
+@pytest.mark.parametrize("lead,m,n,k,trans_b", [((), 64, 96, 128, True), ((), 37, 40, 72, False), ((), 37, 41, 75, True),
+                                                ((), 300, 264, 520, False),
                                                 ((3,), 40, 64, 96, False), ((2,), 33, 50, 77, True), ((2, 5), 8, 24, 64, True)])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_gradients(lead, m, n, k, trans_b, dtype):
@@ -202,11 +212,13 @@ def test_gradients(lead, m, n, k, trans_b, dtype):
     assert (dr == 1).all()
 
 
-@pytest.mark.parametrize("E,M,N,k", [(0, 1, 8, 16), (0, 5, 64, 256), (0, 128, 128, 272), (0, 129, 200, 512), (0, 256, 72, 1000), (0, 300, 1408, 2048), (0, 2000, 520, 640),
+@pytest.mark.parametrize("E,M,N,k", [(0, 1, 8, 16), (0, 5, 64, 256), (0, 128, 128, 272), (0, 129, 200, 512), (0, 256, 72, 1000),
+                                     (0, 300, 1408, 2048), (0, 2000, 520, 640),
                                      (3, 40, 136, 96), (64, 160, 264, 512), (2, 513, 640, 1040)])
 @pytest.mark.parametrize("out_dtype", [BF16, F32])
 def test_products_with_the_values_of_codes(kernels, E, M, N, k, out_dtype):
-    """The kernel that turns codes to values on the way (whatever the size), and the operator, against 64 bits; the values themselves bit by bit."""
+    """The kernel that turns codes to values on the way (whatever the size), and the operator, against 64 bits; the values themselves bit by
+    bit."""
     lead = (E,) if E else ()
     a, w = torch.randn(*lead, M, N, device="cuda", dtype=BF16), randn(*lead, N, k, seed=2)
     if M == 5:
@@ -215,7 +227,8 @@ def test_products_with_the_values_of_codes(kernels, E, M, N, k, out_dtype):
     values = K.mx4_dequantize(codes, scales, k, F32).double()
     want = a.double() @ values
     bound = (a.double().abs() @ values.abs()) * (N * 2.0**-24) + (want.abs() * 2.0**-8 if out_dtype == BF16 else 0) + 1e-300
-    for c in (kernels.extension().mx4_mm_values(a, codes, scales, k, out_dtype == F32, True), K.mx4_mm_values(a, codes, scales, k, out_dtype)):
+    for c in (kernels.extension().mx4_mm_values(a, codes, scales, k, out_dtype == F32, True),
+              K.mx4_mm_values(a, codes, scales, k, out_dtype)):
         near = ((c.double() - want).abs() <= bound) | (c == want.to(F32).to(out_dtype))  # (or both beyond the type's range)
         assert c.shape == want.shape and c.dtype == out_dtype and near.all()
     n = min(M, N)
@@ -305,10 +318,14 @@ def test_refusals_of_the_operators():
     x, w = randn(8, 64), randn(8, 64, seed=1)
     a, b = K.mx4_quantize(x), K.mx4_quantize(w)
     for call in (
-        lambda: apb.mx4_quantize(x.half()), lambda: apb.mx4_quantize(x[0]), lambda: apb.mx4_dequantize(*a, 65, F32), lambda: apb.mx4_dequantize(*a, 64, torch.half),
-        lambda: apb.mx4_dequantize(a[0], a[1][..., :256], 64, F32), lambda: apb.mx4_dequantize(a[0], a[1].cpu(), 64, F32), lambda: apb.mx4_round(x, 0),
-        lambda: apb.mx4_mm(*a, *K.mx4_quantize(w[:, :32]), F32), lambda: apb.mx4_mm(*a, b[0][None], b[1][None], F32), lambda: apb.mx4_mm(*a, *b, torch.half),
-        lambda: apb.mx4_linear(x[:, :32], *b, F32), lambda: apb.mx4_linear(x.double(), *b, F32), lambda: apb.mx4_linear(x, b[0].cpu(), b[1].cpu(), F32),
+        lambda: apb.mx4_quantize(x.half()), lambda: apb.mx4_quantize(x[0]), lambda: apb.mx4_dequantize(*a, 65, F32),
+        lambda: apb.mx4_dequantize(*a, 64, torch.half),
+        lambda: apb.mx4_dequantize(a[0], a[1][..., :256], 64, F32), lambda: apb.mx4_dequantize(a[0], a[1].cpu(), 64, F32),
+        lambda: apb.mx4_round(x, 0),
+        lambda: apb.mx4_mm(*a, *K.mx4_quantize(w[:, :32]), F32), lambda: apb.mx4_mm(*a, b[0][None], b[1][None], F32),
+        lambda: apb.mx4_mm(*a, *b, torch.half),
+        lambda: apb.mx4_linear(x[:, :32], *b, F32), lambda: apb.mx4_linear(x.double(), *b, F32),
+        lambda: apb.mx4_linear(x, b[0].cpu(), b[1].cpu(), F32),
         lambda: apb.mx4_matmul(x, w, False, F32), lambda: apb.mx4_matmul(x, w[:, :32], True, F32),
     ):
         with pytest.raises(RuntimeError):
@@ -323,7 +340,8 @@ def test_c_entries_refuse_what_they_cannot_take():
     x, out = torch.zeros(4, 64, device="cuda"), torch.zeros(1 << 16, device="cuda", dtype=torch.uint8)
     p = out.data_ptr()
     quantize, mm, rows = so.apb_mx4_quantize, so.apb_gemm_mx4, so.apb_gemm_mx4_rows
-    q = lambda codes, scales, K_=64: quantize(ptr(x.data_ptr()), ptr(codes), ptr(scales), i64(1), i64(4), i64(K_), i64(0), i64(64), 0, 0, ptr(0))  # noqa: E731
+    q = lambda codes, scales, K_=64: quantize(ptr(x.data_ptr()), ptr(codes), ptr(scales), i64(1), i64(4), i64(K_), i64(0), i64(64), 0, 0,
+                                              ptr(0))  # noqa: E731
     assert q(p, p + 4096) == 0 and q(p + 8, p + 4096) == 3 and q(p, p + 4) == 3 and q(p, p + 4096, -1) == 3
     status = torch.zeros(4, dtype=torch.int32, device="cuda")
 
@@ -331,7 +349,8 @@ def test_c_entries_refuse_what_they_cannot_take():
         return f(ptr(a), ptr(p + 8192), ptr(p + 16384), ptr(p + 20480), ptr(c), i64(1), i64(4), i64(n), i64(kp), *tail)
 
     tail = (1, -1, ptr(status.data_ptr()), 148, ptr(0))
-    assert product(mm, tail) == 0 and product(mm, tail, a=p + 4) == 3 and product(mm, tail, c=p + 32776) == 3 and product(mm, tail, kp=48) == 3
+    assert product(mm, tail) == 0 and product(mm, tail, a=p + 4) == 3 and product(mm, tail, c=p + 32776) == 3
+    assert product(mm, tail, kp=48) == 3
     assert product(mm, tail, n=-1) == 3
     tail = (i64(0), i64(0), 2, 1, 0, ptr(status.data_ptr()), 148, ptr(0))
     assert product(rows, tail) == 0 and product(rows, tail, a=p + 4) == 3
