@@ -5,9 +5,11 @@
 // Bound by reading B once.  B's rows take the 128 rows of the MMA and A's few rows its N, so that a stage brings in 16 KB of B and next to
 // nothing of A.  A cluster of S CTAs takes a slice of K each for one tile of 128 rows of B: with as many CTAs as two to an SM, all of B's bytes that
 // fit the chip's shared memory are on their way as soon as the launch has begun.  The slices' sums meet in shared memory: every CTA sends each other
-// one its share of the rows, and adds up what it gets in the order of the slices - the same result every time.
-// Measured: 1 x 14336 x 4096 from bf16 8.0 us with the weights in L2, 9.9 from memory (31 MB: 3.2 TB/s; a launch with its TMEM, first bytes and last stores is
-// 3 us), 17 x 4096 x 14336 from codes 9.4, 32 x 4096 x 4096 7.1; 64 experts of 1408 x 2048, one row each, from memory 24.6 (4.0 TB/s).
+// one its share of the rows, and adds up what it gets in the order of the slices - the same result every time.  With more tiles than CTAs at once a CTA has
+// several, one after the other: loads, rounding and MMAs go on into the next tile while the last one's sums (two accumulators in turn) are stored.
+// Measured: 1 x 14336 x 4096 from bf16 7.8 us with the weights in L2, 10 from memory (31 MB: 3.1 TB/s; a launch with its TMEM, first bytes and last stores is
+// 3 us), 17 x 4096 x 14336 from codes 9.4, 32 x 4096 x 4096 7.1; 64 experts of 1408 x 2048, one row each, from memory 19 (98 MB: 80 % of the copy rate; 24.6
+// with a CTA for each tile).
 //   warp 0: TMA producer | warp 1: TMEM owner, scale copies, MMAs | warps 2..9: rounding of A, a stage a warp, then the epilogue
 #include <algorithm>
 
@@ -21,7 +23,8 @@ constexpr int MR_SMEM = 112 * 1024;  // two CTAs to an SM
 struct MxRowsParams {
   const void* x;  // values of A (rounded here), or null
   void* C;
-  int M, N, K, n_tiles, num_kb, k_steps, slices, stages, vec, out_fp32;
+  int M, N, K, tiles, n_tiles, num_kb, k_steps, slices, stages, vec, out_fp32;
+  FastDiv div_tiles, div_blocks;  // by the tiles of a matrix, by the k-blocks of a tile
   long long gs, ld;
   uint32_t* status;
 };
@@ -33,7 +36,7 @@ struct MxRowsShape {
   static constexpr int PART = NT * 128 * 4;  // sums of all slices for a CTA's share of the rows
   static constexpr int STAGES = std::min(MR_MAX_STAGES, (MR_SMEM - 1024 - 256 - PART) / STAGE);
   static constexpr int SMEM = 1024 + STAGES * STAGE + PART + 256;
-  static constexpr uint32_t COLS = NT <= 16 ? 32 : 2 * NT;  // TMEM: NT of sums, 16 of scales
+  static constexpr uint32_t COLS = NT <= 16 ? 64 : 128;  // TMEM: sums of two tiles, 16 columns of scales
 };
 
 // Four rows of a stage of A, one warp: a lane has 8 values of each, four lanes a block.
@@ -97,21 +100,27 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_const
   uint8_t* sSc = sA + p.stages * NT * MX_ROW_BYTES;         // [stages] scales of B, of A
   float* part = reinterpret_cast<float*>(sSc + p.stages * 2 * MX_SC_BYTES);  // [slices][NT][rows of this CTA's share]
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(part) + S::PART);
-  uint64_t *full = bars, *empty = bars + MR_MAX_STAGES, *acc_full = bars + 2 * MR_MAX_STAGES, *parts_in = acc_full + 1;
+  uint64_t *full = bars, *empty = bars + MR_MAX_STAGES, *acc_full = bars + 2 * MR_MAX_STAGES, *acc_free = acc_full + 2, *parts_in = acc_free + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(parts_in + 1);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  static_assert((2 * MR_MAX_STAGES + 3) * 8 <= 256, "barrier block");
+  static_assert((2 * MR_MAX_STAGES + 6) * 8 <= 256, "barrier block");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = p.slices > 1 ? (int)cluster_ctarank() : 0, tile_id = blockIdx.x / p.slices;
-  const int grp = tile_id / p.n_tiles, n0 = (tile_id - grp * p.n_tiles) * 128;
+  const int rank = p.slices > 1 ? (int)cluster_ctarank() : 0, first_tile = blockIdx.x / p.slices, tile_step = gridDim.x / p.slices;
   const int kb0 = p.num_kb * rank / p.slices, kb1 = p.num_kb * (rank + 1) / p.slices;
+  auto place = [&](int tile, int& grp, int& n0) {
+    grp = p.div_tiles.div(tile);
+    n0 = (tile - grp * p.n_tiles) * 128;
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], VALUES ? 1 + (p.M + 3) / 4 : 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(acc_full, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_free[b], MR_WARPS);
+    }
     mbar_init(parts_in, p.slices * MR_WARPS);
     *abort_flag = 0;
     mbar_fence_init();
@@ -142,19 +151,27 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_const
   };
   if (warp == 0) {
     if (elect_one()) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, stage = i % p.stages;
-        if (!mbar_wait(&empty[stage], (i / p.stages & 1) ^ 1, abort_flag)) {
-          fail(ST_TIMEOUT_EMPTY);
-          break;
-        }
-        mbar_expect_tx(&full[stage], MX_OP_BYTES + MX_SC_BYTES + (VALUES ? 0 : NT * MX_ROW_BYTES + MX_SC_BYTES));
-        uint8_t* sc = sSc + stage * 2 * MX_SC_BYTES;
-        tma_load_3d(sB + stage * MX_OP_BYTES, &tmB, &full[stage], kb * MX_ROW_BYTES, n0, grp);
-        tma_load_3d(sc, &tmSB, &full[stage], kb * (MX_SC_BYTES / 4), n0 / 128, grp);
-        if (!VALUES) {
-          tma_load_3d(sA + stage * NT * MX_ROW_BYTES, &tmA, &full[stage], kb * MX_ROW_BYTES, 0, grp);
-          tma_load_3d(sc + MX_SC_BYTES, &tmSA, &full[stage], kb * (MX_SC_BYTES / 4), 0, grp);
+      int stage = 0;
+      uint32_t phase = 1;
+      bool ok = true;
+      for (int t = first_tile; t < p.tiles && ok; t += tile_step) {
+        int grp, n0;
+        place(t, grp, n0);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&empty[stage], phase, abort_flag)) {
+            ok = false;
+            fail(ST_TIMEOUT_EMPTY);
+            break;
+          }
+          mbar_expect_tx(&full[stage], MX_OP_BYTES + MX_SC_BYTES + (VALUES ? 0 : NT * MX_ROW_BYTES + MX_SC_BYTES));
+          uint8_t* sc = sSc + stage * 2 * MX_SC_BYTES;
+          tma_load_3d(sB + stage * MX_OP_BYTES, &tmB, &full[stage], kb * MX_ROW_BYTES, n0, grp);
+          tma_load_3d(sc, &tmSB, &full[stage], kb * (MX_SC_BYTES / 4), n0 / 128, grp);
+          if (!VALUES) {
+            tma_load_3d(sA + stage * NT * MX_ROW_BYTES, &tmA, &full[stage], kb * MX_ROW_BYTES, 0, grp);
+            tma_load_3d(sc + MX_SC_BYTES, &tmSA, &full[stage], kb * (MX_SC_BYTES / 4), 0, grp);
+          }
+          if (++stage == p.stages) stage = 0, phase ^= 1;
         }
       }
       let_next_in();
@@ -164,39 +181,107 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_const
       const uint32_t idesc[2] = {make_idesc_mx4(128, NT, 0), make_idesc_mx4(128, NT, 2)};
       const uint64_t b_desc = make_smem_desc(smem_u32(sB), 16, 1024), a_desc = make_smem_desc(smem_u32(sA), 16, 1024);
       const uint64_t sc_desc = make_scale_desc(smem_u32(sSc));
-      const uint32_t sb_tmem = tmem + NT, sa_tmem = sb_tmem + 4 * MX_STAGE_TILES;
+      const uint32_t sb_tmem = tmem + 2 * NT, sa_tmem = sb_tmem + 4 * MX_STAGE_TILES;
+      int stage = 0;
+      uint32_t phase = 0, seq = 0;
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, stage = i % p.stages;
-        if (!mbar_wait(&full[stage], i / p.stages & 1, abort_flag)) {
-          ok = false;
-          fail(ST_TIMEOUT_FULL);
+      for (int t = first_tile; t < p.tiles && ok; t += tile_step, ++seq) {
+        const uint32_t buf = seq & 1u, d_tmem = tmem + buf * NT;
+        if (seq > 1 && !mbar_wait(&acc_free[buf], ((seq >> 1) - 1) & 1u, abort_flag)) {
+          fail(ST_TIMEOUT_TMEM_EMPTY);
           break;
         }
         tc_fence_after();
-        const int steps = min(MX_BK / 64, p.k_steps - kb * (MX_BK / 64));
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&full[stage], phase, abort_flag)) {
+            ok = false;
+            fail(ST_TIMEOUT_FULL);
+            break;
+          }
+          tc_fence_after();
+          const int steps = min(MX_BK / 64, p.k_steps - kb * (MX_BK / 64));
 #pragma unroll
-        for (int a = 0; a < MX_STAGE_TILES; ++a) {
-          tmem_copy_scales(sb_tmem + 4 * a, sc_desc + desc_offset(stage * 2 * MX_SC_BYTES + a * MX_SCALE_TILE));
-          tmem_copy_scales(sa_tmem + 4 * a, sc_desc + desc_offset(stage * 2 * MX_SC_BYTES + MX_SC_BYTES + a * MX_SCALE_TILE));
-        }
+          for (int a = 0; a < MX_STAGE_TILES; ++a) {
+            tmem_copy_scales(sb_tmem + 4 * a, sc_desc + desc_offset(stage * 2 * MX_SC_BYTES + a * MX_SCALE_TILE));
+            tmem_copy_scales(sa_tmem + 4 * a, sc_desc + desc_offset(stage * 2 * MX_SC_BYTES + MX_SC_BYTES + a * MX_SCALE_TILE));
+          }
 #pragma unroll
-        for (int s = 0; s < MX_BK / 64; ++s) {
-          if (s >= steps) break;
-          umma_mx4(tmem, b_desc + desc_offset(stage * MX_OP_BYTES + 32 * s), a_desc + desc_offset(stage * NT * MX_ROW_BYTES + 32 * s), idesc[s & 1],
-                   sb_tmem + 4 * (s / 2), sa_tmem + 4 * (s / 2), i > 0 || s > 0 ? 1u : 0u);
+          for (int s = 0; s < MX_BK / 64; ++s) {
+            if (s >= steps) break;
+            umma_mx4(d_tmem, b_desc + desc_offset(stage * MX_OP_BYTES + 32 * s), a_desc + desc_offset(stage * NT * MX_ROW_BYTES + 32 * s), idesc[s & 1],
+                     sb_tmem + 4 * (s / 2), sa_tmem + 4 * (s / 2), kb > kb0 || s > 0 ? 1u : 0u);
+          }
+          umma_commit(&empty[stage]);
+          if (++stage == p.stages) stage = 0, phase ^= 1;
         }
-        umma_commit(&empty[stage]);
+        if (ok) umma_commit(&acc_full[buf]);
       }
-      if (ok) umma_commit(acc_full);
     }
   } else {
-    const int w = warp - 2;
+    // Epilogue of this CTA's ``seq``-th tile: a warp has 32 rows of B (a TMEM lane quarter) and half of A's rows.
+    const int w = warp - 2, quarter = warp & 3, half = w >> 2, row = quarter * 32 + lane;
+    constexpr int COLS = NT / 2;
+    auto columns = [&](uint32_t buf, auto store) {  // store(row of A, sum)
+#pragma unroll
+      for (int c0 = 0; c0 < COLS; c0 += 8) {
+        if (half * COLS + c0 >= p.M) break;
+        uint32_t r[8];
+        tmem_ld_32x8(tmem + (uint32_t(quarter * 32) << 16) + buf * NT + half * COLS + c0, r);
+        tmem_ld_wait_for8(r);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) store(half * COLS + c0 + c, r[c]);
+      }
+    };
+    auto put = [&](long long at, float v) {
+      if (p.out_fp32) reinterpret_cast<float*>(p.C)[at] = v;
+      else reinterpret_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16(v);
+    };
+    auto epilogue = [&](int seq) {
+      const uint32_t buf = seq & 1;
+      int grp, n0;
+      place(first_tile + seq * tile_step, grp, n0);
+      const bool done = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], seq >> 1 & 1, abort_flag));
+      if (!done) fail(ST_TIMEOUT_TMEM_FULL);
+      tc_fence_after();
+      if (p.slices == 1) {
+        if (!done) return false;
+        const long long at = (long long)grp * p.M * p.N + n0 + row;
+        const bool in = n0 + row < p.N;
+        columns(buf, [&](int m, uint32_t v) {
+          if (in && m < p.M) put(at + (long long)m * p.N, __uint_as_float(v));
+        });
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_free[buf]);
+        return true;
+      }
+      const int share = 128 / p.slices;  // rows of B that a CTA of the cluster adds up
+      if (done) {
+        const uint32_t dst = map_to_cta(part + (rank * NT) * share + row % share, row / share);
+        columns(buf, [&](int m, uint32_t v) { st_cluster_u32(dst + m * share * 4, v); });
+      }
+      __syncwarp();
+      if (lane == 0)
+        for (int s = 0; s < p.slices; ++s) mbar_arrive_cluster(map_to_cta(parts_in, s));
+      const bool got = __all_sync(0xffffffffu, mbar_wait_cluster(parts_in, 0, abort_flag));
+      if (!got) fail(ST_TIMEOUT_TMEM_FULL);
+      if (!got || !done) return false;
+      const int first = n0 + rank * share;
+      for (int i = threadIdx.x - 64; i < p.M * share; i += 32 * MR_WARPS) {
+        const int m = i / share, r = i - m * share;
+        float v = 0.f;
+        for (int s = 0; s < p.slices; ++s) v += part[(s * NT + m) * share + r];
+        if (first + r < p.N) put(((long long)grp * p.M + m) * p.N + first + r, v);
+      }
+      return true;
+    };
+    const int my_tiles = (p.tiles - first_tile + tile_step - 1) / tile_step, per_tile = kb1 - kb0;
+    int read_out = 0;  // tiles
+    bool ok = true;
     if constexpr (VALUES) {
-      const T* x = reinterpret_cast<const T*>(p.x) + grp * p.gs;
       // Units of four rows of a stage.  Every unit of a ring slot belongs to one warp, in every round of the ring: a warp that skipped a round could
       // not tell from a barrier's parity whether the slot is free or two rounds behind.
-      const int groups = (p.M + 3) / 4, units = p.stages * groups, count = kb1 - kb0;
+      const int groups = (p.M + 3) / 4, units = p.stages * groups, count = my_tiles * per_tile;
       struct At {
         int round, unit;
       };
@@ -208,7 +293,12 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_const
         return a;
       };
       auto load = [&](MxRowsUnit<T>& u, const At& a) {
-        if (block_of(a) < count) u.load(p, x, a.unit % groups * 4, (kb0 + block_of(a)) * MX_BK + lane * 8);
+        const int b = block_of(a);
+        if (b >= count) return;
+        const int seq = p.slices > 1 ? 0 : (int)p.div_blocks.div(b);
+        int grp, n0;
+        place(first_tile + seq * tile_step, grp, n0);
+        u.load(p, reinterpret_cast<const T*>(p.x) + grp * p.gs, a.unit % groups * 4, (kb0 + b - seq * per_tile) * MX_BK + lane * 8);
       };
       MxRowsUnit<T> next;
       At at{0, w};
@@ -218,9 +308,14 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_const
         const MxRowsUnit<T> unit = next;
         const At then = after(at);
         if (then.round < rounds) load(next, then);
-        if (block_of(at) < count) {
+        const int b = block_of(at);
+        if (b < count) {
+          // A tile is read out a ring behind its last block.  What this slot waits for is an MMA of the next tile then, whose accumulator was free
+          // before: no warp waits for a tile that another one has still to read out.
+          while (ok && (read_out + 1) * per_tile + p.stages <= b) ok = epilogue(read_out++);
           const int stage = stage_of(at);
-          if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], (at.round & 1) ^ 1, abort_flag))) {
+          if (!ok || !__all_sync(0xffffffffu, mbar_wait(&empty[stage], (at.round & 1) ^ 1, abort_flag))) {
+            ok = false;
             fail(ST_TIMEOUT_EMPTY);
             break;
           }
@@ -232,51 +327,7 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_const
         at = then;
       }
     }
-    // ---- epilogue: a warp has 32 rows of B (a TMEM lane quarter) and half of A's rows
-    const int quarter = warp & 3, half = w >> 2, share = 128 / p.slices;  // share: rows of B that a CTA of the cluster adds up
-    const bool done = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_flag));
-    if (!done) fail(ST_TIMEOUT_TMEM_FULL);
-    tc_fence_after();
-    if (done) {
-      const int row = quarter * 32 + lane, owner = row / share;
-      const uint32_t dst = p.slices > 1 ? map_to_cta(part + (rank * NT) * share + row % share, owner) : smem_u32(part + row);
-      constexpr int COLS = NT / 2;
-#pragma unroll
-      for (int c0 = 0; c0 < COLS; c0 += 8) {
-        if (half * COLS + c0 >= p.M) break;
-        uint32_t r[8];
-        tmem_ld_32x8(tmem + (uint32_t(quarter * 32) << 16) + half * COLS + c0, r);
-        tmem_ld_wait_for8(r);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint32_t at = dst + (half * COLS + c0 + c) * share * 4;
-          if (p.slices > 1) st_cluster_u32(at, r[c]);
-          else asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(r[c]) : "memory");
-        }
-      }
-    }
-    __syncwarp();
-    if (lane == 0) {
-      if (p.slices > 1) {
-        for (int s = 0; s < p.slices; ++s) mbar_arrive_cluster(map_to_cta(parts_in, s));
-      } else {
-        mbar_arrive(parts_in);
-      }
-    }
-    const bool got = __all_sync(0xffffffffu, mbar_wait_cluster(parts_in, 0, abort_flag));
-    if (!got) fail(ST_TIMEOUT_TMEM_FULL);
-    if (got && done) {
-      const int first = n0 + rank * share;
-      for (int i = threadIdx.x - 64; i < p.M * share; i += 32 * MR_WARPS) {
-        const int m = i / share, r = i - m * share;
-        float v = 0.f;
-        for (int s = 0; s < p.slices; ++s) v += part[(s * NT + m) * share + r];
-        if (first + r >= p.N) continue;
-        const long long at = ((long long)grp * p.M + m) * p.N + first + r;
-        if (p.out_fp32) reinterpret_cast<float*>(p.C)[at] = v;
-        else reinterpret_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16(v);
-      }
-    }
+    while (read_out < my_tiles && (ok || p.slices > 1)) ok = epilogue(read_out++) && ok;  // (a cluster waits for all its CTAs' parts)
   }
   tc_fence_before();
   __syncthreads();
@@ -294,6 +345,8 @@ gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_const
 
 using namespace apb;
 
+extern "C" int apb_gemm_get_reserved_sms();
+
 // Slices of K for a product of ``tiles`` tiles of 128 rows of B: as many as are resident at once, each with a stage at least.
 static int mx_rows_slices(long long tiles, int num_kb, long long resident) {
   int s = 1;
@@ -301,17 +354,17 @@ static int mx_rows_slices(long long tiles, int num_kb, long long resident) {
   return s;
 }
 
-// Whether a product with M rows of A is this file's.  us, this kernel / the persistent ones of gemm_mx4.cu (behind a launch that rounds A, where A comes
-// as ``values``):
-//   values, rounded here   1 x 14336 x 4096 8.0 / 12.6, 4 rows 9.0 / 11.9, 8 10.6 / 12.2, 16 14.4 / 12.3; 1 x 4096 x 14336 9.4 / 24.4; 64 experts of 1408 x
-//                          2048 (704 tiles): 1 row 20.4 / 25.9, 4 rows 23.6 / 24.4, 16 41 / 26.  Every CTA rounds all of A's slice, so more rows are
-//                          better rounded once, by a launch before.
-//   codes                  16 x 14336 x 4096 8.6 / 10.1, 32 9.9 / 10.1, 17 x 4096 x 14336 9.4 / 15.3, 32 x 4096 x 4096 7.1 / 9.6; 704 tiles 16 rows 32 / 24:
-//                          a second wave of CTAs pays its start again.
+// Whether a product with M rows of A is this file's.  us, with weights from memory:
+//   codes                  this kernel / the persistent ones of gemm_mx4.cu: 64 experts of 1408 x 2048 2 rows 19.3 / 20.9, 16 rows 20.0 / 21.6, 32 rows 20.4 / 22.1;
+//                          16 of 4096 x 4096 26.5 / 29.0 (8 rows); 128 of 768 x 2048 21.0 / 22.5; 16 x 14336 x 4096 10.9, in L2 8.6 / 10.1; 32 x 40000 x 4096
+//                          21.7 / 25.7; 32 x 128256 x 4096 49.6 / 56.7; in L2 17 x 4096 x 14336 9.4 / 15.3, 32 x 4096 x 4096 7.1 / 9.6
+//   values, rounded here   this kernel / a launch that rounds A and the codes: every CTA rounds all of A's slice, so more rows are better rounded once.  1 x
+//                          14336 x 4096 10.0 / 12.1, 8 rows 12.4 / 12.4, 16 14.4 / 10.1 (in L2); 64 experts 1 row 19.2 / 22.7, 4 rows 19.7 / 23.1, 8 24.5 /
+//                          23.1, 16 34.8 / 23.9; 8 x 40000 x 4096 27.4 / 22.7, 8 x 1024 x 1024 5.5 / 6.3
 extern "C" int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, int values, int num_sms) {
   const long long tiles = G * ((N + 127) / 128);
   if (values) return M <= 4 || (M <= 8 && tiles <= 2 * num_sms);
-  return M <= 32 && tiles <= num_sms;
+  return M <= 32;
 }
 
 // A: values [G, M, K] with unit stride along K (x_type 0: fp32, 1: bf16), or codes (x_type 2) with scales SA; B: codes [G, N, kp / 2], scales SB;
@@ -327,10 +380,13 @@ extern "C" int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, c
   MxRowsParams p{};
   p.x = x_type == 2 ? nullptr : A;
   p.C = C;
-  p.M = (int)M, p.N = (int)N, p.K = (int)K, p.n_tiles = (int)n_tiles;
+  p.M = (int)M, p.N = (int)N, p.K = (int)K, p.tiles = (int)tiles, p.n_tiles = (int)n_tiles;
   p.num_kb = (int)((kp + MX_BK - 1) / MX_BK);
   p.k_steps = (int)((kp + 63) / 64);
-  p.slices = slices > 0 ? slices : mx_rows_slices(tiles, p.num_kb, 2ll * num_sms);
+  const long long resident = 2ll * std::max(1, num_sms - apb_gemm_get_reserved_sms());
+  p.slices = slices > 0 ? slices : mx_rows_slices(tiles, p.num_kb, resident);
+  p.div_tiles = FastDiv((uint32_t)n_tiles);
+  p.div_blocks = FastDiv((uint32_t)p.num_kb);
   if ((p.slices & (p.slices - 1)) || p.slices > 8 || p.slices > p.num_kb || tiles * p.slices >= 1ll << 31) return 3;
   p.out_fp32 = out_fp32;
   p.gs = gs, p.ld = ld;
@@ -355,7 +411,7 @@ extern "C" int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, c
     ++n;
     if (!apb_gemm_makes_room()) attr[n++] = overlap_attribute();
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * p.slices));
+    cfg.gridDim = dim3((unsigned)(p.slices > 1 ? tiles * p.slices : std::min(tiles, resident)));
     cfg.blockDim = dim3(MR_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;

@@ -150,6 +150,20 @@ def test_few_rows(M, dtype):
         check_product(view, w, K.mx4_linear(view, *K.mx4_quantize(w), out_dtype=F32), F32)
 
 
+@pytest.mark.parametrize("M", [1, 3, 4, 8, 16, 32])
+@pytest.mark.parametrize("E,N,k", [(0, 80000, 300), (0, 120000, 64), (64, 1408, 1100), (700, 128, 520), (5, 20010, 96), (300, 260, 4000)])
+def test_few_rows_of_many_tiles(M, E, N, k):
+    """More tiles than CTAs at once: tiles of one k-block, of fewer than a ring has slots, of more; rows that several matrices have."""
+    lead = (E,) if E else ()
+    x, w = randn(*lead, M, k, seed=M), randn(*lead, N, k, seed=5)
+    b = K.mx4_quantize(w)
+    for dtype in (BF16, F32):
+        y = K.mx4_linear(x.to(dtype), *b, out_dtype=F32)
+        check_product(x.to(dtype), w, y, F32)
+        assert torch.equal(y, K.mx4_linear(x.to(dtype), *b, out_dtype=F32))
+    check_product(x, w, K.mx4_mm(*K.mx4_quantize(x), *b), BF16)
+
+
 def test_shapes_of_x():
     w = randn(48, 64, seed=1)
     b = K.mx4_quantize(w)
