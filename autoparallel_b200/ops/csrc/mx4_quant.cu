@@ -8,8 +8,8 @@
 // largest magnitude is an integer maximum of the values' bits, its scale a shift of them, the rounding the hardware's conversion (to nearest, ties to
 // even), a value from its code the bits moved to an exponent and one multiplication.
 // Measured for 64 x 1280 x 2048 bf16 (335 MB of values, 89 MB of codes), share of the copy rate: mx4_quantize 75 us (87 %), 64 x 2048 x 1408 with unit stride
-// along the rows 80 (88 %), mx4_dequantize 75 to 80 (85 to 90 %), mx4_round 107 along K (96 %) and 117 to 128 along the rows.  Rows that are no whole 16
-// bytes (16 x 695 x 1429) take 1.5 to 2 times as long per byte.
+// along the rows 80 (88 %), mx4_dequantize 75 to 80 (85 to 90 %), mx4_round 107 along K (96 %) and 117 to 128 along the rows.  Of 64 x 1279 x
+// 2047, whose rows begin anywhere, hot: 89, 104 and 164 us, where 64 x 1280 x 2048 takes 67, 69 and 101; values of fp32, 16 x 695 x 1429: 16, 20 and 27.
 // Compiled without --use_fast_math: denormals count.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -24,7 +24,7 @@ namespace apb {
 constexpr int MX_THREADS = 256, MX_TILE = 128, MX_FEW_TILES = 4;
 
 struct MxParams {
-  const void* x;
+  const void *x, *x_end;  // (the byte after x's last value)
   uint8_t* codes;
   uint8_t* scales;
   void* y;
@@ -115,12 +115,50 @@ __device__ __forceinline__ void mx_store_codes(const MxParams& p, const MxTile& 
 template <typename T>
 constexpr int mx_pitch() { return MX_TILE * (int)sizeof(T) + 16; }
 
-// A row of the tile between memory and shared memory, a warp, element by element: for rows that begin anywhere.
-template <typename T>
-__device__ __forceinline__ void mx_row_in(T* row, const T* src, int columns, int lane) {
+// 32 bytes of a row that begins anywhere, ``n`` of its values in the matrix: the 16-byte pieces of memory that have them, three at most, moved into place
+// afterwards, so that several rows can be under way.  A piece may have values of the neighbours in memory, but none outside of x as a whole: the first and the last
+// are put together value by value.  INSIDE: neither is among them, and all values are in the matrix.
+template <typename T, bool INSIDE>
+struct MxAnyRow {
+  uint32_t w[12];
+  uint32_t off;  // of the values in the pieces, bytes
+  int n;
+  __device__ __forceinline__ void load(const MxParams& p, const T* src, int count) {
+    n = count;
+    off = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 15);
+    const uint8_t* piece = reinterpret_cast<const uint8_t*>(src) - off;
 #pragma unroll
-  for (int c = 0; c < MX_TILE; c += 32) row[c + lane] = c + lane < columns ? src[c + lane] : T(0.f);
-}
+    for (int q = 0; q < 3; ++q, piece += 16) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (INSIDE || (n > 0 && 16 * q < (int)off + n * (int)sizeof(T))) {
+        if (INSIDE || (piece >= p.x && piece + 16 <= p.x_end)) v = *reinterpret_cast<const uint4*>(piece);
+        else v = ends(p, piece);
+      }
+      w[4 * q] = v.x, w[4 * q + 1] = v.y, w[4 * q + 2] = v.z, w[4 * q + 3] = v.w;
+    }
+  }
+  static __device__ __noinline__ uint4 ends(const MxParams& p, const uint8_t* piece) {
+    uint32_t v[4] = {};
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
+      const T* at = reinterpret_cast<const T*>(piece) + i;
+      if ((const void*)at >= p.x && (const void*)(at + 1) <= p.x_end) mx_put(v, i, *at);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  __device__ __forceinline__ void words(uint32_t (&u)[8]) {
+#pragma unroll
+    for (int i = 0; i < 10; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 9; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+    constexpr int PER_WORD = 4 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      u[i] = PER_WORD == 1 ? w[i] : __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+      if (!INSIDE) u[i] = i * PER_WORD >= n ? 0u : PER_WORD == 2 && i * PER_WORD + 1 >= n ? u[i] & 0xFFFFu : u[i];
+    }
+  }
+};
 template <typename T>
 __device__ __forceinline__ void mx_row_out(T* dst, const T* row, int columns, int lane) {
 #pragma unroll
@@ -128,56 +166,63 @@ __device__ __forceinline__ void mx_row_out(T* dst, const T* row, int columns, in
     if (c + lane < columns) dst[c + lane] = row[c + lane];
 }
 
-// Unit stride along K, rows that are no whole 16 bytes: 32 rows at a time through shared memory, read and written element by element but in whole sectors.
+// Unit stride along K, rows that are no whole 16 bytes.  Rounded values leave through shared memory, element by element but in whole sectors.  (Values that
+// come in that way, too: 124 us for the codes of 64 x 1279 x 2047 bf16, 89 in 16-byte pieces; with the tests of the ends in every load 105.)
 template <typename T, bool ROUND>
 __global__ void __launch_bounds__(MX_THREADS) mx4_rows_any_kernel(MxParams p) {
   after_previous();
-  constexpr int PER = 32 / (int)sizeof(T), ROW_THREADS = MX_TILE / PER, CHUNK = 32;
+  constexpr int PER = 32 / (int)sizeof(T), ROW_THREADS = MX_TILE / PER, PASS = MX_THREADS / ROW_THREADS, ROWS = 2, CHUNK = ROWS * PASS;
   __shared__ __align__(16) uint8_t tile[512];
-  __shared__ __align__(16) uint8_t rows[CHUNK * mx_pitch<T>()];
+  __shared__ __align__(16) uint8_t rows[ROUND ? CHUNK * mx_pitch<T>() : 16];
   uint8_t* scale_tile = nullptr;
   const MxTile at = mx_tile(p, &scale_tile);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kp = (p.K + 31) / 32 * 32, columns = min(MX_TILE, p.K - at.k0);
-  const T* x = reinterpret_cast<const T*>(p.x) + at.g * p.gs + at.k0;
+  const int col = threadIdx.x % ROW_THREADS * PER, k = at.k0 + col, r_first = threadIdx.x / ROW_THREADS;
+  const T* x = reinterpret_cast<const T*>(p.x) + at.g * p.gs + k;
   T* y = reinterpret_cast<T*>(p.y) + at.g * p.R * (long long)p.K + at.k0;
-  auto row = [&](int r) { return reinterpret_cast<T*>(rows + r * mx_pitch<T>()); };
-  for (int r0 = 0; r0 < MX_TILE; r0 += CHUNK) {
-    if (at.r0 + r0 < p.R) {
+  auto run = [&](auto inside) {
+#pragma unroll 1
+    for (int r0 = 0; r0 < MX_TILE; r0 += CHUNK) {
+      MxAnyRow<T, decltype(inside)::value> in[ROWS];
 #pragma unroll
-      for (int i = 0; i < CHUNK / 8; ++i) {
-        const int r = at.r0 + r0 + warp + 8 * i;
-        mx_row_in(row(warp + 8 * i), x + r * p.ld, r < p.R ? columns : 0, lane);
+      for (int i = 0; i < ROWS; ++i) {
+        const int r = at.r0 + r0 + r_first + PASS * i;
+        in[i].load(p, x + r * p.ld, r < p.R ? min(PER, p.K - k) : 0);
       }
-    }
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < CHUNK * ROW_THREADS / MX_THREADS; ++i) {
-      const int rr = i * (MX_THREADS / ROW_THREADS) + threadIdx.x / ROW_THREADS, col = threadIdx.x % ROW_THREADS * PER;
-      const int r = at.r0 + r0 + rr, k = at.k0 + col;
-      uint4* own = reinterpret_cast<uint4*>(rows + rr * mx_pitch<T>() + col * sizeof(T));
-      uint32_t u[8], packed[PER / 8];
-      const uint4 a = own[0], b = own[1];
-      u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w, u[4] = b.x, u[5] = b.y, u[6] = b.z, u[7] = b.w;
-      const uint32_t code = mx_round_32<T, ROUND>(u, packed);
+      for (int i = 0; i < ROWS; ++i) {
+        const int rr = r0 + r_first + PASS * i, r = at.r0 + rr;
+        uint32_t u[8], packed[PER / 8];
+        in[i].words(u);
+        const uint32_t code = mx_round_32<T, ROUND>(u, packed);
+        if (ROUND) {
+          uint4* own = reinterpret_cast<uint4*>(rows + (rr - r0) * mx_pitch<T>() + col * sizeof(T));
+          own[0] = make_uint4(u[0], u[1], u[2], u[3]);
+          own[1] = make_uint4(u[4], u[5], u[6], u[7]);
+        } else {
+          mx_store_codes<PER>(p, at, r, k, kp, packed);
+          if (col % 32 == 0) tile[mx_scale_at(rr, col / 32)] = (uint8_t)(r < p.R && k < kp ? code : 127u);
+        }
+      }
       if (ROUND) {
-        own[0] = make_uint4(u[0], u[1], u[2], u[3]);
-        own[1] = make_uint4(u[4], u[5], u[6], u[7]);
-      } else {
-        mx_store_codes<PER>(p, at, r, k, kp, packed);
-        if (col % 32 == 0) tile[mx_scale_at(r0 + rr, col / 32)] = (uint8_t)(r < p.R && k < kp ? code : 127u);
-      }
-    }
-    __syncthreads();
-    if (ROUND) {
+        __syncthreads();
 #pragma unroll
-      for (int i = 0; i < CHUNK / 8; ++i) {
-        const int r = at.r0 + r0 + warp + 8 * i;
-        if (r < p.R) mx_row_out(y + (long long)r * p.K, row(warp + 8 * i), columns, lane);
+        for (int i = 0; i < CHUNK / 8; ++i) {
+          const int rr = warp + 8 * i, r = at.r0 + r0 + rr;
+          if (r < p.R) mx_row_out(y + (long long)r * p.K, reinterpret_cast<const T*>(rows + rr * mx_pitch<T>()), columns, lane);
+        }
+        __syncthreads();
       }
-      __syncthreads();
     }
+  };
+  const uint8_t* first = reinterpret_cast<const uint8_t*>(x - col + at.r0 * p.ld);
+  const uint8_t* end = reinterpret_cast<const uint8_t*>(x - col + (at.r0 + MX_TILE - 1) * p.ld + MX_TILE);
+  if (at.r0 + MX_TILE <= p.R && at.k0 + MX_TILE <= p.K && first - 15 >= p.x && end + 31 <= p.x_end) run(std::true_type{});
+  else run(std::false_type{});
+  if (!ROUND) {
+    __syncthreads();
+    if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(scale_tile)[threadIdx.x] = reinterpret_cast<const uint32_t*>(tile)[threadIdx.x];
   }
-  if (!ROUND && threadIdx.x < 128) reinterpret_cast<uint32_t*>(scale_tile)[threadIdx.x] = reinterpret_cast<const uint32_t*>(tile)[threadIdx.x];
 }
 
 // Unit stride along K, rows of whole 16 bytes.  A thread has 32 bytes of a row (16 bf16 or 8 fp32), two or four threads a block; the loads of four rows are
@@ -483,6 +528,7 @@ static int mx_from_values(MxParams& p, unsigned grid, int transposed, int is_bf1
       return p.ld * esz % bytes == 0 && p.gs * esz % bytes == 0 && (long long)p.K * esz % bytes == 0 && aligned(p.x, bytes) && (!ROUND || aligned(p.y, bytes));
     };
     p.vec = whole(32) ? 2 : whole(16) ? 1 : 0;
+    p.x_end = reinterpret_cast<const uint8_t*>(p.x) + ((p.G - 1) * p.gs + (p.R - 1) * p.ld + p.K) * esz;
     if (!ROUND && p.vec && p.R <= MX_THREADS * (32 / esz) / MX_TILE) {
       const unsigned few = (unsigned)(p.G * ((p.k_tiles + MX_FEW_TILES - 1) / MX_FEW_TILES));
       is_bf16 ? launch_after(mx4_few_rows_kernel<__nv_bfloat16>, few, MX_THREADS, 0, st, p) : launch_after(mx4_few_rows_kernel<float>, few, MX_THREADS, 0, st, p);
