@@ -42,8 +42,62 @@ struct MxGemmParams {
 };
 enum : int { MX_SCALAR = 0, MX_STAGED = 1, MX_DIRECT = 2 };
 
+// 32 rows of 128 bytes from shared memory (16-byte units swizzled by the row) to rows that begin anywhere, of which ``rows`` and ``lim`` columns are in the
+// matrix: a word a lane.  A bf16 row that begins in the middle of a word of memory has words of the second half of a lane's and the first of the next one's, and its
+// first and last value by themselves; rows of an odd stride begin there every other time, so the even and the odd ones go by themselves, with the same
+// addresses and conditions in all of them: two warps a scheduler wait for their own instructions here, and every one counts.  64 x 1280 x 1407 x 2048 133
+// us this way (1408: 110), 175 with the conditions worked out in each row, 418 element by element; fp32 176, 182, 610 (141).
+__device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void mx_rows_anywhere(uint8_t* dst, long long step, const uint8_t* stg, int rows, int lim, bool fp32, int lane) {
+  if (fp32) {
+    const uint32_t from = smem_u32(stg) + lane * 4;
+    uint8_t* at = dst + 4 * lane;
+    if (lane >= lim) rows = 0;
+#pragma unroll 1
+    for (int b = 0; b < 32; b += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = ld_shared((from ^ (j << 4)) + (b + j) * 128);
+#pragma unroll
+      for (int j = 0; j < 8; ++j, at += step)
+        if (b + j < rows) *reinterpret_cast<uint32_t*>(at) = w[j];
+    }
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c, dst += step) {
+      const uint32_t from = smem_u32(stg) + c * 128 + ((((lane >> 2) ^ c) << 4) | (lane & 3) * 4);
+      const bool odd = (reinterpret_cast<uintptr_t>(dst) & 2) != 0;  // (in all lanes)
+      const int e = 2 * lane + odd;                                  // first value of the lane's word
+      const bool word = e + 1 < lim, tail = e + 1 == lim, head = odd && lane == 0;
+      uint8_t* at = dst + 2 * e;
+#pragma unroll 1
+      for (int b = 0; b < 32; b += 8) {
+        uint32_t w[4], own[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = own[j] = ld_shared((from ^ (j << 5)) + (b + 2 * j) * 128);
+        if (odd) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(own[j], __shfl_down_sync(0xffffffffu, own[j], 1), 16);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j, at += 2 * step) {
+          const bool in = b + 2 * j + c < rows;
+          if (in && word) *reinterpret_cast<uint32_t*>(at) = w[j];
+          if (in && tail) *reinterpret_cast<uint16_t*>(at) = (uint16_t)w[j];
+          if (in && head) *reinterpret_cast<uint16_t*>(at - 2) = (uint16_t)own[j];
+        }
+      }
+    }
+  }
+  __syncwarp();  // (together to the next load from TMEM)
+}
+
 // The epilogue where rows are no whole sectors (mx_store_direct where they are), 64 columns at a time: through shared memory in 16-byte pieces of whole
-// 128-byte lines, or element by element.  64 x 1280 x 1408 x 256 66 us this way, 55 straight from registers.
+// 128-byte lines, or word by word.  64 x 1280 x 1408 x 256 66 us this way, 55 straight from registers.
 template <typename Release>
 __device__ __forceinline__ void mx_store_staged(const MxGemmParams& q, uint8_t* C, uint8_t* stg, uint32_t taddr, int row0, int n0, int ncols, bool down,
                                                 int lane, Release release) {
@@ -89,15 +143,8 @@ __device__ __forceinline__ void mx_store_staged(const MxGemmParams& q, uint8_t* 
           const uint4 x = *reinterpret_cast<const uint4*>(stg + row * 128 + ((unit ^ (row & 7)) << 4));
           if (col < p.N && row0 + row < p.M) *reinterpret_cast<uint4*>(C + ((row0 + row) * p.ldc + col) * esz) = x;
         }
-      } else {  // rows that are no whole vectors: element by element, a row at a time
-        for (int row = 0; row < 32 && row0 + row < p.M; ++row)
-          for (int e = lane; e < 128 / esz; e += 32) {
-            const uint8_t* src = stg + row * 128 + (((e * esz / 16) ^ (row & 7)) << 4) + e * esz % 16;
-            if (col0 + e >= p.N) continue;
-            uint8_t* dst = C + ((row0 + row) * p.ldc + col0 + e) * esz;
-            if (p.out_fp32) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
-            else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
-          }
+      } else {
+        mx_rows_anywhere(C + (row0 * p.ldc + col0) * esz, p.ldc * esz, stg, min(32, p.M - row0), min(128 / esz, p.N - col0), p.out_fp32, lane);
       }
     }
   }

@@ -122,7 +122,8 @@ def test_products(E, M, N, k, out_dtype):
 @pytest.mark.parametrize("form", [0, 1, 2])
 @pytest.mark.parametrize("E,M,N,k", [(0, 1, 1, 1), (0, 200, 300, 1000), (2, 257, 129, 2080), (0, 600, 640, 512), (3, 100, 1000, 333),
                                      (2, 260, 1408, 1280),
-                                     (0, 700, 2064, 300), (0, 256, 6000, 1024), (9, 700, 1760, 1100), (64, 300, 1152, 640)])
+                                     (0, 700, 2064, 300), (0, 256, 6000, 1024), (9, 700, 1760, 1100), (64, 300, 1152, 640),
+                                     (2, 260, 1407, 300), (3, 131, 390, 256), (0, 513, 131, 512), (5, 97, 641, 96), (0, 2050, 66, 64)])
 def test_every_tile_shape(kernels, form, E, M, N, k):
     lead = (E,) if E else ()
     x, w = randn(*lead, M, k, seed=3), randn(*lead, N, k, seed=4)
