@@ -117,8 +117,8 @@ constexpr int mx_pitch() { return MX_TILE * (int)sizeof(T) + 16; }
 
 // 32 bytes of a row that begins anywhere, ``n`` of its values in the matrix: the 16-byte pieces of memory that have them, three at most, moved into place
 // afterwards, so that several rows can be under way.  A piece may have values of the neighbours in memory, but none outside of x as a whole: the first and the last
-// are put together value by value.  INSIDE: neither is among them, and all values are in the matrix.
-template <typename T, bool INSIDE>
+// are put together value by value.  INSIDE: neither is among them; FULL: and all values are in the matrix.
+template <typename T, bool INSIDE, bool FULL>
 struct MxAnyRow {
   uint32_t w[12];
   uint32_t off;  // of the values in the pieces, bytes
@@ -130,7 +130,7 @@ struct MxAnyRow {
 #pragma unroll
     for (int q = 0; q < 3; ++q, piece += 16) {
       uint4 v = make_uint4(0, 0, 0, 0);
-      if (INSIDE || (n > 0 && 16 * q < (int)off + n * (int)sizeof(T))) {
+      if (FULL || (n > 0 && 16 * q < (int)off + n * (int)sizeof(T))) {
         if (INSIDE || (piece >= p.x && piece + 16 <= p.x_end)) v = *reinterpret_cast<const uint4*>(piece);
         else v = ends(p, piece);
       }
@@ -155,7 +155,7 @@ struct MxAnyRow {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       u[i] = PER_WORD == 1 ? w[i] : __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
-      if (!INSIDE) u[i] = i * PER_WORD >= n ? 0u : PER_WORD == 2 && i * PER_WORD + 1 >= n ? u[i] & 0xFFFFu : u[i];
+      if (!FULL) u[i] = i * PER_WORD >= n ? 0u : PER_WORD == 2 && i * PER_WORD + 1 >= n ? u[i] & 0xFFFFu : u[i];
     }
   }
 };
@@ -180,10 +180,10 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_any_kernel(MxParams p) {
   const int col = threadIdx.x % ROW_THREADS * PER, k = at.k0 + col, r_first = threadIdx.x / ROW_THREADS;
   const T* x = reinterpret_cast<const T*>(p.x) + at.g * p.gs + k;
   T* y = reinterpret_cast<T*>(p.y) + at.g * p.R * (long long)p.K + at.k0;
-  auto run = [&](auto inside) {
+  auto run = [&](auto inside, auto full) {
 #pragma unroll 1
     for (int r0 = 0; r0 < MX_TILE; r0 += CHUNK) {
-      MxAnyRow<T, decltype(inside)::value> in[ROWS];
+      MxAnyRow<T, decltype(inside)::value, decltype(full)::value> in[ROWS];
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int r = at.r0 + r0 + r_first + PASS * i;
@@ -216,9 +216,11 @@ __global__ void __launch_bounds__(MX_THREADS) mx4_rows_any_kernel(MxParams p) {
     }
   };
   const uint8_t* first = reinterpret_cast<const uint8_t*>(x - col + at.r0 * p.ld);
-  const uint8_t* end = reinterpret_cast<const uint8_t*>(x - col + (at.r0 + MX_TILE - 1) * p.ld + MX_TILE);
-  if (at.r0 + MX_TILE <= p.R && at.k0 + MX_TILE <= p.K && first - 15 >= p.x && end + 31 <= p.x_end) run(std::true_type{});
-  else run(std::false_type{});
+  const uint8_t* end = reinterpret_cast<const uint8_t*>(x - col + (min(at.r0 + MX_TILE, p.R) - 1) * p.ld + MX_TILE);
+  const bool inside = first - 15 >= p.x && end + 31 <= p.x_end;
+  if (inside && at.r0 + MX_TILE <= p.R && at.k0 + MX_TILE <= p.K) run(std::true_type{}, std::true_type{});
+  else if (inside) run(std::true_type{}, std::false_type{});
+  else run(std::false_type{}, std::false_type{});
   if (!ROUND) {
     __syncthreads();
     if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(scale_tile)[threadIdx.x] = reinterpret_cast<const uint32_t*>(tile)[threadIdx.x];
