@@ -1057,8 +1057,8 @@ Tensor op_mx4_mm_values(const Tensor& a, const Tensor& codes, const Tensor& scal
     auto c = mx4_mm_values(a, codes, scales, k, dtype);
     if (c.has_value()) return *c;
     if (a.scalar_type() == at::kBFloat16 && a.size(-1) % 8 == 0 && a.size(-1) > 0 && !native().diag_library_gemm) {
-      // the values as a matrix of their own (whole blocks: rows of whole 16 bytes), and the 16-bit product
-      Tensor w = mx4_dequantize(codes, scales, 2 * codes.size(-1), at::kBFloat16);
+      // the values as a matrix of their own (rows of whole 16 bytes), and the 16-bit product
+      Tensor w = mx4_dequantize(codes, scales, (k + 7) / 8 * 8, at::kBFloat16);
       if (w.dim() == 2) {
         c = mm_nd(a, w, false, dtype == at::kFloat, status_of(a));
       } else {

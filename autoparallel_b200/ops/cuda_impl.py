@@ -351,8 +351,8 @@ def _mx4_mm_values(a, codes, scales, k, out_dtype):
     c = _C.mx4_mm_values(a, codes, scales, k, _fp32_result("mx4_mm_values", out_dtype), False)
     if c is not None:
         return c
-    # the values as a matrix of their own (whole blocks, and rows and columns of whole 16 bytes), and the 16-bit product
-    w = _C.mx4_dequantize(codes, scales, 2 * codes.shape[-1], a.dtype is torch.float32)
+    # the values as a matrix of their own (rows and columns of whole 16 bytes), and the 16-bit product
+    w = _C.mx4_dequantize(codes, scales, -(-k // 8) * 8, a.dtype is torch.float32)
     extra = -a.shape[-1] % 8
     if extra:
         a, w = torch.nn.functional.pad(a, (0, extra)), torch.nn.functional.pad(w, (0, 0, 0, extra))
