@@ -842,7 +842,7 @@ Two moe_route(const Tensor& logits_, const c10::optional<Tensor>& bias, int64_t 
   if (bias.has_value()) {
     TORCH_CHECK(bias->is_cuda() && bias->device() == logits.device() && bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == E,
                 "moe_route: bias is fp32 [experts] on the logits' device");
-    b = bias->contiguous();
+    b = dense(*bias);  // (the kernel reads it in 16-byte pieces)
   }
   auto shape = logits.sizes().vec();
   shape.back() = k;

@@ -483,12 +483,12 @@ static dim3 route_grid(long long tokens) {
 
 using namespace apb;
 
-// logits [tokens, E] (bf16 or fp32, rows after each other, 16-byte base), bias fp32 [E] or null -> w fp32 [tokens, k], idx [tokens, k].
+// logits [tokens, E] (bf16 or fp32, rows after each other, 16-byte base), bias fp32 [E] (16-byte base) or null -> w fp32 [tokens, k], idx [tokens, k].
 // Returns 0, or an argument / launch error (nothing launched).
 extern "C" int apb_moe_route(const void* logits, const float* bias, float* w, long long* idx, long long tokens, int E, int k, int sigmoid, int groups,
                              int top_groups, int renorm, float scale, int is_bf16, cudaStream_t st) {
   if (!route_args_ok(tokens, E, k) || groups < 1 || groups > ROUTE_MAX_GROUPS || E % groups || top_groups < 1 || top_groups > groups ||
-      k > top_groups * (E / groups) || (reinterpret_cast<uintptr_t>(logits) & 15))
+      k > top_groups * (E / groups) || ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(bias)) & 15))
     return 3;
   if (tokens == 0) return 0;
   uint32_t mask = 1;

@@ -1,4 +1,6 @@
 """The routing kernels against the formula of ops/moe_ops.py, evaluated by torch on the same device, and in 64 bits."""
+import ctypes
+
 import pytest
 import torch
 
@@ -160,3 +162,34 @@ def test_refusals_of_the_operator():
     # a number that names no expert has no gradient, and touches nothing
     idx[0, 0], idx[1, 0] = 64, -1
     assert torch.isfinite(apb.moe_route_bwd(w, x, idx, False, True, 1.0)).all()
+
+
+def test_a_bias_that_begins_anywhere():
+    """One layer's part of a flat buffer: dense, four bytes off the alignment that the kernel's 16-byte loads need."""
+    g = torch.Generator("cuda").manual_seed(2)
+    flat = 0.1 * torch.randn(2100, device="cuda", generator=g)
+    for E in (60, 64, 256, 1024):
+        for dtype in (BF16, F32):
+            x = logits(300, E, dtype)
+            for first in (1, 2, 3, 4):
+                for score in ("softmax", "sigmoid"):
+                    check(x, 5, score, flat[first : first + E])
+            check(x, 5, "sigmoid", flat[: 2 * E : 2])
+
+
+def test_the_c_entry_refuses_what_it_cannot_take():
+    from autoparallel_b200.ops import build
+
+    route, i64, ptr = ctypes.CDLL(build.so_path()).apb_moe_route, ctypes.c_longlong, ctypes.c_void_p
+    x, bias = torch.zeros(8, 64, device="cuda"), torch.zeros(128, device="cuda")
+    w, idx = torch.full((4, 8), 7.0, device="cuda"), torch.full((4, 8), -7, device="cuda")
+
+    def call(x_bytes=0, bias_bytes=0, E=64, k=8):
+        return route(ptr(x.data_ptr() + x_bytes), ptr(bias.data_ptr() + bias_bytes), ptr(w.data_ptr()), ptr(idx.data_ptr()), i64(4), E, k, 1, 1, 1, 1,
+                     ctypes.c_float(1.0), 0, ptr(0))
+
+    assert call(x_bytes=4) == 3 and call(bias_bytes=4) == 3 and call(bias_bytes=8) == 3 and call(k=33) == 3 and call(E=1025) == 3
+    assert (w == 7).all() and (idx == -7).all()  # nothing ran
+    assert call(bias_bytes=16) == 0
+    torch.cuda.synchronize()
+    assert (w == 0.125).all() and (idx == torch.arange(8, device="cuda")).all()
