@@ -3,8 +3,8 @@
 //
 // L lanes have a token, V experts each, all in registers; the k best are found by k rounds of "largest, lowest index first".  That takes instructions, and
 // they are the bound, not memory (131072 x 128: 67 % of the issue slots, 13 % of DRAM; backward 52 and 26), so a token has the fewest lanes that hold it.
-//   forward   8192 x 64 bf16, 8 of softmax: 3.0 us, 131072 x 64: 16.7, 131072 x 128, 6: 27.4 (1.5 TB/s); 16383 x 256 fp32 sigmoid, 8 of the 4 best of 8
-//             groups: 22.0, 65536 x 256 bf16 the same way: 53.5, without groups and sigmoid 25.6
+//   forward   8192 x 64 bf16, 8 of softmax: 2.6 us, 131072 x 64: 16.3, 131072 x 128, 6, with bias: 27.2 (1.5 TB/s); 16383 x 256 fp32 sigmoid, 8 of the 4 best
+//             of 8 groups, with bias: 21.6, 65536 x 256 bf16 the same way: 50.6, without groups 41.8, without bias 29.5, of softmax 25.0
 //   backward  2.1, 7.9, 15.6 (4.5 TB/s), 8.0, 13.7, 13.8: the scores are computed again from the logits, which the forward would write as 4 bytes an expert
 //             for this to read; a choice's gradient is written by the lane that has the choice, so there are no atomics
 //
@@ -114,6 +114,16 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // How far two choice values have to be apart for their order to be sure, when they come from the fast sigmoid: twice its error, and the rounding of
 // the sum with the bias.
 __device__ __forceinline__ float route_margin(float c) { return 1e-6f + 2.4e-7f * fabsf(c); }
+
+// Whether all experts with keys in the range of ``key`` have the logit ``x``: the sigmoids of its neighbours among the bf16 numbers lie outside.  (Among the
+// fp32 numbers they never do.  Neighbours of 0 and of infinities come out as NaN or too close: no.)
+template <typename T>
+__device__ __forceinline__ bool route_alone(float x, uint32_t key, uint32_t mask) {
+  if (std::is_same<T, float>::value) return false;
+  const uint32_t u = __float_as_uint(x);
+  const float a = route_sigmoid_fast(__uint_as_float(u + 0x10000u)), b = route_sigmoid_fast(__uint_as_float(u - 0x10000u)), m = 2.f * route_margin(1.f);
+  return fmaxf(a, b) - route_unorder(key | mask) > m && route_unorder(key & ~mask) - fminf(a, b) > m;
+}
 
 // Orders of the choice values of a lane's experts; 0 for what cannot be chosen.
 template <typename T, int V, bool SIGMOID, bool FAST>
@@ -262,11 +272,16 @@ __device__ __forceinline__ int route_select_exact(const uint32_t (&o)[V], int e0
 // The choice takes keys in place of the choice values: the upper bits of the value's order, and in the lower b bits (2^b >= E) the expert's number,
 // inverted, so that the larger of two keys is the one to be chosen.  All keys differ, which makes a step of the selection - the largest key below
 // the last - max(key - last) + last in wrapping arithmetic: two instructions a key.  Two things are left out at first: the lower bits of a
-// value, and for sigmoid scores the last bits of a sigmoid, which is taken from the hardware's approximations.  They matter only where neighbours in the
-// result (the last chosen and the best of the rest among them) are closer than that; their exact values tell, and then the warp does the choice
-// again with exact values and numbers (256 experts: about 1 token in 100; bf16 logits without bias: never, the keys have all their 16 bits).
+// value, and for sigmoid scores the last bits of a sigmoid, which is taken from the hardware's approximations (softmax of bf16 logits without bias: neither,
+// the keys have all their 16 bits).  So the choice is proved afterwards.  Its own experts have to stand in the order of their exact values, neighbour by
+// neighbour.  And the rest has to lie below the last of them.  Where the range of values that the rest's largest key stands for comes close (1 token in
+// 100, or 1 in 5 for equal bf16 logits), that expert's exact value is compared, and one more step of the selection gives the range of all the
+// others: a key names the lowest number of its range, not the largest value.  Others in the same range do no harm if they can only have the same logit.
+// Where the proof fails, the warp does the choice again with exact values and numbers.
+//
+// (48, 64 and 80 registers for 8, 16 and 32 experts a lane: left to itself the compiler takes a few more for the code that few warps come to.)
 template <typename T, int L, int V, bool SIGMOID>
-__global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_kernel(RouteParams p) {
+__global__ void __launch_bounds__(32 * ROUTE_WARPS, V == 8 ? 5 : V == 16 ? 4 : 3) moe_route_kernel(RouteParams p) {
   after_previous();
   constexpr int TPW = 32 / L;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tok = lane / L, sub = lane % L;
@@ -276,8 +291,10 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_kernel(RouteParams
   const int e0 = sub * V;
   const bool chosen = sub < p.k;
   float m_all = -CUDART_INF_F, total_all = 0.f;
-  uint32_t mine = 0, last = 0;
-  bool unsure;
+  const bool proved = SIGMOID || std::is_same<T, float>::value || p.bias != nullptr;
+  auto range = [&](uint32_t key) { return key & ~p.mask; };
+  uint32_t mine = 0, last = 0, others = 0;  // keys: this lane's choice, the largest of the rest, the one after it (0: there is none)
+  bool unsure, near = false;                // near: the last choice to the range of the rest's largest key
   {
     float x[V];
     uint32_t o[V], key[V];
@@ -305,22 +322,37 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_kernel(RouteParams
       for (int i = 0; i < V; ++i) best = max(best, key[i] - last);
       last += lanes_max<L>(best);
     }
-    if (sub == p.k) mine = last;  // the best of the rest; 0 if there is none
+    if (proved) {
+      near = sub + 1 == p.k && last != 0;
+      if (SIGMOID) {
+        const float lo = route_unorder(range(mine));
+        near = near && !(lo - route_unorder(last | p.mask) > route_margin(lo));
+      } else {
+        near = near && range(mine) == range(last) && range(last) != range(0x007FFFFFu);  // (-inf has a range to itself)
+      }
+      if (__any_sync(0xffffffffu, near)) {
+        uint32_t best = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) best = max(best, key[i] - last);
+        others = last + lanes_max<L>(best);
+      }
+    }
   }
   int e = mine != 0 ? (int)(p.mask - (mine & p.mask)) : 0;
   float xe = route_load(row + e), se = SIGMOID ? route_sigmoid(xe) : 0.f;
-  if (SIGMOID || std::is_same<T, float>::value || p.bias != nullptr) {
-    float c = SIGMOID ? se : xe;
-    if (p.bias != nullptr) c += p.bias[e];
-    const uint32_t next = __shfl_down_sync(0xffffffffu, mine, 1, L);
-    const float next_c = __shfl_down_sync(0xffffffffu, c, 1, L), next_x = __shfl_down_sync(0xffffffffu, xe, 1, L);
-    if (sub + 1 < L) {
-      const bool close = SIGMOID ? !(c - next_c > route_margin(c)) && !(p.bias == nullptr && xe == next_x) : c != next_c;
-      unsure |= chosen && next != 0 && close && (SIGMOID || ((mine ^ next) & ~p.mask) == 0);
-      if (SIGMOID) unsure |= chosen && next != 0 && ((mine ^ next) & ~p.mask) == 0 && c != next_c;
-    } else if (chosen && last != 0) {  // (every lane has a choice: the next key's upper end stands for the best of the rest)
-      const float lo = route_unorder(mine & ~p.mask);
-      unsure |= SIGMOID ? !(lo - route_unorder(last | p.mask) > route_margin(lo)) : ((mine ^ last) & ~p.mask) == 0;
+  if (proved) {
+    auto before = [](float c0, int e0, float c1, int e1) { return c0 > c1 || (c0 == c1 && e0 < e1); };
+    auto value = [&](float x, float s, int i) { return (SIGMOID ? s : x) + (p.bias != nullptr ? p.bias[i] : 0.f); };
+    const float c = value(xe, se, e), next_c = __shfl_down_sync(0xffffffffu, c, 1, L);
+    const int next_e = __shfl_down_sync(0xffffffffu, e, 1, L);
+    unsure |= sub + 1 < p.k && !before(c, e, next_c, next_e);
+    if (near) {
+      const int r = (int)(p.mask - (last & p.mask));
+      const float xr = route_load(row + r);
+      const bool tie = p.bias == nullptr && xr == xe;  // (the keys have them in the order of their numbers)
+      bool open = others != 0 && (SIGMOID ? !(c - route_unorder(others | p.mask) > route_margin(c)) : range(others) == range(last));
+      if (SIGMOID && open && tie) open = !route_alone<T>(xe, last, p.mask);
+      unsure |= open || !(tie || before(c, e, value(xr, SIGMOID ? route_sigmoid(xr) : 0.f, r), r));
     }
     if (__any_sync(0xffffffffu, unsure)) {
       float x[V];

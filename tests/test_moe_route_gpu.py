@@ -193,3 +193,80 @@ def test_the_c_entry_refuses_what_it_cannot_take():
     assert call(bias_bytes=16) == 0
     torch.cuda.synchronize()
     assert (w == 0.125).all() and (idx == torch.arange(8, device="cuda")).all()
+
+
+def experts_at_random(T, E, n, g):
+    """``n`` different experts of each of ``T`` tokens, in no order."""
+    return torch.rand(T, E, device="cuda", generator=g).argsort(-1)[:, :n]
+
+
+def same_choice(x, k, score, bias=None, groups=1, top_groups=1):
+    _, idx = K.moe_route(x, k, score=score, bias=bias, num_groups=groups, top_groups=top_groups)
+    wrong = (idx != formula(x, bias, k, score, groups, top_groups, True, 1.0)[1]).any(-1)
+    assert not wrong.any(), f"{int(wrong.sum())} of {len(x)} tokens, first {wrong.nonzero()[0].item()}"
+
+
+LAST_PLACE = [(64, 1), (64, 6), (64, 7), (64, 8), (128, 6), (256, 1), (256, 8), (256, 16), (1024, 10), (1024, 31), (60, 3)]
+
+
+@pytest.mark.parametrize("E,k", LAST_PLACE)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_the_last_place_among_near_and_equal_values(E, k, score):
+    """The last choice and the best of the rest may be equal where a third expert, with a higher number, is larger by a unit in the last place: several
+    experts a few units apart contend for the last places, below others that are chosen for sure."""
+    g = torch.Generator("cuda").manual_seed(E + k)
+    T = 2000
+    at = experts_at_random(T, E, k - 1 + 6, g)
+    sure = 2 + 0.1 * torch.rand(T, k - 1, device="cuda", generator=g)
+    for near in (1 + 2.0**-23 * torch.randint(0, 4, (T, 6), device="cuda", generator=g),     # fp32 neighbours
+                 1 + 2.0**-20 * torch.randint(0, 3, (T, 6), device="cuda", generator=g),     # sigmoids some units apart
+                 torch.full((T, 6), 1.0, device="cuda")):
+        x = (torch.rand(T, E, device="cuda", generator=g) - 5).scatter_(1, at, torch.cat((sure, near.float()), 1))
+        same_choice(x, k, score)
+        same_choice(x, k, score, bias=3e-8 * torch.randint(-4, 5, (E,), device="cuda", generator=g).float())
+        if E % 4 == 0:
+            same_choice(x, k, score, groups=4, top_groups=4)
+    # scores that are all but 1: different logits, the same or neighbouring sigmoids
+    x = (8 + 2 * torch.randn(T, E, device="cuda", generator=g)).bfloat16()
+    same_choice(x, k, score)
+    same_choice(x.float(), k, score)
+    same_choice(x.float() + 4, k, score)
+    # few values: equal logits in most last places
+    x = (0.25 * torch.randint(-8, 9, (T, E), device="cuda", generator=g)).bfloat16()
+    for bias in (None, 3e-8 * torch.randint(-4, 5, (E,), device="cuda", generator=g).float()):
+        same_choice(x, k, score, bias)
+        same_choice(x.float(), k, score, bias)
+
+
+@pytest.mark.parametrize("E,k", LAST_PLACE)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_the_last_place_by_hand(E, k, score):
+    sure = list(range(E - k + 1, E))
+    x = torch.full((4, E), -5.0, device="cuda")
+    x[:, sure] = 40.0 - torch.arange(k - 1, device="cuda") / 4
+    x[0, :3] = torch.tensor([12.0, 12.0, 13.0])
+    x[1, :3] = torch.tensor([10.0625, 10.0625, 10.125])
+    x[2, :3] = torch.tensor([1.0, 1.0, 1.0 + 2.0**-20])
+    x[3, :3] = torch.tensor([1.0, 1.0, 1.0 + 2.0**-23])
+    rows = 4 if score == "softmax" else 2  # (two units of a logit are less than one of a sigmoid)
+    _, idx = K.moe_route(x[:rows], k, score=score)
+    assert idx[:, -1].tolist() == [2] * rows and idx[:, :-1].tolist() == [sure] * rows
+    _, idx = K.moe_route(x[:2].bfloat16(), k, score=score)
+    assert idx[:, -1].tolist() == [2, 2]
+
+
+@pytest.mark.parametrize("E,k", [(64, 1), (128, 6), (256, 8), (1024, 10)])
+def test_the_last_place_at_the_ends_of_keys(E, k):
+    """Keys hold the upper bits of a score.  Two scores lie within the error of a fast sigmoid to both sides of a multiple of the lower ones' range, and a
+    smaller one, with a lower number, just below in the same range as the lower of the two."""
+    g = torch.Generator("cuda").manual_seed(E)
+    T, bits = 50000, (E - 1).bit_length()
+    unit = 2.0 ** (bits - 24)  # of scores in [0.5, 1)
+    at = experts_at_random(T, E, k + 2, g)
+    at[:, :3] = at[:, :3].sort(-1).values
+    end = (torch.randint(int(0.55 / unit), int(0.8 / unit), (T,), device="cuda", generator=g) * unit).double()
+    score = torch.stack((end - 0.6 * unit, end, end), 1)
+    score[:, 1:] += 4e-7 * (2 * torch.rand(T, 2, device="cuda", generator=g, dtype=torch.float64) - 1)
+    x = (torch.rand(T, E, device="cuda", generator=g) - 5).scatter_(1, at, 3.0)
+    x = x.scatter_(1, at[:, :3], torch.logit(score).float())
+    same_choice(x, k, "sigmoid")
