@@ -160,6 +160,10 @@ template <int L, int V, bool SIGMOID, bool FAST>
 __device__ __forceinline__ bool route_groups(const RouteParams& p, int warp, int tok, int sub, uint32_t (&o)[V]) {
   extern __shared__ uint32_t route_words[];
   auto value = [&](uint32_t a, uint32_t b) { return SIGMOID && p.size > 1 ? route_order(route_unorder(a) + route_unorder(b)) : a; };
+  // A sum of unlike signs is smaller than what was rounded for it, which the margin below does not count: up to 1 it is within what the margin has to
+  // spare (the two sigmoids differ by 1.8e-7 at most, of 5e-7), beyond that nothing is sure.
+  auto cancels = [&](uint32_t a, uint32_t b) { return SIGMOID && FAST && p.size > 1 && route_unorder(a) > 1.f && route_unorder(b) < -1.f; };
+  bool vague = false;
   uint32_t kept_min = 0xFFFFFFFFu, dropped_max = 0;
   if (p.size % V == 0) {
     const int per = p.size / V, g = sub / per, first = g * per;
@@ -177,6 +181,7 @@ __device__ __forceinline__ bool route_groups(const RouteParams& p, int warp, int
       a = max(a, a1);
     }
     const uint32_t mine = g < p.groups ? value(a, b) : 0u;
+    vague = cancels(a, b);
     int before = 0;
     for (int h = 0; h < p.groups; ++h) {
       const uint32_t v = __shfl_sync(0xffffffffu, mine, tok * L + h * per);
@@ -202,6 +207,7 @@ __device__ __forceinline__ bool route_groups(const RouteParams& p, int warp, int
         a = max(a, v);
       }
       val[g] = value(a, b);
+      vague |= cancels(a, b);
     }
     __syncwarp();
     unsigned long long kept = 0;  // bit i: this lane's i-th group
@@ -234,7 +240,7 @@ __device__ __forceinline__ bool route_groups(const RouteParams& p, int warp, int
   const uint32_t lowest = ~lanes_max<L>(~kept_min), highest = lanes_max<L>(dropped_max);
   if (highest == 0) return false;
   const float low = route_unorder(lowest);
-  return !(low - route_unorder(highest) > 2.f * route_margin(low));
+  return vague || !(low - route_unorder(highest) > 2.f * route_margin(low));
 }
 
 // Lane j's choice from whole values and numbers: the largest (value, -number) below the last.

@@ -270,3 +270,15 @@ def test_the_last_place_at_the_ends_of_keys(E, k):
     x = (torch.rand(T, E, device="cuda", generator=g) - 5).scatter_(1, at, 3.0)
     x = x.scatter_(1, at[:, :3], torch.logit(score).float())
     same_choice(x, k, "sigmoid")
+
+
+def test_groups_whose_two_largest_cancel():
+    """The sum of two large values of unlike sign is small, but has their rounding."""
+    g = torch.Generator("cuda").manual_seed(5)
+    for E, groups in ((64, 8), (256, 8), (48, 3), (16, 8)):
+        size = E // groups
+        bias = torch.full((groups, size), -300.0, device="cuda")
+        bias[:, 0], bias[:, 1] = 100.0, -100.0
+        x = 0.0005 * torch.randn(100000, E, device="cuda", generator=g) - 1.5
+        kept = max(1, groups // 2)
+        same_choice(x, kept, "sigmoid", bias.flatten(), groups, kept)  # (the largest of every group that stays)
