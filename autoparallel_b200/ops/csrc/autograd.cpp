@@ -404,7 +404,7 @@ struct MxMatmul : torch::autograd::Function<MxMatmul> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, bool trans_b, ScalarType dtype) {
     at::AutoDispatchBelowAutograd guard;
     const bool flat = w.dim() == 2 && x.dim() != 2;
-    auto [a, sa] = op_mx_quantize()(flat ? x.reshape({x.numel() / std::max<int64_t>(x.size(-1), 1), x.size(-1)}) : x);
+    auto [a, sa] = op_mx_quantize()(flat ? x.reshape({c10::multiply_integers(x.sizes().slice(0, x.dim() - 1)), x.size(-1)}) : x);
     auto [b, sb] = op_mx_quantize()(trans_b ? w : w.transpose(-1, -2));
     Tensor y = op_mx_mm()(a, sa, b, sb, dtype);
     const bool of_x = x.requires_grad(), of_w = w.requires_grad();
@@ -426,11 +426,16 @@ struct MxMatmul : torch::autograd::Function<MxMatmul> {
     Tensor dx, dw;
     if (ctx->needs_input_grad(0)) dx = op_mx_mm_values()(g[0], s[2], s[3], k, ctx->saved_data["x"].toScalarType());
     if (ctx->needs_input_grad(1)) {
+      const ScalarType type = ctx->saved_data["w"].toScalarType();
+      if (k == 0 || n == 0) {  // (the products take no matrices without columns)
+        std::vector<int64_t> shape{tb ? n : k, tb ? k : n};
+        if (s[0].dim() == 3) shape.insert(shape.begin(), s[0].size(0));
+        return {dx, at::zeros(shape, g[0].options().dtype(type)), Tensor(), Tensor()};
+      }
       const Tensor dy = pad_last(g[0]);
       const Tensor xq = op_mx_values()(s[0], s[1], kp, dy.scalar_type());  // [rows, kp], or [E, rows, kp]
       const Tensor d = xq.dim() == 3 ? dy : dy.reshape({xq.size(0), dy.size(-1)});
       const Op<WgradSig>& wgrad = xq.dim() == 3 ? op_grouped_wgrad() : op_mm_wgrad();
-      const ScalarType type = ctx->saved_data["w"].toScalarType();
       dw = tb ? cut(cut(wgrad(d, xq, type), -1, k), -2, n) : cut(cut(wgrad(xq, d, type), -1, n), -2, k);
     }
     return {dx, dw, Tensor(), Tensor()};
@@ -447,6 +452,7 @@ struct MxMatmulTraced : torch::autograd::Function<MxMatmulTraced> {
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &w = s[1], dy = pad_last(g[0]);
     const bool tb = ctx->saved_data["tb"].toBool();
+    if (x.size(-1) == 0 || dy.size(-1) == 0) return {at::zeros_like(x), at::zeros_like(w), Tensor(), Tensor(), Tensor()};
     Tensor dx, dw;
     if (ctx->needs_input_grad(0))
       dx = cut(times(dy, pad8(op_mx_round()(w, tb ? -1 : -2).to(dy.scalar_type()), true, true), !tb, x.scalar_type()), -1, x.size(-1));

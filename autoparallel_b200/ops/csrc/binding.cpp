@@ -888,6 +888,8 @@ struct MxView {
   }
 };
 int64_t mx_blocks(int64_t k) { return (k + 31) / 32; }
+// The rows of x [.., K] as one matrix, also where K is 0.
+Tensor mx_flat(const Tensor& x) { return x.reshape({c10::multiply_integers(x.sizes().slice(0, x.dim() - 1)), x.size(-1)}); }
 
 Two mx4_quantize(const Tensor& x_) {
   c10::cuda::CUDAGuard g(x_.device());
@@ -970,7 +972,7 @@ Tensor mx4_linear(const Tensor& x_, const Tensor& codes_, const Tensor& scales_,
               "mx4_linear: x ", x_.sizes(), " and codes ", codes_.sizes(), " do not multiply");
   TORCH_CHECK(codes_.is_cuda() && codes_.device() == x_.device() && float_or_bf16(dtype), "mx4_linear: weights on x's device, a result in bf16 or fp32");
   const int64_t K = x_.size(-1), N = codes_.size(-2);
-  const MxView v(codes_.dim() == 3 || x_.dim() == 2 ? x_ : x_.reshape({x_.numel() / std::max<int64_t>(K, 1), K}), "mx4_linear");
+  const MxView v(codes_.dim() == 3 || x_.dim() == 2 ? x_ : mx_flat(x_), "mx4_linear");
   auto shape = x_.sizes().vec();
   shape.back() = N;
   Tensor c = at::empty(shape, x_.options().dtype(dtype)), codes = dense(codes_), scales = dense(scales_), rounded;
@@ -1007,17 +1009,18 @@ c10::optional<Tensor> mx4_mm_values(const Tensor& a_, const Tensor& codes_, cons
                   (codes_.dim() == 2 || (a_.dim() == 3 && a_.size(0) == codes_.size(0))),
               "mx4_mm_values: a ", a_.sizes(), ", codes ", codes_.sizes(), ", ", k, " columns");
   TORCH_CHECK(float_or_bf16(a_.scalar_type()) && float_or_bf16(dtype), "mx4_mm_values: bf16 or fp32");
-  const int64_t G = codes_.dim() == 3 ? codes_.size(0) : 1, M = N == 0 ? 0 : a_.numel() / (G * N > 0 ? G * N : 1);
-  const bool fp32 = dtype == at::kFloat;
-  if (a_.scalar_type() != at::kBFloat16 || N == 0 || N % 8 || !(always || apb_gemm_mx4_values_takes(G, M, k, num_sms()))) return c10::nullopt;
-  Tensor a = dense(a_), codes = dense(codes_), scales = dense(scales_);
-  auto shape = a.sizes().vec();
+  auto shape = a_.sizes().vec();
   shape.back() = k;
+  if (c10::multiply_integers(shape) == 0 || N == 0) return at::zeros(shape, a_.options().dtype(dtype));
+  const int64_t G = codes_.dim() == 3 ? codes_.size(0) : 1, M = a_.numel() / (G * N);
+  const bool fp32 = dtype == at::kFloat;
+  if (a_.scalar_type() != at::kBFloat16 || N % 8 || !(always || apb_gemm_mx4_values_takes(G, M, k, num_sms()))) return c10::nullopt;
+  Tensor a = dense(a_), codes = dense(codes_), scales = dense(scales_);
   Tensor c = at::empty(shape, a.options().dtype(dtype));
   check(apb_gemm_mx4_values(a.data_ptr(), codes.data_ptr(), scales.data_ptr(), c.data_ptr(), G, M, N, k, fp32,
                             reinterpret_cast<uint32_t*>(status_of(a).data_ptr()), num_sms(), stream()),
         "apb_gemm_mx4_values");
-  count(c.numel() > 0);
+  count();
   return c;
 }
 

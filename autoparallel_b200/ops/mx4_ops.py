@@ -198,6 +198,8 @@ def _matmul_setup(ctx, inputs, output):
 def _matmul_bwd(ctx, dy):
     x, w = ctx.saved_tensors
     tb, grouped = ctx.trans_b, w.ndim == 3
+    if x.shape[-1] == 0 or dy.shape[-1] == 0:  # (the products take no matrices without columns)
+        return torch.zeros_like(x), torch.zeros_like(w), None, None
     dyp = _pad8(dy, -1)
     dx = dw = None
     if ctx.needs_input_grad[0]:

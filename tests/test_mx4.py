@@ -287,3 +287,18 @@ def test_example():
                        cwd=root)
     assert r.returncode == 0, r.stderr[-2000:]
     assert "mx4_matmul" in r.stdout and "served" in r.stdout
+
+
+@pytest.mark.parametrize("x_shape,w_shape", [((0,), (48, 0)), ((2, 5, 0), (48, 0)), ((2, 3, 64), (0, 64)), ((0, 64), (48, 64)),
+                                             ((3, 5, 0), (3, 48, 0)), ((3, 5, 64), (3, 0, 64))])
+def test_matrices_of_nothing(x_shape, w_shape):
+    x, w = torch.zeros(x_shape, requires_grad=True), torch.zeros(w_shape, requires_grad=True)
+    for trans_b in (True, False):
+        m = w if trans_b else w.transpose(-1, -2).contiguous()
+        y = K.mx4_matmul(x, m, trans_b=trans_b)
+        dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        assert y.shape == (*x_shape[:-1], w_shape[-2]) and dx.shape == x_shape and dw.shape == w_shape
+    codes, scales = K.mx4_quantize(w.detach())
+    y = K.mx4_linear(x, codes, scales)
+    assert (y == 0).all() and torch.autograd.grad(y, x, torch.ones_like(y))[0].shape == x_shape
+    assert K.mx4_mm_values(y.detach(), codes, scales, x_shape[-1]).shape == x_shape

@@ -371,3 +371,41 @@ def test_c_entries_refuse_what_they_cannot_take():
     assert product(rows, tail) == 0 and product(rows, tail, a=p + 4) == 3
     assert product(rows, (i64(0), i64(0), 2, 1, 3, ptr(status.data_ptr()), 148, ptr(0))) == 3
     torch.cuda.synchronize()
+
+@pytest.mark.parametrize("shape", [(0,), (4, 0), (2, 5, 0), (2, 3, 40, 0)])
+def test_contractions_of_nothing_are_zero(shape):
+    """Whatever the dims of x, and in memory that held something else."""
+    w = torch.zeros(48, 0, device="cuda", requires_grad=True)
+    b = K.mx4_quantize(w.detach())
+    for dtype in (BF16, F32):
+        held = torch.full((*shape[:-1], 48), 7.0, device="cuda", dtype=dtype)
+        del held
+        x = torch.zeros(shape, device="cuda", dtype=dtype, requires_grad=True)
+        y = K.mx4_linear(x, *b)
+        assert y.shape == (*shape[:-1], 48) and y.dtype == dtype and (y == 0).all()
+        (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert dx.shape == shape
+        y = K.mx4_matmul(x, w)
+        assert y.shape == (*shape[:-1], 48) and (y == 0).all()
+        dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        assert dx.shape == shape and dw.shape == w.shape
+        assert K.mx4_mm_values(y.detach(), *b, 0).shape == shape
+
+
+@pytest.mark.parametrize("lead,m,n,k", [((), 5, 0, 64), ((), 0, 48, 64), ((3,), 5, 0, 64), ((3,), 5, 48, 0), ((3,), 0, 48, 64),
+                                        ((0,), 5, 48, 64), ((2, 3), 5, 0, 64), ((), 5, 0, 0)])
+@pytest.mark.parametrize("trans_b", [True, False])
+def test_matrices_of_nothing(lead, m, n, k, trans_b):
+    """Products and gradients without rows, columns, experts or a contraction."""
+    wl = lead if len(lead) == 1 else ()
+    for dtype in (BF16, F32):
+        x = torch.randn(*lead, m, k, device="cuda").to(dtype).requires_grad_()
+        w = torch.randn(*wl, *((n, k) if trans_b else (k, n)), device="cuda").to(dtype).requires_grad_()
+        y = K.mx4_matmul(x, w, trans_b=trans_b)
+        dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        codes, scales = K.mx4_quantize(w.detach() if trans_b else w.detach().transpose(-1, -2))
+        z = K.mx4_linear(x, codes, scales)
+        (dz,) = torch.autograd.grad(z, x, torch.ones_like(z))
+        v = K.mx4_mm_values(y.detach(), codes, scales, k)
+        assert y.shape == z.shape == (*lead, m, n) and dx.shape == dz.shape == v.shape == x.shape and dw.shape == w.shape
+        assert all((t == 0).all() for t in (y, z, dx, dz, dw, v))
