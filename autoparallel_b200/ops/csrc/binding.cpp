@@ -857,8 +857,8 @@ Two moe_route(const Tensor& logits_, const c10::optional<Tensor>& bias, int64_t 
 Tensor moe_route_bwd(const Tensor& dw_, const Tensor& logits_, const Tensor& idx_, bool sigmoid, bool renorm, double scale) {
   c10::cuda::CUDAGuard g(logits_.device());
   TORCH_CHECK(logits_.dim() >= 1 && logits_.size(-1) >= 1 && dw_.sizes() == idx_.sizes() && idx_.dim() == logits_.dim() &&
-                  idx_.scalar_type() == at::kLong && dw_.is_cuda() && idx_.is_cuda(),
-              "moe_route_bwd: dweights and idx [.., k], logits [.., experts]");
+                  idx_.scalar_type() == at::kLong && dw_.device() == logits_.device() && idx_.device() == logits_.device(),
+              "moe_route_bwd: dweights and idx [.., k], logits [.., experts], on one device");
   const int64_t E = logits_.size(-1), k = idx_.size(-1), tokens = logits_.numel() / E;
   TORCH_CHECK(E <= 1024 && k >= 1 && k <= 32 && k <= E && idx_.numel() == tokens * k, "moe_route_bwd: ", k, " of ", E, " experts");
   Tensor logits = dense(logits_), dw = dw_.to(at::kFloat).contiguous(), idx = idx_.contiguous(), dx = at::empty_like(logits);

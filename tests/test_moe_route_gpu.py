@@ -282,3 +282,20 @@ def test_groups_whose_two_largest_cancel():
         x = 0.0005 * torch.randn(100000, E, device="cuda", generator=g) - 1.5
         kept = max(1, groups // 2)
         same_choice(x, kept, "sigmoid", bias.flatten(), groups, kept)  # (the largest of every group that stays)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="two devices")
+def test_the_gradient_refuses_tensors_of_another_device():
+    x = torch.zeros(4, 64, device="cuda:0")
+    w, idx = K.moe_route(x, 8)
+    for dw, i in ((w.to("cuda:1"), idx), (w, idx.to("cuda:1"))):
+        with pytest.raises(RuntimeError, match="one device"):
+            torch.ops.apb200.moe_route_bwd(dw, x, i, False, True, 1.0)
+
+
+def test_the_gradient_refuses_tensors_of_the_host():
+    x = torch.zeros(4, 64, device="cuda")
+    w, idx = K.moe_route(x, 8)
+    for dw, i in ((w.cpu(), idx), (w, idx.cpu())):
+        with pytest.raises(RuntimeError, match="one device"):
+            torch.ops.apb200.moe_route_bwd(dw, x, i, False, True, 1.0)
