@@ -378,6 +378,32 @@ struct MxRound : torch::autograd::Function<MxRound> {
 Tensor mx4_round(DispatchKeySet ks, const Tensor& x, int64_t dim) {
   return records(x) ? MxRound::apply(x, dim, Keys{ks}) : op_mx_round().below(ks, x, dim);
 }
+struct MxMmValues : torch::autograd::Function<MxMmValues> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& a, const Tensor& codes, const Tensor& scales, int64_t k, ScalarType dtype, Keys ks) {
+    ctx->save_for_backward({codes, scales});
+    ctx->saved_data["k"] = k;
+    ctx->saved_data["dtype"] = a.scalar_type();
+    return op_mx_mm_values().below(ks.ks, a, codes, scales, k, dtype);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor& dc = g[0];
+    const int64_t n = s[0].size(-2), k8 = (ctx->saved_data["k"].toInt() + 7) / 8 * 8;
+    const ScalarType dtype = ctx->saved_data["dtype"].toScalarType();
+    Tensor da;
+    if (n == 0 || k8 == 0) {
+      auto shape = dc.sizes().vec();
+      shape.back() = n;
+      da = at::zeros(shape, dc.options().dtype(dtype));
+    } else {
+      da = cut(times(pad_last(dc), pad8(op_mx_values()(s[0], s[1], k8, dc.scalar_type()), true, false), true, dtype), -1, n);
+    }
+    return {da, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor mx4_mm_values(DispatchKeySet ks, const Tensor& a, const Tensor& codes, const Tensor& scales, int64_t k, ScalarType dtype) {
+  return records(a) ? MxMmValues::apply(a, codes, scales, k, dtype, Keys{ks}) : op_mx_mm_values().below(ks, a, codes, scales, k, dtype);
+}
 struct MxLinear : torch::autograd::Function<MxLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& codes, const Tensor& scales, ScalarType dtype, Keys k) {
     ctx->save_for_backward({codes, scales});
@@ -488,6 +514,7 @@ TORCH_LIBRARY_IMPL(apb200, AutogradCUDA, m) {
   m.impl("moe_gather", moe_gather);
   m.impl("moe_route", moe_route);
   m.impl("mx4_round", mx4_round);
+  m.impl("mx4_mm_values", mx4_mm_values);
   m.impl("mx4_linear", mx4_linear);
   m.impl("mx4_matmul", mx4_matmul);
 }

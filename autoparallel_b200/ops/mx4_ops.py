@@ -22,7 +22,7 @@ Operators (``apb200::``; the functions below them check arguments and fill in de
     mx4_mm(a, sa, b, sb, dtype)                      a [.., M, K] x b [.., N, K] -> [.., M, N], sums in fp32
     mx4_linear(x, codes, scales, dtype)              activations (rounded on the way) by weights held in 4 bits; gradient of ``x``
     mx4_matmul(x, w, trans_b, dtype)                 both operands rounded on the way; gradients of both
-    mx4_mm_values(a, codes, scales, k, dtype)        a [.., N] (16 or 32 bits) by the values [N, k] of codes: gradients of ``x`` above
+    mx4_mm_values(a, codes, scales, k, dtype)        a [.., N] (16 or 32 bits) by the values [N, k] of codes: gradients of ``x`` above; gradient of ``a``
 
 The rounding has no useful derivative; gradients go straight through it: with ``q`` for rounding and ``y = q(x) q(w)^T``,
 ``dx = dy q(w)`` and ``dw = dy^T q(x)``, 16-bit products of the framework's own GEMM.
@@ -214,6 +214,23 @@ def _matmul_bwd(ctx, dy):
     return dx, dw, None, None
 
 
+def _values_setup(ctx, inputs, output):
+    a, codes, scales, k, _ = inputs
+    ctx.save_for_backward(codes, scales)
+    ctx.k, ctx.dtype = k, a.dtype
+
+
+def _values_bwd(ctx, dc):
+    codes, scales = ctx.saved_tensors
+    n, k8 = codes.shape[-2], -(-ctx.k // 8) * 8
+    if n == 0 or k8 == 0:
+        return dc.new_zeros((*dc.shape[:-1], n), dtype=ctx.dtype), None, None, None, None
+    w = _pad8(ops.mx4_dequantize(codes, scales, k8, dc.dtype), -2)
+    da = _times(_pad8(dc, -1), w, True, ctx.dtype)
+    return (da[..., :n] if da.shape[-1] != n else da), None, None, None, None
+
+
+_ag("mx4_mm_values", _values_bwd, _values_setup)
 _ag("mx4_linear", _linear_bwd, _linear_setup)
 _ag("mx4_matmul", _matmul_bwd, _matmul_setup)
 _ag("mx4_round", lambda ctx, dy: (dy, None), lambda ctx, inputs, output: None)

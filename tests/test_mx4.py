@@ -302,3 +302,19 @@ def test_matrices_of_nothing(x_shape, w_shape):
     y = K.mx4_linear(x, codes, scales)
     assert (y == 0).all() and torch.autograd.grad(y, x, torch.ones_like(y))[0].shape == x_shape
     assert K.mx4_mm_values(y.detach(), codes, scales, x_shape[-1]).shape == x_shape
+
+
+@pytest.mark.parametrize("lead,m,n,k", [((), 5, 7, 33), ((3,), 4, 9, 96), ((2, 3), 4, 16, 40)])
+def test_gradient_of_products_with_values(lead, m, n, k):
+    torch.manual_seed(0)
+    codes, scales = K.mx4_quantize(torch.randn(*(lead if len(lead) == 1 else ()), n, k))
+    values = K.mx4_dequantize(codes, scales, k, torch.float32).double()
+    a, dc, x = torch.randn(*lead, m, n, requires_grad=True), torch.randn(*lead, m, k), torch.randn(*lead, m, k, requires_grad=True)
+    ad = a.detach().double().requires_grad_()
+    (want,) = torch.autograd.grad(ad @ values, ad, dc.double())
+    assert torch.autograd.gradcheck(lambda t: t @ values, ad)
+    (da,) = torch.autograd.grad(K.mx4_mm_values(a, codes, scales, k), a, dc)
+    assert torch.allclose(da.double(), want, rtol=1e-5, atol=1e-5)
+    (dx,) = torch.autograd.grad(K.mx4_linear(x, codes, scales), x, a, create_graph=True)
+    (da,) = torch.autograd.grad(dx, a, dc)
+    assert torch.allclose(da.double(), want, rtol=1e-5, atol=1e-5)

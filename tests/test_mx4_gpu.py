@@ -409,3 +409,29 @@ def test_matrices_of_nothing(lead, m, n, k, trans_b):
         v = K.mx4_mm_values(y.detach(), codes, scales, k)
         assert y.shape == z.shape == (*lead, m, n) and dx.shape == dz.shape == v.shape == x.shape and dw.shape == w.shape
         assert all((t == 0).all() for t in (y, z, dx, dz, dw, v))
+
+
+@pytest.mark.parametrize("lead,m,n,k", [((), 64, 96, 128), ((), 37, 40, 72), ((), 37, 41, 75), ((3,), 40, 64, 96), ((2,), 33, 50, 77),
+                                        ((2, 5), 8, 24, 64), ((160,), 20, 96, 256)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradient_of_products_with_values(lead, m, n, k, dtype):
+    """a . values has the gradient dc . values^T; so has the gradient of mx4_linear, which is such a product."""
+    wl = lead if len(lead) == 1 else ()
+    codes, scales = K.mx4_quantize(randn(*wl, n, k, seed=2, dtype=dtype))
+    values = K.mx4_dequantize(codes, scales, k, F32).double().transpose(-1, -2)
+    a = torch.randn(*lead, m, n, device="cuda").to(dtype).requires_grad_()
+    dc = torch.randn(*lead, m, k, device="cuda").to(dtype)
+    want = dc.double() @ values
+    tol = 2.0**-7 if dtype == BF16 else 1e-4  # (the type of the result, of the norm)
+
+    def near(g):
+        return g.dtype == dtype and g.shape == a.shape and ((g.double() - want).norm() / want.norm()).item() <= tol
+
+    (da,) = torch.autograd.grad(K.mx4_mm_values(a, codes, scales, k), a, dc)
+    assert near(da)
+    x = torch.randn(*lead, m, k, device="cuda").to(dtype).requires_grad_()
+    (dx,) = torch.autograd.grad(K.mx4_linear(x, codes, scales), x, a, create_graph=True)
+    (da,) = torch.autograd.grad(dx, a, dc)
+    assert near(da)
+    with torch.no_grad():
+        assert not K.mx4_mm_values(a, codes, scales, k).requires_grad
