@@ -11,6 +11,8 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -71,6 +73,25 @@ using GatherSig = Tensor(const Tensor&, const Tensor&, const Tensor&);
 // the second one's gradient, which no formula reads: a launch, an allocation and 8 us of host time per call (RMSNorm of 2047 x 2048 fp32, forward
 // and backward, 81 -> 73 us).  So these operators take gradients as they come; where only the second output was used, the first one's is zeros.
 Tensor first_grad(const variable_list& g, const Tensor& like) { return g[0].defined() ? g[0] : at::zeros_like(like); }
+
+// Gradients that cannot be differentiated again: where a second derivative could be asked for (create_graph) they come with a node that refuses, on every way
+// to an input of the forward call and to the gradient that came in.  Without it they would count as constants, and the second derivative would be
+// wrong without a word.
+template <typename F>
+variable_list once(const char* what, const variable_list& g, F gradients) {
+  if (!at::GradMode::is_enabled()) return gradients();
+  auto edges = torch::autograd::get_current_node()->next_edges();
+  for (auto& e : torch::autograd::collect_next_edges(g)) edges.push_back(std::move(e));
+  variable_list out;
+  {
+    at::AutoGradMode off(false);
+    out = gradients();
+  }
+  auto refuse = std::make_shared<torch::autograd::Error>(std::string(what) + ": no second derivatives on CUDA", std::move(edges));
+  for (Tensor& t : out)
+    if (t.defined()) torch::autograd::set_history(t, refuse);
+  return out;
+}
 
 // The dispatch keys of the call travel to ``forward`` in a wrapper, so that they are not taken for an input.
 struct Keys {
@@ -335,11 +356,13 @@ struct Route : torch::autograd::Function<Route> {
     return {w, idx};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    const auto s = ctx->get_saved_variables();
-    Tensor dx;
-    if (g[0].defined())
-      dx = op_route_bwd()(g[0], s[0], s[1], ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
-    return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return once("moe_route", g, [&]() -> variable_list {
+      const auto s = ctx->get_saved_variables();
+      Tensor dx;
+      if (g[0].defined())
+        dx = op_route_bwd()(g[0], s[0], s[1], ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
+      return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    });
   }
 };
 Pair moe_route(DispatchKeySet ks, const Tensor& x, const c10::optional<Tensor>& bias, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups,
@@ -446,6 +469,9 @@ struct MxMatmul : torch::autograd::Function<MxMatmul> {
     return y.view(shape);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    return once("mx4_matmul", g, [&] { return gradients(ctx, g); });  // (the operands themselves are not kept)
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& g) {
     const auto s = ctx->get_saved_variables();
     const bool tb = ctx->saved_data["tb"].toBool();
     const int64_t k = ctx->saved_data["k"].toInt(), kp = (k + 31) / 32 * 32, n = ctx->saved_data["n"].toInt();

@@ -276,7 +276,7 @@ _ag("grouped_mm", _gmm_bwd, _gmm_setup)
 def moe_route(logits, top_k: int, score: str = "softmax", bias=None, num_groups: int = 1, top_groups: int = 1, renormalize: bool = True,
               scale: float = 1.0):
     """(gate weights [.., top_k] fp32, experts [.., top_k] int64) from router logits [.., E] (bf16 or fp32); ``bias`` [E] fp32 enters the
-    choice alone.  The weights are differentiable with respect to the logits."""
+    choice alone.  The weights are differentiable with respect to the logits, on CUDA once."""
     E = logits.shape[-1] if logits.ndim else 0
     size = E // num_groups if num_groups > 0 else 0
     # (one test for the calls that are right: this is the path of single tokens)

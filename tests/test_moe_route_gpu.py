@@ -299,3 +299,15 @@ def test_the_gradient_refuses_tensors_of_the_host():
     for dw, i in ((w.cpu(), idx), (w, idx.cpu())):
         with pytest.raises(RuntimeError, match="one device"):
             torch.ops.apb200.moe_route_bwd(dw, x, i, False, True, 1.0)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_second_derivatives_are_refused(score):
+    x, dw = logits(20, 64, F32).requires_grad_(), torch.randn(20, 8, device="cuda").requires_grad_()
+    w, _ = K.moe_route(x, 8, score=score)
+    (want,) = torch.autograd.grad(w, x, dw, retain_graph=True)
+    (dx,) = torch.autograd.grad(w, x, dw, create_graph=True)
+    assert torch.equal(dx, want) and not want.requires_grad
+    for t in (x, dw):
+        with pytest.raises(RuntimeError, match="moe_route: no second derivatives"):
+            torch.autograd.grad((dx * dx).sum() + x.sum() + dw.sum(), t, retain_graph=True)

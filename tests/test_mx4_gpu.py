@@ -435,3 +435,17 @@ def test_gradient_of_products_with_values(lead, m, n, k, dtype):
     assert near(da)
     with torch.no_grad():
         assert not K.mx4_mm_values(a, codes, scales, k).requires_grad
+
+
+@pytest.mark.parametrize("wrt", ["x", "w", "dy"])
+def test_second_derivatives_of_matmul_are_refused(wrt):
+    """The operands are kept in 4 bits alone, so the gradients cannot be differentiated: they say so where they are, and are themselves as ever."""
+    x, w = randn(40, 64).requires_grad_(), randn(32, 64, seed=1).requires_grad_()
+    dy = torch.randn(40, 32, device="cuda").requires_grad_()
+    y = K.mx4_matmul(x, w)
+    want = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    dx, dw = torch.autograd.grad(y, (x, w), dy, create_graph=True)
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[1]) and not want[0].requires_grad
+    for g in (dx, dw):
+        with pytest.raises(RuntimeError, match="mx4_matmul: no second derivatives"):
+            torch.autograd.grad((g * g).sum() + w.sum() + x.sum() + dy.sum(), {"x": x, "w": w, "dy": dy}[wrt], retain_graph=True)
