@@ -367,11 +367,11 @@ extern "C" int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, in
   return M <= 32;
 }
 
-// A: values [G, M, K] with unit stride along K (x_type 0: fp32, 1: bf16), or codes (x_type 2) with scales SA; B: codes [G, N, kp / 2], scales SB;
-// C [G, M, N] dense.  ``slices`` 0: chosen here.
+// A: values [G, M, K] with unit stride along K (x_type 0: fp32, 1: bf16; up to 16 rows, more are rounded before), or codes (x_type 2) with scales SA;
+// B: codes [G, N, kp / 2], scales SB; C [G, M, N] dense.  ``slices``: 1, 2 or 4, 0: chosen here.
 extern "C" int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K,
                                  long long gs, long long ld, int x_type, int out_fp32, int slices, uint32_t* status, int num_sms, cudaStream_t stream) {
-  if (G < 0 || M < 0 || N < 0 || K < 0 || M > 32 || N >= 1ll << 31 || K >= 1ll << 30 || G >= 1ll << 31) return 3;
+  if (G < 0 || M < 0 || N < 0 || K < 0 || M > (x_type == 2 ? 32 : 16) || N >= 1ll << 31 || K >= 1ll << 30 || G >= 1ll << 31) return 3;
   if (G == 0 || M == 0 || N == 0) return 0;
   if ((reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(SB) | reinterpret_cast<uintptr_t>(C)) & 15) return 3;
   if (x_type == 2 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(SA)) & 15)) return 3;
@@ -387,7 +387,7 @@ extern "C" int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, c
   p.slices = slices > 0 ? slices : mx_rows_slices(tiles, p.num_kb, resident);
   p.div_tiles = FastDiv((uint32_t)n_tiles);
   p.div_blocks = FastDiv((uint32_t)p.num_kb);
-  if ((p.slices & (p.slices - 1)) || p.slices > 8 || p.slices > p.num_kb || tiles * p.slices >= 1ll << 31) return 3;
+  if ((p.slices & (p.slices - 1)) || p.slices > 4 || p.slices > p.num_kb || tiles * p.slices >= 1ll << 31) return 3;
   p.out_fp32 = out_fp32;
   p.gs = gs, p.ld = ld;
   p.status = status;
@@ -424,11 +424,7 @@ extern "C" int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, c
     if (nt == 16) APB_MX_ROWS(16, void);
     APB_MX_ROWS(32, void);
   }
-  if (x_type == 1) {
-    if (nt == 16) APB_MX_ROWS(16, __nv_bfloat16);
-    APB_MX_ROWS(32, __nv_bfloat16);
-  }
-  if (nt == 16) APB_MX_ROWS(16, float);
-  APB_MX_ROWS(32, float);
+  if (x_type == 1) APB_MX_ROWS(16, __nv_bfloat16);
+  APB_MX_ROWS(16, float);
 #undef APB_MX_ROWS
 }

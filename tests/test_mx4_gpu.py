@@ -449,3 +449,32 @@ def test_second_derivatives_of_matmul_are_refused(wrt):
     for g in (dx, dw):
         with pytest.raises(RuntimeError, match="mx4_matmul: no second derivatives"):
             torch.autograd.grad((g * g).sum() + w.sum() + x.sum() + dy.sum(), {"x": x, "w": w, "dy": dy}[wrt], retain_graph=True)
+
+
+@pytest.mark.parametrize("M", [1, 3, 16, 17, 32])
+def test_every_number_of_slices(M):
+    """The kernel for few rows with the slices of K that it is told to take, one to four CTAs a cluster, from codes and from values; more are refused."""
+    from autoparallel_b200.ops import build, cuda_impl
+
+    rows, i64, ptr = ctypes.CDLL(build.so_path()).apb_gemm_mx4_rows, ctypes.c_longlong, ctypes.c_void_p
+    N, k = 300, 1100
+    x, w = randn(M, k, seed=1), randn(N, k, seed=2)
+    (a, sa), (b, sb) = K.mx4_quantize(x), K.mx4_quantize(w)
+    status = cuda_impl.status_buffer(x.device)
+    torch.cuda.synchronize()
+
+    def call(A, SA, kind, K_, slices, y):
+        return rows(ptr(A.data_ptr()), ptr(SA.data_ptr()), ptr(b.data_ptr()), ptr(sb.data_ptr()), ptr(y.data_ptr()), i64(1), i64(M), i64(N), i64(K_),
+                    i64(0), i64(k), kind, 1, slices, ptr(status.data_ptr()), 148, ptr(0))
+
+    for slices in (1, 2, 4):
+        y = torch.zeros(M, N, device="cuda")
+        assert call(a, sa, 2, 2 * a.shape[1], slices, y) == 0
+        torch.cuda.synchronize()
+        check_product(x, w, y, F32)
+        for kind, v in ((0, x), (1, x.to(BF16))):
+            y = torch.zeros(M, N, device="cuda")
+            assert call(v, v, kind, k, slices, y) == (0 if M <= 16 else 3)
+            torch.cuda.synchronize()
+            check_product(v, w, y, F32) if M <= 16 else None
+    assert call(a, sa, 2, 2 * a.shape[1], 8, y) == 3
