@@ -76,7 +76,7 @@ int apb_mx4_round(const void* x, void* y, long long G, long long R, long long K,
 int apb_mx4_dequantize(const void* codes, const void* scales, void* y, long long G, long long R, long long K, int is_bf16, cudaStream_t st);
 int apb_gemm_mx4(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long kp,
                  int out_fp32, int form, uint32_t* status, int num_sms, cudaStream_t stream);
-int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, int values, int num_sms);
+int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, long long K, int values, int num_sms);
 int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K,
                       long long gs, long long ld, int x_type, int out_fp32, int slices, uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_gemm_mx4_values_takes(long long G, long long M, long long K, int num_sms);
@@ -979,7 +979,7 @@ Tensor mx4_linear(const Tensor& x_, const Tensor& codes_, const Tensor& scales_,
   const bool empty = c.numel() == 0 || K == 0, bf16 = is_bf16(v.x), fp32 = dtype == at::kFloat;
   const cudaStream_t st = stream();
   uint32_t* status = reinterpret_cast<uint32_t*>(status_of(x_).data_ptr());
-  if (!v.transposed && apb_gemm_mx4_rows_takes(v.G, v.R, N, 1, num_sms())) {  // a few rows are rounded in the product's launch
+  if (!v.transposed && apb_gemm_mx4_rows_takes(v.G, v.R, N, K, 1, num_sms())) {  // a few rows are rounded in the product's launch
     check(apb_gemm_mx4_rows(v.x.data_ptr(), nullptr, codes.data_ptr(), scales.data_ptr(), c.data_ptr(), v.G, v.R, N, K, v.gs, v.ld, bf16, fp32, 0, status,
                             num_sms(), st),
           "apb_gemm_mx4_rows");

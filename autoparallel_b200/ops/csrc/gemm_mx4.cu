@@ -387,7 +387,7 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 
 using namespace apb;
 
-extern "C" int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, int values, int num_sms);
+extern "C" int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, long long K, int values, int num_sms);
 extern "C" int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K,
                                  long long gs, long long ld, int x_type, int out_fp32, int slices, uint32_t* status, int num_sms, cudaStream_t stream);
 extern "C" int apb_gemm_resident_pairs(int num_sms);
@@ -404,7 +404,7 @@ extern "C" int apb_gemm_mx4(const void* A, const void* SA, const void* B, const 
   for (const void* ptr : {A, SA, B, SB, (const void*)C})
     if (reinterpret_cast<uintptr_t>(ptr) & 15) return 3;
   if (kp == 0) return zero_result(C, G * M, N, N, out_fp32, stream);
-  if (form < 0 && apb_gemm_mx4_rows_takes(G, M, N, 0, num_sms))
+  if (form < 0 && apb_gemm_mx4_rows_takes(G, M, N, kp, 0, num_sms))
     return apb_gemm_mx4_rows(A, SA, B, SB, C, G, M, N, kp, 0, 0, 2, out_fp32, 0, status, num_sms, stream);
   // Small tiles where they all run at once: 999 x 1408 x 2048 5.8 us (single 128 x 256 7.4, pairs 7.5), 128 x 4096 x 4096 7.1 (9.7, 9.7); otherwise pairs
   // (8192 x 8192 x 8192 178 us, single 128 x 256 237, 128 x 128 257; 2048 x 4096 x 4096 17.4, 18.9, 22.0), or 128 x 256 where a pair's second half

@@ -347,6 +347,9 @@ using namespace apb;
 
 extern "C" int apb_gemm_get_reserved_sms();
 
+// CTAs that are there at once: two to an SM.
+static long long mx_rows_resident(int num_sms) { return 2ll * std::max(1, num_sms - apb_gemm_get_reserved_sms()); }
+
 // Slices of K for a product of ``tiles`` tiles of 128 rows of B: as many as are resident at once, each with a stage at least.
 static int mx_rows_slices(long long tiles, int num_kb, long long resident) {
   int s = 1;
@@ -358,13 +361,16 @@ static int mx_rows_slices(long long tiles, int num_kb, long long resident) {
 //   codes                  this kernel / the persistent ones of gemm_mx4.cu: 64 experts of 1408 x 2048 2 rows 19.3 / 20.9, 16 rows 20.0 / 21.6, 32 rows 20.4 / 22.1;
 //                          16 of 4096 x 4096 26.5 / 29.0 (8 rows); 128 of 768 x 2048 21.0 / 22.5; 16 x 14336 x 4096 10.9, in L2 8.6 / 10.1; 32 x 40000 x 4096
 //                          21.7 / 25.7; 32 x 128256 x 4096 49.6 / 56.7; in L2 17 x 4096 x 14336 9.4 / 15.3, 32 x 4096 x 4096 7.1 / 9.6
-//   values, rounded here   this kernel / a launch that rounds A and the codes: every CTA rounds all of A's slice, so more rows are better rounded once.  1 x
-//                          14336 x 4096 10.0 / 12.1, 8 rows 12.4 / 12.4, 16 14.4 / 10.1 (in L2); 64 experts 1 row 19.2 / 22.7, 4 rows 19.7 / 23.1, 8 24.5 /
-//                          23.1, 16 34.8 / 23.9; 8 x 40000 x 4096 27.4 / 22.7, 8 x 1024 x 1024 5.5 / 6.3
-extern "C" int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, int values, int num_sms) {
-  const long long tiles = G * ((N + 127) / 128);
-  if (values) return M <= 4 || (M <= 8 && tiles <= 2 * num_sms);
-  return M <= 32;
+//   values, rounded here   this kernel / a launch that rounds A and the codes.  Every CTA rounds all rows of its slices of A, so more rows, and more blocks of K
+//                          a CTA, are better rounded once.  Up to 4 rows (in L2, from memory): 1 x 14336 x 4096 7.3 / 9.3, 9.5 / 10.9, 4 rows 8.4 / 9.9, 9.9 / 11.0;
+//                          4 x 4096 x 14336 9.3 / 9.7, 10.2 / 11.6; 64 experts of 1408 x 2048, 4 rows, 15.1 / 16.6, 18.1 / 21.2.  8 rows with 4 blocks a CTA or
+//                          fewer: 4096 x 4096 6.2 / 6.6, 6.8 / 7.6; 14336 x 2048 7.5 / 7.5, 8.5 / 9.6; 8 experts of 4096 x 1024 5.8 / 5.9, 7.3 / 7.8.  With more:
+//                          4096 x 6144 8.3 / 7.1, 9.0 / 8.4; 14336 x 4096 10.6 / 8.8, 11.8 / 11.5; 8 experts of 4096 x 2048 9.0 / 7.2, 10.9 / 10.9.
+//                          (9 of 140 pairs, 5 and 8 rows of 8 to 256 tiles of 2 to 56 blocks, lie on the wrong side, by 5 % at most.)
+extern "C" int apb_gemm_mx4_rows_takes(long long G, long long M, long long N, long long K, int values, int num_sms) {
+  if (!values || M <= 4) return M <= 32;
+  const long long tiles = G * ((N + 127) / 128), resident = mx_rows_resident(num_sms), blocks = (K + MX_BK - 1) / MX_BK;
+  return M <= 8 && tiles <= resident && blocks <= 4 * mx_rows_slices(tiles, (int)blocks, resident);
 }
 
 // A: values [G, M, K] with unit stride along K (x_type 0: fp32, 1: bf16; up to 16 rows, more are rounded before), or codes (x_type 2) with scales SA;
@@ -383,7 +389,7 @@ extern "C" int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, c
   p.M = (int)M, p.N = (int)N, p.K = (int)K, p.tiles = (int)tiles, p.n_tiles = (int)n_tiles;
   p.num_kb = (int)((kp + MX_BK - 1) / MX_BK);
   p.k_steps = (int)((kp + 63) / 64);
-  const long long resident = 2ll * std::max(1, num_sms - apb_gemm_get_reserved_sms());
+  const long long resident = mx_rows_resident(num_sms);
   p.slices = slices > 0 ? slices : mx_rows_slices(tiles, p.num_kb, resident);
   p.div_tiles = FastDiv((uint32_t)n_tiles);
   p.div_blocks = FastDiv((uint32_t)p.num_kb);

@@ -478,3 +478,16 @@ def test_every_number_of_slices(M):
             torch.cuda.synchronize()
             check_product(v, w, y, F32) if M <= 16 else None
     assert call(a, sa, 2, 2 * a.shape[1], 8, y) == 3
+
+
+@pytest.mark.parametrize("E,M,N,k,launches", [(0, 4, 4096, 14336, 1), (0, 5, 4096, 4096, 1), (0, 8, 4096, 4096, 1), (0, 9, 4096, 4096, 2),
+                                              (0, 8, 4096, 6144, 2), (0, 8, 14336, 2048, 1), (0, 8, 14336, 4096, 2), (8, 8, 4096, 1024, 1),
+                                              (8, 8, 4096, 2048, 2), (64, 8, 1408, 1024, 2), (64, 4, 1408, 2048, 1)])
+def test_where_few_rows_are_rounded(kernels, E, M, N, k, launches):
+    """Inside the product's launch, or before it where a CTA would have many blocks of all rows to round; the same bits either way."""
+    lead = (E,) if E else ()
+    x, b = randn(*lead, M, k, seed=1, dtype=BF16), K.mx4_quantize(randn(*lead, N, k, seed=2, dtype=BF16))
+    before = kernels.launch_count
+    y = K.mx4_linear(x, *b)
+    assert kernels.launch_count - before == launches
+    assert torch.equal(y, K.mx4_mm(*K.mx4_quantize(x), *b))
