@@ -2,7 +2,7 @@
 // Semantics in ops/moe_ops.py; everything in fp32, in one pass over the logits.
 //
 // L lanes have a token, V experts each, all in registers; the k best are found by k rounds of "largest, lowest index first".  That takes instructions, and
-// they are the bound, not memory (131072 x 128: 67 % of the issue slots, 13 % of DRAM; backward 52 and 26), so a token has the fewest lanes that hold it.
+// they are the bound, not memory (131072 x 128: 69 % of the issue slots, 13 % of DRAM; backward 52 and 26), so a token has the fewest lanes that hold it.
 //   forward   8192 x 64 bf16, 8 of softmax: 2.6 us, 131072 x 64: 16.3, 131072 x 128, 6, with bias: 27.2 (1.5 TB/s); 16383 x 256 fp32 sigmoid, 8 of the 4 best
 //             of 8 groups, with bias: 21.6, 65536 x 256 bf16 the same way: 50.6, without groups 41.8, without bias 29.5, of softmax 25.0
 //   backward  2.1, 7.9, 15.6 (4.5 TB/s), 8.0, 13.7, 13.8: the scores are computed again from the logits, which the forward would write as 4 bytes an expert

@@ -113,9 +113,11 @@ def _grouped_mm_wgrad(a, b, out_dtype):
 #   idx = the experts with the ``top_k`` largest c, descending; w = s[idx], divided by their sum if ``renormalize``, times ``scale``
 #
 # Everything in fp32.  Ties (of experts, of groups) go to the lower index; a NaN counts as larger than everything.  The bias balances the
-# load: it enters the choice alone and has no gradient.  A row of nothing but -inf (all experts masked), and a sum of chosen sigmoid scores
-# that is zero, give weights and gradients of zero.  (Reference: softmax or sigmoid scores, the bias for the choice and the scale in the
-# router of the DeepSeek-V3 test model, autoparallel/_testing/models/dsv3.py:388-444.)
+# load: it enters the choice alone and has no gradient.  With softmax it is added to the logits, the order of this framework's default
+# router (``models/moe.py``), with sigmoid to the scores; a bias that was balanced on softmax scores, of about 1 / E each, is none for the
+# logits.  A row of nothing but -inf (all experts masked), and a sum of chosen sigmoid scores that is zero, give weights and gradients of
+# zero.  (Reference: sigmoid scores with the bias on them, and the scale, in the router of the DeepSeek-V3 test model,
+# autoparallel/_testing/models/dsv3.py:388-444.  Its softmax form, with the bias on the scores, is not offered.)
 lib.define("moe_route(Tensor logits, Tensor? bias, int top_k, bool sigmoid, int num_groups, int top_groups, bool renormalize, float scale)"
            " -> (Tensor, Tensor)")
 lib.define("moe_route_bwd(Tensor dweights, Tensor logits, Tensor idx, bool sigmoid, bool renormalize, float scale) -> Tensor")
@@ -276,7 +278,8 @@ _ag("grouped_mm", _gmm_bwd, _gmm_setup)
 def moe_route(logits, top_k: int, score: str = "softmax", bias=None, num_groups: int = 1, top_groups: int = 1, renormalize: bool = True,
               scale: float = 1.0):
     """(gate weights [.., top_k] fp32, experts [.., top_k] int64) from router logits [.., E] (bf16 or fp32); ``bias`` [E] fp32 enters the
-    choice alone.  The weights are differentiable with respect to the logits, on CUDA once."""
+    choice alone, added to the logits with softmax and to the scores with sigmoid.  The weights are differentiable with respect to the
+    logits, on CUDA once."""
     E = logits.shape[-1] if logits.ndim else 0
     size = E // num_groups if num_groups > 0 else 0
     # (one test for the calls that are right: this is the path of single tokens)

@@ -22,12 +22,13 @@ Operators (``apb200::``; the functions below them check arguments and fill in de
     mx4_mm(a, sa, b, sb, dtype)                      a [.., M, K] x b [.., N, K] -> [.., M, N], sums in fp32
     mx4_linear(x, codes, scales, dtype)              activations (rounded on the way) by weights held in 4 bits; gradient of ``x``
     mx4_matmul(x, w, trans_b, dtype)                 both operands rounded on the way; gradients of both
-    mx4_mm_values(a, codes, scales, k, dtype)        a [.., N] (16 or 32 bits) by the values [N, k] of codes: gradients of ``x`` above; gradient of ``a``
+    mx4_mm_values(a, codes, scales, k, dtype)        a [.., N] (16 or 32 bits) by the values [N, k] of codes: gradients of ``x`` above; has
+                                                     a gradient of ``a``
 
 The rounding has no useful derivative; gradients go straight through it: with ``q`` for rounding and ``y = q(x) q(w)^T``,
-``dx = dy q(w)`` and ``dw = dy^T q(x)``, products of the framework (``mm_nd``, ``grouped_mm``, ``mm_wgrad``): its own GEMM for bf16 operands, a
-library product, counted as such, for fp32 ones.  ``mx4_linear`` has second derivatives too; on CUDA ``mx4_matmul``, which keeps its operands in 4 bits
-alone, refuses them.
+``dx = dy q(w)`` and ``dw = dy^T q(x)``, products of the framework (``mm_nd``, ``grouped_mm``, ``mm_wgrad``): its own GEMM for bf16
+operands, a library product, counted as such, for fp32 ones.  ``mx4_linear`` has second derivatives too; on CUDA ``mx4_matmul``, which keeps
+its operands in 4 bits alone, refuses them.
 
 The planner shards ``mx4_matmul`` like ``mm_nd`` / ``grouped_mm``; a contraction is split only into whole blocks.  The reference has no
 4-bit formats; its float8 products are the nearest thing (autoparallel/graph_passes/async_tp/asynctp_ops.py:363-393).

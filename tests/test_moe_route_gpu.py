@@ -185,8 +185,8 @@ def test_the_c_entry_refuses_what_it_cannot_take():
     w, idx = torch.full((4, 8), 7.0, device="cuda"), torch.full((4, 8), -7, device="cuda")
 
     def call(x_bytes=0, bias_bytes=0, E=64, k=8):
-        return route(ptr(x.data_ptr() + x_bytes), ptr(bias.data_ptr() + bias_bytes), ptr(w.data_ptr()), ptr(idx.data_ptr()), i64(4), E, k, 1, 1, 1, 1,
-                     ctypes.c_float(1.0), 0, ptr(0))
+        return route(ptr(x.data_ptr() + x_bytes), ptr(bias.data_ptr() + bias_bytes), ptr(w.data_ptr()), ptr(idx.data_ptr()), i64(4), E, k,
+                     1, 1, 1, 1, ctypes.c_float(1.0), 0, ptr(0))
 
     assert call(x_bytes=4) == 3 and call(bias_bytes=4) == 3 and call(bias_bytes=8) == 3 and call(k=33) == 3 and call(E=1025) == 3
     assert (w == 7).all() and (idx == -7).all()  # nothing ran
@@ -212,8 +212,8 @@ LAST_PLACE = [(64, 1), (64, 6), (64, 7), (64, 8), (128, 6), (256, 1), (256, 8), 
 @pytest.mark.parametrize("E,k", LAST_PLACE)
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_the_last_place_among_near_and_equal_values(E, k, score):
-    """The last choice and the best of the rest may be equal where a third expert, with a higher number, is larger by a unit in the last place: several
-    experts a few units apart contend for the last places, below others that are chosen for sure."""
+    """The last choice and the best of the rest may be equal where a third expert, with a higher number, is larger by a unit in the last
+    place: several experts a few units apart contend for the last places, below others that are chosen for sure."""
     g = torch.Generator("cuda").manual_seed(E + k)
     T = 2000
     at = experts_at_random(T, E, k - 1 + 6, g)
@@ -257,8 +257,8 @@ def test_the_last_place_by_hand(E, k, score):
 
 @pytest.mark.parametrize("E,k", [(64, 1), (128, 6), (256, 8), (1024, 10)])
 def test_the_last_place_at_the_ends_of_keys(E, k):
-    """Keys hold the upper bits of a score.  Two scores lie within the error of a fast sigmoid to both sides of a multiple of the lower ones' range, and a
-    smaller one, with a lower number, just below in the same range as the lower of the two."""
+    """Keys hold the upper bits of a score.  Two scores lie within the error of a fast sigmoid to both sides of a multiple of the lower
+    ones' range, and a smaller one, with a lower number, just below in the same range as the lower of the two."""
     g = torch.Generator("cuda").manual_seed(E)
     T, bits = 50000, (E - 1).bit_length()
     unit = 2.0 ** (bits - 24)  # of scores in [0.5, 1)

@@ -439,7 +439,8 @@ def test_gradient_of_products_with_values(lead, m, n, k, dtype):
 
 @pytest.mark.parametrize("wrt", ["x", "w", "dy"])
 def test_second_derivatives_of_matmul_are_refused(wrt):
-    """The operands are kept in 4 bits alone, so the gradients cannot be differentiated: they say so where they are, and are themselves as ever."""
+    """The operands are kept in 4 bits alone, so the gradients cannot be differentiated: they say so where they are, and are themselves as
+    ever."""
     x, w = randn(40, 64).requires_grad_(), randn(32, 64, seed=1).requires_grad_()
     dy = torch.randn(40, 32, device="cuda").requires_grad_()
     y = K.mx4_matmul(x, w)
@@ -453,7 +454,8 @@ def test_second_derivatives_of_matmul_are_refused(wrt):
 
 @pytest.mark.parametrize("M", [1, 3, 16, 17, 32])
 def test_every_number_of_slices(M):
-    """The kernel for few rows with the slices of K that it is told to take, one to four CTAs a cluster, from codes and from values; more are refused."""
+    """The kernel for few rows with the slices of K that it is told to take, one to four CTAs a cluster, from codes and from values; more
+    are refused."""
     from autoparallel_b200.ops import build, cuda_impl
 
     rows, i64, ptr = ctypes.CDLL(build.so_path()).apb_gemm_mx4_rows, ctypes.c_longlong, ctypes.c_void_p
@@ -464,8 +466,8 @@ def test_every_number_of_slices(M):
     torch.cuda.synchronize()
 
     def call(A, SA, kind, K_, slices, y):
-        return rows(ptr(A.data_ptr()), ptr(SA.data_ptr()), ptr(b.data_ptr()), ptr(sb.data_ptr()), ptr(y.data_ptr()), i64(1), i64(M), i64(N), i64(K_),
-                    i64(0), i64(k), kind, 1, slices, ptr(status.data_ptr()), 148, ptr(0))
+        return rows(*[ptr(t.data_ptr()) for t in (A, SA, b, sb, y)], i64(1), i64(M), i64(N), i64(K_), i64(0), i64(k), kind, 1, slices,
+                    ptr(status.data_ptr()), 148, ptr(0))
 
     for slices in (1, 2, 4):
         y = torch.zeros(M, N, device="cuda")
