@@ -523,6 +523,119 @@ Tensor mx4_matmul(DispatchKeySet ks, const Tensor& x, const Tensor& w, bool tran
   return MxMatmul::apply(x, w, trans_b, dtype);
 }
 
+// ---------------------------------------------------------------------------------------------- the feed-forward block
+using Five = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
+using AddNormSig = Triple(const Tensor&, const Tensor&, const Tensor&, double);
+using AddNormBwdSig = Pair(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&);
+using AddNorm8Sig = Five(const Tensor&, const c10::optional<Tensor>&, const Tensor&, double, bool);
+using Mx8ValuesSig = Tensor(const Tensor&, const Tensor&, ScalarType);
+using GatedDgradSig = Pair(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t);
+using GatedDxSig = Tensor(const Tensor&, const Tensor&, const Tensor&);
+using GatedWgradSig = Pair(const Tensor&, const Tensor&, ScalarType);
+using GatedFfnSig = Five(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, int64_t);
+const Op<AddNormSig>& op_add_norm() { APB_OP(o, "add_rms_norm", AddNormSig); return o; }
+const Op<AddNormBwdSig>& op_add_norm_bwd() { APB_OP(o, "add_rms_norm_bwd", AddNormBwdSig); return o; }
+const Op<AddNorm8Sig>& op_add_norm8() { APB_OP(o, "add_rms_norm_fp8", AddNorm8Sig); return o; }
+const Op<Mx8ValuesSig>& op_mx8_values() { APB_OP(o, "mx8_dequantize", Mx8ValuesSig); return o; }
+const Op<GatedDgradSig>& op_gated_dgrad() { APB_OP(o, "gated_dgrad", GatedDgradSig); return o; }
+const Op<GatedDxSig>& op_gated_dx() { APB_OP(o, "gated_dx", GatedDxSig); return o; }
+const Op<GatedWgradSig>& op_gated_wgrad() { APB_OP(o, "gated_wgrad", GatedWgradSig); return o; }
+const Op<GatedFfnSig>& op_gated_ffn() { APB_OP(o, "gated_ffn", GatedFfnSig); return o; }
+
+// (dx, dw) of h and the weight, of whichever of both results have been used.
+Pair add_norm_gradients(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& w, const Tensor& rstd) {
+  if (!dy.defined()) return {dh.detach(), at::zeros_like(w)};
+  return dh.defined() ? op_add_norm_bwd()(dy, dh, h, w, rstd) : op_rms_bwd()(dy, h, w, rstd);
+}
+struct AddNorm : torch::autograd::Function<AddNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& res, const Tensor& w, double eps, Keys k) {
+    auto [y, h, rstd] = op_add_norm().below(k.ks, x, res, w, eps);
+    ctx->save_for_backward({h, w, rstd});
+    ctx->mark_non_differentiable({rstd});
+    ctx->set_materialize_grads(false);
+    return {y, h, rstd};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    if (!g[0].defined() && !g[1].defined()) return variable_list(5);
+    return once("add_rms_norm", {g[0], g[1]}, [&]() -> variable_list {
+      const auto s = ctx->get_saved_variables();
+      auto [dx, dw] = add_norm_gradients(g[0], g[1], s[0], s[1], s[2]);
+      return {dx, dx, dw, Tensor(), Tensor()};
+    });
+  }
+};
+Triple add_rms_norm(DispatchKeySet ks, const Tensor& x, const Tensor& res, const Tensor& w, double eps) {
+  if (!records(x, res, w)) return op_add_norm().below(ks, x, res, w, eps);
+  auto o = AddNorm::apply(x, res, w, eps, Keys{ks});
+  return {o[0], o[1], o[2]};
+}
+struct AddNorm8 : torch::autograd::Function<AddNorm8> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& res, const Tensor& w, double eps, bool keep, Keys k) {
+    auto [y, h, rstd, q, scale] = op_add_norm8().below(k.ks, x, res, w, eps, keep);
+    ctx->save_for_backward({res.has_value() ? h : x, w, rstd});
+    variable_list fixed{rstd, q, scale};
+    if (!keep) fixed.push_back(y);
+    if (!res.has_value()) fixed.push_back(h);
+    ctx->mark_non_differentiable(fixed);
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["res"] = res.has_value();
+    return {y, h, rstd, q, scale};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    if (!g[0].defined() && !g[1].defined()) return variable_list(6);
+    return once("add_rms_norm_fp8", {g[0], g[1]}, [&]() -> variable_list {
+      const auto s = ctx->get_saved_variables();
+      auto [dx, dw] = add_norm_gradients(g[0], g[1], s[0], s[1], s[2]);
+      return {dx, ctx->saved_data["res"].toBool() ? dx : Tensor(), dw, Tensor(), Tensor(), Tensor()};
+    });
+  }
+};
+bool records_optional(const c10::optional<Tensor>& t) { return t.has_value() && records(*t); }
+Five add_rms_norm_fp8(DispatchKeySet ks, const Tensor& x, const c10::optional<Tensor>& res, const Tensor& w, double eps, bool keep) {
+  if (!records(x, w) && !records_optional(res)) return op_add_norm8().below(ks, x, res, w, eps, keep);
+  auto o = AddNorm8::apply(x, res, w, eps, keep, Keys{ks});
+  return {o[0], o[1], o[2], o[3], o[4]};
+}
+
+struct GatedFfn : torch::autograd::Function<GatedFfn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w1, const Tensor& w3, const Tensor& w2, int64_t act, int64_t bits,
+                               Keys k) {
+    auto [y, ab, scales, xq, xs] = op_gated_ffn().below(k.ks, x, w1, w3, w2, act, bits);
+    ctx->save_for_backward({bits == 8 ? Tensor() : x, w1, w3, w2, ab, scales, xq, xs});
+    ctx->mark_non_differentiable({ab, scales, xq, xs});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bits"] = bits;
+    ctx->saved_data["dtype"] = x.scalar_type();
+    return {y, ab, scales, xq, xs};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    if (!g[0].defined()) return variable_list(7);
+    TORCH_CHECK(ctx->saved_data["bits"].toInt() != 0, "gated_ffn: a call that kept nothing has no gradients");
+    return once("gated_ffn", {g[0]}, [&] { return gradients(ctx, g[0]); });
+  }
+  static variable_list gradients(AutogradContext* ctx, const Tensor& dy) {
+    const auto s = ctx->get_saved_variables();
+    const bool of_x = ctx->needs_input_grad(0), of_up = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    auto [dab, h] = op_gated_dgrad()(dy, s[3], s[4], s[5], ctx->saved_data["act"].toInt());
+    Tensor dx, dw1, dw3, dw2;
+    if (ctx->needs_input_grad(3))  // (the products take no matrices without columns)
+      dw2 = dy.numel() && h.numel() ? op_mm_wgrad()(dy, h, s[3].scalar_type()) : at::zeros_like(s[3]);
+    h = Tensor();  // (as large as a projection, and not needed any more)
+    if (of_up) {
+      const Tensor x = ctx->saved_data["bits"].toInt() == 8 ? op_mx8_values()(s[6], s[7], ctx->saved_data["dtype"].toScalarType()) : s[0];
+      std::tie(dw1, dw3) = op_gated_wgrad()(dab, x, s[1].scalar_type());
+    }
+    if (of_x) dx = op_gated_dx()(dab, s[1], s[2]);
+    return {dx, dw1, dw3, dw2, Tensor(), Tensor(), Tensor()};
+  }
+};
+Five gated_ffn(DispatchKeySet ks, const Tensor& x, const Tensor& w1, const Tensor& w3, const Tensor& w2, int64_t act, int64_t bits) {
+  if (!records(x, w1, w3, w2)) return op_gated_ffn().below(ks, x, w1, w3, w2, act, bits);
+  auto o = GatedFfn::apply(x, w1, w3, w2, act, bits, Keys{ks});
+  return {o[0], o[1], o[2], o[3], o[4]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(apb200, AutogradCUDA, m) {
@@ -543,4 +656,7 @@ TORCH_LIBRARY_IMPL(apb200, AutogradCUDA, m) {
   m.impl("mx4_mm_values", mx4_mm_values);
   m.impl("mx4_linear", mx4_linear);
   m.impl("mx4_matmul", mx4_matmul);
+  m.impl("add_rms_norm", add_rms_norm);
+  m.impl("add_rms_norm_fp8", add_rms_norm_fp8);
+  m.impl("gated_ffn", gated_ffn);
 }

@@ -82,6 +82,21 @@ int apb_gemm_mx4_rows(const void* A, const void* SA, const void* B, const void* 
 int apb_gemm_mx4_values_takes(long long G, long long M, long long K, int num_sms);
 int apb_gemm_mx4_values(const void* A, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K, int out_fp32,
                         uint32_t* status, int num_sms, cudaStream_t stream);
+int apb_add_rms_norm(const void* x, const void* res, const void* w, void* h, void* y, float* rstd, void* q, float* scale, long long rows, int D, float eps,
+                     int is_bf16, int num_sms, cudaStream_t st);
+long long apb_add_rms_norm_bwd_workspace(long long rows, int D, int num_sms);
+int apb_add_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dw, float* part, long long rows,
+                         int D, int is_bf16, int num_sms, cudaStream_t st);
+int apb_mx8_quantize(const void* x, void* codes, void* scales, long long R, long long K, int is_bf16, cudaStream_t st);
+int apb_mx8_dequantize(const void* codes, const void* scales, void* y, long long R, long long K, int is_bf16, cudaStream_t st);
+int apb_gated_act(const float* ab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st);
+int apb_gated_act_bwd(const float* dh, const float* ab, void* dab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st);
+int apb_gemm_gated(const void* x, const void* w1, const void* w3, void* h, void* ab, void* scales, int M, int H, int K, long long ldx, long long ldw1,
+                   long long ldw3, int act, uint32_t* status, int num_sms, cudaStream_t stream);
+int apb_gemm_gated_grad(const void* dy, const void* w2, const void* ab, const void* scales, void* dab, void* h, int M, int H, int K, long long ldy,
+                        long long ldw, int act, uint32_t* status, int num_sms, cudaStream_t stream);
+int apb_gemm_dual(const void* a1, const void* a2, const void* b1, const void* b2, void* C, int M, int N, int K, long long lda, long long ldb1, long long ldb2,
+                  long long ldc, uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_symm_header_bytes();
 int apb_symm_wait_probe(const uint32_t* flag, unsigned target, unsigned limit_ms, uint32_t* status, cudaStream_t st);
 int apb_symm_collective(int mode, const unsigned long long* peer_ptrs, int rank, int n, unsigned epoch, const void* src,
@@ -576,17 +591,20 @@ std::map<std::string, std::vector<std::array<int, 3>>> kernel_footprints() {
 enum Entry : int {
   MM_ND, MM_WGRAD, GROUPED_MM, GROUPED_MM_WGRAD, DTYPE_CAST, RMS_NORM, RMS_NORM_BWD, ROPE, SWIGLU, SWIGLU_BWD, CROSS_ENTROPY, CROSS_ENTROPY_BWD,
   EMBEDDING, EMBEDDING_BWD, MOE_SLOTS, MOE_SCATTER, MOE_GATHER, MOE_GATE_GRAD, CAST_MANY, MOE_ROUTE, MOE_ROUTE_BWD, MX4_QUANTIZE, MX4_DEQUANTIZE,
-  MX4_ROUND, MX4_MM, MX4_LINEAR, MX4_MATMUL, MX4_MM_VALUES, NUM_ENTRIES
+  MX4_ROUND, MX4_MM, MX4_LINEAR, MX4_MATMUL, MX4_MM_VALUES, ADD_RMS_NORM, ADD_RMS_NORM_BWD, ADD_RMS_NORM_FP8, MX8_QUANTIZE, MX8_DEQUANTIZE, GATED_MM,
+  GATED_DGRAD, GATED_DX, GATED_WGRAD, GATED_FFN, NUM_ENTRIES
 };
-static_assert(NUM_ENTRIES <= 32, "a bit per entry");
+static_assert(NUM_ENTRIES <= 64, "a bit per entry");
 constexpr const char* ENTRY_NAMES[NUM_ENTRIES] = {
     "mm_nd", "mm_wgrad", "grouped_mm", "grouped_mm_wgrad", "dtype_cast", "rms_norm", "rms_norm_bwd", "rope", "swiglu", "swiglu_bwd", "cross_entropy",
     "cross_entropy_bwd", "embedding", "embedding_bwd", "moe_slots", "moe_scatter", "moe_gather", "moe_gate_grad", "cast_many", "moe_route",
-    "moe_route_bwd", "mx4_quantize", "mx4_dequantize", "mx4_round", "mx4_mm", "mx4_linear", "mx4_matmul", "mx4_mm_values"};
+    "moe_route_bwd", "mx4_quantize", "mx4_dequantize", "mx4_round", "mx4_mm", "mx4_linear", "mx4_matmul", "mx4_mm_values",
+    "add_rms_norm", "add_rms_norm_bwd", "add_rms_norm_fp8", "mx8_quantize", "mx8_dequantize", "gated_mm", "gated_dgrad", "gated_dx", "gated_wgrad",
+    "gated_ffn"};
 struct Native {
   py::object table;  // operator name -> Python function, as it is at the time of a call
   py::object status_buffer;
-  std::atomic<uint32_t> installed{0};  // bit per entry: the table's function is not the one of ops/cuda_impl.py
+  std::atomic<uint64_t> installed{0};  // bit per entry: the table's function is not the one of ops/cuda_impl.py
   bool diag_library_gemm = false, moe_kernels = true;
   std::atomic<bool> shadows{false};  // low-precision copies of parameters may exist: casts ask Python for them
   std::atomic<int64_t> launches{0};
@@ -1078,12 +1096,14 @@ Tensor op_mx4_mm_values(const Tensor& a, const Tensor& codes, const Tensor& scal
   return in_python<Tensor>(MX4_MM_VALUES, a, codes, scales, k, py_dtype(dtype));
 }
 
+#include "binding_ffn.h"
+
 // What register_cuda_impl installed for ``name``: ``on`` if it is not the function that the native entry stands for.
 void native_installed(const std::string& name, bool on) {
   for (int e = 0; e < NUM_ENTRIES; ++e)
     if (name == ENTRY_NAMES[e]) {
-      if (on) native().installed.fetch_or(1u << e, std::memory_order_relaxed);
-      else native().installed.fetch_and(~(1u << e), std::memory_order_relaxed);
+      if (on) native().installed.fetch_or(uint64_t(1) << e, std::memory_order_relaxed);
+      else native().installed.fetch_and(~(uint64_t(1) << e), std::memory_order_relaxed);
     }
 }
 
@@ -1128,6 +1148,16 @@ void register_native(py::dict table, py::object status_buffer, bool diag_library
   lib->impl(ENTRY_NAMES[MX4_LINEAR], op_mx4_linear);
   lib->impl(ENTRY_NAMES[MX4_MATMUL], op_mx4_matmul);
   lib->impl(ENTRY_NAMES[MX4_MM_VALUES], op_mx4_mm_values);
+  lib->impl(ENTRY_NAMES[ADD_RMS_NORM], op_add_rms_norm);
+  lib->impl(ENTRY_NAMES[ADD_RMS_NORM_BWD], op_add_rms_norm_bwd);
+  lib->impl(ENTRY_NAMES[ADD_RMS_NORM_FP8], op_add_rms_norm_fp8);
+  lib->impl(ENTRY_NAMES[MX8_QUANTIZE], op_mx8_quantize);
+  lib->impl(ENTRY_NAMES[MX8_DEQUANTIZE], op_mx8_dequantize);
+  lib->impl(ENTRY_NAMES[GATED_MM], op_gated_mm);
+  lib->impl(ENTRY_NAMES[GATED_DGRAD], op_gated_dgrad);
+  lib->impl(ENTRY_NAMES[GATED_DX], op_gated_dx);
+  lib->impl(ENTRY_NAMES[GATED_WGRAD], op_gated_wgrad);
+  lib->impl(ENTRY_NAMES[GATED_FFN], op_gated_ffn);
 }
 
 }  // namespace
@@ -1204,6 +1234,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mx4_matmul", [](const Tensor& x, const Tensor& w, bool trans_b, bool fp32) {
     return mx4_matmul(x, w, trans_b, fp32 ? at::kFloat : at::kBFloat16);
   });
+  m.def("add_rms_norm", &add_rms_norm);
+  m.def("add_rms_norm_bwd", &add_rms_norm_bwd);
+  m.def("add_rms_norm_fp8", &add_rms_norm_fp8);
+  m.def("mx8_quantize", &mx8_quantize);
+  m.def("mx8_dequantize", [](const Tensor& codes, const Tensor& scales, bool fp32) {
+    return mx8_dequantize(codes, scales, fp32 ? at::kFloat : at::kBFloat16);
+  });
+  m.def("gated_mm", &gated_mm);
+  m.def("gated_dgrad", &gated_dgrad);
+  m.def("gated_dx", &gated_dx);
+  m.def("gated_wgrad", [](const Tensor& dab, const Tensor& x, bool fp32) { return gated_wgrad(dab, x, fp32 ? at::kFloat : at::kBFloat16); });
+  m.def("gated_ffn", &gated_ffn);
   m.def("symm_header_bytes", &symm_header_bytes);
   m.def("symm_wait_probe", &symm_wait_probe);
   m.def("symm_collective", &symm_collective);

@@ -1,0 +1,389 @@
+// The middle of a gated feed-forward block: h = act(a) * b with a = x w1^T and b = x w3^T, and its derivative, as the ends of two products.
+//
+//   forward    both projections come out of one product, a and b of the same column of h in the same thread; h leaves in bf16, and for the backward
+//              pass a and b, in bf16 or as 8-bit codes (mx8.cuh)
+//   backward   dh = dy w2 stays in fp32; da = dh b act'(a) and db = dh act(a) leave in bf16, and h, made again, for the gradient of w2
+//
+// ab, dab [M, 2, H]: a row of a (da), then the same row of b (db), so that one product makes the gradients of both weights.  Codes lie in the same way, the
+// scales are [M, 2, ceil(H / 32)].  H % 8 == 0.
+#pragma once
+#include <type_traits>
+
+#include "mx8.cuh"
+#include "ptx.cuh"
+
+namespace apb {
+
+enum : int { ACT_SILU = 0, ACT_GELU = 1, ACT_GELU_TANH = 2 };
+
+// act(a), and its derivative in ``d``.  Both forms of the sigmoid are relative: x / (1 + exp(-x)) keeps its digits where 1 + tanh would cancel, and
+// erfc keeps them where 1 + erf would.
+template <int ACT>
+__device__ __forceinline__ float act_value(float a, float& d) {
+  if (ACT == ACT_GELU) {
+    const float phi = 0.5f * erfcf(-0.70710678f * a);
+    d = fmaf(a * 0.39894228f, __expf(-0.5f * a * a), phi);
+    return a * phi;
+  }
+  // silu: a s(a); gelu_tanh: a s(2 sqrt(2 / pi) (a + 0.044715 a^3)), s the logistic function
+  float u = a, du = 1.f;
+  if (ACT == ACT_GELU_TANH) {
+    const float a2 = a * a;
+    u = 1.59576912f * a * fmaf(0.044715f, a2, 1.f);
+    du = fmaf(0.21406820f, a2, 1.59576912f);
+  }
+  const float s = __fdividef(1.f, 1.f + __expf(-u));
+  const float v = a * s;
+  d = fmaf(v * (1.f - s), du, s);
+  return v;
+}
+
+struct GatedOut {  // forward
+  __nv_bfloat16* h;
+  void* ab;         // bf16, or codes; null: not kept
+  uint8_t* scales;  // of codes; null: bf16
+  int act;
+};
+struct GatedGrad {  // backward
+  const void* ab;
+  const uint8_t* scales;
+  __nv_bfloat16 *dab, *h;
+  int act;
+};
+
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
+  if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>{});
+  else if (act == ACT_GELU) f(std::integral_constant<int, ACT_GELU>{});
+  else f(std::integral_constant<int, ACT_GELU_TANH>{});
+}
+
+// ---------------------------------------------------------------------------- a warp's 32 rows, 32 columns at a time, a row to a thread
+// Staging in shared memory, 32 rows of 64 bytes: a thread writes or reads its own row, and the warp moves whole rows, four lanes to one.
+__device__ __forceinline__ uint32_t stage64(int row, int unit) { return row * 64 + ((unit ^ (row >> 1 & 3)) << 4); }
+__device__ __forceinline__ void stage_put(uint8_t* stg, int lane, const uint32_t (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stg + stage64(lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+// rows row0 ... of ``dst`` (``ld`` elements apart), columns col ... col + 31 that are inside the matrix
+__device__ __forceinline__ void stage_store(const uint8_t* stg, __nv_bfloat16* dst, long long ld, int row0, int col, int M, int H, int lane) {
+  const int unit = lane & 3, sub = lane >> 2;
+  if (col + unit * 8 >= H) return;
+  __nv_bfloat16* p = dst + (long long)(row0 + sub) * ld + col + unit * 8;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = sub + 8 * j;
+    if (row0 + row < M) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(stg + stage64(row, unit));
+    p += 8 * ld;
+  }
+}
+// the same for codes: rows of 32 bytes, in pieces of 8 (a row of b begins H bytes behind a's, which 8 divides)
+__device__ __forceinline__ uint32_t stage32(int row, int unit) { return row * 32 + ((unit ^ (row >> 2 & 3)) << 3); }
+__device__ __forceinline__ void stage_store8(const uint8_t* stg, uint8_t* dst, long long ld, int row0, int col, int M, int H, int lane) {
+  const int unit = lane & 3, sub = lane >> 2;
+  if (col + unit * 8 >= H) return;
+  uint8_t* p = dst + (long long)(row0 + sub) * ld + col + unit * 8;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = sub + 8 * j;
+    if (row0 + row < M) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(stg + stage32(row, unit));
+    p += 8 * ld;
+  }
+}
+
+__device__ __forceinline__ void pack32(const uint32_t (&r)[32], uint32_t (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+}
+// 32 values of a thread to codes in its row of the staging block; the scale byte
+__device__ __forceinline__ uint32_t codes32(const uint32_t (&r)[32], uint8_t* stg, int lane) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = max(top, r[i] & 0x7fffffffu);
+  const uint32_t byte = mx8_scale_byte(top);
+  const float to_code = mx8_to_code(byte);
+  auto four = [&](int i) {
+    return mx8_codes4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]), to_code);
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(stg + stage32(lane, i)) = make_uint2(four(8 * i), four(8 * i + 4));
+  return byte;
+}
+
+// Forward: columns col ... col + ncols - 1 of h from the accumulators at ``ta`` and ``tb``; ``stg``: 4096 bytes of the warp's own.
+template <typename Release>
+__device__ __forceinline__ void gated_tile(const GatedOut& o, uint8_t* stg, uint32_t ta, uint32_t tb, int row0, int col, int ncols, int M, int H, int lane,
+                                           Release release) {
+  const int used = row0 < M ? min(ncols, H - col) : 0;  // (rows and columns past the matrix are not read)
+  if (used <= 0) {
+    release();
+    return;
+  }
+  const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
+#pragma unroll 1
+  for (int c = 0; c < used; c += 32) {
+    uint32_t a[32], b[32], v[16];
+    tmem_ld_32x32(ta + c, a);
+    tmem_ld_32x32(tb + c, b);
+    tmem_ld_wait_for(a);
+    tmem_ld_wait_for(b);
+    if (c + 32 >= used) release();
+    with_act(o.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float d;
+        const float h0 = act_value<decltype(act)::value>(__uint_as_float(a[2 * i]), d) * __uint_as_float(b[2 * i]);
+        const float h1 = act_value<decltype(act)::value>(__uint_as_float(a[2 * i + 1]), d) * __uint_as_float(b[2 * i + 1]);
+        v[i] = pack_bf16(h0, h1);
+      }
+    });
+    __syncwarp();  // what was there before has been read
+    stage_put(stg, lane, v);
+    if (o.ab != nullptr) {
+      if (o.scales != nullptr) {
+        const uint32_t sa = codes32(a, stg + 2048, lane), sb = codes32(b, stg + 3072, lane);
+        if (row0 + lane < M) {
+          uint8_t* s = o.scales + (long long)(row0 + lane) * 2 * blocks + (col + c) / MX8_BLOCK;
+          s[0] = (uint8_t)sa;
+          s[blocks] = (uint8_t)sb;
+        }
+      } else {
+        pack32(a, v);
+        stage_put(stg + 2048, lane, v);
+      }
+    }
+    __syncwarp();
+    stage_store(stg, o.h, H, row0, col + c, M, H, lane);
+    if (o.ab != nullptr) {
+      if (o.scales != nullptr) {
+        uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab);
+        stage_store8(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);
+        stage_store8(stg + 3072, codes + H, 2ll * H, row0, col + c, M, H, lane);
+      } else {
+        __nv_bfloat16* ab = reinterpret_cast<__nv_bfloat16*>(o.ab);
+        stage_store(stg + 2048, ab, 2ll * H, row0, col + c, M, H, lane);
+        pack32(b, v);
+        __syncwarp();
+        stage_put(stg, lane, v);
+        __syncwarp();
+        stage_store(stg, ab + H, 2ll * H, row0, col + c, M, H, lane);
+      }
+    }
+  }
+}
+
+// The values a and b of a warp's 32 rows and 32 columns on their way from memory: whole rows, four lanes to one; rows and columns past the matrix are zeros.
+template <bool EIGHT>
+struct AbFetch {
+  uint4 a[EIGHT ? 2 : 4], b[EIGHT ? 2 : 4];  // (codes: two pieces of 8 bytes in a vector)
+  uint32_t sa, sb;
+  __device__ __forceinline__ void load(const GatedGrad& g, int row0, int col, int M, int H, int lane) {
+    const int unit = lane & 3, sub = lane >> 2;
+    const bool in = col + unit * 8 < H;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = row0 + sub + 8 * j;
+      const long long at = (long long)row * 2 * H + col + unit * 8;
+      if (EIGHT) {
+        uint2 x = make_uint2(0, 0), y = x;
+        if (in && row < M) {
+          const uint8_t* p = reinterpret_cast<const uint8_t*>(g.ab) + at;
+          x = *reinterpret_cast<const uint2*>(p);
+          y = *reinterpret_cast<const uint2*>(p + H);
+        }
+        (j & 1 ? a[j >> 1].z : a[j >> 1].x) = x.x;
+        (j & 1 ? a[j >> 1].w : a[j >> 1].y) = x.y;
+        (j & 1 ? b[j >> 1].z : b[j >> 1].x) = y.x;
+        (j & 1 ? b[j >> 1].w : b[j >> 1].y) = y.y;
+      } else {
+        a[EIGHT ? 0 : j] = b[EIGHT ? 0 : j] = make_uint4(0, 0, 0, 0);
+        if (in && row < M) {
+          const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(g.ab) + at;
+          a[EIGHT ? 0 : j] = *reinterpret_cast<const uint4*>(p);
+          b[EIGHT ? 0 : j] = *reinterpret_cast<const uint4*>(p + H);
+        }
+      }
+    }
+    if (EIGHT) {
+      sa = sb = MX8_LOWEST;
+      if (row0 + lane < M && col < H) {
+        const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
+        const uint8_t* s = g.scales + (long long)(row0 + lane) * 2 * blocks + col / MX8_BLOCK;
+        sa = s[0];
+        sb = s[blocks];
+      }
+    }
+  }
+  __device__ __forceinline__ void put(uint8_t* stg, int lane) const {
+    const int unit = lane & 3, sub = lane >> 2;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = sub + 8 * j;
+      if (EIGHT) {
+        const uint4 x = a[j >> 1], y = b[j >> 1];
+        *reinterpret_cast<uint2*>(stg + stage32(row, unit)) = j & 1 ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y);
+        *reinterpret_cast<uint2*>(stg + 1024 + stage32(row, unit)) = j & 1 ? make_uint2(y.z, y.w) : make_uint2(y.x, y.y);
+      } else {
+        *reinterpret_cast<uint4*>(stg + stage64(row, unit)) = a[EIGHT ? 0 : j];
+        *reinterpret_cast<uint4*>(stg + 2048 + stage64(row, unit)) = b[EIGHT ? 0 : j];
+      }
+    }
+  }
+};
+
+// da, db and h of one element
+template <int ACT>
+__device__ __forceinline__ void gated_grad(float dh, float a, float b, float& da, float& db, float& h) {
+  float d;
+  const float v = act_value<ACT>(a, d);
+  da = dh * b * d;
+  db = dh * v;
+  h = v * b;
+}
+
+// Backward: columns col ... of dh from the accumulator at ``taddr``.  ``next`` holds the first 32 columns of a and b (loaded while the product was under
+// way), and from then on the block after the one in work.
+template <bool EIGHT, typename Release>
+__device__ __forceinline__ void gated_grad_tile(const GatedGrad& g, AbFetch<EIGHT>& next, uint8_t* stg, uint32_t taddr, int row0, int col, int ncols, int M,
+                                                int H, int lane, Release release) {
+  const int used = row0 < M ? min(ncols, H - col) : 0;
+  if (used <= 0) {
+    release();
+    return;
+  }
+#pragma unroll 1
+  for (int c = 0; c < used; c += 32) {
+    uint32_t r[32], da[16], db[16], h[16];
+    tmem_ld_32x32(taddr + c, r);
+    __syncwarp();
+    next.put(stg, lane);
+    const float va = EIGHT ? mx8_to_value(next.sa) : 1.f, vb = EIGHT ? mx8_to_value(next.sb) : 1.f;
+    if (c + 32 < used) next.load(g, row0, col + c + 32, M, H, lane);
+    __syncwarp();
+    uint32_t a[EIGHT ? 8 : 16], b[EIGHT ? 8 : 16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (EIGHT) {
+        const uint2 x = *reinterpret_cast<const uint2*>(stg + stage32(lane, i)), y = *reinterpret_cast<const uint2*>(stg + 1024 + stage32(lane, i));
+        a[2 * i] = x.x; a[2 * i + 1] = x.y;
+        b[2 * i] = y.x; b[2 * i + 1] = y.y;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(stg + stage64(lane, i)), y = *reinterpret_cast<const uint4*>(stg + 2048 + stage64(lane, i));
+        a[(4 * i) % (EIGHT ? 8 : 16)] = x.x; a[(4 * i + 1) % (EIGHT ? 8 : 16)] = x.y; a[(4 * i + 2) % (EIGHT ? 8 : 16)] = x.z;
+        a[(4 * i + 3) % (EIGHT ? 8 : 16)] = x.w;
+        b[(4 * i) % (EIGHT ? 8 : 16)] = y.x; b[(4 * i + 1) % (EIGHT ? 8 : 16)] = y.y; b[(4 * i + 2) % (EIGHT ? 8 : 16)] = y.z;
+        b[(4 * i + 3) % (EIGHT ? 8 : 16)] = y.w;
+      }
+    }
+    tmem_ld_wait_for(r);
+    if (c + 32 >= used) release();
+    with_act(g.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float a2[2], b2[2], o[3][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (EIGHT) {
+            a2[k] = mx8_value(a[i / 2], 2 * (i & 1) + k, va);
+            b2[k] = mx8_value(b[i / 2], 2 * (i & 1) + k, vb);
+          } else {  // (a bf16 is the upper half of its fp32)
+            a2[k] = __uint_as_float(k ? a[i % (EIGHT ? 8 : 16)] & 0xffff0000u : a[i % (EIGHT ? 8 : 16)] << 16);
+            b2[k] = __uint_as_float(k ? b[i % (EIGHT ? 8 : 16)] & 0xffff0000u : b[i % (EIGHT ? 8 : 16)] << 16);
+          }
+          gated_grad<decltype(act)::value>(__uint_as_float(r[2 * i + k]), a2[k], b2[k], o[0][k], o[1][k], o[2][k]);
+        }
+        da[i] = pack_bf16(o[0][0], o[0][1]);
+        db[i] = pack_bf16(o[1][0], o[1][1]);
+        h[i] = pack_bf16(o[2][0], o[2][1]);
+      }
+    });
+    __syncwarp();
+    stage_put(stg, lane, da);
+    stage_put(stg + 2048, lane, db);
+    __syncwarp();
+    stage_store(stg, g.dab, 2ll * H, row0, col + c, M, H, lane);
+    stage_store(stg + 2048, g.dab + H, 2ll * H, row0, col + c, M, H, lane);
+    __syncwarp();
+    stage_put(stg, lane, h);
+    __syncwarp();
+    stage_store(stg, g.h, H, row0, col + c, M, H, lane);
+  }
+}
+
+// ---------------------------------------------------------------------------- four columns of a row to a thread, eight threads to 32 columns
+__device__ __forceinline__ uint2 pack4(const float (&v)[4]) { return make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); }
+__device__ __forceinline__ void unpack4(uint2 p, float (&v)[4]) {
+  v[0] = __uint_as_float(p.x << 16); v[1] = __uint_as_float(p.x & 0xffff0000u);
+  v[2] = __uint_as_float(p.y << 16); v[3] = __uint_as_float(p.y & 0xffff0000u);
+}
+// The eight threads come together, those with columns past the matrix (whose a and b are zeros) among them.
+__device__ __forceinline__ uint32_t codes4(const float (&v)[4], uint32_t& byte) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  const uint32_t eight = 0xffu << (threadIdx.x & 24);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(eight, top, o));
+  byte = mx8_scale_byte(top);
+  return mx8_codes4(v[0], v[1], v[2], v[3], mx8_to_code(byte));
+}
+__device__ __forceinline__ void gated_four(const GatedOut& o, long long row, int col, int H, const float (&a)[4], const float (&b)[4]) {
+  float h[4];
+  with_act(o.act, [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float d;
+      h[i] = act_value<decltype(act)::value>(a[i], d) * b[i];
+    }
+  });
+  const bool in = col < H;
+  if (in) *reinterpret_cast<uint2*>(o.h + row * H + col) = pack4(h);
+  if (o.ab == nullptr) return;
+  if (o.scales != nullptr) {
+    uint32_t sa, sb;
+    const uint32_t ca = codes4(a, sa), cb = codes4(b, sb);
+    if (!in) return;
+    const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
+    uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab) + row * 2 * H + col;
+    *reinterpret_cast<uint32_t*>(codes) = ca;
+    *reinterpret_cast<uint32_t*>(codes + H) = cb;
+    if (col % MX8_BLOCK == 0) {
+      uint8_t* s = o.scales + row * 2 * blocks + col / MX8_BLOCK;
+      s[0] = (uint8_t)sa;
+      s[blocks] = (uint8_t)sb;
+    }
+  } else if (in) {
+    __nv_bfloat16* ab = reinterpret_cast<__nv_bfloat16*>(o.ab) + row * 2 * H + col;
+    *reinterpret_cast<uint2*>(ab) = pack4(a);
+    *reinterpret_cast<uint2*>(ab + H) = pack4(b);
+  }
+}
+__device__ __forceinline__ void gated_grad_four(const GatedGrad& g, long long row, int col, int H, const float (&dh)[4]) {
+  float a[4], b[4], da[4], db[4], h[4];
+  const long long at = row * 2 * H + col;
+  if (g.scales != nullptr) {
+    const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
+    const uint8_t* s = g.scales + row * 2 * blocks + col / MX8_BLOCK;
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(g.ab) + at;
+    const uint32_t ca = *reinterpret_cast<const uint32_t*>(codes), cb = *reinterpret_cast<const uint32_t*>(codes + H);
+    const float va = mx8_to_value(s[0]), vb = mx8_to_value(s[blocks]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = mx8_value(ca, i, va);
+      b[i] = mx8_value(cb, i, vb);
+    }
+  } else {
+    const __nv_bfloat16* ab = reinterpret_cast<const __nv_bfloat16*>(g.ab) + at;
+    unpack4(*reinterpret_cast<const uint2*>(ab), a);
+    unpack4(*reinterpret_cast<const uint2*>(ab + H), b);
+  }
+  with_act(g.act, [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) gated_grad<decltype(act)::value>(dh[i], a[i], b[i], da[i], db[i], h[i]);
+  });
+  *reinterpret_cast<uint2*>(g.dab + at) = pack4(da);
+  *reinterpret_cast<uint2*>(g.dab + at + H) = pack4(db);
+  *reinterpret_cast<uint2*>(g.h + row * H + col) = pack4(h);
+}
+
+}  // namespace apb

@@ -25,7 +25,10 @@
 //                   rank's staging area in peer memory (16-byte stores over NVLink); the owner
 //                   sums the n slots once every rank has signalled completion
 #pragma once
+#include <type_traits>
+
 #include "footprint.cuh"
+#include "gated.cuh"
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "symm_proto.cuh"
@@ -94,6 +97,38 @@ struct GemmParams {
   int whole_tiles = 0, all_tiles = 0;  // CTA pairs, plain GEMM: tiles that stay whole, and all there are (see set_pair_tiles)
   int vec_store = 0;  // C leaves through shared memory in whole 128-byte lines (plain GEMM; needs 16-byte rows)
 };
+
+// What a product does besides, as the kind of its last argument (plain GEMM body, no grouping):
+//   EXT_NONE   nothing
+//   EXT_GATED  two K-major matrices of weights, whose columns alternate in halves of a column tile: a tile of 256 has 128 columns of both
+//              projections of a gated feed-forward block, and the epilogue makes h of them (gated.cuh).  N counts the columns of both.
+//   EXT_GRAD   the epilogue takes the derivative of that through the result, dh
+//   EXT_DUAL   C = opA * opB + opA2 * opB2 in one accumulation: K counts the blocks of both contractions, in whole blocks of BK
+enum : int { EXT_NONE = 0, EXT_GATED = 1, EXT_GRAD = 2, EXT_DUAL = 3 };
+struct NoExt {
+  static constexpr int KIND = EXT_NONE;
+};
+struct GatedExt {
+  static constexpr int KIND = EXT_GATED;
+  CUtensorMap tmB2;
+  GatedOut out;
+};
+template <bool EIGHT_BITS>
+struct GradExt {
+  static constexpr int KIND = EXT_GRAD;
+  static constexpr bool EIGHT = EIGHT_BITS;
+  GatedGrad grad;
+};
+struct DualExt {
+  static constexpr int KIND = EXT_DUAL;
+  CUtensorMap tmA2, tmB2;
+};
+
+template <typename Ext>
+constexpr bool ext_eight() {
+  if constexpr (Ext::KIND == EXT_GRAD) return Ext::EIGHT;
+  else return false;
+}
 
 struct FuseParams {
   apbs::Peers peers;
@@ -438,9 +473,13 @@ constexpr int TILE_RING = 4;
 // buffer each.  The turns are one k-block long, but WIDE_RUN at the ends of the contraction: the first accumulator is complete that much before
 // the second and is read out meanwhile, and the next tile begins with it.  Runs of 4 / 2 / 1 blocks: 8192 x 128256 x 4096 6129 / 6255 / 6348 us.
 constexpr int WIDE_RUN = 4;  // (stages that the first accumulator takes before the second gives one back: no more than there are)
-template <bool A_MN, bool B_MN, int FUSE, bool PAIR = false, bool GROUPED = false, int ST_ARG = 0, bool DYN = false, bool WIDE = false>
+template <bool A_MN, bool B_MN, int FUSE, bool PAIR = false, bool GROUPED = false, int ST_ARG = 0, bool DYN = false, bool WIDE = false,
+          typename Ext = NoExt>
 __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams& p,
-                                         const FuseParams& f, int cta, int num_ctas, uint8_t* smem_raw) {
+                                         const FuseParams& f, int cta, int num_ctas, uint8_t* smem_raw, const Ext& ext = Ext{}) {
+  constexpr int EXT = Ext::KIND;
+  static_assert(EXT == EXT_NONE || (FUSE == FUSE_NONE && !GROUPED && ST_ARG == 0 && !DYN), "extended products: plain GEMM");
+  static_assert(EXT != EXT_GATED || (!A_MN && !B_MN), "both projections: K-major operands");
   constexpr int STAGING = FUSE == FUSE_NONE && ST_ARG == 0 ? STAGING_BYTES : 0;  // (fewer stages: to leave shared memory free)
   constexpr int EPI = STAGING > 0 ? EPI_WARPS : 4;
   constexpr int EPI_COLS = BN * 4 / EPI;  // columns of the tile per epilogue warp
@@ -692,6 +731,12 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
           // one load helper for the four cases (pair or not, 2-D or grouped 3-D)
           const uint32_t full_addr = full_pair + stage * 8;
           auto load = [&](uint8_t* dst, const CUtensorMap* tm_, int x, int y) {
+            if constexpr (EXT == EXT_DUAL) {  // the second half of the blocks belongs to the second pair of operands
+              if (kb >= num_kb / 2) {
+                tm_ = tm_ == &tmA ? &ext.tmA2 : &ext.tmB2;
+                (A_MN && tm_ == &ext.tmA2) || (B_MN && tm_ == &ext.tmB2) ? y -= num_kb / 2 * BK : x -= num_kb / 2 * BK;
+              }
+            }
             if (PAIR) {
               if (GROUPED) tma_load_3d_pair(dst, tm_, full_addr, x, y, grp);
               else tma_load_2d_pair(dst, tm_, full_addr, x, y);
@@ -711,7 +756,12 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
 #pragma unroll
             for (int c = 0; c < BM / 64; ++c) load(a_dst + c * CHUNK_BYTES, &tmA, m0 + c * 64, kb * BK);
           }
-          if (!B_MN) {
+          if constexpr (EXT == EXT_GATED) {  // columns col / 2 ... of both projections; in a pair each CTA brings in one of them
+            const CUtensorMap* w = PAIR && half ? &ext.tmB2 : &tmB;
+            load(b_dst, w, kb * BK, x.col / 2);
+            if (!PAIR) load(b_dst + B_BYTES / 2, &ext.tmB2, kb * BK, x.col / 2);
+            if (WIDE && rows1 > 0) load(b_dst + SUB_BYTES, w, kb * BK, (x.col + BN) / 2);
+          } else if (!B_MN) {
             load(b_dst, &tmB, kb * BK, n0);
             if (WIDE && rows1 > 0) load(b_dst + SUB_BYTES, &tmB, kb * BK, n1);
           } else {
@@ -849,6 +899,9 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
       for (int sub = 0; sub < (NARROW ? x.subs : 1); ++sub, ++seq) {
         const uint32_t buf = seq & 1u;
         const long long cta_row0 = (long long)x.tm * TM + (long long)half * BM;  // first of this CTA's 128 rows
+        [[maybe_unused]] std::conditional_t<EXT == EXT_GRAD, AbFetch<ext_eight<Ext>()>, int> fetch;
+        if constexpr (EXT == EXT_GRAD)  // (on their way while the product is)
+          fetch.load(ext.grad, (int)cta_row0 + q * 32, x.col + sub * BN + part * (narrow(x, sub) ? EPI_COLS / 2 : EPI_COLS), p.M, p.N, lane);
         // (the TMEM loads are warp-wide: the warp goes on together or not at all)
         if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[buf], seq >> 1 & 1u, abort_flag))) {
           atomicCAS(p.status, 0u, (uint32_t)ST_TIMEOUT_TMEM_FULL);
@@ -889,6 +942,18 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
             else mbar_arrive(&tmem_empty[buf]);
           }
         };
+        if constexpr (EXT == EXT_GATED || EXT == EXT_GRAD) {
+          uint8_t* stg = smem + ST * (A_BYTES + B_BYTES) + (warp - 2) * STORE_BYTES;
+          const int r0 = (int)cta_row0 + q * 32;
+          if constexpr (EXT == EXT_GATED) {  // this warp's columns: the same of both projections
+            const int both = cols / 2, first = part * both;
+            const uint32_t ta = tmem_base + (uint32_t(q * 32) << 16) + buf * BN + first;
+            gated_tile(ext.out, stg, ta, ta + EPI * both / 4, r0, (x.col + sub * BN) / 2 + first, both, p.M, p.N / 2, lane, release);
+          } else {
+            gated_grad_tile<Ext::EIGHT>(ext.grad, fetch, stg, taddr, r0, n0, cols, p.M, p.N, lane, release);
+          }
+          continue;
+        }
         const bool staged = STAGING > 0 && p.vec_store;
         if (staged) {
           uint8_t* stg = smem + ST * (A_BYTES + B_BYTES) + (warp - 2) * STORE_BYTES;

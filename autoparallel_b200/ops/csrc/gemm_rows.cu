@@ -13,6 +13,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
+#include "gated.cuh"
 #include "launch.cuh"
 
 namespace apb {
@@ -30,24 +33,41 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// What becomes of the sums.  ``pair``: of the 16 rows of the operand, 8 are W's and 8 a second matrix's (the two projections of a gated feed-forward block,
+// N columns each).
+struct RowsPlain {
+  static constexpr bool PAIR = false;
+  void* C;
+  long long ldc;
+  int out_fp32;
+};
+struct RowsGated {
+  static constexpr bool PAIR = true;
+  const __nv_bfloat16* W3;
+  long long ldw3;
+  GatedOut out;
+};
+
 // MB: blocks of 8 rows of X; U: steps of 32 elements of K whose loads are under way together
-template <int MB, int U, int MIN_BLOCKS>
-__global__ void __launch_bounds__(32 * ROWS_WARPS, MIN_BLOCKS)
-gemm_rows_kernel(const __nv_bfloat16* X, const __nv_bfloat16* W, void* C, int M, int N, int K, long long ldx,
-                 long long ldw, long long ldc, int out_fp32) {
-  after_previous();
+template <int MB, int U, typename Out>
+__device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bfloat16* W, int M, int N, int K, long long ldx, long long ldw, const Out& out) {
   constexpr int TM = 8 * MB;
   __shared__ float part[ROWS_WARPS][TM * ROWS_TILE];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = (lane & 3) * 8;
-  const int n0 = blockIdx.x * ROWS_TILE;
+  const int n0 = blockIdx.x * (Out::PAIR ? ROWS_TILE / 2 : ROWS_TILE);
   const int steps = (K + 31) / 32, s0 = steps * warp / ROWS_WARPS, s1 = steps * (warp + 1) / ROWS_WARPS;
   const __nv_bfloat16* w[2];
   const __nv_bfloat16* x[MB];
   bool wk[2], xk[MB];  // rows outside the matrices load nothing
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    wk[i] = n0 + g + 8 * i < N;
-    w[i] = W + (wk[i] ? n0 + g + 8 * i : 0) * ldw + c;
+    if constexpr (Out::PAIR) {
+      wk[i] = n0 + g < N;
+      w[i] = (i ? out.W3 : W) + (wk[i] ? n0 + g : 0) * (i ? out.ldw3 : ldw) + c;
+    } else {
+      wk[i] = n0 + g + 8 * i < N;
+      w[i] = W + (wk[i] ? n0 + g + 8 * i : 0) * ldw + c;
+    }
   }
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
@@ -88,16 +108,53 @@ gemm_rows_kernel(const __nv_bfloat16* X, const __nv_bfloat16* W, void* C, int M,
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[warp][(8 * m + m2 + (i & 1)) * ROWS_TILE + g + 8 * (i >> 1)] = acc[m][i];
   __syncthreads();
-  for (int t = threadIdx.x; t < M * ROWS_TILE; t += 32 * ROWS_WARPS) {
-    float v = 0.f;
+  if constexpr (Out::PAIR) {
+    for (int t = threadIdx.x; t < M * (ROWS_TILE / 2); t += 32 * ROWS_WARPS) {
+      const int m = t / (ROWS_TILE / 2), n = n0 + t % (ROWS_TILE / 2), at = m * ROWS_TILE + t % (ROWS_TILE / 2);
+      float a = 0.f, b = 0.f, h = 0.f;
 #pragma unroll
-    for (int i = 0; i < ROWS_WARPS; ++i) v += part[i][t];
-    const int m = t / ROWS_TILE, n = n0 + t % ROWS_TILE;
-    if (n < N) {
-      if (out_fp32) reinterpret_cast<float*>(C)[m * ldc + n] = v;
-      else reinterpret_cast<__nv_bfloat16*>(C)[m * ldc + n] = __float2bfloat16(v);
+      for (int i = 0; i < ROWS_WARPS; ++i) {
+        a += part[i][at];
+        b += part[i][at + ROWS_TILE / 2];
+      }
+      if (n >= N) continue;
+      with_act(out.out.act, [&](auto act) {
+        float d;
+        h = act_value<decltype(act)::value>(a, d) * b;
+      });
+      out.out.h[(long long)m * N + n] = __float2bfloat16(h);
+      if (out.out.ab != nullptr) {
+        __nv_bfloat16* ab = reinterpret_cast<__nv_bfloat16*>(out.out.ab) + 2ll * m * N + n;
+        ab[0] = __float2bfloat16(a);
+        ab[N] = __float2bfloat16(b);
+      }
+    }
+  } else {
+    for (int t = threadIdx.x; t < M * ROWS_TILE; t += 32 * ROWS_WARPS) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < ROWS_WARPS; ++i) v += part[i][t];
+      const int m = t / ROWS_TILE, n = n0 + t % ROWS_TILE;
+      if (n < N) {
+        if (out.out_fp32) reinterpret_cast<float*>(out.C)[m * out.ldc + n] = v;
+        else reinterpret_cast<__nv_bfloat16*>(out.C)[m * out.ldc + n] = __float2bfloat16(v);
+      }
     }
   }
+}
+
+template <int MB, int U, int MIN_BLOCKS>
+__global__ void __launch_bounds__(32 * ROWS_WARPS, MIN_BLOCKS)
+gemm_rows_kernel(const __nv_bfloat16* X, const __nv_bfloat16* W, void* C, int M, int N, int K, long long ldx,
+                 long long ldw, long long ldc, int out_fp32) {
+  after_previous();
+  rows_cta<MB, U>(X, W, M, N, K, ldx, ldw, RowsPlain{C, ldc, out_fp32});
+}
+template <int MB, int U, int MIN_BLOCKS>
+__global__ void __launch_bounds__(32 * ROWS_WARPS, MIN_BLOCKS)
+gemm_rows_gated_kernel(const __nv_bfloat16* X, const __nv_bfloat16* W, int M, int N, int K, long long ldx, long long ldw, const RowsGated out) {
+  after_previous();
+  rows_cta<MB, U>(X, W, M, N, K, ldx, ldw, out);
 }
 
 }  // namespace apb
@@ -138,5 +195,25 @@ extern "C" int apb_gemm_rows(const void* X, const void* W, void* C, int M, int N
   if (M <= 8) deep ? launch(gemm_rows_kernel<1, 4, 1>) : launch(gemm_rows_kernel<1, 3, 2>);
   else if (M <= 16) launch(gemm_rows_kernel<2, 3, 2>);
   else deep ? launch(gemm_rows_kernel<4, 4, 1>) : launch(gemm_rows_kernel<4, 3, 2>);
+  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
+// h[M, H] = act(X W1^T) * (X W3^T) (gated.cuh), and the two products themselves in bf16 where ``ab`` is given.  The rules of the plain product with 2 H
+// columns hold: it reads the same.
+extern "C" int apb_gemm_rows_gated(const void* X, const void* W1, const void* W3, void* h, void* ab, int M, int H, int K, long long ldx, long long ldw1,
+                                   long long ldw3, int act, int num_sms, cudaStream_t st) {
+  if (M <= 0 || H <= 0) return 0;
+  if (M > ROWS_MAX || K <= 0 || (K & 7) || ((ldx | ldw1 | ldw3) & 7) ||
+      ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(W1) | reinterpret_cast<uintptr_t>(W3)) & 15))
+    return 3;
+  const unsigned grid = (unsigned)((H + ROWS_TILE / 2 - 1) / (ROWS_TILE / 2));
+  const RowsGated out{(const __nv_bfloat16*)W3, ldw3, GatedOut{(__nv_bfloat16*)h, ab, nullptr, act}};
+  auto launch = [&](auto kern) {
+    launch_after(kern, grid, 32 * ROWS_WARPS, 0, st, (const __nv_bfloat16*)X, (const __nv_bfloat16*)W1, M, H, K, ldx, ldw1, out);
+  };
+  const bool deep = grid <= (unsigned)num_sms && K >= 2048;
+  if (M <= 8) deep ? launch(gemm_rows_gated_kernel<1, 4, 1>) : launch(gemm_rows_gated_kernel<1, 3, 2>);
+  else if (M <= 16) launch(gemm_rows_gated_kernel<2, 3, 2>);
+  else deep ? launch(gemm_rows_gated_kernel<4, 4, 1>) : launch(gemm_rows_gated_kernel<4, 3, 2>);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }

@@ -360,6 +360,47 @@ def _mx4_mm_values(a, codes, scales, k, out_dtype):
     return out if out.shape[-1] == k else out[..., :k].contiguous()
 
 
+# ----------------------------------------------------------------------------------- the feed-forward block (these count their own launches)
+def _add_rms_norm(x, residual, weight, eps):
+    return _C.add_rms_norm(x, residual, weight, eps)
+
+
+def _add_rms_norm_bwd(dy, dh, h, weight, rstd):
+    return _C.add_rms_norm_bwd(dy, dh, h, weight, rstd)
+
+
+def _add_rms_norm_fp8(x, residual, weight, eps, keep):
+    return _C.add_rms_norm_fp8(x, residual, weight, eps, keep)
+
+
+def _mx8_quantize(x):
+    return _C.mx8_quantize(x)
+
+
+def _mx8_dequantize(codes, scales, dtype):
+    return _C.mx8_dequantize(codes, scales, _fp32_result("mx8_dequantize", dtype))
+
+
+def _gated_mm(x, w1, w3, act, bits):
+    return _C.gated_mm(x, w1, w3, act, bits)
+
+
+def _gated_dgrad(dy, w2, ab, scales, act):
+    return _C.gated_dgrad(dy, w2, ab, scales, act)
+
+
+def _gated_dx(dab, w1, w3):
+    return _C.gated_dx(dab, w1, w3)
+
+
+def _gated_wgrad(dab, x, dtype):
+    return _C.gated_wgrad(dab, x, _fp32_result("gated_wgrad", dtype))
+
+
+def _gated_ffn(x, w1, w3, w2, act, bits):
+    return _C.gated_ffn(x, w1, w3, w2, act, bits)
+
+
 # ----------------------------------------------------------------------------------- pointwise etc.
 def _dtype_cast(x, dtype):
     if x.dtype == dtype:
@@ -543,6 +584,16 @@ def _register() -> None:
     R("mx4_linear", _mx4_linear)
     R("mx4_matmul", _mx4_matmul)
     R("mx4_mm_values", _mx4_mm_values)
+    R("add_rms_norm", _add_rms_norm)
+    R("add_rms_norm_bwd", _add_rms_norm_bwd)
+    R("add_rms_norm_fp8", _add_rms_norm_fp8)
+    R("mx8_quantize", _mx8_quantize)
+    R("mx8_dequantize", _mx8_dequantize)
+    R("gated_mm", _gated_mm)
+    R("gated_dgrad", _gated_dgrad)
+    R("gated_dx", _gated_dx)
+    R("gated_wgrad", _gated_wgrad)
+    R("gated_ffn", _gated_ffn)
     R("dtype_cast", _dtype_cast)
     R("cast_many", _cast_many)
     R("rms_norm", _rms_norm)

@@ -1,0 +1,290 @@
+"""The feed-forward block's operators (ops/ffn_ops.py): formulas, gradients and refusals, on the CPU."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import autoparallel_b200.ops as K
+from autoparallel_b200.ops import ffn_ops as FFN
+from autoparallel_b200.ops.library import ops
+
+ACTS = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh")}
+EPS = {torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24}  # half a step of a rounding, relative
+
+
+def _gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def _randn(*shape, dtype=torch.float32, gen=None):
+    return torch.randn(*shape, generator=gen).to(dtype)
+
+
+def _near(got, want, dtype, roundings):
+    """``roundings`` of the type (and the fp32 arithmetic behind them, sums of a few dozen terms) relative to the result's size."""
+    tol = roundings * EPS[dtype] + 64 * 2.0**-24
+    assert got.dtype == dtype and (got.double() - want).abs().max() <= tol * want.abs().max().clamp_min(1e-30), (got.double() - want).abs().max()
+
+
+# ------------------------------------------------------------------------------------ 8-bit checkpoints
+def _mx8_exact(x):
+    """The definition, block by block in 64 bits: (codes, scale bytes, values)."""
+    *lead, k = x.shape
+    rows = x.double().reshape(math.prod(lead), k)
+    nb = -(-k // 32)
+    codes, byte, values = torch.zeros(rows.shape), torch.zeros(rows.shape[0], nb), torch.zeros(rows.shape, dtype=torch.float64)
+    for r in range(rows.shape[0]):
+        for j in range(nb):
+            v = rows[r, 32 * j:32 * j + 32]
+            if not torch.isfinite(v).all():
+                byte[r, j], values[r, 32 * j:32 * j + 32] = 255, float("nan")
+                continue
+            top = float(v.abs().max())
+            e = -120
+            while e < 127 and 2.0**(e + 1) <= top:
+                e += 1
+            c = torch.clamp(torch.round(v / 2.0**(e - 6)), -127, 127)
+            codes[r, 32 * j:32 * j + 32], byte[r, j], values[r, 32 * j:32 * j + 32] = c, e + 127, c * 2.0**(e - 6)
+    return codes.reshape(x.shape), byte.reshape(*lead, nb), values.reshape(x.shape)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 32), (2, 5, 33), (7, 100), (64,), (0, 40), (3, 0)])
+def test_mx8(shape, dtype):
+    x = _randn(*shape, dtype=dtype, gen=_gen(3)) * 3
+    if x.numel() > 3:
+        x.view(-1)[1] = 0.0
+        x.view(-1)[2] = 63.9 * x.view(-1)[0]
+    codes, scales = K.mx8_quantize(x)
+    c, s, v = _mx8_exact(x)
+    assert codes.shape == x.shape and codes.dtype == torch.int8 and scales.shape == (*shape[:-1], -(-shape[-1] // 32))
+    assert torch.equal(codes.float(), c.float()) and torch.equal(scales.float(), s.float())
+    for t in (torch.bfloat16, torch.float32):
+        assert torch.equal(K.mx8_dequantize(codes, scales, t).double(), v)
+    meta = ops.mx8_quantize(x.to("meta"))
+    assert [tuple(m.shape) for m in meta] == [tuple(codes.shape), tuple(scales.shape)] and [m.dtype for m in meta] == [torch.int8, torch.uint8]
+
+
+def test_mx8_of_extreme_values():
+    big, tiny, inf = torch.finfo(torch.float32).max, 2.0**-126, float("inf")
+    x = torch.zeros(8, 32)
+    x[1, 0], x[1, 1] = big, -big
+    x[2, 0] = tiny
+    x[3, 0] = 2.0**-149
+    x[4, 3] = inf
+    x[5, 4] = float("nan")
+    x[6] = 127.6  # (rounds to 128, which is not held)
+    x[7] = torch.arange(32) / 32.0 * 2.0**-125
+    codes, scales = K.mx8_quantize(x)
+    c, s, v = _mx8_exact(x)
+    assert torch.equal(scales.float(), s)
+    assert torch.equal(codes.float(), c)
+    assert torch.equal(K.mx8_dequantize(codes, scales, torch.float32).double().nan_to_num(nan=7.0), v.nan_to_num(nan=7.0))
+    assert codes[6].eq(127).all() and scales[0].item() == 7
+
+
+# ------------------------------------------------------------------------------------ norm
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 1), (5, 37), (2, 3, 64), (64,), (0, 16)])
+def test_add_rms_norm(shape, dtype):
+    g = _gen(1)
+    x, r, dy, dh = (_randn(*shape, dtype=dtype, gen=g) for _ in range(4))
+    w = _randn(shape[-1], dtype=dtype, gen=g)
+    leaves = [t.clone().requires_grad_() for t in (x, r, w)]
+    y, h = K.add_rms_norm(*leaves, 1e-5)
+    assert torch.equal(h, (x.float() + r.float()).to(dtype))
+    hd, wd = h.detach().double().requires_grad_(), w.double().requires_grad_()
+    yd = hd * torch.rsqrt(hd.pow(2).mean(-1, keepdim=True) + 1e-5) * wd
+    if not x.numel():
+        assert y.shape == x.shape
+        return
+    _near(y, yd.detach(), dtype, 1)
+    assert torch.equal(y, ops.rms_norm(h, w, 1e-5)[0])
+    got = torch.autograd.grad((y, h), leaves, (dy, dh))
+    dx, dw = torch.autograd.grad((yd, hd * 1), (hd, wd), (dy.double(), dh.double()))
+    _near(got[0], dx, dtype, 1)
+    assert torch.equal(got[0], got[1])
+    _near(got[2], dw, dtype, 1)
+
+
+def test_add_rms_norm_where_one_result_is_used():
+    x, r = (_randn(4, 24, gen=_gen(s)).requires_grad_() for s in (1, 2))
+    w = torch.ones(24, requires_grad=True)
+    y, h = K.add_rms_norm(x, r, w)
+    (gx,) = torch.autograd.grad(h.sum(), x)
+    assert torch.equal(gx, torch.ones_like(x))
+    y, h = K.add_rms_norm(x, r, w)
+    got = torch.autograd.grad(y.square().sum(), (x, r, w))
+    s = (x + r).detach().requires_grad_()
+    want = torch.autograd.grad(ops.rms_norm(s, w, 1e-5)[0].square().sum(), (s, w))
+    assert torch.allclose(got[0], want[0], atol=1e-5) and torch.allclose(got[1], want[0], atol=1e-5) and torch.allclose(got[2], want[1], rtol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("residual", [True, False])
+def test_add_rms_norm_fp8(residual, dtype):
+    g = _gen(5)
+    x = _randn(6, 40, dtype=dtype, gen=g)
+    r = _randn(6, 40, dtype=dtype, gen=g) if residual else None
+    x[3] = 0
+    if residual:
+        r[3] = 0
+    w = _randn(40, dtype=dtype, gen=g)
+    y, h, q, scale = K.add_rms_norm_fp8(x, r, w)
+    want_y, want_h = K.add_rms_norm(x, r if residual else torch.zeros_like(x), w)
+    assert torch.equal(y, want_y) and torch.equal(h, want_h) and (residual or h is x)
+    assert q.dtype == torch.float8_e4m3fn and scale.shape == (6, 1) and scale[3].item() == 1.0 and not q[3].float().any()
+    hd = h.double()
+    yd = hd * torch.rsqrt(hd.pow(2).mean(-1, keepdim=True) + 1e-5) * w.double()
+    # half a step of e4m3 (2^-4 relative, 2^-10 in the lowest binade), in units of the scale
+    err = (q.double() * scale.double() - yd).abs()
+    assert (err <= 1.001 * torch.maximum(yd.abs() * 2.0**-4, scale.double() * 2.0**-10)).all()
+    assert ((yd.abs().amax(-1, keepdim=True) / 448 - scale.double()).abs()[:3] <= 2.0**-20 * scale.double()[:3]).all()
+    none = K.add_rms_norm_fp8(x, r, w, keep=False)
+    assert none[0] is None and torch.equal(none[2].float(), q.float()) and torch.equal(none[3], scale) and torch.equal(none[1], h)
+    # the gradient reaches the operands through the 16-bit result
+    leaves = [t.clone().requires_grad_() for t in (x, r, w) if t is not None]
+    y, h, q, scale = K.add_rms_norm_fp8(leaves[0], leaves[1] if residual else None, leaves[-1])
+    assert not q.requires_grad and not scale.requires_grad
+    dy = _randn(6, 40, dtype=dtype, gen=g)
+    got = torch.autograd.grad(y, leaves, dy)
+    h2 = want_h.clone().requires_grad_()
+    w2 = w.clone().requires_grad_()
+    want = torch.autograd.grad(ops.rms_norm(h2, w2, 1e-5)[0], (h2, w2), dy)
+    assert all(torch.equal(a, want[0]) for a in got[:-1]) and torch.equal(got[-1], want[1])
+
+
+# ------------------------------------------------------------------------------------ gated block
+@pytest.mark.parametrize("checkpoint", ["full", "mx8"])
+@pytest.mark.parametrize("act", sorted(ACTS))
+@pytest.mark.parametrize("shape,hidden,out", [((5, 24), 40, 24), ((2, 3, 8), 33, 16), ((1, 1), 1, 1), ((12,), 20, 12)])
+def test_gated_ffn(shape, hidden, out, act, checkpoint):
+    g = _gen(9)
+    x = _randn(*shape, gen=g)
+    w1, w3, w2 = _randn(hidden, shape[-1], gen=g), _randn(hidden, shape[-1], gen=g), _randn(out, hidden, gen=g)
+    dy = _randn(*shape[:-1], out, gen=g)
+    leaves = [t.clone().requires_grad_() for t in (x, w1, w3, w2)]
+    y = K.gated_ffn(*leaves, act=act, checkpoint=checkpoint)
+    d = [t.double() for t in (x, w1, w3, w2)]
+    a, b = d[0] @ d[1].t(), d[0] @ d[2].t()
+    _near(y.detach(), (ACTS[act](a) * b) @ d[3].t(), torch.float32, 2)
+    assert torch.equal(y, K.gated_ffn(x, w1, w3, w2, act=act))
+    got = torch.autograd.grad(y, leaves, dy)
+    # the gradients at what was kept
+    xk = d[0]
+    if checkpoint == "mx8":
+        xk = _mx8_exact(x)[2]
+        _, ab, scales = ops.gated_mm(x, w1, w3, FFN.ACTS[act], 8)
+        a, b = K.mx8_dequantize(ab, scales, torch.float32).double().unbind(-2)
+    a, b = a.detach().requires_grad_(), b.detach().requires_grad_()
+    h = ACTS[act](a) * b
+    da, db = torch.autograd.grad(h, (a, b), dy.double() @ d[3])
+    flat = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
+    want = (da @ d[1] + db @ d[2], flat(da).t() @ flat(xk), flat(db).t() @ flat(xk), flat(dy.double()).t() @ flat(h.detach()))
+    for u, v in zip(got, want):
+        _near(u, v, torch.float32, 4)
+
+
+@pytest.mark.parametrize("act", sorted(ACTS))
+def test_gated_ffn_against_differences(act):
+    g = _gen(11)
+    x, w1, w3, w2 = (_randn(*s, gen=g).requires_grad_() for s in ((4, 8), (12, 8), (12, 8), (6, 12)))
+    d = [t.detach().double() for t in (x, w1, w3, w2)]
+    dy = _randn(4, 6, gen=g)
+    grads = torch.autograd.grad(K.gated_ffn(x, w1, w3, w2, act=act), (x, w1, w3, w2), dy)
+
+    def f(i, t):
+        p = list(d)
+        p[i] = p[i] + t
+        return (((ACTS[act](p[0] @ p[1].t()) * (p[0] @ p[2].t())) @ p[3].t()) * dy.double()).sum()
+
+    for i, grad in enumerate(grads):
+        step = torch.randn(grad.shape, generator=g, dtype=torch.float64)
+        diff = (f(i, 1e-5 * step) - f(i, -1e-5 * step)) / 2e-5
+        # fp32 products of a few dozen terms: 64 roundings of 2^-24 against the sum of magnitudes; differences: 1e-10 of the third derivative
+        assert abs(float((grad.double() * step).sum() - diff)) <= 64 * 2.0**-24 * float((grad.double() * step).abs().sum()) * 4 + 1e-6
+
+
+def test_gated_block_of_nothing():
+    for m, d, h, n in ((0, 8, 16, 8), (3, 0, 16, 8), (3, 8, 0, 8), (3, 8, 16, 0)):
+        x, w1, w3, w2 = (torch.randn(*s).requires_grad_() for s in ((m, d), (h, d), (h, d), (n, h)))
+        for checkpoint in ("full", "mx8"):
+            y = K.gated_ffn(x, w1, w3, w2, checkpoint=checkpoint)
+            assert y.shape == (m, n) and not y.any()
+            for t, g in zip((x, w1, w3, w2), torch.autograd.grad(y.sum(), (x, w1, w3, w2))):
+                assert g.shape == t.shape and not g.any()
+
+
+def test_what_the_backward_pass_keeps():
+    """Bytes held between the passes: x, a and b in their type, or in 33/32 of a byte."""
+    x, w1, w3, w2 = (torch.randn(*s).bfloat16().requires_grad_() for s in ((64, 128), (256, 128), (256, 128), (128, 256)))
+    held = {}
+    for checkpoint in ("full", "mx8"):
+        seen = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t) or t, lambda t: t):
+            K.gated_ffn(x, w1, w3, w2, checkpoint=checkpoint)
+        held[checkpoint] = sum(t.numel() * t.element_size() for t in seen if all(t is not w for w in (w1, w3, w2)))
+    n = 64 * (128 + 2 * 256)
+    assert held == {"full": 2 * n, "mx8": n + n // 32}
+
+
+# ------------------------------------------------------------------------------------ refusals
+def _refused(match, fn, *args, **kw):
+    with pytest.raises(ValueError, match=match):
+        fn(*args, **kw)
+
+
+def test_refusals():
+    x, w = torch.randn(4, 8), torch.ones(8)
+    _refused("not alike", K.add_rms_norm, x, x[:2], w)
+    _refused("not alike", K.add_rms_norm, x, x[0], w)
+    _refused("not alike", K.add_rms_norm, x, x.bfloat16(), w)
+    _refused("expected", K.add_rms_norm, x, x, w[:4])
+    _refused("expected", K.add_rms_norm, x, x, w.half())
+    _refused("bf16 or fp32", K.add_rms_norm, x.half(), x.half(), w)
+    _refused("at most 32768", K.add_rms_norm, torch.zeros(1, 32776), torch.zeros(1, 32776), torch.zeros(32776))
+    _refused("D at least 1", K.add_rms_norm, torch.zeros(2, 0), torch.zeros(2, 0), torch.zeros(0))
+    _refused("different devices", K.add_rms_norm, x, x.to("meta"), w)
+    _refused("leaves out", K.add_rms_norm_fp8, x.clone().requires_grad_(), x, w, keep=False)
+    with torch.no_grad():
+        K.add_rms_norm_fp8(x.clone().requires_grad_(), x, w, keep=False)
+    _refused("bf16 or fp32", K.mx8_quantize, x.double())
+    _refused("no dims", K.mx8_quantize, torch.tensor(1.0))
+    codes, scales = K.mx8_quantize(x)
+    _refused("do not belong", K.mx8_dequantize, codes, scales[:2])
+    _refused("expected, not", K.mx8_dequantize, codes.view(torch.uint8), scales)
+    _refused("not offered", K.mx8_dequantize, codes, scales, torch.float16)
+    w1, w2 = torch.randn(16, 8), torch.randn(8, 16)
+    _refused("act is one of", K.gated_ffn, x, w1, w1, w2, act="relu")
+    _refused("checkpoint is one of", K.gated_ffn, x, w1, w1, w2, checkpoint="fp8")
+    _refused("all bf16 or all fp32", K.gated_ffn, x, w1, w1, w2.bfloat16())
+    _refused("all bf16 or all fp32", K.gated_ffn, x.half(), w1.half(), w1.half(), w2.half())
+    _refused("expected", K.gated_ffn, x, w1, w1[:8], w2)
+    _refused("expected", K.gated_ffn, x, w1, w1, w2.t())
+    _refused("expected", K.gated_ffn, x[:, :4], w1, w1, w2)
+    _refused("expected", K.gated_ffn, torch.tensor(1.0), w1, w1, w2)
+    _refused("different devices", K.gated_ffn, x, w1, w1.to("meta"), w2)
+    y = ops.gated_ffn(x.clone().requires_grad_(), w1, w1, w2, 0, 0)[0]
+    with pytest.raises(RuntimeError, match="kept nothing"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("bits", [0, 8, 16])
+def test_meta_shapes(bits):
+    x, w1, w3, w2 = (torch.randn(*s) for s in ((2, 3, 24), (40, 24), (40, 24), (16, 40)))
+    for name, args in (("gated_mm", (x, w1, w3, 0, bits)), ("gated_ffn", (x, w1, w3, w2, 0, bits)), ("add_rms_norm", (x, x, x[0, 0], 1e-5)),
+                       ("add_rms_norm_fp8", (x, x, x[0, 0], 1e-5, bits > 0)), ("add_rms_norm_fp8", (x, None, x[0, 0], 1e-5, bits > 0))):
+        real = getattr(ops, name)(*args)
+        meta = getattr(ops, name)(*(t.to("meta") if isinstance(t, torch.Tensor) else t for t in args))
+        assert [(tuple(a.shape), a.dtype) for a in real] == [(tuple(a.shape), a.dtype) for a in meta], name
+    if bits:
+        _, ab, scales = ops.gated_mm(x, w1, w3, 0, bits)
+        dy = torch.randn(2, 3, 16)
+        real = ops.gated_dgrad(dy, w2, ab, scales, 0)
+        meta = ops.gated_dgrad(*(t.to("meta") for t in (dy, w2, ab, scales)), 0)
+        assert [(tuple(a.shape), a.dtype) for a in real] == [(tuple(a.shape), a.dtype) for a in meta]
+        dab = real[0]
+        assert ops.gated_dx(dab.to("meta"), w1.to("meta"), w3.to("meta")).shape == ops.gated_dx(dab, w1, w3).shape
+        real, meta = ops.gated_wgrad(dab, x, torch.float32), ops.gated_wgrad(dab.to("meta"), x.to("meta"), torch.float32)
+        assert [tuple(a.shape) for a in real] == [tuple(a.shape) for a in meta]
