@@ -83,8 +83,8 @@ int apb_gemm_mx4_values_takes(long long G, long long M, long long K, int num_sms
 int apb_gemm_mx4_values(const void* A, const void* B, const void* SB, void* C, long long G, long long M, long long N, long long K, int out_fp32,
                         uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_add_rms_norm(const void* x, const void* res, const void* w, void* h, void* y, float* rstd, void* q, float* scale, long long rows, int D, float eps,
-                     int is_bf16, int num_sms, cudaStream_t st);
-long long apb_add_rms_norm_bwd_workspace(long long rows, int D, int num_sms);
+                     int is_bf16, cudaStream_t st);
+long long apb_add_rms_norm_bwd_workspace(long long rows, int D, int is_bf16, int num_sms);
 int apb_add_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dw, float* part, long long rows,
                          int D, int is_bf16, int num_sms, cudaStream_t st);
 int apb_mx8_quantize(const void* x, void* codes, void* scales, long long R, long long K, int is_bf16, cudaStream_t st);

@@ -32,7 +32,7 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& r
   const NormArgs a("add_rms_norm", x, residual, weight);
   Tensor y = at::empty_like(a.x), h = at::empty_like(a.x), rstd = at::empty(lead_of(a.x), a.x.options().dtype(at::kFloat));
   check(apb_add_rms_norm(a.x.data_ptr(), a.res.data_ptr(), a.w.data_ptr(), h.data_ptr(), y.data_ptr(), rstd.data_ptr<float>(), nullptr, nullptr, a.rows,
-                         (int)a.D, (float)eps, is_bf16(a.x), num_sms(), stream()),
+                         (int)a.D, (float)eps, is_bf16(a.x), stream()),
         "apb_add_rms_norm");
   count(a.rows > 0);
   return {y, h, rstd};
@@ -46,7 +46,7 @@ Five add_rms_norm_fp8(const Tensor& x, const c10::optional<Tensor>& residual, co
   Tensor q = at::empty(a.x.sizes(), a.x.options().dtype(at::kFloat8_e4m3fn));
   check(apb_add_rms_norm(a.x.data_ptr(), a.res.defined() ? a.res.data_ptr() : nullptr, a.w.data_ptr(), a.res.defined() ? h.data_ptr() : nullptr,
                          keep ? y.data_ptr() : nullptr, rstd.data_ptr<float>(), q.data_ptr(), scale.data_ptr<float>(), a.rows, (int)a.D, (float)eps,
-                         is_bf16(a.x), num_sms(), stream()),
+                         is_bf16(a.x), stream()),
         "apb_add_rms_norm");
   count(a.rows > 0);
   return {y, h, rstd, q, scale};
@@ -60,7 +60,7 @@ Two add_rms_norm_bwd(const Tensor& dy_, const Tensor& dh_, const Tensor& h_, con
   Tensor dx = at::empty_like(a.x), dw = at::empty({a.D}, a.x.options());
   if (a.rows == 0) return {dx, dw.zero_().to(weight.scalar_type())};
   Tensor dy = dense(dy_), dh = dense(dh_), rstd = rstd_.contiguous();
-  Tensor part = at::empty({(int64_t)apb_add_rms_norm_bwd_workspace(a.rows, (int)a.D, num_sms())}, rstd.options());  // partial sums of dw
+  Tensor part = at::empty({(int64_t)apb_add_rms_norm_bwd_workspace(a.rows, (int)a.D, is_bf16(a.x), num_sms())}, rstd.options());  // partial sums of dw
   check(apb_add_rms_norm_bwd(dy.data_ptr(), dh.data_ptr(), a.x.data_ptr(), a.w.data_ptr(), rstd.data_ptr<float>(), dx.data_ptr(), dw.data_ptr(),
                              part.data_ptr<float>(), a.rows, (int)a.D, is_bf16(a.x), num_sms(), stream()),
         "apb_add_rms_norm_bwd");

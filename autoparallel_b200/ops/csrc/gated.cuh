@@ -16,13 +16,35 @@ namespace apb {
 
 enum : int { ACT_SILU = 0, ACT_GELU = 1, ACT_GELU_TANH = 2 };
 
-// act(a), and its derivative in ``d``.  Both forms of the sigmoid are relative: x / (1 + exp(-x)) keeps its digits where 1 + tanh would cancel, and
-// erfc keeps them where 1 + erf would.
-template <int ACT>
+// Phi(-x) exp(x^2 / 2) for x >= 0, Phi the normal distribution: a polynomial in t = 1 / (1 + 0.275 x) without a constant, as the function falls off like
+// 1 / x.  Fitted to the smallest largest relative error over all x (weighted least squares, the weights moved to where the error is): 2.2e-6.
+__device__ __forceinline__ float normal_tail(float x) {
+  const float t = __fdividef(1.f, fmaf(0.275f, x, 1.f));
+  float p = -0.0552612767f;
+  p = fmaf(p, t, 0.129859090f);
+  p = fmaf(p, t, 0.00389011344f);
+  p = fmaf(p, t, 0.103644602f);
+  p = fmaf(p, t, 0.0981924608f);
+  p = fmaf(p, t, 0.109972589f);
+  p = fmaf(p, t, 0.109701321f);
+  return p * t;
+}
+
+// act(a), and its derivative in ``d``, relative to the value: x / (1 + exp(-x)) keeps its digits where 1 + tanh would cancel, and a tail of the normal
+// distribution those that 1 + erf would lose.  FINE: for fp32 results, to their precision.  By the error function, 8192 x 4096 x 14336 backward: 988 us
+// with erfc, 708 so (one of the sigmoids 708).
+template <int ACT, bool FINE = false>
 __device__ __forceinline__ float act_value(float a, float& d) {
   if (ACT == ACT_GELU) {
-    const float phi = 0.5f * erfcf(-0.70710678f * a);
-    d = fmaf(a * 0.39894228f, __expf(-0.5f * a * a), phi);
+    const float e = __expf(-0.5f * a * a);
+    float phi;
+    if (FINE) {
+      phi = 0.5f * erfcf(-0.70710678f * a);
+    } else {
+      phi = e * normal_tail(fabsf(a));
+      phi = a > 0.f ? 1.f - phi : phi;
+    }
+    d = fmaf(a * 0.39894228f, e, phi);
     return a * phi;
   }
   // silu: a s(a); gelu_tanh: a s(2 sqrt(2 / pi) (a + 0.044715 a^3)), s the logistic function
@@ -91,22 +113,26 @@ __device__ __forceinline__ void stage_store8(const uint8_t* stg, uint8_t* dst, l
   }
 }
 
+__device__ __forceinline__ void unpack8(const uint4& v, float* f) {  // (a bf16 is the upper half of its fp32)
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
 __device__ __forceinline__ void pack32(const uint32_t (&r)[32], uint32_t (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
 // 32 values of a thread to codes in its row of the staging block; the scale byte
 __device__ __forceinline__ uint32_t codes32(const uint32_t (&r)[32], uint8_t* stg, int lane) {
-  uint32_t top = 0;
+  const uint32_t byte = mx8_scale_byte(mx8_top(r));
+  const Mx8Coder coder(byte, mx8_top(r));
 #pragma unroll
-  for (int i = 0; i < 32; ++i) top = max(top, r[i] & 0x7fffffffu);
-  const uint32_t byte = mx8_scale_byte(top);
-  const float to_code = mx8_to_code(byte);
-  auto four = [&](int i) {
-    return mx8_codes4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]), to_code);
-  };
-#pragma unroll
-  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint2*>(stg + stage32(lane, i)) = make_uint2(four(8 * i), four(8 * i + 4));
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<uint2*>(stg + stage32(lane, i)) =
+        make_uint2(coder.four(r[8 * i], r[8 * i + 1], r[8 * i + 2], r[8 * i + 3]), coder.four(r[8 * i + 4], r[8 * i + 5], r[8 * i + 6], r[8 * i + 7]));
   return byte;
 }
 
@@ -172,36 +198,35 @@ __device__ __forceinline__ void gated_tile(const GatedOut& o, uint8_t* stg, uint
   }
 }
 
-// The values a and b of a warp's 32 rows and 32 columns on their way from memory: whole rows, four lanes to one; rows and columns past the matrix are zeros.
+// The values a and b of a warp's 32 rows and 32 columns, on their way from memory to its staging block while the product is under way: whole rows, four
+// lanes to one; rows and columns past the matrix are zeros.  bf16: a's 32 x 64 bytes, then b's; codes: 32 x 32 bytes each.
+__device__ __forceinline__ void copy_async16(uint8_t* dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async8(uint8_t* dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <bool EIGHT>
 struct AbFetch {
-  uint4 a[EIGHT ? 2 : 4], b[EIGHT ? 2 : 4];  // (codes: two pieces of 8 bytes in a vector)
-  uint32_t sa, sb;
-  __device__ __forceinline__ void load(const GatedGrad& g, int row0, int col, int M, int H, int lane) {
+  uint32_t sa, sb;  // scale bytes of this thread's row
+  __device__ __forceinline__ void start(const GatedGrad& g, uint8_t* stg, int row0, int col, int M, int H, int lane) {
     const int unit = lane & 3, sub = lane >> 2;
     const bool in = col + unit * 8 < H;
+    const uint8_t* ab = reinterpret_cast<const uint8_t*>(g.ab);
+    constexpr int SIZE = EIGHT ? 1 : 2;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int row = row0 + sub + 8 * j;
-      const long long at = (long long)row * 2 * H + col + unit * 8;
+      const int row = sub + 8 * j;
+      const bool ok = in && row0 + row < M;
+      const uint8_t* src = ab + (ok ? (long long)(row0 + row) * 2 * H + col + unit * 8 : 0) * SIZE;  // (not read where it is not inside)
+      const long long b = ok ? (long long)H * SIZE : 0;
       if (EIGHT) {
-        uint2 x = make_uint2(0, 0), y = x;
-        if (in && row < M) {
-          const uint8_t* p = reinterpret_cast<const uint8_t*>(g.ab) + at;
-          x = *reinterpret_cast<const uint2*>(p);
-          y = *reinterpret_cast<const uint2*>(p + H);
-        }
-        (j & 1 ? a[j >> 1].z : a[j >> 1].x) = x.x;
-        (j & 1 ? a[j >> 1].w : a[j >> 1].y) = x.y;
-        (j & 1 ? b[j >> 1].z : b[j >> 1].x) = y.x;
-        (j & 1 ? b[j >> 1].w : b[j >> 1].y) = y.y;
+        copy_async8(stg + stage32(row, unit), src, ok);
+        copy_async8(stg + 1024 + stage32(row, unit), src + b, ok);
       } else {
-        a[EIGHT ? 0 : j] = b[EIGHT ? 0 : j] = make_uint4(0, 0, 0, 0);
-        if (in && row < M) {
-          const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(g.ab) + at;
-          a[EIGHT ? 0 : j] = *reinterpret_cast<const uint4*>(p);
-          b[EIGHT ? 0 : j] = *reinterpret_cast<const uint4*>(p + H);
-        }
+        copy_async16(stg + stage64(row, unit), src, ok);
+        copy_async16(stg + 2048 + stage64(row, unit), src + b, ok);
       }
     }
     if (EIGHT) {
@@ -214,92 +239,73 @@ struct AbFetch {
       }
     }
   }
-  __device__ __forceinline__ void put(uint8_t* stg, int lane) const {
-    const int unit = lane & 3, sub = lane >> 2;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = sub + 8 * j;
-      if (EIGHT) {
-        const uint4 x = a[j >> 1], y = b[j >> 1];
-        *reinterpret_cast<uint2*>(stg + stage32(row, unit)) = j & 1 ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y);
-        *reinterpret_cast<uint2*>(stg + 1024 + stage32(row, unit)) = j & 1 ? make_uint2(y.z, y.w) : make_uint2(y.x, y.y);
-      } else {
-        *reinterpret_cast<uint4*>(stg + stage64(row, unit)) = a[EIGHT ? 0 : j];
-        *reinterpret_cast<uint4*>(stg + 2048 + stage64(row, unit)) = b[EIGHT ? 0 : j];
-      }
-    }
-  }
 };
 
 // da, db and h of one element
-template <int ACT>
+template <int ACT, bool FINE = false>
 __device__ __forceinline__ void gated_grad(float dh, float a, float b, float& da, float& db, float& h) {
   float d;
-  const float v = act_value<ACT>(a, d);
+  const float v = act_value<ACT, FINE>(a, d);
   da = dh * b * d;
   db = dh * v;
   h = v * b;
 }
 
-// Backward: columns col ... of dh from the accumulator at ``taddr``.  ``next`` holds the first 32 columns of a and b (loaded while the product was under
-// way), and from then on the block after the one in work.
+// Backward: columns col ... of dh from the accumulator at ``taddr``.  ``fetch`` has started to bring the first 32 columns of a and b into ``stg``.
 template <bool EIGHT, typename Release>
-__device__ __forceinline__ void gated_grad_tile(const GatedGrad& g, AbFetch<EIGHT>& next, uint8_t* stg, uint32_t taddr, int row0, int col, int ncols, int M,
+__device__ __forceinline__ void gated_grad_tile(const GatedGrad& g, AbFetch<EIGHT>& fetch, uint8_t* stg, uint32_t taddr, int row0, int col, int ncols, int M,
                                                 int H, int lane, Release release) {
   const int used = row0 < M ? min(ncols, H - col) : 0;
+  copy_async_wait();
   if (used <= 0) {
     release();
     return;
   }
 #pragma unroll 1
   for (int c = 0; c < used; c += 32) {
-    uint32_t r[32], da[16], db[16], h[16];
+    uint32_t r[32], h[16];
     tmem_ld_32x32(taddr + c, r);
+    copy_async_wait();
     __syncwarp();
-    next.put(stg, lane);
-    const float va = EIGHT ? mx8_to_value(next.sa) : 1.f, vb = EIGHT ? mx8_to_value(next.sb) : 1.f;
-    if (c + 32 < used) next.load(g, row0, col + c + 32, M, H, lane);
-    __syncwarp();
-    uint32_t a[EIGHT ? 8 : 16], b[EIGHT ? 8 : 16];
+    uint2 ca[EIGHT ? 4 : 1], cb[EIGHT ? 4 : 1];
+    Mx8Reader ra, rb;
+    if (EIGHT) {  // (this thread's codes, before da and db take their place)
+      ra = Mx8Reader(fetch.sa);
+      rb = Mx8Reader(fetch.sb);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (EIGHT) {
-        const uint2 x = *reinterpret_cast<const uint2*>(stg + stage32(lane, i)), y = *reinterpret_cast<const uint2*>(stg + 1024 + stage32(lane, i));
-        a[2 * i] = x.x; a[2 * i + 1] = x.y;
-        b[2 * i] = y.x; b[2 * i + 1] = y.y;
-      } else {
-        const uint4 x = *reinterpret_cast<const uint4*>(stg + stage64(lane, i)), y = *reinterpret_cast<const uint4*>(stg + 2048 + stage64(lane, i));
-        a[(4 * i) % (EIGHT ? 8 : 16)] = x.x; a[(4 * i + 1) % (EIGHT ? 8 : 16)] = x.y; a[(4 * i + 2) % (EIGHT ? 8 : 16)] = x.z;
-        a[(4 * i + 3) % (EIGHT ? 8 : 16)] = x.w;
-        b[(4 * i) % (EIGHT ? 8 : 16)] = y.x; b[(4 * i + 1) % (EIGHT ? 8 : 16)] = y.y; b[(4 * i + 2) % (EIGHT ? 8 : 16)] = y.z;
-        b[(4 * i + 3) % (EIGHT ? 8 : 16)] = y.w;
+      for (int i = 0; i < 4; ++i) {
+        ca[i % (EIGHT ? 4 : 1)] = *reinterpret_cast<const uint2*>(stg + stage32(lane, i));
+        cb[i % (EIGHT ? 4 : 1)] = *reinterpret_cast<const uint2*>(stg + 1024 + stage32(lane, i));
       }
+      __syncwarp();
     }
     tmem_ld_wait_for(r);
     if (c + 32 >= used) release();
     with_act(g.act, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float a2[2], b2[2], o[3][2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (EIGHT) {
-            a2[k] = mx8_value(a[i / 2], 2 * (i & 1) + k, va);
-            b2[k] = mx8_value(b[i / 2], 2 * (i & 1) + k, vb);
-          } else {  // (a bf16 is the upper half of its fp32)
-            a2[k] = __uint_as_float(k ? a[i % (EIGHT ? 8 : 16)] & 0xffff0000u : a[i % (EIGHT ? 8 : 16)] << 16);
-            b2[k] = __uint_as_float(k ? b[i % (EIGHT ? 8 : 16)] & 0xffff0000u : b[i % (EIGHT ? 8 : 16)] << 16);
-          }
-          gated_grad<decltype(act)::value>(__uint_as_float(r[2 * i + k]), a2[k], b2[k], o[0][k], o[1][k], o[2][k]);
+      for (int i = 0; i < 4; ++i) {  // eight columns at a time, in this thread's row: a and b out, da and db into their place
+        uint4* pa = reinterpret_cast<uint4*>(stg + stage64(lane, i));
+        uint4* pb = reinterpret_cast<uint4*>(stg + 2048 + stage64(lane, i));
+        float a[8], b[8];
+        if (EIGHT) {
+          ra.four(ca[i % (EIGHT ? 4 : 1)].x, a);
+          ra.four(ca[i % (EIGHT ? 4 : 1)].y, a + 4);
+          rb.four(cb[i % (EIGHT ? 4 : 1)].x, b);
+          rb.four(cb[i % (EIGHT ? 4 : 1)].y, b + 4);
+        } else {
+          const uint4 x = *pa, y = *pb;
+          unpack8(x, a);
+          unpack8(y, b);
         }
-        da[i] = pack_bf16(o[0][0], o[0][1]);
-        db[i] = pack_bf16(o[1][0], o[1][1]);
-        h[i] = pack_bf16(o[2][0], o[2][1]);
+        float da[8], db[8], v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) gated_grad<decltype(act)::value>(__uint_as_float(r[8 * i + k]), a[k], b[k], da[k], db[k], v[k]);
+        *pa = make_uint4(pack_bf16(da[0], da[1]), pack_bf16(da[2], da[3]), pack_bf16(da[4], da[5]), pack_bf16(da[6], da[7]));
+        *pb = make_uint4(pack_bf16(db[0], db[1]), pack_bf16(db[2], db[3]), pack_bf16(db[4], db[5]), pack_bf16(db[6], db[7]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[4 * i + k] = pack_bf16(v[2 * k], v[2 * k + 1]);
       }
     });
-    __syncwarp();
-    stage_put(stg, lane, da);
-    stage_put(stg + 2048, lane, db);
     __syncwarp();
     stage_store(stg, g.dab, 2ll * H, row0, col + c, M, H, lane);
     stage_store(stg + 2048, g.dab + H, 2ll * H, row0, col + c, M, H, lane);
@@ -307,6 +313,8 @@ __device__ __forceinline__ void gated_grad_tile(const GatedGrad& g, AbFetch<EIGH
     stage_put(stg, lane, h);
     __syncwarp();
     stage_store(stg, g.h, H, row0, col + c, M, H, lane);
+    __syncwarp();
+    if (c + 32 < used) fetch.start(g, stg, row0, col + c + 32, M, H, lane);
   }
 }
 
@@ -325,7 +333,7 @@ __device__ __forceinline__ uint32_t codes4(const float (&v)[4], uint32_t& byte) 
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(eight, top, o));
   byte = mx8_scale_byte(top);
-  return mx8_codes4(v[0], v[1], v[2], v[3], mx8_to_code(byte));
+  return Mx8Coder(byte, top).four(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
 }
 __device__ __forceinline__ void gated_four(const GatedOut& o, long long row, int col, int H, const float (&a)[4], const float (&b)[4]) {
   float h[4];
@@ -358,24 +366,38 @@ __device__ __forceinline__ void gated_four(const GatedOut& o, long long row, int
     *reinterpret_cast<uint2*>(ab + H) = pack4(b);
   }
 }
-__device__ __forceinline__ void gated_grad_four(const GatedGrad& g, long long row, int col, int H, const float (&dh)[4]) {
+// a and b of four columns as they lie in memory (codes: .x), and the scale bytes
+struct AbFour {
+  uint2 a, b;
+  uint32_t sa, sb;
+  template <bool EIGHT>
+  __device__ __forceinline__ void load(const GatedGrad& g, long long row, int col, int H) {
+    const long long at = row * 2 * H + col;
+    if (EIGHT) {
+      const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
+      const uint8_t* s = g.scales + row * 2 * blocks + col / MX8_BLOCK;
+      const uint8_t* codes = reinterpret_cast<const uint8_t*>(g.ab) + at;
+      a.x = *reinterpret_cast<const uint32_t*>(codes);
+      b.x = *reinterpret_cast<const uint32_t*>(codes + H);
+      sa = s[0];
+      sb = s[blocks];
+    } else {
+      const __nv_bfloat16* ab = reinterpret_cast<const __nv_bfloat16*>(g.ab) + at;
+      a = *reinterpret_cast<const uint2*>(ab);
+      b = *reinterpret_cast<const uint2*>(ab + H);
+    }
+  }
+};
+template <bool EIGHT>
+__device__ __forceinline__ void gated_grad_four(const GatedGrad& g, const AbFour& ab, long long row, int col, int H, const float (&dh)[4]) {
   float a[4], b[4], da[4], db[4], h[4];
   const long long at = row * 2 * H + col;
-  if (g.scales != nullptr) {
-    const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
-    const uint8_t* s = g.scales + row * 2 * blocks + col / MX8_BLOCK;
-    const uint8_t* codes = reinterpret_cast<const uint8_t*>(g.ab) + at;
-    const uint32_t ca = *reinterpret_cast<const uint32_t*>(codes), cb = *reinterpret_cast<const uint32_t*>(codes + H);
-    const float va = mx8_to_value(s[0]), vb = mx8_to_value(s[blocks]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = mx8_value(ca, i, va);
-      b[i] = mx8_value(cb, i, vb);
-    }
+  if (EIGHT) {
+    Mx8Reader(ab.sa).four(ab.a.x, a);
+    Mx8Reader(ab.sb).four(ab.b.x, b);
   } else {
-    const __nv_bfloat16* ab = reinterpret_cast<const __nv_bfloat16*>(g.ab) + at;
-    unpack4(*reinterpret_cast<const uint2*>(ab), a);
-    unpack4(*reinterpret_cast<const uint2*>(ab + H), b);
+    unpack4(ab.a, a);
+    unpack4(ab.b, b);
   }
   with_act(g.act, [&](auto act) {
 #pragma unroll

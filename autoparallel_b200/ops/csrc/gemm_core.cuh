@@ -473,13 +473,13 @@ constexpr int TILE_RING = 4;
 // buffer each.  The turns are one k-block long, but WIDE_RUN at the ends of the contraction: the first accumulator is complete that much before
 // the second and is read out meanwhile, and the next tile begins with it.  Runs of 4 / 2 / 1 blocks: 8192 x 128256 x 4096 6129 / 6255 / 6348 us.
 constexpr int WIDE_RUN = 4;  // (stages that the first accumulator takes before the second gives one back: no more than there are)
-template <bool A_MN, bool B_MN, int FUSE, bool PAIR = false, bool GROUPED = false, int ST_ARG = 0, bool DYN = false, bool WIDE = false,
-          typename Ext = NoExt>
+template <bool A_MN, bool B_MN, int FUSE, bool PAIR = false, bool GROUPED = false, int ST_ARG = 0, bool DYN = false, bool WIDE = false, typename Ext = NoExt>
 __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorMap& tmB, const GemmParams& p,
                                          const FuseParams& f, int cta, int num_ctas, uint8_t* smem_raw, const Ext& ext = Ext{}) {
   constexpr int EXT = Ext::KIND;
   static_assert(EXT == EXT_NONE || (FUSE == FUSE_NONE && !GROUPED && ST_ARG == 0 && !DYN), "extended products: plain GEMM");
   static_assert(EXT != EXT_GATED || (!A_MN && !B_MN), "both projections: K-major operands");
+  static_assert(EXT != EXT_GATED || EPI_WARPS == 8, "two warps to a lane quarter, each half of both projections' columns");
   constexpr int STAGING = FUSE == FUSE_NONE && ST_ARG == 0 ? STAGING_BYTES : 0;  // (fewer stages: to leave shared memory free)
   constexpr int EPI = STAGING > 0 ? EPI_WARPS : 4;
   constexpr int EPI_COLS = BN * 4 / EPI;  // columns of the tile per epilogue warp
@@ -900,8 +900,11 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
         const uint32_t buf = seq & 1u;
         const long long cta_row0 = (long long)x.tm * TM + (long long)half * BM;  // first of this CTA's 128 rows
         [[maybe_unused]] std::conditional_t<EXT == EXT_GRAD, AbFetch<ext_eight<Ext>()>, int> fetch;
-        if constexpr (EXT == EXT_GRAD)  // (on their way while the product is)
-          fetch.load(ext.grad, (int)cta_row0 + q * 32, x.col + sub * BN + part * (narrow(x, sub) ? EPI_COLS / 2 : EPI_COLS), p.M, p.N, lane);
+        [[maybe_unused]] uint8_t* stg = smem + ST * (A_BYTES + B_BYTES) + (warp - 2) * STORE_BYTES;
+        if constexpr (EXT == EXT_GRAD) {  // (on their way while the product is; the warp has read out what was there before)
+          __syncwarp();
+          fetch.start(ext.grad, stg, (int)cta_row0 + q * 32, x.col + sub * BN + part * (narrow(x, sub) ? EPI_COLS / 2 : EPI_COLS), p.M, p.N, lane);
+        }
         // (the TMEM loads are warp-wide: the warp goes on together or not at all)
         if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[buf], seq >> 1 & 1u, abort_flag))) {
           atomicCAS(p.status, 0u, (uint32_t)ST_TIMEOUT_TMEM_FULL);
@@ -943,12 +946,11 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
           }
         };
         if constexpr (EXT == EXT_GATED || EXT == EXT_GRAD) {
-          uint8_t* stg = smem + ST * (A_BYTES + B_BYTES) + (warp - 2) * STORE_BYTES;
           const int r0 = (int)cta_row0 + q * 32;
           if constexpr (EXT == EXT_GATED) {  // this warp's columns: the same of both projections
             const int both = cols / 2, first = part * both;
             const uint32_t ta = tmem_base + (uint32_t(q * 32) << 16) + buf * BN + first;
-            gated_tile(ext.out, stg, ta, ta + EPI * both / 4, r0, (x.col + sub * BN) / 2 + first, both, p.M, p.N / 2, lane, release);
+            gated_tile(ext.out, stg, ta, ta + 2 * both, r0, (x.col + sub * BN) / 2 + first, both, p.M, p.N / 2, lane, release);
           } else {
             gated_grad_tile<Ext::EIGHT>(ext.grad, fetch, stg, taddr, r0, n0, cols, p.M, p.N, lane, release);
           }
@@ -956,7 +958,6 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
         }
         const bool staged = STAGING > 0 && p.vec_store;
         if (staged) {
-          uint8_t* stg = smem + ST * (A_BYTES + B_BYTES) + (warp - 2) * STORE_BYTES;
           const long long c_off = GROUPED ? (long long)x.grp * p.M * p.ldc : 0;
           const int r0 = (int)cta_row0 + q * 32;
           if (p.out_fp32) store_tile<true>(reinterpret_cast<float*>(p.C) + c_off, p.ldc, stg, taddr, r0, n0, cols, p.M, p.N, lane, release);
@@ -1027,6 +1028,7 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
         if (!staged) release();
       }
     }
+    if constexpr (EXT == EXT_GRAD) copy_async_wait();  // (a wait that ran out leaves copies under way)
   }
 
   tc_fence_before();

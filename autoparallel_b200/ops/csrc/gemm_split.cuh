@@ -228,11 +228,20 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
     static_assert(RSTEP * VPR == SPLIT_THREADS && VPR % 8 == 0, "whole rows");
     const int c = (threadIdx.x % VPR) * 4, H = EXT == EXT_GATED ? p.N / 2 : p.N, col = (EXT == EXT_GATED ? n0 / 2 : n0) + c;
     const uint32_t src0 = smem_u32(tile) + c * 4;
+    const int first = slice * RSTEP + threadIdx.x / VPR, step = S * RSTEP;
+    auto add = [](float (&a)[4], const float4& x) { a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w; };
+    [[maybe_unused]] AbFour next;  // (backward: a and b of the row after the one in work are under way)
+    if constexpr (EXT == EXT_GRAD) {
+      if (first < rows && col < H) next.template load<Ext::EIGHT>(ext.grad, m0 + first, col, H);
+    }
 #pragma unroll 1
-    for (int r = *abort_flag == 0 ? slice * RSTEP + threadIdx.x / VPR : rows; r < rows; r += S * RSTEP) {
+    for (int r = *abort_flag == 0 ? first : rows; r < rows; r += step) {
       const uint32_t src = src0 + r * (LD * 4);
       float v[4] = {}, w[4] = {};
-      auto add = [](float (&a)[4], const float4& x) { a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w; };
+      [[maybe_unused]] const AbFour ab = next;
+      if constexpr (EXT == EXT_GRAD) {
+        if (r + step < rows && col < H) next.template load<Ext::EIGHT>(ext.grad, m0 + r + step, col, H);
+      }
 #pragma unroll 2
       for (int s = 0; s < S; ++s) {
         const uint32_t from = map_to_cta(src, (uint32_t)s);
@@ -240,8 +249,11 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
         if constexpr (EXT == EXT_GATED) add(w, ld_cluster_f4(from + WIDTH * 4));
         add(v, x);
       }
-      if constexpr (EXT == EXT_GATED) gated_four(ext.out, m0 + r, col, H, v, w);
-      else if (col < H) gated_grad_four(ext.grad, m0 + r, col, H, v);
+      if constexpr (EXT == EXT_GATED) {
+        gated_four(ext.out, m0 + r, col, H, v, w);
+      } else {
+        if (col < H) gated_grad_four<Ext::EIGHT>(ext.grad, ab, m0 + r, col, H, v);
+      }
     }
   } else if (*abort_flag == 0) {
     constexpr int VPR = BN_T / 4, RSTEP = SPLIT_THREADS / VPR;  // threads per row, rows per pass of the CTA

@@ -20,14 +20,47 @@ __device__ __forceinline__ uint32_t mx8_scale_byte(uint32_t top) {
 __device__ __forceinline__ float mx8_to_code(uint32_t byte) { return byte == MX8_NAN ? 0.f : __uint_as_float((260u - byte) << 23); }
 __device__ __forceinline__ float mx8_to_value(uint32_t byte) { return __uint_as_float(byte == MX8_NAN ? 0x7fc00000u : (byte - 6u) << 23); }
 
-// A broken block has codes of zero: zero times an infinity would be a NaN, which converts to zero as well.
-__device__ __forceinline__ uint32_t mx8_code(float v, float to_code) {
-  const int c = __float2int_rn(v * to_code);
-  return (uint32_t)max(-127, min(127, c)) & 255u;
+// Largest magnitude (its bits) of 32 values, of which a NaN is larger than everything.
+__device__ __forceinline__ uint32_t mx8_top(const uint32_t (&r)[32]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(__uint_as_float(r[i]))));
+  return __float_as_uint(top);
 }
-__device__ __forceinline__ uint32_t mx8_codes4(float a, float b, float c, float d, float to_code) {
-  return mx8_code(a, to_code) | mx8_code(b, to_code) << 8 | mx8_code(c, to_code) << 16 | mx8_code(d, to_code) << 24;
-}
-__device__ __forceinline__ float mx8_value(uint32_t word, int i, float to_value) { return (float)(int)(int8_t)(word >> (8 * i)) * to_value; }
+
+// Values of one block to codes.  Added to 1.5 2^23, a number below 2^22 is rounded to a whole one, ties to even, whose lower byte is the code; one addition
+// with the scaling, one byte permutation for two codes.  What rounds to 128 is clamped, and a broken block has codes of zero: ``exact`` says that neither
+// occurs, which is so where the block's largest value does not round to 128.
+struct Mx8Coder {
+  float m;
+  bool exact;
+  __device__ __forceinline__ Mx8Coder(uint32_t byte, uint32_t top) : m(mx8_to_code(byte)), exact(byte != MX8_NAN && (top & 0x7fffffu) < 0x7f0000u) {}
+  __device__ __forceinline__ uint32_t four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
+    constexpr float ROUND = 12582912.f;
+    float f[4] = {__uint_as_float(a), __uint_as_float(b), __uint_as_float(c), __uint_as_float(d)};
+    if (!exact) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = m == 0.f ? 0.f : fminf(127.f, fmaxf(-127.f, f[i] * m));
+    }
+    const float k = exact ? m : 1.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = fmaf(f[i], k, ROUND);
+    const uint32_t lo = __byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040), hi = __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+  }
+};
+
+// Codes of one block to values: with 128 added, a code is the lowest byte of 2^23 + (code + 128) as fp32; one permutation, and a multiplication by the power
+// of two that takes 2^23 + 128 times it off again, exactly.
+struct Mx8Reader {
+  float m, off;
+  Mx8Reader() = default;
+  __device__ __forceinline__ explicit Mx8Reader(uint32_t byte) : m(mx8_to_value(byte)), off(-8388736.f * m) {}
+  __device__ __forceinline__ void four(uint32_t codes, float* f) const {
+    const uint32_t u = codes ^ 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = fmaf(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | i)), m, off);
+  }
+};
 
 }  // namespace apb

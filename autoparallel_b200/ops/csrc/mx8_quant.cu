@@ -33,9 +33,9 @@ __global__ void __launch_bounds__(256) mx8_quantize_kernel(const T* x, uint8_t* 
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   if (!in) return;
   const uint32_t byte = mx8_scale_byte(top);
-  const float m = mx8_to_code(byte);
-  reinterpret_cast<uint4*>(codes)[i] = make_uint4(mx8_codes4(f[0], f[1], f[2], f[3], m), mx8_codes4(f[4], f[5], f[6], f[7], m),
-                                                  mx8_codes4(f[8], f[9], f[10], f[11], m), mx8_codes4(f[12], f[13], f[14], f[15], m));
+  const Mx8Coder coder(byte, top);
+  auto four = [&](int k) { return coder.four(__float_as_uint(f[k]), __float_as_uint(f[k + 1]), __float_as_uint(f[k + 2]), __float_as_uint(f[k + 3])); };
+  reinterpret_cast<uint4*>(codes)[i] = make_uint4(four(0), four(4), four(8), four(12));
   if ((i & 1) == 0) scales[i >> 1] = (uint8_t)byte;
 }
 template <typename T>
@@ -44,13 +44,13 @@ __global__ void __launch_bounds__(256) mx8_dequantize_kernel(const uint8_t* code
   const long long i = blockIdx.x * 256ll + threadIdx.x;
   if (i >= n16) return;
   const uint4 c = reinterpret_cast<const uint4*>(codes)[i];
-  const float m = mx8_to_value(scales[i >> 1]);
+  const Mx8Reader reader(scales[i >> 1]);
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float f[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = mx8_value(w[2 * h + k / 4], k % 4, m);
+    reader.four(w[2 * h], f);
+    reader.four(w[2 * h + 1], f + 4);
     Vec8<T> o;
     o.from_float(f);
     o.store(y + i * 16 + 8 * h);
@@ -75,9 +75,9 @@ __global__ void __launch_bounds__(256) mx8_quantize_ragged_kernel(const T* x, ui
   }
 #pragma unroll
   for (int j = 0; j < RAGGED; ++j) {
-    const uint32_t byte = mx8_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v[j]) & 0x7fffffffu));
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v[j]) & 0x7fffffffu), byte = mx8_scale_byte(top);
     const int c = (b0 + j) * MX8_BLOCK + lane;
-    if (c < K) codes[row * K + c] = (uint8_t)mx8_code(v[j], mx8_to_code(byte));
+    if (c < K) codes[row * K + c] = (uint8_t)Mx8Coder(byte, top).four(__float_as_uint(v[j]), 0, 0, 0);
     if (lane == 0 && b0 + j < blocks) scales[row * blocks + b0 + j] = (uint8_t)byte;
   }
 }
@@ -102,7 +102,11 @@ __global__ void __launch_bounds__(256) mx8_dequantize_ragged_kernel(const uint8_
 #pragma unroll
   for (int j = 0; j < RAGGED; ++j) {
     const int c = (b0 + j) * MX8_BLOCK + lane;
-    if (c < K) y[row * K + c] = T(mx8_value(code[j], 0, mx8_to_value(byte[j])));
+    if (c < K) {
+      float f[4];
+      Mx8Reader(byte[j]).four(code[j], f);
+      y[row * K + c] = T(f[0]);
+    }
   }
 }
 
@@ -116,7 +120,7 @@ __global__ void __launch_bounds__(256) gated_act_kernel(const float* ab, T* h, l
   const float a = ab[i + row * H], b = ab[i + row * H + H];
   with_act(act, [&](auto k) {
     float d;
-    h[i] = T(act_value<decltype(k)::value>(a, d) * b);
+    h[i] = T(act_value<decltype(k)::value, true>(a, d) * b);
   });
 }
 template <typename T>
@@ -126,7 +130,7 @@ __global__ void __launch_bounds__(256) gated_act_bwd_kernel(const float* dh, con
   if (i >= n) return;
   const long long at = i + i / H * H;
   float da, db, v;
-  with_act(act, [&](auto k) { gated_grad<decltype(k)::value>(dh[i], ab[at], ab[at + H], da, db, v); });
+  with_act(act, [&](auto k) { gated_grad<decltype(k)::value, true>(dh[i], ab[at], ab[at + H], da, db, v); });
   dab[at] = T(da);
   dab[at + H] = T(db);
   h[i] = T(v);
