@@ -35,8 +35,12 @@ struct Mx8Coder {
   float m;
   bool exact;
   __device__ __forceinline__ Mx8Coder(uint32_t byte, uint32_t top) : m(mx8_to_code(byte)), exact(byte != MX8_NAN && (top & 0x7fffffu) < 0x7f0000u) {}
+  static constexpr float ROUND = 12582912.f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {  // lowest bytes
+    const uint32_t lo = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), hi = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+  }
   __device__ __forceinline__ uint32_t four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
-    constexpr float ROUND = 12582912.f;
     float f[4] = {__uint_as_float(a), __uint_as_float(b), __uint_as_float(c), __uint_as_float(d)};
     if (!exact) {
 #pragma unroll
@@ -45,8 +49,7 @@ struct Mx8Coder {
     const float k = exact ? m : 1.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = fmaf(f[i], k, ROUND);
-    const uint32_t lo = __byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040), hi = __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040);
-    return __byte_perm(lo, hi, 0x5410);
+    return pack(f[0], f[1], f[2], f[3]);
   }
 };
 

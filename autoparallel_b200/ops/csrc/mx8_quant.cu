@@ -41,6 +41,29 @@ __global__ void __launch_bounds__(256) mx8_quantize_kernel(const T* x, uint8_t* 
 template <typename T>
 __global__ void __launch_bounds__(256) mx8_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, T* y, long long n16) {
   after_previous();
+  if constexpr (sizeof(T) == 4) {
+    // sixteen fp32 values of a thread would be pieces of 16 bytes in every line that a warp stores; four times four, a warp's width apart, are whole lines
+    // (8192 x 4096 38.9 -> 28.4 us)
+    const long long first = (blockIdx.x * 256ll + (threadIdx.x & ~31)) * 4 + (threadIdx.x & 31);  // (in pieces of four)
+    uint32_t c[4];
+    uint8_t b[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long long i = first + 32 * k;
+      if (i < n16 * 4) {
+        c[k] = reinterpret_cast<const uint32_t*>(codes)[i];
+        b[k] = scales[i >> 3];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long long i = first + 32 * k;
+      float f[4];
+      Mx8Reader(b[k]).four(c[k], f);
+      if (i < n16 * 4) reinterpret_cast<float4*>(y)[i] = make_float4(f[0], f[1], f[2], f[3]);
+    }
+    return;
+  }
   const long long i = blockIdx.x * 256ll + threadIdx.x;
   if (i >= n16) return;
   const uint4 c = reinterpret_cast<const uint4*>(codes)[i];
@@ -57,56 +80,180 @@ __global__ void __launch_bounds__(256) mx8_dequantize_kernel(const uint8_t* code
   }
 }
 
-// Rows whose last block is not full begin anywhere: a warp to a block, an element to a lane, RAGGED blocks of a row under way together.
-constexpr int RAGGED = 4;
+// Rows of whole vectors whose last block is not full: eight elements to a thread, four threads to a block, ``vecs`` threads (four to every block) to a row.
+template <typename T>
+__global__ void __launch_bounds__(256) mx8_quantize_vec_kernel(const T* x, uint8_t* codes, uint8_t* scales, uint32_t rows, int K, uint32_t vecs) {
+  after_previous();
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x, row = i / vecs, c = (i - row * vecs) * 8;
+  const bool in = row < rows && c < (uint32_t)K;
+  const long long e = (long long)row * K + c;
+  float f[8] = {};
+  if (in) {
+    Vec8<T> v;
+    v.load(x + e);
+    v.to_float(f);
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(f[k]) & 0x7fffffffu);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  if (!in) return;
+  const uint32_t byte = mx8_scale_byte(top);
+  const Mx8Coder coder(byte, top);
+  auto four = [&](int k) { return coder.four(__float_as_uint(f[k]), __float_as_uint(f[k + 1]), __float_as_uint(f[k + 2]), __float_as_uint(f[k + 3])); };
+  *reinterpret_cast<uint2*>(codes + e) = make_uint2(four(0), four(4));
+  if (c % MX8_BLOCK == 0) scales[(long long)row * (vecs / 4) + c / MX8_BLOCK] = (uint8_t)byte;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) mx8_dequantize_vec_kernel(const uint8_t* codes, const uint8_t* scales, T* y, uint32_t rows, int K, uint32_t vecs) {
+  after_previous();
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x, row = i / vecs, c = (i - row * vecs) * 8;
+  if (row >= rows || c >= (uint32_t)K) return;
+  const long long e = (long long)row * K + c;
+  const uint2 w = *reinterpret_cast<const uint2*>(codes + e);
+  const Mx8Reader reader(scales[(long long)row * (vecs / 4) + c / MX8_BLOCK]);
+  float f[8];
+  reader.four(w.x, f);
+  reader.four(w.y, f + 4);
+  Vec8<T> o;
+  o.from_float(f);
+  o.store(y + e);
+}
+
+// Other rows begin anywhere.  A warp has seven blocks of a row, 224 elements, and takes them in the tensor's own aligned vectors of
+// eight elements (at most 29 of them, one to a lane): a lane's elements belong to one block or to two neighbours, ``first`` and the one after.  Codes lie like
+// the elements, so their vectors of eight bytes are aligned too.  Elements of other rows, and those past the tensor's end, are left alone.
+constexpr int RAGGED_BLOCKS = 7, RAGGED_COLUMNS = RAGGED_BLOCKS * MX8_BLOCK;
+struct Ragged {
+  long long row, base;  // element that the warp's columns count from
+  int block0, n;        // the row's block that the warp begins with; columns
+  int c, first, next;   // this lane's first column (below 0: elements of what lies before), its first block (-1: those), and how many elements come before the next
+  bool any;
+  __device__ __forceinline__ Ragged(long long rows, int K, int groups) {
+    const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), r = w / (uint32_t)groups;  // (32 bits: a division of 64 is as long as the rest of the kernel)
+    row = r;
+    block0 = (int)(w - r * (uint32_t)groups) * RAGGED_BLOCKS;
+    base = row * K + block0 * MX8_BLOCK;
+    n = row < rows ? min(RAGGED_COLUMNS, K - block0 * MX8_BLOCK) : 0;
+    c = (int)(threadIdx.x & 31) * 8 - (int)(base & 7);
+    any = c < n;
+    first = c < 0 ? -1 : c / MX8_BLOCK;
+    next = (first + 1) * MX8_BLOCK - c;
+  }
+  __device__ __forceinline__ bool in(int i) const { return c + i >= 0 && c + i < n; }
+  __device__ __forceinline__ bool whole() const { return c >= 0 && c + 8 <= n; }
+};
 template <typename T>
 __global__ void __launch_bounds__(256) mx8_quantize_ragged_kernel(const T* x, uint8_t* codes, uint8_t* scales, long long rows, int K, int blocks, int groups) {
   after_previous();
-  const long long w = blockIdx.x * 8ll + (threadIdx.x >> 5);  // (a warp: RAGGED blocks of one row)
-  const int lane = threadIdx.x & 31;
-  const long long row = w / groups;
-  if (row >= rows) return;
-  const int b0 = (int)(w - row * groups) * RAGGED;
-  float v[RAGGED];
+  const Ragged at(rows, K, groups);
+  if (at.n == 0) return;  // (the whole warp)
+  float f[8] = {};
+  if (at.any) {
+    const long long e = at.base + at.c;
+    if (e + 8 <= rows * K) {
+      Vec8<T> v;
+      v.load(x + e);
+      v.to_float(f);
+    } else {
 #pragma unroll
-  for (int j = 0; j < RAGGED; ++j) {
-    const int c = (b0 + j) * MX8_BLOCK + lane;
-    v[j] = c < K ? float(x[row * K + c]) : 0.f;
+      for (int i = 0; i < 8; ++i) f[i] = e + i < rows * K ? float(x[e + i]) : 0.f;
+    }
   }
+  if (!at.whole()) {
 #pragma unroll
-  for (int j = 0; j < RAGGED; ++j) {
-    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v[j]) & 0x7fffffffu), byte = mx8_scale_byte(top);
-    const int c = (b0 + j) * MX8_BLOCK + lane;
-    if (c < K) codes[row * K + c] = (uint8_t)Mx8Coder(byte, top).four(__float_as_uint(v[j]), 0, 0, 0);
-    if (lane == 0 && b0 + j < blocks) scales[row * blocks + b0 + j] = (uint8_t)byte;
+    for (int i = 0; i < 8; ++i) f[i] = at.in(i) ? f[i] : 0.f;
+  }
+  uint32_t own = 0, after = 0;  // largest magnitudes of this lane's first block and of the one after
+  if (at.next >= 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) own = max(own, __float_as_uint(f[i]) & 0x7fffffffu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t m = __float_as_uint(f[i]) & 0x7fffffffu;
+      if (i < at.next) own = max(own, m);
+      else after = max(after, m);
+    }
+  }
+  // Four lanes have the same first block, one after the other, counted from the lane that begins in block 0 or on it; the lane before them has the block's
+  // first elements where it does not begin on a lane.
+  const int lane = threadIdx.x & 31, from0 = (at.base & 7) != 0, l = lane - from0;
+  const uint32_t before = __shfl_up_sync(0xffffffffu, after, 1);
+  uint32_t top = lane > 0 && (l & 3) == 0 ? max(own, before) : own;
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_sync(0xffffffffu, top, (max(l, 0) ^ o) + from0));  // (lanes without columns may read any)
+  const uint32_t top_after = __shfl_sync(0xffffffffu, top, l < 0 ? from0 : (l / 4 + 1) * 4 + from0);
+  const uint32_t byte = mx8_scale_byte(top);
+  if (l >= 0 && (l & 3) == 0 && at.first * MX8_BLOCK < at.n) scales[at.row * blocks + at.block0 + at.first] = (uint8_t)byte;
+  if (!at.any) return;
+  const Mx8Coder here(byte, top), there(mx8_scale_byte(top_after), top_after);
+  uint32_t a[2];
+  if (at.next >= 8) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      a[h] = here.four(__float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1]), __float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3]));
+  } else if (here.exact && there.exact) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      a[h] = Mx8Coder::pack(fmaf(f[4 * h], 4 * h < at.next ? here.m : there.m, Mx8Coder::ROUND), fmaf(f[4 * h + 1], 4 * h + 1 < at.next ? here.m : there.m, Mx8Coder::ROUND),
+                            fmaf(f[4 * h + 2], 4 * h + 2 < at.next ? here.m : there.m, Mx8Coder::ROUND),
+                            fmaf(f[4 * h + 3], 4 * h + 3 < at.next ? here.m : there.m, Mx8Coder::ROUND));
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t w[4] = {__float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1]), __float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3])};
+      const int own_bytes = max(0, min(4, at.next - 4 * h));
+      const uint32_t mask = own_bytes == 4 ? 0xffffffffu : (1u << (8 * own_bytes)) - 1u;
+      a[h] = (here.four(w[0], w[1], w[2], w[3]) & mask) | (there.four(w[0], w[1], w[2], w[3]) & ~mask);
+    }
+  }
+  uint8_t* to = codes + at.base + at.c;
+  if (at.whole()) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at.in(i)) to[i] = (uint8_t)(a[i / 4] >> (8 * (i % 4)));
   }
 }
 template <typename T>
 __global__ void __launch_bounds__(256) mx8_dequantize_ragged_kernel(const uint8_t* codes, const uint8_t* scales, T* y, long long rows, int K, int blocks,
                                                                    int groups) {
   after_previous();
-  const long long w = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const long long row = w / groups;
-  if (row >= rows) return;
-  const int b0 = (int)(w - row * groups) * RAGGED;
-  uint32_t code[RAGGED], byte[RAGGED];
+  const Ragged at(rows, K, groups);
+  if (!at.any) return;
+  const long long e = at.base + at.c;
+  uint2 w = make_uint2(0, 0);
+  if (e + 8 <= rows * K) {
+    w = *reinterpret_cast<const uint2*>(codes + e);
+  } else {
 #pragma unroll
-  for (int j = 0; j < RAGGED; ++j) {
-    const int c = (b0 + j) * MX8_BLOCK + lane;
-    if (c < K) {
-      code[j] = codes[row * K + c];
-      byte[j] = scales[row * blocks + b0 + j];
-    }
+    for (int i = 0; i < 8; ++i)
+      if (e + i < rows * K) (i < 4 ? w.x : w.y) |= (uint32_t)codes[e + i] << (8 * (i % 4));
   }
+  const uint8_t* s = scales + at.row * blocks + at.block0;
+  const bool second = at.next < 8 && (at.first + 1) * MX8_BLOCK < at.n;
+  float f[8], g[8];
+  const Mx8Reader here(at.first < 0 ? MX8_LOWEST : s[at.first]);
+  here.four(w.x, f);
+  here.four(w.y, f + 4);
+  if (second) {
+    const Mx8Reader there(s[at.first + 1]);
+    there.four(w.x, g);
+    there.four(w.y, g + 4);
 #pragma unroll
-  for (int j = 0; j < RAGGED; ++j) {
-    const int c = (b0 + j) * MX8_BLOCK + lane;
-    if (c < K) {
-      float f[4];
-      Mx8Reader(byte[j]).four(code[j], f);
-      y[row * K + c] = T(f[0]);
-    }
+    for (int i = 0; i < 8; ++i) f[i] = i < at.next ? f[i] : g[i];
+  }
+  if (at.whole()) {
+    Vec8<T> o;
+    o.from_float(f);
+    o.store(y + e);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at.in(i)) y[e + i] = T(f[i]);
   }
 }
 
@@ -145,32 +292,37 @@ static unsigned blocks_of(long long n) { return (n + 255) / 256 > 0x7fffffffll ?
 
 using namespace apb;
 
-// x [R, K], codes [R, K], scales [R, ceil(K / 32)], all dense, x and codes on 16-byte bases.
+// x [R, K], codes [R, K], scales [R, ceil(K / 32)], all dense, x and codes on 16-byte bases.  Whole rows of blocks, rows of whole vectors, other rows:
+// 8192 x 14336 bf16 54, 14344 75, 14343 224 us (and back 58, 68, 108).
+template <typename T>
+static int quantize(const T* x, uint8_t* codes, uint8_t* scales, long long R, long long K, cudaStream_t st) {
+  const long long blocks = (K + MX8_BLOCK - 1) / MX8_BLOCK, groups = (blocks + RAGGED_BLOCKS - 1) / RAGGED_BLOCKS;
+  if (K % MX8_BLOCK == 0) return done(launch_after(mx8_quantize_kernel<T>, blocks_of(R * K / 16), 256, 0, st, x, codes, scales, R * K / 16));
+  if (K % 8 == 0) return done(launch_after(mx8_quantize_vec_kernel<T>, blocks_of(R * blocks * 4), 256, 0, st, x, codes, scales, (uint32_t)R, (int)K, (uint32_t)blocks * 4));
+  return done(launch_after(mx8_quantize_ragged_kernel<T>, blocks_of(R * groups * 32), 256, 0, st, x, codes, scales, R, (int)K, (int)blocks, (int)groups));
+}
+template <typename T>
+static int dequantize(const uint8_t* codes, const uint8_t* scales, T* y, long long R, long long K, cudaStream_t st) {
+  const long long blocks = (K + MX8_BLOCK - 1) / MX8_BLOCK, groups = (blocks + RAGGED_BLOCKS - 1) / RAGGED_BLOCKS;
+  if (K % MX8_BLOCK == 0) return done(launch_after(mx8_dequantize_kernel<T>, blocks_of(R * K / 16), 256, 0, st, codes, scales, y, R * K / 16));
+  if (K % 8 == 0) return done(launch_after(mx8_dequantize_vec_kernel<T>, blocks_of(R * blocks * 4), 256, 0, st, codes, scales, y, (uint32_t)R, (int)K, (uint32_t)blocks * 4));
+  return done(launch_after(mx8_dequantize_ragged_kernel<T>, blocks_of(R * groups * 32), 256, 0, st, codes, scales, y, R, (int)K, (int)blocks, (int)groups));
+}
+// (the threads of the forms for other rows are counted in 32 bits: 2^32 of them are 2^35 elements or, of a row of one element, 2^30)
+static bool too_many(long long R, long long K) {
+  const long long blocks = (K + MX8_BLOCK - 1) / MX8_BLOCK;
+  return K > 0x7fffffe0ll || R > 0x7fffffffll * 64 / blocks || (K % MX8_BLOCK && R > 0x3fffff00ll / blocks) || R * K / 16 / 256 >= 0x7fffffffll;
+}
 extern "C" int apb_mx8_quantize(const void* x, void* codes, void* scales, long long R, long long K, int is_bf16, cudaStream_t st) {
   if (R <= 0 || K <= 0) return 0;
-  if (off16(x) || off16(codes) || K > 0x7fffffe0ll) return 3;
-  uint8_t *c = (uint8_t*)codes, *s = (uint8_t*)scales;
-  const long long blocks = (K + MX8_BLOCK - 1) / MX8_BLOCK, groups = (blocks + RAGGED - 1) / RAGGED;
-  const unsigned grid = blocks_of(K % MX8_BLOCK == 0 ? R * K / 16 : R * groups * 32);
-  if (grid == 0) return 3;
-  if (K % MX8_BLOCK == 0)
-    return done(is_bf16 ? launch_after(mx8_quantize_kernel<bf16>, grid, 256, 0, st, (const bf16*)x, c, s, R * K / 16)
-                        : launch_after(mx8_quantize_kernel<float>, grid, 256, 0, st, (const float*)x, c, s, R * K / 16));
-  return done(is_bf16 ? launch_after(mx8_quantize_ragged_kernel<bf16>, grid, 256, 0, st, (const bf16*)x, c, s, R, (int)K, (int)blocks, (int)groups)
-                      : launch_after(mx8_quantize_ragged_kernel<float>, grid, 256, 0, st, (const float*)x, c, s, R, (int)K, (int)blocks, (int)groups));
+  if (off16(x) || off16(codes) || too_many(R, K)) return 3;
+  return is_bf16 ? quantize((const bf16*)x, (uint8_t*)codes, (uint8_t*)scales, R, K, st) : quantize((const float*)x, (uint8_t*)codes, (uint8_t*)scales, R, K, st);
 }
 extern "C" int apb_mx8_dequantize(const void* codes, const void* scales, void* y, long long R, long long K, int is_bf16, cudaStream_t st) {
   if (R <= 0 || K <= 0) return 0;
-  if (off16(y) || off16(codes) || K > 0x7fffffe0ll) return 3;
-  const uint8_t *c = (const uint8_t*)codes, *s = (const uint8_t*)scales;
-  const long long blocks = (K + MX8_BLOCK - 1) / MX8_BLOCK, groups = (blocks + RAGGED - 1) / RAGGED;
-  const unsigned grid = blocks_of(K % MX8_BLOCK == 0 ? R * K / 16 : R * groups * 32);
-  if (grid == 0) return 3;
-  if (K % MX8_BLOCK == 0)
-    return done(is_bf16 ? launch_after(mx8_dequantize_kernel<bf16>, grid, 256, 0, st, c, s, (bf16*)y, R * K / 16)
-                        : launch_after(mx8_dequantize_kernel<float>, grid, 256, 0, st, c, s, (float*)y, R * K / 16));
-  return done(is_bf16 ? launch_after(mx8_dequantize_ragged_kernel<bf16>, grid, 256, 0, st, c, s, (bf16*)y, R, (int)K, (int)blocks, (int)groups)
-                      : launch_after(mx8_dequantize_ragged_kernel<float>, grid, 256, 0, st, c, s, (float*)y, R, (int)K, (int)blocks, (int)groups));
+  if (off16(y) || off16(codes) || too_many(R, K)) return 3;
+  return is_bf16 ? dequantize((const uint8_t*)codes, (const uint8_t*)scales, (bf16*)y, R, K, st)
+                 : dequantize((const uint8_t*)codes, (const uint8_t*)scales, (float*)y, R, K, st);
 }
 
 extern "C" int apb_gated_act(const float* ab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st) {

@@ -296,7 +296,11 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: tor
     """``add_rms_norm`` (of x alone where ``residual`` is None) with the norm in 8 bits: (y, h, q, scale), ``q`` float8_e4m3fn and
     ``scale`` fp32 [.., 1], the row-wise operands of ``scaled_mm``; ``q * scale`` stands for the norm.  q and scale have no gradient: a
     training step hands the gradient of what it made of them to ``y``, the norm itself, which ``keep=False`` leaves out (None)."""
-    _check_norm("add_rms_norm_fp8", x, residual, weight)
+    xs = x.shape
+    # (one test for the calls that are right: this is the path of single tokens)
+    if not (x.dtype in _FLOATS and xs and 1 <= xs[-1] <= 32768 and weight.shape == xs[-1:] and weight.dtype in _FLOATS and weight.device == x.device
+            and (residual is None or (residual.shape == xs and residual.dtype is x.dtype and residual.device == x.device))):
+        _check_norm("add_rms_norm_fp8", x, residual, weight)
     if not keep and torch.is_grad_enabled():
         _need(not any(t is not None and t.requires_grad for t in (x, residual, weight)),
               "add_rms_norm_fp8: gradients go through y, which keep=False leaves out")
