@@ -38,6 +38,12 @@ class LlamaConfig:
     max_seq_len: int = 8192
     init_std: float = 0.02
     depth_init: bool = False
+    #: the feed-forward block as one operator (``ops.gated_ffn``): both projections, the activation and their product in one kernel
+    fused_ffn: bool = False
+    #: what ``fused_ffn`` keeps for the backward pass: "full" (in the type of the activations) or "mx8" (in 8 bits)
+    ffn_checkpoint: str = "full"
+    #: the residual's addition and the norm before the feed-forward block in one kernel (``ops.add_rms_norm``)
+    fused_norm: bool = False
 
     @property
     def head_dim(self) -> int:
@@ -152,13 +158,20 @@ class Attention(nn.Module):
 
 
 class FeedForward(nn.Module):
-    def __init__(self, dim: int, hidden: int):
+    def __init__(self, dim: int, hidden: int, fused: bool = False, checkpoint: str = "full"):
         super().__init__()
+        if checkpoint not in K.ffn_ops.CHECKPOINTS:
+            raise ValueError(f"ffn_checkpoint is one of {sorted(K.ffn_ops.CHECKPOINTS)}, not {checkpoint!r}")
+        if checkpoint != "full" and not fused:
+            raise ValueError(f"ffn_checkpoint {checkpoint!r} needs fused_ffn")
+        self.fused, self.checkpoint = fused, checkpoint
         self.w1 = nn.Linear(dim, hidden, bias=False)
         self.w3 = nn.Linear(dim, hidden, bias=False)
         self.w2 = nn.Linear(hidden, dim, bias=False)
 
     def forward(self, x):
+        if self.fused:
+            return K.gated_ffn(x, self.w1.weight, self.w3.weight, self.w2.weight, checkpoint=self.checkpoint)
         return self.w2(K.swiglu(self.w1(x), self.w3(x)))
 
     def init_weights(self, std: float, out_std: float):
@@ -171,7 +184,8 @@ class TransformerBlock(nn.Module):
     def __init__(self, layer_id: int, cfg: LlamaConfig):
         super().__init__()
         self.attention = Attention(cfg)
-        self.feed_forward = FeedForward(cfg.dim, cfg.hidden_dim())
+        self.feed_forward = FeedForward(cfg.dim, cfg.hidden_dim(), cfg.fused_ffn, cfg.ffn_checkpoint)
+        self.fused_norm = cfg.fused_norm
         self.attention_norm = RMSNorm(cfg.dim, cfg.norm_eps)
         self.ffn_norm = RMSNorm(cfg.dim, cfg.norm_eps)
         depth = (layer_id + 1) if cfg.depth_init else cfg.n_layers
@@ -179,7 +193,11 @@ class TransformerBlock(nn.Module):
         self.out_std = cfg.init_std / (2 * depth) ** 0.5 if cfg.depth_init else cfg.init_std
 
     def forward(self, x, cos, sin):
-        h = x + self.attention(self.attention_norm(x), cos, sin)
+        a = self.attention(self.attention_norm(x), cos, sin)
+        if self.fused_norm:
+            n, h = K.add_rms_norm(a, x, self.ffn_norm.weight, self.ffn_norm.eps)
+            return h + self.feed_forward(n)
+        h = x + a
         return h + self.feed_forward(self.ffn_norm(h))
 
     def init_weights(self):

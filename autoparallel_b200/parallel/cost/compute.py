@@ -81,6 +81,17 @@ def _flops(op, args, in_shapes: list[list[int]], out_shapes: list[list[int]]) ->
         return 2.0 * _numel(in_shapes[0]) * args[3]
     if op is apb.mx4_mm.default:
         return 0.5 * 2 * _numel(in_shapes[0]) * in_shapes[2][-2]
+    if op is apb.gated_ffn.default:
+        rows = _numel(in_shapes[0]) // max(1, in_shapes[0][-1])
+        return 2.0 * rows * (2 * _numel(in_shapes[1]) + _numel(in_shapes[3]))
+    if op is apb.gated_mm.default:
+        return 2.0 * _numel(in_shapes[0]) * 2 * in_shapes[1][0]
+    if op is apb.gated_dgrad.default:
+        return 2.0 * _numel(in_shapes[0]) * in_shapes[1][1]
+    if op is apb.gated_dx.default:
+        return 2.0 * _numel(in_shapes[0]) * in_shapes[1][1]
+    if op is apb.gated_wgrad.default:
+        return 2.0 * _numel(in_shapes[0]) * in_shapes[1][-1]
     if op is apb.gemm.default or op is aten.mm.default:
         a = in_shapes[0]
         return 2.0 * _numel(a) * out_shapes[0][-1] if op is aten.mm.default else 2.0 * _numel(a) * out_shapes[0][-1]

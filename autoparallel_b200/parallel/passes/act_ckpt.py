@@ -41,6 +41,8 @@ _EXPENSIVE = {
     apb.mm_wgrad.default,
     apb.gemm.default,
     apb.mx4_matmul.default,
+    apb.gated_mm.default,
+    apb.gated_ffn.default,
     apb.attention.default,
     aten.mm.default,
     aten.bmm.default,

@@ -346,6 +346,103 @@ def _mx4_matmul(ctx):
     return expand_rows(ctx, rows)
 
 
+# ---- the feed-forward block (ops/ffn_ops.py).  What a call leaves out is an empty tensor of one dim and stays whole.
+def _is_left_out(v):
+    return v.ndim == 1 and v.shape[0] == 0
+
+
+def _kept(v, place):
+    return R if _is_left_out(v) else place
+
+
+@register_rule(apb.add_rms_norm.default)
+def _add_rms_norm(ctx):
+    # (y, h, rstd, x, residual, weight)
+    return expand_rows(ctx, [(S(i),) * 5 + (R,) for i in _lead_dims(ctx.in_vals[0])])
+
+
+@register_rule(apb.add_rms_norm_bwd.default)
+def _add_rms_norm_bwd(ctx):
+    # (dx, dw, dy, dh, h, weight, rstd)
+    return expand_rows(ctx, [(S(i), P, S(i), S(i), S(i), R, S(i)) for i in _lead_dims(ctx.in_vals[2])])
+
+
+@register_rule(apb.add_rms_norm_fp8.default)
+def _add_rms_norm_fp8(ctx):
+    # (y, h, rstd, q, scale, x[, residual], weight)
+    outs, n = ctx.out_vals, len(ctx.in_vals) - 1
+    return expand_rows(ctx, [tuple(_kept(v, S(i)) for v in outs) + (S(i),) * n + (R,) for i in _lead_dims(ctx.in_vals[0])])
+
+
+@register_rule(apb.mx8_quantize.default)
+def _mx8_quantize(ctx):
+    # (codes, scales, x): the last dim in whole blocks
+    x = ctx.in_vals[0]
+    return expand_rows(ctx, [(S(i),) * 3 for i in range(x.ndim) if i < x.ndim - 1 or _splits(ctx, x.shape[i], 32)])
+
+
+@register_rule(apb.mx8_dequantize.default)
+def _mx8_dequantize(ctx):
+    # (values, codes, scales)
+    codes = ctx.in_vals[0]
+    return expand_rows(ctx, [(S(i),) * 3 for i in range(codes.ndim) if i < codes.ndim - 1 or _splits(ctx, codes.shape[i], 32)])
+
+
+def _hidden_splits(ctx, ab, hidden):
+    """Whether the hidden dim of both projections may be split: of codes, in whole blocks."""
+    return ab.dtype != torch.int8 or _splits(ctx, hidden, 32)
+
+
+@register_rule(apb.gated_ffn.default)
+def _gated_ffn(ctx):
+    # (y, ab, scales, xq, xs, x, w1, w3, w2): rows of x; the hidden dim, whose products are summed up; columns of the result
+    x, w1 = ctx.in_vals[:2]
+    _, ab, scales, xq, xs = ctx.out_vals
+    last, hidden = x.ndim - 1, x.ndim
+    rows = [(S(i), *(_kept(v, S(i)) for v in (ab, scales, xq, xs)), S(i), R, R, R) for i in range(last)]
+    if _hidden_splits(ctx, ab, w1.shape[0]):
+        rows.append((P, _kept(ab, S(hidden)), _kept(scales, S(hidden)), R, R, R, S(0), S(0), S(1)))
+    rows.append((S(last), R, R, R, R, R, R, R, S(0)))
+    return expand_rows(ctx, rows)
+
+
+@register_rule(apb.gated_mm.default)
+def _gated_mm(ctx):
+    # (h, ab, scales, x, w1, w3)
+    x, w1 = ctx.in_vals[:2]
+    _, ab, scales = ctx.out_vals
+    last, hidden = x.ndim - 1, x.ndim
+    rows = [(S(i), _kept(ab, S(i)), _kept(scales, S(i)), S(i), R, R) for i in range(last)]
+    if _hidden_splits(ctx, ab, w1.shape[0]):
+        rows.append((S(last), _kept(ab, S(hidden)), _kept(scales, S(hidden)), R, S(0), S(0)))
+    return expand_rows(ctx, rows)
+
+
+@register_rule(apb.gated_dgrad.default)
+def _gated_dgrad(ctx):
+    # (dab, h, dy, w2, ab, scales); dh goes through a product, so its contraction stays whole
+    dy, w2, ab, scales = ctx.in_vals
+    last, hidden = dy.ndim - 1, dy.ndim
+    rows = [(S(i), S(i), S(i), R, S(i), _kept(scales, S(i))) for i in range(last)]
+    if _hidden_splits(ctx, ab, w2.shape[1]):
+        rows.append((S(hidden), S(last), R, S(1), S(hidden), _kept(scales, S(hidden))))
+    return expand_rows(ctx, rows)
+
+
+@register_rule(apb.gated_dx.default)
+def _gated_dx(ctx):
+    # (dx, dab, w1, w3)
+    last = ctx.in_vals[0].ndim - 2
+    return expand_rows(ctx, [(S(i), S(i), R, R) for i in range(last)] + [(P, S(last + 1), S(0), S(0)), (S(last), R, S(1), S(1))])
+
+
+@register_rule(apb.gated_wgrad.default)
+def _gated_wgrad(ctx):
+    # (dw1, dw3, dab, x)
+    last = ctx.in_vals[1].ndim - 1
+    return expand_rows(ctx, [(P, P, S(i), S(i)) for i in range(last)] + [(S(0), S(0), S(last + 1), R), (S(1), S(1), R, S(last))])
+
+
 @register_rule(apb.embedding.default)
 def _embedding(ctx):
     # (out [*ids, D], weight [V, D], ids): split the tokens, or the hidden dim of the table; a table split by rows

@@ -288,3 +288,130 @@ def test_meta_shapes(bits):
         assert ops.gated_dx(dab.to("meta"), w1.to("meta"), w3.to("meta")).shape == ops.gated_dx(dab, w1, w3).shape
         real, meta = ops.gated_wgrad(dab, x, torch.float32), ops.gated_wgrad(dab.to("meta"), x.to("meta"), torch.float32)
         assert [tuple(a.shape) for a in real] == [tuple(a.shape) for a in meta]
+
+
+# ------------------------------------------------------------------------------------ planner and model
+def _rows(mesh, name, *args):
+    from autoparallel_b200.parallel.strategies import rules
+
+    op = getattr(torch.ops.apb200, name).default
+    ctx = rules.RuleCtx(mesh, op, args, {}, [a for a in args if isinstance(a, torch.Tensor)], None, op(*args), True)
+    found = set()
+    for s in rules.get_rule(op)(ctx).strategies:
+        outs = s.output_specs if isinstance(s.output_specs, (tuple, list)) else [s.output_specs]
+        found.add(tuple(o.placements[0] for o in outs) + tuple(i.placements[0] for i in s.input_specs))
+    return found
+
+
+def test_rules(mesh_1d):
+    from torch.distributed.tensor.placement_types import Partial, Replicate, Shard
+
+    S, R, P = Shard, Replicate(), Partial()
+    x, w1, w2 = torch.randn(8, 16, 64), torch.randn(256, 64), torch.randn(64, 256)
+    assert _rows(mesh_1d, "add_rms_norm", x, x, x[0, 0], 1e-5) == {(R,) * 6, (S(0),) * 5 + (R,), (S(1),) * 5 + (R,)}
+    assert _rows(mesh_1d, "add_rms_norm_fp8", x, None, x[0, 0], 1e-5, False) == {
+        (R,) * 7, *((R, R, S(i), S(i), S(i), S(i), R) for i in (0, 1))}
+    assert _rows(mesh_1d, "add_rms_norm_bwd", x, x, x, x[0, 0], x[..., 0]) == {
+        (R,) * 7, *((S(i), P, S(i), S(i), S(i), R, S(i)) for i in (0, 1))}
+    assert _rows(mesh_1d, "mx8_quantize", x) == {(R,) * 3, (S(0),) * 3, (S(1),) * 3}
+    assert _rows(mesh_1d, "mx8_quantize", w2) == {(R,) * 3, (S(0),) * 3, (S(1),) * 3}
+    full = {(R,) * 9, *((S(i), S(i), R, R, R, S(i), R, R, R) for i in (0, 1)), (P, S(3), R, R, R, R, S(0), S(0), S(1)),
+            (S(2), R, R, R, R, R, R, R, S(0))}
+    assert _rows(mesh_1d, "gated_ffn", x, w1, w1, w2, 0, 16) == full
+    assert _rows(mesh_1d, "gated_ffn", x, w1, w1, w2, 0, 8) == {
+        (R,) * 9, *((S(i),) * 6 + (R,) * 3 for i in (0, 1)), (P, S(3), S(3), R, R, R, S(0), S(0), S(1)), (S(2), R, R, R, R, R, R, R, S(0))}
+    half = torch.randn(128, 64)  # 16 columns a rank: half a block
+    assert (P, S(3), S(3), R, R, R, S(0), S(0), S(1)) not in _rows(mesh_1d, "gated_ffn", x, half, half, half.t().contiguous(), 0, 8)
+    _, ab, scales = ops.gated_mm(x, w1, w1, 0, 8)
+    assert _rows(mesh_1d, "gated_dgrad", x, w2, ab, scales, 0) == {
+        (R,) * 6, *((S(i), S(i), S(i), R, S(i), S(i)) for i in (0, 1)), (S(3), S(2), R, S(1), S(3), S(3))}
+    dab = torch.randn(8, 16, 2, 256)
+    assert _rows(mesh_1d, "gated_dx", dab, w1, w1) == {(R,) * 4, *((S(i), S(i), R, R) for i in (0, 1)), (P, S(3), S(0), S(0)), (S(2), R, S(1), S(1))}
+    assert _rows(mesh_1d, "gated_wgrad", dab, x, torch.float32) == {
+        (R,) * 4, *((P, P, S(i), S(i)) for i in (0, 1)), (S(0), S(0), S(3), R), (S(1), S(1), R, S(2))}
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_splits_of_the_rules_compute_the_same(bits):
+    g = _gen(3)
+    x, w1, w3, w2 = (_randn(*s, gen=g) for s in ((4, 6, 24), (128, 24), (128, 24), (16, 128)))
+    y, ab, scales, _, _ = ops.gated_ffn(x, w1, w3, w2, 0, bits)
+    parts = [ops.gated_ffn(x, a, b, c.contiguous(), 0, bits) for a, b, c in zip(w1.chunk(2), w3.chunk(2), w2.chunk(2, 1))]
+    assert torch.allclose(sum(p[0] for p in parts), y, atol=1e-4) and torch.equal(torch.cat([p[1] for p in parts], 3), ab)
+    if bits == 8:
+        assert torch.equal(torch.cat([p[2] for p in parts], 3), scales)
+    dy = _randn(4, 6, 16, gen=g)
+    dab, h = ops.gated_dgrad(dy, w2, ab, scales, 0)
+    halves = [ops.gated_dgrad(dy, c.contiguous(), a.contiguous(), s.contiguous() if bits == 8 else s, 0)
+              for c, a, s in zip(w2.chunk(2, 1), ab.chunk(2, 3), scales.chunk(2, 3) if bits == 8 else (scales, scales))]
+    assert torch.allclose(torch.cat([p[0] for p in halves], 3), dab, atol=1e-5) and torch.allclose(torch.cat([p[1] for p in halves], 2), h, atol=1e-5)
+    dx = ops.gated_dx(dab, w1, w3)
+    assert torch.allclose(sum(ops.gated_dx(d.contiguous(), a, b) for d, a, b in zip(dab.chunk(2, 3), w1.chunk(2), w3.chunk(2))), dx, atol=1e-4)
+    dw = ops.gated_wgrad(dab, x, torch.float32)
+    rows = [ops.gated_wgrad(d.contiguous(), t.contiguous(), torch.float32) for d, t in zip(dab.chunk(2, 1), x.chunk(2, 1))]
+    assert all(torch.allclose(rows[0][i] + rows[1][i], dw[i], atol=1e-4) for i in (0, 1))
+
+
+def _llama(**kw):
+    from autoparallel_b200.models.llama3 import Transformer, llama3_debug
+
+    m = Transformer(llama3_debug(**kw))
+    m.init_weights(0)
+    return m
+
+
+def test_model_with_the_fused_block():
+    """Same weights, same inputs: the fused forms give the loss and the gradients of the separate operators, with 8-bit checkpoints the same
+    loss and gradients of the rounded activations."""
+    tokens, labels = (torch.randint(0, 1024, (2, 33), generator=_gen(s)) for s in (1, 2))
+
+    def step(**kw):
+        m = _llama(**kw)
+        loss = m(tokens, labels)
+        loss.backward()
+        return loss.detach(), {n: p.grad for n, p in m.named_parameters()}
+
+    loss, grads = step()
+    for kw, off in ((dict(fused_ffn=True), 1e-4), (dict(fused_norm=True), 1e-4), (dict(fused_ffn=True, fused_norm=True, ffn_checkpoint="mx8"), 2.0**-6)):
+        l2, g2 = step(**kw)
+        # (8 bits: a rounding of at most 2^-7 of a block's largest value in each of x, a and b)
+        assert abs(float(l2 - loss)) < 1e-5 and all(float((g2[n] - g).norm() / g.norm()) < off for n, g in grads.items()), kw
+    with pytest.raises(ValueError, match="ffn_checkpoint is one of"):
+        _llama(fused_ffn=True, ffn_checkpoint="fp8")
+    with pytest.raises(ValueError, match="needs fused_ffn"):
+        _llama(ffn_checkpoint="mx8")
+
+
+@pytest.mark.parametrize("checkpoint", ["full", "mx8"])
+def test_planned_model(mesh_2d, checkpoint):
+    from torch.distributed.tensor.placement_types import Replicate, Shard
+
+    from autoparallel_b200 import AutoParallel, ForwardInputs
+    from autoparallel_b200.models.llama3 import Transformer, llama3_debug
+
+    with torch.device("meta"):
+        model = Transformer(llama3_debug(fused_ffn=True, fused_norm=True, ffn_checkpoint=checkpoint))
+
+    def input_fn():
+        return ForwardInputs((torch.randint(0, 1024, (8, 64)),), {"labels": torch.randint(0, 1024, (8, 64))})
+
+    with AutoParallel(model, input_fn, mesh_2d) as ap:
+        ap.add_input_constraints([(Shard(0), Replicate())] * 2)
+        ap.optimize_placement()
+        low = ap.lower()
+        names = {str(n.target) for n in low.gm.graph.nodes if n.op == "call_function"}
+        for op in ("gated_ffn", "gated_dgrad", "gated_dx", "gated_wgrad", "add_rms_norm", "add_rms_norm_bwd", *(("mx8_dequantize",) if checkpoint == "mx8" else ())):
+            assert f"apb200.{op}.default" in names, op
+
+
+def test_costs(mesh_1d):
+    from autoparallel_b200.parallel.cost import compute
+
+    apb = torch.ops.apb200
+    m, d, h, n = 10, 64, 96, 32
+    ffn = compute._flops(apb.gated_ffn.default, (), [[2, 5, d], [h, d], [h, d], [n, h]], [])
+    assert ffn == 2.0 * m * (2 * d * h + h * n)
+    back = (compute._flops(apb.gated_dgrad.default, (), [[2, 5, n], [n, h], [2, 5, 2, h], [0]], []) + compute._flops(apb.gated_dx.default, (), [[2, 5, 2, h], [h, d], [h, d]], [])
+            + compute._flops(apb.gated_wgrad.default, (), [[2, 5, 2, h], [2, 5, d]], []) + 2.0 * m * n * h)
+    assert back == 2 * ffn
+    assert compute._flops(apb.gated_mm.default, (), [[2, 5, d], [h, d], [h, d]], []) == 4.0 * m * d * h
