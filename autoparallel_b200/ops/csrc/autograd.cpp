@@ -544,6 +544,7 @@ const Op<GatedFfnSig>& op_gated_ffn() { APB_OP(o, "gated_ffn", GatedFfnSig); ret
 
 // (dx, dw) of h and the weight, of whichever of both results have been used.
 Pair add_norm_gradients(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& w, const Tensor& rstd) {
+  at::AutoDispatchBelowAutograd guard;  // (nothing is recorded here; without it every operator goes through the boxed kernel of those without a formula)
   if (!dy.defined()) return {dh.detach(), at::zeros_like(w)};
   return dh.defined() ? op_add_norm_bwd()(dy, dh, h, w, rstd) : op_rms_bwd()(dy, h, w, rstd);
 }
@@ -616,6 +617,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
   }
   static variable_list gradients(AutogradContext* ctx, const Tensor& dy) {
     const auto s = ctx->get_saved_variables();
+    at::AutoDispatchBelowAutograd guard;  // (as above)
     const bool of_x = ctx->needs_input_grad(0), of_up = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     auto [dab, h] = op_gated_dgrad()(dy, s[3], s[4], s[5], ctx->saved_data["act"].toInt());
     Tensor dx, dw1, dw3, dw2;

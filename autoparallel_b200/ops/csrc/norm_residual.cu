@@ -88,17 +88,24 @@ struct AddNormOut {
   float* scale;
 };
 
-// largest of the block's values (bits of magnitudes: a NaN is larger than everything); ``red``: 32 words
-__device__ __forceinline__ uint32_t block_top(uint32_t v, uint32_t* red) {
-  v = __reduce_max_sync(0xffffffffu, v);
+// block_sum, and the largest of the block's values with it (bits of magnitudes: a NaN is larger than everything); ``red``, ``red_top``: 32 words each
+__device__ __forceinline__ float block_sum_top(float v, uint32_t& top, float* red, uint32_t* red_top) {
+  v = warp_sum(v);
+  top = __reduce_max_sync(0xffffffffu, top);
   const int w = threadIdx.x >> 5, l = threadIdx.x & 31, nw = blockDim.x >> 5;
   __syncthreads();
-  if (l == 0) red[w] = v;
+  if (l == 0) {
+    red[w] = v;
+    red_top[w] = top;
+  }
   __syncthreads();
-  return __reduce_max_sync(0xffffffffu, l < nw ? red[l] : 0u);
+  top = __reduce_max_sync(0xffffffffu, l < nw ? red_top[l] : 0u);
+  return warp_sum(l < nw ? red[l] : 0.f);
 }
 
 // A warp (WARP_ROWS) or a block has a row, each thread up to NP vectors.
+// In 8 bits 1 / rms cancels: with m = max |h w|, y / (max |y| / 448) = h w 448 / m, where h w of two bf16 is exact in fp32.  So q takes one rounded factor, is
+// nearer to the formula than y / s would be (a third of the values that round the other way), and m is found in the same reduction as the sum of squares.
 template <typename T, bool EVEN, int NP, bool WARP_ROWS, bool FP8>
 __global__ void __launch_bounds__(WARP_ROWS ? 256 : 1024) add_rms_norm_kernel(const T* x, const T* res, const T* w, const AddNormOut o, long long rows, int D,
                                                                               float eps) {
@@ -112,6 +119,7 @@ __global__ void __launch_bounds__(WARP_ROWS ? 256 : 1024) add_rms_norm_kernel(co
     const Row<T, EVEN> at(row, rows, D);
     Vec8<T> v[NP], u[NP];
     float ss = 0.f;
+    uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       const int c = at.col(t + j * tpr);
@@ -138,12 +146,31 @@ __global__ void __launch_bounds__(WARP_ROWS ? 256 : 1024) add_rms_norm_kernel(co
         at.mask(f, c);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
+        if (FP8) {
+          float g[8];
+          at.weight(g, w, c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i] * g[i]) & 0x7fffffffu);
+        }
       }
     }
-    ss = WARP_ROWS ? warp_sum(ss) : block_sum(ss, red);
+    if (!FP8) {
+      ss = WARP_ROWS ? warp_sum(ss) : block_sum(ss, red);
+    } else if (WARP_ROWS) {
+      ss = warp_sum(ss);
+      top = __reduce_max_sync(0xffffffffu, top);
+    } else {
+      ss = block_sum_top(ss, top, red, red_top);
+    }
     const float r = rsqrtf(ss / D + eps);
     if (t == 0) o.rstd[row] = r;
-    uint32_t top = 0;
+    float k = 0.f;  // q = h w k
+    if (FP8) {
+      const float m = __uint_as_float(top), r8 = __frsqrt_rn(__fdiv_rn(ss, (float)D) + eps), amax = m * r8;
+      const bool tiny = amax < 0x1p-100f;
+      k = tiny ? r8 : __fdiv_rn(448.f, m);
+      if (t == 0) o.scale[row] = tiny ? 1.f : __fdiv_rn(amax, 448.f);
+    }
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       const int c = at.col(t + j * tpr);
@@ -151,38 +178,18 @@ __global__ void __launch_bounds__(WARP_ROWS ? 256 : 1024) add_rms_norm_kernel(co
         float f[8], g[8];
         v[j].to_float(f);
         at.weight(g, w, c);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g[i];
         if (FP8) {
-          float m[8];
+          float q[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) m[i] = f[i];
-          at.mask(m, c);  // (not by the weight's zeros: an infinity of the row before would be a NaN)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(m[i]) & 0x7fffffffu);
+          for (int i = 0; i < 8; ++i) q[i] = f[i] * g[i] * k;
+          at.store_e4m3(q, o.q, c);
         }
         if (!FP8 || o.y != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g[i];
           Vec8<T> ov;
           ov.from_float(f);
           at.store(ov, reinterpret_cast<T*>(o.y), c);
-        }
-      }
-    }
-    if (FP8) {
-      const float amax = __uint_as_float(WARP_ROWS ? __reduce_max_sync(0xffffffffu, top) : block_top(top, red_top));
-      const float s = amax < 0x1p-100f ? 1.f : __fdiv_rn(amax, 448.f);
-      const float inv = __frcp_rn(s);
-      if (t == 0) o.scale[row] = s;
-#pragma unroll
-      for (int j = 0; j < NP; ++j) {
-        const int c = at.col(t + j * tpr);
-        if (c < D) {
-          float f[8], g[8];
-          v[j].to_float(f);
-          at.weight(g, w, c);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g[i] * inv;
-          at.store_e4m3(f, o.q, c);
         }
       }
     }
