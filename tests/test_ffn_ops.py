@@ -415,3 +415,89 @@ def test_costs(mesh_1d):
             + compute._flops(apb.gated_wgrad.default, (), [[2, 5, 2, h], [2, 5, d]], []) + 2.0 * m * n * h)
     assert back == 2 * ffn
     assert compute._flops(apb.gated_mm.default, (), [[2, 5, d], [h, d], [h, d]], []) == 4.0 * m * d * h
+
+
+# ------------------------------------------------------------------------------------ the extension's C entries, without a GPU
+def _entries(code):
+    import os
+    import subprocess
+    import sys
+
+    from autoparallel_b200.ops import build
+
+    if not os.path.exists(build.so_path()):
+        pytest.skip("the extension is not built")
+    head = f"import ctypes, torch\nso = ctypes.CDLL({build.so_path()!r})\nV, LL, F, N = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_float, None\n"
+    r = subprocess.run([sys.executable, "-c", head + code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return r.stdout.split()
+
+
+def test_entries_refuse_what_the_kernels_do_not_take():
+    """Bases off a 16-byte boundary, widths and strides that are not whole vectors, rows past the widest: code 3, nothing launched."""
+    out = _entries("""
+p, bad = V(1 << 20), V((1 << 20) + 8)  # (never read)
+norm = [p, p, p, p, p, p, p, p, LL(4), 64, F(1e-5), 1, N]
+for i in (0, 1, 2, 3, 4, 6):
+    print(so.apb_add_rms_norm(*norm[:i], bad, *norm[i + 1:]))
+print(so.apb_add_rms_norm(*norm[:9], 32769, *norm[10:]), so.apb_add_rms_norm(*norm[:9], 0, *norm[10:]))
+print(so.apb_add_rms_norm(*norm[:3], N, *norm[4:]), so.apb_add_rms_norm(*norm[:4], N, p, N, p, *norm[8:]))  # a residual without h; no result
+back = [p, p, p, p, p, p, p, p, LL(4), 64, 1, 148, N]
+for i in (0, 1, 2, 3, 5):
+    print(so.apb_add_rms_norm_bwd(*back[:i], bad, *back[i + 1:]))
+for f in (so.apb_mx8_quantize, so.apb_mx8_dequantize):
+    for i in (0, 2 if f is so.apb_mx8_dequantize else 1):
+        a = [p, p, p, LL(4), LL(64), 1, N]
+        a[i] = bad
+        print(f(*a))
+    print(f(p, p, p, LL(1 << 31), LL(33), 1, N))
+gated = [p, p, p, p, p, p, 4, 64, 64, LL(64), LL(64), LL(64), 0, p, 148, N]
+for i in (0, 1, 2, 3, 4):
+    print(so.apb_gemm_gated(*gated[:i], bad, *gated[i + 1:]))
+for i in (7, 8):
+    print(so.apb_gemm_gated(*gated[:i], 60, *gated[i + 1:]))
+for i in (9, 10, 11):
+    print(so.apb_gemm_gated(*gated[:i], LL(60), *gated[i + 1:]))
+grad = [p, p, p, p, p, p, 4, 64, 64, LL(64), LL(64), 0, p, 148, N]
+for i in (0, 1, 2, 4, 5):
+    print(so.apb_gemm_gated_grad(*grad[:i], bad, *grad[i + 1:]))
+dual = [p, p, p, p, p, 4, 64, 64, LL(128), LL(64), LL(64), LL(64), p, 148, N]
+for i in (0, 1, 2, 3, 4):
+    print(so.apb_gemm_dual(*dual[:i], bad, *dual[i + 1:]))
+""")
+    assert out == ["3"] * len(out) and len(out) == 6 + 2 + 2 + 5 + 6 + 5 + 2 + 3 + 5 + 5, out
+    out = _entries("""
+p = V(1 << 20)
+print(so.apb_add_rms_norm(p, p, p, p, p, p, N, N, LL(0), 64, F(1e-5), 1, N), so.apb_mx8_quantize(p, p, p, LL(0), LL(5), 1, N),
+      so.apb_gated_act(p, p, LL(0), 4, 0, 1, N))
+so.apb_gemm_set_dynamic_tiles(1)
+print(so.apb_gemm_gated(p, p, p, p, p, p, 4, 64, 64, LL(64), LL(64), LL(64), 0, p, 148, N))
+""")
+    assert out == ["0", "0", "0", "-1"]
+
+
+def test_workspace_of_the_norm_gradient():
+    """A row of partial sums per block; a multiple of eight blocks where rows begin anywhere, so that those of a block begin alike."""
+    cases = [(1, 8, 1), (5, 4096, 1), (8192, 4096, 1), (1, 7, 1), (999, 1001, 0), (3, 32767, 0), (100000, 33, 1), (0, 64, 1)]
+    out = _entries("f = so.apb_add_rms_norm_bwd_workspace\nf.restype = ctypes.c_longlong\n"
+                   f"for rows, d, bf in {cases!r}:\n    print(f(LL(rows), d, bf, 148))")
+    for (rows, d, _), n in zip(cases, map(int, out)):
+        blocks = n // max(d, 1)
+        assert n == blocks * d and (rows == 0) == (n == 0) and blocks <= max(148 * 16, 8) + 8
+        if d % 8 and rows:
+            assert blocks % 8 == 0
+        else:
+            assert blocks <= max(rows, 0)
+
+
+@pytest.mark.parametrize("name", ["add_rms_norm", "add_rms_norm_fp8", "mx8_quantize", "mx8_dequantize", "gated_ffn8", "gated_ffn16"])
+def test_registration(name):
+    """Schema, fake tensors and the traced gradient agree with the operator."""
+    g = _gen(2)
+    x, w = _randn(3, 40, gen=g).requires_grad_(), _randn(40, gen=g).requires_grad_()
+    w1, w3, w2 = (_randn(*s, gen=g).requires_grad_() for s in ((48, 40), (48, 40), (24, 48)))
+    codes, scales = K.mx8_quantize(x.detach())
+    args = {"add_rms_norm": (x, x.detach(), w, 1e-5), "add_rms_norm_fp8": (x, None, w, 1e-5, True), "mx8_quantize": (x.detach(),),
+            "mx8_dequantize": (codes, scales, torch.float32), "gated_ffn8": (x, w1, w3, w2, 1, 8), "gated_ffn16": (x, w1, w3, w2, 0, 16)}[name]
+    op = getattr(ops, name.rstrip("0123456789") if name.startswith("gated") else name).default
+    torch.library.opcheck(op, args, test_utils=("test_schema", "test_autograd_registration", "test_faketensor"))

@@ -540,3 +540,93 @@ def test_refusals():
         ops.add_rms_norm_bwd(x, x[:2], x, x[0], x[:, 0].contiguous())
     with pytest.raises(RuntimeError, match="int8 codes"):
         ops.mx8_dequantize(ab, scales[:1], F32)
+
+
+def test_single_rows_without_leading_dims():
+    g = _gen(31)
+    x = _randn(64, gen=g)
+    w1, w3, w2 = _randn(96, 64, gen=g, scale=0.2), _randn(96, 64, gen=g, scale=0.2), _randn(64, 96, gen=g, scale=0.2)
+    for checkpoint in ("full", "mx8"):
+        leaves = [t.clone().requires_grad_() for t in (x, w1, w3, w2)]
+        y = K.gated_ffn(*leaves, checkpoint=checkpoint)
+        rows = [t.clone().requires_grad_() for t in (x[None], w1, w3, w2)]
+        y2 = K.gated_ffn(*rows, checkpoint=checkpoint)
+        assert y.shape == (64,) and torch.equal(y, y2[0])
+        for a, b in zip(torch.autograd.grad(y.float().sum(), leaves), torch.autograd.grad(y2.float().sum(), rows)):
+            assert torch.equal(a, b.view_as(a))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows are what a call of their own gives."""
+    M, D = 67000, 32768
+    g = _gen(41)
+    tail = _randn(300, D, gen=g)
+    x = torch.empty(M, D, device="cuda", dtype=BF).fill_(0.5)
+    x[-300:] = tail
+    codes, scales = K.mx8_quantize(x)
+    want = K.mx8_quantize(tail)
+    assert torch.equal(codes[-300:], want[0]) and torch.equal(scales[-300:], want[1])
+    y = K.mx8_dequantize(codes, scales)
+    assert torch.equal(y[-300:], K.mx8_dequantize(*want))
+    del codes, scales, y
+    w = (1 + 0.1 * torch.randn(D, device="cuda", generator=g)).to(BF)
+    n, h, rstd = ops.add_rms_norm(x, x, w, 1e-5)
+    n2, h2, rstd2 = ops.add_rms_norm(tail, tail, w, 1e-5)
+    assert torch.equal(n[-300:], n2) and torch.equal(h[-300:], h2)
+    dx, _ = ops.add_rms_norm_bwd(n, x, h, w, rstd)
+    assert torch.equal(dx[-300:], ops.add_rms_norm_bwd(n2, tail, h2, w, rstd2)[0])
+    del dx, n, h, x
+    torch.cuda.empty_cache()
+    x = torch.empty(70000, 31999, device="cuda", dtype=BF).fill_(0.25)  # rows that begin anywhere
+    tail = _randn(8, 31999, gen=g)
+    x[-8:] = tail
+    codes, scales = K.mx8_quantize(x)
+    want = K.mx8_quantize(tail)
+    assert torch.equal(codes[-8:], want[0]) and torch.equal(scales[-8:], want[1])
+    w = torch.ones(31999, device="cuda", dtype=BF)
+    _, _, _, q, scale = ops.add_rms_norm_fp8(x, None, w, 1e-5, False)
+    _, _, _, q2, scale2 = ops.add_rms_norm_fp8(tail, None, w, 1e-5, False)
+    assert torch.equal(q[-8:].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(scale[-8:], scale2)
+    del x, codes, scales, q
+    torch.cuda.empty_cache()
+    M, H = 70016, 16384  # 2 M H of a and b
+    x = torch.zeros(M, 64, device="cuda", dtype=BF)
+    x[-256:] = _randn(256, 64, gen=g)
+    w1, w3, w2 = _randn(H, 64, gen=g, scale=0.1), _randn(H, 64, gen=g, scale=0.1), _randn(64, H, gen=g, scale=0.01)
+    for bits in (16, 8):
+        h, ab, scales = ops.gated_mm(x, w1, w3, 0, bits)
+        a, b = _products(x[-256:], w1, w3)
+        _close(h[-256:], F.silu(a) * b, 1.2 * HALF_STEP[BF])
+        got = K.mx8_dequantize(ab[-256:], scales[-256:], F32) if bits == 8 else ab[-256:]
+        _close(got, torch.stack((a, b), 1), 2.0**-4 if bits == 8 else 1.2 * HALF_STEP[BF])  # (8 bits: at most 2^-7 of a block's top, itself below 8 times the mean square root)
+        dab, h = ops.gated_dgrad(x, w2, ab, scales, 0)
+        few, h2 = ops.gated_dgrad(x[-256:].contiguous(), w2, ab[-256:].contiguous(), scales[-256:].contiguous() if bits == 8 else scales, 0)
+        _close(dab[-256:], few.double(), 2 * HALF_STEP[BF])
+        assert torch.equal(h[-256:], h2)
+        _close(ops.gated_dx(dab, w1, w3)[-256:], ops.gated_dx(dab[-256:].contiguous(), w1, w3).double(), 2 * HALF_STEP[BF])
+        del h, ab, dab
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("checkpoint", ["full", "mx8"])
+def test_llama_with_the_fused_block(checkpoint):
+    """The model's step on the GPU, fused against separate operators, from the same weights."""
+    from autoparallel_b200.models.llama3 import Transformer, llama3_debug
+
+    tokens, labels = (torch.randint(0, 1024, (2, 128), device="cuda", generator=_gen(s)) for s in (1, 2))
+
+    def step(**kw):
+        m = Transformer(llama3_debug(**kw))
+        m.init_weights(0)
+        m = m.to("cuda", BF)
+        m.rope_cos, m.rope_sin = m.rope_cos.float(), m.rope_sin.float()
+        loss = m(tokens, labels)
+        loss.backward()
+        return float(loss), {n: p.grad for n, p in m.named_parameters()}
+
+    loss, grads = step()
+    fused, g2 = step(fused_ffn=True, fused_norm=True, ffn_checkpoint=checkpoint)
+    # bf16 activations of two layers, rounded at about ten places a layer: each 2^-9 of a value on average
+    assert abs(fused - loss) < 20 * 2.0**-9 * abs(loss)
+    for n, g in grads.items():
+        assert torch.isfinite(g2[n]).all() and float((g2[n].double() - g.double()).norm() / g.double().norm()) < 20 * 2.0**-9 * (1 if checkpoint == "full" else 2), n
