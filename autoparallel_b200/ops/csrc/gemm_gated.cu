@@ -136,6 +136,13 @@ static bool off16(std::initializer_list<const void*> ps) {
 
 using namespace apb;
 
+// Whether a call is the few-row kernel's: as a plain product with 2 H columns (0 to 5 % from the better one of both in 96 sizes), and with up to 8 rows and many
+// columns also where the contraction is long, few-row / split kernel, us: 1 x 8192 x 28672 144 / 195, 4 x 8192 x 8192 49 / 57, 8 x 7168 x 9216 46 / 66, 8 x 7168
+// x 18432 86 / 104, 6 x 14336 x 4096 43 / 43; with few columns 8 x 8192 x 2560 22 / 19.
+static bool few_rows(int M, int H, int K, int num_sms) {
+  return M <= 32 && (apb_gemm_rows_takes(M, 2 * H, K, num_sms) || (M <= 8 && H >= 4096));
+}
+
 // ``ab``: null, [M, 2, H] bf16, or with ``scales`` [M, 2, ceil(H / 32)] codes [M, 2, H].  Returns 0, -1 (the caller's plain products), > 0: argument or
 // driver error (nothing launched).
 extern "C" int apb_gemm_gated(const void* x, const void* w1, const void* w3, void* h, void* ab, void* scales, int M, int H, int K, long long ldx,
@@ -144,7 +151,7 @@ extern "C" int apb_gemm_gated(const void* x, const void* w1, const void* w3, voi
   if (no) return no;
   if (off16({x, w1, w3, h, ab}) || ((ldx | ldw1 | ldw3) & 7)) return 3;
   if (H > 0x3fffffff) return 3;
-  if (scales == nullptr && apb_gemm_get_reserved_sms() == 0 && apb_gemm_rows_takes(M, 2 * H, K, num_sms))
+  if (scales == nullptr && apb_gemm_get_reserved_sms() == 0 && few_rows(M, H, K, num_sms))
     return apb_gemm_rows_gated(x, w1, w3, h, ab, M, H, K, ldx, ldw1, ldw3, act, num_sms, stream);
   GatedExt ext{};
   ext.out = GatedOut{(__nv_bfloat16*)h, ab, (uint8_t*)scales, act};
