@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(1024) add_rms_norm_bwd_kernel(const T* dy, con
 __host__ __device__ inline int bwd_slot_bytes(int D, int elem) { return (D % 8 == 0 ? D : (D + 14) / 8 * 8) * elem; }
 __host__ __device__ inline int bwd_ring_bytes(int D, int elem, int stages) { return stages * 3 * bwd_slot_bytes(D, elem) + 128; }
 template <typename T, bool EVEN, int NVEC, int THREADS, int ST>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 && NVEC <= 2 ? 3 : 1)
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? (NVEC == 1 ? 4 : 3) : 1)
 add_rms_norm_bwd_bulk_kernel(const T* dy, const T* dh, const T* h, const T* w, const float* rstd, T* dx, float* part, long long rows, int D) {
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t bars[ST];
@@ -431,8 +431,8 @@ static bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) 
 struct BwdPlan {
   int threads, np, grid, stages, smem;  // vectors of a thread, stages of the ring (0: none)
 };
-// The ring: a warp per row up to 32 vectors, a vector to a thread up to 256 threads, then two, then 512 threads; blocks as shared memory holds, up to 768
-// threads of an SM (1024 of the widest).  At least four rows to a block where there are enough, so that few rows do not leave as many partial rows of dw.
+// The ring: a warp per row up to 32 vectors, a vector to a thread up to 256 threads, then two, then 512 threads; blocks as shared memory holds, up to 1024
+// threads of an SM (768 in small blocks, which leave more partial rows: 8192 x 1024 18.0 -> 19.0 us with 1024, x 2048 32 -> 28, x 4096 50.2 -> 48.5).  At least four rows to a block where there are enough, so that few rows do not leave as many partial rows of dw.
 static BwdPlan bwd_plan(long long rows, int D, int elem, int num_sms) {
   BwdPlan p{};
   const int vecs = row_vectors(D), room = 220 * 1024;
@@ -444,7 +444,8 @@ static BwdPlan bwd_plan(long long rows, int D, int elem, int num_sms) {
     const int np = (vecs + p.threads - 1) / p.threads;
     p.np = np <= 2 ? np : 4;
     p.smem = bwd_ring_bytes(D, elem, p.stages);
-    const int by_smem = room / (p.smem + 2048), by_threads = p.threads == 32 ? 16 : p.threads == 512 ? 2 : 768 / p.threads;
+    // (a block takes 1024 bytes more, and its barriers)
+    const int by_smem = 228 * 1024 / (p.smem + 1536), by_threads = p.threads == 32 ? 16 : (p.threads < 256 ? 768 : 1024) / p.threads;
     per_sm = by_smem < 1 ? 1 : by_smem < by_threads ? by_smem : by_threads;
   } else {
     p.threads = 1024;
