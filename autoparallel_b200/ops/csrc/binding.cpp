@@ -91,9 +91,11 @@ int apb_mx8_quantize(const void* x, void* codes, void* scales, long long R, long
 int apb_mx8_dequantize(const void* codes, const void* scales, void* y, long long R, long long K, int is_bf16, cudaStream_t st);
 int apb_gated_act(const float* ab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st);
 int apb_gated_act_bwd(const float* dh, const float* ab, void* dab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st);
-int apb_gemm_gated(const void* x, const void* w1, const void* w3, void* h, void* ab, void* scales, int M, int H, int K, long long ldx, long long ldw1,
-                   long long ldw3, int act, uint32_t* status, int num_sms, cudaStream_t stream);
-int apb_gemm_gated_grad(const void* dy, const void* w2, const void* ab, const void* scales, void* dab, void* h, int M, int H, int K, long long ldy,
+int apb_mx16_quantize(const float* x, void* codes, void* scales, long long R, int K, cudaStream_t st);
+int apb_mx16_dequantize(const void* codes, const void* scales, float* y, long long R, int K, cudaStream_t st);
+int apb_gemm_gated(const void* x, const void* w1, const void* w3, void* h, void* ab, void* scales, int bits, int M, int H, int K, long long ldx,
+                   long long ldw1, long long ldw3, int act, uint32_t* status, int num_sms, cudaStream_t stream);
+int apb_gemm_gated_grad(const void* dy, const void* w2, const void* ab, const void* scales, int bits, void* dab, void* h, int M, int H, int K, long long ldy,
                         long long ldw, int act, uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_gemm_dual(const void* a1, const void* a2, const void* b1, const void* b2, void* C, int M, int N, int K, long long lda, long long ldb1, long long ldb2,
                   long long ldc, uint32_t* status, int num_sms, cudaStream_t stream);

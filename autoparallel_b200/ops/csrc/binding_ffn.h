@@ -78,14 +78,14 @@ Two mx8_quantize(const Tensor& x_) {
   count(x.numel() > 0);
   return {codes, scales};
 }
-void mx8_check(const Tensor& codes, const Tensor& scales, const char* what) {
-  TORCH_CHECK(codes.scalar_type() == at::kChar && scales.scalar_type() == at::kByte && codes.dim() >= 1 && scales.device() == codes.device() &&
+void mx_check(const Tensor& codes, const Tensor& scales, at::ScalarType type, const char* what) {
+  TORCH_CHECK(codes.scalar_type() == type && scales.scalar_type() == at::kByte && codes.dim() >= 1 && scales.device() == codes.device() &&
                   scales.sizes() == at::IntArrayRef(with_last(lead_of(codes), {mx_blocks(codes.size(-1))})),
-              what, ": int8 codes [.., K] and uint8 scales [.., ceil(K / 32)]");
+              what, ": ", type == at::kChar ? "int8" : "int16", " codes [.., K] and uint8 scales [.., ceil(K / 32)]");
 }
 Tensor mx8_dequantize(const Tensor& codes_, const Tensor& scales_, at::ScalarType dtype) {
   c10::cuda::CUDAGuard g(codes_.device());
-  mx8_check(codes_, scales_, "mx8_dequantize");
+  mx_check(codes_, scales_, at::kChar, "mx8_dequantize");
   TORCH_CHECK(float_or_bf16(dtype), "mx8_dequantize: bf16 or fp32");
   Tensor codes = dense(codes_), scales = scales_.contiguous(), y = at::empty(codes.sizes(), codes.options().dtype(dtype));
   const int64_t K = codes.size(-1);
@@ -129,14 +129,13 @@ std::tuple<Tensor, Tensor, Tensor> gated_mm(const Tensor& x, const Tensor& w1, c
   const auto u8 = x.options().dtype(at::kByte);
   Tensor h = at::empty(with_last(lead, {H}), x.options()), ab = at::empty({0}, x.options()), scales = at::empty({0}, u8);
   if (gated_form({&x}, {D, H}) && M > 0 && M <= 0x7fffffff) {
-    if (bits == 16) ab = at::empty(with_last(lead, {2, H}), x.options());
-    if (bits == 8) {
-      ab = at::empty(with_last(lead, {2, H}), x.options().dtype(at::kChar));
+    if (bits) {
+      ab = at::empty(with_last(lead, {2, H}), x.options().dtype(bits == 8 ? at::kChar : at::kShort));
       scales = at::empty(with_last(lead, {2, mx_blocks(H)}), u8);
     }
     Tensor x2 = as2d(x), a = as2d(w1), b = as2d(w3);
     const int err = apb_gemm_gated(x2.data_ptr(), a.data_ptr(), b.data_ptr(), h.data_ptr(), bits ? ab.data_ptr() : nullptr,
-                                   bits == 8 ? scales.data_ptr() : nullptr, (int)M, (int)H, (int)D, x2.stride(0), a.stride(0), b.stride(0), (int)act,
+                                   bits ? scales.data_ptr() : nullptr, (int)bits, (int)M, (int)H, (int)D, x2.stride(0), a.stride(0), b.stride(0), (int)act,
                                    status_word(x), num_sms(), stream());
     if (err == 0) count();
     if (err == 0) return {h, ab, scales};
@@ -145,8 +144,14 @@ std::tuple<Tensor, Tensor, Tensor> gated_mm(const Tensor& x, const Tensor& w1, c
   Tensor both = at::stack({product32(x, w1, true), product32(x, w3, true)}, 1);  // [M, 2, H]
   check(apb_gated_act(both.data_ptr<float>(), h.data_ptr(), M, (int)H, (int)act, is_bf16(x), stream()), "apb_gated_act");
   count(both.numel() > 0);
-  if (bits == 16) ab = both.to(x.scalar_type()).view(with_last(lead, {2, H}));
-  if (bits == 8) {
+  if (bits == 16 && x.scalar_type() == at::kFloat) {
+    ab = both.view(with_last(lead, {2, H}));
+  } else if (bits == 16) {
+    ab = at::empty(with_last(lead, {2, H}), x.options().dtype(at::kShort));
+    scales = at::empty(with_last(lead, {2, mx_blocks(H)}), u8);
+    check(apb_mx16_quantize(both.data_ptr<float>(), ab.data_ptr(), scales.data_ptr(), 2 * M, (int)H, stream()), "apb_mx16_quantize");
+    count(both.numel() > 0);
+  } else if (bits == 8) {
     auto [c, s] = mx8_quantize(both);
     ab = c.view(with_last(lead, {2, H}));
     scales = s.view(with_last(lead, {2, mx_blocks(H)}));
@@ -157,23 +162,33 @@ std::tuple<Tensor, Tensor, Tensor> gated_mm(const Tensor& x, const Tensor& w1, c
 Two gated_dgrad(const Tensor& dy, const Tensor& w2, const Tensor& ab_, const Tensor& scales_, int64_t act) {
   c10::cuda::CUDAGuard g(dy.device());
   gated_check(dy, {&w2}, "gated_dgrad");
-  const bool eight = ab_.scalar_type() == at::kChar;
+  const bool eight = ab_.scalar_type() == at::kChar, codes = dy.scalar_type() == at::kBFloat16 || eight;
   const int64_t N = dy.size(-1), H = w2.size(1), M = rows_of(dy, 1);
   TORCH_CHECK(w2.size(0) == N && ab_.sizes() == at::IntArrayRef(with_last(lead_of(dy), {2, H})) && ab_.device() == dy.device() &&
-                  (eight || ab_.scalar_type() == dy.scalar_type()),
-              "gated_dgrad: dy [.., N], w2 [N, H], ab [.., 2, H] of dy's type or int8");
-  if (eight) mx8_check(ab_, scales_, "gated_dgrad");
+                  (codes || ab_.scalar_type() == at::kFloat),
+              "gated_dgrad: dy [.., N], w2 [N, H], ab [.., 2, H] in 8 bits, or in 16 for bf16 and fp32 for fp32");
+  if (codes) mx_check(ab_, scales_, eight ? at::kChar : at::kShort, "gated_dgrad");
   TORCH_CHECK(act >= 0 && act <= 2, "gated_dgrad: act 0 to 2");
   Tensor dab = at::empty(ab_.sizes(), dy.options()), h = at::empty(with_last(lead_of(dy), {H}), dy.options());
   if (gated_form({&dy}, {N, H}) && M > 0 && M <= 0x7fffffff) {
-    Tensor a = as2d(dy), b = as2d(w2), ab = dense(ab_), scales = eight ? scales_.contiguous() : Tensor();
-    const int err = apb_gemm_gated_grad(a.data_ptr(), b.data_ptr(), ab.data_ptr(), eight ? scales.data_ptr() : nullptr, dab.data_ptr(), h.data_ptr(), (int)M,
-                                        (int)H, (int)N, a.stride(0), b.stride(0), (int)act, status_word(dy), num_sms(), stream());
+    Tensor a = as2d(dy), b = as2d(w2), ab = dense(ab_), scales = scales_.contiguous();
+    const int err = apb_gemm_gated_grad(a.data_ptr(), b.data_ptr(), ab.data_ptr(), scales.data_ptr(), eight ? 8 : 16, dab.data_ptr(), h.data_ptr(),
+                                        (int)M, (int)H, (int)N, a.stride(0), b.stride(0), (int)act, status_word(dy), num_sms(), stream());
     if (err == 0) count();
     if (err == 0) return {dab, h};
     if (err > 0) check(err, "apb_gemm_gated_grad");
   }
-  Tensor dh = product32(dy, w2, false), v = (eight ? mx8_dequantize(ab_, scales_, at::kFloat) : ab_.to(at::kFloat)).contiguous();
+  Tensor dh = product32(dy, w2, false), v;
+  if (eight) {
+    v = mx8_dequantize(ab_, scales_, at::kFloat);
+  } else if (codes) {
+    Tensor c = ab_.contiguous(), s = scales_.contiguous();
+    v = at::empty(c.sizes(), c.options().dtype(at::kFloat));
+    check(apb_mx16_dequantize(c.data_ptr(), s.data_ptr(), v.data_ptr<float>(), 2 * M, (int)H, stream()), "apb_mx16_dequantize");
+    count(v.numel() > 0);
+  } else {
+    v = ab_.contiguous();
+  }
   check(apb_gated_act_bwd(dh.data_ptr<float>(), v.data_ptr<float>(), dab.data_ptr(), h.data_ptr(), M, (int)H, (int)act, is_bf16(dy), stream()),
         "apb_gated_act_bwd");
   count(dh.numel() > 0);

@@ -1,11 +1,12 @@
 // The middle of a gated feed-forward block: h = act(a) * b with a = x w1^T and b = x w3^T, and its derivative, as the ends of two products.
 //
 //   forward    both projections come out of one product, a and b of the same column of h in the same thread; h leaves in bf16, and for the backward
-//              pass a and b, in bf16 or as 8-bit codes (mx8.cuh)
+//              pass a and b, as codes of 8 or 16 bits (mx8.cuh): in as many bits as bf16 they are off by 2^-15 of a block's largest value and not by 2^-9 of
+//              each, and the gradients by 0.0024 and not 0.0034 of their size (both: da, db and the results are rounded to bf16)
 //   backward   dh = dy w2 stays in fp32; da = dh b act'(a) and db = dh act(a) leave in bf16, and h, made again, for the gradient of w2
 //
-// ab, dab [M, 2, H]: a row of a (da), then the same row of b (db), so that one product makes the gradients of both weights.  Codes lie in the same way, the
-// scales are [M, 2, ceil(H / 32)].  H % 8 == 0.
+// ab, dab [M, 2, H]: a row of a (da), then the same row of b (db), so that one product makes the gradients of both weights.  The scales of codes are
+// [M, 2, ceil(H / 32)].  H % 8 == 0.
 #pragma once
 #include <type_traits>
 
@@ -62,12 +63,12 @@ __device__ __forceinline__ float act_value(float a, float& d) {
 
 struct GatedOut {  // forward
   __nv_bfloat16* h;
-  void* ab;         // bf16, or codes; null: not kept
-  uint8_t* scales;  // of codes; null: bf16
-  int act;
+  void* ab;  // codes; null: not kept
+  uint8_t* scales;
+  int act, bits;  // of a code
 };
 struct GatedGrad {  // backward
-  const void* ab;
+  const void* ab;  // codes
   const uint8_t* scales;
   __nv_bfloat16 *dab, *h;
   int act;
@@ -113,26 +114,20 @@ __device__ __forceinline__ void stage_store8(const uint8_t* stg, uint8_t* dst, l
   }
 }
 
-__device__ __forceinline__ void unpack8(const uint4& v, float* f) {  // (a bf16 is the upper half of its fp32)
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// 32 values of a thread to codes in its row of the staging block; the scale byte
+template <int BITS>
+__device__ __forceinline__ uint32_t codes32(const uint32_t (&r)[32], uint8_t* stg, int lane) {
+  const uint32_t top = mx_top(r), byte = mx_scale_byte<BITS>(top);
+  const MxCoder<BITS> coder(byte, top);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    const uint32_t* v = r + 8 * i;
+    if constexpr (BITS == 8)
+      *reinterpret_cast<uint2*>(stg + stage32(lane, i)) = make_uint2(coder.four(v[0], v[1], v[2], v[3]), coder.four(v[4], v[5], v[6], v[7]));
+    else
+      *reinterpret_cast<uint4*>(stg + stage64(lane, i)) =
+          make_uint4(coder.two(v[0], v[1]), coder.two(v[2], v[3]), coder.two(v[4], v[5]), coder.two(v[6], v[7]));
   }
-}
-__device__ __forceinline__ void pack32(const uint32_t (&r)[32], uint32_t (&v)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = pack_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-}
-// 32 values of a thread to codes in its row of the staging block; the scale byte
-__device__ __forceinline__ uint32_t codes32(const uint32_t (&r)[32], uint8_t* stg, int lane) {
-  const uint32_t byte = mx8_scale_byte(mx8_top(r));
-  const Mx8Coder coder(byte, mx8_top(r));
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<uint2*>(stg + stage32(lane, i)) =
-        make_uint2(coder.four(r[8 * i], r[8 * i + 1], r[8 * i + 2], r[8 * i + 3]), coder.four(r[8 * i + 4], r[8 * i + 5], r[8 * i + 6], r[8 * i + 7]));
   return byte;
 }
 
@@ -145,7 +140,7 @@ __device__ __forceinline__ void gated_tile(const GatedOut& o, uint8_t* stg, uint
     release();
     return;
   }
-  const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
+  const int blocks = (H + MX_BLOCK - 1) / MX_BLOCK;
 #pragma unroll 1
   for (int c = 0; c < used; c += 32) {
     uint32_t a[32], b[32], v[16];
@@ -165,41 +160,40 @@ __device__ __forceinline__ void gated_tile(const GatedOut& o, uint8_t* stg, uint
     });
     __syncwarp();  // what was there before has been read
     stage_put(stg, lane, v);
+    uint32_t sa = 0, sb = 0;
     if (o.ab != nullptr) {
-      if (o.scales != nullptr) {
-        const uint32_t sa = codes32(a, stg + 2048, lane), sb = codes32(b, stg + 3072, lane);
-        if (row0 + lane < M) {
-          uint8_t* s = o.scales + (long long)(row0 + lane) * 2 * blocks + (col + c) / MX8_BLOCK;
-          s[0] = (uint8_t)sa;
-          s[blocks] = (uint8_t)sb;
-        }
+      if (o.bits == 8) {
+        sa = codes32<8>(a, stg + 2048, lane);
+        sb = codes32<8>(b, stg + 3072, lane);
       } else {
-        pack32(a, v);
-        stage_put(stg + 2048, lane, v);
+        sa = codes32<16>(a, stg + 2048, lane);
       }
     }
     __syncwarp();
     stage_store(stg, o.h, H, row0, col + c, M, H, lane);
-    if (o.ab != nullptr) {
-      if (o.scales != nullptr) {
-        uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab);
-        stage_store8(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);
-        stage_store8(stg + 3072, codes + H, 2ll * H, row0, col + c, M, H, lane);
-      } else {
-        __nv_bfloat16* ab = reinterpret_cast<__nv_bfloat16*>(o.ab);
-        stage_store(stg + 2048, ab, 2ll * H, row0, col + c, M, H, lane);
-        pack32(b, v);
-        __syncwarp();
-        stage_put(stg, lane, v);
-        __syncwarp();
-        stage_store(stg, ab + H, 2ll * H, row0, col + c, M, H, lane);
-      }
+    if (o.ab == nullptr) continue;
+    if (o.bits == 8) {
+      uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab);
+      stage_store8(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);
+      stage_store8(stg + 3072, codes + H, 2ll * H, row0, col + c, M, H, lane);
+    } else {
+      __nv_bfloat16* codes = reinterpret_cast<__nv_bfloat16*>(o.ab);  // (two bytes each)
+      stage_store(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);
+      __syncwarp();
+      sb = codes32<16>(b, stg, lane);
+      __syncwarp();
+      stage_store(stg, codes + H, 2ll * H, row0, col + c, M, H, lane);
+    }
+    if (row0 + lane < M) {
+      uint8_t* s = o.scales + (long long)(row0 + lane) * 2 * blocks + (col + c) / MX_BLOCK;
+      s[0] = (uint8_t)sa;
+      s[blocks] = (uint8_t)sb;
     }
   }
 }
 
 // The values a and b of a warp's 32 rows and 32 columns, on their way from memory to its staging block while the product is under way: whole rows, four
-// lanes to one; rows and columns past the matrix are zeros.  bf16: a's 32 x 64 bytes, then b's; codes: 32 x 32 bytes each.
+// lanes to one; rows and columns past the matrix are zeros.  16 bits: a's 32 x 64 bytes, then b's; 8 bits: 32 x 32 bytes each.
 __device__ __forceinline__ void copy_async16(uint8_t* dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
@@ -207,21 +201,21 @@ __device__ __forceinline__ void copy_async8(uint8_t* dst, const void* src, bool 
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 8 : 0) : "memory");
 }
 __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-template <bool EIGHT>
+template <int BITS>
 struct AbFetch {
   uint32_t sa, sb;  // scale bytes of this thread's row
   __device__ __forceinline__ void start(const GatedGrad& g, uint8_t* stg, int row0, int col, int M, int H, int lane) {
     const int unit = lane & 3, sub = lane >> 2;
     const bool in = col + unit * 8 < H;
     const uint8_t* ab = reinterpret_cast<const uint8_t*>(g.ab);
-    constexpr int SIZE = EIGHT ? 1 : 2;
+    constexpr int SIZE = BITS / 8;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = sub + 8 * j;
       const bool ok = in && row0 + row < M;
       const uint8_t* src = ab + (ok ? (long long)(row0 + row) * 2 * H + col + unit * 8 : 0) * SIZE;  // (not read where it is not inside)
       const long long b = ok ? (long long)H * SIZE : 0;
-      if (EIGHT) {
+      if (BITS == 8) {
         copy_async8(stg + stage32(row, unit), src, ok);
         copy_async8(stg + 1024 + stage32(row, unit), src + b, ok);
       } else {
@@ -229,14 +223,12 @@ struct AbFetch {
         copy_async16(stg + 2048 + stage64(row, unit), src + b, ok);
       }
     }
-    if (EIGHT) {
-      sa = sb = MX8_LOWEST;
-      if (row0 + lane < M && col < H) {
-        const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
-        const uint8_t* s = g.scales + (long long)(row0 + lane) * 2 * blocks + col / MX8_BLOCK;
-        sa = s[0];
-        sb = s[blocks];
-      }
+    sa = sb = MX_LOWEST<BITS>;
+    if (row0 + lane < M && col < H) {
+      const int blocks = (H + MX_BLOCK - 1) / MX_BLOCK;
+      const uint8_t* s = g.scales + (long long)(row0 + lane) * 2 * blocks + col / MX_BLOCK;
+      sa = s[0];
+      sb = s[blocks];
     }
   }
 };
@@ -252,8 +244,8 @@ __device__ __forceinline__ void gated_grad(float dh, float a, float b, float& da
 }
 
 // Backward: columns col ... of dh from the accumulator at ``taddr``.  ``fetch`` has started to bring the first 32 columns of a and b into ``stg``.
-template <bool EIGHT, typename Release>
-__device__ __forceinline__ void gated_grad_tile(const GatedGrad& g, AbFetch<EIGHT>& fetch, uint8_t* stg, uint32_t taddr, int row0, int col, int ncols, int M,
+template <int BITS, typename Release>
+__device__ __forceinline__ void gated_grad_tile(const GatedGrad& g, AbFetch<BITS>& fetch, uint8_t* stg, uint32_t taddr, int row0, int col, int ncols, int M,
                                                 int H, int lane, Release release) {
   const int used = row0 < M ? min(ncols, H - col) : 0;
   copy_async_wait();
@@ -267,15 +259,13 @@ __device__ __forceinline__ void gated_grad_tile(const GatedGrad& g, AbFetch<EIGH
     tmem_ld_32x32(taddr + c, r);
     copy_async_wait();
     __syncwarp();
-    uint2 ca[EIGHT ? 4 : 1], cb[EIGHT ? 4 : 1];
-    Mx8Reader ra, rb;
-    if (EIGHT) {  // (this thread's codes, before da and db take their place)
-      ra = Mx8Reader(fetch.sa);
-      rb = Mx8Reader(fetch.sb);
+    const MxReader<BITS> ra(fetch.sa), rb(fetch.sb);
+    uint2 ca[BITS == 8 ? 4 : 1], cb[BITS == 8 ? 4 : 1];
+    if constexpr (BITS == 8) {  // (this thread's codes, before da and db take their place)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        ca[i % (EIGHT ? 4 : 1)] = *reinterpret_cast<const uint2*>(stg + stage32(lane, i));
-        cb[i % (EIGHT ? 4 : 1)] = *reinterpret_cast<const uint2*>(stg + 1024 + stage32(lane, i));
+        ca[i] = *reinterpret_cast<const uint2*>(stg + stage32(lane, i));
+        cb[i] = *reinterpret_cast<const uint2*>(stg + 1024 + stage32(lane, i));
       }
       __syncwarp();
     }
@@ -287,15 +277,19 @@ __device__ __forceinline__ void gated_grad_tile(const GatedGrad& g, AbFetch<EIGH
         uint4* pa = reinterpret_cast<uint4*>(stg + stage64(lane, i));
         uint4* pb = reinterpret_cast<uint4*>(stg + 2048 + stage64(lane, i));
         float a[8], b[8];
-        if (EIGHT) {
-          ra.four(ca[i % (EIGHT ? 4 : 1)].x, a);
-          ra.four(ca[i % (EIGHT ? 4 : 1)].y, a + 4);
-          rb.four(cb[i % (EIGHT ? 4 : 1)].x, b);
-          rb.four(cb[i % (EIGHT ? 4 : 1)].y, b + 4);
+        if constexpr (BITS == 8) {
+          ra.four(ca[i].x, a);
+          ra.four(ca[i].y, a + 4);
+          rb.four(cb[i].x, b);
+          rb.four(cb[i].y, b + 4);
         } else {
           const uint4 x = *pa, y = *pb;
-          unpack8(x, a);
-          unpack8(y, b);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            ra.two(xs[k], a + 2 * k);
+            rb.two(ys[k], b + 2 * k);
+          }
         }
         float da[8], db[8], v[8];
 #pragma unroll
@@ -320,20 +314,19 @@ __device__ __forceinline__ void gated_grad_tile(const GatedGrad& g, AbFetch<EIGH
 
 // ---------------------------------------------------------------------------- four columns of a row to a thread, eight threads to 32 columns
 __device__ __forceinline__ uint2 pack4(const float (&v)[4]) { return make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); }
-__device__ __forceinline__ void unpack4(uint2 p, float (&v)[4]) {
-  v[0] = __uint_as_float(p.x << 16); v[1] = __uint_as_float(p.x & 0xffff0000u);
-  v[2] = __uint_as_float(p.y << 16); v[3] = __uint_as_float(p.y & 0xffff0000u);
-}
-// The eight threads come together, those with columns past the matrix (whose a and b are zeros) among them.
-__device__ __forceinline__ uint32_t codes4(const float (&v)[4], uint32_t& byte) {
+// The eight threads come together, those with columns past the matrix (whose a and b are zeros) among them.  8 bits: the codes in .x.
+template <int BITS>
+__device__ __forceinline__ uint2 codes4(const float (&v)[4], uint32_t& byte) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
   const uint32_t eight = 0xffu << (threadIdx.x & 24);
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(eight, top, o));
-  byte = mx8_scale_byte(top);
-  return Mx8Coder(byte, top).four(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  byte = mx_scale_byte<BITS>(top);
+  const MxCoder<BITS> coder(byte, top);
+  const uint32_t w[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+  return BITS == 8 ? make_uint2(coder.four(w[0], w[1], w[2], w[3]), 0) : make_uint2(coder.two(w[0], w[1]), coder.two(w[2], w[3]));
 }
 __device__ __forceinline__ void gated_four(const GatedOut& o, long long row, int col, int H, const float (&a)[4], const float (&b)[4]) {
   float h[4];
@@ -347,57 +340,61 @@ __device__ __forceinline__ void gated_four(const GatedOut& o, long long row, int
   const bool in = col < H;
   if (in) *reinterpret_cast<uint2*>(o.h + row * H + col) = pack4(h);
   if (o.ab == nullptr) return;
-  if (o.scales != nullptr) {
-    uint32_t sa, sb;
-    const uint32_t ca = codes4(a, sa), cb = codes4(b, sb);
+  uint32_t sa, sb;
+  const long long at = row * 2 * H + col;
+  if (o.bits == 8) {
+    const uint2 ca = codes4<8>(a, sa), cb = codes4<8>(b, sb);
     if (!in) return;
-    const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
-    uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab) + row * 2 * H + col;
-    *reinterpret_cast<uint32_t*>(codes) = ca;
-    *reinterpret_cast<uint32_t*>(codes + H) = cb;
-    if (col % MX8_BLOCK == 0) {
-      uint8_t* s = o.scales + row * 2 * blocks + col / MX8_BLOCK;
-      s[0] = (uint8_t)sa;
-      s[blocks] = (uint8_t)sb;
-    }
-  } else if (in) {
-    __nv_bfloat16* ab = reinterpret_cast<__nv_bfloat16*>(o.ab) + row * 2 * H + col;
-    *reinterpret_cast<uint2*>(ab) = pack4(a);
-    *reinterpret_cast<uint2*>(ab + H) = pack4(b);
+    uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab) + at;
+    *reinterpret_cast<uint32_t*>(codes) = ca.x;
+    *reinterpret_cast<uint32_t*>(codes + H) = cb.x;
+  } else {
+    const uint2 ca = codes4<16>(a, sa), cb = codes4<16>(b, sb);
+    if (!in) return;
+    uint16_t* codes = reinterpret_cast<uint16_t*>(o.ab) + at;
+    *reinterpret_cast<uint2*>(codes) = ca;
+    *reinterpret_cast<uint2*>(codes + H) = cb;
+  }
+  if (col % MX_BLOCK == 0) {
+    const int blocks = (H + MX_BLOCK - 1) / MX_BLOCK;
+    uint8_t* s = o.scales + row * 2 * blocks + col / MX_BLOCK;
+    s[0] = (uint8_t)sa;
+    s[blocks] = (uint8_t)sb;
   }
 }
-// a and b of four columns as they lie in memory (codes: .x), and the scale bytes
+// a and b of four columns as they lie in memory (8 bits: .x), and the scale bytes
+template <int BITS>
 struct AbFour {
   uint2 a, b;
   uint32_t sa, sb;
-  template <bool EIGHT>
   __device__ __forceinline__ void load(const GatedGrad& g, long long row, int col, int H) {
-    const long long at = row * 2 * H + col;
-    if (EIGHT) {
-      const int blocks = (H + MX8_BLOCK - 1) / MX8_BLOCK;
-      const uint8_t* s = g.scales + row * 2 * blocks + col / MX8_BLOCK;
-      const uint8_t* codes = reinterpret_cast<const uint8_t*>(g.ab) + at;
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(g.ab) + (row * 2 * H + col) * (BITS / 8);
+    if (BITS == 8) {
       a.x = *reinterpret_cast<const uint32_t*>(codes);
       b.x = *reinterpret_cast<const uint32_t*>(codes + H);
-      sa = s[0];
-      sb = s[blocks];
     } else {
-      const __nv_bfloat16* ab = reinterpret_cast<const __nv_bfloat16*>(g.ab) + at;
-      a = *reinterpret_cast<const uint2*>(ab);
-      b = *reinterpret_cast<const uint2*>(ab + H);
+      a = *reinterpret_cast<const uint2*>(codes);
+      b = *reinterpret_cast<const uint2*>(codes + 2ll * H);
     }
+    const int blocks = (H + MX_BLOCK - 1) / MX_BLOCK;
+    const uint8_t* s = g.scales + row * 2 * blocks + col / MX_BLOCK;
+    sa = s[0];
+    sb = s[blocks];
   }
 };
-template <bool EIGHT>
-__device__ __forceinline__ void gated_grad_four(const GatedGrad& g, const AbFour& ab, long long row, int col, int H, const float (&dh)[4]) {
+template <int BITS>
+__device__ __forceinline__ void gated_grad_four(const GatedGrad& g, const AbFour<BITS>& ab, long long row, int col, int H, const float (&dh)[4]) {
   float a[4], b[4], da[4], db[4], h[4];
   const long long at = row * 2 * H + col;
-  if (EIGHT) {
-    Mx8Reader(ab.sa).four(ab.a.x, a);
-    Mx8Reader(ab.sb).four(ab.b.x, b);
+  const MxReader<BITS> ra(ab.sa), rb(ab.sb);
+  if (BITS == 8) {
+    ra.four(ab.a.x, a);
+    rb.four(ab.b.x, b);
   } else {
-    unpack4(ab.a, a);
-    unpack4(ab.b, b);
+    ra.two(ab.a.x, a);
+    ra.two(ab.a.y, a + 2);
+    rb.two(ab.b.x, b);
+    rb.two(ab.b.y, b + 2);
   }
   with_act(g.act, [&](auto act) {
 #pragma unroll

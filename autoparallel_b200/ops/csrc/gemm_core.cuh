@@ -113,10 +113,10 @@ struct GatedExt {
   CUtensorMap tmB2;
   GatedOut out;
 };
-template <bool EIGHT_BITS>
+template <int CODE_BITS>
 struct GradExt {
   static constexpr int KIND = EXT_GRAD;
-  static constexpr bool EIGHT = EIGHT_BITS;
+  static constexpr int BITS = CODE_BITS;
   GatedGrad grad;
 };
 struct DualExt {
@@ -125,9 +125,9 @@ struct DualExt {
 };
 
 template <typename Ext>
-constexpr bool ext_eight() {
-  if constexpr (Ext::KIND == EXT_GRAD) return Ext::EIGHT;
-  else return false;
+constexpr int ext_bits() {
+  if constexpr (Ext::KIND == EXT_GRAD) return Ext::BITS;
+  else return 8;
 }
 
 struct FuseParams {
@@ -899,7 +899,7 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
       for (int sub = 0; sub < (NARROW ? x.subs : 1); ++sub, ++seq) {
         const uint32_t buf = seq & 1u;
         const long long cta_row0 = (long long)x.tm * TM + (long long)half * BM;  // first of this CTA's 128 rows
-        [[maybe_unused]] std::conditional_t<EXT == EXT_GRAD, AbFetch<ext_eight<Ext>()>, int> fetch;
+        [[maybe_unused]] std::conditional_t<EXT == EXT_GRAD, AbFetch<ext_bits<Ext>()>, int> fetch;
         [[maybe_unused]] uint8_t* stg = smem + ST * (A_BYTES + B_BYTES) + (warp - 2) * STORE_BYTES;
         if constexpr (EXT == EXT_GRAD) {  // (on their way while the product is; the warp has read out what was there before)
           __syncwarp();
@@ -952,7 +952,7 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
             const uint32_t ta = tmem_base + (uint32_t(q * 32) << 16) + buf * BN + first;
             gated_tile(ext.out, stg, ta, ta + 2 * both, r0, (x.col + sub * BN) / 2 + first, both, p.M, p.N / 2, lane, release);
           } else {
-            gated_grad_tile<Ext::EIGHT>(ext.grad, fetch, stg, taddr, r0, n0, cols, p.M, p.N, lane, release);
+            gated_grad_tile<Ext::BITS>(ext.grad, fetch, stg, taddr, r0, n0, cols, p.M, p.N, lane, release);
           }
           continue;
         }

@@ -1,6 +1,6 @@
 // The products of a gated feed-forward block, sm_100a:
 //
-//   apb_gemm_gated        h = act(x w1^T) * (x w3^T), and x w1^T, x w3^T themselves in bf16 or as 8-bit codes     x [M, K], w [H, K]
+//   apb_gemm_gated        h = act(x w1^T) * (x w3^T), and codes of x w1^T and x w3^T                               x [M, K], w [H, K]
 //   apb_gemm_gated_grad   from dh = dy w2: da, db and h again (gated.cuh)                                            dy [M, K], w2 [K, H]
 //   apb_gemm_dual         dx = da w1 + db w3                                                                         da, db [M, K], w [K, N]
 //
@@ -16,8 +16,8 @@ int apb_gemm_get_pair_stages();
 int apb_gemm_get_pair_mode();
 void apb_gemm_split_choice(int G, int M, int N, int K, int num_sms, int reserved, int* bn, int* s);
 int apb_gemm_rows_takes(int M, int N, int K, int num_sms);
-int apb_gemm_rows_gated(const void* X, const void* W1, const void* W3, void* h, void* ab, int M, int H, int K, long long ldx, long long ldw1,
-                        long long ldw3, int act, int num_sms, cudaStream_t st);
+int apb_gemm_rows_gated(const void* X, const void* W1, const void* W3, void* h, int M, int H, int K, long long ldx, long long ldw1, long long ldw3,
+                        int act, int num_sms, cudaStream_t st);
 }
 
 namespace apb {
@@ -143,32 +143,32 @@ static bool few_rows(int M, int H, int K, int num_sms) {
   return M <= 32 && (apb_gemm_rows_takes(M, 2 * H, K, num_sms) || (M <= 8 && H >= 4096));
 }
 
-// ``ab``: null, [M, 2, H] bf16, or with ``scales`` [M, 2, ceil(H / 32)] codes [M, 2, H].  Returns 0, -1 (the caller's plain products), > 0: argument or
+// ``bits`` 0, or 8 or 16: the codes ``ab`` [M, 2, H] and ``scales`` [M, 2, ceil(H / 32)] are kept.  Returns 0, -1 (the caller's plain products), > 0: argument or
 // driver error (nothing launched).
-extern "C" int apb_gemm_gated(const void* x, const void* w1, const void* w3, void* h, void* ab, void* scales, int M, int H, int K, long long ldx,
-                              long long ldw1, long long ldw3, int act, uint32_t* status, int num_sms, cudaStream_t stream) {
+extern "C" int apb_gemm_gated(const void* x, const void* w1, const void* w3, void* h, void* ab, void* scales, int bits, int M, int H, int K,
+                              long long ldx, long long ldw1, long long ldw3, int act, uint32_t* status, int num_sms, cudaStream_t stream) {
   const int no = ext_takes(M, H, K);
   if (no) return no;
   if (off16({x, w1, w3, h, ab}) || ((ldx | ldw1 | ldw3) & 7)) return 3;
-  if (H > 0x3fffffff) return 3;
-  if (scales == nullptr && apb_gemm_get_reserved_sms() == 0 && few_rows(M, H, K, num_sms))
-    return apb_gemm_rows_gated(x, w1, w3, h, ab, M, H, K, ldx, ldw1, ldw3, act, num_sms, stream);
+  if (H > 0x3fffffff || (bits != 0 && bits != 8 && bits != 16) || (bits != 0 && (ab == nullptr || scales == nullptr))) return 3;
+  if (bits == 0 && apb_gemm_get_reserved_sms() == 0 && few_rows(M, H, K, num_sms))
+    return apb_gemm_rows_gated(x, w1, w3, h, M, H, K, ldx, ldw1, ldw3, act, num_sms, stream);
   GatedExt ext{};
-  ext.out = GatedOut{(__nv_bfloat16*)h, ab, (uint8_t*)scales, act};
+  ext.out = GatedOut{(__nv_bfloat16*)h, bits ? ab : nullptr, (uint8_t*)scales, act, bits};
   return launch_ext<false>(Operand{x, K, M, ldx}, Operand{w1, K, H, ldw1}, ext_params(M, 2 * H, K, status), ext, num_sms, stream,
                            [&](GatedExt& e, int box) { return Operand{w3, K, H, ldw3}.map(&e.tmB2, box); });
 }
 
-extern "C" int apb_gemm_gated_grad(const void* dy, const void* w2, const void* ab, const void* scales, void* dab, void* h, int M, int H, int K,
-                                   long long ldy, long long ldw, int act, uint32_t* status, int num_sms, cudaStream_t stream) {
+extern "C" int apb_gemm_gated_grad(const void* dy, const void* w2, const void* ab, const void* scales, int bits, void* dab, void* h, int M, int H,
+                                   int K, long long ldy, long long ldw, int act, uint32_t* status, int num_sms, cudaStream_t stream) {
   const int no = ext_takes(M, H, K);
   if (no) return no;
-  if (off16({dy, w2, ab, dab, h})) return 3;
+  if (off16({dy, w2, ab, dab, h}) || (bits != 8 && bits != 16) || ab == nullptr || scales == nullptr) return 3;
   const GatedGrad g{ab, (const uint8_t*)scales, (__nv_bfloat16*)dab, (__nv_bfloat16*)h, act};
   const Operand A{dy, K, M, ldy}, B{w2, H, K, ldw};
   const GemmParams p = ext_params(M, H, K, status);
   auto none = [](auto&, int) { return 0; };
-  return scales ? launch_ext<true>(A, B, p, GradExt<true>{g}, num_sms, stream, none) : launch_ext<true>(A, B, p, GradExt<false>{g}, num_sms, stream, none);
+  return bits == 8 ? launch_ext<true>(A, B, p, GradExt<8>{g}, num_sms, stream, none) : launch_ext<true>(A, B, p, GradExt<16>{g}, num_sms, stream, none);
 }
 
 // C[M, N] = a1[M, K] b1[K, N] + a2[M, K] b2[K, N], bf16; one accumulation over both contractions.

@@ -45,7 +45,8 @@ struct RowsGated {
   static constexpr bool PAIR = true;
   const __nv_bfloat16* W3;
   long long ldw3;
-  GatedOut out;
+  __nv_bfloat16* h;
+  int act;
 };
 
 // MB: blocks of 8 rows of X; U: steps of 32 elements of K whose loads are under way together
@@ -118,16 +119,11 @@ __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bflo
         b += part[i][at + ROWS_TILE / 2];
       }
       if (n >= N) continue;
-      with_act(out.out.act, [&](auto act) {
+      with_act(out.act, [&](auto act) {
         float d;
         h = act_value<decltype(act)::value>(a, d) * b;
       });
-      out.out.h[(long long)m * N + n] = __float2bfloat16(h);
-      if (out.out.ab != nullptr) {
-        __nv_bfloat16* ab = reinterpret_cast<__nv_bfloat16*>(out.out.ab) + 2ll * m * N + n;
-        ab[0] = __float2bfloat16(a);
-        ab[N] = __float2bfloat16(b);
-      }
+      out.h[(long long)m * N + n] = __float2bfloat16(h);
     }
   } else {
     for (int t = threadIdx.x; t < M * ROWS_TILE; t += 32 * ROWS_WARPS) {
@@ -198,16 +194,15 @@ extern "C" int apb_gemm_rows(const void* X, const void* W, void* C, int M, int N
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
-// h[M, H] = act(X W1^T) * (X W3^T) (gated.cuh), and the two products themselves in bf16 where ``ab`` is given.  The rules of the plain product with 2 H
-// columns hold: it reads the same.
-extern "C" int apb_gemm_rows_gated(const void* X, const void* W1, const void* W3, void* h, void* ab, int M, int H, int K, long long ldx, long long ldw1,
+// h[M, H] = act(X W1^T) * (X W3^T) (gated.cuh).
+extern "C" int apb_gemm_rows_gated(const void* X, const void* W1, const void* W3, void* h, int M, int H, int K, long long ldx, long long ldw1,
                                    long long ldw3, int act, int num_sms, cudaStream_t st) {
   if (M <= 0 || H <= 0) return 0;
   if (M > ROWS_MAX || K <= 0 || (K & 7) || ((ldx | ldw1 | ldw3) & 7) ||
       ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(W1) | reinterpret_cast<uintptr_t>(W3)) & 15))
     return 3;
   const unsigned grid = (unsigned)((H + ROWS_TILE / 2 - 1) / (ROWS_TILE / 2));
-  const RowsGated out{(const __nv_bfloat16*)W3, ldw3, GatedOut{(__nv_bfloat16*)h, ab, nullptr, act}};
+  const RowsGated out{(const __nv_bfloat16*)W3, ldw3, (__nv_bfloat16*)h, act};
   auto launch = [&](auto kern) {
     launch_after(kern, grid, 32 * ROWS_WARPS, 0, st, (const __nv_bfloat16*)X, (const __nv_bfloat16*)W1, M, H, K, ldx, ldw1, out);
   };

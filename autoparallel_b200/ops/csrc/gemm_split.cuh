@@ -230,17 +230,17 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
     const uint32_t src0 = smem_u32(tile) + c * 4;
     const int first = slice * RSTEP + threadIdx.x / VPR, step = S * RSTEP;
     auto add = [](float (&a)[4], const float4& x) { a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w; };
-    [[maybe_unused]] AbFour next;  // (backward: a and b of the row after the one in work are under way)
+    [[maybe_unused]] AbFour<ext_bits<Ext>()> next;  // (backward: a and b of the row after the one in work are under way)
     if constexpr (EXT == EXT_GRAD) {
-      if (first < rows && col < H) next.template load<Ext::EIGHT>(ext.grad, m0 + first, col, H);
+      if (first < rows && col < H) next.load(ext.grad, m0 + first, col, H);
     }
 #pragma unroll 1
     for (int r = *abort_flag == 0 ? first : rows; r < rows; r += step) {
       const uint32_t src = src0 + r * (LD * 4);
       float v[4] = {}, w[4] = {};
-      [[maybe_unused]] const AbFour ab = next;
+      [[maybe_unused]] const AbFour<ext_bits<Ext>()> ab = next;
       if constexpr (EXT == EXT_GRAD) {
-        if (r + step < rows && col < H) next.template load<Ext::EIGHT>(ext.grad, m0 + r + step, col, H);
+        if (r + step < rows && col < H) next.load(ext.grad, m0 + r + step, col, H);
       }
 #pragma unroll 2
       for (int s = 0; s < S; ++s) {
@@ -252,7 +252,7 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
       if constexpr (EXT == EXT_GATED) {
         gated_four(ext.out, m0 + r, col, H, v, w);
       } else {
-        if (col < H) gated_grad_four<Ext::EIGHT>(ext.grad, ab, m0 + r, col, H, v);
+        if (col < H) gated_grad_four<Ext::BITS>(ext.grad, ab, m0 + r, col, H, v);
       }
     }
   } else if (*abort_flag == 0) {

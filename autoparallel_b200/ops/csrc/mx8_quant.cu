@@ -32,8 +32,8 @@ __global__ void __launch_bounds__(256) mx8_quantize_kernel(const T* x, uint8_t* 
   }
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   if (!in) return;
-  const uint32_t byte = mx8_scale_byte(top);
-  const Mx8Coder coder(byte, top);
+  const uint32_t byte = mx_scale_byte<8>(top);
+  const MxCoder<8> coder(byte, top);
   auto four = [&](int k) { return coder.four(__float_as_uint(f[k]), __float_as_uint(f[k + 1]), __float_as_uint(f[k + 2]), __float_as_uint(f[k + 3])); };
   reinterpret_cast<uint4*>(codes)[i] = make_uint4(four(0), four(4), four(8), four(12));
   if ((i & 1) == 0) scales[i >> 1] = (uint8_t)byte;
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(256) mx8_dequantize_kernel(const uint8_t* code
     for (int k = 0; k < 4; ++k) {
       const long long i = first + 32 * k;
       float f[4];
-      Mx8Reader(b[k]).four(c[k], f);
+      MxReader<8>(b[k]).four(c[k], f);
       if (i < n16 * 4) reinterpret_cast<float4*>(y)[i] = make_float4(f[0], f[1], f[2], f[3]);
     }
     return;
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) mx8_dequantize_kernel(const uint8_t* code
   const long long i = blockIdx.x * 256ll + threadIdx.x;
   if (i >= n16) return;
   const uint4 c = reinterpret_cast<const uint4*>(codes)[i];
-  const Mx8Reader reader(scales[i >> 1]);
+  const MxReader<8> reader(scales[i >> 1]);
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -99,11 +99,11 @@ __global__ void __launch_bounds__(256) mx8_quantize_vec_kernel(const T* x, uint8
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   if (!in) return;
-  const uint32_t byte = mx8_scale_byte(top);
-  const Mx8Coder coder(byte, top);
+  const uint32_t byte = mx_scale_byte<8>(top);
+  const MxCoder<8> coder(byte, top);
   auto four = [&](int k) { return coder.four(__float_as_uint(f[k]), __float_as_uint(f[k + 1]), __float_as_uint(f[k + 2]), __float_as_uint(f[k + 3])); };
   *reinterpret_cast<uint2*>(codes + e) = make_uint2(four(0), four(4));
-  if (c % MX8_BLOCK == 0) scales[(long long)row * (vecs / 4) + c / MX8_BLOCK] = (uint8_t)byte;
+  if (c % MX_BLOCK == 0) scales[(long long)row * (vecs / 4) + c / MX_BLOCK] = (uint8_t)byte;
 }
 template <typename T>
 __global__ void __launch_bounds__(256) mx8_dequantize_vec_kernel(const uint8_t* codes, const uint8_t* scales, T* y, uint32_t rows, int K, uint32_t vecs) {
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(256) mx8_dequantize_vec_kernel(const uint8_t* 
   if (row >= rows || c >= (uint32_t)K) return;
   const long long e = (long long)row * K + c;
   const uint2 w = *reinterpret_cast<const uint2*>(codes + e);
-  const Mx8Reader reader(scales[(long long)row * (vecs / 4) + c / MX8_BLOCK]);
+  const MxReader<8> reader(scales[(long long)row * (vecs / 4) + c / MX_BLOCK]);
   float f[8];
   reader.four(w.x, f);
   reader.four(w.y, f + 4);
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(256) mx8_dequantize_vec_kernel(const uint8_t* 
 // Other rows begin anywhere.  A warp has seven blocks of a row, 224 elements, and takes them in the tensor's own aligned vectors of
 // eight elements (at most 29 of them, one to a lane): a lane's elements belong to one block or to two neighbours, ``first`` and the one after.  Codes lie like
 // the elements, so their vectors of eight bytes are aligned too.  Elements of other rows, and those past the tensor's end, are left alone.
-constexpr int RAGGED_BLOCKS = 7, RAGGED_COLUMNS = RAGGED_BLOCKS * MX8_BLOCK;
+constexpr int RAGGED_BLOCKS = 7, RAGGED_COLUMNS = RAGGED_BLOCKS * MX_BLOCK;
 struct Ragged {
   long long row, base;  // element that the warp's columns count from
   int block0, n;        // the row's block that the warp begins with; columns
@@ -134,12 +134,12 @@ struct Ragged {
     const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), r = w / (uint32_t)groups;  // (32 bits: a division of 64 is as long as the rest of the kernel)
     row = r;
     block0 = (int)(w - r * (uint32_t)groups) * RAGGED_BLOCKS;
-    base = row * K + block0 * MX8_BLOCK;
-    n = row < rows ? min(RAGGED_COLUMNS, K - block0 * MX8_BLOCK) : 0;
+    base = row * K + block0 * MX_BLOCK;
+    n = row < rows ? min(RAGGED_COLUMNS, K - block0 * MX_BLOCK) : 0;
     c = (int)(threadIdx.x & 31) * 8 - (int)(base & 7);
     any = c < n;
-    first = c < 0 ? -1 : c / MX8_BLOCK;
-    next = (first + 1) * MX8_BLOCK - c;
+    first = c < 0 ? -1 : c / MX_BLOCK;
+    next = (first + 1) * MX_BLOCK - c;
   }
   __device__ __forceinline__ bool in(int i) const { return c + i >= 0 && c + i < n; }
   __device__ __forceinline__ bool whole() const { return c >= 0 && c + 8 <= n; }
@@ -185,10 +185,10 @@ __global__ void __launch_bounds__(256) mx8_quantize_ragged_kernel(const T* x, ui
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) top = max(top, __shfl_sync(0xffffffffu, top, (max(l, 0) ^ o) + from0));  // (lanes without columns may read any)
   const uint32_t top_after = __shfl_sync(0xffffffffu, top, l < 0 ? from0 : (l / 4 + 1) * 4 + from0);
-  const uint32_t byte = mx8_scale_byte(top);
-  if (l >= 0 && (l & 3) == 0 && at.first * MX8_BLOCK < at.n) scales[at.row * blocks + at.block0 + at.first] = (uint8_t)byte;
+  const uint32_t byte = mx_scale_byte<8>(top);
+  if (l >= 0 && (l & 3) == 0 && at.first * MX_BLOCK < at.n) scales[at.row * blocks + at.block0 + at.first] = (uint8_t)byte;
   if (!at.any) return;
-  const Mx8Coder here(byte, top), there(mx8_scale_byte(top_after), top_after);
+  const MxCoder<8> here(byte, top), there(mx_scale_byte<8>(top_after), top_after);
   uint32_t a[2];
   if (at.next >= 8) {
 #pragma unroll
@@ -197,9 +197,9 @@ __global__ void __launch_bounds__(256) mx8_quantize_ragged_kernel(const T* x, ui
   } else if (here.exact && there.exact) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      a[h] = Mx8Coder::pack(fmaf(f[4 * h], 4 * h < at.next ? here.m : there.m, Mx8Coder::ROUND), fmaf(f[4 * h + 1], 4 * h + 1 < at.next ? here.m : there.m, Mx8Coder::ROUND),
-                            fmaf(f[4 * h + 2], 4 * h + 2 < at.next ? here.m : there.m, Mx8Coder::ROUND),
-                            fmaf(f[4 * h + 3], 4 * h + 3 < at.next ? here.m : there.m, Mx8Coder::ROUND));
+      a[h] = MxCoder<8>::pack(fmaf(f[4 * h], 4 * h < at.next ? here.m : there.m, MxCoder<8>::ROUND), fmaf(f[4 * h + 1], 4 * h + 1 < at.next ? here.m : there.m, MxCoder<8>::ROUND),
+                            fmaf(f[4 * h + 2], 4 * h + 2 < at.next ? here.m : there.m, MxCoder<8>::ROUND),
+                            fmaf(f[4 * h + 3], 4 * h + 3 < at.next ? here.m : there.m, MxCoder<8>::ROUND));
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -234,13 +234,13 @@ __global__ void __launch_bounds__(256) mx8_dequantize_ragged_kernel(const uint8_
       if (e + i < rows * K) (i < 4 ? w.x : w.y) |= (uint32_t)codes[e + i] << (8 * (i % 4));
   }
   const uint8_t* s = scales + at.row * blocks + at.block0;
-  const bool second = at.next < 8 && (at.first + 1) * MX8_BLOCK < at.n;
+  const bool second = at.next < 8 && (at.first + 1) * MX_BLOCK < at.n;
   float f[8], g[8];
-  const Mx8Reader here(at.first < 0 ? MX8_LOWEST : s[at.first]);
+  const MxReader<8> here(at.first < 0 ? MX_LOWEST<8> : s[at.first]);
   here.four(w.x, f);
   here.four(w.y, f + 4);
   if (second) {
-    const Mx8Reader there(s[at.first + 1]);
+    const MxReader<8> there(s[at.first + 1]);
     there.four(w.x, g);
     there.four(w.y, g + 4);
 #pragma unroll
@@ -255,6 +255,25 @@ __global__ void __launch_bounds__(256) mx8_dequantize_ragged_kernel(const uint8_
     for (int i = 0; i < 8; ++i)
       if (at.in(i)) y[e + i] = T(f[i]);
   }
+}
+
+// The 16-bit codes of what gated_act_kernel takes, and back: a warp to a block, an element to a lane (only products in fp32 come here).
+__global__ void __launch_bounds__(256) mx16_quantize_kernel(const float* x, uint16_t* codes, uint8_t* scales, uint32_t warps, int K, uint32_t blocks) {
+  after_previous();
+  const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), row = w / blocks, c = (w - row * blocks) * MX_BLOCK + (threadIdx.x & 31);
+  if (w >= warps) return;
+  const uint32_t v = c < (uint32_t)K ? __float_as_uint(x[(long long)row * K + c]) : 0u, top = __reduce_max_sync(0xffffffffu, v & 0x7fffffffu);
+  const uint32_t byte = mx_scale_byte<16>(top);
+  if (c < (uint32_t)K) codes[(long long)row * K + c] = (uint16_t)MxCoder<16>(byte, top).two(v, 0);
+  if ((threadIdx.x & 31) == 0) scales[w] = (uint8_t)byte;
+}
+__global__ void __launch_bounds__(256) mx16_dequantize_kernel(const uint16_t* codes, const uint8_t* scales, float* y, uint32_t warps, int K, uint32_t blocks) {
+  after_previous();
+  const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), row = w / blocks, c = (w - row * blocks) * MX_BLOCK + (threadIdx.x & 31);
+  if (w >= warps || c >= (uint32_t)K) return;
+  float f[2];
+  MxReader<16>(scales[w]).two(codes[(long long)row * K + c], f);
+  y[(long long)row * K + c] = f[0];
 }
 
 // ab fp32 [M, 2, H] -> h [M, H]; and dh fp32 [M, H] with ab -> dab [M, 2, H], h
@@ -296,22 +315,22 @@ using namespace apb;
 // 8192 x 14336 bf16 54, 14344 75, 14343 224 us (and back 58, 68, 108).
 template <typename T>
 static int quantize(const T* x, uint8_t* codes, uint8_t* scales, long long R, long long K, cudaStream_t st) {
-  const long long blocks = (K + MX8_BLOCK - 1) / MX8_BLOCK, groups = (blocks + RAGGED_BLOCKS - 1) / RAGGED_BLOCKS;
-  if (K % MX8_BLOCK == 0) return done(launch_after(mx8_quantize_kernel<T>, blocks_of(R * K / 16), 256, 0, st, x, codes, scales, R * K / 16));
+  const long long blocks = (K + MX_BLOCK - 1) / MX_BLOCK, groups = (blocks + RAGGED_BLOCKS - 1) / RAGGED_BLOCKS;
+  if (K % MX_BLOCK == 0) return done(launch_after(mx8_quantize_kernel<T>, blocks_of(R * K / 16), 256, 0, st, x, codes, scales, R * K / 16));
   if (K % 8 == 0) return done(launch_after(mx8_quantize_vec_kernel<T>, blocks_of(R * blocks * 4), 256, 0, st, x, codes, scales, (uint32_t)R, (int)K, (uint32_t)blocks * 4));
   return done(launch_after(mx8_quantize_ragged_kernel<T>, blocks_of(R * groups * 32), 256, 0, st, x, codes, scales, R, (int)K, (int)blocks, (int)groups));
 }
 template <typename T>
 static int dequantize(const uint8_t* codes, const uint8_t* scales, T* y, long long R, long long K, cudaStream_t st) {
-  const long long blocks = (K + MX8_BLOCK - 1) / MX8_BLOCK, groups = (blocks + RAGGED_BLOCKS - 1) / RAGGED_BLOCKS;
-  if (K % MX8_BLOCK == 0) return done(launch_after(mx8_dequantize_kernel<T>, blocks_of(R * K / 16), 256, 0, st, codes, scales, y, R * K / 16));
+  const long long blocks = (K + MX_BLOCK - 1) / MX_BLOCK, groups = (blocks + RAGGED_BLOCKS - 1) / RAGGED_BLOCKS;
+  if (K % MX_BLOCK == 0) return done(launch_after(mx8_dequantize_kernel<T>, blocks_of(R * K / 16), 256, 0, st, codes, scales, y, R * K / 16));
   if (K % 8 == 0) return done(launch_after(mx8_dequantize_vec_kernel<T>, blocks_of(R * blocks * 4), 256, 0, st, codes, scales, y, (uint32_t)R, (int)K, (uint32_t)blocks * 4));
   return done(launch_after(mx8_dequantize_ragged_kernel<T>, blocks_of(R * groups * 32), 256, 0, st, codes, scales, y, R, (int)K, (int)blocks, (int)groups));
 }
 // (the threads of the forms for other rows are counted in 32 bits: 2^32 of them are 2^35 elements or, of a row of one element, 2^30)
 static bool too_many(long long R, long long K) {
-  const long long blocks = (K + MX8_BLOCK - 1) / MX8_BLOCK;
-  return K > 0x7fffffe0ll || R > 0x7fffffffll * 64 / blocks || (K % MX8_BLOCK && R > 0x3fffff00ll / blocks) || R * K / 16 / 256 >= 0x7fffffffll;
+  const long long blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
+  return K > 0x7fffffe0ll || R > 0x7fffffffll * 64 / blocks || (K % MX_BLOCK && R > 0x3fffff00ll / blocks) || R * K / 16 / 256 >= 0x7fffffffll;
 }
 extern "C" int apb_mx8_quantize(const void* x, void* codes, void* scales, long long R, long long K, int is_bf16, cudaStream_t st) {
   if (R <= 0 || K <= 0) return 0;
@@ -323,6 +342,20 @@ extern "C" int apb_mx8_dequantize(const void* codes, const void* scales, void* y
   if (off16(y) || off16(codes) || too_many(R, K)) return 3;
   return is_bf16 ? dequantize((const uint8_t*)codes, (const uint8_t*)scales, (bf16*)y, R, K, st)
                  : dequantize((const uint8_t*)codes, (const uint8_t*)scales, (float*)y, R, K, st);
+}
+
+extern "C" int apb_mx16_quantize(const float* x, void* codes, void* scales, long long R, int K, cudaStream_t st) {
+  const long long blocks = (K + MX_BLOCK - 1) / MX_BLOCK, warps = R * blocks;
+  if (warps <= 0) return 0;
+  if (warps > 0xfffffff0ll) return 3;
+  return done(launch_after(mx16_quantize_kernel, blocks_of(warps * 32), 256, 0, st, x, (uint16_t*)codes, (uint8_t*)scales, (uint32_t)warps, K, (uint32_t)blocks));
+}
+extern "C" int apb_mx16_dequantize(const void* codes, const void* scales, float* y, long long R, int K, cudaStream_t st) {
+  const long long blocks = (K + MX_BLOCK - 1) / MX_BLOCK, warps = R * blocks;
+  if (warps <= 0) return 0;
+  if (warps > 0xfffffff0ll) return 3;
+  return done(launch_after(mx16_dequantize_kernel, blocks_of(warps * 32), 256, 0, st, (const uint16_t*)codes, (const uint8_t*)scales, y, (uint32_t)warps, K,
+                           (uint32_t)blocks));
 }
 
 extern "C" int apb_gated_act(const float* ab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st) {

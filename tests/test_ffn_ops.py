@@ -66,6 +66,23 @@ def test_mx8(shape, dtype):
     assert [tuple(m.shape) for m in meta] == [tuple(codes.shape), tuple(scales.shape)] and [m.dtype for m in meta] == [torch.int8, torch.uint8]
 
 
+def test_16_bit_codes():
+    """What "full" keeps of both projections of bf16 operands: the same format with 14 for 6, -112 for -120 and 32767 for 127."""
+    x = _randn(5, 70, gen=_gen(8)) * 3
+    x[1, :32], x[2, 0], x[3, 40], x[4, 33] = 0, 2.0**-126, float("inf"), float("nan")
+    x[1, 32:64] = 0.5  # (nothing in the block above the two that round to 32768)
+    x[1, 40], x[1, 41] = 32767.6 * 2.0**-14, -32767.6 * 2.0**-14
+    codes, scales = FFN._quantize(x, 16)
+    assert codes.dtype == torch.int16 and scales.shape == (5, 3) and scales[1, 0] == 15 and scales[3, 1] == scales[4, 1] == 255
+    v = FFN._dequantize(codes, scales, torch.float32)
+    assert v[3, 32:64].isnan().all() and v[4, 32:64].isnan().all() and codes[1, 40] == 32767 and codes[1, 41] == -32767
+    top = F.pad(x, (0, 26)).unflatten(-1, (3, 32)).abs().amax(-1, keepdim=True).expand(5, 3, 32).flatten(1)[:, :70]
+    ok = torch.isfinite(top)
+    step = torch.exp2(torch.floor(torch.log2(top[ok].double().clamp_min(2.0**-112))) - 14)
+    err = (v[ok].double() - x[ok].double()).abs()
+    assert (err <= torch.where(x[ok].abs() > 32767.4 * step, 1.0, 0.5) * step).all()
+
+
 def test_mx8_of_extreme_values():
     big, tiny, inf = torch.finfo(torch.float32).max, 2.0**-126, float("inf")
     x = torch.zeros(8, 32)
@@ -217,7 +234,7 @@ def test_gated_block_of_nothing():
 
 
 def test_what_the_backward_pass_keeps():
-    """Bytes held between the passes: x, a and b in their type, or in 33/32 of a byte."""
+    """Bytes held between the passes: x in bf16, a and b in 16 bits and a 32nd of a byte, or all in 33/32 of a byte."""
     x, w1, w3, w2 = (torch.randn(*s).bfloat16().requires_grad_() for s in ((64, 128), (256, 128), (256, 128), (128, 256)))
     held = {}
     for checkpoint in ("full", "mx8"):
@@ -225,8 +242,8 @@ def test_what_the_backward_pass_keeps():
         with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t) or t, lambda t: t):
             K.gated_ffn(x, w1, w3, w2, checkpoint=checkpoint)
         held[checkpoint] = sum(t.numel() * t.element_size() for t in seen if all(t is not w for w in (w1, w3, w2)))
-    n = 64 * (128 + 2 * 256)
-    assert held == {"full": 2 * n, "mx8": n + n // 32}
+    x, ab = 64 * 128, 64 * 2 * 256
+    assert held == {"full": 2 * (x + ab) + ab // 32, "mx8": (x + ab) + (x + ab) // 32}
 
 
 # ------------------------------------------------------------------------------------ refusals
@@ -270,9 +287,10 @@ def test_refusals():
         y.sum().backward()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("bits", [0, 8, 16])
-def test_meta_shapes(bits):
-    x, w1, w3, w2 = (torch.randn(*s) for s in ((2, 3, 24), (40, 24), (40, 24), (16, 40)))
+def test_meta_shapes(bits, dtype):
+    x, w1, w3, w2 = (torch.randn(*s).to(dtype) for s in ((2, 3, 24), (40, 24), (40, 24), (16, 40)))
     for name, args in (("gated_mm", (x, w1, w3, 0, bits)), ("gated_ffn", (x, w1, w3, w2, 0, bits)), ("add_rms_norm", (x, x, x[0, 0], 1e-5)),
                        ("add_rms_norm_fp8", (x, x, x[0, 0], 1e-5, bits > 0)), ("add_rms_norm_fp8", (x, None, x[0, 0], 1e-5, bits > 0))):
         real = getattr(ops, name)(*args)
@@ -280,7 +298,7 @@ def test_meta_shapes(bits):
         assert [(tuple(a.shape), a.dtype) for a in real] == [(tuple(a.shape), a.dtype) for a in meta], name
     if bits:
         _, ab, scales = ops.gated_mm(x, w1, w3, 0, bits)
-        dy = torch.randn(2, 3, 16)
+        dy = torch.randn(2, 3, 16).to(dtype)
         real = ops.gated_dgrad(dy, w2, ab, scales, 0)
         meta = ops.gated_dgrad(*(t.to("meta") for t in (dy, w2, ab, scales)), 0)
         assert [(tuple(a.shape), a.dtype) for a in real] == [(tuple(a.shape), a.dtype) for a in meta]
@@ -451,27 +469,29 @@ for f in (so.apb_mx8_quantize, so.apb_mx8_dequantize):
         a[i] = bad
         print(f(*a))
     print(f(p, p, p, LL(1 << 31), LL(33), 1, N))
-gated = [p, p, p, p, p, p, 4, 64, 64, LL(64), LL(64), LL(64), 0, p, 148, N]
+gated = [p, p, p, p, p, p, 16, 4, 64, 64, LL(64), LL(64), LL(64), 0, p, 148, N]
 for i in (0, 1, 2, 3, 4):
     print(so.apb_gemm_gated(*gated[:i], bad, *gated[i + 1:]))
-for i in (7, 8):
+for i in (8, 9):
     print(so.apb_gemm_gated(*gated[:i], 60, *gated[i + 1:]))
-for i in (9, 10, 11):
+for i in (10, 11, 12):
     print(so.apb_gemm_gated(*gated[:i], LL(60), *gated[i + 1:]))
-grad = [p, p, p, p, p, p, 4, 64, 64, LL(64), LL(64), 0, p, 148, N]
-for i in (0, 1, 2, 4, 5):
+print(so.apb_gemm_gated(*gated[:6], 4, *gated[7:]), so.apb_gemm_gated(*gated[:5], N, *gated[6:]))  # bits; codes without scales
+grad = [p, p, p, p, 8, p, p, 4, 64, 64, LL(64), LL(64), 0, p, 148, N]
+print(so.apb_gemm_gated_grad(*grad[:4], 0, *grad[5:]), so.apb_gemm_gated_grad(*grad[:3], N, *grad[4:]))
+for i in (0, 1, 2, 5, 6):
     print(so.apb_gemm_gated_grad(*grad[:i], bad, *grad[i + 1:]))
 dual = [p, p, p, p, p, 4, 64, 64, LL(128), LL(64), LL(64), LL(64), p, 148, N]
 for i in (0, 1, 2, 3, 4):
     print(so.apb_gemm_dual(*dual[:i], bad, *dual[i + 1:]))
 """)
-    assert out == ["3"] * len(out) and len(out) == 6 + 2 + 2 + 5 + 6 + 5 + 2 + 3 + 5 + 5, out
+    assert out == ["3"] * len(out) and len(out) == 6 + 2 + 2 + 5 + 6 + 5 + 2 + 3 + 2 + 2 + 5 + 5, out
     out = _entries("""
 p = V(1 << 20)
 print(so.apb_add_rms_norm(p, p, p, p, p, p, N, N, LL(0), 64, F(1e-5), 1, N), so.apb_mx8_quantize(p, p, p, LL(0), LL(5), 1, N),
       so.apb_gated_act(p, p, LL(0), 4, 0, 1, N))
 so.apb_gemm_set_dynamic_tiles(1)
-print(so.apb_gemm_gated(p, p, p, p, p, p, 4, 64, 64, LL(64), LL(64), LL(64), 0, p, 148, N))
+print(so.apb_gemm_gated(p, p, p, p, p, p, 16, 4, 64, 64, LL(64), LL(64), LL(64), 0, p, 148, N))
 """)
     assert out == ["0", "0", "0", "-1"]
 

@@ -52,6 +52,20 @@ def _held(x):
     return (torch.clamp(torch.round(b / torch.exp2(e - 6)), -127, 127) * torch.exp2(e - 6)).flatten(-2)[..., :k]
 
 
+def _kept(ab, scales):
+    """The values of what was kept of both projections, in 64 bits."""
+    if ab.is_floating_point():
+        return ab.double()
+    unit = torch.exp2(scales.double() - 127 - (6 if ab.dtype is torch.int8 else 14)).masked_fill(scales == 255, float("nan"))
+    return ab.double() * unit.repeat_interleave(32, -1)[..., : ab.shape[-1]]
+
+
+def _tops(v):
+    """The largest magnitude of every value's block of 32."""
+    k = v.shape[-1]
+    return F.pad(v, (0, -k % 32)).unflatten(-1, (-1, 32)).abs().amax(-1, keepdim=True).expand(*v.shape[:-1], -1, 32).flatten(-2)[..., :k]
+
+
 # ------------------------------------------------------------------------------------ 8-bit checkpoints
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("shape", [(1, 1), (1, 32), (3, 31), (5, 33), (2, 3, 64), (7, 1000), (64, 4096), (129, 257), (0, 64), (4, 0), (9,), (1023, 96)])
@@ -233,21 +247,19 @@ def test_gated_mm(M, D, H, bits):
     a, b = _products(x, w1, w3)
     acc = 4 * math.sqrt(D) * 2.0**-24  # of the products' size
     _close(h, ACTS[act](a) * b, HALF_STEP[BF] + 8 * acc)
-    if bits == 16:
-        _close(ab, torch.stack((a, b), 1), HALF_STEP[BF] + acc)
-    elif bits == 8:
+    if bits:
         exact = torch.stack((a, b), 1)
-        got = K.mx8_dequantize(ab, scales, F32).double()
-        # half a step of the block's codes, a whole one at the block's top, which rounds to 128 and is held as 127; a top at a power of two may fall on
-        # either side of it
-        top = F.pad(exact, (0, -H % 32)).unflatten(-1, (-1, 32)).abs().amax(-1, keepdim=True)
-        step = torch.exp2(torch.floor(torch.log2(top * (1 + 2.0**-16))) - 6).expand(*top.shape[:-1], 32).flatten(-2)[..., :H]
-        near = exact.abs() > 127.4 * step
+        assert ab.dtype == (torch.int8 if bits == 8 else torch.int16) and scales.shape == (M, 2, -(-H // 32))
+        got = _kept(ab, scales)
+        # half a step of the block's codes, a whole one at the block's top, which rounds to 2^(bits - 1) and is held as one less; a top at a power of two may
+        # fall on either side of it
+        step = torch.exp2(torch.floor(torch.log2(_tops(exact) * (1 + 2.0**-15))) - (bits - 2))
+        near = exact.abs() > (2 ** (bits - 1) - 0.6 - 2.0**-14 * 2 ** (bits - 1)) * step
         # and the product's own error, which is of the size of the terms and not of a value that they cancel to: the accumulator is rounded D / 16
         # times at its running size, about the root mean square of the results, D / 16 2^-24 <= 4 sqrt(D) 2^-24 for D <= 4096 and 1.04 of it for 4416
         size = torch.maximum(exact.abs(), 1.04 * exact.square().mean().sqrt())
         assert bool(((got - exact).abs() <= torch.where(near, 1.0, 0.5) * step + 1e-4 * step + acc * size).all())
-        assert bool((scales.int() >= 7).all())
+        assert bool((scales.int() >= bits - 1).all())
     else:
         assert ab.numel() == 0 and scales.numel() == 0
 
@@ -259,8 +271,7 @@ def test_gated_dgrad(M, N, H, bits):
     x, w1, w3, w2, dy = _gated(M, 64, H, N, seed=M + 1)
     _, ab, scales = ops.gated_mm(x, w1, w3, FFN.ACTS[act], bits)
     dab, h = ops.gated_dgrad(dy, w2, ab, scales, FFN.ACTS[act])
-    a, b = (K.mx8_dequantize(ab, scales, F32) if bits == 8 else ab).double().unbind(1)
-    a, b = a.requires_grad_(), b.requires_grad_()
+    a, b = (t.clone().requires_grad_() for t in _kept(ab, scales).unbind(1))
     hd = ACTS[act](a) * b
     da, db = torch.autograd.grad(hd, (a, b), dy.double() @ w2.double())
     tol = HALF_STEP[BF] + 32 * math.sqrt(N) * 2.0**-24
@@ -310,20 +321,20 @@ def test_gated_ffn_training(M, D, H, N, dtype, checkpoint):
             for u, v in zip(got, want):
                 _close(u, v, 5 * step)
             continue
-        # What each rounding can do to a term, in magnitudes: a and b are off by a half step of themselves ("full"; codes are exact in bf16), da, db and h
-        # by one of theirs; |act'| <= 1.13 and |act''| <= 0.8 for all three.  The bound of a sum is the sum of the bounds (1.02: products of two errors),
-        # then the result's own rounding and 2^-16 for the fp32 sums.
+        # What each rounding can do to a term, in magnitudes: a and b are off by 2^-15 of their block's top ("full": 16-bit codes; the 8-bit ones are known
+        # here), da, db and h by a half step of theirs; |act'| <= 1.13 and |act''| <= 0.8 for all three.  The bound of a sum is the sum of the bounds (1.02:
+        # products of two errors, and twice 2^-15 at a block's top), then the result's own rounding and 2^-16 for the fp32 sums.
         e, dh = HALF_STEP[BF], (dy.double() @ d[3]).abs()
         av, bv, hv = a.detach().abs(), b.detach().abs(), h.detach().abs()
-        k = 1.0 if checkpoint == "full" else 0.0
-        off_a = e * (da.abs() + k * dh * (0.8 * av * bv + 1.13 * bv))
-        off_b = e * (db.abs() + k * dh * 1.13 * av)
-        off_h = e * (hv + k * (1.13 * av * bv + ACTS[act](a.detach()).abs() * bv))
+        ka, kb = ((2.0**-14 * _tops(t) if checkpoint == "full" else torch.zeros_like(t)) for t in (av, bv))
+        off_a = e * da.abs() + dh * (0.8 * ka * bv + 1.13 * kb)
+        off_b = e * db.abs() + dh * 1.13 * ka
+        off_h = e * hv + 1.13 * ka * bv + ACTS[act](a.detach()).abs() * kb
         w1a, w3a, xa, dya = d[1].abs(), d[2].abs(), xk.abs(), dy.double().abs()
         for u, v, off in zip(got, want, (off_a @ w1a + off_b @ w3a, off_a.t() @ xa, off_b.t() @ xa, dya.t() @ off_h)):
             assert bool(((u.double() - v).abs() <= 1.02 * off + e * v.abs() + 2.0**-16 * v.square().mean().sqrt()).all())
-            # and as noise: a rounding's error is at most a half step, spread evenly, sqrt(1/3) of it; five of them on the way of a result
-            assert u.numel() < 1000 or float((u.double() - v).norm() / v.norm()) <= math.sqrt(5 / 3) * e
+            # and as noise: a rounding's error is at most a half step, spread evenly, sqrt(1/3) of it; two of them on the way of a result, and the codes'
+            assert u.numel() < 1000 or float((u.double() - v).norm() / v.norm()) <= math.sqrt(3 / 3) * e
 
 
 def test_gated_ffn_leading_dims_strides_and_partial_gradients():
@@ -530,7 +541,7 @@ def test_refusals():
     _, ab, scales = ops.gated_mm(x, w1, w1, 0, 8)
     with pytest.raises(RuntimeError, match="uint8 scales"):
         ops.gated_dgrad(x, w2, ab, scales[:2], 0)
-    with pytest.raises(RuntimeError, match="of dy's type or int8"):
+    with pytest.raises(RuntimeError, match="in 8 bits, or in 16"):
         ops.gated_dgrad(x, w2, ab[:2], scales, 0)
     with pytest.raises(RuntimeError, match="dab"):
         ops.gated_dx(x, w1, w1)
@@ -597,10 +608,10 @@ def test_offsets_past_32_bits():
         h, ab, scales = ops.gated_mm(x, w1, w3, 0, bits)
         a, b = _products(x[-256:], w1, w3)
         _close(h[-256:], F.silu(a) * b, 1.2 * HALF_STEP[BF])
-        got = K.mx8_dequantize(ab[-256:], scales[-256:], F32) if bits == 8 else ab[-256:]
-        _close(got, torch.stack((a, b), 1), 2.0**-4 if bits == 8 else 1.2 * HALF_STEP[BF])  # (8 bits: at most 2^-7 of a block's top, itself below 8 times the mean square root)
+        # at most 2^-7 or 2^-15 of a block's top, itself below 8 times the root mean square; the sums' own error
+        _close(_kept(ab[-256:], scales[-256:]), torch.stack((a, b), 1), 2.0**-4 if bits == 8 else 2.0**-12 + 2.0**-18)
         dab, h = ops.gated_dgrad(x, w2, ab, scales, 0)
-        few, h2 = ops.gated_dgrad(x[-256:].contiguous(), w2, ab[-256:].contiguous(), scales[-256:].contiguous() if bits == 8 else scales, 0)
+        few, h2 = ops.gated_dgrad(x[-256:].contiguous(), w2, ab[-256:].contiguous(), scales[-256:].contiguous(), 0)
         _close(dab[-256:], few.double(), 2 * HALF_STEP[BF])
         assert torch.equal(h[-256:], h2)
         _close(ops.gated_dx(dab, w1, w3)[-256:], ops.gated_dx(dab[-256:].contiguous(), w1, w3).double(), 2 * HALF_STEP[BF])
