@@ -63,9 +63,9 @@ __device__ __forceinline__ float act_value(float a, float& d) {
 
 struct GatedOut {  // forward
   __nv_bfloat16* h;
-  void* ab;  // codes; null: not kept
+  void* ab;  // codes
   uint8_t* scales;
-  int act, bits;  // of a code
+  int act;
 };
 struct GatedGrad {  // backward
   const void* ab;  // codes
@@ -119,20 +119,18 @@ template <int BITS>
 __device__ __forceinline__ uint32_t codes32(const uint32_t (&r)[32], uint8_t* stg, int lane) {
   const uint32_t top = mx_top(r), byte = mx_scale_byte<BITS>(top);
   const MxCoder<BITS> coder(byte, top);
+  uint32_t w[BITS];
+  coder.words(r, w);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t* v = r + 8 * i;
-    if constexpr (BITS == 8)
-      *reinterpret_cast<uint2*>(stg + stage32(lane, i)) = make_uint2(coder.four(v[0], v[1], v[2], v[3]), coder.four(v[4], v[5], v[6], v[7]));
-    else
-      *reinterpret_cast<uint4*>(stg + stage64(lane, i)) =
-          make_uint4(coder.two(v[0], v[1]), coder.two(v[2], v[3]), coder.two(v[4], v[5]), coder.two(v[6], v[7]));
+    if constexpr (BITS == 8) *reinterpret_cast<uint2*>(stg + stage32(lane, i)) = make_uint2(w[2 * i], w[2 * i + 1]);
+    else *reinterpret_cast<uint4*>(stg + stage64(lane, i)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
   return byte;
 }
 
-// Forward: columns col ... col + ncols - 1 of h from the accumulators at ``ta`` and ``tb``; ``stg``: 4096 bytes of the warp's own.
-template <typename Release>
+// Forward: columns col ... col + ncols - 1 of h from the accumulators at ``ta`` and ``tb``, and codes of BITS bits (0: none); ``stg``: 4096 bytes of the warp's own.
+template <int BITS, typename Release>
 __device__ __forceinline__ void gated_tile(const GatedOut& o, uint8_t* stg, uint32_t ta, uint32_t tb, int row0, int col, int ncols, int M, int H, int lane,
                                            Release release) {
   const int used = row0 < M ? min(ncols, H - col) : 0;  // (rows and columns past the matrix are not read)
@@ -161,22 +159,16 @@ __device__ __forceinline__ void gated_tile(const GatedOut& o, uint8_t* stg, uint
     __syncwarp();  // what was there before has been read
     stage_put(stg, lane, v);
     uint32_t sa = 0, sb = 0;
-    if (o.ab != nullptr) {
-      if (o.bits == 8) {
-        sa = codes32<8>(a, stg + 2048, lane);
-        sb = codes32<8>(b, stg + 3072, lane);
-      } else {
-        sa = codes32<16>(a, stg + 2048, lane);
-      }
-    }
+    if constexpr (BITS > 0) sa = codes32<BITS>(a, stg + 2048, lane);
+    if constexpr (BITS == 8) sb = codes32<8>(b, stg + 3072, lane);
     __syncwarp();
     stage_store(stg, o.h, H, row0, col + c, M, H, lane);
-    if (o.ab == nullptr) continue;
-    if (o.bits == 8) {
+    if constexpr (BITS == 0) continue;
+    if constexpr (BITS == 8) {
       uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab);
       stage_store8(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);
       stage_store8(stg + 3072, codes + H, 2ll * H, row0, col + c, M, H, lane);
-    } else {
+    } else if constexpr (BITS == 16) {
       __nv_bfloat16* codes = reinterpret_cast<__nv_bfloat16*>(o.ab);  // (two bytes each)
       stage_store(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);
       __syncwarp();
@@ -325,9 +317,12 @@ __device__ __forceinline__ uint2 codes4(const float (&v)[4], uint32_t& byte) {
   for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(eight, top, o));
   byte = mx_scale_byte<BITS>(top);
   const MxCoder<BITS> coder(byte, top);
-  const uint32_t w[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-  return BITS == 8 ? make_uint2(coder.four(w[0], w[1], w[2], w[3]), 0) : make_uint2(coder.two(w[0], w[1]), coder.two(w[2], w[3]));
+  const uint32_t u[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+  uint32_t w[BITS / 8];
+  coder.words(u, w);
+  return make_uint2(w[0], BITS == 8 ? 0 : w[BITS / 8 - 1]);
 }
+template <int BITS>
 __device__ __forceinline__ void gated_four(const GatedOut& o, long long row, int col, int H, const float (&a)[4], const float (&b)[4]) {
   float h[4];
   with_act(o.act, [&](auto act) {
@@ -339,16 +334,16 @@ __device__ __forceinline__ void gated_four(const GatedOut& o, long long row, int
   });
   const bool in = col < H;
   if (in) *reinterpret_cast<uint2*>(o.h + row * H + col) = pack4(h);
-  if (o.ab == nullptr) return;
-  uint32_t sa, sb;
+  if constexpr (BITS == 0) return;
+  uint32_t sa = 0, sb = 0;
   const long long at = row * 2 * H + col;
-  if (o.bits == 8) {
+  if constexpr (BITS == 8) {
     const uint2 ca = codes4<8>(a, sa), cb = codes4<8>(b, sb);
     if (!in) return;
     uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab) + at;
     *reinterpret_cast<uint32_t*>(codes) = ca.x;
     *reinterpret_cast<uint32_t*>(codes + H) = cb.x;
-  } else {
+  } else if constexpr (BITS == 16) {
     const uint2 ca = codes4<16>(a, sa), cb = codes4<16>(b, sb);
     if (!in) return;
     uint16_t* codes = reinterpret_cast<uint16_t*>(o.ab) + at;

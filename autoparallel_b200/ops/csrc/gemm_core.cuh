@@ -108,8 +108,9 @@ enum : int { EXT_NONE = 0, EXT_GATED = 1, EXT_GRAD = 2, EXT_DUAL = 3 };
 struct NoExt {
   static constexpr int KIND = EXT_NONE;
 };
+template <int CODE_BITS>  // of what is kept of the projections; 0: nothing
 struct GatedExt {
-  static constexpr int KIND = EXT_GATED;
+  static constexpr int KIND = EXT_GATED, BITS = CODE_BITS;
   CUtensorMap tmB2;
   GatedOut out;
 };
@@ -950,7 +951,7 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
           if constexpr (EXT == EXT_GATED) {  // this warp's columns: the same of both projections
             const int both = cols / 2, first = part * both;
             const uint32_t ta = tmem_base + (uint32_t(q * 32) << 16) + buf * BN + first;
-            gated_tile(ext.out, stg, ta, ta + 2 * both, r0, (x.col + sub * BN) / 2 + first, both, p.M, p.N / 2, lane, release);
+            gated_tile<Ext::BITS>(ext.out, stg, ta, ta + 2 * both, r0, (x.col + sub * BN) / 2 + first, both, p.M, p.N / 2, lane, release);
           } else {
             gated_grad_tile<Ext::BITS>(ext.grad, fetch, stg, taddr, r0, n0, cols, p.M, p.N, lane, release);
           }

@@ -153,10 +153,12 @@ extern "C" int apb_gemm_gated(const void* x, const void* w1, const void* w3, voi
   if (H > 0x3fffffff || (bits != 0 && bits != 8 && bits != 16) || (bits != 0 && (ab == nullptr || scales == nullptr))) return 3;
   if (bits == 0 && apb_gemm_get_reserved_sms() == 0 && few_rows(M, H, K, num_sms))
     return apb_gemm_rows_gated(x, w1, w3, h, M, H, K, ldx, ldw1, ldw3, act, num_sms, stream);
-  GatedExt ext{};
-  ext.out = GatedOut{(__nv_bfloat16*)h, bits ? ab : nullptr, (uint8_t*)scales, act, bits};
-  return launch_ext<false>(Operand{x, K, M, ldx}, Operand{w1, K, H, ldw1}, ext_params(M, 2 * H, K, status), ext, num_sms, stream,
-                           [&](GatedExt& e, int box) { return Operand{w3, K, H, ldw3}.map(&e.tmB2, box); });
+  auto launch = [&](auto ext) {
+    ext.out = GatedOut{(__nv_bfloat16*)h, ab, (uint8_t*)scales, act};
+    return launch_ext<false>(Operand{x, K, M, ldx}, Operand{w1, K, H, ldw1}, ext_params(M, 2 * H, K, status), ext, num_sms, stream,
+                             [&](auto& e, int box) { return Operand{w3, K, H, ldw3}.map(&e.tmB2, box); });
+  };
+  return bits == 0 ? launch(GatedExt<0>{}) : bits == 8 ? launch(GatedExt<8>{}) : launch(GatedExt<16>{});
 }
 
 extern "C" int apb_gemm_gated_grad(const void* dy, const void* w2, const void* ab, const void* scales, int bits, void* dab, void* h, int M, int H,

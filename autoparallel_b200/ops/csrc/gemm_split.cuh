@@ -250,7 +250,7 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
         add(v, x);
       }
       if constexpr (EXT == EXT_GATED) {
-        gated_four(ext.out, m0 + r, col, H, v, w);
+        gated_four<Ext::BITS>(ext.out, m0 + r, col, H, v, w);
       } else {
         if (col < H) gated_grad_four<Ext::BITS>(ext.grad, ab, m0 + r, col, H, v);
       }

@@ -49,20 +49,33 @@ struct MxCoder {
   bool exact;
   __device__ __forceinline__ MxCoder(uint32_t byte, uint32_t top)
       : m(mx_unit(byte, 252 + BITS - (int)byte, 0u)), exact(byte != MX_NAN && (top & 0x7fffffu) < TIE) {}
+  template <bool EXACT>
   __device__ __forceinline__ float add(uint32_t bits) const {
     const float f = mx_bits(bits);
-    if (!exact) return ROUND + (m == 0.f ? 0.f : fminf(LIMIT, fmaxf(-LIMIT, f * m)));
-    return fmaf(f, m, ROUND);
+    return EXACT ? fmaf(f, m, ROUND) : ROUND + (m == 0.f ? 0.f : fminf(LIMIT, fmaxf(-LIMIT, f * m)));
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {  // four lowest bytes
     const uint32_t lo = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), hi = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
     return __byte_perm(lo, hi, 0x5410);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410); }  // two lower halves
-  __device__ __forceinline__ uint32_t four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {  // (8 bits)
-    return pack(add(a), add(b), add(c), add(d));
+  // four codes of 8 bits, two of 16
+  template <bool EXACT>
+  __device__ __forceinline__ uint32_t word(const uint32_t* v) const {
+    if constexpr (BITS == 8) return pack(add<EXACT>(v[0]), add<EXACT>(v[1]), add<EXACT>(v[2]), add<EXACT>(v[3]));
+    else return pack(add<EXACT>(v[0]), add<EXACT>(v[1]));
   }
-  __device__ __forceinline__ uint32_t two(uint32_t a, uint32_t b) const { return pack(add(a), add(b)); }  // (16 bits)
+  // ``n`` words of codes; one branch for all of them
+  template <int n>
+  __device__ __forceinline__ void words(const uint32_t* v, uint32_t (&w)[n]) const {
+    if (exact) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) w[i] = word<true>(v + 32 / BITS * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < n; ++i) w[i] = word<false>(v + 32 / BITS * i);
+    }
+  }
 };
 
 // Codes of one block to values: with 2^(n+1) added, a code is the lowest byte (or two) of 2^23 + (code + 2^(n+1)) as fp32; one permutation, and a multiplication

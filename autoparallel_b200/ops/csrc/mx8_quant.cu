@@ -34,8 +34,9 @@ __global__ void __launch_bounds__(256) mx8_quantize_kernel(const T* x, uint8_t* 
   if (!in) return;
   const uint32_t byte = mx_scale_byte<8>(top);
   const MxCoder<8> coder(byte, top);
-  auto four = [&](int k) { return coder.four(__float_as_uint(f[k]), __float_as_uint(f[k + 1]), __float_as_uint(f[k + 2]), __float_as_uint(f[k + 3])); };
-  reinterpret_cast<uint4*>(codes)[i] = make_uint4(four(0), four(4), four(8), four(12));
+  uint32_t c[4];
+  coder.words(reinterpret_cast<const uint32_t*>(f), c);
+  reinterpret_cast<uint4*>(codes)[i] = make_uint4(c[0], c[1], c[2], c[3]);
   if ((i & 1) == 0) scales[i >> 1] = (uint8_t)byte;
 }
 template <typename T>
@@ -101,8 +102,9 @@ __global__ void __launch_bounds__(256) mx8_quantize_vec_kernel(const T* x, uint8
   if (!in) return;
   const uint32_t byte = mx_scale_byte<8>(top);
   const MxCoder<8> coder(byte, top);
-  auto four = [&](int k) { return coder.four(__float_as_uint(f[k]), __float_as_uint(f[k + 1]), __float_as_uint(f[k + 2]), __float_as_uint(f[k + 3])); };
-  *reinterpret_cast<uint2*>(codes + e) = make_uint2(four(0), four(4));
+  uint32_t w[2];
+  coder.words(reinterpret_cast<const uint32_t*>(f), w);
+  *reinterpret_cast<uint2*>(codes + e) = make_uint2(w[0], w[1]);
   if (c % MX_BLOCK == 0) scales[(long long)row * (vecs / 4) + c / MX_BLOCK] = (uint8_t)byte;
 }
 template <typename T>
@@ -190,23 +192,15 @@ __global__ void __launch_bounds__(256) mx8_quantize_ragged_kernel(const T* x, ui
   if (!at.any) return;
   const MxCoder<8> here(byte, top), there(mx_scale_byte<8>(top_after), top_after);
   uint32_t a[2];
-  if (at.next >= 8) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      a[h] = here.four(__float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1]), __float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3]));
-  } else if (here.exact && there.exact) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      a[h] = MxCoder<8>::pack(fmaf(f[4 * h], 4 * h < at.next ? here.m : there.m, MxCoder<8>::ROUND), fmaf(f[4 * h + 1], 4 * h + 1 < at.next ? here.m : there.m, MxCoder<8>::ROUND),
-                            fmaf(f[4 * h + 2], 4 * h + 2 < at.next ? here.m : there.m, MxCoder<8>::ROUND),
-                            fmaf(f[4 * h + 3], 4 * h + 3 < at.next ? here.m : there.m, MxCoder<8>::ROUND));
-  } else {
+  here.words(reinterpret_cast<const uint32_t*>(f), a);
+  if (at.next < 8) {
+    uint32_t b[2];
+    there.words(reinterpret_cast<const uint32_t*>(f), b);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t w[4] = {__float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1]), __float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3])};
       const int own_bytes = max(0, min(4, at.next - 4 * h));
       const uint32_t mask = own_bytes == 4 ? 0xffffffffu : (1u << (8 * own_bytes)) - 1u;
-      a[h] = (here.four(w[0], w[1], w[2], w[3]) & mask) | (there.four(w[0], w[1], w[2], w[3]) & ~mask);
+      a[h] = (a[h] & mask) | (b[h] & ~mask);
     }
   }
   uint8_t* to = codes + at.base + at.c;
@@ -258,13 +252,19 @@ __global__ void __launch_bounds__(256) mx8_dequantize_ragged_kernel(const uint8_
 }
 
 // The 16-bit codes of what gated_act_kernel takes, and back: a warp to a block, an element to a lane (only products in fp32 come here).
+__device__ __forceinline__ uint32_t code(const MxCoder<16>& coder, uint32_t v) {
+  const uint32_t pair[2] = {v, 0};
+  uint32_t w[1];
+  coder.words(pair, w);
+  return w[0];
+}
 __global__ void __launch_bounds__(256) mx16_quantize_kernel(const float* x, uint16_t* codes, uint8_t* scales, uint32_t warps, int K, uint32_t blocks) {
   after_previous();
   const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), row = w / blocks, c = (w - row * blocks) * MX_BLOCK + (threadIdx.x & 31);
   if (w >= warps) return;
   const uint32_t v = c < (uint32_t)K ? __float_as_uint(x[(long long)row * K + c]) : 0u, top = __reduce_max_sync(0xffffffffu, v & 0x7fffffffu);
   const uint32_t byte = mx_scale_byte<16>(top);
-  if (c < (uint32_t)K) codes[(long long)row * K + c] = (uint16_t)MxCoder<16>(byte, top).two(v, 0);
+  if (c < (uint32_t)K) codes[(long long)row * K + c] = (uint16_t)code(MxCoder<16>(byte, top), v);
   if ((threadIdx.x & 31) == 0) scales[w] = (uint8_t)byte;
 }
 __global__ void __launch_bounds__(256) mx16_dequantize_kernel(const uint16_t* codes, const uint8_t* scales, float* y, uint32_t warps, int K, uint32_t blocks) {
