@@ -34,8 +34,10 @@ __global__ void __launch_bounds__(256) mx8_quantize_kernel(const T* x, uint8_t* 
   if (!in) return;
   const uint32_t byte = mx_scale_byte<8>(top);
   const MxCoder<8> coder(byte, top);
-  uint32_t c[4];
-  coder.words(reinterpret_cast<const uint32_t*>(f), c);
+  uint32_t u[16], c[4];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(f[k]);
+  coder.words(u, c);
   reinterpret_cast<uint4*>(codes)[i] = make_uint4(c[0], c[1], c[2], c[3]);
   if ((i & 1) == 0) scales[i >> 1] = (uint8_t)byte;
 }
@@ -102,8 +104,10 @@ __global__ void __launch_bounds__(256) mx8_quantize_vec_kernel(const T* x, uint8
   if (!in) return;
   const uint32_t byte = mx_scale_byte<8>(top);
   const MxCoder<8> coder(byte, top);
-  uint32_t w[2];
-  coder.words(reinterpret_cast<const uint32_t*>(f), w);
+  uint32_t u[8], w[2];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) u[k] = __float_as_uint(f[k]);
+  coder.words(u, w);
   *reinterpret_cast<uint2*>(codes + e) = make_uint2(w[0], w[1]);
   if (c % MX_BLOCK == 0) scales[(long long)row * (vecs / 4) + c / MX_BLOCK] = (uint8_t)byte;
 }
@@ -192,10 +196,13 @@ __global__ void __launch_bounds__(256) mx8_quantize_ragged_kernel(const T* x, ui
   if (!at.any) return;
   const MxCoder<8> here(byte, top), there(mx_scale_byte<8>(top_after), top_after);
   uint32_t a[2];
-  here.words(reinterpret_cast<const uint32_t*>(f), a);
+  uint32_t u[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) u[k] = __float_as_uint(f[k]);
+  here.words(u, a);
   if (at.next < 8) {
     uint32_t b[2];
-    there.words(reinterpret_cast<const uint32_t*>(f), b);
+    there.words(u, b);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int own_bytes = max(0, min(4, at.next - 4 * h));
@@ -312,7 +319,7 @@ static unsigned blocks_of(long long n) { return (n + 255) / 256 > 0x7fffffffll ?
 using namespace apb;
 
 // x [R, K], codes [R, K], scales [R, ceil(K / 32)], all dense, x and codes on 16-byte bases.  Whole rows of blocks, rows of whole vectors, other rows:
-// 8192 x 14336 bf16 54, 14344 75, 14343 224 us (and back 58, 68, 108).
+// 8192 x 14336 bf16 53, 14344 75, 14343 205 us (and back 59, 68, 108).
 template <typename T>
 static int quantize(const T* x, uint8_t* codes, uint8_t* scales, long long R, long long K, cudaStream_t st) {
   const long long blocks = (K + MX_BLOCK - 1) / MX_BLOCK, groups = (blocks + RAGGED_BLOCKS - 1) / RAGGED_BLOCKS;
