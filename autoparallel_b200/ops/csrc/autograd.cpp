@@ -88,8 +88,12 @@ variable_list once(const char* what, const variable_list& g, F gradients) {
     out = gradients();
   }
   auto refuse = std::make_shared<torch::autograd::Error>(std::string(what) + ": no second derivatives on CUDA", std::move(edges));
-  for (Tensor& t : out)
-    if (t.defined()) torch::autograd::set_history(t, refuse);
+  for (Tensor& t : out) {
+    if (!t.defined()) continue;
+    for (const Tensor& from : g)
+      if (t.is_same(from)) t = t.detach();  // (a gradient that is passed on has a history of its own)
+    torch::autograd::set_history(t, refuse);
+  }
   return out;
 }
 
@@ -545,7 +549,7 @@ const Op<GatedFfnSig>& op_gated_ffn() { APB_OP(o, "gated_ffn", GatedFfnSig); ret
 // (dx, dw) of h and the weight, of whichever of both results have been used.
 Pair add_norm_gradients(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& w, const Tensor& rstd) {
   at::AutoDispatchBelowAutograd guard;  // (nothing is recorded here; without it every operator goes through the boxed kernel of those without a formula)
-  if (!dy.defined()) return {dh.detach(), at::zeros_like(w)};
+  if (!dy.defined()) return {dh, at::zeros_like(w)};  // (itself: the engine copies a gradient that someone else holds, and does not see that of an alias)
   return dh.defined() ? op_add_norm_bwd()(dy, dh, h, w, rstd) : op_rms_bwd()(dy, h, w, rstd);
 }
 struct AddNorm : torch::autograd::Function<AddNorm> {

@@ -408,7 +408,9 @@ at::Tensor dense(const at::Tensor& t) {
 at::Tensor as2d(const at::Tensor& t) {
   // (a single row is reshaped too: contiguous() does not look at its stride, which TMA does; the reshape makes it the width)
   at::Tensor m = t.dim() == 2 && t.size(0) > 1 && t.size(1) > 0 ? t : t.reshape({-1, t.size(-1)});
-  if (m.stride(1) != 1 || m.stride(0) % 8 != 0 || reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 != 0) m = dense(m);
+  // (rows that lie on one another, as those of an expanded gradient do, are written out: TMA has strides of at least a row)
+  const bool apart = m.size(0) <= 1 || m.stride(0) >= m.size(1);
+  if (m.stride(1) != 1 || m.stride(0) % 8 != 0 || !apart || reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 != 0) m = dense(m);
   return m;
 }
 

@@ -2,7 +2,6 @@
 // its anonymous namespace.
 using Five = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
 
-// Dense, and on a 16-byte base where the rows are taken in vectors.
 at::IntArrayRef lead_of(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
 std::vector<int64_t> with_last(at::IntArrayRef lead, std::initializer_list<int64_t> last) {
   auto s = lead.vec();
@@ -102,7 +101,7 @@ bool gated_form(std::initializer_list<const Tensor*> ts, std::initializer_list<i
   for (const Tensor* t : ts)
     if (t->scalar_type() != at::kBFloat16) return false;
   for (int64_t w : widths)
-    if (w == 0 || w % 8 != 0 || w > 0x3fffffff) return false;
+    if (w == 0 || w % 8 != 0 || w > 0x1fffffff) return false;  // (twice a width is counted too)
   return true;
 }
 int64_t rows_of(const Tensor& t, int dims) { return c10::multiply_integers(t.sizes().slice(0, t.dim() - dims)); }
@@ -111,6 +110,7 @@ void gated_check(const Tensor& x, std::initializer_list<const Tensor*> ws, const
   TORCH_CHECK(x.dim() >= 1 && float_or_bf16(x.scalar_type()), what, ": [.., D] in bf16 or fp32");
   for (const Tensor* w : ws)
     TORCH_CHECK(w->dim() == 2 && w->scalar_type() == x.scalar_type() && w->device() == x.device(), what, ": weights are matrices of the operand's type and device");
+  for (const Tensor* w : ws) TORCH_CHECK(w->size(0) <= 0x3fffffff && w->size(1) <= 0x3fffffff, what, ": weights of at most 2^30 - 1 rows and columns");
 }
 // x w^T or x w in fp32
 Tensor product32(const Tensor& x, const Tensor& w, bool trans) {

@@ -160,14 +160,14 @@ __device__ __forceinline__ void gated_tile(const GatedOut& o, uint8_t* stg, uint
     stage_put(stg, lane, v);
     uint32_t sa = 0, sb = 0;
     if constexpr (BITS > 0) sa = codes32<BITS>(a, stg + 2048, lane);
-    if constexpr (BITS == 8) sb = codes32<8>(b, stg + 3072, lane);
+    if constexpr (BITS == 8) sb = codes32<8>(b, stg + 2048 + 1024, lane);
     __syncwarp();
     stage_store(stg, o.h, H, row0, col + c, M, H, lane);
     if constexpr (BITS == 0) continue;
     if constexpr (BITS == 8) {
       uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab);
       stage_store8(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);
-      stage_store8(stg + 3072, codes + H, 2ll * H, row0, col + c, M, H, lane);
+      stage_store8(stg + 2048 + 1024, codes + H, 2ll * H, row0, col + c, M, H, lane);
     } else if constexpr (BITS == 16) {
       __nv_bfloat16* codes = reinterpret_cast<__nv_bfloat16*>(o.ab);  // (two bytes each)
       stage_store(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);

@@ -128,7 +128,7 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 # ----------------------------------------------------------------------------------- GEMM family
 def _as2d(t: torch.Tensor) -> torch.Tensor:
     t2 = t.reshape(-1, t.shape[-1])
-    if t2.stride(-1) != 1 or (t2.stride(0) % 8) != 0 or (t2.data_ptr() % 16) != 0:
+    if t2.stride(-1) != 1 or (t2.stride(0) % 8) != 0 or (t2.data_ptr() % 16) != 0 or 1 < t2.shape[0] and t2.stride(0) < t2.shape[1]:
         t2 = _dense(t2)
     return t2
 

@@ -221,6 +221,20 @@ def test_norm_where_one_result_is_used():
     assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[1])
 
 
+def test_gradients_do_not_share_memory():
+    """Where only the sum is used its gradient is passed on; what becomes of one leaf's gradient is not seen in another's, nor in the caller's."""
+    w = torch.ones(264, device="cuda", dtype=BF)
+    for used, f in ((0, lambda *a: K.add_rms_norm(*a)[1]), (1, lambda *a: K.add_rms_norm_fp8(*a)[1]), (2, lambda *a: sum(K.add_rms_norm(*a)))):
+        x, r = (_randn(9, 264, gen=_gen(s)).requires_grad_() for s in (1, 2))
+        dy = torch.ones_like(x)
+        f(x, r, w).backward(dy)
+        assert len({t.data_ptr() for t in (dy, x.grad, r.grad)}) == 3, used
+        x.grad.zero_()
+        assert bool((dy == 1).all()) and (used == 2 or bool((r.grad == 1).all())), used
+        r.grad.zero_()
+        assert bool((dy == 1).all()), used
+
+
 # ------------------------------------------------------------------------------------ gated block
 def _gated(M, D, H, N, dtype=BF, seed=0):
     g = _gen(seed)
@@ -358,6 +372,24 @@ def test_gated_ffn_leading_dims_strides_and_partial_gradients():
         a, b = (torch.autograd.grad(f(K.gated_ffn(*every, checkpoint=checkpoint)), every[0])[0]
                 for f in (lambda t: t.float().sum(), lambda t: (t * torch.ones_like(t)).float().sum()))
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("M", [5, 33, 300])
+@pytest.mark.parametrize("checkpoint", ["full", "mx8"])
+def test_gated_ffn_of_rows_that_lie_on_one_another(M, checkpoint):
+    """An expanded x, expanded weights, and the expanded gradient that a sum over rows has: the results of the same values written out."""
+    x, w1, w3, w2, dy = _gated(M, 128, 264, 96)
+    x, w1, w3, w2, dy = x[:1].expand(M, 128), w1[:1].expand(264, 128), w3, w2[:1].expand(96, 264), dy[:1].expand(M, 96)
+    out = []
+    for f in (lambda t: t, lambda t: t.contiguous()):
+        leaves = [f(t.detach()).requires_grad_() for t in (x, w1, w3, w2)]
+        y = K.gated_ffn(*leaves, checkpoint=checkpoint)
+        out.append((y, *torch.autograd.grad(y, leaves, f(dy))))
+        out[-1] += (*torch.autograd.grad(K.gated_ffn(*leaves, checkpoint=checkpoint).sum(0), leaves, dy[0]),)
+    for i, (a, b) in enumerate(zip(*out)):
+        assert torch.equal(a, b), i
+    three = x.unsqueeze(0).expand(3, M, 128)
+    assert torch.equal(K.gated_ffn(three, w1, w3, w2), K.gated_ffn(three.contiguous(), w1, w3, w2))
 
 
 def test_gated_ffn_where_values_are_not_numbers():
@@ -633,7 +665,7 @@ def test_llama_with_the_fused_block(checkpoint):
         m.rope_cos, m.rope_sin = m.rope_cos.float(), m.rope_sin.float()
         loss = m(tokens, labels)
         loss.backward()
-        return float(loss), {n: p.grad for n, p in m.named_parameters()}
+        return float(loss.detach()), {n: p.grad for n, p in m.named_parameters()}
 
     loss, grads = step()
     fused, g2 = step(fused_ffn=True, fused_norm=True, ffn_checkpoint=checkpoint)
