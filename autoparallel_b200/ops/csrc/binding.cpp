@@ -93,6 +93,10 @@ int apb_gated_act(const float* ab, void* h, long long M, int H, int act, int is_
 int apb_gated_act_bwd(const float* dh, const float* ab, void* dab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st);
 int apb_mx16_quantize(const float* x, void* codes, void* scales, long long R, int K, cudaStream_t st);
 int apb_mx16_dequantize(const void* codes, const void* scales, float* y, long long R, int K, cudaStream_t st);
+int apb_gemm_get_reserved_sms();
+int apb_gemm_rows_takes(int M, int N, int K, int num_sms);
+int apb_gemm_rows_behind(const void* X, const void* W, void* C, int M, int N, int K, long long ldx, long long ldw, long long ldc, int out_fp32, int num_sms,
+                         cudaStream_t st);
 int apb_gemm_gated(const void* x, const void* w1, const void* w3, void* h, void* ab, void* scales, int bits, int M, int H, int K, long long ldx,
                    long long ldw1, long long ldw3, int act, uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_gemm_gated_grad(const void* dy, const void* w2, const void* ab, const void* scales, int bits, void* dab, void* h, int M, int H, int K, long long ldy,

@@ -228,13 +228,30 @@ Two gated_wgrad(const Tensor& dab, const Tensor& x, at::ScalarType dtype) {
   return {first, dense(second)};  // (a half that begins off a 16-byte boundary is copied)
 }
 
+// Whether the product with w2 is the few-row kernel's, with w2 as it lies in memory (a copy would be made by the kernel before it).
+bool few_rows_behind(const Tensor& h, const Tensor& w2, int64_t M, int64_t N, int64_t H) {
+  return gated_form({&h}, {N, H}) && M <= 32 && apb_gemm_get_reserved_sms() == 0 && apb_gemm_rows_takes((int)M, (int)N, (int)H, num_sms()) &&
+         w2.stride(1) == 1 && w2.stride(0) >= H && w2.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(w2.data_ptr()) % 16 == 0;
+}
+
 Five gated_ffn(const Tensor& x, const Tensor& w1, const Tensor& w3, const Tensor& w2, int64_t act, int64_t bits) {
   c10::cuda::CUDAGuard g(x.device());
   gated_check(x, {&w1, &w3, &w2}, "gated_ffn");
   TORCH_CHECK(w2.size(1) == w1.size(0), "gated_ffn: w1 and w3 [H, D], w2 [N, H]");
   auto [h, ab, scales] = gated_mm(x, w1, w3, act, bits);
   const int64_t N = w2.size(0);
-  Tensor y = h.numel() == 0 || N == 0 ? at::zeros(with_last(lead_of(x), {N}), x.options()) : op_mm_nd(h, w2, true, x.scalar_type());
+  const int64_t M = rows_of(h, 1), H = h.size(-1);
+  Tensor y;
+  if (h.numel() == 0 || N == 0) {
+    y = at::zeros(with_last(lead_of(x), {N}), x.options());
+  } else if (ours(MM_ND) && few_rows_behind(h, w2, M, N, H)) {
+    y = at::empty(with_last(lead_of(x), {N}), x.options());
+    check(apb_gemm_rows_behind(h.data_ptr(), w2.data_ptr(), y.data_ptr(), (int)M, (int)N, (int)H, H, w2.stride(0), N, 0, num_sms(), stream()),
+          "apb_gemm_rows_behind");
+    count();
+  } else {
+    y = op_mm_nd(h, w2, true, x.scalar_type());
+  }
   const auto u8 = x.options().dtype(at::kByte);
   if (bits != 8) return {y, ab, scales, at::empty({0}, u8), at::empty({0}, u8)};
   auto [xq, xs] = mx8_quantize(x);

@@ -49,8 +49,9 @@ struct RowsGated {
   int act;
 };
 
-// MB: blocks of 8 rows of X; U: steps of 32 elements of K whose loads are under way together
-template <int MB, int U, typename Out>
+// MB: blocks of 8 rows of X; U: steps of 32 elements of K whose loads are under way together.  EARLY: the kernel before does not write W, nor can one before
+// that be writing it still (it lets this one in behind its own wait), so the first loads of W do not wait for it.
+template <int MB, int U, bool EARLY, typename Out>
 __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bfloat16* W, int M, int N, int K, long long ldx, long long ldw, const Out& out) {
   constexpr int TM = 8 * MB;
   __shared__ float part[ROWS_WARPS][TM * ROWS_TILE];
@@ -76,8 +77,7 @@ __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bflo
     x[i] = X + (xk[i] ? g + 8 * i : 0) * ldx + c;
   }
   float acc[MB][4] = {};
-  for (int s = s0; s < s1; s += U) {
-    uint4 wv[U][2], xv[U][MB];
+  auto load_w = [&](uint4 (&wv)[U][2], int s) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = (s + u) * 32;
@@ -87,6 +87,14 @@ __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bflo
         wv[u][i] = make_uint4(0, 0, 0, 0);
         if (in && wk[i]) wv[u][i] = ld_stream(w[i] + k);
       }
+    }
+  };
+  auto step = [&](const uint4 (&wv)[U][2], int s) {
+    uint4 xv[U][MB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (s + u) * 32;
+      const bool in = s + u < s1 && k + c < K;
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
         xv[u][i] = make_uint4(0, 0, 0, 0);
@@ -102,6 +110,18 @@ __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bflo
         mma_bf16(acc[m], a.z, b.z, a.w, b.w, xv[u][m].z, xv[u][m].w);
       }
     }
+  };
+  uint4 wv[U][2];
+  int s = s0;
+  if constexpr (EARLY) {
+    load_w(wv, s);
+    after_previous();
+    step(wv, s);  // (a warp without steps has zeros)
+    s += U;
+  }
+  for (; s < s1; s += U) {
+    load_w(wv, s);
+    step(wv, s);
   }
   const int m2 = (lane & 3) * 2;
 #pragma unroll
@@ -139,18 +159,18 @@ __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bflo
   }
 }
 
-template <int MB, int U, int MIN_BLOCKS>
+template <int MB, int U, int MIN_BLOCKS, bool EARLY>
 __global__ void __launch_bounds__(32 * ROWS_WARPS, MIN_BLOCKS)
 gemm_rows_kernel(const __nv_bfloat16* X, const __nv_bfloat16* W, void* C, int M, int N, int K, long long ldx,
                  long long ldw, long long ldc, int out_fp32) {
-  after_previous();
-  rows_cta<MB, U>(X, W, M, N, K, ldx, ldw, RowsPlain{C, ldc, out_fp32});
+  if (!EARLY) after_previous();
+  rows_cta<MB, U, EARLY>(X, W, M, N, K, ldx, ldw, RowsPlain{C, ldc, out_fp32});
 }
 template <int MB, int U, int MIN_BLOCKS>
 __global__ void __launch_bounds__(32 * ROWS_WARPS, MIN_BLOCKS)
 gemm_rows_gated_kernel(const __nv_bfloat16* X, const __nv_bfloat16* W, int M, int N, int K, long long ldx, long long ldw, const RowsGated out) {
   after_previous();
-  rows_cta<MB, U>(X, W, M, N, K, ldx, ldw, out);
+  rows_cta<MB, U, false>(X, W, M, N, K, ldx, ldw, out);
 }
 
 }  // namespace apb
@@ -176,9 +196,10 @@ extern "C" int apb_gemm_rows_takes(int M, int N, int K, int num_sms) {
   return M <= ROWS_MAX && (size <= 8192 || (K >= 192 && x <= 49152 && size <= 2048 * 2048 && N <= 8ll * K));
 }
 
-// X, W: 16-byte bases and rows.  Returns 0, or an argument / launch error (nothing launched).
-extern "C" int apb_gemm_rows(const void* X, const void* W, void* C, int M, int N, int K, long long ldx, long long ldw, long long ldc, int out_fp32,
-                             int num_sms, cudaStream_t st) {
+namespace apb {
+template <bool EARLY>
+static int gemm_rows(const void* X, const void* W, void* C, int M, int N, int K, long long ldx, long long ldw, long long ldc, int out_fp32, int num_sms,
+                     cudaStream_t st) {
   if (M <= 0 || N <= 0) return 0;
   if (M > ROWS_MAX || K <= 0 || (K & 7) || (ldx & 7) || (ldw & 7) || ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(W)) & 15)) return 3;
   const unsigned grid = (unsigned)((N + ROWS_TILE - 1) / ROWS_TILE);
@@ -188,10 +209,22 @@ extern "C" int apb_gemm_rows(const void* X, const void* W, void* C, int M, int N
   // Two blocks to an SM and three steps under way; where there is no second block and K is long enough for it, four (8 x 2048 x 2048 4.0 -> 3.7 us, 32
   // x 2048 x 2048 6.4 -> 5.3; 8 x 512 x 512 2.0 -> 2.2).
   const bool deep = grid <= (unsigned)num_sms && K >= 2048;
-  if (M <= 8) deep ? launch(gemm_rows_kernel<1, 4, 1>) : launch(gemm_rows_kernel<1, 3, 2>);
-  else if (M <= 16) launch(gemm_rows_kernel<2, 3, 2>);
-  else deep ? launch(gemm_rows_kernel<4, 4, 1>) : launch(gemm_rows_kernel<4, 3, 2>);
+  if (M <= 8) deep ? launch(gemm_rows_kernel<1, 4, 1, EARLY>) : launch(gemm_rows_kernel<1, 3, 2, EARLY>);
+  else if (M <= 16) launch(gemm_rows_kernel<2, 3, 2, EARLY>);
+  else deep ? launch(gemm_rows_kernel<4, 4, 1, EARLY>) : launch(gemm_rows_kernel<4, 3, 2, EARLY>);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+}  // namespace apb
+
+// X, W: 16-byte bases and rows.  Returns 0, or an argument / launch error (nothing launched).
+extern "C" int apb_gemm_rows(const void* X, const void* W, void* C, int M, int N, int K, long long ldx, long long ldw, long long ldc, int out_fp32,
+                             int num_sms, cudaStream_t st) {
+  return gemm_rows<false>(X, W, C, M, N, K, ldx, ldw, ldc, out_fp32, num_sms, st);
+}
+// The same behind a kernel of ``launch_after`` that has made X and does not write W, whatever that one is: the first loads of W do not wait for its end.
+extern "C" int apb_gemm_rows_behind(const void* X, const void* W, void* C, int M, int N, int K, long long ldx, long long ldw, long long ldc, int out_fp32,
+                                    int num_sms, cudaStream_t st) {
+  return gemm_rows<true>(X, W, C, M, N, K, ldx, ldw, ldc, out_fp32, num_sms, st);
 }
 
 // h[M, H] = act(X W1^T) * (X W3^T) (gated.cuh).

@@ -360,7 +360,7 @@ def _mx4_mm_values(a, codes, scales, k, out_dtype):
     return out if out.shape[-1] == k else out[..., :k].contiguous()
 
 
-# ----------------------------------------------------------------------------------- the feed-forward block (these count their own launches)
+# ----------------------------------------------------------------------------------- the feed-forward block (counts its own launches)
 def _add_rms_norm(x, residual, weight, eps):
     return _C.add_rms_norm(x, residual, weight, eps)
 

@@ -3,12 +3,13 @@
 Operators (``apb200::``; the functions at the end of this file check arguments and fill in defaults)
 
     add_rms_norm(x, residual, weight, eps)        h = x + residual (rounded to its type) and y = rms_norm(h)
-    add_rms_norm_fp8(.., keep)                    the same with y in e4m3, one scale a row, as ``scaled_mm`` takes them; the residual may be left out
+    add_rms_norm_fp8(.., keep)                    the same with y in e4m3, one scale a row, as ``scaled_mm`` takes them; the residual may
+                                                  be left out
     gated_ffn(x, w1, w3, w2, act, bits)           (act(x w1^T) * (x w3^T)) w2^T
     mx8_quantize(x), mx8_dequantize(..)           activations in 8 bits
 
-and what the gradients of the block are made with: ``add_rms_norm_bwd``, ``gated_mm`` (both projections and their product), ``gated_dgrad`` (through w2 and
-the product), ``gated_dx``, ``gated_wgrad``.
+and what the gradients of the block are made with: ``add_rms_norm_bwd``, ``gated_mm`` (both projections and their product),
+``gated_dgrad`` (through w2 and the product), ``gated_dx``, ``gated_wgrad``.
 
 Norm.  With ``r = 1 / sqrt(mean(h^2) + eps)``, ``n = h r``, ``g = dy w``:
 
@@ -21,20 +22,22 @@ Gated block.  With ``a = x w1^T``, ``b = x w3^T``, ``h = act(a) * b``, ``y = h w
     dh = dy w2       da = dh b act'(a)       db = dh act(a)
     dx = da w1 + db w3       dw1 = da^T x       dw3 = db^T x       dw2 = dy^T h
 
-a and b are kept for the backward pass, ``ab`` [.., 2, H], h is made again from them.  ``bits`` 16 keeps x as it is, and a, b as 16-bit codes (below) where x is
-bf16, as they are where it is fp32; 8 keeps all three as 8-bit checkpoints, from which all gradients are made; 0 keeps nothing (no gradients).  da, db and the
-h of the backward pass are rounded to x's type, which is what the products of the gradients take.
+a and b are kept for the backward pass, ``ab`` [.., 2, H], h is made again from them.  ``bits`` 16 keeps x as it is, and a, b as 16-bit
+codes (below) where x is bf16, as they are where it is fp32; 8 keeps all three as 8-bit checkpoints, from which all gradients are made;
+0 keeps nothing (no gradients).  da, db and the h of the backward pass are rounded to x's type, which is what the products of the
+gradients take.
 
 8-bit checkpoints (MXINT8 of the OCP Microscaling Formats specification, version 1.0).  32 values along the last dim share a power of two,
 
     e = max(floor(log2 of the largest magnitude), -120)     code = v 2^(6-e), rounded to even, within +-127     value = code 2^(e-6)
 
-codes int8 of the values' shape, scales uint8 [.., ceil(K / 32)]: e + 127, and 255 for a block with an infinity or a NaN, which reads as NaN.  A value is
-off by at most 2^(e-7), but 2^(e-6) where it is the block's largest and rounds to 128; it is exact in bf16.  The 16-bit codes are the same with 14 for 6,
--112 for -120 and 32767 for 127: in as many bits as bf16, off by 2^-15 of the block's largest value and not by 2^-9 of each.
+codes int8 of the values' shape, scales uint8 [.., ceil(K / 32)]: e + 127, and 255 for a block with an infinity or a NaN, which reads as
+NaN.  A value is off by at most 2^(e-7), but 2^(e-6) where it is the block's largest and rounds to 128; it is exact in bf16.  The 16-bit
+codes are the same with 14 for 6, -112 for -120 and 32767 for 127: in as many bits as bf16, off by 2^-15 of the block's largest value and
+not by 2^-9 of each.
 
-The reference leaves these to the tracing compiler (``x + attention``, RMSNorm and SwiGLU of autoparallel/_testing/models/llama3.py:320-429); it has no 8-bit
-checkpoints.
+The reference leaves these to the tracing compiler (``x + attention``, RMSNorm and SwiGLU of
+autoparallel/_testing/models/llama3.py:320-429); it has no 8-bit checkpoints.
 """
 from __future__ import annotations
 
@@ -205,9 +208,9 @@ _META = {
     "gated_wgrad": lambda dab, x, dtype: tuple(_new(x, (dab.shape[-1], x.shape[-1]), dtype) for _ in range(2)),
     "gated_ffn": _gated_ffn_meta,
 }
-_REFS = {"add_rms_norm": _add_rms_norm, "add_rms_norm_bwd": _add_rms_norm_bwd, "add_rms_norm_fp8": _add_rms_norm_fp8, "mx8_quantize": _mx8_quantize,
-         "mx8_dequantize": _mx8_dequantize, "gated_mm": _gated_mm, "gated_dgrad": _gated_dgrad, "gated_dx": _gated_dx, "gated_wgrad": _gated_wgrad,
-         "gated_ffn": _gated_ffn}
+_REFS = {"add_rms_norm": _add_rms_norm, "add_rms_norm_bwd": _add_rms_norm_bwd, "add_rms_norm_fp8": _add_rms_norm_fp8,
+         "mx8_quantize": _mx8_quantize, "mx8_dequantize": _mx8_dequantize, "gated_mm": _gated_mm, "gated_dgrad": _gated_dgrad,
+         "gated_dx": _gated_dx, "gated_wgrad": _gated_wgrad, "gated_ffn": _gated_ffn}
 for _name, _fn in _REFS.items():
     lib.impl(_name, _fn, "CPU")
     lib.impl(_name, _META[_name], "Meta")
@@ -294,8 +297,8 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     """``h = x + residual``, rounded to their type, and ``rms_norm(h, weight)``: (norm, h).  Gradients of both results reach x, the
     residual and the weight in one pass."""
     xs = x.shape
-    if not (x.dtype in _FLOATS and xs and 1 <= xs[-1] <= 32768 and residual.shape == xs and residual.dtype is x.dtype and weight.shape == xs[-1:]
-            and weight.dtype in _FLOATS and x.device == residual.device == weight.device):
+    if not (x.dtype in _FLOATS and xs and 1 <= xs[-1] <= 32768 and residual.shape == xs and residual.dtype is x.dtype
+            and weight.shape == xs[-1:] and weight.dtype in _FLOATS and x.device == residual.device == weight.device):
         _check_norm("add_rms_norm", x, residual, weight)
     y, h, _ = ops.add_rms_norm(x, residual, weight, eps)
     return y, h
@@ -307,7 +310,8 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: tor
     training step hands the gradient of what it made of them to ``y``, the norm itself, which ``keep=False`` leaves out (None)."""
     xs = x.shape
     # (one test for the calls that are right: this is the path of single tokens)
-    if not (x.dtype in _FLOATS and xs and 1 <= xs[-1] <= 32768 and weight.shape == xs[-1:] and weight.dtype in _FLOATS and weight.device == x.device
+    if not (x.dtype in _FLOATS and xs and 1 <= xs[-1] <= 32768 and weight.shape == xs[-1:] and weight.dtype in _FLOATS
+            and weight.device == x.device
             and (residual is None or (residual.shape == xs and residual.dtype is x.dtype and residual.device == x.device))):
         _check_norm("add_rms_norm_fp8", x, residual, weight)
     if not keep and torch.is_grad_enabled():
@@ -335,7 +339,8 @@ def mx8_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype
     return ops.mx8_dequantize(codes, scales, dtype)
 
 
-def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor, act: str = "silu", checkpoint: str = "full") -> torch.Tensor:
+def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor, act: str = "silu",
+              checkpoint: str = "full") -> torch.Tensor:
     """``(act(x w1^T) * (x w3^T)) w2^T``: x [.., D], w1 and w3 [H, D], w2 [N, H] -> [.., N].  ``act``: "silu", "gelu" (by the error
     function) or "gelu_tanh".  ``checkpoint``: what the backward pass finds, "full" (x, and both projections in as many bits as its type
     has) or "mx8" (the same in 8 bits, about half the memory; the gradients are those of the rounded values)."""
@@ -348,6 +353,7 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Ten
         _need(x.dtype in _FLOATS and x.dtype is w1.dtype is w3.dtype is w2.dtype,
               f"gated_ffn: x, w1, w3, w2 are {x.dtype}, {w1.dtype}, {w3.dtype}, {w2.dtype}; all bf16 or all fp32 expected")
         _need(x.device == w1.device == w3.device == w2.device, "gated_ffn: operands on different devices")
-        _need(False, f"gated_ffn: x {tuple(xs)}, w1 {tuple(ws)}, w3 {tuple(w3.shape)}, w2 {tuple(w2.shape)}: [.., D], [H, D], [H, D], [N, H] expected")
+        _need(False, f"gated_ffn: x {tuple(xs)}, w1 {tuple(ws)}, w3 {tuple(w3.shape)}, w2 {tuple(w2.shape)}: "
+                     "[.., D], [H, D], [H, D], [N, H] expected")
     records = torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w3.requires_grad or w2.requires_grad)
     return ops.gated_ffn(x, w1, w3, w2, ACTS[act], CHECKPOINTS[checkpoint] if records else 0)[0]

@@ -2,7 +2,7 @@
 
 Tolerances are relative to the size of the result (its root mean square over the tensor, or the value where that is larger).  A rounding to bf16 is off by at
 most 2^-8 of the value, a sum of n products in fp32 by at most n 2^-24 of the sum of the magnitudes and by about sqrt(n) 2^-24 of it; what a formula rounds on its
-way (h, da, db, and a, b where they are kept in bf16) adds its own half step, spread over a sum of n terms like noise: the factors below count those."""
+way (h, da, db, and the codes of a, b) adds its own half step, spread over a sum of n terms like noise: the factors below count those."""
 import math
 
 import pytest
