@@ -228,9 +228,13 @@ Two gated_wgrad(const Tensor& dab, const Tensor& x, at::ScalarType dtype) {
   return {first, dense(second)};  // (a half that begins off a 16-byte boundary is copied)
 }
 
-// Whether the product with w2 is the few-row kernel's, with w2 as it lies in memory (a copy would be made by the kernel before it).
+// Whether the product with w2 is the few-row kernel's, whose first loads do not wait for h, with w2 as it lies in memory (a copy would be made by the kernel
+// before it): where a product of its own would be, and up to 16 rows for a round of blocks (two to an SM, of 16 columns) also where the contraction is longer; both
+// products of the block, us, so / with the split kernel: 8 x 4096 x 14336 57 / 67, 16 x 4096 x 14336 70 / 73, 16 x 2048 x 14336 39 / 41; with fewer columns
+// 16 x 512 x 14336 24 / 19.
 bool few_rows_behind(const Tensor& h, const Tensor& w2, int64_t M, int64_t N, int64_t H) {
-  return gated_form({&h}, {N, H}) && M <= 32 && apb_gemm_get_reserved_sms() == 0 && apb_gemm_rows_takes((int)M, (int)N, (int)H, num_sms()) &&
+  return gated_form({&h}, {N, H}) && M <= 32 && apb_gemm_get_reserved_sms() == 0 &&
+         (apb_gemm_rows_takes((int)M, (int)N, (int)H, num_sms()) || (M <= 16 && N >= 2048 && N <= 32 * num_sms())) &&
          w2.stride(1) == 1 && w2.stride(0) >= H && w2.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(w2.data_ptr()) % 16 == 0;
 }
 

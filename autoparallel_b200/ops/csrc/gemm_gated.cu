@@ -136,9 +136,9 @@ static bool off16(std::initializer_list<const void*> ps) {
 
 using namespace apb;
 
-// Whether a call is the few-row kernel's: as a plain product with 2 H columns (0 to 5 % from the better one of both in 96 sizes), and with up to 8 rows and many
-// columns also where the contraction is long, few-row / split kernel, us: 1 x 8192 x 28672 144 / 195, 4 x 8192 x 8192 49 / 57, 8 x 7168 x 9216 46 / 66, 8 x 7168
-// x 18432 86 / 104, 6 x 14336 x 4096 43 / 43; with few columns 8 x 8192 x 2560 22 / 19.
+// Whether a call is the few-row kernel's: as a plain product with 2 H columns, and with up to 8 rows and many columns also where the contraction is long.  385 sizes
+// (1 to 32 rows, 256 <= K <= 4096, 256 <= H <= 28672): 1 to 3 % from the better one of both; few-row / split kernel, us: 1 x 4096 x 14336 37 / 42, 8 x 4096 x 5632
+// 17 / 19, 1 x 8192 x 28672 144 / 195, 12 x 2048 x 5632 12 / 14, 32 x 1024 x 1024 3.7 / 5.0; 16 x 4096 x 14336 46 / 42, 32 x 2048 x 14336 36 / 24.
 static bool few_rows(int M, int H, int K, int num_sms) {
   return M <= 32 && (apb_gemm_rows_takes(M, 2 * H, K, num_sms) || (M <= 8 && H >= 4096));
 }

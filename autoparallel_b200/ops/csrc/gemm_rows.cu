@@ -49,15 +49,15 @@ struct RowsGated {
   int act;
 };
 
-// MB: blocks of 8 rows of X; U: steps of 32 elements of K whose loads are under way together.  EARLY: the kernel before does not write W, nor can one before
+// MB: blocks of 8 rows of X; U: steps of 32 elements of K whose loads are under way together; RW: warps of a block, which share K.  EARLY: the kernel before does not write W, nor can one before
 // that be writing it still (it lets this one in behind its own wait), so the first loads of W do not wait for it.
-template <int MB, int U, bool EARLY, typename Out>
+template <int MB, int U, int RW, bool EARLY, typename Out>
 __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bfloat16* W, int M, int N, int K, long long ldx, long long ldw, const Out& out) {
   constexpr int TM = 8 * MB;
-  __shared__ float part[ROWS_WARPS][TM * ROWS_TILE];
+  __shared__ float part[RW][TM * ROWS_TILE];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = (lane & 3) * 8;
   const int n0 = blockIdx.x * (Out::PAIR ? ROWS_TILE / 2 : ROWS_TILE);
-  const int steps = (K + 31) / 32, s0 = steps * warp / ROWS_WARPS, s1 = steps * (warp + 1) / ROWS_WARPS;
+  const int steps = (K + 31) / 32, s0 = steps * warp / RW, s1 = steps * (warp + 1) / RW;
   const __nv_bfloat16* w[2];
   const __nv_bfloat16* x[MB];
   bool wk[2], xk[MB];  // rows outside the matrices load nothing
@@ -130,11 +130,11 @@ __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bflo
     for (int i = 0; i < 4; ++i) part[warp][(8 * m + m2 + (i & 1)) * ROWS_TILE + g + 8 * (i >> 1)] = acc[m][i];
   __syncthreads();
   if constexpr (Out::PAIR) {
-    for (int t = threadIdx.x; t < M * (ROWS_TILE / 2); t += 32 * ROWS_WARPS) {
+    for (int t = threadIdx.x; t < M * (ROWS_TILE / 2); t += 32 * RW) {
       const int m = t / (ROWS_TILE / 2), n = n0 + t % (ROWS_TILE / 2), at = m * ROWS_TILE + t % (ROWS_TILE / 2);
       float a = 0.f, b = 0.f, h = 0.f;
 #pragma unroll
-      for (int i = 0; i < ROWS_WARPS; ++i) {
+      for (int i = 0; i < RW; ++i) {
         a += part[i][at];
         b += part[i][at + ROWS_TILE / 2];
       }
@@ -146,10 +146,10 @@ __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bflo
       out.h[(long long)m * N + n] = __float2bfloat16(h);
     }
   } else {
-    for (int t = threadIdx.x; t < M * ROWS_TILE; t += 32 * ROWS_WARPS) {
+    for (int t = threadIdx.x; t < M * ROWS_TILE; t += 32 * RW) {
       float v = 0.f;
 #pragma unroll
-      for (int i = 0; i < ROWS_WARPS; ++i) v += part[i][t];
+      for (int i = 0; i < RW; ++i) v += part[i][t];
       const int m = t / ROWS_TILE, n = n0 + t % ROWS_TILE;
       if (n < N) {
         if (out.out_fp32) reinterpret_cast<float*>(out.C)[m * out.ldc + n] = v;
@@ -159,18 +159,18 @@ __device__ __forceinline__ void rows_cta(const __nv_bfloat16* X, const __nv_bflo
   }
 }
 
-template <int MB, int U, int MIN_BLOCKS, bool EARLY>
-__global__ void __launch_bounds__(32 * ROWS_WARPS, MIN_BLOCKS)
+template <int MB, int U, int MIN_BLOCKS, bool EARLY, int RW = ROWS_WARPS>
+__global__ void __launch_bounds__(32 * RW, MIN_BLOCKS)
 gemm_rows_kernel(const __nv_bfloat16* X, const __nv_bfloat16* W, void* C, int M, int N, int K, long long ldx,
                  long long ldw, long long ldc, int out_fp32) {
   if (!EARLY) after_previous();
-  rows_cta<MB, U, EARLY>(X, W, M, N, K, ldx, ldw, RowsPlain{C, ldc, out_fp32});
+  rows_cta<MB, U, RW, EARLY>(X, W, M, N, K, ldx, ldw, RowsPlain{C, ldc, out_fp32});
 }
-template <int MB, int U, int MIN_BLOCKS>
-__global__ void __launch_bounds__(32 * ROWS_WARPS, MIN_BLOCKS)
+template <int MB, int RW, int MIN_BLOCKS>
+__global__ void __launch_bounds__(32 * RW, MIN_BLOCKS)
 gemm_rows_gated_kernel(const __nv_bfloat16* X, const __nv_bfloat16* W, int M, int N, int K, long long ldx, long long ldw, const RowsGated out) {
   after_previous();
-  rows_cta<MB, U, false>(X, W, M, N, K, ldx, ldw, out);
+  rows_cta<MB, 4, RW, false>(X, W, M, N, K, ldx, ldw, out);
 }
 
 }  // namespace apb
@@ -203,15 +203,23 @@ static int gemm_rows(const void* X, const void* W, void* C, int M, int N, int K,
   if (M <= 0 || N <= 0) return 0;
   if (M > ROWS_MAX || K <= 0 || (K & 7) || (ldx & 7) || (ldw & 7) || ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(W)) & 15)) return 3;
   const unsigned grid = (unsigned)((N + ROWS_TILE - 1) / ROWS_TILE);
-  auto launch = [&](auto kern) {
-    launch_after(kern, grid, 32 * ROWS_WARPS, 0, st, (const __nv_bfloat16*)X, (const __nv_bfloat16*)W, C, M, N, K, ldx, ldw, ldc, out_fp32);
+  auto launch = [&](auto kern, int warps = ROWS_WARPS) {
+    launch_after(kern, grid, 32 * warps, 0, st, (const __nv_bfloat16*)X, (const __nv_bfloat16*)W, C, M, N, K, ldx, ldw, ldc, out_fp32);
   };
   // Two blocks to an SM and three steps under way; where there is no second block and K is long enough for it, four (8 x 2048 x 2048 4.0 -> 3.7 us, 32
-  // x 2048 x 2048 6.4 -> 5.3; 8 x 512 x 512 2.0 -> 2.2).
-  const bool deep = grid <= (unsigned)num_sms && K >= 2048;
-  if (M <= 8) deep ? launch(gemm_rows_kernel<1, 4, 1, EARLY>) : launch(gemm_rows_kernel<1, 3, 2, EARLY>);
-  else if (M <= 16) launch(gemm_rows_kernel<2, 3, 2, EARLY>);
-  else deep ? launch(gemm_rows_kernel<4, 4, 1, EARLY>) : launch(gemm_rows_kernel<4, 3, 2, EARLY>);
+  // x 2048 x 2048 6.4 -> 5.3; 8 x 512 x 512 2.0 -> 2.2).  EARLY: four whatever K is, as they are on their way while the kernel before ends (both
+  // products of a gated block with up to 2368 columns of this one, 308 sizes, 6 % less in the mean); more than 16 rows in two blocks of eight warps, which do
+  // not spill (7 % less).
+  const bool deep = grid <= (unsigned)num_sms && (EARLY || K >= 2048);
+  if (M <= 8) {
+    deep ? launch(gemm_rows_kernel<1, 4, 1, EARLY>) : launch(gemm_rows_kernel<1, 3, 2, EARLY>);
+  } else if constexpr (EARLY) {
+    if (M <= 16) deep ? launch(gemm_rows_kernel<2, 4, 1, true>) : launch(gemm_rows_kernel<2, 3, 2, true>);
+    else deep ? launch(gemm_rows_kernel<4, 4, 1, true>) : launch(gemm_rows_kernel<4, 4, 2, true, 8>, 8);
+  } else {
+    if (M <= 16) launch(gemm_rows_kernel<2, 3, 2, false>);
+    else deep ? launch(gemm_rows_kernel<4, 4, 1, false>) : launch(gemm_rows_kernel<4, 3, 2, false>);
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 }  // namespace apb
@@ -236,12 +244,16 @@ extern "C" int apb_gemm_rows_gated(const void* X, const void* W1, const void* W3
     return 3;
   const unsigned grid = (unsigned)((H + ROWS_TILE / 2 - 1) / (ROWS_TILE / 2));
   const RowsGated out{(const __nv_bfloat16*)W3, ldw3, (__nv_bfloat16*)h, act};
-  auto launch = [&](auto kern) {
-    launch_after(kern, grid, 32 * ROWS_WARPS, 0, st, (const __nv_bfloat16*)X, (const __nv_bfloat16*)W1, M, H, K, ldx, ldw1, out);
+  auto launch = [&](auto kern, int warps) {
+    launch_after(kern, grid, 32 * warps, 0, st, (const __nv_bfloat16*)X, (const __nv_bfloat16*)W1, M, H, K, ldx, ldw1, out);
   };
-  const bool deep = grid <= (unsigned)num_sms && K >= 2048;
-  if (M <= 8) deep ? launch(gemm_rows_gated_kernel<1, 4, 1>) : launch(gemm_rows_gated_kernel<1, 3, 2>);
-  else if (M <= 16) launch(gemm_rows_gated_kernel<2, 3, 2>);
-  else deep ? launch(gemm_rows_gated_kernel<4, 4, 1>) : launch(gemm_rows_gated_kernel<4, 3, 2>);
+  // Blocks of eight warps with four steps under way, two or three to an SM (three have 80 registers a thread, which pays with more than eight rows only where
+  // there are as many blocks); sixteen warps where an SM has one block.  Against the plain product's blocks (sixteen warps, three steps, two to an SM), us: 1 x
+  // 4096 x 14336 42.7 -> 37.0, 8 x 4096 x 14336 44.2 -> 38.0, 1 x 2048 x 8192 16.0 -> 12.4, 8 x 1024 x 4096 6.4 -> 4.9, 16 x 1024 x 2816 6.5 -> 4.4, 32 x 512 x
+  // 2048 5.7 -> 3.9: a block of half the length waits half as long for its own end.  In 385 sizes 2 to 4 % from the best of six such forms.
+  const bool two = grid <= 2u * num_sms;
+  if (M <= 8) grid <= (unsigned)num_sms ? launch(gemm_rows_gated_kernel<1, 16, 1>, 16) : launch(gemm_rows_gated_kernel<1, 8, 2>, 8);
+  else if (M <= 16) two ? launch(gemm_rows_gated_kernel<2, 8, 2>, 8) : launch(gemm_rows_gated_kernel<2, 8, 3>, 8);
+  else two ? launch(gemm_rows_gated_kernel<4, 8, 2>, 8) : launch(gemm_rows_gated_kernel<4, 8, 3>, 8);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
