@@ -515,6 +515,41 @@ def test_decoding_in_a_graph():
         g.reset()
 
 
+@pytest.mark.parametrize("M,D,H", [(1, 1024, 4096), (8, 2048, 1408), (16, 512, 2816), (20, 512, 1024), (4, 4096, 512)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_weights_that_are_written_just_before(M, D, H, graph):
+    """A few rows: the second product's weights are read while the first product runs, but never before what wrote them has ended."""
+    x, w1, w3, w2, _ = _gated(M, D, H, D, seed=5)
+    source, one = w2.float(), torch.ones((), device="cuda")
+    kept = w2.clone()
+
+    def calls():
+        out = []
+        for i in range(12):
+            one.neg_()
+            if i % 2:
+                out.append(K.gated_ffn(x, w1, w3, ops.dtype_cast(source * one, BF)))  # (by a kernel of the framework's own)
+            else:
+                torch.mul(kept, one.to(BF), out=w2)
+                out.append(K.gated_ffn(x, w1, w3, w2))
+        return out
+
+    want = K.gated_ffn(x, w1, w3, kept)
+    torch.cuda.synchronize()
+    if graph:
+        g = torch.cuda.CUDAGraph()
+        calls()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            got = calls()
+        for _ in range(3):
+            g.replay()
+    else:
+        got = calls()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want if i % 2 else -want), i
+
+
 def test_rows_do_not_depend_on_each_other():
     """A row of a batch is the row by itself where both go to the same kernel, and as near as the products' sums elsewhere."""
     x, w1, w3, w2, _ = _gated(1030, 256, 520, 256, seed=8)
