@@ -78,23 +78,24 @@ struct MxCoder {
   }
 };
 
-// Codes of one block to values: with 2^(n+1) added, a code is the lowest byte (or two) of 2^23 + (code + 2^(n+1)) as fp32; one permutation, and a multiplication
-// by the power of two that takes 2^23 + 2^(n+1) times it off again, exactly.
+// Codes of one block to values: with 2^(n+1) added, a code is the lowest byte (or two) of 2^23 + (code + 2^(n+1)) as fp32; one permutation, a subtraction and a
+// multiplication by the power of two, both exact.  (In one step, with 2^23 + 2^(n+1) times the power of two taken off, that product would be infinite from e = 111 on,
+// or 119.)
 template <int BITS>
 struct MxReader {
-  float m, off;
+  static constexpr float BIAS = 8388608.f + (1 << (BITS - 1));
+  float m;
   MxReader() = default;
-  __device__ __forceinline__ explicit MxReader(uint32_t byte)
-      : m(mx_unit(byte, (int)byte + 2 - BITS, 0x7fc00000u)), off(-(8388608.f + (1 << (BITS - 1))) * m) {}
+  __device__ __forceinline__ explicit MxReader(uint32_t byte) : m(mx_unit(byte, (int)byte + 2 - BITS, 0x7fc00000u)) {}
   __device__ __forceinline__ void four(uint32_t codes, float* f) const {  // (8 bits)
     const uint32_t u = codes ^ 0x80808080u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = fmaf(mx_bits(__byte_perm(u, 0x4b000000u, 0x7440 | i)), m, off);
+    for (int i = 0; i < 4; ++i) f[i] = (mx_bits(__byte_perm(u, 0x4b000000u, 0x7440 | i)) - BIAS) * m;
   }
   __device__ __forceinline__ void two(uint32_t codes, float* f) const {  // (16 bits)
     const uint32_t u = codes ^ 0x80008000u;
-    f[0] = fmaf(mx_bits(__byte_perm(u, 0x4b000000u, 0x7410)), m, off);
-    f[1] = fmaf(mx_bits(__byte_perm(u, 0x4b000000u, 0x7432)), m, off);
+    f[0] = (mx_bits(__byte_perm(u, 0x4b000000u, 0x7410)) - BIAS) * m;
+    f[1] = (mx_bits(__byte_perm(u, 0x4b000000u, 0x7432)) - BIAS) * m;
   }
 };
 

@@ -96,6 +96,26 @@ def test_mx8_extremes():
     assert torch.equal(codes.cpu(), want[0]) and torch.equal(scales.cpu(), want[1])
 
 
+@pytest.mark.parametrize("k", [1, 31, 223, 225, 231, 449, 457, 900, 1003])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_mx8_of_rows_that_begin_anywhere(k, dtype):
+    """Every way for a row to begin, blocks of very different sizes, of zeros, at the clamp, and with values that are not numbers."""
+    g = _gen(k)
+    x = _randn(37, k, gen=g, dtype=F32) * torch.exp2(torch.randint(-90, 90, (37, k), device="cuda", generator=g).float().div(16).floor().mul(16))
+    draw = torch.rand(37, k, device="cuda", generator=g)
+    x = torch.where(draw < 0.01, 0.0, torch.where(draw < 0.02, 255.75 / 256 * torch.exp2(torch.log2(x.abs()).ceil()), x))
+    x[3::7] = 0.0
+    for i, v in enumerate((math.nan, math.inf, -math.inf, 3e38, -1e-40)):
+        x[5 * i + 2, (i * 97) % k] = v
+    x = x.to(dtype)
+    codes, scales = K.mx8_quantize(x)
+    want = K.mx8_quantize(x.cpu())
+    assert torch.equal(codes.cpu(), want[0]) and torch.equal(scales.cpu(), want[1])
+    for to in (BF, F32):
+        a, b = K.mx8_dequantize(codes, scales, to).cpu(), K.mx8_dequantize(*want, to)
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
 def test_mx8_of_strided_and_shifted_operands():
     base = _randn(65, 130, gen=_gen(2), dtype=F32)
     for x in (base.t(), base[:, 1:], base[1:, 2:66], base[::2], base.flatten()[3:].view(-1)[:8192].view(64, 128)):
@@ -292,6 +312,28 @@ def test_gated_dgrad(M, N, H, bits):
     _close(dab[:, 0], da, tol)
     _close(dab[:, 1], db, tol)
     _close(h, hd.detach(), HALF_STEP[BF] + 2.0**-18)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("M,H", [(5, 64), (5, 63), (300, 2056)])
+def test_gated_dgrad_of_values_near_the_largest(M, H, bits):
+    """The codes' values are exact up to the end of fp32's range."""
+    g = _gen(M + H)
+    a, b = (_randn(M, H, gen=g, dtype=F32, scale=s).clamp(-2e38, 2e38) for s in (1.0, 1e38))
+    w2, dy = _randn(64, H, gen=g, scale=0.125), _randn(M, 64, gen=g, scale=1e-33)
+    ab, scales = FFN._quantize(torch.stack((a, b), 1), bits)
+    dab, h = ops.gated_dgrad(dy, w2, ab, scales, 0)
+    a, b = (t.clone().requires_grad_() for t in _kept(ab, scales).unbind(1))
+    hd = F.silu(a) * b
+    da, db = torch.autograd.grad(hd, (a, b), dy.double() @ w2.double())
+    tol = HALF_STEP[BF] + 32 * math.sqrt(64) * 2.0**-24
+    _close(dab[:, 0], da, tol)
+    _close(dab[:, 1].double() * 2.0**110, db * 2.0**110, tol)  # (away from the 1e-30 of _close)
+    # silu(a) b passes the largest bf16 number, 3.39e38, for some: with |b| <= 2e38 wherever silu(a) > 1.7.  Those are infinities; next to it either is right.
+    hd, top = hd.detach(), torch.finfo(BF).max
+    over, below = hd.abs() > top * (1 + 2.0**-8), hd.abs() < top * (1 - 2.0**-8)
+    assert torch.equal(h[over].double(), math.inf * hd[over].sign())
+    _close(torch.where(below, h, 0), torch.where(below, hd, 0), HALF_STEP[BF] + 2.0**-18)
 
 
 @pytest.mark.parametrize("M,D,H", FORMS)
