@@ -530,7 +530,7 @@ Tensor mx4_matmul(DispatchKeySet ks, const Tensor& x, const Tensor& w, bool tran
 // ---------------------------------------------------------------------------------------------- the feed-forward block
 using Five = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
 using AddNormSig = Triple(const Tensor&, const Tensor&, const Tensor&, double);
-using AddNormBwdSig = Pair(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&);
+using AddNormBwdSig = Pair(const Tensor&, const c10::optional<Tensor>&, const Tensor&, const Tensor&, const Tensor&);
 using AddNorm8Sig = Five(const Tensor&, const c10::optional<Tensor>&, const Tensor&, double, bool);
 using Mx8ValuesSig = Tensor(const Tensor&, const Tensor&, ScalarType);
 using GatedDgradSig = Pair(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t);
@@ -550,7 +550,7 @@ const Op<GatedFfnSig>& op_gated_ffn() { APB_OP(o, "gated_ffn", GatedFfnSig); ret
 Pair add_norm_gradients(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& w, const Tensor& rstd) {
   at::AutoDispatchBelowAutograd guard;  // (nothing is recorded here; without it every operator goes through the boxed kernel of those without a formula)
   if (!dy.defined()) return {dh, at::zeros_like(w)};  // (itself: the engine copies a gradient that someone else holds, and does not see that of an alias)
-  return dh.defined() ? op_add_norm_bwd()(dy, dh, h, w, rstd) : op_rms_bwd()(dy, h, w, rstd);
+  return op_add_norm_bwd()(dy, dh.defined() ? c10::optional<Tensor>(dh) : c10::nullopt, h, w, rstd);
 }
 struct AddNorm : torch::autograd::Function<AddNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& res, const Tensor& w, double eps, Keys k) {

@@ -50,17 +50,20 @@ Five add_rms_norm_fp8(const Tensor& x, const c10::optional<Tensor>& residual, co
   count(a.rows > 0);
   return {y, h, rstd, q, scale};
 }
-Two add_rms_norm_bwd(const Tensor& dy_, const Tensor& dh_, const Tensor& h_, const Tensor& weight, const Tensor& rstd_) {
+// Without ``dh`` (h is not used further on, or there is no residual) it is the plain norm's gradient: that kernel's, two operands instead of three, for the widths it
+// takes (those of its forward pass); this one's for the others.
+Two add_rms_norm_bwd(const Tensor& dy_, const c10::optional<Tensor>& dh_, const Tensor& h_, const Tensor& weight, const Tensor& rstd_) {
   c10::cuda::CUDAGuard g(h_.device());
   const NormArgs a("add_rms_norm_bwd", h_, c10::nullopt, weight);
-  for (const Tensor* t : {&dy_, &dh_})
+  for (const Tensor* t : {&dy_, dh_.has_value() ? &*dh_ : &dy_})
     TORCH_CHECK(t->sizes() == h_.sizes() && t->scalar_type() == h_.scalar_type() && t->device() == h_.device(), "add_rms_norm_bwd: gradients like h");
   TORCH_CHECK(rstd_.scalar_type() == at::kFloat && rstd_.numel() == a.rows && rstd_.device() == h_.device(), "add_rms_norm_bwd: rstd fp32, one a row");
   Tensor dx = at::empty_like(a.x), dw = at::empty({a.D}, a.x.options());
   if (a.rows == 0) return {dx, dw.zero_().to(weight.scalar_type())};
-  Tensor dy = dense(dy_), dh = dense(dh_), rstd = rstd_.contiguous();
+  if (!dh_.has_value() && a.D % 8 == 0 && a.D <= 16384) return op_rms_norm_bwd(dy_, h_, weight, rstd_);
+  Tensor dy = dense(dy_), dh = dh_.has_value() ? dense(*dh_) : Tensor(), rstd = rstd_.contiguous();
   Tensor part = at::empty({(int64_t)apb_add_rms_norm_bwd_workspace(a.rows, (int)a.D, is_bf16(a.x), num_sms())}, rstd.options());  // partial sums of dw
-  check(apb_add_rms_norm_bwd(dy.data_ptr(), dh.data_ptr(), a.x.data_ptr(), a.w.data_ptr(), rstd.data_ptr<float>(), dx.data_ptr(), dw.data_ptr(),
+  check(apb_add_rms_norm_bwd(dy.data_ptr(), dh.defined() ? dh.data_ptr() : nullptr, a.x.data_ptr(), a.w.data_ptr(), rstd.data_ptr<float>(), dx.data_ptr(), dw.data_ptr(),
                              part.data_ptr<float>(), a.rows, (int)a.D, is_bf16(a.x), num_sms(), stream()),
         "apb_add_rms_norm_bwd");
   count(2);
@@ -267,7 +270,7 @@ using Three = std::tuple<Tensor, Tensor, Tensor>;
 Three op_add_rms_norm(const Tensor& x, const Tensor& r, const Tensor& w, double eps) {
   return ours(ADD_RMS_NORM) ? add_rms_norm(x, r, w, eps) : in_python<Three>(ADD_RMS_NORM, x, r, w, eps);
 }
-Two op_add_rms_norm_bwd(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& w, const Tensor& rstd) {
+Two op_add_rms_norm_bwd(const Tensor& dy, const c10::optional<Tensor>& dh, const Tensor& h, const Tensor& w, const Tensor& rstd) {
   return ours(ADD_RMS_NORM_BWD) ? add_rms_norm_bwd(dy, dh, h, w, rstd) : in_python<Two>(ADD_RMS_NORM_BWD, dy, dh, h, w, rstd);
 }
 Five op_add_rms_norm_fp8(const Tensor& x, const c10::optional<Tensor>& r, const Tensor& w, double eps, bool keep) {

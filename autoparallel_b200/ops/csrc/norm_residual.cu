@@ -2,7 +2,7 @@
 //
 //   forward    h = round(x + residual)    r = 1 / sqrt(mean(h^2) + eps)    y = h r w
 //              in 8 bits: q = e4m3(y / s), s = max |y| of the row / 448 (1 where that maximum is below 2^-100)
-//   backward   with n = h r and g = dy w:  dx = dresidual = dh + r (g - n mean(g n))    dw = sum over rows of dy n
+//   backward   with n = h r and g = dy w:  dx = dresidual = dh + r (g - n mean(g n))    dw = sum over rows of dy n    (dh: null where h is not used)
 //
 // Both are bound by memory: x and residual are read once, h and y (or q) written once; backward h, dy and dh are read and dx is written.  A row stays in
 // registers from its load to the last result.  The sum of squares is that of the plain norm's kernel (elementwise.cu), thread by thread, so that y has the bits
@@ -254,11 +254,13 @@ __global__ void __launch_bounds__(1024) add_rms_norm_bwd_kernel(const T* dy, con
         Vec8<T> hv, gv, ev;
         at.load(hv, h, c);
         at.load(gv, dy, c);
-        at.load(ev, dh, c);
-        float hf[8], gf[8], ef[8], wf[8];
+        float hf[8], gf[8], ef[8] = {}, wf[8];
+        if (dh != nullptr) {
+          at.load(ev, dh, c);
+          ev.to_float(ef);
+        }
         hv.to_float(hf);
         gv.to_float(gf);
-        ev.to_float(ef);
         at.weight(wf, w, c);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ef[i] += fmaf(gf[i], r * wf[i], -hf[i] * k);
@@ -315,11 +317,11 @@ add_rms_norm_bwd_bulk_kernel(const T* dy, const T* dh, const T* h, const T* w, c
     const long long from = at.base - at.lead;
     const uint32_t bytes = (uint32_t)max(copied(at), 0) * (uint32_t)sizeof(T);
     uint8_t* to = smem + 3 * st * slot;
-    mbar_expect_tx(&bars[st], 3u * bytes);
+    mbar_expect_tx(&bars[st], (dh != nullptr ? 3u : 2u) * bytes);
     if (bytes == 0) return;
     bulk_load(to, h + from, bytes, &bars[st]);
     bulk_load(to + slot, dy + from, bytes, &bars[st]);
-    bulk_load(to + 2 * slot, dh + from, bytes, &bars[st]);
+    if (dh != nullptr) bulk_load(to + 2 * slot, dh + from, bytes, &bars[st]);
   };
   if (threadIdx.x == 0)
     for (int it = 0; it < ST - 1; ++it) issue(it);
@@ -406,11 +408,13 @@ add_rms_norm_bwd_bulk_kernel(const T* dy, const T* dh, const T* h, const T* w, c
         Vec8<T> hv, gv, ev;
         read(hv, 0, h, col[j]);
         read(gv, 1, dy, col[j]);
-        read(ev, 2, dh, col[j]);
-        float hf[8], gf[8], ef[8], wf[8];
+        float hf[8], gf[8], ef[8] = {}, wf[8];
+        if (dh != nullptr) {
+          read(ev, 2, dh, col[j]);
+          ev.to_float(ef);
+        }
         hv.to_float(hf);
         gv.to_float(gf);
-        ev.to_float(ef);
         weight(wf, j);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ef[i] += fmaf(gf[i], r * wf[i], -hf[i] * k);

@@ -44,7 +44,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from .library import _ag, _make_cuda_entry, _rms_norm_ref, lib, ops, reference_impls
+from .library import _ag, _make_cuda_entry, _rms_norm_bwd_ref, _rms_norm_ref, lib, ops, reference_impls
 
 ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 CHECKPOINTS = {"full": 16, "mx8": 8}
@@ -54,7 +54,7 @@ F8 = torch.float8_e4m3fn
 F8_MAX = 448.0
 
 lib.define("add_rms_norm(Tensor x, Tensor residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)")
-lib.define("add_rms_norm_bwd(Tensor dy, Tensor dh, Tensor h, Tensor weight, Tensor rstd) -> (Tensor, Tensor)")
+lib.define("add_rms_norm_bwd(Tensor dy, Tensor? dh, Tensor h, Tensor weight, Tensor rstd) -> (Tensor, Tensor)")
 lib.define("add_rms_norm_fp8(Tensor x, Tensor? residual, Tensor weight, float eps, bool keep) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
 lib.define("mx8_quantize(Tensor x) -> (Tensor, Tensor)")
 lib.define("mx8_dequantize(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor")
@@ -77,6 +77,8 @@ def _add_rms_norm(x, residual, weight, eps):
 
 
 def _add_rms_norm_bwd(dy, dh, h, weight, rstd):
+    if dh is None:
+        return _rms_norm_bwd_ref(dy, h, weight, rstd)
     n = h.float() * rstd.unsqueeze(-1)
     g = dy.float() * weight.float()
     dx = dh.float() + rstd.unsqueeze(-1) * (g - n * (g * n).mean(-1, keepdim=True))
@@ -239,12 +241,8 @@ def _norm8_setup(ctx, inputs, output):
 
 
 def _norm8_bwd(ctx, dy, dh, _drstd, _dq, _dscale):
-    h, weight, rstd = ctx.saved_tensors
-    if not ctx.residual:
-        dx, dw = ops.rms_norm_bwd(dy, h, weight, rstd)
-        return dx, None, dw, None, None
-    dx, dw = ops.add_rms_norm_bwd(dy, dh, h, weight, rstd)
-    return dx, dx, dw, None, None
+    dx, dw = ops.add_rms_norm_bwd(dy, dh if ctx.residual else None, *ctx.saved_tensors)
+    return dx, dx if ctx.residual else None, dw, None, None
 
 
 _ag("add_rms_norm_fp8", _norm8_bwd, _norm8_setup)

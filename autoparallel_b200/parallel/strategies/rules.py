@@ -363,8 +363,9 @@ def _add_rms_norm(ctx):
 
 @register_rule(apb.add_rms_norm_bwd.default)
 def _add_rms_norm_bwd(ctx):
-    # (dx, dw, dy, dh, h, weight, rstd)
-    return expand_rows(ctx, [(S(i), P, S(i), S(i), S(i), R, S(i)) for i in _lead_dims(ctx.in_vals[2])])
+    # (dx, dw, dy[, dh], h, weight, rstd)
+    n = len(ctx.in_vals) - 2
+    return expand_rows(ctx, [(S(i), P) + (S(i),) * n + (R, S(i)) for i in _lead_dims(ctx.in_vals[0])])
 
 
 @register_rule(apb.add_rms_norm_fp8.default)

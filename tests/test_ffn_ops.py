@@ -521,3 +521,22 @@ def test_registration(name):
             "mx8_dequantize": (codes, scales, torch.float32), "gated_ffn8": (x, w1, w3, w2, 1, 8), "gated_ffn16": (x, w1, w3, w2, 0, 16)}[name]
     op = getattr(ops, name.rstrip("0123456789") if name.startswith("gated") else name).default
     torch.library.opcheck(op, args, test_utils=("test_schema", "test_autograd_registration", "test_faketensor"))
+
+
+def test_norm_gradient_without_one_of_the_sum(mesh_1d):
+    """``add_rms_norm_bwd`` without ``dh``: the plain norm's gradient, its shapes and its ways to be split."""
+    from torch.distributed.tensor.placement_types import Partial, Replicate, Shard
+
+    g = _gen(12)
+    for dtype in (torch.bfloat16, torch.float32):
+        for shape in ((4, 1), (2, 3, 37), (5, 64)):
+            h, dy = (_randn(*shape, dtype=dtype, gen=g) for _ in range(2))
+            w = _randn(shape[-1], dtype=dtype, gen=g)
+            rstd = ops.rms_norm(h, w, 1e-5)[1]
+            got, want = ops.add_rms_norm_bwd(dy, None, h, w, rstd), ops.add_rms_norm_bwd(dy, torch.zeros_like(h), h, w, rstd)
+            assert all(torch.allclose(a.float(), b.float(), rtol=2 * EPS[dtype], atol=1e-5) for a, b in zip(got, want))
+            meta = ops.add_rms_norm_bwd(dy.to("meta"), None, h.to("meta"), w.to("meta"), rstd.to("meta"))
+            assert [(a.shape, a.dtype) for a in meta] == [(a.shape, a.dtype) for a in got]
+    S, R, P = Shard, Replicate(), Partial()
+    x = torch.randn(8, 16, 64)
+    assert _rows(mesh_1d, "add_rms_norm_bwd", x, None, x, x[0, 0], x[..., 0]) == {(R,) * 6, *((S(i), P, S(i), S(i), R, S(i)) for i in (0, 1))}
