@@ -3,8 +3,9 @@
 //
 //   e = max(floor(log2 of the largest magnitude), n - 126)     code = v 2^(n-e), rounded to even, within +-(2^(n+1) - 1)     value = code 2^(e-n)
 //
-// The scale byte is e + 127; a block with an infinity or a NaN has the byte 255 and reads as NaN.  Units are never below 2^-126, so every value is a normal fp32
-// number, and with 8 bits exact in bf16: products of the values on the tensor cores lose nothing to the format.
+// The scale byte is e + 127; a block with an infinity or a NaN has the byte 255 and reads as NaN.  The format's e goes down to -127; what is written here stops where
+// the unit is 2^-126, so every value is a normal fp32 number, and with 8 bits exact in bf16: products of the values on the tensor cores lose nothing to the format.
+// What is read may come from elsewhere and have any byte; 8-bit values below 2^-126 are multiples of 2^-133, exact in both types too.
 #pragma once
 #include <stdint.h>
 
@@ -14,8 +15,10 @@ constexpr int MX_BLOCK = 32, MX_NAN = 255;
 template <int BITS>
 constexpr int MX_LOWEST = BITS - 1;  // the scale byte of the smallest e
 
-// 2^(field - 127), or the bits ``broken`` for a block that holds an infinity or a NaN.
-__device__ __forceinline__ float mx_unit(uint32_t byte, int field, uint32_t broken) { return __uint_as_float(byte == MX_NAN ? broken : (uint32_t)field << 23); }
+// 2^(field - 127), field from -22 on, or the bits ``broken`` for a block that holds an infinity or a NaN.
+__device__ __forceinline__ float mx_unit(uint32_t byte, int field, uint32_t broken) {
+  return __uint_as_float(byte == MX_NAN ? broken : field > 0 ? (uint32_t)field << 23 : 0x400000u >> -field);
+}
 __device__ __forceinline__ float mx_bits(uint32_t v) { return __uint_as_float(v); }
 
 // ``top``: the largest of the magnitudes' bits, in which a NaN is larger than everything.

@@ -32,7 +32,8 @@ gradients take.
     e = max(floor(log2 of the largest magnitude), -120)     code = v 2^(6-e), rounded to even, within +-127     value = code 2^(e-6)
 
 codes int8 of the values' shape, scales uint8 [.., ceil(K / 32)]: e + 127, and 255 for a block with an infinity or a NaN, which reads as
-NaN.  A value is off by at most 2^(e-7), but 2^(e-6) where it is the block's largest and rounds to 128; it is exact in bf16.  The 16-bit
+NaN.  (The format's e goes down to -127.  What is written here stops at -120, where the unit is the smallest normal fp32 number; what is read
+may have any scale.)  A value is off by at most 2^(e-7), but 2^(e-6) where it is the block's largest and rounds to 128; it is exact in bf16.  The 16-bit
 codes are the same with 14 for 6, -112 for -120 and 32767 for 127: in as many bits as bf16, off by 2^-15 of the block's largest value and
 not by 2^-9 of each.
 
@@ -110,7 +111,8 @@ def _quantize(x, bits):
 
 def _dequantize(codes, scales, dtype):
     s = scales.int()
-    unit = ((s + 2 - 8 * codes.element_size()).clamp(min=1) << 23).to(torch.int32).view(torch.float32).masked_fill(s == 255, float("nan"))
+    field = s + 2 - 8 * codes.element_size()  # (of the unit, 2^(field - 127); scales from elsewhere may go below 1)
+    unit = torch.where(field > 0, field << 23, 0x400000 >> (-field).clamp(0, 31)).to(torch.int32).view(torch.float32).masked_fill(s == 255, float("nan"))
     return (codes.float() * unit.repeat_interleave(BLOCK, -1)[..., : codes.shape[-1]]).to(dtype)
 
 

@@ -75,3 +75,18 @@ def test_gradients_where_only_the_norm_is_used(D, form, dtype):
             y = (K.add_rms_norm if form == "norm" else K.add_rms_norm_fp8)(*leaves)[0]
         got = torch.autograd.grad(y, leaves, dy)
         _check_norm_gradients(got, _norm_gradients(h, w, dy, None, 1e-5), dtype, dtype)
+
+
+# ------------------------------------------------------------------------------------ 8-bit checkpoints
+@pytest.mark.parametrize("k", [256, 264, 257, 1003])
+def test_mx8_values_of_every_scale(k):
+    """Codes from elsewhere may come with any scale byte of the format, and with the code -128."""
+    codes = (torch.arange(k, device="cuda") % 256 - 128).to(torch.int8).expand(256, k).contiguous()
+    scales = torch.arange(256, device="cuda").to(torch.uint8).unsqueeze(1).expand(256, -(-k // 32)).contiguous()
+    want = codes.double() * torch.exp2(scales[:, :1].double() - 133)
+    want[255] = math.nan
+    for dtype in (BF, F32):  # (exact in both but for -2^128)
+        got = K.mx8_dequantize(codes, scales, dtype)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got[:255].double(), want[:255].masked_fill(want[:255] <= -(2.0**128), -math.inf))
+        assert torch.equal(K.mx8_dequantize(codes.cpu(), scales.cpu(), dtype).nan_to_num(nan=3.0), got.cpu().nan_to_num(nan=3.0))

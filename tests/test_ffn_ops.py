@@ -540,3 +540,14 @@ def test_norm_gradient_without_one_of_the_sum(mesh_1d):
     S, R, P = Shard, Replicate(), Partial()
     x = torch.randn(8, 16, 64)
     assert _rows(mesh_1d, "add_rms_norm_bwd", x, None, x, x[0, 0], x[..., 0]) == {(R,) * 6, *((S(i), P, S(i), S(i), R, S(i)) for i in (0, 1))}
+
+
+@pytest.mark.parametrize("k", [256, 257])
+def test_mx8_values_of_every_scale(k):
+    """Codes from elsewhere may come with any scale byte of the format, and with the code -128."""
+    codes = (torch.arange(k) % 256 - 128).to(torch.int8).expand(256, k)
+    scales = torch.arange(256).to(torch.uint8).unsqueeze(1).expand(256, -(-k // 32))
+    want = codes.double() * torch.exp2(scales[:, :1].double() - 133)
+    for dtype in (torch.bfloat16, torch.float32):  # (exact in both but for -2^128)
+        got = K.mx8_dequantize(codes, scales, dtype)
+        assert got[255].isnan().all() and torch.equal(got[:255].double(), want[:255].masked_fill(want[:255] <= -(2.0**128), -math.inf))
