@@ -40,7 +40,7 @@ class LlamaConfig:
     depth_init: bool = False
     #: the feed-forward block as one operator (``ops.gated_ffn``): both projections, the activation and their product in one kernel
     fused_ffn: bool = False
-    #: what ``fused_ffn`` keeps for the backward pass: "full" (in the type of the activations) or "mx8" (in 8 bits)
+    #: what ``fused_ffn`` keeps for the backward pass: "full" (in as many bits as the activations have), "mx16" or "mx8" (in 8 bits); see ``ops.gated_ffn``
     ffn_checkpoint: str = "full"
     #: the residual's addition and the norm before the feed-forward block in one kernel (``ops.add_rms_norm``)
     fused_norm: bool = False

@@ -91,8 +91,8 @@ int apb_mx8_quantize(const void* x, void* codes, void* scales, long long R, long
 int apb_mx8_dequantize(const void* codes, const void* scales, void* y, long long R, long long K, int is_bf16, cudaStream_t st);
 int apb_gated_act(const float* ab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st);
 int apb_gated_act_bwd(const float* dh, const float* ab, void* dab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st);
-int apb_mx16_quantize(const float* x, void* codes, void* scales, long long R, int K, cudaStream_t st);
-int apb_mx16_dequantize(const void* codes, const void* scales, float* y, long long R, int K, cudaStream_t st);
+int apb_mx16_quantize(const float* x, void* codes, void* scales, long long R, int K, int bits, cudaStream_t st);
+int apb_mx16_dequantize(const void* codes, const void* scales, float* y, long long R, int K, int bits, cudaStream_t st);
 int apb_gemm_get_reserved_sms();
 int apb_gemm_rows_takes(int M, int N, int K, int num_sms);
 int apb_gemm_rows_behind(const void* X, const void* W, void* C, int M, int N, int K, long long ldx, long long ldw, long long ldc, int out_fp32, int num_sms,

@@ -83,8 +83,12 @@ Two mx8_quantize(const Tensor& x_) {
 void mx_check(const Tensor& codes, const Tensor& scales, at::ScalarType type, const char* what) {
   TORCH_CHECK(codes.scalar_type() == type && scales.scalar_type() == at::kByte && codes.dim() >= 1 && scales.device() == codes.device() &&
                   scales.sizes() == at::IntArrayRef(with_last(lead_of(codes), {mx_blocks(codes.size(-1))})),
-              what, ": ", type == at::kChar ? "int8" : "int16", " codes [.., K] and uint8 scales [.., ceil(K / 32)]");
+              what, ": ", type == at::kChar ? "int8" : type == at::kShort ? "int16" : "fp16", " codes [.., K] and uint8 scales [.., ceil(K / 32)]");
 }
+// What is kept of both projections: the codes' type for ``bits`` (8 or 16: whole numbers, 11: fp16 numbers), and back.
+constexpr int64_t HALF_BITS = 11;
+at::ScalarType code_type(int64_t bits) { return bits == 8 ? at::kChar : bits == 16 ? at::kShort : at::kHalf; }
+int code_bits(at::ScalarType type) { return type == at::kChar ? 8 : type == at::kShort ? 16 : type == at::kHalf ? (int)HALF_BITS : 0; }
 Tensor mx8_dequantize(const Tensor& codes_, const Tensor& scales_, at::ScalarType dtype) {
   c10::cuda::CUDAGuard g(codes_.device());
   mx_check(codes_, scales_, at::kChar, "mx8_dequantize");
@@ -127,13 +131,13 @@ std::tuple<Tensor, Tensor, Tensor> gated_mm(const Tensor& x, const Tensor& w1, c
   gated_check(x, {&w1, &w3}, "gated_mm");
   const int64_t D = x.size(-1), H = w1.size(0), M = rows_of(x, 1);
   TORCH_CHECK(w1.size(1) == D && w3.sizes() == w1.sizes(), "gated_mm: x [.., D], w1 and w3 [H, D]");
-  TORCH_CHECK(act >= 0 && act <= 2 && (bits == 0 || bits == 8 || bits == 16), "gated_mm: act 0 to 2, bits 0, 8 or 16");
+  TORCH_CHECK(act >= 0 && act <= 2 && (bits == 0 || bits == 8 || bits == 16 || bits == HALF_BITS), "gated_mm: act 0 to 2, bits 0, 8 or 16, or 11 for fp16 numbers");
   const auto lead = lead_of(x);
   const auto u8 = x.options().dtype(at::kByte);
   Tensor h = at::empty(with_last(lead, {H}), x.options()), ab = at::empty({0}, x.options()), scales = at::empty({0}, u8);
   if (gated_form({&x}, {D, H}) && M > 0 && M <= 0x7fffffff) {
     if (bits) {
-      ab = at::empty(with_last(lead, {2, H}), x.options().dtype(bits == 8 ? at::kChar : at::kShort));
+      ab = at::empty(with_last(lead, {2, H}), x.options().dtype(code_type(bits)));
       scales = at::empty(with_last(lead, {2, mx_blocks(H)}), u8);
     }
     Tensor x2 = as2d(x), a = as2d(w1), b = as2d(w3);
@@ -147,17 +151,17 @@ std::tuple<Tensor, Tensor, Tensor> gated_mm(const Tensor& x, const Tensor& w1, c
   Tensor both = at::stack({product32(x, w1, true), product32(x, w3, true)}, 1);  // [M, 2, H]
   check(apb_gated_act(both.data_ptr<float>(), h.data_ptr(), M, (int)H, (int)act, is_bf16(x), stream()), "apb_gated_act");
   count(both.numel() > 0);
-  if (bits == 16 && x.scalar_type() == at::kFloat) {
-    ab = both.view(with_last(lead, {2, H}));
-  } else if (bits == 16) {
-    ab = at::empty(with_last(lead, {2, H}), x.options().dtype(at::kShort));
-    scales = at::empty(with_last(lead, {2, mx_blocks(H)}), u8);
-    check(apb_mx16_quantize(both.data_ptr<float>(), ab.data_ptr(), scales.data_ptr(), 2 * M, (int)H, stream()), "apb_mx16_quantize");
-    count(both.numel() > 0);
-  } else if (bits == 8) {
+  if (bits == 8) {
     auto [c, s] = mx8_quantize(both);
     ab = c.view(with_last(lead, {2, H}));
     scales = s.view(with_last(lead, {2, mx_blocks(H)}));
+  } else if (bits && x.scalar_type() == at::kFloat) {
+    ab = both.view(with_last(lead, {2, H}));
+  } else if (bits) {
+    ab = at::empty(with_last(lead, {2, H}), x.options().dtype(code_type(bits)));
+    scales = at::empty(with_last(lead, {2, mx_blocks(H)}), u8);
+    check(apb_mx16_quantize(both.data_ptr<float>(), ab.data_ptr(), scales.data_ptr(), 2 * M, (int)H, (int)bits, stream()), "apb_mx16_quantize");
+    count(both.numel() > 0);
   }
   return {h, ab, scales};
 }
@@ -165,29 +169,30 @@ std::tuple<Tensor, Tensor, Tensor> gated_mm(const Tensor& x, const Tensor& w1, c
 Two gated_dgrad(const Tensor& dy, const Tensor& w2, const Tensor& ab_, const Tensor& scales_, int64_t act) {
   c10::cuda::CUDAGuard g(dy.device());
   gated_check(dy, {&w2}, "gated_dgrad");
-  const bool eight = ab_.scalar_type() == at::kChar, codes = dy.scalar_type() == at::kBFloat16 || eight;
+  const int bits = code_bits(ab_.scalar_type());  // (0: values in fp32)
+  const bool codes = dy.scalar_type() == at::kBFloat16 || bits == 8;
   const int64_t N = dy.size(-1), H = w2.size(1), M = rows_of(dy, 1);
   TORCH_CHECK(w2.size(0) == N && ab_.sizes() == at::IntArrayRef(with_last(lead_of(dy), {2, H})) && ab_.device() == dy.device() &&
-                  (codes || ab_.scalar_type() == at::kFloat),
+                  (codes ? bits != 0 : ab_.scalar_type() == at::kFloat),
               "gated_dgrad: dy [.., N], w2 [N, H], ab [.., 2, H] in 8 bits, or in 16 for bf16 and fp32 for fp32");
-  if (codes) mx_check(ab_, scales_, eight ? at::kChar : at::kShort, "gated_dgrad");
+  if (codes) mx_check(ab_, scales_, ab_.scalar_type(), "gated_dgrad");
   TORCH_CHECK(act >= 0 && act <= 2, "gated_dgrad: act 0 to 2");
   Tensor dab = at::empty(ab_.sizes(), dy.options()), h = at::empty(with_last(lead_of(dy), {H}), dy.options());
   if (gated_form({&dy}, {N, H}) && M > 0 && M <= 0x7fffffff) {
     Tensor a = as2d(dy), b = as2d(w2), ab = dense(ab_), scales = scales_.contiguous();
-    const int err = apb_gemm_gated_grad(a.data_ptr(), b.data_ptr(), ab.data_ptr(), scales.data_ptr(), eight ? 8 : 16, dab.data_ptr(), h.data_ptr(),
+    const int err = apb_gemm_gated_grad(a.data_ptr(), b.data_ptr(), ab.data_ptr(), scales.data_ptr(), bits, dab.data_ptr(), h.data_ptr(),
                                         (int)M, (int)H, (int)N, a.stride(0), b.stride(0), (int)act, status_word(dy), num_sms(), stream());
     if (err == 0) count();
     if (err == 0) return {dab, h};
     if (err > 0) check(err, "apb_gemm_gated_grad");
   }
   Tensor dh = product32(dy, w2, false), v;
-  if (eight) {
+  if (bits == 8) {
     v = mx8_dequantize(ab_, scales_, at::kFloat);
   } else if (codes) {
     Tensor c = ab_.contiguous(), s = scales_.contiguous();
     v = at::empty(c.sizes(), c.options().dtype(at::kFloat));
-    check(apb_mx16_dequantize(c.data_ptr(), s.data_ptr(), v.data_ptr<float>(), 2 * M, (int)H, stream()), "apb_mx16_dequantize");
+    check(apb_mx16_dequantize(c.data_ptr(), s.data_ptr(), v.data_ptr<float>(), 2 * M, (int)H, bits, stream()), "apb_mx16_dequantize");
     count(v.numel() > 0);
   } else {
     v = ab_.contiguous();

@@ -1,8 +1,10 @@
 // The middle of a gated feed-forward block: h = act(a) * b with a = x w1^T and b = x w3^T, and its derivative, as the ends of two products.
 //
 //   forward    both projections come out of one product, a and b of the same column of h in the same thread; h leaves in bf16, and for the backward
-//              pass a and b, as codes of 8 or 16 bits (mx8.cuh): in as many bits as bf16 they are off by 2^-15 of a block's largest value and not by 2^-9 of
-//              each, and the gradients by 0.0024 and not 0.0034 of their size (both: da, db and the results are rounded to bf16)
+//              pass a and b, as codes of 8 or 16 bits (mx8.cuh).  Two forms of 16: fp16 numbers under the power of two of a block, off by 2^-11 of each value and
+//              not by 2^-8 as bf16 would be, and whole numbers, off by 2^-15 of the block's largest value.  The gradients are off by 0.0024 of their size, not
+//              0.0034 (both: da, db and the results are rounded to bf16); with whole numbers only while the values of a block are within some 150 times of each
+//              other (a column 4096 times the others of its block: their weights' gradients off by 0.058 of their size).
 //   backward   dh = dy w2 stays in fp32; da = dh b act'(a) and db = dh act(a) leave in bf16, and h, made again, for the gradient of w2
 //
 // ab, dab [M, 2, H]: a row of a (da), then the same row of b (db), so that one product makes the gradients of both weights.  The scales of codes are
@@ -119,7 +121,7 @@ template <int BITS>
 __device__ __forceinline__ uint32_t codes32(const uint32_t (&r)[32], uint8_t* stg, int lane) {
   const uint32_t top = mx_top(r), byte = mx_scale_byte<BITS>(top);
   const MxCoder<BITS> coder(byte, top);
-  uint32_t w[BITS];
+  uint32_t w[8 * MX_BYTES<BITS>];
   coder.words(r, w);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -129,7 +131,7 @@ __device__ __forceinline__ uint32_t codes32(const uint32_t (&r)[32], uint8_t* st
   return byte;
 }
 
-// Forward: columns col ... col + ncols - 1 of h from the accumulators at ``ta`` and ``tb``, and codes of BITS bits (0: none); ``stg``: 4096 bytes of the warp's own.
+// Forward: columns col ... col + ncols - 1 of h from the accumulators at ``ta`` and ``tb``, and codes (BITS 0: none); ``stg``: 4096 bytes of the warp's own.
 template <int BITS, typename Release>
 __device__ __forceinline__ void gated_tile(const GatedOut& o, uint8_t* stg, uint32_t ta, uint32_t tb, int row0, int col, int ncols, int M, int H, int lane,
                                            Release release) {
@@ -168,11 +170,11 @@ __device__ __forceinline__ void gated_tile(const GatedOut& o, uint8_t* stg, uint
       uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab);
       stage_store8(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);
       stage_store8(stg + 2048 + 1024, codes + H, 2ll * H, row0, col + c, M, H, lane);
-    } else if constexpr (BITS == 16) {
+    } else if constexpr (BITS != 0) {
       __nv_bfloat16* codes = reinterpret_cast<__nv_bfloat16*>(o.ab);  // (two bytes each)
       stage_store(stg + 2048, codes, 2ll * H, row0, col + c, M, H, lane);
       __syncwarp();
-      sb = codes32<16>(b, stg, lane);
+      sb = codes32<BITS>(b, stg, lane);
       __syncwarp();
       stage_store(stg, codes + H, 2ll * H, row0, col + c, M, H, lane);
     }
@@ -200,7 +202,7 @@ struct AbFetch {
     const int unit = lane & 3, sub = lane >> 2;
     const bool in = col + unit * 8 < H;
     const uint8_t* ab = reinterpret_cast<const uint8_t*>(g.ab);
-    constexpr int SIZE = BITS / 8;
+    constexpr int SIZE = MX_BYTES<BITS>;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = sub + 8 * j;
@@ -318,9 +320,9 @@ __device__ __forceinline__ uint2 codes4(const float (&v)[4], uint32_t& byte) {
   byte = mx_scale_byte<BITS>(top);
   const MxCoder<BITS> coder(byte, top);
   const uint32_t u[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-  uint32_t w[BITS / 8];
+  uint32_t w[MX_BYTES<BITS>];
   coder.words(u, w);
-  return make_uint2(w[0], BITS == 8 ? 0 : w[BITS / 8 - 1]);
+  return make_uint2(w[0], BITS == 8 ? 0 : w[MX_BYTES<BITS> - 1]);
 }
 template <int BITS>
 __device__ __forceinline__ void gated_four(const GatedOut& o, long long row, int col, int H, const float (&a)[4], const float (&b)[4]) {
@@ -343,8 +345,8 @@ __device__ __forceinline__ void gated_four(const GatedOut& o, long long row, int
     uint8_t* codes = reinterpret_cast<uint8_t*>(o.ab) + at;
     *reinterpret_cast<uint32_t*>(codes) = ca.x;
     *reinterpret_cast<uint32_t*>(codes + H) = cb.x;
-  } else if constexpr (BITS == 16) {
-    const uint2 ca = codes4<16>(a, sa), cb = codes4<16>(b, sb);
+  } else if constexpr (BITS != 0) {
+    const uint2 ca = codes4<BITS>(a, sa), cb = codes4<BITS>(b, sb);
     if (!in) return;
     uint16_t* codes = reinterpret_cast<uint16_t*>(o.ab) + at;
     *reinterpret_cast<uint2*>(codes) = ca;
@@ -363,7 +365,7 @@ struct AbFour {
   uint2 a, b;
   uint32_t sa, sb;
   __device__ __forceinline__ void load(const GatedGrad& g, long long row, int col, int H) {
-    const uint8_t* codes = reinterpret_cast<const uint8_t*>(g.ab) + (row * 2 * H + col) * (BITS / 8);
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(g.ab) + (row * 2 * H + col) * MX_BYTES<BITS>;
     if (BITS == 8) {
       a.x = *reinterpret_cast<const uint32_t*>(codes);
       b.x = *reinterpret_cast<const uint32_t*>(codes + H);
@@ -382,7 +384,7 @@ __device__ __forceinline__ void gated_grad_four(const GatedGrad& g, const AbFour
   float a[4], b[4], da[4], db[4], h[4];
   const long long at = row * 2 * H + col;
   const MxReader<BITS> ra(ab.sa), rb(ab.sb);
-  if (BITS == 8) {
+  if constexpr (BITS == 8) {
     ra.four(ab.a.x, a);
     rb.four(ab.b.x, b);
   } else {

@@ -143,14 +143,14 @@ static bool few_rows(int M, int H, int K, int num_sms) {
   return M <= 32 && (apb_gemm_rows_takes(M, 2 * H, K, num_sms) || (M <= 8 && H >= 4096));
 }
 
-// ``bits`` 0, or 8 or 16: the codes ``ab`` [M, 2, H] and ``scales`` [M, 2, ceil(H / 32)] are kept.  Returns 0, -1 (the caller's plain products), > 0: argument or
+// ``bits`` 0, or 8, 16 or MX_HALF: the codes ``ab`` [M, 2, H] and ``scales`` [M, 2, ceil(H / 32)] are kept.  Returns 0, -1 (the caller's plain products), > 0: argument or
 // driver error (nothing launched).
 extern "C" int apb_gemm_gated(const void* x, const void* w1, const void* w3, void* h, void* ab, void* scales, int bits, int M, int H, int K,
                               long long ldx, long long ldw1, long long ldw3, int act, uint32_t* status, int num_sms, cudaStream_t stream) {
   const int no = ext_takes(M, H, K);
   if (no) return no;
   if (off16({x, w1, w3, h, ab}) || ((ldx | ldw1 | ldw3) & 7)) return 3;
-  if (H > 0x3fffffff || (bits != 0 && bits != 8 && bits != 16) || (bits != 0 && (ab == nullptr || scales == nullptr))) return 3;
+  if (H > 0x3fffffff || (bits != 0 && bits != 8 && bits != 16 && bits != MX_HALF) || (bits != 0 && (ab == nullptr || scales == nullptr))) return 3;
   if (bits == 0 && apb_gemm_get_reserved_sms() == 0 && few_rows(M, H, K, num_sms))
     return apb_gemm_rows_gated(x, w1, w3, h, M, H, K, ldx, ldw1, ldw3, act, num_sms, stream);
   auto launch = [&](auto ext) {
@@ -158,19 +158,21 @@ extern "C" int apb_gemm_gated(const void* x, const void* w1, const void* w3, voi
     return launch_ext<false>(Operand{x, K, M, ldx}, Operand{w1, K, H, ldw1}, ext_params(M, 2 * H, K, status), ext, num_sms, stream,
                              [&](auto& e, int box) { return Operand{w3, K, H, ldw3}.map(&e.tmB2, box); });
   };
-  return bits == 0 ? launch(GatedExt<0>{}) : bits == 8 ? launch(GatedExt<8>{}) : launch(GatedExt<16>{});
+  return bits == 0 ? launch(GatedExt<0>{}) : bits == 8 ? launch(GatedExt<8>{}) : bits == 16 ? launch(GatedExt<16>{}) : launch(GatedExt<MX_HALF>{});
 }
 
 extern "C" int apb_gemm_gated_grad(const void* dy, const void* w2, const void* ab, const void* scales, int bits, void* dab, void* h, int M, int H,
                                    int K, long long ldy, long long ldw, int act, uint32_t* status, int num_sms, cudaStream_t stream) {
   const int no = ext_takes(M, H, K);
   if (no) return no;
-  if (off16({dy, w2, ab, dab, h}) || (bits != 8 && bits != 16) || ab == nullptr || scales == nullptr) return 3;
+  if (off16({dy, w2, ab, dab, h}) || (bits != 8 && bits != 16 && bits != MX_HALF) || ab == nullptr || scales == nullptr) return 3;
   const GatedGrad g{ab, (const uint8_t*)scales, (__nv_bfloat16*)dab, (__nv_bfloat16*)h, act};
   const Operand A{dy, K, M, ldy}, B{w2, H, K, ldw};
   const GemmParams p = ext_params(M, H, K, status);
   auto none = [](auto&, int) { return 0; };
-  return bits == 8 ? launch_ext<true>(A, B, p, GradExt<8>{g}, num_sms, stream, none) : launch_ext<true>(A, B, p, GradExt<16>{g}, num_sms, stream, none);
+  return bits == 8    ? launch_ext<true>(A, B, p, GradExt<8>{g}, num_sms, stream, none)
+         : bits == 16 ? launch_ext<true>(A, B, p, GradExt<16>{g}, num_sms, stream, none)
+                      : launch_ext<true>(A, B, p, GradExt<MX_HALF>{g}, num_sms, stream, none);
 }
 
 // C[M, N] = a1[M, K] b1[K, N] + a2[M, K] b2[K, N], bf16; one accumulation over both contractions.

@@ -6,14 +6,21 @@
 // The scale byte is e + 127; a block with an infinity or a NaN has the byte 255 and reads as NaN.  The format's e goes down to -127; what is written here stops where
 // the unit is 2^-126, so every value is a normal fp32 number, and with 8 bits exact in bf16: products of the values on the tensor cores lose nothing to the format.
 // What is read may come from elsewhere and have any byte; 8-bit values below 2^-126 are multiples of 2^-133, exact in both types too.
+//
+// MX_HALF: fp16 numbers under the block's power of two, v 2^(14-e), with n = 14 otherwise.  A value keeps its own exponent: it is off by at most 2^-11 of itself
+// down to 2^-28 of its block's largest (bf16: 2^-8), and by 2^-39 of that below; whole numbers of 16 bits are off by 2^-15 of the block's largest, whatever the value.
 #pragma once
+#include <cuda_fp16.h>
 #include <stdint.h>
 
 namespace apb {
 
 constexpr int MX_BLOCK = 32, MX_NAN = 255;
+constexpr int MX_HALF = 11;  // (as BITS: those of a value)
 template <int BITS>
-constexpr int MX_LOWEST = BITS - 1;  // the scale byte of the smallest e
+constexpr int MX_BYTES = BITS == 8 ? 1 : 2;  // of a code
+template <int BITS>
+constexpr int MX_LOWEST = 8 * MX_BYTES<BITS> - 1;  // the scale byte of the smallest e
 
 // 2^(field - 127), field from -22 on, or the bits ``broken`` for a block that holds an infinity or a NaN.
 __device__ __forceinline__ float mx_unit(uint32_t byte, int field, uint32_t broken) {
@@ -80,6 +87,24 @@ struct MxCoder {
     }
   }
 };
+template <>
+struct MxCoder<MX_HALF> {
+  float m;
+  __device__ __forceinline__ MxCoder(uint32_t byte, uint32_t) : m(mx_unit(byte, 268 - (int)byte, 0u)) {}
+  template <int n>
+  __device__ __forceinline__ void words(const uint32_t* v, uint32_t (&w)[n]) const {
+    if (m != 0.f) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const __half2 h = __floats2half2_rn(mx_bits(v[2 * i]) * m, mx_bits(v[2 * i + 1]) * m);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    } else {  // (a broken block)
+#pragma unroll
+      for (int i = 0; i < n; ++i) w[i] = 0;
+    }
+  }
+};
 
 // Codes of one block to values: with 2^(n+1) added, a code is the lowest byte (or two) of 2^23 + (code + 2^(n+1)) as fp32; one permutation, a subtraction and a
 // multiplication by the power of two, both exact.  (In one step, with 2^23 + 2^(n+1) times the power of two taken off, that product would be infinite from e = 111 on,
@@ -99,6 +124,17 @@ struct MxReader {
     const uint32_t u = codes ^ 0x80008000u;
     f[0] = (mx_bits(__byte_perm(u, 0x4b000000u, 0x7410)) - BIAS) * m;
     f[1] = (mx_bits(__byte_perm(u, 0x4b000000u, 0x7432)) - BIAS) * m;
+  }
+};
+template <>
+struct MxReader<MX_HALF> {
+  float m;
+  MxReader() = default;
+  __device__ __forceinline__ explicit MxReader(uint32_t byte) : m(mx_unit(byte, (int)byte - 14, 0x7fc00000u)) {}
+  __device__ __forceinline__ void two(uint32_t codes, float* f) const {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&codes));
+    f[0] = v.x * m;
+    f[1] = v.y * m;
   }
 };
 

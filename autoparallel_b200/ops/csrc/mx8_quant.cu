@@ -362,27 +362,30 @@ __global__ void __launch_bounds__(256) mx8_dequantize_ragged_kernel(const uint8_
 }
 
 // The 16-bit codes of what gated_act_kernel takes, and back: a warp to a block, an element to a lane (only products in fp32 come here).
-__device__ __forceinline__ uint32_t code(const MxCoder<16>& coder, uint32_t v) {
+template <int BITS>
+__device__ __forceinline__ uint32_t code(const MxCoder<BITS>& coder, uint32_t v) {
   const uint32_t pair[2] = {v, 0};
   uint32_t w[1];
   coder.words(pair, w);
   return w[0];
 }
+template <int BITS>
 __global__ void __launch_bounds__(256) mx16_quantize_kernel(const float* x, uint16_t* codes, uint8_t* scales, uint32_t warps, int K, uint32_t blocks) {
   after_previous();
   const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), row = w / blocks, c = (w - row * blocks) * MX_BLOCK + (threadIdx.x & 31);
   if (w >= warps) return;
   const uint32_t v = c < (uint32_t)K ? __float_as_uint(x[(long long)row * K + c]) : 0u, top = __reduce_max_sync(0xffffffffu, v & 0x7fffffffu);
-  const uint32_t byte = mx_scale_byte<16>(top);
-  if (c < (uint32_t)K) codes[(long long)row * K + c] = (uint16_t)code(MxCoder<16>(byte, top), v);
+  const uint32_t byte = mx_scale_byte<BITS>(top);
+  if (c < (uint32_t)K) codes[(long long)row * K + c] = (uint16_t)code(MxCoder<BITS>(byte, top), v);
   if ((threadIdx.x & 31) == 0) scales[w] = (uint8_t)byte;
 }
+template <int BITS>
 __global__ void __launch_bounds__(256) mx16_dequantize_kernel(const uint16_t* codes, const uint8_t* scales, float* y, uint32_t warps, int K, uint32_t blocks) {
   after_previous();
   const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), row = w / blocks, c = (w - row * blocks) * MX_BLOCK + (threadIdx.x & 31);
   if (w >= warps || c >= (uint32_t)K) return;
   float f[2];
-  MxReader<16>(scales[w]).two(codes[(long long)row * K + c], f);
+  MxReader<BITS>(scales[w]).two(codes[(long long)row * K + c], f);
   y[(long long)row * K + c] = f[0];
 }
 
@@ -454,17 +457,18 @@ extern "C" int apb_mx8_dequantize(const void* codes, const void* scales, void* y
                  : dequantize((const uint8_t*)codes, (const uint8_t*)scales, (float*)y, R, K, st);
 }
 
-extern "C" int apb_mx16_quantize(const float* x, void* codes, void* scales, long long R, int K, cudaStream_t st) {
+// ``bits`` 16 or MX_HALF
+extern "C" int apb_mx16_quantize(const float* x, void* codes, void* scales, long long R, int K, int bits, cudaStream_t st) {
   const long long blocks = (K + MX_BLOCK - 1) / MX_BLOCK, warps = R * blocks;
   if (warps <= 0) return 0;
-  if (warps > 0xfffffff0ll) return 3;
-  return done(launch_after(mx16_quantize_kernel, blocks_of(warps * 32), 256, 0, st, x, (uint16_t*)codes, (uint8_t*)scales, (uint32_t)warps, K, (uint32_t)blocks));
+  if (warps > 0xfffffff0ll || (bits != 16 && bits != MX_HALF)) return 3;
+  return done(launch_after(bits == 16 ? mx16_quantize_kernel<16> : mx16_quantize_kernel<MX_HALF>, blocks_of(warps * 32), 256, 0, st, x, (uint16_t*)codes, (uint8_t*)scales, (uint32_t)warps, K, (uint32_t)blocks));
 }
-extern "C" int apb_mx16_dequantize(const void* codes, const void* scales, float* y, long long R, int K, cudaStream_t st) {
+extern "C" int apb_mx16_dequantize(const void* codes, const void* scales, float* y, long long R, int K, int bits, cudaStream_t st) {
   const long long blocks = (K + MX_BLOCK - 1) / MX_BLOCK, warps = R * blocks;
   if (warps <= 0) return 0;
-  if (warps > 0xfffffff0ll) return 3;
-  return done(launch_after(mx16_dequantize_kernel, blocks_of(warps * 32), 256, 0, st, (const uint16_t*)codes, (const uint8_t*)scales, y, (uint32_t)warps, K,
+  if (warps > 0xfffffff0ll || (bits != 16 && bits != MX_HALF)) return 3;
+  return done(launch_after(bits == 16 ? mx16_dequantize_kernel<16> : mx16_dequantize_kernel<MX_HALF>, blocks_of(warps * 32), 256, 0, st, (const uint16_t*)codes, (const uint8_t*)scales, y, (uint32_t)warps, K,
                            (uint32_t)blocks));
 }
 

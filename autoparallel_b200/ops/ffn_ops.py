@@ -22,9 +22,9 @@ Gated block.  With ``a = x w1^T``, ``b = x w3^T``, ``h = act(a) * b``, ``y = h w
     dh = dy w2       da = dh b act'(a)       db = dh act(a)
     dx = da w1 + db w3       dw1 = da^T x       dw3 = db^T x       dw2 = dy^T h
 
-a and b are kept for the backward pass, ``ab`` [.., 2, H], h is made again from them.  ``bits`` 16 keeps x as it is, and a, b as 16-bit
-codes (below) where x is bf16, as they are where it is fp32; 8 keeps all three as 8-bit checkpoints, from which all gradients are made;
-0 keeps nothing (no gradients).  da, db and the h of the backward pass are rounded to x's type, which is what the products of the
+a and b are kept for the backward pass, ``ab`` [.., 2, H], h is made again from them.  ``bits`` 11 keeps x as it is, and a, b as fp16 numbers
+under a power of two (below) where x is bf16, as they are where it is fp32; 16 the same with 16-bit codes; 8 keeps all three as 8-bit
+checkpoints, from which all gradients are made; 0 keeps nothing (no gradients).  da, db and the h of the backward pass are rounded to x's type, which is what the products of the
 gradients take.
 
 8-bit checkpoints (MXINT8 of the OCP Microscaling Formats specification, version 1.0).  32 values along the last dim share a power of two,
@@ -35,7 +35,8 @@ codes int8 of the values' shape, scales uint8 [.., ceil(K / 32)]: e + 127, and 2
 NaN.  (The format's e goes down to -127.  What is written here stops at -120, where the unit is the smallest normal fp32 number; what is read
 may have any scale.)  A value is off by at most 2^(e-7), but 2^(e-6) where it is the block's largest and rounds to 128; it is exact in bf16.  The 16-bit
 codes are the same with 14 for 6, -112 for -120 and 32767 for 127: in as many bits as bf16, off by 2^-15 of the block's largest value and
-not by 2^-9 of each.
+not by 2^-8 of each, which is more where that is 128 times the value.  fp16 numbers, v 2^(14-e) with the same e and scales, keep a value's own
+exponent: off by at most 2^-11 of it down to 2^-28 of the block's largest, and by 2^-39 of that below.
 
 The reference leaves these to the tracing compiler (``x + attention``, RMSNorm and SwiGLU of
 autoparallel/_testing/models/llama3.py:320-429); it has no 8-bit checkpoints.
@@ -48,9 +49,9 @@ import torch.nn.functional as F
 from .library import _ag, _make_cuda_entry, _rms_norm_bwd_ref, _rms_norm_ref, lib, ops, reference_impls
 
 ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
-CHECKPOINTS = {"full": 16, "mx8": 8}
+CHECKPOINTS = {"full": 11, "mx16": 16, "mx8": 8}
 BLOCK = 32
-_CODES = {8: torch.int8, 16: torch.int16}
+_CODES = {8: torch.int8, 11: torch.float16, 16: torch.int16}
 F8 = torch.float8_e4m3fn
 F8_MAX = 448.0
 
@@ -103,9 +104,12 @@ def _quantize(x, bits):
     v = F.pad(x.float(), (0, -k % BLOCK)).unflatten(-1, (mx8_blocks(k), BLOCK))
     field = (v.contiguous().view(torch.int32) & 0x7FFFFFFF).amax(-1) >> 23  # (as integers: a NaN is larger than everything)
     broken = field == 255
-    byte = field.clamp(min=bits - 1)
-    to_code = ((252 + bits - byte).clamp(min=1) << 23).to(torch.int32).view(torch.float32).masked_fill(broken, 0.0)
-    code = torch.nan_to_num(torch.round(v * to_code.unsqueeze(-1)), nan=0.0).clamp(1 - 2 ** (bits - 1), 2 ** (bits - 1) - 1)
+    n = 8 if bits == 8 else 16
+    byte = field.clamp(min=n - 1)
+    to_code = ((252 + n - byte).clamp(min=1) << 23).to(torch.int32).view(torch.float32).masked_fill(broken, 0.0)
+    code = torch.nan_to_num(v * to_code.unsqueeze(-1), nan=0.0)
+    if bits != 11:
+        code = torch.round(code).clamp(1 - 2 ** (n - 1), 2 ** (n - 1) - 1)
     return code.flatten(-2)[..., :k].to(_CODES[bits]).contiguous(), byte.to(torch.uint8)
 
 
@@ -139,11 +143,11 @@ def _kept(ab, bits, dtype):
     none = ab.new_empty(0, dtype=torch.uint8)
     if bits == 0:
         return ab.new_empty(0, dtype=dtype), none
-    return (ab, none) if bits == 16 and dtype is torch.float32 else _quantize(ab, bits)
+    return (ab, none) if bits != 8 and dtype is torch.float32 else _quantize(ab, bits)
 
 
 def _values(ab, scales):
-    return ab if ab.is_floating_point() else _dequantize(ab, scales, torch.float32)
+    return ab if ab.dtype is torch.float32 else _dequantize(ab, scales, torch.float32)
 
 
 def _gated_mm(x, w1, w3, act, bits):
@@ -183,7 +187,7 @@ def _new(x, shape, dtype=None):
 
 def _kept_meta(x, lead, n, bits):
     """(ab, scales) for [.., n]"""
-    if bits == 0 or (bits == 16 and x.dtype is torch.float32):
+    if bits == 0 or (bits != 8 and x.dtype is torch.float32):
         return _new(x, (*lead, n) if bits else (0,)), _new(x, (0,), torch.uint8)
     return _new(x, (*lead, n), _CODES[bits]), _new(x, (*lead, mx8_blocks(n)), torch.uint8)
 
@@ -343,7 +347,8 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Ten
               checkpoint: str = "full") -> torch.Tensor:
     """``(act(x w1^T) * (x w3^T)) w2^T``: x [.., D], w1 and w3 [H, D], w2 [N, H] -> [.., N].  ``act``: "silu", "gelu" (by the error
     function) or "gelu_tanh".  ``checkpoint``: what the backward pass finds, "full" (x, and both projections in as many bits as its type
-    has) or "mx8" (the same in 8 bits, about half the memory; the gradients are those of the rounded values)."""
+    has, of bf16 to 2^-11 of each value), "mx16" (the same of bf16 as whole numbers, to 2^-15 of the largest of 32 neighbours) or "mx8" (all
+    in 8 bits, about half the memory; the gradients are those of the rounded values)."""
     xs, ws = x.shape, w1.shape
     fits = (len(xs) >= 1 and len(ws) == 2 and w3.shape == ws and w2.ndim == 2 and ws[1] == xs[-1] and w2.shape[1] == ws[0]
             and x.dtype in _FLOATS and x.dtype is w1.dtype is w3.dtype is w2.dtype and x.device == w1.device == w3.device == w2.device)

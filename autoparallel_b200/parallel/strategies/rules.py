@@ -391,7 +391,7 @@ def _mx8_dequantize(ctx):
 
 def _hidden_splits(ctx, ab, hidden):
     """Whether the hidden dim of both projections may be split: of codes, in whole blocks."""
-    return ab.is_floating_point() or _splits(ctx, hidden, 32)
+    return ab.dtype is torch.float32 or _splits(ctx, hidden, 32)
 
 
 @register_rule(apb.gated_ffn.default)

@@ -90,3 +90,71 @@ def test_mx8_values_of_every_scale(k):
         assert torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got[:255].double(), want[:255].masked_fill(want[:255] <= -(2.0**128), -math.inf))
         assert torch.equal(K.mx8_dequantize(codes.cpu(), scales.cpu(), dtype).nan_to_num(nan=3.0), got.cpu().nan_to_num(nan=3.0))
+
+
+# ------------------------------------------------------------------------------------ gated block
+@pytest.mark.parametrize("M,D,H", [(256, 128, 128), (300, 72, 1000), (2100, 256, 520), (40, 36, 100)])
+@pytest.mark.parametrize("times", [1, 64, 4096, 2.0**15, 2.0**24])
+def test_full_keeps_small_values_beside_large_ones(M, D, H, times):
+    """One column of every block of 32 is much larger than the others; the gradients of the others' weights are as near to 64 bits as they are without it."""
+    g = _gen(M)
+    x, dy = _randn(M, D, gen=g), _randn(M, 64, gen=g)
+    w1, w3, w2 = _randn(H, D, gen=g, scale=D**-0.5), _randn(H, D, gen=g, scale=D**-0.5), _randn(64, H, gen=g, scale=H**-0.5)
+    large = torch.arange(H, device="cuda") % 32 == 5
+    w1[large] *= times
+    w3[large] *= times
+    leaves = [t.requires_grad_() for t in (x, w1, w3, w2)]
+    got = torch.autograd.grad(K.gated_ffn(*leaves), leaves, dy)
+    d = [t.detach().double().requires_grad_() for t in leaves]
+    want = torch.autograd.grad((F.silu(d[0] @ d[1].t()) * (d[0] @ d[2].t())) @ d[3].t(), d, dy.double())
+    for u, v in ((got[1][~large], want[1][~large]), (got[2][~large], want[2][~large]), (got[3][:, ~large], want[3][:, ~large])):
+        # two roundings to bf16 (da, db or h, and the result), each at most 2^-8 and evenly spread: sqrt(2 / 3) 2^-8; what is kept adds 2^-11 of each value at most
+        assert float((u.double() - v).norm() / v.norm()) <= math.sqrt(2 / 3) * 2.0**-8 + 2.0**-11
+
+
+# rows: split kernel, single CTAs, pairs, wide pairs, the plain products; columns: parts of tiles and of blocks of 32
+@pytest.mark.parametrize("M,D,H", [(1, 64, 8), (3, 256, 40), (17, 2048, 1408), (33, 64, 136), (130, 1288, 520), (300, 136, 2056), (999, 2048, 1408), (2100, 72, 1000), (4096, 4416, 1032),
+                                   (20, 60, 64), (37, 64, 63)])
+def test_fp16_numbers_of_both_projections(M, D, H):
+    act = ("silu", "gelu", "gelu_tanh")[(M + D + H) % 3]
+    fn = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh")}[act]
+    g = _gen(M)
+    x, dy = _randn(M, D, gen=g), _randn(M, 128, gen=g)
+    # columns of very different sizes within a block
+    w1, w3 = ((_randn(H, D, gen=g, dtype=F32, scale=D**-0.5) * torch.exp2(torch.randint(-20, 1, (H, 1), device="cuda", generator=g).float())).to(BF) for _ in range(2))
+    w2 = _randn(128, H, gen=g, scale=H**-0.5)
+    h, ab, scales = ops.gated_mm(x, w1, w3, FFN.ACTS[act], 11)
+    assert ab.dtype == torch.float16 and ab.shape == (M, 2, H) and scales.shape == (M, 2, -(-H // 32)) and bool((scales >= 15).all())
+    exact = torch.stack([x.double() @ w.double().t() for w in (w1, w3)], 1)
+    kept = ab.double() * torch.exp2(scales.double() - 141).repeat_interleave(32, -1)[..., :H]
+    # fp16's half step, and the products' own error: a step of 16 terms rounds the accumulator, which may cut it off (2^-23 and not a half of that), at its running
+    # size; that is a partial sum of independent terms with random signs, so within 6 times the root of the sum of their squares (normal: 2e-9 of all are not)
+    acc = (D / 16 + 1) * 2.0**-23 * 6 * torch.stack([(x.double().square() @ w.double().square().t()).sqrt() for w in (w1, w3)], 1)
+    off = (kept - exact).abs() - 2.0**-11 * exact.abs()
+    assert bool((off <= 1.01 * acc).all()), float((off / acc).max())
+    dab, h2 = ops.gated_dgrad(dy, w2, ab, scales, FFN.ACTS[act])
+    a, b = (t.clone().requires_grad_() for t in kept.unbind(1))
+    hd = fn(a) * b
+    dh = dy.double() @ w2.double()
+    da, db = torch.autograd.grad(hd, (a, b), dh)
+    hd, a, b = hd.detach(), a.detach(), b.detach()
+    # a half step of bf16; of dh: the terms' sum in fp32; of the activation and its derivative: 2^-18 of their terms (|act| <= |a|, |act'| <= 1.13 for all three)
+    off = (128 / 16 + 1) * 2.0**-23 * 6 * (dy.double().square() @ w2.double().square()).sqrt()
+    for got, want, slope in ((dab[:, 0], da, 1.13 * b.abs()), (dab[:, 1], db, a.abs())):
+        assert bool(((got.double() - want).abs() <= 2.0**-8 * want.abs() + 1.01 * (off + 2.0**-18 * dh.abs()) * slope).all())
+    assert bool(((h2.double() - hd).abs() <= (2.0**-8 + 2.0**-17) * hd.abs() + 2.0**-140).all())
+
+
+def test_fp16_numbers_at_the_ends_of_the_range():
+    """A block of any size, with infinities and NaN, of zeros: as the formula on the CPU has it, in the form for the plain products (63 columns) too."""
+    for H in (64, 63):
+        x = torch.zeros(12, 8, device="cuda", dtype=BF)
+        x[:, 0] = torch.tensor([0, 1, 2.0**-60, 2.0**60, 2.0**-110, 2.0**126, -(2.0**126), math.inf, math.nan, 3, -0.0, 2.0**-20], device="cuda").to(BF)
+        w1 = torch.zeros(H, 8, device="cuda", dtype=BF)
+        w1[:, 0] = _randn(H, gen=_gen(3)).clamp(-3.5, 3.5)
+        _, ab, scales = ops.gated_mm(x, w1, w1, 0, 11)
+        want = FFN._quantize((x[:, :1].float() * w1[:, 0].float()).unsqueeze(1).expand(12, 2, H), 11)
+        rows = [0, 1, 2, 3, 4, 5, 6, 9, 10, 11]
+        assert torch.equal(ab[rows], want[0][rows]) and torch.equal(scales, want[1]) and bool((scales[7:9] == 255).all())
+        dab, h = ops.gated_dgrad(x, torch.ones(8, H, device="cuda", dtype=BF), ab, scales, 0)
+        assert dab[7:9].isnan().all() and h[7:9].isnan().all()

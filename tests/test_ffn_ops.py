@@ -551,3 +551,56 @@ def test_mx8_values_of_every_scale(k):
     for dtype in (torch.bfloat16, torch.float32):  # (exact in both but for -2^128)
         got = K.mx8_dequantize(codes, scales, dtype)
         assert got[255].isnan().all() and torch.equal(got[:255].double(), want[:255].masked_fill(want[:255] <= -(2.0**128), -math.inf))
+
+
+def test_fp16_numbers_under_a_power_of_two():
+    """What "full" keeps of both projections of bf16 operands: every value to fp16's half step down to 2^-28 of its block's largest."""
+    g = _gen(15)
+    x = _randn(6, 70, gen=g) * torch.exp2(torch.randint(-34, 1, (6, 70), generator=g).float())
+    x[1, :32], x[2, 32:64], x[3, 40], x[4, 3] = 0, x[2, 32:64] * 2.0**-125, float("inf"), float("nan")
+    x[5, 0] = -1.7 * 2.0**127
+    codes, scales = FFN._quantize(x, 11)
+    assert codes.dtype == torch.float16 and scales.shape == (6, 3) and scales[1, 0] == 15 and scales[3, 1] == scales[4, 0] == 255 and scales[5, 0] == 254
+    v = FFN._dequantize(codes, scales, torch.float32)
+    assert v[3, 32:64].isnan().all() and v[4, :32].isnan().all()
+    top = F.pad(x, (0, 26)).unflatten(-1, (3, 32)).abs().amax(-1, keepdim=True).expand(6, 3, 32).flatten(1)[:, :70].double()
+    ok = torch.isfinite(top)
+    err, e = (v[ok].double() - x[ok].double()).abs(), torch.floor(torch.log2(top[ok].clamp_min(2.0**-112)))
+    # (a last 2^-150: values below fp32's normal numbers)
+    assert (err <= torch.maximum(2.0**-11 * x[ok].double().abs(), torch.exp2(e - 39)) + 2.0**-150).all()
+    assert (err[x[ok].abs() >= top[ok] * 2.0**-28] <= 2.0**-11 * x[ok].double().abs()[x[ok].abs() >= top[ok] * 2.0**-28] + 2.0**-150).all()
+
+
+@pytest.mark.parametrize("times", [1, 4096, 2.0**24])
+def test_full_keeps_small_values_beside_large_ones(times):
+    """One column of every block of 32 is much larger than the others: the gradients of the others' weights are as near as they are without it."""
+    g = _gen(16)
+    x, dy = _randn(64, 48, dtype=torch.bfloat16, gen=g), _randn(64, 40, dtype=torch.bfloat16, gen=g)
+    w1, w3, w2 = _randn(70, 48, gen=g) / 7, _randn(70, 48, gen=g) / 7, _randn(40, 70, gen=g) / 8
+    large = torch.arange(70) % 32 == 5
+    w1[large] *= times
+    w3[large] *= times
+    leaves = [t.bfloat16().requires_grad_() for t in (x, w1, w3, w2)]
+    got = torch.autograd.grad(K.gated_ffn(*leaves), leaves, dy)
+    d = [t.detach().double().requires_grad_() for t in leaves]
+    want = torch.autograd.grad((F.silu(d[0] @ d[1].t()) * (d[0] @ d[2].t())) @ d[3].t(), d, dy.double())
+    for u, v in ((got[1][~large], want[1][~large]), (got[2][~large], want[2][~large]), (got[3][:, ~large], want[3][:, ~large])):
+        # two roundings to bf16 (da, db or h, and the result), each at most 2^-8 and evenly spread: sqrt(2 / 3) 2^-8; what is kept adds 2^-11 of each value at most
+        assert float((u.double() - v).norm() / v.norm()) <= math.sqrt(2 / 3) * 2.0**-8 + 2.0**-11
+
+
+def test_16_bit_whole_numbers_as_a_checkpoint():
+    """"mx16": a and b of bf16 operands as whole numbers; of fp32 operands as they are."""
+    g = _gen(17)
+    for dtype, kept in ((torch.bfloat16, torch.int16), (torch.float32, torch.float32)):
+        leaves = [_randn(*s, dtype=dtype, gen=g).requires_grad_() for s in ((5, 24), (40, 24), (40, 24), (16, 40))]
+        dy = _randn(5, 16, dtype=dtype, gen=g)
+        _, ab, scales = ops.gated_mm(*(t.detach() for t in leaves[:3]), 0, 16)
+        assert ab.dtype == kept
+        got = torch.autograd.grad(K.gated_ffn(*leaves, checkpoint="mx16"), leaves, dy)
+        x, w1, w3, w2 = (t.detach() for t in leaves)
+        dab, h = ops.gated_dgrad(dy, w2, ab, scales, 0)
+        want = (ops.gated_dx(dab, w1, w3), *ops.gated_wgrad(dab, x, dtype), ops.mm_wgrad(dy, h, dtype))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    m = _llama(fused_ffn=True, ffn_checkpoint="mx16")
+    assert m.layers["0"].feed_forward.checkpoint == "mx16"
