@@ -103,6 +103,8 @@ int apb_gemm_gated_grad(const void* dy, const void* w2, const void* ab, const vo
                         long long ldw, int act, uint32_t* status, int num_sms, cudaStream_t stream);
 int apb_gemm_dual(const void* a1, const void* a2, const void* b1, const void* b2, void* C, int M, int N, int K, long long lda, long long ldb1, long long ldb2,
                   long long ldc, uint32_t* status, int num_sms, cudaStream_t stream);
+int apb_gemm_two(const void* A, const void* B, void* c1, void* c2, int H, int N, int K, long long lda, long long ldb, int out_fp32, uint32_t* status,
+                 int num_sms, cudaStream_t stream);
 int apb_symm_header_bytes();
 int apb_symm_wait_probe(const uint32_t* flag, unsigned target, unsigned limit_ms, uint32_t* status, cudaStream_t st);
 int apb_symm_collective(int mode, const unsigned long long* peer_ptrs, int rank, int n, unsigned epoch, const void* src,

@@ -223,7 +223,7 @@ Tensor gated_dx(const Tensor& dab_, const Tensor& w1, const Tensor& w3) {
   return (product32(m.select(1, 0), w1, false) + product32(m.select(1, 1), w3, false)).to(dab.scalar_type()).view(shape);
 }
 
-// One product for both: rows of da and db side by side are one operand.  The gradients are the halves of its result.
+// One product for both: rows of da and db side by side are one operand, whose product goes to two tensors.
 Two gated_wgrad(const Tensor& dab, const Tensor& x, at::ScalarType dtype) {
   c10::cuda::CUDAGuard g(dab.device());
   TORCH_CHECK(dab.dim() >= 2 && dab.size(-2) == 2 && x.dim() >= 1 && rows_of(dab, 2) == rows_of(x, 1) && float_or_bf16(x.scalar_type()) &&
@@ -231,9 +231,17 @@ Two gated_wgrad(const Tensor& dab, const Tensor& x, at::ScalarType dtype) {
               "gated_wgrad: dab [.., 2, H] and x [.., D] of one type and as many rows");
   const int64_t M = rows_of(x, 1), H = dab.size(-1), D = x.size(-1);
   if (M == 0 || H == 0 || D == 0) return {at::zeros({H, D}, x.options().dtype(dtype)), at::zeros({H, D}, x.options().dtype(dtype))};
-  Tensor dw = op_mm_wgrad(dab.reshape({M, 2 * H}), x.reshape({M, D}), dtype);
-  Tensor first = dw.narrow(0, 0, H), second = dw.narrow(0, H, H);
-  return {first, dense(second)};  // (a half that begins off a 16-byte boundary is copied)
+  if (gated_form({&dab, &x}, {H, D}) && M <= 0x7fffffff) {
+    Tensor a = as2d(dab.reshape({M, 2 * H})), b = as2d(x.reshape({M, D}));
+    Tensor dw1 = at::empty({H, D}, x.options().dtype(dtype)), dw3 = at::empty_like(dw1);
+    const int err = apb_gemm_two(a.data_ptr(), b.data_ptr(), dw1.data_ptr(), dw3.data_ptr(), (int)H, (int)D, (int)M, a.stride(0), b.stride(0), dtype == at::kFloat,
+                                 status_word(x), num_sms(), stream());
+    if (err == 0) count();
+    if (err == 0) return {dw1, dw3};
+    if (err > 0) check(err, "apb_gemm_two");
+  }
+  Tensor both = dab.reshape({M, 2, H}), x2 = x.reshape({M, D});
+  return {op_mm_wgrad(both.select(1, 0), x2, dtype), op_mm_wgrad(both.select(1, 1), x2, dtype)};
 }
 
 // Whether the product with w2 is the few-row kernel's, whose first loads do not wait for h, with w2 as it lies in memory (a copy would be made by the kernel

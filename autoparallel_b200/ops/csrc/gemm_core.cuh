@@ -104,7 +104,8 @@ struct GemmParams {
 //              projections of a gated feed-forward block, and the epilogue makes h of them (gated.cuh).  N counts the columns of both.
 //   EXT_GRAD   the epilogue takes the derivative of that through the result, dh
 //   EXT_DUAL   C = opA * opB + opA2 * opB2 in one accumulation: K counts the blocks of both contractions, in whole blocks of BK
-enum : int { EXT_NONE = 0, EXT_GATED = 1, EXT_GRAD = 2, EXT_DUAL = 3 };
+//   EXT_TWO    the result's rows from ``cut`` on lie in memory of their own, ``jump`` bytes behind where they would be
+enum : int { EXT_NONE = 0, EXT_GATED = 1, EXT_GRAD = 2, EXT_DUAL = 3, EXT_TWO = 4 };
 struct NoExt {
   static constexpr int KIND = EXT_NONE;
 };
@@ -124,6 +125,18 @@ struct DualExt {
   static constexpr int KIND = EXT_DUAL;
   CUtensorMap tmA2, tmB2;
 };
+
+struct TwoExt {
+  static constexpr int KIND = EXT_TWO;
+  int cut;
+  long long jump;  // of whole vectors
+};
+// bytes that row ``row`` of the result lies away from its place
+template <typename Ext>
+__device__ __forceinline__ long long row_jump(const Ext& ext, long long row) {
+  if constexpr (Ext::KIND == EXT_TWO) return row >= ext.cut ? ext.jump : 0;
+  else return 0;
+}
 
 template <typename Ext>
 constexpr int ext_bits() {
@@ -259,9 +272,9 @@ __device__ __forceinline__ void store_row_chunk(const GemmParams& p, long long r
 // chain of dependent instructions (900 cycles a block) fills neither the load-store unit nor the memory.  Weight gradients of 64 experts,
 // 2048 x 1408 over 160 rows: 162 us with TMA stores, 130 with four warps and these stores, 93 with eight, 84 with the stores in groups of four (the
 // result alone takes 64).
-template <bool OUT_FP32, typename Release>
+template <bool OUT_FP32, typename Release, typename Ext = NoExt>
 __device__ __forceinline__ void store_tile(void* C, long long ldc, uint8_t* stg, uint32_t taddr, int row0, int n0, int ncols, int M, int N, int lane,
-                                           Release release) {
+                                           Release release, const Ext& ext = Ext{}) {
   constexpr int CC = OUT_FP32 ? 32 : 64, PER = OUT_FP32 ? 4 : 8;  // columns of 128 and of 16 bytes
   const int used = row0 < M ? min(ncols, N - n0) : 0;             // (rows and columns past the matrix are not read)
   if (used <= 0) {
@@ -312,7 +325,8 @@ __device__ __forceinline__ void store_tile(void* C, long long ldc, uint8_t* stg,
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (in_cols && row0 + (h + i) * 4 + sub < M) *reinterpret_cast<uint4*>(dst) = x[i];
+        const int row = row0 + (h + i) * 4 + sub;
+        if (in_cols && row < M) *reinterpret_cast<uint4*>(dst + row_jump(ext, row)) = x[i];
         dst += 4 * row_bytes;
       }
     }
@@ -961,8 +975,8 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
         if (staged) {
           const long long c_off = GROUPED ? (long long)x.grp * p.M * p.ldc : 0;
           const int r0 = (int)cta_row0 + q * 32;
-          if (p.out_fp32) store_tile<true>(reinterpret_cast<float*>(p.C) + c_off, p.ldc, stg, taddr, r0, n0, cols, p.M, p.N, lane, release);
-          else store_tile<false>(reinterpret_cast<__nv_bfloat16*>(p.C) + c_off, p.ldc, stg, taddr, r0, n0, cols, p.M, p.N, lane, release);
+          if (p.out_fp32) store_tile<true>(reinterpret_cast<float*>(p.C) + c_off, p.ldc, stg, taddr, r0, n0, cols, p.M, p.N, lane, release, ext);
+          else store_tile<false>(reinterpret_cast<__nv_bfloat16*>(p.C) + c_off, p.ldc, stg, taddr, r0, n0, cols, p.M, p.N, lane, release, ext);
         }
 #pragma unroll 1
         for (int c = 0; c < cols / 32 && !staged; ++c) {

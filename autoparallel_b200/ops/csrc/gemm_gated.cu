@@ -3,9 +3,11 @@
 //   apb_gemm_gated        h = act(x w1^T) * (x w3^T), and codes of x w1^T and x w3^T                               x [M, K], w [H, K]
 //   apb_gemm_gated_grad   from dh = dy w2: da, db and h again (gated.cuh)                                            dy [M, K], w2 [K, H]
 //   apb_gemm_dual         dx = da w1 + db w3                                                                         da, db [M, K], w [K, N]
+//   apb_gemm_two          dw1 = da^T x, dw3 = db^T x, da and db side by side in one operand                          dab [K, 2 H], x [K, N]
 //
 // They are the bodies of the plain products (gemm_core.cuh, gemm_split.cuh) with other ends, so tiles, CTA pairs, slices and their choice are the same: a tile of
-// both projections counts as one of a product with 2 H columns, the two contractions of dx as one of twice the length.
+// both projections counts as one of a product with 2 H columns, the two contractions of dx as one of twice the length.  The two gradients are one product with 2 H rows whose
+// halves go to two tensors.
 #include "gemm_split.cuh"
 
 extern "C" {
@@ -22,26 +24,26 @@ int apb_gemm_rows_gated(const void* X, const void* W1, const void* W3, void* h, 
 
 namespace apb {
 
-// B_MN: as stored; WIDE: gemm_core.cuh
-template <bool B_MN, bool WIDE, typename Ext>
+// A_MN, B_MN: as stored; WIDE: gemm_core.cuh
+template <bool A_MN, bool B_MN, bool WIDE, typename Ext>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_PLAIN_THREADS, 1)
 gemm_ext_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p, const __grid_constant__ Ext ext) {
   extern __shared__ uint8_t smem_raw[];
   FuseParams f{};
-  gemm_cta<false, B_MN, FUSE_NONE, true, false, 0, false, WIDE>(tmA, tmB, p, f, blockIdx.x, gridDim.x, smem_raw, ext);
+  gemm_cta<A_MN, B_MN, FUSE_NONE, true, false, 0, false, WIDE>(tmA, tmB, p, f, blockIdx.x, gridDim.x, smem_raw, ext);
 }
-template <bool B_MN, typename Ext>
+template <bool A_MN, bool B_MN, typename Ext>
 __global__ void __launch_bounds__(GEMM_PLAIN_THREADS, 1)
 gemm_ext_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p, const __grid_constant__ Ext ext) {
   extern __shared__ uint8_t smem_raw[];
   FuseParams f{};
-  gemm_cta<false, B_MN, FUSE_NONE>(tmA, tmB, p, f, blockIdx.x, gridDim.x, smem_raw, ext);
+  gemm_cta<A_MN, B_MN, FUSE_NONE>(tmA, tmB, p, f, blockIdx.x, gridDim.x, smem_raw, ext);
 }
-template <bool B_MN, int BN_T, typename Ext>
+template <bool A_MN, bool B_MN, int BN_T, typename Ext>
 __global__ void __launch_bounds__(SPLIT_THREADS, 1)
 gemm_ext_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p,
                       const __grid_constant__ Ext ext) {
-  split::gemm_cta<false, B_MN, BN_T, false>(tmA, tmB, p, ext);
+  split::gemm_cta<A_MN, B_MN, BN_T, false>(tmA, tmB, p, ext);
 }
 
 struct Operand {  // a 16-bit matrix; ``inner`` contiguous
@@ -51,13 +53,13 @@ struct Operand {  // a 16-bit matrix; ``inner`` contiguous
 };
 
 // One product with 128 rows of A, ``b_box`` rows (of a K-major B) or columns a tile.  ``second``: maps of the second operands, given the tile.
-template <bool B_MN, typename Ext, typename Second>
+template <bool A_MN, bool B_MN, typename Ext, typename Second>
 int launch_ext(const Operand& A, const Operand& B, GemmParams p, Ext ext, int num_sms, cudaStream_t stream, Second second) {
   constexpr bool HALVES = Ext::KIND == EXT_GATED;  // half of a tile's rows of B are the second matrix's
   if (((reinterpret_cast<uintptr_t>(A.ptr) | reinterpret_cast<uintptr_t>(B.ptr)) & 15) || ((A.ld | B.ld) & 7)) return 3;
   const int reserved = apb_gemm_get_reserved_sms();
   CUtensorMap tmA, tmB;
-  int e = A.map(&tmA, BM);
+  int e = A.map(&tmA, A_MN ? BK : BM);
   if (e) return e;
   auto maps = [&](int b_box) {
     const int e2 = B.map(&tmB, b_box);
@@ -87,8 +89,8 @@ int launch_ext(const Operand& A, const Operand& B, GemmParams p, Ext ext, int nu
       cfg.numAttrs = apb_gemm_makes_room() ? 1 : 2;
       return cudaLaunchKernelEx(&cfg, kern, tmA, tmB, p, ext) == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : 4;
     };
-    return bn == 64 ? launch(gemm_ext_split_kernel<B_MN, 64, Ext>) : bn == 128 ? launch(gemm_ext_split_kernel<B_MN, 128, Ext>)
-                                                                              : launch(gemm_ext_split_kernel<B_MN, 256, Ext>);
+    return bn == 64 ? launch(gemm_ext_split_kernel<A_MN, B_MN, 64, Ext>) : bn == 128 ? launch(gemm_ext_split_kernel<A_MN, B_MN, 128, Ext>)
+                                                                              : launch(gemm_ext_split_kernel<A_MN, B_MN, 256, Ext>);
   }
   p.num_n_tiles = (p.N + BN - 1) / BN;
   const bool pair = apb_gemm_get_pair_mode() && pair_shape(p.M, p.N, p.K);
@@ -106,11 +108,11 @@ int launch_ext(const Operand& A, const Operand& B, GemmParams p, Ext ext, int nu
     if (resident < 1) resident = 1;
     const bool wide = set_pair_tiles(p, (p.M + 2 * BM - 1) / (2 * BM), resident, true);
     const int units = 2 * p.all_tiles - p.whole_tiles, grid = 2 * (units < resident ? units : resident);
-    return wide ? launch(gemm_ext_pair_kernel<B_MN, true, Ext>, grid) : launch(gemm_ext_pair_kernel<B_MN, false, Ext>, grid);
+    return wide ? launch(gemm_ext_pair_kernel<A_MN, B_MN, true, Ext>, grid) : launch(gemm_ext_pair_kernel<A_MN, B_MN, false, Ext>, grid);
   }
   set_tile_order(p, p.num_m_tiles, p.num_n_tiles);
   const int tiles = p.num_m_tiles * p.num_n_tiles, usable = num_sms - reserved > 0 ? num_sms - reserved : 1;
-  return launch(gemm_ext_kernel<B_MN, Ext>, tiles < usable ? tiles : usable);
+  return launch(gemm_ext_kernel<A_MN, B_MN, Ext>, tiles < usable ? tiles : usable);
 }
 
 static GemmParams ext_params(int M, int N, int K, uint32_t* status) {
@@ -122,8 +124,8 @@ static GemmParams ext_params(int M, int N, int K, uint32_t* status) {
 
 // Shapes of these kernels: rows of whole 16 bytes.  Where GEMMs are set to hand out their tiles at run time or to leave shared memory free for
 // communication kernels, plain products do that (-1: the caller's).
-static int ext_takes(int M, int H, int K) {
-  if (M <= 0 || H <= 0 || K <= 0 || (H & 7) || (K & 7)) return 3;
+static int ext_takes(int M, int H, int K, bool a_mn = false) {
+  if (M <= 0 || H <= 0 || K <= 0 || (H & 7) || ((a_mn ? M : K) & 7)) return 3;
   return apb_gemm_get_dynamic_tiles() || apb_gemm_get_pair_stages() != PAIR_STAGES ? -1 : 0;
 }
 static bool off16(std::initializer_list<const void*> ps) {
@@ -155,7 +157,7 @@ extern "C" int apb_gemm_gated(const void* x, const void* w1, const void* w3, voi
     return apb_gemm_rows_gated(x, w1, w3, h, M, H, K, ldx, ldw1, ldw3, act, num_sms, stream);
   auto launch = [&](auto ext) {
     ext.out = GatedOut{(__nv_bfloat16*)h, ab, (uint8_t*)scales, act};
-    return launch_ext<false>(Operand{x, K, M, ldx}, Operand{w1, K, H, ldw1}, ext_params(M, 2 * H, K, status), ext, num_sms, stream,
+    return launch_ext<false, false>(Operand{x, K, M, ldx}, Operand{w1, K, H, ldw1}, ext_params(M, 2 * H, K, status), ext, num_sms, stream,
                              [&](auto& e, int box) { return Operand{w3, K, H, ldw3}.map(&e.tmB2, box); });
   };
   return bits == 0 ? launch(GatedExt<0>{}) : bits == 8 ? launch(GatedExt<8>{}) : bits == 16 ? launch(GatedExt<16>{}) : launch(GatedExt<MX_HALF>{});
@@ -170,9 +172,9 @@ extern "C" int apb_gemm_gated_grad(const void* dy, const void* w2, const void* a
   const Operand A{dy, K, M, ldy}, B{w2, H, K, ldw};
   const GemmParams p = ext_params(M, H, K, status);
   auto none = [](auto&, int) { return 0; };
-  return bits == 8    ? launch_ext<true>(A, B, p, GradExt<8>{g}, num_sms, stream, none)
-         : bits == 16 ? launch_ext<true>(A, B, p, GradExt<16>{g}, num_sms, stream, none)
-                      : launch_ext<true>(A, B, p, GradExt<MX_HALF>{g}, num_sms, stream, none);
+  return bits == 8    ? launch_ext<false, true>(A, B, p, GradExt<8>{g}, num_sms, stream, none)
+         : bits == 16 ? launch_ext<false, true>(A, B, p, GradExt<16>{g}, num_sms, stream, none)
+                      : launch_ext<false, true>(A, B, p, GradExt<MX_HALF>{g}, num_sms, stream, none);
 }
 
 // C[M, N] = a1[M, K] b1[K, N] + a2[M, K] b2[K, N], bf16; one accumulation over both contractions.
@@ -186,8 +188,25 @@ extern "C" int apb_gemm_dual(const void* a1, const void* a2, const void* b1, con
   p.C = C;
   p.ldc = ldc;
   p.vec_store = 1;
-  return launch_ext<true>(Operand{a1, K, M, lda}, Operand{b1, N, K, ldb1}, p, DualExt{}, num_sms, stream, [&](DualExt& e, int box) {
+  return launch_ext<false, true>(Operand{a1, K, M, lda}, Operand{b1, N, K, ldb1}, p, DualExt{}, num_sms, stream, [&](DualExt& e, int box) {
     const int bad = Operand{a2, K, M, lda}.map(&e.tmA2, BM);
     return bad ? bad : Operand{b2, N, K, ldb2}.map(&e.tmB2, box);
   });
+}
+
+// c1[H, N] = a1^T b, c2[H, N] = a2^T b, bf16 or fp32: ``A`` [K, 2 H] has a1 and a2 side by side, ``B`` [K, N].
+extern "C" int apb_gemm_two(const void* A, const void* B, void* c1, void* c2, int H, int N, int K, long long lda, long long ldb, int out_fp32,
+                            uint32_t* status, int num_sms, cudaStream_t stream) {
+  if (H > 0x3fffffff) return 3;
+  const int no = ext_takes(H, N, K, true);
+  if (no) return no;
+  if (off16({A, B, c1, c2})) return 3;
+  GemmParams p = ext_params(2 * H, N, K, status);
+  p.C = c1;
+  p.ldc = N;
+  p.out_fp32 = out_fp32;
+  p.vec_store = 1;
+  const long long behind = (long long)H * N * (out_fp32 ? 4 : 2);
+  const TwoExt ext{H, (long long)(reinterpret_cast<intptr_t>(c2) - reinterpret_cast<intptr_t>(c1)) - behind};
+  return launch_ext<true, true>(Operand{A, 2 * H, K, lda}, Operand{B, N, K, ldb}, p, ext, num_sms, stream, [](auto&, int) { return 0; });
 }

@@ -184,8 +184,8 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
       const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + col0;
       const long long c_off = GROUPED ? (long long)grp * p.M * p.ldc : 0;
       auto nothing = []() {};
-      if (p.out_fp32) store_tile<true>(reinterpret_cast<float*>(p.C) + c_off, p.ldc, stg, taddr, m0 + q * 32, n0 + col0, COLS, p.M, p.N, lane, nothing);
-      else store_tile<false>(reinterpret_cast<__nv_bfloat16*>(p.C) + c_off, p.ldc, stg, taddr, m0 + q * 32, n0 + col0, COLS, p.M, p.N, lane, nothing);
+      if (p.out_fp32) store_tile<true>(reinterpret_cast<float*>(p.C) + c_off, p.ldc, stg, taddr, m0 + q * 32, n0 + col0, COLS, p.M, p.N, lane, nothing, ext);
+      else store_tile<false>(reinterpret_cast<__nv_bfloat16*>(p.C) + c_off, p.ldc, stg, taddr, m0 + q * 32, n0 + col0, COLS, p.M, p.N, lane, nothing, ext);
     } else if (q * 32 < rows) {
       tc_fence_after();
       float* row = tile + (q * 32 + lane) * LD + col0;
@@ -266,7 +266,7 @@ __device__ __forceinline__ void gemm_cta(const CUtensorMap& tmA, const CUtensorM
     const long long ld_bytes = p.ldc * esz;
     auto add = [](float4& a, const float4& x) { a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w; };
     auto store = [&](int r, const float4& v) {
-      uint8_t* dst = dst0 + r * ld_bytes;
+      uint8_t* dst = dst0 + r * ld_bytes + row_jump(ext, m0 + r);
       if (whole) {
         if (p.out_fp32) *reinterpret_cast<float4*>(dst) = v;
         else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));

@@ -158,3 +158,26 @@ def test_fp16_numbers_at_the_ends_of_the_range():
         assert torch.equal(ab[rows], want[0][rows]) and torch.equal(scales, want[1]) and bool((scales[7:9] == 255).all())
         dab, h = ops.gated_dgrad(x, torch.ones(8, H, device="cuda", dtype=BF), ab, scales, 0)
         assert dab[7:9].isnan().all() and h[7:9].isnan().all()
+
+
+@pytest.mark.parametrize("M,D,H,dtype", [(64, 64, 64, BF), (300, 72, 1000, BF), (999, 2048, 1408, BF), (2100, 256, 5632, BF), (40, 36, 100, BF), (40, 36, 100, F32), (7, 64, 64, F32)])
+def test_gradients_of_both_projections_are_tensors_of_their_own(M, D, H, dtype):
+    g = _gen(H)
+    x, dab = _randn(M, D, gen=g, dtype=dtype), _randn(M, 2, H, gen=g, dtype=dtype)
+    for to in (BF, F32) if dtype == BF else (F32,):
+        both = ops.gated_wgrad(dab, x, to)
+        for i, t in enumerate(both):
+            assert t.is_contiguous() and t.storage_offset() == 0 and t.untyped_storage().nbytes() == t.numel() * t.element_size()
+            want = dab[:, i].double().t() @ x.double()
+            size = dab[:, i].double().abs().t() @ x.double().abs()
+            assert bool(((t.double() - want).abs() <= HALF_STEP[to] * want.abs() + M * 2.0**-24 * size).all())
+        assert both[0].untyped_storage().data_ptr() != both[1].untyped_storage().data_ptr()
+    if dtype == F32:
+        return
+    x, w1, w3, w2 = (t.requires_grad_() for t in (x, _randn(H, D, gen=g), _randn(H, D, gen=g), _randn(64, H, gen=g)))
+    K.gated_ffn(x, w1, w3, w2).float().sum().backward()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    nbytes = w3.grad.numel() * w3.grad.element_size()
+    w3.grad = None
+    assert before - torch.cuda.memory_allocated() >= nbytes

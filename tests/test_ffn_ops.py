@@ -604,3 +604,25 @@ def test_16_bit_whole_numbers_as_a_checkpoint():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     m = _llama(fused_ffn=True, ffn_checkpoint="mx16")
     assert m.layers["0"].feed_forward.checkpoint == "mx16"
+
+
+def test_entry_of_two_results_refuses_what_it_does_not_take():
+    out = _entries("""
+p, bad = V(1 << 20), V((1 << 20) + 8)  # (never read)
+two = [p, p, p, p, 64, 64, 5, LL(128), LL(64), 1, p, 148, N]
+for i in (0, 1, 2, 3):
+    print(so.apb_gemm_two(*two[:i], bad, *two[i + 1:]))
+for i in (4, 5):
+    print(so.apb_gemm_two(*two[:i], 60, *two[i + 1:]), so.apb_gemm_two(*two[:i], 0, *two[i + 1:]))
+print(so.apb_gemm_two(*two[:6], 0, *two[7:]), so.apb_gemm_two(*two[:4], 1 << 30, *two[5:]))
+for i in (7, 8):
+    print(so.apb_gemm_two(*two[:i], LL(60), *two[i + 1:]))
+""")
+    assert out == ["3"] * 12, out
+    out = _entries("p = V(1 << 20)\nso.apb_gemm_set_dynamic_tiles(1)\nprint(so.apb_gemm_two(p, p, p, p, 64, 64, 5, LL(128), LL(64), 1, p, 148, N))")
+    assert out == ["-1"]
+
+
+def test_gradients_of_both_projections_are_tensors_of_their_own():
+    dw1, dw3 = ops.gated_wgrad(torch.randn(5, 2, 16), torch.randn(5, 8), torch.float32)
+    assert dw1.untyped_storage().data_ptr() != dw3.untyped_storage().data_ptr() and dw1.untyped_storage().nbytes() == 16 * 8 * 4
