@@ -9,6 +9,8 @@ std::vector<int64_t> with_last(at::IntArrayRef lead, std::initializer_list<int64
   return s;
 }
 
+uint32_t* status_word(const Tensor& t) { return reinterpret_cast<uint32_t*>(status_of(t).data_ptr()); }
+
 struct NormArgs {
   Tensor x, res, w;
   int64_t rows, D;
@@ -64,7 +66,7 @@ Two add_rms_norm_bwd(const Tensor& dy_, const c10::optional<Tensor>& dh_, const 
   Tensor dy = dense(dy_), dh = dh_.has_value() ? dense(*dh_) : Tensor(), rstd = rstd_.contiguous();
   Tensor part = at::empty({(int64_t)apb_add_rms_norm_bwd_workspace(a.rows, (int)a.D, is_bf16(a.x), num_sms())}, rstd.options());  // partial sums of dw
   check(apb_add_rms_norm_bwd(dy.data_ptr(), dh.defined() ? dh.data_ptr() : nullptr, a.x.data_ptr(), a.w.data_ptr(), rstd.data_ptr<float>(), dx.data_ptr(), dw.data_ptr(),
-                             part.data_ptr<float>(), a.rows, (int)a.D, is_bf16(a.x), num_sms(), stream()),
+                             part.data_ptr<float>(), a.rows, (int)a.D, is_bf16(a.x), num_sms(), stream(), status_word(a.x)),
         "apb_add_rms_norm_bwd");
   count(2);
   return {dx, dw.to(weight.scalar_type())};
@@ -112,7 +114,6 @@ bool gated_form(std::initializer_list<const Tensor*> ts, std::initializer_list<i
   return true;
 }
 int64_t rows_of(const Tensor& t, int dims) { return c10::multiply_integers(t.sizes().slice(0, t.dim() - dims)); }
-uint32_t* status_word(const Tensor& t) { return reinterpret_cast<uint32_t*>(status_of(t).data_ptr()); }
 void gated_check(const Tensor& x, std::initializer_list<const Tensor*> ws, const char* what) {
   TORCH_CHECK(x.dim() >= 1 && float_or_bf16(x.scalar_type()), what, ": [.., D] in bf16 or fp32");
   for (const Tensor* w : ws)

@@ -280,14 +280,14 @@ __global__ void __launch_bounds__(1024) add_rms_norm_bwd_kernel(const T* dy, con
 // Where two or three rows of all three operands fit into shared memory: the rows arrive as bulk copies, issued ST - 1 steps ahead by one thread, so what is
 // under way costs no registers and does not wait for the reduction (the ring of the plain norm's backward kernel, elementwise.cu, with a third operand).
 // One block barrier a step: the sums of consecutive steps sit in alternating slots, and a stage is refilled behind the barrier of the step after its own,
-// which every thread reaches when it has read the stage for the last time.  Waits are bounded: if a stage never arrives, the block stops.
+// which every thread reaches when it has read the stage for the last time.  Waits are bounded: if a stage never arrives, the block records that in ``status`` and stops.
 // A row that begins anywhere is copied with the vectors it touches; the last few elements of the tensor, where they are no whole vector, are read from
 // memory.
 __host__ __device__ inline int bwd_slot_bytes(int D, int elem) { return (D % 8 == 0 ? D : (D + 14) / 8 * 8) * elem; }
 __host__ __device__ inline int bwd_ring_bytes(int D, int elem, int stages) { return stages * 3 * bwd_slot_bytes(D, elem) + 128; }
 template <typename T, bool EVEN, int NVEC, int THREADS, int ST>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? (NVEC == 1 ? 4 : 3) : 1)
-add_rms_norm_bwd_bulk_kernel(const T* dy, const T* dh, const T* h, const T* w, const float* rstd, T* dx, float* part, long long rows, int D) {
+add_rms_norm_bwd_bulk_kernel(const T* dy, const T* dh, const T* h, const T* w, const float* rstd, T* dx, float* part, long long rows, int D, uint32_t* status) {
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t bars[ST];
   __shared__ float red[2][THREADS / 32];
@@ -357,7 +357,10 @@ add_rms_norm_bwd_bulk_kernel(const T* dy, const T* dh, const T* h, const T* w, c
     const int st = (int)(it % ST);
     const float r = r_next;
     if (row + step < rows) r_next = rstd[row + step];
-    if (!mbar_wait(&bars[st], (uint32_t)((it / ST) & 1), abort_flag)) *abort_flag = 1;
+    if (!mbar_wait(&bars[st], (uint32_t)((it / ST) & 1), abort_flag)) {
+      atomicCAS(status, 0u, (uint32_t)ST_TIMEOUT_FULL);
+      *abort_flag = 1;
+    }
     const uint8_t* in = smem + 3 * st * slot;
     const int have = copied(at) - at.lead;  // columns that the copies brought
     auto read = [&](Vec8<T>& v, int operand, const T* p, int c) {
@@ -490,15 +493,15 @@ static cudaError_t launch_fwd(const void* x, const void* res, const void* w, con
 
 template <typename T, bool EVEN>
 static cudaError_t launch_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dw, float* part,
-                              long long rows, int D, int num_sms, cudaStream_t st) {
+                              long long rows, int D, int num_sms, cudaStream_t st, uint32_t* status) {
   const BwdPlan p = bwd_plan(rows, D, (int)sizeof(T), num_sms);
-  auto launch = [&](auto kern) {
+  auto launch = [&](auto kern, auto... more) {
     if (p.smem && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem) != cudaSuccess) return cudaErrorInvalidValue;
-    return launch_after(kern, p.grid, p.threads, p.smem, st, (const T*)dy, (const T*)dh, (const T*)h, (const T*)w, rstd, (T*)dx, part, rows, D);
+    return launch_after(kern, p.grid, p.threads, p.smem, st, (const T*)dy, (const T*)dh, (const T*)h, (const T*)w, rstd, (T*)dx, part, rows, D, more...);
   };
   cudaError_t e = cudaErrorInvalidValue;
 #define APB_RING(NV, TH, ST) \
-  if (p.np == NV && p.threads == TH && p.stages == ST) e = launch(add_rms_norm_bwd_bulk_kernel<T, EVEN, NV, TH, ST>)
+  if (p.np == NV && p.threads == TH && p.stages == ST) e = launch(add_rms_norm_bwd_bulk_kernel<T, EVEN, NV, TH, ST>, status)
   if (p.stages) {
     APB_RING(1, 32, 3);
     APB_RING(1, 64, 3);
@@ -544,15 +547,16 @@ extern "C" int apb_add_rms_norm(const void* x, const void* res, const void* w, v
 extern "C" long long apb_add_rms_norm_bwd_workspace(long long rows, int D, int is_bf16, int num_sms) {
   return rows <= 0 || D <= 0 ? 0 : (long long)bwd_plan(rows, D, is_bf16 ? 2 : 4, num_sms).grid * D;
 }
+// ``status``: a word of device memory, which a wait that runs out is recorded in
 extern "C" int apb_add_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dw, float* part,
-                                    long long rows, int D, int is_bf16, int num_sms, cudaStream_t st) {
-  if (rows <= 0 || D <= 0 || D > ADD_NORM_MAX) return 3;
+                                    long long rows, int D, int is_bf16, int num_sms, cudaStream_t st, uint32_t* status) {
+  if (rows <= 0 || D <= 0 || D > ADD_NORM_MAX || status == nullptr) return 3;
   for (const void* p : {dy, dh, h, w, (const void*)dx})
     if (off16(p)) return 3;
   auto go = [&](auto even) {
     constexpr bool E = decltype(even)::value;
-    return is_bf16 ? launch_bwd<bf16, E>(dy, dh, h, w, rstd, dx, dw, part, rows, D, num_sms, st)
-                   : launch_bwd<float, E>(dy, dh, h, w, rstd, dx, dw, part, rows, D, num_sms, st);
+    return is_bf16 ? launch_bwd<bf16, E>(dy, dh, h, w, rstd, dx, dw, part, rows, D, num_sms, st, status)
+                   : launch_bwd<float, E>(dy, dh, h, w, rstd, dx, dw, part, rows, D, num_sms, st, status);
   };
   const cudaError_t e = D % 8 == 0 ? go(std::true_type{}) : go(std::false_type{});
   return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : 4;

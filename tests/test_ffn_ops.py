@@ -626,3 +626,13 @@ for i in (7, 8):
 def test_gradients_of_both_projections_are_tensors_of_their_own():
     dw1, dw3 = ops.gated_wgrad(torch.randn(5, 2, 16), torch.randn(5, 8), torch.float32)
     assert dw1.untyped_storage().data_ptr() != dw3.untyped_storage().data_ptr() and dw1.untyped_storage().nbytes() == 16 * 8 * 4
+
+
+def test_norm_gradient_entry_needs_a_status_word():
+    """A wait that runs out is recorded there, so the entry launches nothing without one."""
+    out = _entries("""
+p = V(1 << 20)  # (never read)
+for d in (64, 63, 32768):
+    print(so.apb_add_rms_norm_bwd(p, p, p, p, p, p, p, p, LL(4), d, 1, 148, N, N), so.apb_add_rms_norm_bwd(p, N, p, p, p, p, p, p, LL(4), d, 1, 148, N, N))
+""")
+    assert out == ["3"] * 6, out
