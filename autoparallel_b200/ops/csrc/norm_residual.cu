@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(WARP_ROWS ? 256 : 1024) add_rms_norm_kernel(co
 }
 
 // Backward.  Blocks take rows in turn and keep their sums of dw in registers; each leaves one row of partial sums, which rms_dw_kernel adds up in order: the
-// same result every time.  Where rows begin anywhere, the number of blocks is a multiple of 8, so that all rows of a block begin alike and a thread
+// same result every time.  No power of r is formed: rows of any size that the forward pass takes have a gradient (r^3 would be no fp32 number from rms 2e12 on).  Where rows begin anywhere, the number of blocks is a multiple of 8, so that all rows of a block begin alike and a thread
 // keeps its columns.
 template <typename T, bool EVEN>
 __device__ __forceinline__ void put_partial(const Row<T, EVEN>& at, float* part, const float (&dw)[8], int c) {
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(1024) add_rms_norm_bwd_kernel(const T* dy, con
       }
     }
     dot = block_sum(dot, red);
-    const float k = r * r * r * dot * inv_d;
+    const float mean = r * dot * inv_d;  // of g n
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       const int c = at.col(threadIdx.x + j * blockDim.x);
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(1024) add_rms_norm_bwd_kernel(const T* dy, con
         gv.to_float(gf);
         at.weight(wf, w, c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ef[i] += fmaf(gf[i], r * wf[i], -hf[i] * k);
+        for (int i = 0; i < 8; ++i) ef[i] = fmaf(r, fmaf(-(hf[i] * r), mean, gf[i] * wf[i]), ef[i]);
         ev.from_float(ef);
         at.store(ev, dx, c);
       }
@@ -404,7 +404,7 @@ add_rms_norm_bwd_bulk_kernel(const T* dy, const T* dh, const T* h, const T* w, c
       break;
     }
     if (threadIdx.x == 0) issue(it + ST - 1);
-    const float k = r * r * r * dot * inv_d;
+    const float mean = r * dot * inv_d;  // of g n
 #pragma unroll
     for (int j = 0; j < NVEC; ++j) {
       if (col[j] < D) {
@@ -420,7 +420,7 @@ add_rms_norm_bwd_bulk_kernel(const T* dy, const T* dh, const T* h, const T* w, c
         gv.to_float(gf);
         weight(wf, j);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ef[i] += fmaf(gf[i], r * wf[i], -hf[i] * k);
+        for (int i = 0; i < 8; ++i) ef[i] = fmaf(r, fmaf(-(hf[i] * r), mean, gf[i] * wf[i]), ef[i]);
         ev.from_float(ef);
         at.store(ev, dx, col[j]);
       }

@@ -181,3 +181,31 @@ def test_gradients_of_both_projections_are_tensors_of_their_own(M, D, H, dtype):
     nbytes = w3.grad.numel() * w3.grad.element_size()
     w3.grad = None
     assert before - torch.cuda.memory_allocated() >= nbytes
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("both", [True, False])
+@pytest.mark.parametrize("D", [1001, 2048, 16384, 32768])
+@pytest.mark.parametrize("size,eps", [(1e-14, 1e-32), (1e-12, 1e-5), (1.0, 1e-5), (1e14, 1e-5), (1e16, 1e-5)])
+def test_gradients_of_rows_of_unusual_size(size, eps, D, both, dtype):
+    """The norm of rows of any size has a gradient, down to where the square of 1 / rms is no number any more."""
+    g = _gen(D)
+    x, r = (_randn(19, D, gen=g, dtype=dtype, scale=size) for _ in range(2))
+    dy, dh = (_randn(19, D, gen=g, dtype=dtype, scale=s) for s in (1.0, 1 / size))
+    w = (1 + 0.1 * torch.randn(D, device="cuda", generator=g)).to(dtype)
+    leaves = [t.requires_grad_() for t in (x, r, w)]
+    y, h = K.add_rms_norm(*leaves, eps)
+    got = torch.autograd.grad((y, h), leaves, (dy, dh)) if both else torch.autograd.grad(y, leaves, dy)
+    _check_norm_gradients(got, _norm_gradients(h.detach(), w.detach(), dy, dh if both else None, eps), dtype, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 2048, 16384])
+@pytest.mark.parametrize("size,eps", [(1e-14, 1e-32), (1.0, 1e-5), (1e14, 1e-5), (1e16, 1e-5)])
+def test_plain_norm_gradients_of_rows_of_unusual_size(size, eps, D, dtype):
+    g = _gen(D)
+    x, dy = _randn(19, D, gen=g, dtype=dtype, scale=size), _randn(19, D, gen=g, dtype=dtype)
+    w = (1 + 0.1 * torch.randn(D, device="cuda", generator=g)).to(dtype)
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    got = torch.autograd.grad(ops.rms_norm(x, w, eps)[0], leaves, dy)
+    _check_norm_gradients(got, _norm_gradients(x.detach(), w.detach(), dy, None, eps), dtype, dtype)
