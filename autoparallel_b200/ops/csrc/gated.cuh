@@ -55,7 +55,7 @@ __device__ __forceinline__ float act_value(float a, float& d) {
   if (ACT == ACT_GELU_TANH) {
     const float a2 = a * a;
     u = 1.59576912f * a * fmaf(0.044715f, a2, 1.f);
-    du = fmaf(0.21406820f, a2, 1.59576912f);
+    du = fmaf(0.21406445f, a2, 1.59576912f);
   }
   const float s = __fdividef(1.f, 1.f + __expf(-u));
   const float v = a * s;

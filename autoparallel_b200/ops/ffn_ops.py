@@ -136,7 +136,7 @@ def _act(act: int, a):
         s = torch.sigmoid(a)
         return a * s, s * (1 + a * (1 - s))
     s = torch.sigmoid(1.5957691216057308 * a * (1 + 0.044715 * a * a))
-    return a * s, s + a * s * (1 - s) * (1.5957691216057308 + 0.21406820245 * a * a)
+    return a * s, s + a * s * (1 - s) * (1.5957691216057308 + 0.21406444881780073 * a * a)
 
 
 def _kept(ab, bits, dtype):

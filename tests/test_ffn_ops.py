@@ -636,3 +636,19 @@ for d in (64, 63, 32768):
     print(so.apb_add_rms_norm_bwd(p, p, p, p, p, p, p, p, LL(4), d, 1, 148, N, N), so.apb_add_rms_norm_bwd(p, N, p, p, p, p, p, p, LL(4), d, 1, 148, N, N))
 """)
     assert out == ["3"] * 6, out
+
+
+@pytest.mark.parametrize("act", sorted(ACTS))
+def test_activations_against_64_bits(act):
+    """Value and derivative of the formulas, relative to their terms, at single values (a sum over a tensor hides 1e-5 of one)."""
+    a = torch.linspace(-9, 9, 2001)
+    d = a.double().requires_grad_()
+    s = {"silu": lambda t: torch.sigmoid(t), "gelu": lambda t: 0.5 * torch.erfc(-t * 0.5**0.5),
+         "gelu_tanh": lambda t: torch.sigmoid(2 * (2 / math.pi) ** 0.5 * (t + 0.044715 * t**3))}[act](d)
+    (dv,) = torch.autograd.grad((d * s).sum(), d)
+    s, d = s.detach(), d.detach()
+    # a few roundings, and those of an exponential's argument, which are that much of the value: |u| of gelu_tanh, a^2 / 2 and a constant of gelu
+    tol = (32 + 5 * {"silu": d.abs(), "gelu": d.square(), "gelu_tanh": (1.6 * d * (1 + 0.044715 * d * d)).abs()}[act]) * 2.0**-24
+    v, slope = FFN._act(FFN.ACTS[act], a)
+    assert bool(((v.double() - d * s).abs() <= tol * (d * s).abs()).all())
+    assert bool(((slope.double() - dv).abs() <= tol * (s + (dv - s).abs())).all())
