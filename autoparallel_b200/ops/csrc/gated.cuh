@@ -34,12 +34,13 @@ __device__ __forceinline__ float normal_tail(float x) {
 }
 
 // act(a), and its derivative in ``d``, relative to the value: x / (1 + exp(-x)) keeps its digits where 1 + tanh would cancel, and a tail of the normal
-// distribution those that 1 + erf would lose.  FINE: for fp32 results, to their precision.  By the error function, 8192 x 4096 x 14336 backward: 988 us
+// distribution those that 1 + erf would lose.  FINE: for fp32 results, by expf, erfcf and a true division, to a few units in the last place and what the rounding of
+// an exponential's argument makes of it (the short forms: 2 + 1.2 |u| units for exp(u), some 70 of silu(-60)).  By the error function, 8192 x 4096 x 14336 backward: 988 us
 // with erfc, 708 so (one of the sigmoids 708).
 template <int ACT, bool FINE = false>
 __device__ __forceinline__ float act_value(float a, float& d) {
   if (ACT == ACT_GELU) {
-    const float e = __expf(-0.5f * a * a);
+    const float e = FINE ? expf(-0.5f * a * a) : __expf(-0.5f * a * a);
     float phi;
     if (FINE) {
       phi = 0.5f * erfcf(-0.70710678f * a);
@@ -57,7 +58,7 @@ __device__ __forceinline__ float act_value(float a, float& d) {
     u = 1.59576912f * a * fmaf(0.044715f, a2, 1.f);
     du = fmaf(0.21406445f, a2, 1.59576912f);
   }
-  const float s = __fdividef(1.f, 1.f + __expf(-u));
+  const float s = FINE ? __fdiv_rn(1.f, 1.f + expf(-u)) : __fdividef(1.f, 1.f + __expf(-u));
   const float v = a * s;
   d = fmaf(v * (1.f - s), du, s);
   return v;

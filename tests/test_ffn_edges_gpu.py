@@ -209,3 +209,30 @@ def test_plain_norm_gradients_of_rows_of_unusual_size(size, eps, D, dtype):
     leaves = [x.requires_grad_(), w.requires_grad_()]
     got = torch.autograd.grad(ops.rms_norm(x, w, eps)[0], leaves, dy)
     _check_norm_gradients(got, _norm_gradients(x.detach(), w.detach(), dy, None, eps), dtype, dtype)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_fp32_activation_relative_to_the_value(act):
+    """fp32 operands: the activation and its derivative to a few roundings of the value, far out on the negative side too."""
+    a = torch.linspace(-60 if act == "silu" else -9.9, 10, 4001, device="cuda").unsqueeze(1)
+    one = torch.ones(1, 1, device="cuda")
+    # (in forms that keep their digits: 1 + erf and 1 + tanh are zero in 64 bits from -8.3 and 2 u = -37 on)
+    d = a.double().requires_grad_()
+    s = {"silu": lambda t: torch.sigmoid(t), "gelu": lambda t: 0.5 * torch.erfc(-t * 0.5**0.5),
+         "gelu_tanh": lambda t: torch.sigmoid(2 * (2 / math.pi) ** 0.5 * (t + 0.044715 * t**3))}[act](d)
+    v = d * s
+    (dv,) = torch.autograd.grad(v.sum(), d)
+    s, v, d = s.detach(), v.detach(), d.detach()
+    # The argument of the exponential is off by a few of its own roundings, which is that much of the value: none for silu, |u| for gelu_tanh, a^2 / 2 and the
+    # constant in erfc's argument for gelu.  Functions: erfc to 4 units in the last place (2^-23 each), exp to 2, sums and products to a half.
+    u = {"silu": 0 * d, "gelu": d.square(), "gelu_tanh": 1.5957691216 * d * (1 + 0.044715 * d * d)}[act].abs()
+    tol = (16 + 5 * u) * 2.0**-24
+    h, ab, _ = ops.gated_mm(a, one, one, FFN.ACTS[act], 16)
+    assert torch.equal(ab[:, 0], a)
+    assert bool(((h.double() - v * d).abs() <= (tol + 2.0**-24) * (v * d).abs()).all()), float(((h.double() - v * d).abs() / (v * d).abs().clamp_min(1e-300)).max())
+    ab = torch.stack((a, torch.ones_like(a)), 1)
+    dab, h = ops.gated_dgrad(torch.ones_like(a), one, ab, torch.empty(0, dtype=torch.uint8, device="cuda"), FFN.ACTS[act])
+    assert bool(((h.double() - v).abs() <= tol * v.abs()).all()) and torch.equal(dab[:, 1], h)
+    # the derivative is a sum that cancels: relative to its terms, both of which carry the same exponential
+    terms = s + (dv - s).abs()
+    assert bool(((dab[:, 0].double() - dv).abs() <= (tol + 8 * 2.0**-24) * terms).all()), float(((dab[:, 0].double() - dv).abs() / terms).max())
