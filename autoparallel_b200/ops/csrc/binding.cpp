@@ -86,7 +86,7 @@ int apb_add_rms_norm(const void* x, const void* res, const void* w, void* h, voi
                      int is_bf16, cudaStream_t st);
 long long apb_add_rms_norm_bwd_workspace(long long rows, int D, int is_bf16, int num_sms);
 int apb_add_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dw, float* part, long long rows,
-                         int D, int is_bf16, int num_sms, cudaStream_t st, uint32_t* status);
+                         int D, int is_bf16, int num_sms, cudaStream_t st, uint32_t* status, int dw_fp32);
 int apb_mx8_quantize(const void* x, void* codes, void* scales, long long R, long long K, int is_bf16, cudaStream_t st);
 int apb_mx8_dequantize(const void* codes, const void* scales, void* y, long long R, long long K, int is_bf16, cudaStream_t st);
 int apb_gated_act(const float* ab, void* h, long long M, int H, int act, int is_bf16, cudaStream_t st);

@@ -53,20 +53,22 @@ Five add_rms_norm_fp8(const Tensor& x, const c10::optional<Tensor>& residual, co
   return {y, h, rstd, q, scale};
 }
 // Without ``dh`` (h is not used further on, or there is no residual) it is the plain norm's gradient: that kernel's, two operands instead of three, for the widths it
-// takes (those of its forward pass); this one's for the others.
+// takes (those of its forward pass) and weights of the operands' type; this one's for the others.
 Two add_rms_norm_bwd(const Tensor& dy_, const c10::optional<Tensor>& dh_, const Tensor& h_, const Tensor& weight, const Tensor& rstd_) {
   c10::cuda::CUDAGuard g(h_.device());
   const NormArgs a("add_rms_norm_bwd", h_, c10::nullopt, weight);
   for (const Tensor* t : {&dy_, dh_.has_value() ? &*dh_ : &dy_})
     TORCH_CHECK(t->sizes() == h_.sizes() && t->scalar_type() == h_.scalar_type() && t->device() == h_.device(), "add_rms_norm_bwd: gradients like h");
   TORCH_CHECK(rstd_.scalar_type() == at::kFloat && rstd_.numel() == a.rows && rstd_.device() == h_.device(), "add_rms_norm_bwd: rstd fp32, one a row");
-  Tensor dx = at::empty_like(a.x), dw = at::empty({a.D}, a.x.options());
+  // (a weight in fp32 beside bf16 operands is taken in their type, as the plain norm takes it; its gradient is not rounded to that)
+  const bool wide = weight.scalar_type() == at::kFloat;
+  Tensor dx = at::empty_like(a.x), dw = at::empty({a.D}, wide ? weight.options() : a.x.options());
   if (a.rows == 0) return {dx, dw.zero_().to(weight.scalar_type())};
-  if (!dh_.has_value() && a.D % 8 == 0 && a.D <= 16384) return op_rms_norm_bwd(dy_, h_, weight, rstd_);
+  if (!dh_.has_value() && a.D % 8 == 0 && a.D <= 16384 && weight.scalar_type() == a.x.scalar_type()) return op_rms_norm_bwd(dy_, h_, weight, rstd_);
   Tensor dy = dense(dy_), dh = dh_.has_value() ? dense(*dh_) : Tensor(), rstd = rstd_.contiguous();
   Tensor part = at::empty({(int64_t)apb_add_rms_norm_bwd_workspace(a.rows, (int)a.D, is_bf16(a.x), num_sms())}, rstd.options());  // partial sums of dw
   check(apb_add_rms_norm_bwd(dy.data_ptr(), dh.defined() ? dh.data_ptr() : nullptr, a.x.data_ptr(), a.w.data_ptr(), rstd.data_ptr<float>(), dx.data_ptr(), dw.data_ptr(),
-                             part.data_ptr<float>(), a.rows, (int)a.D, is_bf16(a.x), num_sms(), stream(), status_word(a.x)),
+                             part.data_ptr<float>(), a.rows, (int)a.D, is_bf16(a.x), num_sms(), stream(), status_word(a.x), wide),
         "apb_add_rms_norm_bwd");
   count(2);
   return {dx, dw.to(weight.scalar_type())};

@@ -493,7 +493,7 @@ static cudaError_t launch_fwd(const void* x, const void* res, const void* w, con
 
 template <typename T, bool EVEN>
 static cudaError_t launch_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dw, float* part,
-                              long long rows, int D, int num_sms, cudaStream_t st, uint32_t* status) {
+                              long long rows, int D, int num_sms, cudaStream_t st, uint32_t* status, int dw_fp32) {
   const BwdPlan p = bwd_plan(rows, D, (int)sizeof(T), num_sms);
   auto launch = [&](auto kern, auto... more) {
     if (p.smem && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem) != cudaSuccess) return cudaErrorInvalidValue;
@@ -520,7 +520,9 @@ static cudaError_t launch_bwd(const void* dy, const void* dh, const void* h, con
   }
 #undef APB_RING
   if (e != cudaSuccess) return e;
-  return launch_after(rms_dw_kernel<T>, (unsigned)((D + 31) / 32), 1024, 0, st, (const float*)part, (T*)dw, p.grid, D);
+  const unsigned grid = (unsigned)((D + 31) / 32);
+  if (dw_fp32) return launch_after(rms_dw_kernel<float>, grid, 1024, 0, st, (const float*)part, (float*)dw, p.grid, D);
+  return launch_after(rms_dw_kernel<T>, grid, 1024, 0, st, (const float*)part, (T*)dw, p.grid, D);
 }
 
 }  // namespace apb
@@ -547,16 +549,17 @@ extern "C" int apb_add_rms_norm(const void* x, const void* res, const void* w, v
 extern "C" long long apb_add_rms_norm_bwd_workspace(long long rows, int D, int is_bf16, int num_sms) {
   return rows <= 0 || D <= 0 ? 0 : (long long)bwd_plan(rows, D, is_bf16 ? 2 : 4, num_sms).grid * D;
 }
-// ``status``: a word of device memory, which a wait that runs out is recorded in
+// ``status``: a word of device memory, which a wait that runs out is recorded in.  ``dw_fp32``: dw in fp32 (its sums as they are), else in the operands' type.
 extern "C" int apb_add_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dw, float* part,
-                                    long long rows, int D, int is_bf16, int num_sms, cudaStream_t st, uint32_t* status) {
+                                    long long rows, int D, int is_bf16, int num_sms, cudaStream_t st, uint32_t* status,
+                                    int dw_fp32) {
   if (rows <= 0 || D <= 0 || D > ADD_NORM_MAX || status == nullptr) return 3;
   for (const void* p : {dy, dh, h, w, (const void*)dx})
     if (off16(p)) return 3;
   auto go = [&](auto even) {
     constexpr bool E = decltype(even)::value;
-    return is_bf16 ? launch_bwd<bf16, E>(dy, dh, h, w, rstd, dx, dw, part, rows, D, num_sms, st, status)
-                   : launch_bwd<float, E>(dy, dh, h, w, rstd, dx, dw, part, rows, D, num_sms, st, status);
+    return is_bf16 ? launch_bwd<bf16, E>(dy, dh, h, w, rstd, dx, dw, part, rows, D, num_sms, st, status, dw_fp32)
+                   : launch_bwd<float, E>(dy, dh, h, w, rstd, dx, dw, part, rows, D, num_sms, st, status, dw_fp32);
   };
   const cudaError_t e = D % 8 == 0 ? go(std::true_type{}) : go(std::false_type{});
   return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : 4;

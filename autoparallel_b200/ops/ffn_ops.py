@@ -299,7 +299,8 @@ def _check_norm(name, x, residual, weight):
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor]:
     """``h = x + residual``, rounded to their type, and ``rms_norm(h, weight)``: (norm, h).  Gradients of both results reach x, the
-    residual and the weight in one pass."""
+    residual and the weight in one pass.  (On CUDA a weight in fp32 beside bf16 operands is taken in bf16, as ``rms_norm`` takes it; its
+    gradient is fp32.)"""
     xs = x.shape
     if not (x.dtype in _FLOATS and xs and 1 <= xs[-1] <= 32768 and residual.shape == xs and residual.dtype is x.dtype
             and weight.shape == xs[-1:] and weight.dtype in _FLOATS and x.device == residual.device == weight.device):

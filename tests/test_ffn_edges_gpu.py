@@ -236,3 +236,18 @@ def test_fp32_activation_relative_to_the_value(act):
     # the derivative is a sum that cancels: relative to its terms, both of which carry the same exponential
     terms = s + (dv - s).abs()
     assert bool(((dab[:, 0].double() - dv).abs() <= (tol + 8 * 2.0**-24) * terms).all()), float(((dab[:, 0].double() - dv).abs() / terms).max())
+
+
+@pytest.mark.parametrize("form,both", [("norm", True), ("norm", False), ("fp8", True), ("fp8", False), ("fp8 of x alone", False)])
+@pytest.mark.parametrize("D", [64, 1001, 4096, 32768])
+def test_gradient_of_an_fp32_weight_beside_bf16_operands(D, form, both):
+    """It is summed in fp32 and not rounded to the operands' type."""
+    g = _gen(D)
+    x, r, dy, dh = (_randn(300, D, gen=g) for _ in range(4))
+    w = 1 + 0.1 * torch.randn(D, device="cuda", generator=g)
+    alone = form == "fp8 of x alone"
+    leaves = [t.requires_grad_() for t in ((x, w) if alone else (x, r, w))]
+    out = K.add_rms_norm(*leaves) if form == "norm" else K.add_rms_norm_fp8(x, None if alone else r, w)
+    got = torch.autograd.grad(out[:2], leaves, (dy, dh)) if both else torch.autograd.grad(out[0], leaves, dy)
+    # (the weight itself is taken in the operands' type, as ``rms_norm`` takes it)
+    _check_norm_gradients(got, _norm_gradients(x.detach() if alone else out[1].detach(), w.detach().to(BF), dy, dh if both else None, 1e-5), BF, F32)

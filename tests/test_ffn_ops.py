@@ -633,7 +633,7 @@ def test_norm_gradient_entry_needs_a_status_word():
     out = _entries("""
 p = V(1 << 20)  # (never read)
 for d in (64, 63, 32768):
-    print(so.apb_add_rms_norm_bwd(p, p, p, p, p, p, p, p, LL(4), d, 1, 148, N, N), so.apb_add_rms_norm_bwd(p, N, p, p, p, p, p, p, LL(4), d, 1, 148, N, N))
+    print(so.apb_add_rms_norm_bwd(p, p, p, p, p, p, p, p, LL(4), d, 1, 148, N, N, 0), so.apb_add_rms_norm_bwd(p, N, p, p, p, p, p, p, LL(4), d, 1, 148, N, N, 0))
 """)
     assert out == ["3"] * 6, out
 
