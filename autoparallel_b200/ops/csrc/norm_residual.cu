@@ -106,8 +106,10 @@ __device__ __forceinline__ float block_sum_top(float v, uint32_t& top, float* re
 // A warp (WARP_ROWS) or a block has a row, each thread up to NP vectors.
 // In 8 bits 1 / rms cancels: with m = max |h w|, y / (max |y| / 448) = h w 448 / m, where h w of two bf16 is exact in fp32.  So q takes one rounded factor, is
 // nearer to the formula than y / s would be (a third of the values that round the other way), and m is found in the same reduction as the sum of squares.
+// Where h w or 448 / m may be no fp32 number (m below 2^-100, zeros among them, infinite or NaN) the row is gone through once more, with h r w.
+// (Four blocks of eight warps to an SM where the compiler would take a few registers too many for them.)
 template <typename T, bool EVEN, int NP, bool WARP_ROWS, bool FP8>
-__global__ void __launch_bounds__(WARP_ROWS ? 256 : 1024) add_rms_norm_kernel(const T* x, const T* res, const T* w, const AddNormOut o, long long rows, int D,
+__global__ void __launch_bounds__(WARP_ROWS ? 256 : 1024, FP8 && WARP_ROWS && sizeof(T) == 2 && NP <= (EVEN ? 2 : 1) ? 4 : 0) add_rms_norm_kernel(const T* x, const T* res, const T* w, const AddNormOut o, long long rows, int D,
                                                                               float eps) {
   after_previous();
   __shared__ float red[32];
@@ -165,11 +167,48 @@ __global__ void __launch_bounds__(WARP_ROWS ? 256 : 1024) add_rms_norm_kernel(co
     const float r = rsqrtf(ss / D + eps);
     if (t == 0) o.rstd[row] = r;
     float k = 0.f;  // q = h w k
+    bool coded = !FP8;
     if (FP8) {
-      const float m = __uint_as_float(top), r8 = __frsqrt_rn(__fdiv_rn(ss, (float)D) + eps), amax = m * r8;
-      const bool tiny = amax < 0x1p-100f;
-      k = tiny ? r8 : __fdiv_rn(448.f, m);
-      if (t == 0) o.scale[row] = tiny ? 1.f : __fdiv_rn(amax, 448.f);
+      const float m = __uint_as_float(top), r8 = __frsqrt_rn(__fdiv_rn(ss, (float)D) + eps);
+      if (m >= 0x1p-100f && m < INFINITY) {
+        const float amax = m * r8;
+        const bool tiny = amax < 0x1p-100f;
+        k = tiny ? r8 : __fdiv_rn(448.f, m);
+        if (t == 0) o.scale[row] = tiny ? 1.f : __fdiv_rn(amax, 448.f);
+      } else {  // (all threads of the row; apart from the others, whom a factor more would cost registers: 8192 x 2048 codes only 27.7 -> 31 us)
+        coded = true;
+        top = 0;
+        auto each = [&](auto use) {
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            const int c = at.col(t + j * tpr);
+            if (c < D) {
+              float f[8], g[8];
+              v[j].to_float(f);
+              at.mask(f, c);
+              at.weight(g, w, c);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] = f[i] * r8 * g[i];
+              use(f, c);
+            }
+          }
+        };
+        each([&](const float (&f)[8], int) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+        });
+        if (WARP_ROWS) top = __reduce_max_sync(0xffffffffu, top);
+        else block_sum_top(0.f, top, red, red_top);
+        const float amax = __uint_as_float(top);
+        const bool tiny = amax < 0x1p-100f;
+        k = tiny ? 1.f : __fdiv_rn(448.f, amax);
+        each([&](float (&f)[8], int c) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] *= k;
+          at.store_e4m3(f, o.q, c);
+        });
+        if (t == 0) o.scale[row] = tiny ? 1.f : __fdiv_rn(amax, 448.f);
+      }
     }
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
@@ -178,7 +217,7 @@ __global__ void __launch_bounds__(WARP_ROWS ? 256 : 1024) add_rms_norm_kernel(co
         float f[8], g[8];
         v[j].to_float(f);
         at.weight(g, w, c);
-        if (FP8) {
+        if (!coded) {
           float q[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) q[i] = f[i] * g[i] * k;

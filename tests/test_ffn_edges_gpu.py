@@ -251,3 +251,24 @@ def test_gradient_of_an_fp32_weight_beside_bf16_operands(D, form, both):
     got = torch.autograd.grad(out[:2], leaves, (dy, dh)) if both else torch.autograd.grad(out[0], leaves, dy)
     # (the weight itself is taken in the operands' type, as ``rms_norm`` takes it)
     _check_norm_gradients(got, _norm_gradients(x.detach() if alone else out[1].detach(), w.detach().to(BF), dy, dh if both else None, 1e-5), BF, F32)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [200, 1001, 4096, 32768])
+@pytest.mark.parametrize("size,weight,eps", [(2.0**-55, 2.0**-65, 2e-38), (2.0**-55, 2.0**-80, 2e-38), (2.0**50, 2.0**80, 1e-5), (2.0**-20, 2.0**-100, 1e-30), (1.0, 2.0**-120, 1e-5)])
+def test_8_bit_norm_of_products_outside_of_the_range(D, size, weight, eps, dtype):
+    """h w or 448 / max |h w| are no fp32 numbers, the norm and its scale are."""
+    g = _gen(D)
+    x = _randn(9, D, gen=g, dtype=dtype, scale=size)
+    x[4] = 0
+    w = (weight * (1 + 0.1 * torch.randn(D, device="cuda", generator=g))).to(dtype)
+    for keep in (False, True):
+        y, h, q, scale = K.add_rms_norm_fp8(x, None, w, eps, keep)
+        yd = x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + eps) * w.double()
+        top = yd.abs().amax(-1, keepdim=True)
+        want = torch.where(top < 2.0**-100, 1.0, top / 448)
+        assert bool(((scale.double() - want).abs() <= ARITHMETIC * want).all())
+        err = (q.double() * scale.double() - yd).abs()
+        assert bool((err <= (1 + 2.0**-14) * torch.maximum(yd.abs() * 2.0**-4, scale.double() * 2.0**-10)).all())
+        if keep:
+            assert torch.equal(y, K.add_rms_norm(x, torch.zeros_like(x), w, eps)[0])
