@@ -102,16 +102,11 @@ struct RmsDw {
   }
 };
 
-// The gradient's second term, x r^3 (sum g w x) / D.  Rows whose r^3 may leave fp32's range take the factors one by one (the others keep their bits).
-struct RmsTerm {
-  float s, c;
-  __device__ __forceinline__ RmsTerm(float r, float dot, float inv_d) {
-    const bool plain = r > 0x1p-40f && r < 0x1p40f;
-    s = plain ? 1.f : r;
-    c = plain ? r * r * r * dot * inv_d : r * (r * dot * inv_d);
-  }
-  __device__ __forceinline__ float of(float x) const { return (x * s) * c; }
-};
+// The factor of x in the gradient's second term, r^3 (sum g w x) / D.  Rows whose r^3 may leave fp32's range take the factors one by one, which reaches to within about 3
+// times the rms at which the forward pass's sum of squares leaves it; the others keep their bits.
+__device__ __forceinline__ float rms_term(float r, float dot, float inv_d) {
+  return r > 0x1p-40f && r < 0x1p40f ? r * r * r * dot * inv_d : r * (r * (r * dot * inv_d));
+}
 
 // Backward.  One persistent block per SM (a single wave).  Every iteration takes ROWS rows at once and the loads of
 // the next iteration are issued before the current one is reduced and stored (two register sets that swap roles, so
@@ -190,14 +185,14 @@ __global__ void __launch_bounds__(512, 1) rms_norm_bwd_kernel(const T* dy, const
       const long long row = row0 + k;
       const bool row_ok = EXACT || row < rows;
       const float r = rs[k];
-      const RmsTerm c(r, dot[k], inv_d);
+      const float c = rms_term(r, dot[k], inv_d);
       T* dr = dx + row * D;
 #pragma unroll
       for (int j = 0; j < NVEC; ++j) {
         if (row_ok && (EXACT || col[j] < D)) {
           float xf[8], gf[8], o[8]; xs[k][j].to_float(xf); gs[k][j].to_float(gf);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = fmaf(gf[i], r * wreg[j][i], -c.of(xf[i]));
+          for (int i = 0; i < 8; ++i) o[i] = fmaf(gf[i], r * wreg[j][i], -xf[i] * c);
           Vec8<T> ov; ov.from_float(o); ov.store(dr + col[j]);
         }
       }
@@ -314,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, NVEC == 2 && THREADS == 512 ? 2 : 1) 
     }
     if (*abort_flag) break;  // (set before the barrier, so every thread leaves here)
     if (threadIdx.x == 0) issue(it + RMS_STAGES - 1);
-    const RmsTerm c(r, dot, inv_d);
+    const float c = rms_term(r, dot, inv_d);
 #pragma unroll
     for (int j = 0; j < NVEC; ++j) {
       if (col[j] < D) {
@@ -326,7 +321,7 @@ __global__ void __launch_bounds__(THREADS, NVEC == 2 && THREADS == 512 ? 2 : 1) 
         }
         float xf[8], gf[8], wf[8], o[8]; xv.to_float(xf); gv.to_float(gf); wv[j].to_float(wf);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = fmaf(gf[i], r * wf[i], -c.of(xf[i]));
+        for (int i = 0; i < 8; ++i) o[i] = fmaf(gf[i], r * wf[i], -xf[i] * c);
         Vec8<T> ov; ov.from_float(o); ov.store(dx + row * D + col[j]);
       }
     }
