@@ -652,3 +652,33 @@ def test_activations_against_64_bits(act):
     v, slope = FFN._act(FFN.ACTS[act], a)
     assert bool(((v.double() - d * s).abs() <= tol * (d * s).abs()).all())
     assert bool(((slope.double() - dv).abs() <= tol * (s + (dv - s).abs())).all())
+
+
+@pytest.mark.parametrize("bits", [8, 11, 16])
+def test_splits_of_bf16_codes_compute_the_same(bits):
+    """The hidden dim in whole blocks: codes and scales of the parts are parts of the whole's, and so is what is made of them."""
+    g = _gen(18)
+    x, w1, w3, w2 = (_randn(*s, dtype=torch.bfloat16, gen=g) for s in ((4, 6, 24), (128, 24), (128, 24), (16, 128)))
+    dy = _randn(4, 6, 16, dtype=torch.bfloat16, gen=g)
+    h, ab, scales = ops.gated_mm(x, w1, w3, 1, bits)
+    parts = [ops.gated_mm(x, a, b, 1, bits) for a, b in zip(w1.chunk(2), w3.chunk(2))]
+    for i, whole in enumerate((h, ab, scales)):
+        assert torch.equal(torch.cat([p[i] for p in parts], -1), whole)
+    dab, h = ops.gated_dgrad(dy, w2, ab, scales, 1)
+    halves = [ops.gated_dgrad(dy, c, p[1], p[2], 1) for c, p in zip(w2.chunk(2, 1), parts)]
+    # (dh is a product of its own in the parts: a sum of 16 terms in another order, then a rounding to bf16 that may fall the other way)
+    for i, whole in enumerate((dab, h)):
+        part = torch.cat([p[i] for p in halves], -1).float()
+        assert bool(((part - whole.float()).abs() <= 2.0**-7 * whole.float().abs() + 2.0**-20).all())
+
+
+def test_rules_of_fp16_numbers(mesh_1d):
+    from torch.distributed.tensor.placement_types import Partial, Replicate, Shard
+
+    S, R, P = Shard, Replicate(), Partial()
+    for hidden, split in ((256, True), (128, False)):  # 32 and 16 columns a rank
+        x, w1, w2 = torch.randn(8, 16, 64).bfloat16(), torch.randn(hidden, 64).bfloat16(), torch.randn(64, hidden).bfloat16()
+        rows = _rows(mesh_1d, "gated_ffn", x, w1, w1, w2, 0, 11)
+        assert ((P, S(3), S(3), R, R, R, S(0), S(0), S(1)) in rows) == split and (S(0), S(0), S(0), R, R, S(0), R, R, R) in rows
+        _, ab, scales = ops.gated_mm(x, w1, w1, 0, 11)
+        assert ((S(3), S(2), R, S(1), S(3), S(3)) in _rows(mesh_1d, "gated_dgrad", x, w2, ab, scales, 0)) == split
