@@ -495,7 +495,7 @@ static BwdPlan bwd_plan(long long rows, int D, int elem, int num_sms) {
     per_sm = by_smem < 1 ? 1 : by_smem < by_threads ? by_smem : by_threads;
     // Shared memory that one block more would not find: where registers leave room for it, the blocks that come early (launch.cuh) gather on a few SMs (8192 x 2048
     // bf16 33 -> 27 us, x 1024 18 -> 16).  Not for rows that begin anywhere, whose weights are read one by one through what is left as cache (8192 x 249 13.2 -> 15.1).
-    const int alone = 228 * 1024 / (per_sm + 1);
+    const int alone = 228 * 1024 / (per_sm + 1) - 1024;
     if (D % 8 == 0 && p.smem < alone && alone <= room) p.smem = alone;
   } else {
     p.threads = 1024;
