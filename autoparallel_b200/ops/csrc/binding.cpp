@@ -36,7 +36,7 @@ int apb_rms_norm_fwd(const void* x, const void* w, void* y, float* rstd, long lo
                      cudaStream_t st);
 long long apb_rms_norm_bwd_workspace(long long rows, int D, int is_bf16, int num_sms);
 int apb_rms_norm_bwd(const void* dy, const void* x, const void* w, const float* rstd, void* dx, void* dw, float* part,
-                     long long rows, int D, int is_bf16, int num_sms, cudaStream_t st);
+                     long long rows, int D, int is_bf16, int num_sms, cudaStream_t st, uint32_t* status);
 int apb_cast(const void* src, void* dst, long long n, int src_bf16, int dst_bf16, int num_sms, cudaStream_t st);
 int apb_cast_many(const void* const* src, void* const* dst, const long long* n, int count, int* launches, cudaStream_t st);
 int apb_rope(const void* x, const float* cs, const float* sn, void* y, long long B, int S, int H, int D, int conj, int is_bf16,
@@ -240,6 +240,8 @@ void rms_norm_fwd(const at::Tensor& x, const at::Tensor& w, at::Tensor& y, at::T
         "apb_rms_norm_fwd");
 }
 
+at::Tensor& status_of(const at::Tensor& t);
+
 void rms_norm_bwd(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, const at::Tensor& rstd, at::Tensor& dx,
                   at::Tensor& dw) {
   c10::cuda::CUDAGuard g(x.device());
@@ -248,7 +250,7 @@ void rms_norm_bwd(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w
   const bool bf16 = is_bf16(x);
   at::Tensor part = at::empty({(int64_t)apb_rms_norm_bwd_workspace(rows, D, bf16, num_sms())}, rstd.options());  // partial sums of dw
   check(apb_rms_norm_bwd(dy.data_ptr(), x.data_ptr(), w.data_ptr(), rstd.data_ptr<float>(), dx.data_ptr(), dw.data_ptr(),
-                         part.data_ptr<float>(), rows, D, bf16, num_sms(), stream()),
+                         part.data_ptr<float>(), rows, D, bf16, num_sms(), stream(), reinterpret_cast<uint32_t*>(status_of(x).data_ptr())),
         "apb_rms_norm_bwd");
 }
 

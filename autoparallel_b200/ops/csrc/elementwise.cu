@@ -224,12 +224,12 @@ __global__ void __launch_bounds__(512, 1) rms_norm_bwd_kernel(const T* dy, const
 // cast) 59 -> 36, 24 -> 11, 24 -> 14.
 // One block barrier per step: the partial sums of consecutive steps sit in alternating slots, and a stage is refilled
 // after the barrier of the following step, which every thread reaches only when it has read the stage for the last time.
-// Waits are bounded: if a stage never arrives the block stops (its rows keep whatever dx held).
+// Waits are bounded: if a stage never arrives the block records that in ``status`` (where there is one) and stops, when its copies under way have ended.
 constexpr int RMS_STAGES = 3;
 __host__ __device__ inline int rms_ring_bytes(int row_bytes) { return RMS_STAGES * 2 * row_bytes + 128; }
 template <typename T, int NVEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, NVEC == 2 && THREADS == 512 ? 2 : 1) rms_norm_bwd_bulk_kernel(const T* dy, const T* x,
-                                                                    const T* w, const float* rstd, T* dx, RmsDw dw, long long rows, int D) {
+                                                                    const T* w, const float* rstd, T* dx, RmsDw dw, long long rows, int D, uint32_t* status) {
   extern __shared__ uint8_t rms_smem_raw[];
   __shared__ uint64_t bars[RMS_STAGES];
   __shared__ float red[2][THREADS / 32];
@@ -276,7 +276,10 @@ __global__ void __launch_bounds__(THREADS, NVEC == 2 && THREADS == 512 ? 2 : 1) 
     const int st = (int)(it % RMS_STAGES);
     const float r = r_next;
     if (row + step < rows) r_next = rstd[row + step];
-    if (!mbar_wait(&bars[st], (uint32_t)((it / RMS_STAGES) & 1), abort_flag)) *abort_flag = 1;
+    if (!mbar_wait(&bars[st], (uint32_t)((it / RMS_STAGES) & 1), abort_flag)) {
+      if (status != nullptr) atomicCAS(status, 0u, (uint32_t)ST_TIMEOUT_FULL);
+      *abort_flag = 1;
+    }
     const T* xs = reinterpret_cast<const T*>(smem + (2 * st) * row_bytes);
     const T* gs = reinterpret_cast<const T*>(smem + (2 * st + 1) * row_bytes);
     Vec8<T> xk[KEEP ? NVEC : 1], gk[KEEP ? NVEC : 1];
@@ -307,7 +310,12 @@ __global__ void __launch_bounds__(THREADS, NVEC == 2 && THREADS == 512 ? 2 : 1) 
     } else {
       __syncwarp();
     }
-    if (*abort_flag) break;  // (set before the barrier, so every thread leaves here)
+    if (*abort_flag) {  // (set before the barrier, so every thread leaves here)
+      volatile uint32_t none = 0;
+      for (long long k = it; threadIdx.x == 0 && k < it + RMS_STAGES - 1 && first + k * step < rows; ++k)
+        mbar_wait(&bars[k % RMS_STAGES], (uint32_t)((k / RMS_STAGES) & 1), &none);
+      break;
+    }
     if (threadIdx.x == 0) issue(it + RMS_STAGES - 1);
     const float c = rms_term(r, dot, inv_d);
 #pragma unroll
@@ -663,7 +671,7 @@ static inline int rms_grid_shared(long long rows, int D, int num_sms, int per_sm
 // Launches the row kernel; returns the number of partial rows of dw (its blocks, or ``shared``), < 0 on error.
 template <typename T>
 static inline int launch_rms_norm_bwd(const void* dy, const void* x, const void* w, const float* rstd, void* dx, float* dw_base,
-                                      int shared, long long rows, int D, int num_sms, cudaStream_t st) {
+                                      int shared, long long rows, int D, int num_sms, cudaStream_t st, uint32_t* status) {
   const RmsDw dw{dw_base, D, shared};
   if (rms_bulk(D, (int)sizeof(T))) {
     const int smem = rms_ring_bytes(D * (int)sizeof(T));
@@ -673,7 +681,7 @@ static inline int launch_rms_norm_bwd(const void* dy, const void* x, const void*
   if (plan.nvec == NV && plan.threads == TH) {                                                                           \
     auto kern = rms_norm_bwd_bulk_kernel<T, NV, TH>;                                                                     \
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -4;         \
-    launch_after(kern, grid, TH, smem, st, (const T*)dy, (const T*)x, (const T*)w, rstd, (T*)dx, dw, rows, D);                     \
+    launch_after(kern, grid, TH, smem, st, (const T*)dy, (const T*)x, (const T*)w, rstd, (T*)dx, dw, rows, D, status);             \
     return shared ? shared : grid;                                                                                       \
   }
     APB_RMS_BULK(1, 32)
@@ -766,14 +774,15 @@ long long apb_rms_norm_bwd_workspace(long long rows, int D, int is_bf16, int num
   return (long long)rms_grid(rows, num_sms, rms_plan(D, is_bf16 ? 2 : 4).per_sm) * D;
 }
 
+// ``status``: the word that a wait which runs out is recorded in
 int apb_rms_norm_bwd(const void* dy, const void* x, const void* w, const float* rstd, void* dx, void* dw, float* part,
-                     long long rows, int D, int is_bf16, int num_sms, cudaStream_t st) {
+                     long long rows, int D, int is_bf16, int num_sms, cudaStream_t st, uint32_t* status) {
   if (!aligned16(dy, x, w, dx, part)) return 3;
   if (D % 8) return 3;
   if (D > 512 * 8 * RMS_BWD_MAX_VEC) return 3;
   int n = 0;
   if (rows > 0) {
-    DISPATCH(is_bf16, n = launch_rms_norm_bwd<T>(dy, x, w, rstd, dx, part, 0, rows, D, num_sms, st));
+    DISPATCH(is_bf16, n = launch_rms_norm_bwd<T>(dy, x, w, rstd, dx, part, 0, rows, D, num_sms, st, status));
     if (n < 0) return -n;
   }
   DISPATCH(is_bf16, launch_after(rms_dw_kernel<T>, (D + 31) / 32, 1024, 0, st, part, (T*)dw, n, D));
@@ -967,7 +976,7 @@ extern "C" int apb_rms_norm_bwd_noalloc(const void* dy, const void* x, const voi
   if (cudaMemsetAsync(acc, 0, sizeof(float) * shared * D, st) != cudaSuccess) return APB_NOALLOC_ERR_LAUNCH;
   if (rows > 0) {
     int n;
-    DISPATCH(is_bf16, n = launch_rms_norm_bwd<T>(dy, x, w, rstd, dx, acc, shared, rows, D, num_sms, st));
+    DISPATCH(is_bf16, n = launch_rms_norm_bwd<T>(dy, x, w, rstd, dx, acc, shared, rows, D, num_sms, st, nullptr));
     if (n < 0) return APB_NOALLOC_ERR_BAD_SHAPE;
   }
   if (shared > 1) {
