@@ -60,11 +60,12 @@ Two add_rms_norm_bwd(const Tensor& dy_, const c10::optional<Tensor>& dh_, const 
   for (const Tensor* t : {&dy_, dh_.has_value() ? &*dh_ : &dy_})
     TORCH_CHECK(t->sizes() == h_.sizes() && t->scalar_type() == h_.scalar_type() && t->device() == h_.device(), "add_rms_norm_bwd: gradients like h");
   TORCH_CHECK(rstd_.scalar_type() == at::kFloat && rstd_.numel() == a.rows && rstd_.device() == h_.device(), "add_rms_norm_bwd: rstd fp32, one a row");
+  if (!dh_.has_value() && a.rows > 0 && a.D % 8 == 0 && a.D <= 16384 && weight.scalar_type() == a.x.scalar_type())
+    return op_rms_norm_bwd(dy_, h_, weight, rstd_);
   // (a weight in fp32 beside bf16 operands is taken in their type, as the plain norm takes it; its gradient is not rounded to that)
   const bool wide = weight.scalar_type() == at::kFloat;
   Tensor dx = at::empty_like(a.x), dw = at::empty({a.D}, wide ? weight.options() : a.x.options());
   if (a.rows == 0) return {dx, dw.zero_().to(weight.scalar_type())};
-  if (!dh_.has_value() && a.D % 8 == 0 && a.D <= 16384 && weight.scalar_type() == a.x.scalar_type()) return op_rms_norm_bwd(dy_, h_, weight, rstd_);
   Tensor dy = dense(dy_), dh = dh_.has_value() ? dense(*dh_) : Tensor(), rstd = rstd_.contiguous();
   Tensor part = at::empty({(int64_t)apb_add_rms_norm_bwd_workspace(a.rows, (int)a.D, is_bf16(a.x), num_sms())}, rstd.options());  // partial sums of dw
   check(apb_add_rms_norm_bwd(dy.data_ptr(), dh.defined() ? dh.data_ptr() : nullptr, a.x.data_ptr(), a.w.data_ptr(), rstd.data_ptr<float>(), dx.data_ptr(), dw.data_ptr(),

@@ -334,7 +334,8 @@ def mx8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def mx8_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values of codes and scales, exact in both types that are offered (bf16, fp32)."""
+    """The values of codes and scales, of any scale of the format, exact in both types that are offered (bf16, fp32; code -128 of the
+    largest scale, -2^128, is -infinity)."""
     _need(codes.dtype is torch.int8 and scales.dtype is torch.uint8 and codes.ndim >= 1,
           f"mx8_dequantize: int8 codes and uint8 scales expected, not {codes.dtype} and {scales.dtype}")
     want = (*codes.shape[:-1], mx8_blocks(codes.shape[-1]))
